@@ -238,6 +238,86 @@ int mvb_paged_attention_decode_noalloc(void* out, int64_t out_stride, const void
                                        int64_t num_kv_heads, int64_t head_dim, int64_t num_layers, int64_t layer,
                                        int64_t num_blocks, int64_t block_size, float scale, mvb_stream_t stream);
 
+/* ---- 4-bit paged KV cache ------------------------------------------------------------------
+ * No counterpart in the reference, whose pool is in the model's dtype (engine/kv_cache.py:24-29).
+ *
+ * kv4: uint8 [num_layers, num_blocks, Hkv, block_size / 16, 18 * head_dim], 16-byte aligned; a
+ * record of 18 * head_dim bytes holds 16 tokens of a head: K codes [16][D / 2], V codes [16][D / 2],
+ * K pairs [16][D / 64], V pairs [16][D / 64].  The 64 channels of a group share a pair
+ * (scale, min) of bf16; a code u in 0..15 stands for min + scale * u.  Of a row's 32-bit words,
+ * word (D / 64) * w + g holds channels 64 g + 8 w .. + 7, lowest nibble first.
+ * head_dim 64, 128 or 256; block_size a multiple of 16.
+ *
+ * mvb_kv4_write: K and V (bf16, element strides k_stride / v_stride between tokens and
+ * k_head_stride / v_head_stride between heads, multiples of 8; rows 16-byte aligned) of token i are
+ * quantised into slot slots[i] = block * block_size + offset: min = bf16(min x),
+ * scale = bf16((max x - min) / 15), u = round-to-even((x - min) / scale).  A group with a NaN or an
+ * infinity reads back as NaN.  A negative slot is skipped; one past the pool too, with
+ * MVB_DEV_BAD_BLOCK.  Slots of one call are distinct (of a slot given twice, either token's
+ * values may be kept, per group).
+ * mvb_kv4_read: k, v [tokens, Hkv, D] bf16 (contiguous) of the slots; zeros where a slot is
+ * negative or past the pool (MVB_DEV_BAD_BLOCK). */
+int mvb_kv4_write(void* kv4, const void* k, int64_t k_stride, int64_t k_head_stride, const void* v, int64_t v_stride,
+                  int64_t v_head_stride, const int64_t* slots, int64_t tokens, int64_t num_kv_heads,
+                  int64_t head_dim, int64_t num_layers, int64_t layer, int64_t num_blocks, int64_t block_size,
+                  mvb_stream_t stream);
+int mvb_kv4_read(void* k, void* v, const void* kv4, const int64_t* slots, int64_t tokens, int64_t num_kv_heads,
+                 int64_t head_dim, int64_t num_layers, int64_t layer, int64_t num_blocks, int64_t block_size,
+                 mvb_stream_t stream);
+
+/* mvb_paged_attention_decode_ex over a 4-bit pool, for the query_len newest tokens of each sequence
+ * (1: a decode step; more: drafted tokens scored at once).  ctx_lens[b] counts the cached tokens
+ * of sequence b with the query tokens among them: query i of query_len sees the first
+ * n = ctx_lens[b] - query_len + 1 + i keys, or the newest `window` of those (window > 0).  A query
+ * that sees no key gives zeros.  q / out: rows of [Hq, D] bf16, row b * query_len + i at
+ * q_stride / out_stride elements (multiples of 8, 16-byte aligned).  block_tables: row b at
+ * b * table_stride, max_blocks entries of it are used.  A context past its table is cut
+ * (MVB_DEV_BAD_POSITION); a block outside the pool counts as masked (MVB_DEV_BAD_BLOCK).
+ * Scores and softmax statistics in fp32, deterministic.  workspace: at least ..._workspace_bytes()
+ * bytes, 256-byte aligned, of any content; calls that overlap on the GPU need one each. */
+int64_t mvb_paged_attention_decode_kv4_workspace_bytes(int64_t batch, int64_t query_len, int64_t num_q_heads,
+                                                       int64_t num_kv_heads, int64_t head_dim, int device);
+int mvb_paged_attention_decode_kv4(void* out, int64_t out_stride, const void* q, int64_t q_stride, const void* kv4,
+                                   const int32_t* block_tables, int64_t table_stride, int64_t max_blocks,
+                                   const int32_t* ctx_lens, int64_t batch, int64_t query_len, int64_t num_q_heads,
+                                   int64_t num_kv_heads, int64_t head_dim, int64_t num_layers, int64_t layer,
+                                   int64_t num_blocks, int64_t block_size, float scale, float softcap,
+                                   int64_t window, void* workspace, int64_t workspace_bytes, mvb_stream_t stream);
+
+/* Block tables and slot maps of a step from the sequences' lengths (the block growth of
+ * engine/kv_cache.py:40-74 and the slots of models/model.py:233-237, for a batch, on the GPU).
+ * Sequence b holds ctx_lens[b] tokens, i.e. the first ceil(ctx / block_size) entries of its table
+ * row, and takes new_lens[b] more.  The blocks it lacks come off free_blocks[free_head ..
+ * num_free) in row order and are written into its row.  Outputs, tokens packed in row order:
+ * slots[t] = block * block_size + offset, positions[t], seq_start[batch + 1] (first token of each
+ * sequence), granted[batch], and free_head_out (the list's head after this call; free_head NULL
+ * means 0, and the two may not be the same word).  A sequence that does not fit -- in its table row, in
+ * what is left of the free list, or in the num_tokens of the outputs -- takes no block:
+ * granted 0, its tokens' slots -1; those behind it may still fit.  Negative lengths are refused the
+ * same way, with MVB_DEV_BAD_POSITION.  Entries of slots past the last token are -1.  batch <= 8192. */
+int mvb_assign_slots(int64_t* slots, int32_t* positions, int32_t* seq_start, int32_t* granted,
+                     int32_t* free_head_out, int32_t* block_tables, int64_t table_stride, int64_t max_blocks,
+                     const int32_t* ctx_lens, const int32_t* new_lens, const int32_t* free_blocks, int64_t num_free,
+                     const int32_t* free_head, int64_t batch, int64_t block_size, int64_t num_tokens,
+                     mvb_stream_t stream);
+
+/* Verification of drafted tokens (speculative decoding; no counterpart in the reference).
+ * target_probs: fp32 rows, row b * (max_drafts + 1) + i (target_stride elements apart) the target's
+ * distribution at draft i of sequence b, the last one after all drafts; draft_probs: the
+ * drafting distributions, row b * max_drafts + i, or NULL for drafts without one (greedy, looked up:
+ * probability one).  draft_tokens int64 [batch, max_drafts]; draft_lens[b] of them are given (NULL: all);
+ * uniforms fp32 [batch, max_drafts + 1] in [0, 1), the last of a row for the drawn token.
+ * Draft i is accepted while uniforms[i] * q(d) < p(d).  At the first rejection the token is drawn from
+ * max(p - q, 0) (from p if that leaves nothing), after the last draft from the next row of p: the
+ * smallest j with w_0 + .. + w_j > u * sum(w), sums in 64 bits.  out_tokens int64
+ * [batch, max_drafts + 1]: the accepted drafts, the drawn token, then -1; accepted[b]: how many drafts.
+ * A drawn token is -1 where the row has no weight.  A drafted token outside the vocabulary is
+ * rejected (MVB_DEV_BAD_TOKEN).  max_drafts <= 4096. */
+int mvb_verify_drafts(int64_t* out_tokens, int32_t* accepted, const float* target_probs, int64_t target_stride,
+                      const float* draft_probs, int64_t draft_stride, const int64_t* draft_tokens,
+                      const float* uniforms, const int32_t* draft_lens, int64_t batch, int64_t max_drafts,
+                      int64_t vocab, mvb_stream_t stream);
+
 /* ---- dense GEMM on tcgen05 --------------------------------------------------------
  * Replaces the nn.Linear (cuBLAS) projections of the decode step (model_cuda.py:124-126,
  * :180, ops/mlp.py:66/84, model_cuda.py:413): Y[m, n] = sum_k X[m, k] * W[n, k] (bf16 in,

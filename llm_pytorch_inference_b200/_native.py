@@ -58,6 +58,14 @@ SIGNATURES: dict[str, tuple] = {
                                              _i64, _i64, _i64, _i64, _f32, _f32, _i64, _vp, _i64, _vp]),
     "mvb_paged_attention_decode_noalloc": (_i32, [_vp, _i64, _vp, _i64, _vp, _vp, _i64, _vp, _i64, _i64, _i64,
                                                   _i64, _i64, _i64, _i64, _i64, _f32, _vp]),
+    "mvb_kv4_write": (_i32, [_vp, _vp, _i64, _i64, _vp, _i64, _i64, _vp] + [_i64] * 7 + [_vp]),
+    "mvb_kv4_read": (_i32, [_vp, _vp, _vp, _vp] + [_i64] * 7 + [_vp]),
+    "mvb_paged_attention_decode_kv4_workspace_bytes": (_i64, [_i64, _i64, _i64, _i64, _i64, _i32]),
+    "mvb_paged_attention_decode_kv4": (_i32, [_vp, _i64, _vp, _i64, _vp, _vp, _i64, _i64, _vp] + [_i64] * 9 +
+                                       [_f32, _f32, _i64, _vp, _i64, _vp]),
+    "mvb_assign_slots": (_i32, [_vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _vp, _vp, _vp, _i64, _vp, _i64, _i64, _i64,
+                                _vp]),
+    "mvb_verify_drafts": (_i32, [_vp, _vp, _vp, _i64, _vp, _i64, _vp, _vp, _vp, _i64, _i64, _i64, _vp]),
     "mvb_gemm_workspace_bytes": (_i64, [_i64, _i64, _i64, _i32]),
     "mvb_gemm_bf16": (_i32, [_vp, _i64, _vp, _i64, _vp, _i64, _i64, _i64, _i64, _i32, _vp, _i64, _vp, _i64, _vp]),
     "mvb_swiglu_gemm": (_i32, [_vp, _i64, _vp, _i64, _i64, _i64, _vp]),

@@ -42,6 +42,30 @@ def num_blocks_for_budget(block_size: int, num_heads: int, head_dim: int, num_la
     return max(int(avail // block_bytes(block_size, num_heads, head_dim, num_layers, dtype_size)), 1)
 
 
+def kv4_block_bytes(block_size: int, num_heads: int, head_dim: int, num_layers: int) -> int:
+    """``block_bytes`` of a 4-bit pool: 4 bits a value and one 32-bit (scale, min) pair per 64 channels."""
+    return block_size * num_heads * num_layers * (18 * head_dim // 16)
+
+
+def kv4_pool(num_blocks: int, block_size: int, num_layers: int, num_heads: int, head_dim: int,
+             device: str | torch.device = "cuda") -> torch.Tensor:
+    """A 4-bit paged pool, uint8 ``[num_layers, num_blocks, num_heads, block_size / 16, 18 * head_dim]``.
+
+    A record of ``18 * head_dim`` bytes holds 16 tokens of a head: K codes, V codes, K and V (scale, min)
+    pairs of bf16, one per group of 64 channels; a code u stands for ``min + scale * u``
+    (``ops.kv4_write`` / ``ops.kv4_read``, ``ops.paged_attention_decode_kv4``).  Slots are those of the
+    bf16 pool, ``block * block_size + offset``, so one ``KVCacheManager`` (``allocate_pool=False``)
+    serves either.  At head size 128 a block takes 9 / 32 of the bf16 block's bytes."""
+    if block_size <= 0 or block_size % 16:
+        raise ValueError(f"block_size {block_size}: a 4-bit pool takes multiples of 16")
+    if head_dim not in (64, 128, 256):
+        raise ValueError(f"head_dim {head_dim}: a 4-bit pool takes 64, 128 or 256")
+    if min(num_blocks, num_layers, num_heads) <= 0:
+        raise ValueError("a 4-bit pool needs at least one block, layer and head")
+    return torch.zeros(num_layers, num_blocks, num_heads, block_size // 16, 18 * head_dim, dtype=torch.uint8,
+                       device=device)
+
+
 class KVCacheManager:
     def __init__(self, num_blocks: int, block_size: int, num_layers: int, num_heads: int, head_dim: int,
                  device: str | torch.device = "cuda", dtype: torch.dtype = torch.bfloat16,

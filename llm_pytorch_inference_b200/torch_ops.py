@@ -46,6 +46,14 @@ DECODE_SCHEMAS = [
     "paged_attention_decode(Tensor q, Tensor kv_cache, int layer, Tensor block_tables, Tensor ctx_lens, "
     "float scale) -> Tensor",
     "fused_sample(Tensor logits, Tensor temperature, Tensor top_k, Tensor top_p, int seed, int offset) -> Tensor",
+    "kv4_write(Tensor k, Tensor v, Tensor(a!) kv4, int layer, Tensor slots) -> ()",
+    "kv4_read(Tensor kv4, int layer, Tensor slots) -> (Tensor, Tensor)",
+    "paged_attention_decode_kv4(Tensor q, Tensor kv4, int layer, Tensor block_tables, Tensor ctx_lens, "
+    "float scale, float softcap, int window) -> Tensor",
+    "assign_slots(Tensor(a!) block_tables, Tensor ctx_lens, Tensor new_lens, Tensor free_blocks, int block_size, "
+    "int num_tokens, Tensor? free_head) -> (Tensor, Tensor, Tensor, Tensor, Tensor)",
+    "verify_drafts(Tensor target_probs, Tensor draft_tokens, Tensor uniforms, Tensor? draft_probs, "
+    "Tensor? draft_lens) -> (Tensor, Tensor)",
 ]
 
 
@@ -96,6 +104,12 @@ IMPLS = {
     "paged_attention_decode": lambda q, kv_cache, layer, block_tables, ctx_lens, scale:
         ops.paged_attention_decode(q, kv_cache, layer, block_tables, ctx_lens, scale),
     "fused_sample": lambda logits, t, k, p, seed, offset: ops.sample(logits, t, k, p, seed, offset),
+    "kv4_write": ops.kv4_write,
+    "kv4_read": ops.kv4_read,
+    "paged_attention_decode_kv4": lambda q, kv4, layer, block_tables, ctx_lens, scale, softcap, window:
+        ops.paged_attention_decode_kv4(q, kv4, layer, block_tables, ctx_lens, scale, softcap=softcap, window=window),
+    "assign_slots": lambda *args: tuple(ops.assign_slots(*args)),
+    "verify_drafts": ops.verify_drafts,
 }
 
 _LIB: torch.library.Library | None = None
