@@ -66,6 +66,26 @@ int launch(const char* name, void (*kernel)(KArgs...), dim3 grid, dim3 block, si
   return cuda_status(e, name);
 }
 
+// Launch `kernel` as the dependent of the launch just before it in the same entry point: always with
+// the PDL attribute.  It may start while that kernel still runs and waits for it (griddepcontrol.wait)
+// before it reads or writes anything.
+template <typename... KArgs, typename... Args>
+int launch_dependent(const char* name, void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t smem,
+                     cudaStream_t stream, Args&&... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = block;
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, std::forward<Args>(args)...);
+  return cuda_status(e, name);
+}
+
 // Launch with a (cluster_x, 1, 1) thread-block cluster, plus the PDL attribute when enabled.
 template <typename... KArgs, typename... Args>
 int launch_cluster(const char* name, void (*kernel)(KArgs...), dim3 grid, dim3 block, unsigned cluster_x,

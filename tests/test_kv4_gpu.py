@@ -129,14 +129,14 @@ def test_slots_outside_the_pool():
 
 
 # -------------------------------------------------------------------------- attention
-def attend_case(seed, lens, T, Hq, Hkv, D, bs=16, spare=2, wide=0, qscale=1.0):
-    """A pool of quantised keys and values whose unused tokens hold NaN pairs, and shuffled tables whose
-    unused entries are invalid."""
+def attend_case(seed, lens, T, Hq, Hkv, D, bs=16, spare=2, wide=0, qscale=1.0, unused=255):
+    """A pool of quantised keys and values whose unused tokens hold NaN pairs (bytes of 255; 127: pairs of
+    3.4e38), and shuffled tables whose unused entries are invalid."""
     g = gen(seed)
     held = [(n + bs - 1) // bs for n in lens]
     P = sum(held) + spare
     order = torch.randperm(P, generator=g, device=DEV)
-    pool = torch.full((2, P, Hkv, bs // 16, 18 * D), 255, dtype=torch.uint8, device=DEV)    # bf16 0xFFFF: NaN
+    pool = torch.full((2, P, Hkv, bs // 16, 18 * D), unused, dtype=torch.uint8, device=DEV)
     mb = max(held + [1]) + wide
     table = torch.full((len(lens), mb), -7, dtype=torch.int32, device=DEV)
     at = 0
@@ -178,6 +178,18 @@ def test_attention_head_layouts(D, Hq, Hkv):
 def test_attention_lengths(lens, bs):
     c = attend_case(sum(lens) + bs, lens, 1, 8, 2, 128, bs=bs, wide=3)
     check(c, attend(c))
+
+
+@pytest.mark.parametrize("unused", [0, 127, 128, 255])
+def test_attention_unused_tokens_hold_anything(unused):
+    """The tokens behind a sequence in its last page and before its window: zeros, NaN, the largest and lowest pairs."""
+    c = attend_case(40 + unused, [5, 20, 300, 1000], 1, 8, 2, 128, bs=64, unused=unused)
+    check(c, attend(c))
+    c = attend_case(41 + unused, [5, 20, 300, 1000], 3, 8, 2, 128, bs=64, unused=unused)
+    check(c, attend(c))
+    slot = int(c["table"][3, 0]) * 64
+    c["pool"][1, slot // 64] = unused                     # the first block lies before the window
+    check(c, attend(c, window=900), window=900)
 
 
 @pytest.mark.parametrize("T", [1, 2, 3, 5, 8, 16, 33])
