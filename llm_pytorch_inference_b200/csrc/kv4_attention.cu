@@ -3,30 +3,34 @@
 //   out[b, i, h] = sum_t softmax_t(cap(q . k_t * scale)) v_t  over the keys t that query i sees,
 //   k = m + s u,  v = m' + s' u'  per 64 channels (codes u in 0..15, pairs (s, m)).
 //
-// What it must read is 9/16 of a byte per cached value, once: the bound is memory.  That leaves an SM some
-// 40 values a clock, so a value may cost about two instructions of a lane, and codes never become
-// floating-point numbers one by one:
-//   * fp16 holds u * 2^-24 and u * 2^-20 as bit patterns with the code in bits 0-3 or 4-7 (subnormal
-//     numbers, exact).  One AND of a word thus yields two matrix operands, no conversion and no offset.
-//   * The pairs stay outside the products.  Scores: q . k = sum_g s_g (q_g . u_g) + m_g sum(q_g), per group
-//     of 64 channels.  Outputs: the weight of a token times s' is the operand against its codes, and
-//     p m' is summed per group and query, on the side.
-//   * q is scaled per row by a power of two into fp16's range and is exact there; scores and statistics
-//     are fp32.  The weight p s' is the one rounding (11 bits, 8 times finer than the result's bf16); it is
-//     scaled by a power of two that follows the largest s' seen.
-// Both products run transposed on mma.sync m16n8k16, the query rows (query heads of the KV head times T)
-// being the n = 8 side: S^T = K Q^T (16 tokens x 8 NT rows), O^T = V^T P^T.  The k index of the first product
-// runs over the channels in the order in which a lane's words hold them (Q is stored in that order); the
-// tokens of the second are permuted (tile_token) so that lanes reading the same word of different
-// tokens fall into different banks.
+// What it must read is 9/16 of a byte per cached value, once: the bound is memory.  That leaves an SM some 44
+// values a clock, and its integer pipe takes 64 lane-operations a clock, so codes never become floating-point
+// numbers one by one:
+//   * Scores: q . k = sum_g s_g (q_g . u_g) + m_g sum(q_g) over the groups of 64 channels, the pairs outside
+//     the products.  Codes are bytes for the integer tensor cores (u8 x s8, exact): three operations turn a word
+//     of 8 codes into two operands.  q of a row is held in 16 bits of its largest magnitude, as two signed bytes
+//     (planes) that are columns of their own; the rounding is 2^-16 of that magnitude, below what fp32 sums of
+//     the products would lose at long rows.  The sums stay below 2^22 and start at 1.5 * 2^23, so that their bits
+//     are the fp32 number itself and need no conversion.
+//   * Outputs: fp16 holds u * 2^-24 and u * 2^-20 as bit patterns with the code in bits 0-3 or 4-7 (subnormal
+//     numbers, exact), so one AND of a word yields two matrix operands.  The weight of a token times s' is
+//     the other operand, and p m' is summed per group and query, on the side.  That weight is the one
+//     rounding (11 bits, 8 times finer than the result's bf16); it is scaled by a power of two that
+//     follows the largest s' seen.  Scores, statistics and sums are fp32.
+// Both products run transposed on mma.sync, the query rows (query heads of the KV head times T) being the n = 8
+// side: S^T = K Q^T (16 tokens x rows), O^T = V^T P^T.  The k index of the first product runs over the channels
+// in the order in which a lane's words hold them (Q is stored in that order); the tokens of the second are
+// permuted (tile_token) so that lanes reading the same word of different tokens fall into different banks.
+// Up to 4 rows (RT = 0) their two planes fill one n = 8 tile; above that a plane takes a tile of its own.
 //
-// Work split: the cache of an item (sequence, KV head, chunk of 8 NT rows) is cut into rounds of W records
-// (W warps, a record of 16 tokens each).  The rounds of the whole batch are laid end to end and divided
-// evenly over the resident CTAs, whatever the lengths.  Each warp streams its own records through a ring in
-// shared memory (one bulk copy a record, several in flight), and keeps its own running maximum, sum
-// and output; they are joined in shared memory at the end of an item.  An item that spans CTAs
-// leaves partial results, joined in CTA order by a second small kernel: no atomics, nothing to clear.
+// Work split: the cache of an item (sequence, KV head, chunk of query rows) is a run of records of 16 tokens.
+// The records of the whole batch are laid end to end and divided evenly over the resident warps, whatever the
+// lengths: a warp is a worker of its own, without a barrier after the prologue.  It streams its records
+// through a ring in shared memory (one bulk copy a record, several in flight) and keeps the running
+// maximum, sum and output of an item in registers.  An item that spans workers leaves partial results, joined in
+// worker order by a second small kernel: no atomics, nothing to clear, the same bits every time.
 #include <climits>
+#include <type_traits>
 
 #include "common.cuh"
 #include "host.h"
@@ -39,21 +43,37 @@ namespace {
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr int kWarps = 8;
 constexpr int kThreads = kWarps * 32;
+constexpr int kJoinThreads = 128;
+constexpr int kShortRecords = 8;  // items of at most this many records are never split
+
 // A weight is 2^(score - reference): the reference is a row's maximum when last raised, and is raised
 // once a score passes it by more than kSlack (in powers of two), so that most records cost one vote instead
-// of a reduction.  The weight times the scaled s' stays below 2^(kSlack + kScaleMax) = 2^15 in fp16.
+// of a reduction.  The weight times the scaled s' stays below 2^(kSlack + 11) = 2^15 in fp16.
 constexpr float kSlack = 4.0f;
-constexpr float kScaleMax = 2048.0f;  // 2^11; a new scaling puts the largest s' into [2^9, 2^10)
+constexpr float kScaleMax = 2048.0f;  // of s' times its scaling; a new scaling puts the largest s' into [2^9, 2^10)
 constexpr int kScaleTarget = 9;
+constexpr float kFltMax = 3.40282347e38f;
+constexpr float kNone = -kFltMax;     // reference of a row without a key: no special cases, any score passes it
+constexpr float kMagic = 12582912.0f; // 1.5 * 2^23: its bits plus a small integer are the bits of the sum
+constexpr int kMagicBits = 0x4B400000;
+
+// RT: 0 = up to 4 query rows per chunk, 1 = up to 8, 2 = up to 16.
+template <int RT>
+struct Kv4Rows {
+  static constexpr int NT = RT == 0 ? 1 : RT;       // n = 8 tiles of the second product
+  static constexpr int KT = RT == 0 ? 1 : 2 * RT;   // of the first
+  static constexpr int NC = RT == 0 ? 1 : 2 * RT;   // rows per lane
+  static constexpr int ROWS = RT == 0 ? 4 : 8 * RT;
+};
 
 // Records in flight per warp: an SM's share of the bandwidth needs some 45 KB.
-template <int D, int NT>
+template <int D, int RT>
 constexpr int kv4_stages() {
-  return D == 64 ? 6 : D == 256 && NT > 1 ? 2 : 4;
+  return D == 64 ? 6 : D == 256 && RT > 1 ? 2 : 4;
 }
-template <int D, int NT>
+template <int D, int RT>
 constexpr int kv4_ctas_per_sm() {
-  return D == 256 || NT > 1 ? 1 : 2;
+  return D == 256 || RT > 1 ? 1 : 2;
 }
 
 struct Kv4AttnArgs {
@@ -66,34 +86,32 @@ struct Kv4AttnArgs {
   int max_blocks;
   const int32_t* ctx;
   int batch, T, group, hkv;
-  int chunks;  // of 8 NT rows, per KV head
+  int chunks;  // of ROWS query rows, per KV head
   int num_blocks, recs;
   float score_scale;  // scale * log2(e), or scale / softcap under a cap
   float cap_log2;     // softcap * log2(e); 0 = no cap
   int window;
-  int slab_rows;  // rows of a chunk, at most 8 NT
+  int slab_rows;  // rows of the largest chunk
+  int per;        // records of a round, the unit of the division
   // workspace
-  int64_t* head;       // [0]: CTAs that have work
-  struct Kv4Start* starts;  // [grid]
-  float2* part_ml;     // [2 grid][8 NT]
-  float* part_o;       // [2 grid][8 NT][D]
+  int64_t* head;  // [0]: workers, [1]: rounds of the batch
+  struct Kv4Item* items;  // [batch * hkv * chunks]
+  float2* part_ml;        // [2 workers][ROWS]
+  float* part_o;          // [2 workers][ROWS][D]
   unsigned* err;
 };
 
-// Where a CTA's range of rounds begins.
-struct Kv4Start {
-  int64_t item_first;  // first round of the item, counted over the batch
-  int rounds;          // of the item
-  int seq;
-  int sub;             // (KV head, chunk) within the sequence
-  int pad[3];
+// Where an item lies among the rounds of the batch.
+struct Kv4Item {
+  int64_t first;
+  int64_t rounds;
 };
 
-__device__ __forceinline__ int64_t range_start(int c, int64_t total, int grid) {
-  return static_cast<int64_t>(c) * total / grid;
+__device__ __forceinline__ int64_t range_start(int w, int64_t total, int workers) {
+  return static_cast<int64_t>(w) * total / workers;
 }
-__device__ __forceinline__ int cta_of(int64_t x, int64_t total, int grid) {
-  return static_cast<int>(((x + 1) * grid + total - 1) / total - 1);
+__device__ __forceinline__ int worker_of(int64_t x, int64_t total, int workers) {
+  return static_cast<int>(((x + 1) * workers + total - 1) / total - 1);
 }
 
 // exp2 with results below 2^-126 flushed to zero.
@@ -115,6 +133,38 @@ __device__ __forceinline__ void mma_f16_16816(float (&d)[4], uint32_t a0, uint32
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
+__device__ __forceinline__ void mma_u8s8_16832(int (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                                               uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k32.row.col.s32.u8.s8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+      "{%0, %1, %2, %3};"
+      : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+// N consecutive 32-bit words of shared memory, aligned to their size.
+template <int N>
+__device__ __forceinline__ void load_words(const uint8_t* p, uint32_t (&w)[N]) {
+  if constexpr (N == 1) {
+    w[0] = *reinterpret_cast<const uint32_t*>(p);
+  } else if constexpr (N == 2) {
+    const uint2 v = *reinterpret_cast<const uint2*>(p);
+    w[0] = v.x, w[1] = v.y;
+  } else {
+#pragma unroll
+    for (int k = 0; k < N / 4; ++k) {
+      const uint4 v = *reinterpret_cast<const uint4*>(p + 16 * k);
+      w[4 * k] = v.x, w[4 * k + 1] = v.y, w[4 * k + 2] = v.z, w[4 * k + 3] = v.w;
+    }
+  }
+}
+// A pair's scale (low half) and minimum (high half).
+__device__ __forceinline__ float pair_scale(uint32_t p) { return __uint_as_float(p << 16); }
+__device__ __forceinline__ float pair_min(uint32_t p) { return __uint_as_float(p & 0xffff0000u); }
+
+__device__ __noinline__ bool wait_slow(uint64_t* bar, uint32_t parity, volatile int* abort_flag, unsigned* err) {
+  return mbar_wait(bar, parity, abort_flag, err);
+}
+
 __device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
   const __half2 v = __floats2half2_rn(lo, hi);
   return *reinterpret_cast<const uint32_t*>(&v);
@@ -148,42 +198,40 @@ __device__ __forceinline__ Kv4Seq kv4_seq(const Kv4AttnArgs& a, int b, bool tell
   s.first = 0;
   if (a.window > 0) s.first = max(s.ctx - a.T + 1 - a.window, 0) / kKv4Tokens;
   s.last = (s.ctx + kKv4Tokens - 1) / kKv4Tokens;
-  s.rounds = max((s.last - s.first + kWarps - 1) / kWarps, 1);  // one for no keys too: it writes the zeros
+  s.rounds = max((s.last - s.first + a.per - 1) / a.per, 1);  // one for no keys too: it writes the zeros
   return s;
 }
 
-template <int D, int NT>
+template <int D, int RT>
 struct Kv4Smem {
-  static constexpr int STAGES = kv4_stages<D, NT>();
-  static constexpr int RING = kWarps * STAGES * Kv4<D>::RECORD;
-  static constexpr int QF = RING;                              // Q operands [D / 16][NT][32] x 8 bytes
-  static constexpr int COL = QF + D / 16 * NT * 256;           // per row: score factor, then sums of q per group
-  static constexpr int ML = COL + 8 * NT * (1 + Kv4<D>::NG) * 4;  // [warps][8 NT] float2
-  static constexpr int BAR = (ML + kWarps * 8 * NT * 8 + 15) / 16 * 16;
-  static constexpr int SLAB = (BAR + kWarps * STAGES * 8 + 127) / 128 * 128;  // [warps][rows][D + 8] floats
-  static constexpr int SLAB_ROW = D + 8;
-  static constexpr size_t bytes(int rows) { return SLAB + static_cast<size_t>(kWarps) * rows * SLAB_ROW * 4; }
+  static constexpr int STAGES = kv4_stages<D, RT>(), ROWS = Kv4Rows<RT>::ROWS;
+  // per warp: the ring, Q operands [D / 32][KT][32 lanes] x 8 bytes, per row the score factor and the
+  // sums of q per group, the ring's barriers
+  static constexpr int RING = STAGES * Kv4<D>::RECORD;
+  static constexpr int QF = RING;
+  static constexpr int COL = QF + D / 32 * Kv4Rows<RT>::KT * 256;
+  static constexpr int BAR = (COL + ROWS * (1 + Kv4<D>::NG) * 4 + 7) / 8 * 8;
+  static constexpr int WARP = (BAR + STAGES * 8 + 127) / 128 * 128;
+  static constexpr int BYTES = kWarps * WARP;
 };
 
-template <int D, int NT, bool CAP>
-__global__ void __launch_bounds__(kThreads, kv4_ctas_per_sm<D, NT>()) kv4_attn_kernel(const Kv4AttnArgs a) {
+template <int D, int RT, bool CAP>
+__global__ void __launch_bounds__(kThreads, kv4_ctas_per_sm<D, RT>()) kv4_attn_kernel(const Kv4AttnArgs a) {
   using P = Kv4<D>;
-  using S = Kv4Smem<D, NT>;
-  constexpr int NG = P::NG, STAGES = S::STAGES, KS = D / 16, ROWS = 8 * NT;
+  using S = Kv4Smem<D, RT>;
+  using R = Kv4Rows<RT>;
+  constexpr int NG = P::NG, STAGES = S::STAGES, ROWS = R::ROWS, NT = R::NT, KT = R::KT, NC = R::NC;
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ volatile int abort_flag;
   __shared__ int64_t scan_warp[kWarps];
-  __shared__ int64_t found_first;
-  __shared__ int found_seq;
+  __shared__ int64_t scan_end[kThreads];  // rounds up to and with a sequence
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int g = lane >> 2, c = lane & 3;
-  uint2* qf = reinterpret_cast<uint2*>(smem + S::QF);
-  float* col_f = reinterpret_cast<float*>(smem + S::COL);
+  uint8_t* ring = smem + warp * S::WARP;
+  uint2* qf = reinterpret_cast<uint2*>(ring + S::QF);
+  float* col_f = reinterpret_cast<float*>(ring + S::COL);
   float* col_q = col_f + ROWS;  // [ROWS][NG]
-  float2* ml = reinterpret_cast<float2*>(smem + S::ML);
-  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + S::BAR) + warp * STAGES;
-  float* slab = reinterpret_cast<float*>(smem + S::SLAB);
-  uint8_t* ring = smem + warp * STAGES * P::RECORD;
+  uint64_t* bars = reinterpret_cast<uint64_t*>(ring + S::BAR);
 
   pdl_launch_dependents();
   if (lane < STAGES) mbar_init(bars + lane, 1);
@@ -191,13 +239,12 @@ __global__ void __launch_bounds__(kThreads, kv4_ctas_per_sm<D, NT>()) kv4_attn_k
   if (tid == 0) abort_flag = 0;
   pdl_wait();
 
-  // ---- this CTA's rounds: [r0, r1) of the batch's total
+  // ---- this worker's rounds, [r0, r1) of the batch's total, and the sequence that r0 lies in
   const int subs = a.hkv * a.chunks;
-  int64_t carry = 0, incl = 0, own = 0;
-  for (int base = 0; base < a.batch; base += kThreads) {
+  int64_t carry = 0;
+  auto scan = [&](int base, bool tell) {  // rounds of 256 sequences: their running sum into scan_end
     const int b = base + tid;
-    own = b < a.batch ? static_cast<int64_t>(kv4_seq(a, b, blockIdx.x == 0).rounds) * subs : 0;
-    incl = own;
+    int64_t incl = b < a.batch ? static_cast<int64_t>(kv4_seq(a, b, tell).rounds) * subs : 0;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
       const int64_t y = __shfl_up_sync(0xffffffffu, incl, o);
@@ -207,76 +254,58 @@ __global__ void __launch_bounds__(kThreads, kv4_ctas_per_sm<D, NT>()) kv4_attn_k
     if (lane == 31) scan_warp[warp] = incl;
     __syncthreads();
     int64_t all = 0;
+#pragma unroll
     for (int w = 0; w < kWarps; ++w) {
       if (w < warp) incl += scan_warp[w];
       all += scan_warp[w];
     }
-    incl += carry;
+    scan_end[tid] = incl + carry;
     carry += all;
-  }
+    __syncthreads();
+  };
+  for (int base = 0; base < a.batch; base += kThreads) scan(base, blockIdx.x == 0);
   const int64_t total = carry;
-  const int active = static_cast<int>(min(static_cast<int64_t>(gridDim.x), total));
+  const int workers = static_cast<int>(min(static_cast<int64_t>(gridDim.x) * kWarps, total));
   if (blockIdx.x == 0 && tid == 0) {
-    a.head[0] = active;
+    a.head[0] = workers;
     a.head[1] = total;
   }
-  if (static_cast<int>(blockIdx.x) >= active) return;
-  const int64_t r0 = range_start(blockIdx.x, total, active), r1 = range_start(blockIdx.x + 1, total, active);
-  if (a.batch <= kThreads) {
-    if (own > 0 && incl - own <= r0 && r0 < incl) {
-      found_seq = tid;
-      found_first = incl - own;
-    }
-  } else {
-    carry = 0;
-    for (int base = 0; base < a.batch && carry <= r0; base += kThreads) {
-      const int b = base + tid;
-      own = b < a.batch ? static_cast<int64_t>(kv4_seq(a, b, false).rounds) * subs : 0;
-      incl = own;
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const int64_t y = __shfl_up_sync(0xffffffffu, incl, o);
-        if (lane >= o) incl += y;
-      }
-      __syncthreads();
-      if (lane == 31) scan_warp[warp] = incl;
-      __syncthreads();
-      int64_t all = 0;
-      for (int w = 0; w < kWarps; ++w) {
-        if (w < warp) incl += scan_warp[w];
-        all += scan_warp[w];
-      }
-      incl += carry;
-      carry += all;
-      if (own > 0 && incl - own <= r0 && r0 < incl) {
-        found_seq = b;
-        found_first = incl - own;
+  const int worker = warp * gridDim.x + blockIdx.x;  // few rounds: spread over the SMs
+  const bool busy = worker < workers;
+  const int64_t r0 = busy ? range_start(worker, total, workers) : 0;
+  const int64_t r1 = busy ? range_start(worker + 1, total, workers) : 0;
+  int seq = 0;
+  int64_t seq_first = 0;
+  if (a.batch > kThreads) carry = 0;
+  for (int base = 0; base < a.batch; base += kThreads) {
+    const int64_t before = a.batch > kThreads ? carry : 0;
+    if (a.batch > kThreads) scan(base, false);
+    for (int x = lane; x < kThreads && base + (x & ~31) < a.batch; x += 32) {
+      const int64_t end = scan_end[x], begin = x == 0 ? before : scan_end[x - 1];
+      const unsigned hit = __ballot_sync(0xffffffffu, begin <= r0 && r0 < end);
+      if (hit) {
+        const int at = __ffs(hit) - 1;
+        seq = base + (x & ~31) + at;
+        seq_first = __shfl_sync(0xffffffffu, begin, at);
       }
     }
   }
-  __syncthreads();
+  if (!busy) return;
 
-  int seq = found_seq;
   Kv4Seq sq = kv4_seq(a, seq, false);
-  int sub = static_cast<int>((r0 - found_first) / sq.rounds);
-  int ra = static_cast<int>(r0 - found_first - static_cast<int64_t>(sub) * sq.rounds);
+  int sub = static_cast<int>((r0 - seq_first) / sq.rounds);
+  int ra = static_cast<int>(r0 - seq_first - static_cast<int64_t>(sub) * sq.rounds);
   int left = static_cast<int>(r1 - r0);
-  if (tid == 0) {
-    Kv4Start st = {};
-    st.item_first = r0 - ra;
-    st.rounds = sq.rounds;
-    st.seq = seq;
-    st.sub = sub;
-    a.starts[blockIdx.x] = st;
-  }
+  int64_t item_first = r0 - ra;
 
-  // ---- the warp's stream of records, STAGES ahead of the arithmetic
+  // ---- the worker's stream of records, STAGES ahead of the arithmetic
+  const int64_t block_bytes = static_cast<int64_t>(a.hkv) * a.recs * P::RECORD;
   int p_seq = seq, p_sub = sub, p_left = left, p_n = min(sq.rounds - ra, left);
   Kv4Seq p_sq = sq;
-  int p_t = sq.first + ra * kWarps + warp, p_end = min(sq.first + (ra + p_n) * kWarps, sq.last);
+  int p_t = sq.first + ra * a.per, p_end = min(sq.first + (ra + p_n) * a.per, sq.last);
   int p_id = 0, p_rec = 0;
   bool p_ok = true;
-  // Settles on the warp's next record at or after p_t, crossing into the next items, and asks for its block id
+  // Settles on the next record at or after p_t, crossing into the next items, and asks for its block id
   // (one record ahead of the copy that needs it).
   auto settle = [&]() {
     while (p_t >= p_end) {
@@ -290,8 +319,8 @@ __global__ void __launch_bounds__(kThreads, kv4_ctas_per_sm<D, NT>()) kv4_attn_k
         p_sq = kv4_seq(a, ++p_seq, false);
       }
       p_n = min(p_sq.rounds, p_left);
-      p_t = p_sq.first + warp;
-      p_end = min(p_sq.first + p_n * kWarps, p_sq.last);
+      p_t = p_sq.first;
+      p_end = min(p_sq.first + p_n * a.per, p_sq.last);
     }
     const int blk = a.recs == 1 ? p_t : p_t / a.recs;
     p_rec = p_t - blk * a.recs;
@@ -304,19 +333,19 @@ __global__ void __launch_bounds__(kThreads, kv4_ctas_per_sm<D, NT>()) kv4_attn_k
       bad &= ~(1u << st);
       if (lane == 0) {
         const int h = a.chunks == 1 ? p_sub : p_sub / a.chunks;
-        const int64_t rec = (static_cast<int64_t>(p_id) * a.hkv + h) * a.recs + p_rec;
         mbar_arrive_expect_tx(bars + st, P::RECORD);
-        bulk_load(ring + st * P::RECORD, a.pool + rec * P::RECORD, P::RECORD, bars + st);
+        bulk_load(ring + st * P::RECORD, a.pool + p_id * block_bytes + (h * a.recs + p_rec) * P::RECORD, P::RECORD,
+                  bars + st);
       }
     } else {
       bad |= 1u << st;
       if (lane == 0) report(a.err, kDevBadBlock);
     }
-    p_t += kWarps;
+    ++p_t;
     settle();
   };
   settle();
-  int pending = 0;  // stages whose copy is still to be waited for
+  int pending = 0;  // stages whose record is still to be waited for
 #pragma unroll 1
   for (int st = 0; st < STAGES; ++st) {
     pending += p_ok;
@@ -331,346 +360,354 @@ __global__ void __launch_bounds__(kThreads, kv4_ctas_per_sm<D, NT>()) kv4_attn_k
   for (int i = 0; i < 4; ++i) vtok[i] = 4 * c + ((i + c) & 3);
 
   // ---- items
+  auto row_of = [&](int q) { return RT == 0 ? c : (q >> 1) * 8 + 2 * c + (q & 1); };  // row of the lane's column q
   while (left > 0) {
     const int n_rounds = min(sq.rounds - ra, left);
     const int h = a.chunks == 1 ? sub : sub / a.chunks;
     const int row0 = (sub - h * a.chunks) * ROWS;
     const int rows = min(a.group * a.T - row0, ROWS);
 
-    // Q of the item: row per warp, scaled by a power of two so that its largest magnitude lies in [2^10, 2^11)
-    for (int r = warp; r < ROWS; r += kWarps) {
-      constexpr int N = D / 32;
-      float x[N];
-      float big = 0.0f;
+    // Q of the item, four rows at a time, eight lanes each: round(32512 q / max |q|) = 256 hi + lo, signed bytes
+    __syncwarp();
+#pragma unroll 1
+    for (int pass = 0; pass < ROWS / 4; ++pass) {
+      const int r = pass * 4 + (lane >> 3), w = lane & 7;
       const int i = (row0 + r) / a.group, hq = h * a.group + (row0 + r) - i * a.group;
-      const __nv_bfloat16* src = a.q + (static_cast<int64_t>(seq) * a.T + i) * a.q_stride + static_cast<int64_t>(hq) * D;
+      const __nv_bfloat16* src =
+          a.q + (static_cast<int64_t>(seq) * a.T + i) * a.q_stride + static_cast<int64_t>(hq) * D + 8 * w;
+      uint4 raw[NG];
 #pragma unroll
-      for (int j = 0; j < N; ++j) {
-        x[j] = r < rows ? __bfloat162float(src[lane * N + j]) : 0.0f;
-        big = fmaxf(big, fabsf(x[j]));
+      for (int k = 0; k < NG; ++k)
+        raw[k] = r < rows ? *reinterpret_cast<const uint4*>(src + 64 * k) : make_uint4(0u, 0u, 0u, 0u);
+      uint32_t big = 0;  // bits of the largest magnitude: ordered as integers, NaN and infinity on top
+#pragma unroll
+      for (int k = 0; k < NG; ++k) {
+        const uint32_t x[4] = {raw[k].x, raw[k].y, raw[k].z, raw[k].w};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) big = max(big, max((x[j] << 16) & 0x7fffffffu, x[j] & 0x7fff0000u));
       }
-      big = warp_max(big);
-      int e = 0;
-      if (big > 0.0f && big <= 3.3895314e38f) e = 10 - ilogbf(big);
-      e = min(max(e, -126), 126);
-      const float up = ldexpf(1.0f, e);
-      float part = 0.0f;
 #pragma unroll
-      for (int j = 0; j < N; ++j) {
-        x[j] *= up;
-        part += x[j];
+      for (int o = 1; o < 8; o <<= 1) big = max(big, __shfl_xor_sync(0xffffffffu, big, o));
+      const bool fine = big < 0x7f800000u;
+      const float up = big > 0 && fine ? fminf(32512.0f / __uint_as_float(big), 1e38f) : 0.0f;
+      const int n0 = RT == 0 ? 2 * r : r % 8, t0 = RT == 0 ? 0 : 2 * (r / 8);
+      const int n1 = RT == 0 ? 2 * r + 1 : r % 8, t1 = RT == 0 ? 0 : t0 + 1;
+#pragma unroll
+      for (int k = 0; k < NG; ++k) {
+        const uint32_t x[4] = {raw[k].x, raw[k].y, raw[k].z, raw[k].w};
+        // word w of the group is word w % 2 of lane w / 2; its even codes are the first operand, the odd ones the second
+        uint32_t hi[2] = {0, 0}, lo[2] = {0, 0};
+        int sum = 0;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const float xv = __uint_as_float((j & 1) ? x[j >> 1] & 0xffff0000u : x[j >> 1] << 16);
+          const int v = fine ? __float2int_rn(xv * up) : 0, vh = (v + 128) >> 8;
+          sum += v;
+          hi[j & 1] |= (static_cast<uint32_t>(vh) & 255u) << (8 * (j >> 1));
+          lo[j & 1] |= (static_cast<uint32_t>(v) & 255u) << (8 * (j >> 1));  // v - 256 vh in its low byte
+        }
+        const int ks = k * 2 + (w & 1);
+        qf[(ks * KT + t0) * 32 + n0 * 4 + (w >> 1)] = make_uint2(hi[0], hi[1]);
+        qf[(ks * KT + t1) * 32 + n1 * 4 + (w >> 1)] = make_uint2(lo[0], lo[1]);
+#pragma unroll
+        for (int o = 1; o < 8; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+        if (w == 0) col_q[r * NG + k] = static_cast<float>(sum);
       }
-      // lanes of a group of 64 channels: 64 / N of them
-#pragma unroll
-      for (int o = 1; o < 64 / N; o <<= 1) part += __shfl_xor_sync(0xffffffffu, part, o);
-      if (lane == 0) col_f[r] = ldexpf(a.score_scale, 20 - e);
-      if (lane % (64 / N) == 0) col_q[r * NG + lane / (64 / N)] = part * 0x1p-20f;
-      __half* dst = reinterpret_cast<__half*>(qf);
-#pragma unroll
-      for (int j = 0; j < N; ++j) {
-        const int ch = lane * N + j, grp = ch / 64, w = ch % 64 / 8, nib = ch % 8;
-        // word w of the group belongs to lane c = w / 2; nibbles 2h', 2h' + 4 are the low k pair of half h', and
-        // 2h' + 1, 2h' + 5 the high one, whose codes weigh 16 times as much
-        const int ks = (grp * 2 + (w & 1)) * 2 + ((nib & 3) >> 1), hi = nib & 1, el = nib >> 2;
-        dst[((ks * NT + r / 8) * 32 + (r % 8) * 4 + w / 2) * 4 + hi * 2 + el] = __float2half_rn(hi ? x[j] : x[j] * 16.0f);
-      }
+      if (w == 0) col_f[r] = !fine ? __int_as_float(0x7fc00000) : up > 0.0f ? a.score_scale / up : 0.0f;
     }
-    __syncthreads();
+    __syncwarp();
 
-    float f[NT][2], qs[NT][2][NG];
-    int see[NT][2];  // keys that the row sees
+    float f[NC], qs[NC][NG];
+    int see[NC];  // keys that the row sees
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt)
+    for (int q = 0; q < NC; ++q) {
+      const int r = row_of(q);
+      f[q] = col_f[r];
 #pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        const int r = nt * 8 + 2 * c + j;
-        f[nt][j] = col_f[r];
-#pragma unroll
-        for (int k = 0; k < NG; ++k) qs[nt][j][k] = col_q[r * NG + k];
-        see[nt][j] = r < rows ? sq.ctx - a.T + 1 + (row0 + r) / a.group : -(1 << 30);
-      }
+      for (int k = 0; k < NG; ++k) qs[q][k] = col_q[r * NG + k];
+      see[q] = r < rows ? sq.ctx - a.T + 1 + (row0 + r) / a.group : -(1 << 30);
+    }
     const int see_least = sq.ctx - a.T + 1 + row0 / a.group;
     const int see_most = sq.ctx - a.T + 1 + (row0 + rows - 1) / a.group;
 
-    float o[KS][NT][4];  // m tiles: (group, high half of the word, half of that), 16 channels each
-    float l[NT][2], mref[NT][2], mo[NT][2][NG];
+    float o[4 * NG][NT][4];  // m tiles: (group, high half of the word, half of that), 16 channels each
+    float l[NC], mref[NC], mo[NC][NG];
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
+    for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-      for (int k = 0; k < KS; ++k)
+      for (int k = 0; k < 4 * NG; ++k)
 #pragma unroll
         for (int e = 0; e < 4; ++e) o[k][nt][e] = 0.0f;
 #pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        l[nt][j] = 0.0f;
-        mref[nt][j] = -INFINITY;
+    for (int q = 0; q < NC; ++q) {
+      l[q] = 0.0f;
+      mref[q] = kNone;
 #pragma unroll
-        for (int k = 0; k < NG; ++k) mo[nt][j][k] = 0.0f;
-      }
+      for (int k = 0; k < NG; ++k) mo[q][k] = 0.0f;
     }
     float vscale = 1.0f;  // power of two that the value scales are multiplied by
     bool fresh = true;
 
-    const int t_end = min(sq.first + (ra + n_rounds) * kWarps, sq.last);
-    for (int t = sq.first + ra * kWarps + warp; t < t_end; t += kWarps) {
-      const bool came = !(bad >> cur & 1u);
-      if (came && !dead) {
-        const bool ok = mbar_wait(bars + cur, phase >> cur & 1u, &abort_flag, a.err);
-        if (!__all_sync(0xffffffffu, ok)) dead = true;
+    // One record.  MASKED: some row does not see some token of it.
+    auto record = [&](auto masked_tag, int t) {
+      constexpr bool MASKED = decltype(masked_tag)::value;
+      const uint8_t* rec = ring + cur * P::RECORD;
+      uint32_t kw[2][2 * NG], kp[2][NG], vp[2][NG], vw[4][NG];
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const int tok = e ? tok1 : tok0;
+        load_words(rec + tok * P::ROW + c * (8 * NG), kw[e]);
+        load_words(rec + P::K_PAIRS + tok * P::PAIRS, kp[e]);
+        load_words(rec + P::V_PAIRS + tok * P::PAIRS, vp[e]);
       }
-      if (!dead) {
-        if (came) {
-          phase ^= 1u << cur;
-          const uint8_t* rec = ring + cur * P::RECORD;
-          // ---- scores
-          uint32_t kw[2][2 * NG];
 #pragma unroll
-          for (int r = 0; r < 2; ++r) {
-            const uint8_t* at = rec + (r ? tok1 : tok0) * P::ROW + c * (8 * NG);
-            if constexpr (NG == 1) {
-              const uint2 v = *reinterpret_cast<const uint2*>(at);
-              kw[r][0] = v.x, kw[r][1] = v.y;
-            } else {
+      for (int i = 0; i < 4; ++i) load_words(rec + P::V_CODES + vtok[i] * P::ROW + 4 * NG * g, vw[i]);
+      // the record is in registers: its stage takes the next one
+      --pending;
+      __syncwarp();
+      pending += p_ok;
+      issue(cur);
+
+      // ---- scores
+      float s[2][NC];
 #pragma unroll
-              for (int k = 0; k < NG / 2; ++k) {
-                const uint4 v = *reinterpret_cast<const uint4*>(at + 16 * k);
-                kw[r][4 * k] = v.x, kw[r][4 * k + 1] = v.y, kw[r][4 * k + 2] = v.z, kw[r][4 * k + 3] = v.w;
-              }
-            }
-          }
-          float s[NT][4];
+      for (int k = 0; k < NG; ++k) {
+        int acc[KT][4];
 #pragma unroll
-          for (int nt = 0; nt < NT; ++nt)
+        for (int nt = 0; nt < KT; ++nt)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) s[nt][e] = 0.0f;
+          for (int e = 0; e < 4; ++e) acc[nt][e] = kMagicBits;
 #pragma unroll
-          for (int k = 0; k < NG; ++k) {
-            float acc[NT][4];
+        for (int wi = 0; wi < 2; ++wi) {
+          const uint32_t w0 = kw[0][NG * wi + k], w1 = kw[1][NG * wi + k];
+          const uint32_t a0 = w0 & 0x0F0F0F0Fu, a1 = w1 & 0x0F0F0F0Fu, a2 = (w0 >> 4) & 0x0F0F0F0Fu,
+                         a3 = (w1 >> 4) & 0x0F0F0F0Fu;
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-              for (int e = 0; e < 4; ++e) acc[nt][e] = 0.0f;
-#pragma unroll
-            for (int wi = 0; wi < 2; ++wi)
-#pragma unroll
-              for (int hh = 0; hh < 2; ++hh) {
-                const uint32_t x0 = kw[0][NG * wi + k] >> (8 * hh), x1 = kw[1][NG * wi + k] >> (8 * hh);
-                const uint32_t a0 = x0 & 0x000F000Fu, a1 = x1 & 0x000F000Fu, a2 = x0 & 0x00F000F0u,
-                               a3 = x1 & 0x00F000F0u;
-#pragma unroll
-                for (int nt = 0; nt < NT; ++nt) {
-                  const uint2 b = qf[(((k * 2 + wi) * 2 + hh) * NT + nt) * 32 + lane];
-                  mma_f16_16816(acc[nt], a0, a1, a2, a3, b.x, b.y);
-                }
-              }
-            const float2 p0 = __bfloat1622float2(
-                *reinterpret_cast<const __nv_bfloat162*>(rec + P::K_PAIRS + tok0 * P::PAIRS + 4 * k));
-            const float2 p1 = __bfloat1622float2(
-                *reinterpret_cast<const __nv_bfloat162*>(rec + P::K_PAIRS + tok1 * P::PAIRS + 4 * k));
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-              for (int e = 0; e < 4; ++e) {
-                const float2 p = e < 2 ? p0 : p1;
-                s[nt][e] = fmaf(p.x, acc[nt][e], fmaf(p.y, qs[nt][e & 1][k], s[nt][e]));
-              }
-          }
-          float2 vp[2][NG];
-#pragma unroll
-          for (int k = 0; k < NG; ++k)
-#pragma unroll
-            for (int r = 0; r < 2; ++r)
-              vp[r][k] = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(
-                  rec + P::V_PAIRS + (r ? tok1 : tok0) * P::PAIRS + 4 * k));
-          const int pos0 = t * kKv4Tokens + tok0, pos1 = t * kKv4Tokens + tok1;
-          const bool masked = t * kKv4Tokens + kKv4Tokens > see_least ||
-                              (a.window > 0 && t * kKv4Tokens < see_most - a.window);
-          if (masked) {  // pairs of tokens that no row sees hold anything
-            const int low = a.window > 0 ? see_least - a.window : 0;
-            const bool in0 = pos0 < see_most && pos0 >= low, in1 = pos1 < see_most && pos1 >= low;
-#pragma unroll
-            for (int k = 0; k < NG; ++k) {
-              if (!in0) vp[0][k] = make_float2(0.0f, 0.0f);
-              if (!in1) vp[1][k] = make_float2(0.0f, 0.0f);
-            }
-          }
-          bool need = false;
-          unsigned sees = 0;  // bit 4 nt + e: the key belongs to the row
-#pragma unroll
-          for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              float v = s[nt][e] * f[nt][e & 1];
-              if constexpr (CAP) v = a.cap_log2 * tanh_exp(v);
-              if (masked) {
-                const int pos = e < 2 ? pos0 : pos1, n = see[nt][e & 1];
-                const bool in = pos < n && (a.window <= 0 || pos >= n - a.window);
-                sees |= static_cast<unsigned>(in) << (4 * nt + e);
-                v = in ? v : -INFINITY;
-              }
-              s[nt][e] = v;
-              need |= v > mref[nt][e & 1] + kSlack;
-            }
-#pragma unroll
-          for (int k = 0; k < NG; ++k) need |= vp[0][k].x * vscale > kScaleMax || vp[1][k].x * vscale > kScaleMax;
-          // ---- new references and scaling, where a score or a scale outgrew them
-          if (__any_sync(0xffffffffu, need)) {
-            float smax = 0.0f;
-#pragma unroll
-            for (int k = 0; k < NG; ++k)
-#pragma unroll
-              for (int r = 0; r < 2; ++r)
-                if (vp[r][k].x <= 3.3895314e38f) smax = fmaxf(smax, vp[r][k].x);
-#pragma unroll
-            for (int off = 4; off < 32; off <<= 1) smax = fmaxf(smax, __shfl_xor_sync(0xffffffffu, smax, off));
-            float fo = 1.0f;
-            if (smax > 0.0f && (fresh || smax * vscale > kScaleMax)) {
-              const float ns = ldexpf(1.0f, min(kScaleTarget - ilogbf(smax), 126));
-              fo = ns / vscale;
-              vscale = ns;
-              if (fresh) fo = 1.0f;
-              fresh = false;
-            }
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-              for (int j = 0; j < 2; ++j) {
-                float m = fmaxf(s[nt][j], s[nt][j + 2]);
-#pragma unroll
-                for (int off = 4; off < 32; off <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, off));
-                m = fmaxf(m, mref[nt][j]);
-                const float fac = mref[nt][j] == -INFINITY ? 0.0f : ex2(mref[nt][j] - m);
-                mref[nt][j] = m;
-                l[nt][j] *= fac;
-#pragma unroll
-                for (int k = 0; k < NG; ++k) mo[nt][j][k] *= fac;
-#pragma unroll
-                for (int k = 0; k < KS; ++k) {
-                  o[k][nt][j] *= fac * fo;
-                  o[k][nt][j + 2] *= fac * fo;
-                }
-              }
-          }
-          // ---- weights
-#pragma unroll
-          for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const float m = mref[nt][e & 1];
-              s[nt][e] = ex2(s[nt][e] - (m == -INFINITY ? 0.0f : m));
-              l[nt][e & 1] += s[nt][e];
-            }
-          // ---- outputs
-#pragma unroll
-          for (int k = 0; k < NG; ++k) {
-            uint32_t b[NT][2];
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt) {
-              float w[4];
-#pragma unroll
-              for (int e = 0; e < 4; ++e) {
-                const float2 p = vp[e >> 1][k];
-                w[e] = s[nt][e] * (p.x * vscale);
-                float pm = s[nt][e] * p.y;
-                if (masked && !(sees >> (4 * nt + e) & 1u)) w[e] = pm = 0.0f;  // a NaN that only later rows see
-                mo[nt][e & 1][k] += pm;
-              }
-              movmatrix_trans(pack_f16(w[0], w[1]), b[nt][0]);
-              movmatrix_trans(pack_f16(w[2], w[3]), b[nt][1]);
-            }
-            uint32_t vw[4];
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-              vw[i] = *reinterpret_cast<const uint32_t*>(rec + P::V_CODES + vtok[i] * P::ROW + 4 * (NG * g + k));
-#pragma unroll
-            for (int hv = 0; hv < 2; ++hv) {
-              const uint32_t y0 = __byte_perm(vw[0], vw[1], hv ? 0x7632 : 0x5410);
-              const uint32_t y1 = __byte_perm(vw[2], vw[3], hv ? 0x7632 : 0x5410);
-#pragma unroll
-              for (int hh = 0; hh < 2; ++hh) {
-                const uint32_t x0 = y0 >> (8 * hh), x1 = y1 >> (8 * hh);
-                const uint32_t a0 = x0 & 0x000F000Fu, a1 = x0 & 0x00F000F0u, a2 = x1 & 0x000F000Fu,
-                               a3 = x1 & 0x00F000F0u;
-#pragma unroll
-                for (int nt = 0; nt < NT; ++nt) mma_f16_16816(o[(k * 2 + hv) * 2 + hh][nt], a0, a1, a2, a3, b[nt][0], b[nt][1]);
-              }
-            }
+          for (int nt = 0; nt < KT; ++nt) {
+            const uint2 b = qf[((k * 2 + wi) * KT + nt) * 32 + lane];
+            mma_u8s8_16832(acc[nt], a0, a1, a2, a3, b.x, b.y);
           }
         }
+#pragma unroll
+        for (int e = 0; e < 2; ++e)
+#pragma unroll
+          for (int q = 0; q < NC; ++q) {
+            const int hi = RT == 0 ? acc[0][2 * e] : acc[(q >> 1) * 2 % KT][2 * e + (q & 1)];
+            const int lo = RT == 0 ? acc[0][2 * e + 1] : acc[((q >> 1) * 2 + 1) % KT][2 * e + (q & 1)];
+            const float dot = fmaf(__int_as_float(hi) - kMagic, 256.0f, __int_as_float(lo) - kMagic);
+            const float m = pair_min(kp[e][k]) * qs[q][k];
+            s[e][q] = fmaf(pair_scale(kp[e][k]), dot, k == 0 ? m : s[e][q] + m);
+          }
+      }
+      // ---- distance of the scores to their references; the value scales as operands
+      float d[2][NC], vs[2][NG];
+      bool in[2][NC];
+      const int pos = t * kKv4Tokens;
+      if constexpr (MASKED) {
+        const int low = a.window > 0 ? see_least - a.window : 0;
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const int at = pos + (e ? tok1 : tok0);
+          if (!(at < see_most && at >= low))  // no row sees the token: its pairs hold anything
+#pragma unroll
+            for (int k = 0; k < NG; ++k) vp[e][k] = 0;
+#pragma unroll
+          for (int q = 0; q < NC; ++q) in[e][q] = at < see[q] && (a.window <= 0 || at >= see[q] - a.window);
+        }
+      }
+      bool need = false;
+      if constexpr (CAP)
+#pragma unroll
+        for (int e = 0; e < 2; ++e)
+#pragma unroll
+          for (int q = 0; q < NC; ++q) s[e][q] = a.cap_log2 * tanh_exp(s[e][q] * f[q]);
+      auto distance = [&](int e, int q) {
+        const float x = CAP ? s[e][q] - mref[q] : fmaf(s[e][q], f[q], -mref[q]);
+        return !MASKED || in[e][q] ? x : -INFINITY;
+      };
+      auto score = [&](int e, int q) {
+        const float x = CAP ? s[e][q] : s[e][q] * f[q];
+        return !MASKED || in[e][q] ? x : -INFINITY;
+      };
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+#pragma unroll
+        for (int q = 0; q < NC; ++q) {
+          d[e][q] = distance(e, q);
+          need |= d[e][q] > kSlack;
+        }
+        float top = 0.0f;
+#pragma unroll
+        for (int k = 0; k < NG; ++k) {
+          vs[e][k] = pair_scale(vp[e][k]) * vscale;
+          top = fmaxf(top, vs[e][k]);
+        }
+        need |= top > kScaleMax;
+      }
+      // ---- new references and scaling, where a score or a scale outgrew them
+      if (__any_sync(0xffffffffu, need)) {
+        float smax = 0.0f;
+#pragma unroll
+        for (int k = 0; k < NG; ++k)
+#pragma unroll
+          for (int e = 0; e < 2; ++e)
+            if (pair_scale(vp[e][k]) <= kFltMax) smax = fmaxf(smax, pair_scale(vp[e][k]));
+#pragma unroll
+        for (int off = 4; off < 32; off <<= 1) smax = fmaxf(smax, __shfl_xor_sync(0xffffffffu, smax, off));
+        float fo = 1.0f;
+        if (smax > 0.0f && (fresh || smax * vscale > kScaleMax)) {
+          const float ns = ldexpf(1.0f, min(kScaleTarget - ilogbf(smax), 126));
+          fo = fresh ? 1.0f : ns / vscale;
+          vscale = ns;
+          fresh = false;
+        }
+        float fac[NC];
+#pragma unroll
+        for (int q = 0; q < NC; ++q) {
+          float m = fmaxf(score(0, q), score(1, q));
+#pragma unroll
+          for (int off = 4; off < 32; off <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, off));
+          m = fmaxf(m, mref[q]);
+          fac[q] = ex2(mref[q] - m);
+          mref[q] = m;
+          l[q] *= fac[q];
+#pragma unroll
+          for (int k = 0; k < NG; ++k) mo[q][k] *= fac[q];
+        }
+#pragma unroll
+        for (int k = 0; k < 4 * NG; ++k)
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[k][nt][e] *= fac[RT == 0 ? 0 : (nt * 2 + (e & 1)) % NC] * fo;
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+#pragma unroll
+          for (int q = 0; q < NC; ++q) d[e][q] = distance(e, q);
+#pragma unroll
+          for (int k = 0; k < NG; ++k) vs[e][k] = pair_scale(vp[e][k]) * vscale;
+        }
+      }
+      // ---- weights
+#pragma unroll
+      for (int e = 0; e < 2; ++e)
+#pragma unroll
+        for (int q = 0; q < NC; ++q) {
+          d[e][q] = ex2(d[e][q]);
+          l[q] += d[e][q];
+        }
+      // ---- outputs
+#pragma unroll
+      for (int k = 0; k < NG; ++k) {
+        uint32_t b[NT][2];
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          float w[NC];
+#pragma unroll
+          for (int q = 0; q < NC; ++q) {
+            w[q] = d[e][q] * vs[e][k];
+            if constexpr (MASKED) {  // a NaN pair that only later rows see
+              w[q] = in[e][q] ? w[q] : 0.0f;
+              mo[q][k] += in[e][q] ? d[e][q] * pair_min(vp[e][k]) : 0.0f;
+            } else {
+              mo[q][k] = fmaf(d[e][q], pair_min(vp[e][k]), mo[q][k]);
+            }
+          }
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+            movmatrix_trans(RT == 0 ? pack_f16(w[0], 0.0f) : pack_f16(w[2 * nt % NC], w[(2 * nt + 1) % NC]), b[nt][e]);
+        }
+#pragma unroll
+        for (int hv = 0; hv < 2; ++hv) {
+          const uint32_t y0 = __byte_perm(vw[0][k], vw[1][k], hv ? 0x7632 : 0x5410);
+          const uint32_t y1 = __byte_perm(vw[2][k], vw[3][k], hv ? 0x7632 : 0x5410);
+#pragma unroll
+          for (int hh = 0; hh < 2; ++hh) {
+            const uint32_t x0 = y0 >> (8 * hh), x1 = y1 >> (8 * hh);
+            const uint32_t a0 = x0 & 0x000F000Fu, a1 = x0 & 0x00F000F0u, a2 = x1 & 0x000F000Fu,
+                           a3 = x1 & 0x00F000F0u;
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+              mma_f16_16816(o[(k * 2 + hv) * 2 + hh][nt], a0, a1, a2, a3, b[nt][0], b[nt][1]);
+          }
+        }
+      }
+    };
+
+    const int t_end = min(sq.first + (ra + n_rounds) * a.per, sq.last);
+    for (int t = sq.first + ra * a.per; t < t_end && !dead; ++t) {
+      if (bad >> cur & 1u) {  // no such block: its tokens count as masked
         --pending;
-        __syncwarp();
         pending += p_ok;
         issue(cur);
-        cur = cur + 1 == STAGES ? 0 : cur + 1;
+      } else {
+        const uint32_t parity = phase >> cur & 1u;
+        bool ok = mbar_try_wait(smem_u32(bars + cur), parity);
+        if (!__all_sync(0xffffffffu, ok)) {
+          ok = wait_slow(bars + cur, parity, &abort_flag, a.err);
+          if (!__all_sync(0xffffffffu, ok)) {
+            dead = true;
+            break;
+          }
+        }
+        phase ^= 1u << cur;
+        if (t * kKv4Tokens + kKv4Tokens > see_least || (a.window > 0 && t * kKv4Tokens < see_most - a.window))
+          record(std::true_type{}, t);
+        else
+          record(std::false_type{}, t);
       }
+      cur = cur + 1 == STAGES ? 0 : cur + 1;
     }
 
-    // ---- the warps' shares of the item joined
-    const int busy = min(kWarps, max(t_end - (sq.first + ra * kWarps), 0));  // warps that had a record
+    // ---- the item's result, or this worker's part of it
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt)
+    for (int q = 0; q < NC; ++q) {
 #pragma unroll
-      for (int j = 0; j < 2; ++j) {
+      for (int off = 4; off < 32; off <<= 1) {
+        l[q] += __shfl_xor_sync(0xffffffffu, l[q], off);
 #pragma unroll
-        for (int off = 4; off < 32; off <<= 1) {
-          l[nt][j] += __shfl_xor_sync(0xffffffffu, l[nt][j], off);
-#pragma unroll
-          for (int k = 0; k < NG; ++k) mo[nt][j][k] += __shfl_xor_sync(0xffffffffu, mo[nt][j][k], off);
-        }
-        if (g == 0) ml[warp * ROWS + nt * 8 + 2 * c + j] = make_float2(mref[nt][j], l[nt][j]);
+        for (int k = 0; k < NG; ++k) mo[q][k] += __shfl_xor_sync(0xffffffffu, mo[q][k], off);
       }
-    __syncthreads();
-    if (warp < busy) {
-      const float inv = 1.0f / vscale;
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          const int r = nt * 8 + 2 * c + j;
-          if (r >= rows) continue;
-          float top = -INFINITY;
-          for (int w = 0; w < busy; ++w) top = fmaxf(top, ml[w * ROWS + r].x);
-          const float fac = mref[nt][j] == -INFINITY ? 0.0f : ex2(mref[nt][j] - top);
-          float* dst = slab + (warp * a.slab_rows + r) * S::SLAB_ROW + 8 * g;
-#pragma unroll
-          for (int k = 0; k < NG; ++k)
-#pragma unroll
-            for (int hv = 0; hv < 2; ++hv) {
-              // channels 8 g + 4 hv + 2 hh (codes as u 2^-24) and the next one (u 2^-20)
-              const float(&x)[4] = o[(k * 2 + hv) * 2][nt];
-              const float(&y)[4] = o[(k * 2 + hv) * 2 + 1][nt];
-              const float mk = mo[nt][j][k];
-              *reinterpret_cast<float4*>(dst + 64 * k + 4 * hv) = make_float4(
-                  fac * fmaf(x[j] * 0x1p24f, inv, mk), fac * fmaf(x[j + 2] * 0x1p20f, inv, mk),
-                  fac * fmaf(y[j] * 0x1p24f, inv, mk), fac * fmaf(y[j + 2] * 0x1p20f, inv, mk));
-            }
-        }
     }
-    __syncthreads();
+    if (ra == 0 && lane == 0) {
+      Kv4Item it;
+      it.first = item_first;
+      it.rounds = sq.rounds;
+      a.items[static_cast<int64_t>(seq) * subs + sub] = it;
+    }
     const bool whole = ra == 0 && n_rounds == sq.rounds;
-    const int64_t slot = 2 * static_cast<int64_t>(blockIdx.x) + (ra == 0 ? 1 : 0);
-    for (int x = tid; x < rows * (D / 4); x += kThreads) {
-      const int r = x / (D / 4), ch = x % (D / 4) * 4;
-      float top = -INFINITY, sum = 0.0f;
-      for (int w = 0; w < busy; ++w) top = fmaxf(top, ml[w * ROWS + r].x);
-      float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-      for (int w = 0; w < busy; ++w) {
-        const float2 e = ml[w * ROWS + r];
-        sum += e.x == -INFINITY ? 0.0f : e.y * ex2(e.x - top);
-        const float4 y = *reinterpret_cast<const float4*>(slab + (w * a.slab_rows + r) * S::SLAB_ROW + ch);
-        v.x += y.x, v.y += y.y, v.z += y.z, v.w += y.w;
-      }
-      if (whole) {
-        const int i = (row0 + r) / a.group, hq = h * a.group + (row0 + r) - i * a.group;
-        const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-        __nv_bfloat16* dst = a.out + (static_cast<int64_t>(seq) * a.T + i) * a.out_stride + static_cast<int64_t>(hq) * D + ch;
-        *reinterpret_cast<uint2*>(dst) = make_uint2(pack_bf16(v.x * inv, v.y * inv), pack_bf16(v.z * inv, v.w * inv));
-      } else {
-        if (ch == 0) a.part_ml[slot * ROWS + r] = make_float2(top, sum);
-        *reinterpret_cast<float4*>(a.part_o + (slot * ROWS + r) * D + ch) = v;
+    const int64_t slot = 2 * static_cast<int64_t>(worker) + (ra == 0 ? 1 : 0);
+    const float inv = 1.0f / vscale;
+#pragma unroll
+    for (int q = 0; q < NC; ++q) {
+      const int r = row_of(q), nt = q >> 1, j = q & 1;
+      if (r >= rows) continue;
+      const int i = (row0 + r) / a.group, hq = h * a.group + (row0 + r) - i * a.group;
+      __nv_bfloat16* dst =
+          a.out + (static_cast<int64_t>(seq) * a.T + i) * a.out_stride + static_cast<int64_t>(hq) * D + 8 * g;
+      float* part = a.part_o + (slot * ROWS + r) * D + 8 * g;
+      const float over = l[q] == 0.0f ? 0.0f : 1.0f / l[q];
+      if (!whole && g == 0) a.part_ml[slot * ROWS + r] = make_float2(mref[q], l[q]);
+#pragma unroll
+      for (int k = 0; k < NG; ++k) {
+        float v[8];  // channels 8 g + 4 hv + 2 hh (codes as u 2^-24) and the next one (u 2^-20)
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+          v[2 * x] = fmaf(o[k * 4 + x][nt][j] * 0x1p24f, inv, mo[q][k]);
+          v[2 * x + 1] = fmaf(o[k * 4 + x][nt][j + 2] * 0x1p20f, inv, mo[q][k]);
+        }
+        if (whole) {
+          *reinterpret_cast<uint4*>(dst + 64 * k) =
+              make_uint4(pack_bf16(v[0] * over, v[1] * over), pack_bf16(v[2] * over, v[3] * over),
+                         pack_bf16(v[4] * over, v[5] * over), pack_bf16(v[6] * over, v[7] * over));
+        } else {
+          *reinterpret_cast<float4*>(part + 64 * k) = make_float4(v[0], v[1], v[2], v[3]);
+          *reinterpret_cast<float4*>(part + 64 * k + 4) = make_float4(v[4], v[5], v[6], v[7]);
+        }
       }
     }
     left -= n_rounds;
+    item_first += sq.rounds;
     ra = 0;
     if (++sub == subs && left > 0) {
       sub = 0;
@@ -683,101 +720,111 @@ __global__ void __launch_bounds__(kThreads, kv4_ctas_per_sm<D, NT>()) kv4_attn_k
       if (!(bad >> st & 1u)) mbar_wait(bars + st, phase >> st & 1u, nullptr, a.err);
 }
 
-// Joins the parts of the items that span CTAs.  CTA (c - 1, r) looks at the boundary between CTAs c - 1 and c of
-// the first kernel: if it is the first one inside its item, it joins row r of the item, parts in CTA order,
-// eight warps taking every eighth part.
-template <int D, int NT>
-__global__ void __launch_bounds__(kThreads) kv4_join_kernel(const Kv4AttnArgs a) {
-  constexpr int ROWS = 8 * NT, N = D / 32;
-  __shared__ float acc[kWarps][D];
-  __shared__ float2 ml[kWarps];
+// Joins the parts of the items that span workers: a block takes row r of an item, parts in worker order, every
+// fourth one a warp.
+template <int D, int RT>
+__global__ void __launch_bounds__(kJoinThreads) kv4_join_kernel(const Kv4AttnArgs a) {
+  constexpr int ROWS = Kv4Rows<RT>::ROWS, N = D / 32, WARPS = kJoinThreads / 32;
+  __shared__ float acc[WARPS][D];
+  __shared__ float2 ml[WARPS];
   pdl_wait();
   pdl_launch_dependents();
-  const int cta = blockIdx.x + 1, r = blockIdx.y;
-  const int active = static_cast<int>(a.head[0]);
-  if (cta >= active) return;
+  const int workers = static_cast<int>(a.head[0]);
   const int64_t total = a.head[1];
-  const Kv4Start st = a.starts[cta];
-  const int64_t here = range_start(cta, total, active), before = range_start(cta - 1, total, active);
-  if (here == st.item_first || before > st.item_first) return;
-  const int h = st.sub / a.chunks, row0 = (st.sub - h * a.chunks) * ROWS;
-  if (r >= a.group * a.T - row0) return;
-  const int last = cta_of(st.item_first + st.rounds - 1, total, active);
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  float m = -INFINITY, l = 0.0f, o[N];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, subs = a.hkv * a.chunks;
+  const int64_t work = static_cast<int64_t>(a.batch) * subs * a.slab_rows;
+  for (int64_t x = blockIdx.x; x < work; x += gridDim.x) {
+    const int64_t item = x / a.slab_rows;
+    const int r = static_cast<int>(x - item * a.slab_rows);
+    const Kv4Item it = a.items[item];
+    const int first = worker_of(it.first, total, workers), last = worker_of(it.first + it.rounds - 1, total, workers);
+    if (first == last) continue;
+    const int seq = static_cast<int>(item / subs), sub = static_cast<int>(item - static_cast<int64_t>(seq) * subs);
+    const int h = sub / a.chunks, row0 = (sub - h * a.chunks) * ROWS;
+    if (r >= a.group * a.T - row0) continue;
+    float m = kNone, l = 0.0f, o[N];
 #pragma unroll
-  for (int j = 0; j < N; ++j) o[j] = 0.0f;
+    for (int j = 0; j < N; ++j) o[j] = 0.0f;
 #pragma unroll 4
-  for (int p = cta - 1 + warp; p <= last; p += kWarps) {
-    const int64_t slot = (2 * static_cast<int64_t>(p) + (p == cta - 1 ? 1 : 0)) * ROWS + r;
-    const float2 e = a.part_ml[slot];
-    float x[N];
+    for (int p = first + warp; p <= last; p += WARPS) {
+      const int64_t slot = (2 * static_cast<int64_t>(p) + (p == first ? 1 : 0)) * ROWS + r;
+      const float2 e = a.part_ml[slot];
+      float y[N];
 #pragma unroll
-    for (int j = 0; j < N; ++j) x[j] = a.part_o[slot * D + 32 * j + lane];
-    const float top = fmaxf(m, e.x);
-    const float fm = m == -INFINITY ? 0.0f : ex2(m - top), fe = e.x == -INFINITY ? 0.0f : ex2(e.x - top);
-    l = l * fm + e.y * fe;
+      for (int j = 0; j < N; ++j) y[j] = a.part_o[slot * D + 32 * j + lane];
+      const float top = fmaxf(m, e.x);
+      const float fm = ex2(m - top), fe = ex2(e.x - top);
+      l = l * fm + e.y * fe;
 #pragma unroll
-    for (int j = 0; j < N; ++j) o[j] = o[j] * fm + x[j] * fe;
-    m = top;
-  }
-  if (lane == 0) ml[warp] = make_float2(m, l);
-#pragma unroll
-  for (int j = 0; j < N; ++j) acc[warp][32 * j + lane] = o[j];
-  __syncthreads();
-  float top = -INFINITY;
-  for (int w = 0; w < kWarps; ++w) top = fmaxf(top, ml[w].x);
-  const int i = (row0 + r) / a.group, hq = h * a.group + (row0 + r) - i * a.group;
-  __nv_bfloat16* dst = a.out + (static_cast<int64_t>(st.seq) * a.T + i) * a.out_stride + static_cast<int64_t>(hq) * D;
-  for (int ch = threadIdx.x; ch < D; ch += kThreads) {
-    float sum = 0.0f, v = 0.0f;
-    for (int w = 0; w < kWarps; ++w) {
-      const float f = ml[w].x == -INFINITY ? 0.0f : ex2(ml[w].x - top);
-      sum += ml[w].y * f;
-      v += acc[w][ch] * f;
+      for (int j = 0; j < N; ++j) o[j] = o[j] * fm + y[j] * fe;
+      m = top;
     }
-    dst[ch] = __float2bfloat16_rn(sum == 0.0f ? 0.0f : v / sum);
+    __syncthreads();  // the row before has been read
+    if (lane == 0) ml[warp] = make_float2(m, l);
+#pragma unroll
+    for (int j = 0; j < N; ++j) acc[warp][32 * j + lane] = o[j];
+    __syncthreads();
+    float top = kNone;
+#pragma unroll
+    for (int w = 0; w < WARPS; ++w) top = fmaxf(top, ml[w].x);
+    const int i = (row0 + r) / a.group, hq = h * a.group + (row0 + r) - i * a.group;
+    __nv_bfloat16* dst = a.out + (static_cast<int64_t>(seq) * a.T + i) * a.out_stride + static_cast<int64_t>(hq) * D;
+    for (int ch = threadIdx.x; ch < D; ch += kJoinThreads) {
+      float sum = 0.0f, v = 0.0f;
+#pragma unroll
+      for (int w = 0; w < WARPS; ++w) {
+        const float f = ex2(ml[w].x - top);
+        sum += ml[w].y * f;
+        v += acc[w][ch] * f;
+      }
+      dst[ch] = __float2bfloat16_rn(sum == 0.0f ? 0.0f : v / sum);
+    }
   }
 }
 
-// Column tiles of 8 query rows that a CTA carries: up to 16 rows in one pass over the cache.
-int64_t kv4_tiles(int64_t rows) { return rows <= 8 ? 1 : 2; }
+// Query rows that a CTA carries in one pass over the cache: 4, 8 or 16.
+int kv4_rt(int64_t rows) { return rows <= 4 ? 0 : rows <= 8 ? 1 : 2; }
+int64_t kv4_rows(int rt) { return rt == 0 ? 4 : 8 * rt; }
 
-int64_t kv4_grid(int64_t sms, int64_t head_dim, int64_t nt) { return sms * (head_dim == 256 || nt > 1 ? 1 : 2); }
+int64_t kv4_grid(int64_t sms, int64_t head_dim, int rt) { return sms * (head_dim == 256 || rt > 1 ? 1 : 2); }
 
 struct Kv4Workspace {
-  int64_t starts, ml, o, bytes;
+  int64_t items, ml, o, bytes;
 };
-Kv4Workspace kv4_workspace(int64_t grid, int64_t nt, int64_t head_dim) {
+Kv4Workspace kv4_workspace(int64_t grid, int rt, int64_t head_dim, int64_t items) {
   Kv4Workspace w;
   auto up = [](int64_t x) { return (x + 255) / 256 * 256; };
-  w.starts = 256;
-  w.ml = w.starts + up(grid * static_cast<int64_t>(sizeof(Kv4Start)));
-  w.o = w.ml + up(2 * grid * 8 * nt * 8);
-  w.bytes = w.o + 2 * grid * 8 * nt * head_dim * 4;
+  w.items = 256;
+  w.ml = w.items + up(items * static_cast<int64_t>(sizeof(Kv4Item)));
+  w.o = w.ml + up(2 * grid * kWarps * kv4_rows(rt) * 8);
+  w.bytes = w.o + 2 * grid * kWarps * kv4_rows(rt) * head_dim * 4;
   return w;
 }
 
-template <int D, int NT, bool CAP>
-int kv4_launch_cap(const Kv4AttnArgs& a, int64_t grid, int64_t most_rounds, cudaStream_t st) {
-  const size_t smem = Kv4Smem<D, NT>::bytes(a.slab_rows);
-  MVB_TRY(set_smem(kv4_attn_kernel<D, NT, CAP>, smem, "kv4_attention"));
-  MVB_TRY(launch("kv4_attention", kv4_attn_kernel<D, NT, CAP>, dim3(static_cast<unsigned>(grid)), dim3(kThreads), smem,
+template <int D, int RT, bool CAP>
+int kv4_launch_cap(const Kv4AttnArgs& a, int64_t grid, int64_t join_grid, cudaStream_t st) {
+  constexpr size_t smem = Kv4Smem<D, RT>::BYTES;
+  MVB_TRY(set_smem(kv4_attn_kernel<D, RT, CAP>, smem, "kv4_attention"));
+  MVB_TRY(launch("kv4_attention", kv4_attn_kernel<D, RT, CAP>, dim3(static_cast<unsigned>(grid)), dim3(kThreads), smem,
                  st, a));
-  if (most_rounds <= 1 || grid <= 1) return MVB_OK;  // no item can span CTAs
-  return launch_dependent("kv4_attention_join", kv4_join_kernel<D, NT>,
-                          dim3(static_cast<unsigned>(grid - 1), static_cast<unsigned>(a.slab_rows)), dim3(kThreads), 0,
-                          st, a);
+  if (join_grid == 0) return MVB_OK;
+  return launch_dependent("kv4_attention_join", kv4_join_kernel<D, RT>, dim3(static_cast<unsigned>(join_grid)),
+                          dim3(kJoinThreads), 0, st, a);
+}
+
+template <int D, int RT>
+int kv4_launch_rows(const Kv4AttnArgs& a, int64_t grid, int64_t join_grid, cudaStream_t st) {
+  return a.cap_log2 > 0.0f ? kv4_launch_cap<D, RT, true>(a, grid, join_grid, st)
+                           : kv4_launch_cap<D, RT, false>(a, grid, join_grid, st);
 }
 
 template <int D>
-int kv4_launch(const Kv4AttnArgs& a, int64_t nt, int64_t grid, int64_t most_rounds, cudaStream_t st) {
-  const bool cap = a.cap_log2 > 0.0f;
-  if (nt == 1)
-    return cap ? kv4_launch_cap<D, 1, true>(a, grid, most_rounds, st)
-               : kv4_launch_cap<D, 1, false>(a, grid, most_rounds, st);
-  return cap ? kv4_launch_cap<D, 2, true>(a, grid, most_rounds, st)
-             : kv4_launch_cap<D, 2, false>(a, grid, most_rounds, st);
+int kv4_launch(const Kv4AttnArgs& a, int rt, int64_t grid, int64_t join_grid, cudaStream_t st) {
+  switch (rt) {
+    case 0: return kv4_launch_rows<D, 0>(a, grid, join_grid, st);
+    case 1: return kv4_launch_rows<D, 1>(a, grid, join_grid, st);
+    default: return kv4_launch_rows<D, 2>(a, grid, join_grid, st);
+  }
 }
 
 }  // namespace
@@ -788,12 +835,13 @@ using namespace mvb;
 extern "C" int64_t mvb_paged_attention_decode_kv4_workspace_bytes(int64_t batch, int64_t query_len,
                                                                   int64_t num_q_heads, int64_t num_kv_heads,
                                                                   int64_t head_dim, int device) {
-  (void)batch;
-  if (num_kv_heads <= 0 || query_len <= 0) return 0;
+  if (batch <= 0 || num_kv_heads <= 0 || query_len <= 0) return 0;
   int sms = mvb_num_sms(device);
   if (sms <= 0) sms = 148;
-  const int64_t nt = kv4_tiles(num_q_heads / num_kv_heads * query_len);
-  return kv4_workspace(kv4_grid(sms, head_dim, nt), nt, head_dim).bytes;
+  const int64_t rows = num_q_heads / num_kv_heads * query_len;
+  const int rt = kv4_rt(rows);
+  const int64_t chunks = (rows + kv4_rows(rt) - 1) / kv4_rows(rt);
+  return kv4_workspace(kv4_grid(sms, head_dim, rt), rt, head_dim, batch * num_kv_heads * chunks).bytes;
 }
 
 extern "C" int mvb_paged_attention_decode_kv4(void* out, int64_t out_stride, const void* q, int64_t q_stride,
@@ -851,28 +899,34 @@ extern "C" int mvb_paged_attention_decode_kv4(void* out, int64_t out_stride, con
 
   const int sms = current_sm_count();
   MVB_REQUIRE(sms > 0, "%s: no device", what);
-  const int64_t rows = num_q_heads / num_kv_heads * query_len, nt = kv4_tiles(rows);
-  const int64_t chunks = (rows + 8 * nt - 1) / (8 * nt);
-  const int64_t most_rounds = (max_blocks * recs + kWarps - 1) / kWarps;
+  const int64_t rows = num_q_heads / num_kv_heads * query_len;
+  const int rt = kv4_rt(rows);
+  const int64_t chunks = (rows + kv4_rows(rt) - 1) / kv4_rows(rt);
+  const int64_t most = max_blocks * recs;  // records of an item
   MVB_REQUIRE(num_kv_heads * chunks <= INT_MAX, "%s: heads", what);
-  int64_t grid = kv4_grid(sms, head_dim, nt);
-  const Kv4Workspace w = kv4_workspace(grid, nt, head_dim);
+  const int64_t items = batch * num_kv_heads * chunks;
+  // Short tables: an item goes to one worker and nothing is left to join.
+  const bool split = most > kShortRecords;
+  a.per = split ? 1 : static_cast<int>(most);
+  int64_t grid = kv4_grid(sms, head_dim, rt);
+  const Kv4Workspace w = kv4_workspace(grid, rt, head_dim, items);
   MVB_REQUIRE(workspace && aligned(workspace, 256) && workspace_bytes >= w.bytes,
               "%s: a workspace of %lld bytes, 256-byte aligned (got %lld)", what, (long long)w.bytes,
               (long long)workspace_bytes);
-  const int64_t bound = batch * num_kv_heads * chunks;  // items; times the rounds of the longest possible one
-  if (bound < grid && bound * most_rounds < grid) grid = bound * most_rounds;
+  if (items < grid && items * (split ? most : 1) < grid) grid = items * (split ? most : 1);
   a.chunks = static_cast<int>(chunks);
-  a.slab_rows = static_cast<int>(rows < 8 * nt ? rows : 8 * nt);
+  a.slab_rows = static_cast<int>(rows < kv4_rows(rt) ? rows : kv4_rows(rt));
   char* ws = static_cast<char*>(workspace);
   a.head = reinterpret_cast<int64_t*>(ws);
-  a.starts = reinterpret_cast<Kv4Start*>(ws + w.starts);
+  a.items = reinterpret_cast<Kv4Item*>(ws + w.items);
   a.part_ml = reinterpret_cast<float2*>(ws + w.ml);
   a.part_o = reinterpret_cast<float*>(ws + w.o);
+  int64_t join_grid = 0;
+  if (split) join_grid = items * a.slab_rows < 16LL * sms ? items * a.slab_rows : 16LL * sms;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   switch (head_dim) {
-    case 64: return kv4_launch<64>(a, nt, grid, most_rounds, st);
-    case 128: return kv4_launch<128>(a, nt, grid, most_rounds, st);
-    default: return kv4_launch<256>(a, nt, grid, most_rounds, st);
+    case 64: return kv4_launch<64>(a, rt, grid, join_grid, st);
+    case 128: return kv4_launch<128>(a, rt, grid, join_grid, st);
+    default: return kv4_launch<256>(a, rt, grid, join_grid, st);
   }
 }

@@ -89,13 +89,15 @@ def attention(q, pool, layer, tables, ctx, scale, softcap=0.0, window=0):
             if softcap:
                 z = softcap * torch.tanh(z / softcap)
             out[b, t] = torch.einsum("hrn,nhd->hrd", z.softmax(-1), vv).flatten(0, 1)
-            # Score: at most D + 64 fp32 roundings of terms whose magnitudes sum to m (the products, or
-            # scale * code products and the min's part, each within 16 times |q| |k|max): (D + 64) 2^-24 m.  The
-            # softmax turns an error d of the scores into 2 d of a weight.  Weights: rounded to 11 bits
-            # before the product with the codes (2^-11 of the span of a group), plus 2^-21 for exp2 and sums.
+            # Score: q is held in 16 bits of its row's largest magnitude (half a step of |q|max / 32512 a channel, against
+            # k), and at most D + 64 fp32 roundings of terms whose magnitudes sum to m (the products, or scale * code
+            # products and the min's part, each within 4 times |q| |k|max).  The softmax turns an error d of the scores
+            # into 2 d of a weight.  Weights: rounded to 11 bits before the product with the codes (2^-11 of the
+            # span of a group), plus 2^-21 for exp2 and sums.
             span = (vv.unflatten(-1, (-1, 64)).amax(-1) - vv.unflatten(-1, (-1, 64)).amin(-1)).amax()
             m = 4 * torch.einsum("hrd,nhd->hrn", qt.abs(), kk.abs()).amax(-1) * scale    # codes and min apart
-            weight = 2 * ((D + 64) * 2.0 ** -24 * m + 2.0 ** -21)
+            held = qt.abs().amax(-1) / 32512 / 2 * kk.abs().sum(-1).amax(0)[:, None] * scale
+            weight = 2 * (held + (D + 64) * 2.0 ** -24 * m + 2.0 ** -21)
             vmax = vv.abs().amax()
             tol[b, t] = (weight[..., None] * vmax + 2.0 ** -11 * 1.1 * (span + 2.0 ** -10 * vmax)).expand(
                 -1, -1, D).flatten(0, 1)
