@@ -41,8 +41,6 @@ namespace mvb {
 namespace {
 
 constexpr float kLog2e = 1.4426950408889634f;
-constexpr int kWarps = 8;
-constexpr int kThreads = kWarps * 32;
 constexpr int kJoinThreads = 128;
 constexpr int kShortRecords = 8;  // items of at most this many records are never split
 
@@ -57,7 +55,7 @@ constexpr float kNone = -kFltMax;     // reference of a row without a key: no sp
 constexpr float kMagic = 12582912.0f; // 1.5 * 2^23: its bits plus a small integer are the bits of the sum
 constexpr int kMagicBits = 0x4B400000;
 
-// RT: 0 = up to 4 query rows per chunk, 1 = up to 8, 2 = up to 16.
+// RT: 0 = up to 4 query rows per chunk, else up to 8 RT.
 template <int RT>
 struct Kv4Rows {
   static constexpr int NT = RT == 0 ? 1 : RT;       // n = 8 tiles of the second product
@@ -66,15 +64,15 @@ struct Kv4Rows {
   static constexpr int ROWS = RT == 0 ? 4 : 8 * RT;
 };
 
-// Records in flight per warp: an SM's share of the bandwidth needs some 45 KB.
+// BURST: records that a warp takes at once (one wait, one vote, one refill); STAGES of them are held, so that
+// an SM has some 45 KB or more under way while it computes; WARPS and CTAS (per SM) by the registers.
 template <int D, int RT>
-constexpr int kv4_stages() {
-  return D == 64 ? 6 : D == 256 && RT > 1 ? 2 : 4;
-}
-template <int D, int RT>
-constexpr int kv4_ctas_per_sm() {
-  return D == 256 || RT > 1 ? 1 : 2;
-}
+struct Kv4Cfg {
+  static constexpr int BURST = D == 256 || RT > 1 ? 1 : D == 128 ? 2 : RT == 0 ? 4 : 2;
+  static constexpr int STAGES = D == 256 ? (RT > 1 ? 2 : 3) : D == 128 ? (RT > 1 ? 4 : 2) : RT == 0 ? 2 : 4;
+  static constexpr int WARPS = D == 256 && RT == 0 ? 12 : 8;
+  static constexpr int CTAS = D == 256 || RT > 1 ? 1 : 2;
+};
 
 struct Kv4AttnArgs {
   __nv_bfloat16* out;
@@ -107,12 +105,25 @@ struct Kv4Item {
   int64_t rounds;
 };
 
-__device__ __forceinline__ int64_t range_start(int w, int64_t total, int workers) {
-  return static_cast<int64_t>(w) * total / workers;
-}
-__device__ __forceinline__ int worker_of(int64_t x, int64_t total, int workers) {
-  return static_cast<int>(((x + 1) * workers + total - 1) / total - 1);
-}
+// The rounds of the batch among the workers: each `size`, the first `more` one more.
+struct Kv4Split {
+  int64_t size, more;
+  __device__ __forceinline__ Kv4Split(int64_t total, int workers) {
+    if (total >> 32) {
+      size = total / workers;
+    } else {
+      size = static_cast<uint32_t>(total) / static_cast<uint32_t>(workers);
+    }
+    more = total - size * workers;
+  }
+  __device__ __forceinline__ int64_t start(int w) const { return w * size + (w < more ? w : more); }
+  __device__ __forceinline__ int worker(int64_t x) const {
+    const int64_t y = x - more * (size + 1);
+    if (x >> 31) return static_cast<int>(y < 0 ? x / (size + 1) : more + y / size);
+    return y < 0 ? static_cast<uint32_t>(x) / static_cast<uint32_t>(size + 1)
+                 : static_cast<int>(more) + static_cast<uint32_t>(y) / static_cast<uint32_t>(size);
+  }
+};
 
 // exp2 with results below 2^-126 flushed to zero.
 __device__ __forceinline__ float ex2(float x) {
@@ -127,19 +138,30 @@ __device__ __forceinline__ float tanh_exp(float x) {
 
 __device__ __forceinline__ void mma_f16_16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
                                               uint32_t b0, uint32_t b1) {
-  asm volatile(
-      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
       "{%0, %1, %2, %3};"
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 __device__ __forceinline__ void mma_u8s8_16832(int (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
                                                uint32_t b0, uint32_t b1) {
-  asm volatile(
-      "mma.sync.aligned.m16n8k32.row.col.s32.u8.s8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+  asm("mma.sync.aligned.m16n8k32.row.col.s32.u8.s8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
       "{%0, %1, %2, %3};"
       : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+// The first step of a sum: every element starts at `init`.
+__device__ __forceinline__ void mma_u8s8_16832_from(int (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                                                    uint32_t b0, uint32_t b1, int init) {
+  asm("mma.sync.aligned.m16n8k32.row.col.s32.u8.s8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+      "{%10, %10, %10, %10};"
+      : "=r"(d[0]), "=r"(d[1]), "=r"(d[2]), "=r"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "r"(init));
+}
+__device__ __forceinline__ uint32_t transposed(uint32_t x) {  // movmatrix_trans, free to be scheduled
+  uint32_t d;
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(x));
+  return d;
 }
 // N consecutive 32-bit words of shared memory, aligned to their size.
 template <int N>
@@ -204,27 +226,29 @@ __device__ __forceinline__ Kv4Seq kv4_seq(const Kv4AttnArgs& a, int b, bool tell
 
 template <int D, int RT>
 struct Kv4Smem {
-  static constexpr int STAGES = kv4_stages<D, RT>(), ROWS = Kv4Rows<RT>::ROWS;
+  static constexpr int STAGES = Kv4Cfg<D, RT>::STAGES, ROWS = Kv4Rows<RT>::ROWS;
   // per warp: the ring, Q operands [D / 32][KT][32 lanes] x 8 bytes, per row the score factor and the
   // sums of q per group, the ring's barriers
-  static constexpr int RING = STAGES * Kv4<D>::RECORD;
+  static constexpr int RING = STAGES * Kv4Cfg<D, RT>::BURST * Kv4<D>::RECORD;
   static constexpr int QF = RING;
   static constexpr int COL = QF + D / 32 * Kv4Rows<RT>::KT * 256;
   static constexpr int BAR = (COL + ROWS * (1 + Kv4<D>::NG) * 4 + 7) / 8 * 8;
   static constexpr int WARP = (BAR + STAGES * 8 + 127) / 128 * 128;
-  static constexpr int BYTES = kWarps * WARP;
+  static constexpr int BYTES = Kv4Cfg<D, RT>::WARPS * WARP;
 };
 
 template <int D, int RT, bool CAP>
-__global__ void __launch_bounds__(kThreads, kv4_ctas_per_sm<D, RT>()) kv4_attn_kernel(const Kv4AttnArgs a) {
+__global__ void __launch_bounds__(Kv4Cfg<D, RT>::WARPS * 32, Kv4Cfg<D, RT>::CTAS) kv4_attn_kernel(const Kv4AttnArgs a) {
   using P = Kv4<D>;
   using S = Kv4Smem<D, RT>;
   using R = Kv4Rows<RT>;
   constexpr int NG = P::NG, STAGES = S::STAGES, ROWS = R::ROWS, NT = R::NT, KT = R::KT, NC = R::NC;
+  constexpr int BURST = Kv4Cfg<D, RT>::BURST, WARPS = Kv4Cfg<D, RT>::WARPS, THREADS = WARPS * 32;
+  constexpr unsigned ALL = (1u << BURST) - 1;
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ volatile int abort_flag;
-  __shared__ int64_t scan_warp[kWarps];
-  __shared__ int64_t scan_end[kThreads];  // rounds up to and with a sequence
+  __shared__ int64_t scan_warp[WARPS];
+  __shared__ int64_t scan_end[THREADS];  // rounds up to and with a sequence
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int g = lane >> 2, c = lane & 3;
   uint8_t* ring = smem + warp * S::WARP;
@@ -242,7 +266,7 @@ __global__ void __launch_bounds__(kThreads, kv4_ctas_per_sm<D, RT>()) kv4_attn_k
   // ---- this worker's rounds, [r0, r1) of the batch's total, and the sequence that r0 lies in
   const int subs = a.hkv * a.chunks;
   int64_t carry = 0;
-  auto scan = [&](int base, bool tell) {  // rounds of 256 sequences: their running sum into scan_end
+  auto scan = [&](int base, bool tell) {  // rounds of THREADS sequences: their running sum into scan_end
     const int b = base + tid;
     int64_t incl = b < a.batch ? static_cast<int64_t>(kv4_seq(a, b, tell).rounds) * subs : 0;
 #pragma unroll
@@ -255,7 +279,7 @@ __global__ void __launch_bounds__(kThreads, kv4_ctas_per_sm<D, RT>()) kv4_attn_k
     __syncthreads();
     int64_t all = 0;
 #pragma unroll
-    for (int w = 0; w < kWarps; ++w) {
+    for (int w = 0; w < WARPS; ++w) {
       if (w < warp) incl += scan_warp[w];
       all += scan_warp[w];
     }
@@ -263,24 +287,24 @@ __global__ void __launch_bounds__(kThreads, kv4_ctas_per_sm<D, RT>()) kv4_attn_k
     carry += all;
     __syncthreads();
   };
-  for (int base = 0; base < a.batch; base += kThreads) scan(base, blockIdx.x == 0);
+  for (int base = 0; base < a.batch; base += THREADS) scan(base, blockIdx.x == 0);
   const int64_t total = carry;
-  const int workers = static_cast<int>(min(static_cast<int64_t>(gridDim.x) * kWarps, total));
+  const int workers = static_cast<int>(min(static_cast<int64_t>(gridDim.x) * WARPS, total));
   if (blockIdx.x == 0 && tid == 0) {
     a.head[0] = workers;
     a.head[1] = total;
   }
   const int worker = warp * gridDim.x + blockIdx.x;  // few rounds: spread over the SMs
   const bool busy = worker < workers;
-  const int64_t r0 = busy ? range_start(worker, total, workers) : 0;
-  const int64_t r1 = busy ? range_start(worker + 1, total, workers) : 0;
+  const Kv4Split split(total, workers);
+  const int64_t r0 = busy ? split.start(worker) : 0, r1 = busy ? split.start(worker + 1) : 0;
   int seq = 0;
   int64_t seq_first = 0;
-  if (a.batch > kThreads) carry = 0;
-  for (int base = 0; base < a.batch; base += kThreads) {
-    const int64_t before = a.batch > kThreads ? carry : 0;
-    if (a.batch > kThreads) scan(base, false);
-    for (int x = lane; x < kThreads && base + (x & ~31) < a.batch; x += 32) {
+  if (a.batch > THREADS) carry = 0;
+  for (int base = 0; base < a.batch; base += THREADS) {
+    const int64_t before = a.batch > THREADS ? carry : 0;
+    if (a.batch > THREADS) scan(base, false);
+    for (int x = lane; x < THREADS && base + (x & ~31) < a.batch; x += 32) {
       const int64_t end = scan_end[x], begin = x == 0 ? before : scan_end[x - 1];
       const unsigned hit = __ballot_sync(0xffffffffu, begin <= r0 && r0 < end);
       if (hit) {
@@ -293,20 +317,21 @@ __global__ void __launch_bounds__(kThreads, kv4_ctas_per_sm<D, RT>()) kv4_attn_k
   if (!busy) return;
 
   Kv4Seq sq = kv4_seq(a, seq, false);
-  int sub = static_cast<int>((r0 - seq_first) / sq.rounds);
+  int sub = (r0 - seq_first) >> 31 ? static_cast<int>((r0 - seq_first) / sq.rounds)
+                                   : static_cast<int>(r0 - seq_first) / sq.rounds;
   int ra = static_cast<int>(r0 - seq_first - static_cast<int64_t>(sub) * sq.rounds);
   int left = static_cast<int>(r1 - r0);
   int64_t item_first = r0 - ra;
 
-  // ---- the worker's stream of records, STAGES ahead of the arithmetic
+  // ---- the worker's stream of records, STAGES bursts ahead of the arithmetic; lane j sees to record j of a burst
   const int64_t block_bytes = static_cast<int64_t>(a.hkv) * a.recs * P::RECORD;
   int p_seq = seq, p_sub = sub, p_left = left, p_n = min(sq.rounds - ra, left);
   Kv4Seq p_sq = sq;
   int p_t = sq.first + ra * a.per, p_end = min(sq.first + (ra + p_n) * a.per, sq.last);
   int p_id = 0, p_rec = 0;
   bool p_ok = true;
-  // Settles on the next record at or after p_t, crossing into the next items, and asks for its block id
-  // (one record ahead of the copy that needs it).
+  // Settles on the next burst at or after p_t, crossing into the next items, and asks for its block ids
+  // (one burst ahead of the copies that need them).
   auto settle = [&]() {
     while (p_t >= p_end) {
       p_left -= p_n;
@@ -322,30 +347,34 @@ __global__ void __launch_bounds__(kThreads, kv4_ctas_per_sm<D, RT>()) kv4_attn_k
       p_t = p_sq.first;
       p_end = min(p_sq.first + p_n * a.per, p_sq.last);
     }
-    const int blk = a.recs == 1 ? p_t : p_t / a.recs;
-    p_rec = p_t - blk * a.recs;
-    p_id = a.tables[p_seq * a.table_stride + blk];
+    const int t = p_t + lane;
+    if (lane < BURST && t < p_end) {
+      const int blk = a.recs == 1 ? t : t / a.recs;
+      p_rec = t - blk * a.recs;
+      p_id = a.tables[p_seq * a.table_stride + blk];
+    }
   };
-  unsigned bad = 0, phase = 0;  // per stage: no record came (invalid block); parity of its barrier
+  unsigned came = 0, phase = 0;  // per stage: the records that came; parity of its barrier
   auto issue = [&](int st) {
     if (!p_ok) return;
-    if (static_cast<unsigned>(p_id) < static_cast<unsigned>(a.num_blocks)) {
-      bad &= ~(1u << st);
-      if (lane == 0) {
-        const int h = a.chunks == 1 ? p_sub : p_sub / a.chunks;
-        mbar_arrive_expect_tx(bars + st, P::RECORD);
-        bulk_load(ring + st * P::RECORD, a.pool + p_id * block_bytes + (h * a.recs + p_rec) * P::RECORD, P::RECORD,
-                  bars + st);
-      }
-    } else {
-      bad |= 1u << st;
-      if (lane == 0) report(a.err, kDevBadBlock);
+    const bool mine = lane < BURST && p_t + lane < p_end;
+    const bool good = mine && static_cast<unsigned>(p_id) < static_cast<unsigned>(a.num_blocks);
+    const unsigned ok = __ballot_sync(0xffffffffu, good);
+    came = (came & ~(ALL << (st * BURST))) | ok << (st * BURST);
+    if (ok && lane == 0) mbar_arrive_expect_tx(bars + st, __popc(ok) * P::RECORD);
+    __syncwarp();
+    if (good) {
+      const int h = a.chunks == 1 ? p_sub : p_sub / a.chunks;
+      bulk_load(ring + (st * BURST + lane) * P::RECORD,
+                a.pool + p_id * block_bytes + (h * a.recs + p_rec) * P::RECORD, P::RECORD, bars + st);
+    } else if (mine) {
+      report(a.err, kDevBadBlock);
     }
-    ++p_t;
+    p_t += BURST;
     settle();
   };
   settle();
-  int pending = 0;  // stages whose record is still to be waited for
+  int pending = 0;  // stages whose records are still to be waited for
 #pragma unroll 1
   for (int st = 0; st < STAGES; ++st) {
     pending += p_ok;
@@ -448,110 +477,114 @@ __global__ void __launch_bounds__(kThreads, kv4_ctas_per_sm<D, RT>()) kv4_attn_k
     float vscale = 1.0f;  // power of two that the value scales are multiplied by
     bool fresh = true;
 
-    // One record.  MASKED: some row does not see some token of it.
-    auto record = [&](auto masked_tag, int t) {
+    // One burst from record t on, `have`: which of its records came.  MASKED: some row does not see some token.
+    auto burst = [&](auto masked_tag, int t, unsigned have) {
       constexpr bool MASKED = decltype(masked_tag)::value;
-      const uint8_t* rec = ring + cur * P::RECORD;
-      uint32_t kw[2][2 * NG], kp[2][NG], vp[2][NG], vw[4][NG];
-#pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        const int tok = e ? tok1 : tok0;
-        load_words(rec + tok * P::ROW + c * (8 * NG), kw[e]);
-        load_words(rec + P::K_PAIRS + tok * P::PAIRS, kp[e]);
-        load_words(rec + P::V_PAIRS + tok * P::PAIRS, vp[e]);
-      }
-#pragma unroll
-      for (int i = 0; i < 4; ++i) load_words(rec + P::V_CODES + vtok[i] * P::ROW + 4 * NG * g, vw[i]);
-      // the record is in registers: its stage takes the next one
-      --pending;
-      __syncwarp();
-      pending += p_ok;
-      issue(cur);
-
+      const uint8_t* recs = ring + cur * (BURST * P::RECORD);
       // ---- scores
-      float s[2][NC];
+      float s[BURST][2][NC];
 #pragma unroll
-      for (int k = 0; k < NG; ++k) {
-        int acc[KT][4];
-#pragma unroll
-        for (int nt = 0; nt < KT; ++nt)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) acc[nt][e] = kMagicBits;
-#pragma unroll
-        for (int wi = 0; wi < 2; ++wi) {
-          const uint32_t w0 = kw[0][NG * wi + k], w1 = kw[1][NG * wi + k];
-          const uint32_t a0 = w0 & 0x0F0F0F0Fu, a1 = w1 & 0x0F0F0F0Fu, a2 = (w0 >> 4) & 0x0F0F0F0Fu,
-                         a3 = (w1 >> 4) & 0x0F0F0F0Fu;
-#pragma unroll
-          for (int nt = 0; nt < KT; ++nt) {
-            const uint2 b = qf[((k * 2 + wi) * KT + nt) * 32 + lane];
-            mma_u8s8_16832(acc[nt], a0, a1, a2, a3, b.x, b.y);
-          }
-        }
-#pragma unroll
-        for (int e = 0; e < 2; ++e)
-#pragma unroll
-          for (int q = 0; q < NC; ++q) {
-            const int hi = RT == 0 ? acc[0][2 * e] : acc[(q >> 1) * 2 % KT][2 * e + (q & 1)];
-            const int lo = RT == 0 ? acc[0][2 * e + 1] : acc[((q >> 1) * 2 + 1) % KT][2 * e + (q & 1)];
-            const float dot = fmaf(__int_as_float(hi) - kMagic, 256.0f, __int_as_float(lo) - kMagic);
-            const float m = pair_min(kp[e][k]) * qs[q][k];
-            s[e][q] = fmaf(pair_scale(kp[e][k]), dot, k == 0 ? m : s[e][q] + m);
-          }
-      }
-      // ---- distance of the scores to their references; the value scales as operands
-      float d[2][NC], vs[2][NG];
-      bool in[2][NC];
-      const int pos = t * kKv4Tokens;
-      if constexpr (MASKED) {
-        const int low = a.window > 0 ? see_least - a.window : 0;
+      for (int u = 0; u < BURST; ++u) {
+        const uint8_t* rec = recs + u * P::RECORD;
+        uint32_t kw[2][2 * NG], kp[2][NG];
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          const int at = pos + (e ? tok1 : tok0);
-          if (!(at < see_most && at >= low))  // no row sees the token: its pairs hold anything
-#pragma unroll
-            for (int k = 0; k < NG; ++k) vp[e][k] = 0;
-#pragma unroll
-          for (int q = 0; q < NC; ++q) in[e][q] = at < see[q] && (a.window <= 0 || at >= see[q] - a.window);
+          load_words(rec + (e ? tok1 : tok0) * P::ROW + c * (8 * NG), kw[e]);
+          load_words(rec + P::K_PAIRS + (e ? tok1 : tok0) * P::PAIRS, kp[e]);
         }
-      }
-      bool need = false;
-      if constexpr (CAP)
-#pragma unroll
-        for (int e = 0; e < 2; ++e)
-#pragma unroll
-          for (int q = 0; q < NC; ++q) s[e][q] = a.cap_log2 * tanh_exp(s[e][q] * f[q]);
-      auto distance = [&](int e, int q) {
-        const float x = CAP ? s[e][q] - mref[q] : fmaf(s[e][q], f[q], -mref[q]);
-        return !MASKED || in[e][q] ? x : -INFINITY;
-      };
-      auto score = [&](int e, int q) {
-        const float x = CAP ? s[e][q] : s[e][q] * f[q];
-        return !MASKED || in[e][q] ? x : -INFINITY;
-      };
-#pragma unroll
-      for (int e = 0; e < 2; ++e) {
-#pragma unroll
-        for (int q = 0; q < NC; ++q) {
-          d[e][q] = distance(e, q);
-          need |= d[e][q] > kSlack;
-        }
-        float top = 0.0f;
 #pragma unroll
         for (int k = 0; k < NG; ++k) {
-          vs[e][k] = pair_scale(vp[e][k]) * vscale;
-          top = fmaxf(top, vs[e][k]);
-        }
-        need |= top > kScaleMax;
-      }
-      // ---- new references and scaling, where a score or a scale outgrew them
-      if (__any_sync(0xffffffffu, need)) {
-        float smax = 0.0f;
+          int acc[KT][4];
 #pragma unroll
-        for (int k = 0; k < NG; ++k)
+          for (int wi = 0; wi < 2; ++wi) {
+            const uint32_t w0 = kw[0][NG * wi + k], w1 = kw[1][NG * wi + k];
+            const uint32_t a0 = w0 & 0x0F0F0F0Fu, a1 = w1 & 0x0F0F0F0Fu, a2 = (w0 >> 4) & 0x0F0F0F0Fu,
+                           a3 = (w1 >> 4) & 0x0F0F0F0Fu;
+#pragma unroll
+            for (int nt = 0; nt < KT; ++nt) {
+              const uint2 b = qf[((k * 2 + wi) * KT + nt) * 32 + lane];
+              if (wi == 0)
+                mma_u8s8_16832_from(acc[nt], a0, a1, a2, a3, b.x, b.y, kMagicBits);
+              else
+                mma_u8s8_16832(acc[nt], a0, a1, a2, a3, b.x, b.y);
+            }
+          }
 #pragma unroll
           for (int e = 0; e < 2; ++e)
-            if (pair_scale(vp[e][k]) <= kFltMax) smax = fmaxf(smax, pair_scale(vp[e][k]));
+#pragma unroll
+            for (int q = 0; q < NC; ++q) {
+              const int hi = RT == 0 ? acc[0][2 * e] : acc[(q >> 1) * 2 % KT][2 * e + (q & 1)];
+              const int lo = RT == 0 ? acc[0][2 * e + 1] : acc[((q >> 1) * 2 + 1) % KT][2 * e + (q & 1)];
+              const float dot = fmaf(__int_as_float(hi) - kMagic, 256.0f, __int_as_float(lo) - kMagic);
+              const float part = fmaf(pair_scale(kp[e][k]), dot, k == 0 ? 0.0f : s[u][e][q]);
+              s[u][e][q] = fmaf(pair_min(kp[e][k]), qs[q][k], part);
+            }
+        }
+        if constexpr (CAP)
+#pragma unroll
+          for (int e = 0; e < 2; ++e)
+#pragma unroll
+            for (int q = 0; q < NC; ++q) s[u][e][q] = a.cap_log2 * tanh_exp(s[u][e][q] * f[q]);
+      }
+      // ---- distance of the scores to their references; the value scales as operands
+      uint32_t vp[BURST][2][NG];
+      unsigned in[BURST] = {};  // bit e * NC + q
+#pragma unroll
+      for (int u = 0; u < BURST; ++u) {
+        const uint8_t* rec = recs + u * P::RECORD;
+#pragma unroll
+        for (int e = 0; e < 2; ++e) load_words(rec + P::V_PAIRS + (e ? tok1 : tok0) * P::PAIRS, vp[u][e]);
+        if constexpr (MASKED) {
+          const int low = a.window > 0 ? see_least - a.window : 0;
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const int at = (t + u) * kKv4Tokens + (e ? tok1 : tok0);
+            const bool here = have >> u & 1u;
+            if (!(here && at < see_most && at >= low))  // no row sees the token: its pairs hold anything
+#pragma unroll
+              for (int k = 0; k < NG; ++k) vp[u][e][k] = 0;
+#pragma unroll
+            for (int q = 0; q < NC; ++q)
+              in[u] |= static_cast<unsigned>(here && at < see[q] && (a.window <= 0 || at >= see[q] - a.window))
+                       << (e * NC + q);
+          }
+        }
+      }
+      auto distance = [&](int u, int e, int q) {
+        const float x = CAP ? s[u][e][q] - mref[q] : fmaf(s[u][e][q], f[q], -mref[q]);
+        return !MASKED || (in[u] >> (e * NC + q) & 1u) ? x : -INFINITY;
+      };
+      auto score = [&](int u, int e, int q) {
+        const float x = CAP ? s[u][e][q] : s[u][e][q] * f[q];
+        return !MASKED || (in[u] >> (e * NC + q) & 1u) ? x : -INFINITY;
+      };
+      float d[BURST][2][NC], vs[BURST][2][NG];
+      float far = -INFINITY, top = 0.0f;
+#pragma unroll
+      for (int u = 0; u < BURST; ++u)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+#pragma unroll
+          for (int q = 0; q < NC; ++q) {
+            d[u][e][q] = distance(u, e, q);
+            far = fmaxf(far, d[u][e][q]);
+          }
+#pragma unroll
+          for (int k = 0; k < NG; ++k) {
+            vs[u][e][k] = pair_scale(vp[u][e][k]) * vscale;
+            top = fmaxf(top, vs[u][e][k]);
+          }
+        }
+      // ---- new references and scaling, where a score or a scale outgrew them
+      if (__any_sync(0xffffffffu, far > kSlack || top > kScaleMax)) {
+        float smax = 0.0f;
+#pragma unroll
+        for (int u = 0; u < BURST; ++u)
+#pragma unroll
+          for (int k = 0; k < NG; ++k)
+#pragma unroll
+            for (int e = 0; e < 2; ++e)
+              if (pair_scale(vp[u][e][k]) <= kFltMax) smax = fmaxf(smax, pair_scale(vp[u][e][k]));
 #pragma unroll
         for (int off = 4; off < 32; off <<= 1) smax = fmaxf(smax, __shfl_xor_sync(0xffffffffu, smax, off));
         float fo = 1.0f;
@@ -564,7 +597,9 @@ __global__ void __launch_bounds__(kThreads, kv4_ctas_per_sm<D, RT>()) kv4_attn_k
         float fac[NC];
 #pragma unroll
         for (int q = 0; q < NC; ++q) {
-          float m = fmaxf(score(0, q), score(1, q));
+          float m = -INFINITY;
+#pragma unroll
+          for (int u = 0; u < BURST; ++u) m = fmaxf(m, fmaxf(score(u, 0, q), score(u, 1, q)));
 #pragma unroll
           for (int off = 4; off < 32; off <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, off));
           m = fmaxf(m, mref[q]);
@@ -581,66 +616,72 @@ __global__ void __launch_bounds__(kThreads, kv4_ctas_per_sm<D, RT>()) kv4_attn_k
 #pragma unroll
             for (int e = 0; e < 4; ++e) o[k][nt][e] *= fac[RT == 0 ? 0 : (nt * 2 + (e & 1)) % NC] * fo;
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
+        for (int u = 0; u < BURST; ++u)
 #pragma unroll
-          for (int q = 0; q < NC; ++q) d[e][q] = distance(e, q);
+          for (int e = 0; e < 2; ++e) {
 #pragma unroll
-          for (int k = 0; k < NG; ++k) vs[e][k] = pair_scale(vp[e][k]) * vscale;
-        }
+            for (int q = 0; q < NC; ++q) d[u][e][q] = distance(u, e, q);
+#pragma unroll
+            for (int k = 0; k < NG; ++k) vs[u][e][k] = pair_scale(vp[u][e][k]) * vscale;
+          }
       }
-      // ---- weights
+      // ---- weights, and outputs
 #pragma unroll
-      for (int e = 0; e < 2; ++e)
+      for (int u = 0; u < BURST; ++u) {
+        const uint8_t* rec = recs + u * P::RECORD;
+        uint32_t vw[4][NG];
 #pragma unroll
-        for (int q = 0; q < NC; ++q) {
-          d[e][q] = ex2(d[e][q]);
-          l[q] += d[e][q];
-        }
-      // ---- outputs
+        for (int i = 0; i < 4; ++i) load_words(rec + P::V_CODES + vtok[i] * P::ROW + 4 * NG * g, vw[i]);
 #pragma unroll
-      for (int k = 0; k < NG; ++k) {
-        uint32_t b[NT][2];
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          float w[NC];
+        for (int e = 0; e < 2; ++e)
 #pragma unroll
           for (int q = 0; q < NC; ++q) {
-            w[q] = d[e][q] * vs[e][k];
-            if constexpr (MASKED) {  // a NaN pair that only later rows see
-              w[q] = in[e][q] ? w[q] : 0.0f;
-              mo[q][k] += in[e][q] ? d[e][q] * pair_min(vp[e][k]) : 0.0f;
-            } else {
-              mo[q][k] = fmaf(d[e][q], pair_min(vp[e][k]), mo[q][k]);
-            }
+            d[u][e][q] = ex2(d[u][e][q]);
+            l[q] += d[u][e][q];
           }
 #pragma unroll
-          for (int nt = 0; nt < NT; ++nt)
-            movmatrix_trans(RT == 0 ? pack_f16(w[0], 0.0f) : pack_f16(w[2 * nt % NC], w[(2 * nt + 1) % NC]), b[nt][e]);
-        }
+        for (int k = 0; k < NG; ++k) {
+          uint32_t b[NT][2];
 #pragma unroll
-        for (int hv = 0; hv < 2; ++hv) {
-          const uint32_t y0 = __byte_perm(vw[0][k], vw[1][k], hv ? 0x7632 : 0x5410);
-          const uint32_t y1 = __byte_perm(vw[2][k], vw[3][k], hv ? 0x7632 : 0x5410);
+          for (int e = 0; e < 2; ++e) {
+            float w[NC];
 #pragma unroll
-          for (int hh = 0; hh < 2; ++hh) {
-            const uint32_t x0 = y0 >> (8 * hh), x1 = y1 >> (8 * hh);
-            const uint32_t a0 = x0 & 0x000F000Fu, a1 = x0 & 0x00F000F0u, a2 = x1 & 0x000F000Fu,
-                           a3 = x1 & 0x00F000F0u;
+            for (int q = 0; q < NC; ++q) {
+              w[q] = d[u][e][q] * vs[u][e][k];
+              if constexpr (MASKED) {  // a NaN pair that only later rows see
+                const bool x = in[u] >> (e * NC + q) & 1u;
+                w[q] = x ? w[q] : 0.0f;
+                mo[q][k] += x ? d[u][e][q] * pair_min(vp[u][e][k]) : 0.0f;
+              } else {
+                mo[q][k] = fmaf(d[u][e][q], pair_min(vp[u][e][k]), mo[q][k]);
+              }
+            }
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt)
-              mma_f16_16816(o[(k * 2 + hv) * 2 + hh][nt], a0, a1, a2, a3, b[nt][0], b[nt][1]);
+              b[nt][e] = transposed(RT == 0 ? pack_f16(w[0], 0.0f) : pack_f16(w[2 * nt % NC], w[(2 * nt + 1) % NC]));
+          }
+#pragma unroll
+          for (int hv = 0; hv < 2; ++hv) {
+            const uint32_t y0 = __byte_perm(vw[0][k], vw[1][k], hv ? 0x7632 : 0x5410);
+            const uint32_t y1 = __byte_perm(vw[2][k], vw[3][k], hv ? 0x7632 : 0x5410);
+#pragma unroll
+            for (int hh = 0; hh < 2; ++hh) {
+              const uint32_t x0 = y0 >> (8 * hh), x1 = y1 >> (8 * hh);
+              const uint32_t a0 = x0 & 0x000F000Fu, a1 = x0 & 0x00F000F0u, a2 = x1 & 0x000F000Fu,
+                             a3 = x1 & 0x00F000F0u;
+#pragma unroll
+              for (int nt = 0; nt < NT; ++nt)
+                mma_f16_16816(o[(k * 2 + hv) * 2 + hh][nt], a0, a1, a2, a3, b[nt][0], b[nt][1]);
+            }
           }
         }
       }
     };
 
     const int t_end = min(sq.first + (ra + n_rounds) * a.per, sq.last);
-    for (int t = sq.first + ra * a.per; t < t_end && !dead; ++t) {
-      if (bad >> cur & 1u) {  // no such block: its tokens count as masked
-        --pending;
-        pending += p_ok;
-        issue(cur);
-      } else {
+    for (int t = sq.first + ra * a.per; t < t_end && !dead; t += BURST) {
+      const unsigned have = came >> (cur * BURST) & ALL;
+      if (have) {  // else no such blocks: their tokens count as masked
         const uint32_t parity = phase >> cur & 1u;
         bool ok = mbar_try_wait(smem_u32(bars + cur), parity);
         if (!__all_sync(0xffffffffu, ok)) {
@@ -651,11 +692,15 @@ __global__ void __launch_bounds__(kThreads, kv4_ctas_per_sm<D, RT>()) kv4_attn_k
           }
         }
         phase ^= 1u << cur;
-        if (t * kKv4Tokens + kKv4Tokens > see_least || (a.window > 0 && t * kKv4Tokens < see_most - a.window))
-          record(std::true_type{}, t);
+        if (have != ALL || (t + BURST) * kKv4Tokens > see_least || (a.window > 0 && t * kKv4Tokens < see_most - a.window))
+          burst(std::true_type{}, t, have);
         else
-          record(std::false_type{}, t);
+          burst(std::false_type{}, t, have);
       }
+      __syncwarp();
+      --pending;
+      pending += p_ok;
+      issue(cur);
       cur = cur + 1 == STAGES ? 0 : cur + 1;
     }
 
@@ -717,7 +762,7 @@ __global__ void __launch_bounds__(kThreads, kv4_ctas_per_sm<D, RT>()) kv4_attn_k
   // a stream that was given up: its copies land before the block's shared memory goes
   if (dead)
     for (int st = cur; pending > 0; --pending, st = st + 1 == STAGES ? 0 : st + 1)
-      if (!(bad >> st & 1u)) mbar_wait(bars + st, phase >> st & 1u, nullptr, a.err);
+      if (came >> (st * BURST) & ALL) mbar_wait(bars + st, phase >> st & 1u, nullptr, a.err);
 }
 
 // Joins the parts of the items that span workers: a block takes row r of an item, parts in worker order, every
@@ -730,14 +775,14 @@ __global__ void __launch_bounds__(kJoinThreads) kv4_join_kernel(const Kv4AttnArg
   pdl_wait();
   pdl_launch_dependents();
   const int workers = static_cast<int>(a.head[0]);
-  const int64_t total = a.head[1];
+  const Kv4Split split(a.head[1], workers);
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, subs = a.hkv * a.chunks;
   const int64_t work = static_cast<int64_t>(a.batch) * subs * a.slab_rows;
   for (int64_t x = blockIdx.x; x < work; x += gridDim.x) {
     const int64_t item = x / a.slab_rows;
     const int r = static_cast<int>(x - item * a.slab_rows);
     const Kv4Item it = a.items[item];
-    const int first = worker_of(it.first, total, workers), last = worker_of(it.first + it.rounds - 1, total, workers);
+    const int first = split.worker(it.first), last = split.worker(it.first + it.rounds - 1);
     if (first == last) continue;
     const int seq = static_cast<int>(item / subs), sub = static_cast<int>(item - static_cast<int64_t>(seq) * subs);
     const int h = sub / a.chunks, row0 = (sub - h * a.chunks) * ROWS;
@@ -782,30 +827,47 @@ __global__ void __launch_bounds__(kJoinThreads) kv4_join_kernel(const Kv4AttnArg
   }
 }
 
-// Query rows that a CTA carries in one pass over the cache: 4, 8 or 16.
-int kv4_rt(int64_t rows) { return rows <= 4 ? 0 : rows <= 8 ? 1 : 2; }
-int64_t kv4_rows(int rt) { return rt == 0 ? 4 : 8 * rt; }
-
-int64_t kv4_grid(int64_t sms, int64_t head_dim, int rt) { return sms * (head_dim == 256 || rt > 1 ? 1 : 2); }
-
-struct Kv4Workspace {
-  int64_t items, ml, o, bytes;
+// How a call is cut: by its query rows per KV head and the head size.
+struct Kv4Plan {
+  int rt, rows, burst, warps;  // rows of a chunk at most
+  int64_t chunks, grid;
+  int64_t items_at, ml_at, o_at, bytes;  // workspace
 };
-Kv4Workspace kv4_workspace(int64_t grid, int rt, int64_t head_dim, int64_t items) {
-  Kv4Workspace w;
+template <int D, int RT>
+void kv4_plan_rows(Kv4Plan& p, int64_t sms) {
+  p.rt = RT;
+  p.rows = Kv4Rows<RT>::ROWS;
+  p.burst = Kv4Cfg<D, RT>::BURST;
+  p.warps = Kv4Cfg<D, RT>::WARPS;
+  p.grid = sms * Kv4Cfg<D, RT>::CTAS;
+}
+template <int D>
+void kv4_plan_dim(Kv4Plan& p, int64_t rows, int64_t sms) {
+  if (rows <= 4) kv4_plan_rows<D, 0>(p, sms);
+  else if (rows <= 8) kv4_plan_rows<D, 1>(p, sms);
+  else if (rows <= 16 || D == 256) kv4_plan_rows<D, 2>(p, sms);
+  else kv4_plan_rows<D, 3>(p, sms);
+}
+Kv4Plan kv4_plan(int64_t sms, int64_t head_dim, int64_t rows, int64_t batch, int64_t hkv) {
+  Kv4Plan p = {};
+  if (head_dim == 64) kv4_plan_dim<64>(p, rows, sms);
+  else if (head_dim == 128) kv4_plan_dim<128>(p, rows, sms);
+  else kv4_plan_dim<256>(p, rows, sms);
+  p.chunks = (rows + p.rows - 1) / p.rows;
   auto up = [](int64_t x) { return (x + 255) / 256 * 256; };
-  w.items = 256;
-  w.ml = w.items + up(items * static_cast<int64_t>(sizeof(Kv4Item)));
-  w.o = w.ml + up(2 * grid * kWarps * kv4_rows(rt) * 8);
-  w.bytes = w.o + 2 * grid * kWarps * kv4_rows(rt) * head_dim * 4;
-  return w;
+  p.items_at = 256;
+  p.ml_at = p.items_at + up(batch * hkv * p.chunks * static_cast<int64_t>(sizeof(Kv4Item)));
+  p.o_at = p.ml_at + up(2 * p.grid * p.warps * p.rows * 8);
+  p.bytes = p.o_at + 2 * p.grid * p.warps * p.rows * head_dim * 4;
+  return p;
 }
 
 template <int D, int RT, bool CAP>
 int kv4_launch_cap(const Kv4AttnArgs& a, int64_t grid, int64_t join_grid, cudaStream_t st) {
   constexpr size_t smem = Kv4Smem<D, RT>::BYTES;
   MVB_TRY(set_smem(kv4_attn_kernel<D, RT, CAP>, smem, "kv4_attention"));
-  MVB_TRY(launch("kv4_attention", kv4_attn_kernel<D, RT, CAP>, dim3(static_cast<unsigned>(grid)), dim3(kThreads), smem,
+  MVB_TRY(launch("kv4_attention", kv4_attn_kernel<D, RT, CAP>, dim3(static_cast<unsigned>(grid)),
+                 dim3(Kv4Cfg<D, RT>::WARPS * 32), smem,
                  st, a));
   if (join_grid == 0) return MVB_OK;
   return launch_dependent("kv4_attention_join", kv4_join_kernel<D, RT>, dim3(static_cast<unsigned>(join_grid)),
@@ -823,8 +885,11 @@ int kv4_launch(const Kv4AttnArgs& a, int rt, int64_t grid, int64_t join_grid, cu
   switch (rt) {
     case 0: return kv4_launch_rows<D, 0>(a, grid, join_grid, st);
     case 1: return kv4_launch_rows<D, 1>(a, grid, join_grid, st);
-    default: return kv4_launch_rows<D, 2>(a, grid, join_grid, st);
+    case 2: return kv4_launch_rows<D, 2>(a, grid, join_grid, st);
+    default: break;
   }
+  if constexpr (D < 256) return kv4_launch_rows<D, 3>(a, grid, join_grid, st);
+  return fail(MVB_ERR_UNSUPPORTED, "kv4_attention: rows");
 }
 
 }  // namespace
@@ -838,10 +903,7 @@ extern "C" int64_t mvb_paged_attention_decode_kv4_workspace_bytes(int64_t batch,
   if (batch <= 0 || num_kv_heads <= 0 || query_len <= 0) return 0;
   int sms = mvb_num_sms(device);
   if (sms <= 0) sms = 148;
-  const int64_t rows = num_q_heads / num_kv_heads * query_len;
-  const int rt = kv4_rt(rows);
-  const int64_t chunks = (rows + kv4_rows(rt) - 1) / kv4_rows(rt);
-  return kv4_workspace(kv4_grid(sms, head_dim, rt), rt, head_dim, batch * num_kv_heads * chunks).bytes;
+  return kv4_plan(sms, head_dim, num_q_heads / num_kv_heads * query_len, batch, num_kv_heads).bytes;
 }
 
 extern "C" int mvb_paged_attention_decode_kv4(void* out, int64_t out_stride, const void* q, int64_t q_stride,
@@ -900,33 +962,31 @@ extern "C" int mvb_paged_attention_decode_kv4(void* out, int64_t out_stride, con
   const int sms = current_sm_count();
   MVB_REQUIRE(sms > 0, "%s: no device", what);
   const int64_t rows = num_q_heads / num_kv_heads * query_len;
-  const int rt = kv4_rt(rows);
-  const int64_t chunks = (rows + kv4_rows(rt) - 1) / kv4_rows(rt);
-  const int64_t most = max_blocks * recs;  // records of an item
-  MVB_REQUIRE(num_kv_heads * chunks <= INT_MAX, "%s: heads", what);
-  const int64_t items = batch * num_kv_heads * chunks;
+  const Kv4Plan p = kv4_plan(sms, head_dim, rows, batch, num_kv_heads);
+  MVB_REQUIRE(num_kv_heads * p.chunks <= INT_MAX, "%s: heads", what);
+  MVB_REQUIRE(workspace && aligned(workspace, 256) && workspace_bytes >= p.bytes,
+              "%s: a workspace of %lld bytes, 256-byte aligned (got %lld)", what, (long long)p.bytes,
+              (long long)workspace_bytes);
+  const int64_t items = batch * num_kv_heads * p.chunks, most = max_blocks * recs;  // records of an item
   // Short tables: an item goes to one worker and nothing is left to join.
   const bool split = most > kShortRecords;
-  a.per = split ? 1 : static_cast<int>(most);
-  int64_t grid = kv4_grid(sms, head_dim, rt);
-  const Kv4Workspace w = kv4_workspace(grid, rt, head_dim, items);
-  MVB_REQUIRE(workspace && aligned(workspace, 256) && workspace_bytes >= w.bytes,
-              "%s: a workspace of %lld bytes, 256-byte aligned (got %lld)", what, (long long)w.bytes,
-              (long long)workspace_bytes);
-  if (items < grid && items * (split ? most : 1) < grid) grid = items * (split ? most : 1);
-  a.chunks = static_cast<int>(chunks);
-  a.slab_rows = static_cast<int>(rows < kv4_rows(rt) ? rows : kv4_rows(rt));
+  a.per = split ? p.burst : static_cast<int>(most);
+  int64_t grid = p.grid;
+  const int64_t most_rounds = split ? (most + p.burst - 1) / p.burst : 1;
+  if (items < grid && items * most_rounds < grid) grid = items * most_rounds;
+  a.chunks = static_cast<int>(p.chunks);
+  a.slab_rows = static_cast<int>(rows < p.rows ? rows : p.rows);
   char* ws = static_cast<char*>(workspace);
   a.head = reinterpret_cast<int64_t*>(ws);
-  a.items = reinterpret_cast<Kv4Item*>(ws + w.items);
-  a.part_ml = reinterpret_cast<float2*>(ws + w.ml);
-  a.part_o = reinterpret_cast<float*>(ws + w.o);
+  a.items = reinterpret_cast<Kv4Item*>(ws + p.items_at);
+  a.part_ml = reinterpret_cast<float2*>(ws + p.ml_at);
+  a.part_o = reinterpret_cast<float*>(ws + p.o_at);
   int64_t join_grid = 0;
   if (split) join_grid = items * a.slab_rows < 16LL * sms ? items * a.slab_rows : 16LL * sms;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   switch (head_dim) {
-    case 64: return kv4_launch<64>(a, rt, grid, join_grid, st);
-    case 128: return kv4_launch<128>(a, rt, grid, join_grid, st);
-    default: return kv4_launch<256>(a, rt, grid, join_grid, st);
+    case 64: return kv4_launch<64>(a, p.rt, grid, join_grid, st);
+    case 128: return kv4_launch<128>(a, p.rt, grid, join_grid, st);
+    default: return kv4_launch<256>(a, p.rt, grid, join_grid, st);
   }
 }
