@@ -41,15 +41,15 @@ namespace mvb {
 namespace {
 
 constexpr float kLog2e = 1.4426950408889634f;
-constexpr int kJoinThreads = 128;
+constexpr int kJoinThreads = 256;
 constexpr int kShortRecords = 8;  // items of at most this many records are never split
 
 // A weight is 2^(score - reference): the reference is a row's maximum when last raised, and is raised
 // once a score passes it by more than kSlack (in powers of two), so that most records cost one vote instead
-// of a reduction.  The weight times the scaled s' stays below 2^(kSlack + 11) = 2^15 in fp16.
-constexpr float kSlack = 4.0f;
-constexpr float kScaleMax = 2048.0f;  // of s' times its scaling; a new scaling puts the largest s' into [2^9, 2^10)
-constexpr int kScaleTarget = 9;
+// of a reduction.  The weight times the scaled s' stays below 2^(kSlack + 9) = 2^15 in fp16.
+constexpr float kSlack = 6.0f;
+constexpr float kScaleMax = 512.0f;  // of s' times its scaling; a new scaling puts the largest s' into [2^7, 2^8)
+constexpr int kScaleTarget = 7;
 constexpr float kFltMax = 3.40282347e38f;
 constexpr float kNone = -kFltMax;     // reference of a row without a key: no special cases, any score passes it
 constexpr float kMagic = 12582912.0f; // 1.5 * 2^23: its bits plus a small integer are the bits of the sum
@@ -65,13 +65,14 @@ struct Kv4Rows {
 };
 
 // BURST: records that a warp takes at once (one wait, one vote, one refill); STAGES of them are held, so that
-// an SM has some 45 KB or more under way while it computes; WARPS and CTAS (per SM) by the registers.
+// an SM has some 45 KB or more under way while it computes; WARPS of the one block per SM by the registers.
+// One block of 16 warps, not two of 8: the scheduler prefers the older block, whose warps then ended
+// after 21 us of a call where the other's took 27 (batch 64, context 1024-2048).
 template <int D, int RT>
 struct Kv4Cfg {
   static constexpr int BURST = D == 256 || RT > 1 ? 1 : D == 128 ? 2 : RT == 0 ? 4 : 2;
   static constexpr int STAGES = D == 256 ? (RT > 1 ? 2 : 3) : D == 128 ? (RT > 1 ? 4 : 2) : RT == 0 ? 2 : 4;
-  static constexpr int WARPS = D == 256 && RT == 0 ? 12 : 8;
-  static constexpr int CTAS = D == 256 || RT > 1 ? 1 : 2;
+  static constexpr int WARPS = D == 256 ? (RT == 0 ? 12 : 8) : RT > 1 ? 8 : 16;
 };
 
 struct Kv4AttnArgs {
@@ -92,17 +93,15 @@ struct Kv4AttnArgs {
   int slab_rows;  // rows of the largest chunk
   int per;        // records of a round, the unit of the division
   // workspace
-  int64_t* head;  // [0]: workers, [1]: rounds of the batch
   struct Kv4Item* items;  // [batch * hkv * chunks]
   float2* part_ml;        // [2 workers][ROWS]
   float* part_o;          // [2 workers][ROWS][D]
   unsigned* err;
 };
 
-// Where an item lies among the rounds of the batch.
+// The workers that an item spans.
 struct Kv4Item {
-  int64_t first;
-  int64_t rounds;
+  int first, last;
 };
 
 // The rounds of the batch among the workers: each `size`, the first `more` one more.
@@ -238,7 +237,7 @@ struct Kv4Smem {
 };
 
 template <int D, int RT, bool CAP>
-__global__ void __launch_bounds__(Kv4Cfg<D, RT>::WARPS * 32, Kv4Cfg<D, RT>::CTAS) kv4_attn_kernel(const Kv4AttnArgs a) {
+__global__ void __launch_bounds__(Kv4Cfg<D, RT>::WARPS * 32, 1) kv4_attn_kernel(const Kv4AttnArgs a) {
   using P = Kv4<D>;
   using S = Kv4Smem<D, RT>;
   using R = Kv4Rows<RT>;
@@ -290,10 +289,6 @@ __global__ void __launch_bounds__(Kv4Cfg<D, RT>::WARPS * 32, Kv4Cfg<D, RT>::CTAS
   for (int base = 0; base < a.batch; base += THREADS) scan(base, blockIdx.x == 0);
   const int64_t total = carry;
   const int workers = static_cast<int>(min(static_cast<int64_t>(gridDim.x) * WARPS, total));
-  if (blockIdx.x == 0 && tid == 0) {
-    a.head[0] = workers;
-    a.head[1] = total;
-  }
   const int worker = warp * gridDim.x + blockIdx.x;  // few rounds: spread over the SMs
   const bool busy = worker < workers;
   const Kv4Split split(total, workers);
@@ -323,63 +318,66 @@ __global__ void __launch_bounds__(Kv4Cfg<D, RT>::WARPS * 32, Kv4Cfg<D, RT>::CTAS
   int left = static_cast<int>(r1 - r0);
   int64_t item_first = r0 - ra;
 
-  // ---- the worker's stream of records, STAGES bursts ahead of the arithmetic; lane j sees to record j of a burst
+  // ---- the worker's stream of records, STAGES bursts ahead of the arithmetic.  Up to 32 records of an item are
+  // prepared at once, lane j seeing to record j: its block id is asked for a batch ahead, its copy is issued
+  // by that lane when its turn comes.
   const int64_t block_bytes = static_cast<int64_t>(a.hkv) * a.recs * P::RECORD;
-  int p_seq = seq, p_sub = sub, p_left = left, p_n = min(sq.rounds - ra, left);
+  int p_seq = seq, p_sub = sub, p_left = left - min(sq.rounds - ra, left);
   Kv4Seq p_sq = sq;
-  int p_t = sq.first + ra * a.per, p_end = min(sq.first + (ra + p_n) * a.per, sq.last);
-  int p_id = 0, p_rec = 0;
-  bool p_ok = true;
-  // Settles on the next burst at or after p_t, crossing into the next items, and asks for its block ids
-  // (one burst ahead of the copies that need them).
-  auto settle = [&]() {
+  int p_t = sq.first + ra * a.per, p_end = min(sq.first + (ra + left - p_left) * a.per, sq.last);
+  int ask_n = 0, ask_id = 0, ask_rec = 0, ask_sub = 0;  // the next batch: records, the lane's block and record in it
+  auto ask = [&]() {
+    ask_n = 0;
     while (p_t >= p_end) {
-      p_left -= p_n;
-      if (p_left <= 0) {
-        p_ok = false;
-        return;
-      }
+      if (p_left <= 0) return;
       if (++p_sub == subs) {
         p_sub = 0;
         p_sq = kv4_seq(a, ++p_seq, false);
       }
-      p_n = min(p_sq.rounds, p_left);
+      const int n = min(p_sq.rounds, p_left);
+      p_left -= n;
       p_t = p_sq.first;
-      p_end = min(p_sq.first + p_n * a.per, p_sq.last);
+      p_end = min(p_sq.first + n * a.per, p_sq.last);
     }
-    const int t = p_t + lane;
-    if (lane < BURST && t < p_end) {
-      const int blk = a.recs == 1 ? t : t / a.recs;
-      p_rec = t - blk * a.recs;
-      p_id = a.tables[p_seq * a.table_stride + blk];
+    ask_n = min(p_end - p_t, 32);
+    ask_sub = p_sub;
+    if (lane < ask_n) {
+      const int t = p_t + lane, blk = a.recs == 1 ? t : t / a.recs;
+      ask_rec = t - blk * a.recs;
+      ask_id = a.tables[p_seq * a.table_stride + blk];
     }
+    p_t += ask_n;
   };
-  unsigned came = 0, phase = 0;  // per stage: the records that came; parity of its barrier
+  int batch_n = 0, batch_at = 0;  // records of the current batch, the next one to copy
+  unsigned batch_ok = 0;          // those whose block is inside the pool
+  const uint8_t* batch_src = a.pool;
+  unsigned came = 0, phase = 0;   // per stage: the records that came; parity of its barrier
+  int pending = 0;                // stages whose records are still to be waited for
   auto issue = [&](int st) {
-    if (!p_ok) return;
-    const bool mine = lane < BURST && p_t + lane < p_end;
-    const bool good = mine && static_cast<unsigned>(p_id) < static_cast<unsigned>(a.num_blocks);
-    const unsigned ok = __ballot_sync(0xffffffffu, good);
-    came = (came & ~(ALL << (st * BURST))) | ok << (st * BURST);
-    if (ok && lane == 0) mbar_arrive_expect_tx(bars + st, __popc(ok) * P::RECORD);
-    __syncwarp();
-    if (good) {
-      const int h = a.chunks == 1 ? p_sub : p_sub / a.chunks;
-      bulk_load(ring + (st * BURST + lane) * P::RECORD,
-                a.pool + p_id * block_bytes + (h * a.recs + p_rec) * P::RECORD, P::RECORD, bars + st);
-    } else if (mine) {
-      report(a.err, kDevBadBlock);
+    if (batch_at >= batch_n) {
+      if (ask_n == 0) return;
+      batch_n = ask_n;
+      batch_at = 0;
+      const bool mine = lane < ask_n, good = mine && static_cast<unsigned>(ask_id) < static_cast<unsigned>(a.num_blocks);
+      batch_ok = __ballot_sync(0xffffffffu, good);
+      if (mine && !good) report(a.err, kDevBadBlock);
+      const int h = a.chunks == 1 ? ask_sub : ask_sub / a.chunks;
+      if (good) batch_src = a.pool + ask_id * block_bytes + (h * a.recs + ask_rec) * P::RECORD;
+      ask();
     }
-    p_t += BURST;
-    settle();
+    const unsigned ok = batch_ok >> batch_at & ALL;
+    came = (came & ~(ALL << (st * BURST))) | ok << (st * BURST);
+    const unsigned turn = static_cast<unsigned>(lane - batch_at);
+    if (ok && turn == 0) mbar_arrive_expect_tx(bars + st, BURST == 1 ? P::RECORD : __popc(ok) * P::RECORD);
+    if constexpr (BURST > 1) __syncwarp();
+    if (turn < BURST && (ok >> turn & 1u))
+      bulk_load(ring + (st * BURST + turn) * P::RECORD, batch_src, P::RECORD, bars + st);
+    batch_at += BURST;
+    ++pending;
   };
-  settle();
-  int pending = 0;  // stages whose records are still to be waited for
+  ask();
 #pragma unroll 1
-  for (int st = 0; st < STAGES; ++st) {
-    pending += p_ok;
-    issue(st);
-  }
+  for (int st = 0; st < STAGES; ++st) issue(st);
   int cur = 0;
   bool dead = false;
 
@@ -475,7 +473,7 @@ __global__ void __launch_bounds__(Kv4Cfg<D, RT>::WARPS * 32, Kv4Cfg<D, RT>::CTAS
       for (int k = 0; k < NG; ++k) mo[q][k] = 0.0f;
     }
     float vscale = 1.0f;  // power of two that the value scales are multiplied by
-    bool fresh = true;
+    bool fresh = true, none = true;  // no scaling chosen, no reference chosen
 
     // One burst from record t on, `have`: which of its records came.  MASKED: some row does not see some token.
     auto burst = [&](auto masked_tag, int t, unsigned have) {
@@ -595,6 +593,8 @@ __global__ void __launch_bounds__(Kv4Cfg<D, RT>::WARPS * 32, Kv4Cfg<D, RT>::CTAS
           fresh = false;
         }
         float fac[NC];
+        const bool empty = none;  // nothing summed yet
+        none = false;
 #pragma unroll
         for (int q = 0; q < NC; ++q) {
           float m = -INFINITY;
@@ -609,12 +609,13 @@ __global__ void __launch_bounds__(Kv4Cfg<D, RT>::WARPS * 32, Kv4Cfg<D, RT>::CTAS
 #pragma unroll
           for (int k = 0; k < NG; ++k) mo[q][k] *= fac[q];
         }
+        if (!empty)
 #pragma unroll
-        for (int k = 0; k < 4 * NG; ++k)
+          for (int k = 0; k < 4 * NG; ++k)
 #pragma unroll
-          for (int nt = 0; nt < NT; ++nt)
+            for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) o[k][nt][e] *= fac[RT == 0 ? 0 : (nt * 2 + (e & 1)) % NC] * fo;
+              for (int e = 0; e < 4; ++e) o[k][nt][e] *= fac[RT == 0 ? 0 : (nt * 2 + (e & 1)) % NC] * fo;
 #pragma unroll
         for (int u = 0; u < BURST; ++u)
 #pragma unroll
@@ -679,27 +680,27 @@ __global__ void __launch_bounds__(Kv4Cfg<D, RT>::WARPS * 32, Kv4Cfg<D, RT>::CTAS
     };
 
     const int t_end = min(sq.first + (ra + n_rounds) * a.per, sq.last);
+    // bursts that start in [t_low, t_high] hold no token that some row does not see
+    const int t_low = a.window > 0 ? max(see_most - a.window + kKv4Tokens - 1, 0) / kKv4Tokens : 0;
+    const int t_high = max(see_least, 0) / kKv4Tokens - BURST;
     for (int t = sq.first + ra * a.per; t < t_end && !dead; t += BURST) {
       const unsigned have = came >> (cur * BURST) & ALL;
       if (have) {  // else no such blocks: their tokens count as masked
         const uint32_t parity = phase >> cur & 1u;
         bool ok = mbar_try_wait(smem_u32(bars + cur), parity);
+        if (!ok) ok = wait_slow(bars + cur, parity, &abort_flag, a.err);
         if (!__all_sync(0xffffffffu, ok)) {
-          ok = wait_slow(bars + cur, parity, &abort_flag, a.err);
-          if (!__all_sync(0xffffffffu, ok)) {
-            dead = true;
-            break;
-          }
+          dead = true;
+          break;
         }
         phase ^= 1u << cur;
-        if (have != ALL || (t + BURST) * kKv4Tokens > see_least || (a.window > 0 && t * kKv4Tokens < see_most - a.window))
+        if (have != ALL || t > t_high || t < t_low)
           burst(std::true_type{}, t, have);
         else
           burst(std::false_type{}, t, have);
       }
       __syncwarp();
       --pending;
-      pending += p_ok;
       issue(cur);
       cur = cur + 1 == STAGES ? 0 : cur + 1;
     }
@@ -714,13 +715,13 @@ __global__ void __launch_bounds__(Kv4Cfg<D, RT>::WARPS * 32, Kv4Cfg<D, RT>::CTAS
         for (int k = 0; k < NG; ++k) mo[q][k] += __shfl_xor_sync(0xffffffffu, mo[q][k], off);
       }
     }
+    const bool whole = ra == 0 && n_rounds == sq.rounds;
     if (ra == 0 && lane == 0) {
       Kv4Item it;
-      it.first = item_first;
-      it.rounds = sq.rounds;
+      it.first = worker;
+      it.last = whole ? worker : split.worker(item_first + sq.rounds - 1);
       a.items[static_cast<int64_t>(seq) * subs + sub] = it;
     }
-    const bool whole = ra == 0 && n_rounds == sq.rounds;
     const int64_t slot = 2 * static_cast<int64_t>(worker) + (ra == 0 ? 1 : 0);
     const float inv = 1.0f / vscale;
 #pragma unroll
@@ -765,64 +766,111 @@ __global__ void __launch_bounds__(Kv4Cfg<D, RT>::WARPS * 32, Kv4Cfg<D, RT>::CTAS
       if (came >> (st * BURST) & ALL) mbar_wait(bars + st, phase >> st & 1u, nullptr, a.err);
 }
 
-// Joins the parts of the items that span workers: a block takes row r of an item, parts in worker order, every
-// fourth one a warp.
+// Adds parts p0, p0 + STEP, .. up to `last` of row r of an item to (m, l, o); eight of them under way at once.
+template <int D, int RT, int STEP>
+__device__ __forceinline__ void kv4_join_parts(const Kv4AttnArgs& a, const Kv4Item& it, int p0, int r, int lane, float& m,
+                                               float& l, float (&o)[D / 32]) {
+  constexpr int ROWS = Kv4Rows<RT>::ROWS, N = D / 32, AHEAD = 8;
+  for (; p0 <= it.last; p0 += STEP * AHEAD) {
+    float2 e[AHEAD];
+    float y[AHEAD][N];
+#pragma unroll
+    for (int i = 0; i < AHEAD; ++i) {
+      const int p = p0 + i * STEP;
+      const int64_t slot = (2 * static_cast<int64_t>(p) + (p == it.first ? 1 : 0)) * ROWS + r;
+      e[i] = make_float2(kNone, 0.0f);
+      if (p <= it.last) e[i] = a.part_ml[slot];
+#pragma unroll
+      for (int j = 0; j < N; ++j) y[i][j] = p <= it.last ? a.part_o[slot * D + 32 * j + lane] : 0.0f;
+    }
+    float top = m;
+#pragma unroll
+    for (int i = 0; i < AHEAD; ++i) top = fmaxf(top, e[i].x);
+    const float fm = ex2(m - top);
+    l *= fm;
+#pragma unroll
+    for (int j = 0; j < N; ++j) o[j] *= fm;
+#pragma unroll
+    for (int i = 0; i < AHEAD; ++i) {
+      const float fe = ex2(e[i].x - top);
+      l = fmaf(e[i].y, fe, l);
+#pragma unroll
+      for (int j = 0; j < N; ++j) o[j] = fmaf(y[i][j], fe, o[j]);
+    }
+    m = top;
+  }
+}
+
+// Joins the parts of the items that span workers.  A block takes `pairs` (item, row) pairs at a time, eight of them
+// or, where there are few, one: a pair of few parts is one warp's, in worker order; a pair of many is the whole
+// block's, every eighth part a warp.
 template <int D, int RT>
-__global__ void __launch_bounds__(kJoinThreads) kv4_join_kernel(const Kv4AttnArgs a) {
-  constexpr int ROWS = Kv4Rows<RT>::ROWS, N = D / 32, WARPS = kJoinThreads / 32;
+__global__ void __launch_bounds__(kJoinThreads) kv4_join_kernel(const Kv4AttnArgs a, const int pairs) {
+  constexpr int ROWS = Kv4Rows<RT>::ROWS, N = D / 32, WARPS = kJoinThreads / 32, FEW = 16;
   __shared__ float acc[WARPS][D];
   __shared__ float2 ml[WARPS];
   pdl_wait();
   pdl_launch_dependents();
-  const int workers = static_cast<int>(a.head[0]);
-  const Kv4Split split(a.head[1], workers);
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, subs = a.hkv * a.chunks;
   const int64_t work = static_cast<int64_t>(a.batch) * subs * a.slab_rows;
-  for (int64_t x = blockIdx.x; x < work; x += gridDim.x) {
-    const int64_t item = x / a.slab_rows;
-    const int r = static_cast<int>(x - item * a.slab_rows);
-    const Kv4Item it = a.items[item];
-    const int first = split.worker(it.first), last = split.worker(it.first + it.rounds - 1);
-    if (first == last) continue;
+  for (int64_t x0 = static_cast<int64_t>(blockIdx.x) * pairs; x0 < work; x0 += static_cast<int64_t>(gridDim.x) * pairs) {
+    // lane j of every warp looks at pair x0 + j
+    const int64_t x = x0 + lane;
+    const bool mine = lane < pairs && x < work;
+    const int64_t item = x >> 31 ? x / a.slab_rows : static_cast<uint32_t>(x) / static_cast<uint32_t>(a.slab_rows);
+    const int row = static_cast<int>(x - item * a.slab_rows);
+    Kv4Item it = {0, 0};
+    if (mine) it = a.items[item];
     const int seq = static_cast<int>(item / subs), sub = static_cast<int>(item - static_cast<int64_t>(seq) * subs);
-    const int h = sub / a.chunks, row0 = (sub - h * a.chunks) * ROWS;
-    if (r >= a.group * a.T - row0) continue;
+    const int h = sub / a.chunks, at = (sub - h * a.chunks) * ROWS + row;  // row of the KV head
+    const bool split = mine && it.first < it.last && at < a.group * a.T;
+    const int64_t dst_at = (static_cast<int64_t>(seq) * a.T + at / a.group) * a.out_stride +
+                           static_cast<int64_t>(h * a.group + at % a.group) * D;
+    const unsigned many = __ballot_sync(0xffffffffu, split && it.last - it.first >= FEW);
+    const unsigned few = __ballot_sync(0xffffffffu, split && it.last - it.first < FEW);
     float m = kNone, l = 0.0f, o[N];
 #pragma unroll
     for (int j = 0; j < N; ++j) o[j] = 0.0f;
-#pragma unroll 4
-    for (int p = first + warp; p <= last; p += WARPS) {
-      const int64_t slot = (2 * static_cast<int64_t>(p) + (p == first ? 1 : 0)) * ROWS + r;
-      const float2 e = a.part_ml[slot];
-      float y[N];
+    if (few >> warp & 1u) {
+      Kv4Item one;
+      one.first = __shfl_sync(0xffffffffu, it.first, warp);
+      one.last = __shfl_sync(0xffffffffu, it.last, warp);
+      const int r = __shfl_sync(0xffffffffu, row, warp);
+      __nv_bfloat16* dst = a.out + __shfl_sync(0xffffffffu, dst_at, warp);
+      kv4_join_parts<D, RT, 1>(a, one, one.first, r, lane, m, l, o);
+      const float inv = l == 0.0f ? 0.0f : 1.0f / l;
 #pragma unroll
-      for (int j = 0; j < N; ++j) y[j] = a.part_o[slot * D + 32 * j + lane];
-      const float top = fmaxf(m, e.x);
-      const float fm = ex2(m - top), fe = ex2(e.x - top);
-      l = l * fm + e.y * fe;
-#pragma unroll
-      for (int j = 0; j < N; ++j) o[j] = o[j] * fm + y[j] * fe;
-      m = top;
+      for (int j = 0; j < N; ++j) dst[32 * j + lane] = __float2bfloat16_rn(o[j] * inv);
     }
-    __syncthreads();  // the row before has been read
-    if (lane == 0) ml[warp] = make_float2(m, l);
+    for (unsigned left = many; left != 0; left &= left - 1) {
+      const int k = __ffs(left) - 1;
+      Kv4Item one;
+      one.first = __shfl_sync(0xffffffffu, it.first, k);
+      one.last = __shfl_sync(0xffffffffu, it.last, k);
+      const int r = __shfl_sync(0xffffffffu, row, k);
+      __nv_bfloat16* dst = a.out + __shfl_sync(0xffffffffu, dst_at, k);
+      m = kNone, l = 0.0f;
 #pragma unroll
-    for (int j = 0; j < N; ++j) acc[warp][32 * j + lane] = o[j];
-    __syncthreads();
-    float top = kNone;
+      for (int j = 0; j < N; ++j) o[j] = 0.0f;
+      kv4_join_parts<D, RT, WARPS>(a, one, one.first + warp, r, lane, m, l, o);
+      __syncthreads();  // the pair before has been read
+      if (lane == 0) ml[warp] = make_float2(m, l);
 #pragma unroll
-    for (int w = 0; w < WARPS; ++w) top = fmaxf(top, ml[w].x);
-    const int i = (row0 + r) / a.group, hq = h * a.group + (row0 + r) - i * a.group;
-    __nv_bfloat16* dst = a.out + (static_cast<int64_t>(seq) * a.T + i) * a.out_stride + static_cast<int64_t>(hq) * D;
-    for (int ch = threadIdx.x; ch < D; ch += kJoinThreads) {
-      float sum = 0.0f, v = 0.0f;
+      for (int j = 0; j < N; ++j) acc[warp][32 * j + lane] = o[j];
+      __syncthreads();
+      float top = kNone;
 #pragma unroll
-      for (int w = 0; w < WARPS; ++w) {
-        const float f = ex2(ml[w].x - top);
-        sum += ml[w].y * f;
-        v += acc[w][ch] * f;
+      for (int w = 0; w < WARPS; ++w) top = fmaxf(top, ml[w].x);
+      for (int ch = threadIdx.x; ch < D; ch += kJoinThreads) {
+        float sum = 0.0f, v = 0.0f;
+#pragma unroll
+        for (int w = 0; w < WARPS; ++w) {
+          const float f = ex2(ml[w].x - top);
+          sum += ml[w].y * f;
+          v += acc[w][ch] * f;
+        }
+        dst[ch] = __float2bfloat16_rn(sum == 0.0f ? 0.0f : v / sum);
       }
-      dst[ch] = __float2bfloat16_rn(sum == 0.0f ? 0.0f : v / sum);
     }
   }
 }
@@ -839,7 +887,7 @@ void kv4_plan_rows(Kv4Plan& p, int64_t sms) {
   p.rows = Kv4Rows<RT>::ROWS;
   p.burst = Kv4Cfg<D, RT>::BURST;
   p.warps = Kv4Cfg<D, RT>::WARPS;
-  p.grid = sms * Kv4Cfg<D, RT>::CTAS;
+  p.grid = sms;
 }
 template <int D>
 void kv4_plan_dim(Kv4Plan& p, int64_t rows, int64_t sms) {
@@ -855,7 +903,7 @@ Kv4Plan kv4_plan(int64_t sms, int64_t head_dim, int64_t rows, int64_t batch, int
   else kv4_plan_dim<256>(p, rows, sms);
   p.chunks = (rows + p.rows - 1) / p.rows;
   auto up = [](int64_t x) { return (x + 255) / 256 * 256; };
-  p.items_at = 256;
+  p.items_at = 0;
   p.ml_at = p.items_at + up(batch * hkv * p.chunks * static_cast<int64_t>(sizeof(Kv4Item)));
   p.o_at = p.ml_at + up(2 * p.grid * p.warps * p.rows * 8);
   p.bytes = p.o_at + 2 * p.grid * p.warps * p.rows * head_dim * 4;
@@ -863,7 +911,7 @@ Kv4Plan kv4_plan(int64_t sms, int64_t head_dim, int64_t rows, int64_t batch, int
 }
 
 template <int D, int RT, bool CAP>
-int kv4_launch_cap(const Kv4AttnArgs& a, int64_t grid, int64_t join_grid, cudaStream_t st) {
+int kv4_launch_cap(const Kv4AttnArgs& a, int64_t grid, int64_t join_grid, int pairs, cudaStream_t st) {
   constexpr size_t smem = Kv4Smem<D, RT>::BYTES;
   MVB_TRY(set_smem(kv4_attn_kernel<D, RT, CAP>, smem, "kv4_attention"));
   MVB_TRY(launch("kv4_attention", kv4_attn_kernel<D, RT, CAP>, dim3(static_cast<unsigned>(grid)),
@@ -871,24 +919,24 @@ int kv4_launch_cap(const Kv4AttnArgs& a, int64_t grid, int64_t join_grid, cudaSt
                  st, a));
   if (join_grid == 0) return MVB_OK;
   return launch_dependent("kv4_attention_join", kv4_join_kernel<D, RT>, dim3(static_cast<unsigned>(join_grid)),
-                          dim3(kJoinThreads), 0, st, a);
+                          dim3(kJoinThreads), 0, st, a, pairs);
 }
 
 template <int D, int RT>
-int kv4_launch_rows(const Kv4AttnArgs& a, int64_t grid, int64_t join_grid, cudaStream_t st) {
-  return a.cap_log2 > 0.0f ? kv4_launch_cap<D, RT, true>(a, grid, join_grid, st)
-                           : kv4_launch_cap<D, RT, false>(a, grid, join_grid, st);
+int kv4_launch_rows(const Kv4AttnArgs& a, int64_t grid, int64_t join_grid, int pairs, cudaStream_t st) {
+  return a.cap_log2 > 0.0f ? kv4_launch_cap<D, RT, true>(a, grid, join_grid, pairs, st)
+                           : kv4_launch_cap<D, RT, false>(a, grid, join_grid, pairs, st);
 }
 
 template <int D>
-int kv4_launch(const Kv4AttnArgs& a, int rt, int64_t grid, int64_t join_grid, cudaStream_t st) {
+int kv4_launch(const Kv4AttnArgs& a, int rt, int64_t grid, int64_t join_grid, int pairs, cudaStream_t st) {
   switch (rt) {
-    case 0: return kv4_launch_rows<D, 0>(a, grid, join_grid, st);
-    case 1: return kv4_launch_rows<D, 1>(a, grid, join_grid, st);
-    case 2: return kv4_launch_rows<D, 2>(a, grid, join_grid, st);
+    case 0: return kv4_launch_rows<D, 0>(a, grid, join_grid, pairs, st);
+    case 1: return kv4_launch_rows<D, 1>(a, grid, join_grid, pairs, st);
+    case 2: return kv4_launch_rows<D, 2>(a, grid, join_grid, pairs, st);
     default: break;
   }
-  if constexpr (D < 256) return kv4_launch_rows<D, 3>(a, grid, join_grid, st);
+  if constexpr (D < 256) return kv4_launch_rows<D, 3>(a, grid, join_grid, pairs, st);
   return fail(MVB_ERR_UNSUPPORTED, "kv4_attention: rows");
 }
 
@@ -977,16 +1025,20 @@ extern "C" int mvb_paged_attention_decode_kv4(void* out, int64_t out_stride, con
   a.chunks = static_cast<int>(p.chunks);
   a.slab_rows = static_cast<int>(rows < p.rows ? rows : p.rows);
   char* ws = static_cast<char*>(workspace);
-  a.head = reinterpret_cast<int64_t*>(ws);
   a.items = reinterpret_cast<Kv4Item*>(ws + p.items_at);
   a.part_ml = reinterpret_cast<float2*>(ws + p.ml_at);
   a.part_o = reinterpret_cast<float*>(ws + p.o_at);
   int64_t join_grid = 0;
-  if (split) join_grid = items * a.slab_rows < 16LL * sms ? items * a.slab_rows : 16LL * sms;
+  const int64_t all_pairs = items * a.slab_rows;
+  const int pairs = all_pairs > 4LL * sms ? kJoinThreads / 32 : 1;
+  if (split) {
+    join_grid = (all_pairs + pairs - 1) / pairs;
+    if (join_grid > 8LL * sms) join_grid = 8LL * sms;
+  }
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   switch (head_dim) {
-    case 64: return kv4_launch<64>(a, p.rt, grid, join_grid, st);
-    case 128: return kv4_launch<128>(a, p.rt, grid, join_grid, st);
-    default: return kv4_launch<256>(a, p.rt, grid, join_grid, st);
+    case 64: return kv4_launch<64>(a, p.rt, grid, join_grid, pairs, st);
+    case 128: return kv4_launch<128>(a, p.rt, grid, join_grid, pairs, st);
+    default: return kv4_launch<256>(a, p.rt, grid, join_grid, pairs, st);
   }
 }
