@@ -157,6 +157,19 @@ def stream_handle(device: torch.device | None = None) -> int:
     return torch.cuda.current_stream(device).cuda_stream
 
 
+def on_device(index: int, what: str, fn, *args) -> None:
+    """``fn(*args, stream)`` with device ``index`` current and its current stream, checked.  What
+    ``torch.cuda.device`` and ``torch.cuda.current_stream`` cost (3.6 us a call) is spent only where the
+    device is not the current one."""
+    if torch._C._cuda_getDevice() == index:
+        rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+    else:
+        with torch.cuda.device(index):
+            rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+    if rc != MVB_OK:
+        check(rc, what)
+
+
 def device_status(clear: bool = True, stream: int | None = None) -> int:
     """OR of MVB_DEV_* bits the kernels reported on the current device (synchronises)."""
     v = C.c_uint(0)

@@ -5,6 +5,7 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <atomic>
 #include <cstdarg>
 #include <cstdio>
 #include <utility>
@@ -117,6 +118,17 @@ int set_smem(void (*kernel)(KArgs...), size_t bytes, const char* name) {
   cudaError_t e = cudaFuncSetAttribute(reinterpret_cast<const void*>(kernel),
                                        cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(bytes));
   return cuda_status(e, name);
+}
+
+// The same, asked of the driver once per kernel and device: `done` is a static of the call site, a bit per device.
+template <typename... KArgs>
+int set_smem_once(std::atomic<uint64_t>& done, void (*kernel)(KArgs...), size_t bytes, const char* name) {
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return set_smem(kernel, bytes, name);
+  if (done.load(std::memory_order_acquire) >> dev & 1u) return MVB_OK;
+  const int rc = set_smem(kernel, bytes, name);
+  if (rc == MVB_OK) done.fetch_or(uint64_t(1) << dev, std::memory_order_release);
+  return rc;
 }
 
 }  // namespace mvb

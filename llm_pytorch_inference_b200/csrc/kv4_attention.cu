@@ -913,7 +913,8 @@ Kv4Plan kv4_plan(int64_t sms, int64_t head_dim, int64_t rows, int64_t batch, int
 template <int D, int RT, bool CAP>
 int kv4_launch_cap(const Kv4AttnArgs& a, int64_t grid, int64_t join_grid, int pairs, cudaStream_t st) {
   constexpr size_t smem = Kv4Smem<D, RT>::BYTES;
-  MVB_TRY(set_smem(kv4_attn_kernel<D, RT, CAP>, smem, "kv4_attention"));
+  static std::atomic<uint64_t> done{0};
+  MVB_TRY(set_smem_once(done, kv4_attn_kernel<D, RT, CAP>, smem, "kv4_attention"));
   MVB_TRY(launch("kv4_attention", kv4_attn_kernel<D, RT, CAP>, dim3(static_cast<unsigned>(grid)),
                  dim3(Kv4Cfg<D, RT>::WARPS * 32), smem,
                  st, a));

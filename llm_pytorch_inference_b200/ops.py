@@ -12,6 +12,7 @@ shape and indexes it with K's rows, ``mini_vllm/ops/rope.py:59-70``).
 """
 from __future__ import annotations
 
+import functools
 import threading
 from typing import NamedTuple
 
@@ -454,37 +455,45 @@ def paged_attention_decode(q: torch.Tensor, kv_cache: torch.Tensor, layer: int, 
 
 
 # ------------------------------------------------------------------ 4-bit paged KV cache
-def _expect(what: str, device: torch.device, **tensors) -> None:
-    """Each ``name=(tensor, dtype, dims)``: a CUDA tensor of ``device`` with that dtype and number of dimensions."""
-    for name, (t, dtype, dims) in tensors.items():
-        if not isinstance(t, torch.Tensor):
-            raise RuntimeError(f"{what}: {name} must be a tensor")
-        N.require_cuda(t)
-        if t.device != device:
-            raise RuntimeError(f"{what}: {name} is on {t.device}, not on {device}")
-        if t.dtype != dtype:
-            raise RuntimeError(f"{what}: {name} must be {dtype}, not {t.dtype}")
-        if t.dim() != dims:
-            raise RuntimeError(f"{what}: {name} must have {dims} dimensions, not {t.dim()}")
+def _refuse(what: str, name: str, t, index: int, dtype: torch.dtype, dims: int) -> None:
+    if not isinstance(t, torch.Tensor):
+        raise RuntimeError(f"{what}: {name} must be a tensor")
+    N.require_cuda(t)
+    if t.get_device() != index:
+        raise RuntimeError(f"{what}: {name} is on {t.device}, not on cuda:{index}")
+    if t.dtype != dtype:
+        raise RuntimeError(f"{what}: {name} must be {dtype}, not {t.dtype}")
+    raise RuntimeError(f"{what}: {name} must have {dims} dimensions, not {t.dim()}")
 
 
-def _kv4_geometry(what: str, kv4: torch.Tensor, layer: int) -> tuple[int, int, int, int, int]:
-    """(layers, blocks, KV heads, block size, head size) of a pool of ``kv_cache.kv4_pool``."""
-    if not isinstance(kv4, torch.Tensor):
-        raise RuntimeError(f"{what}: kv4 must be a tensor")
-    _expect(what, kv4.device, kv4=(kv4, torch.uint8, 5))
+def _expect(what: str, name: str, t, index: int, dtype: torch.dtype, dims: int) -> None:
+    """A CUDA tensor of device ``index`` with this dtype and number of dimensions."""
+    if not (isinstance(t, torch.Tensor) and t.get_device() == index and index >= 0 and t.dtype is dtype
+            and t.dim() == dims):
+        _refuse(what, name, t, index, dtype, dims)
+
+
+def _kv4_geometry(what: str, kv4: torch.Tensor, layer: int) -> tuple[int, int, int, int, int, int]:
+    """(device, layers, blocks, KV heads, block size, head size) of a pool of ``kv_cache.kv4_pool``."""
+    index = kv4.get_device() if isinstance(kv4, torch.Tensor) else -1
+    _expect(what, "kv4", kv4, index, torch.uint8, 5)
     L, P, nkv, recs, rec = kv4.shape
     if rec % 18 or not kv4.is_contiguous():
         raise RuntimeError(f"{what}: kv4 must be a contiguous pool of kv_cache.kv4_pool, not {tuple(kv4.shape)}")
     if not 0 <= layer < L:
         raise RuntimeError(f"{what}: layer {layer} of {L}")
-    return L, P, nkv, 16 * recs, rec // 18
+    return index, L, P, nkv, 16 * recs, rec // 18
 
 
 def _kv4_rows(t: torch.Tensor) -> torch.Tensor:
     """``t`` [tokens, heads, D] if its rows can be read with 16-byte loads, else a copy."""
-    ok = t.stride(2) == 1 and t.stride(0) % 8 == 0 and t.stride(1) % 8 == 0 and t.data_ptr() % 16 == 0
-    return t if ok else t.clone(memory_format=torch.contiguous_format)
+    if t.data_ptr() % 16 == 0:
+        if t.is_contiguous():
+            return t
+        s0, s1, s2 = t.stride()
+        if s2 == 1 and s0 % 8 == 0 and s1 % 8 == 0:
+            return t
+    return t.clone(memory_format=torch.contiguous_format)
 
 
 def kv4_write(k: torch.Tensor, v: torch.Tensor, kv4: torch.Tensor, layer: int, slots: torch.Tensor) -> None:
@@ -493,35 +502,42 @@ def kv4_write(k: torch.Tensor, v: torch.Tensor, kv4: torch.Tensor, layer: int, s
     ``kv_cache.kv4_pool``.  Per group of 64 channels: ``min``, ``scale = (max - min) / 15`` (both bf16) and
     ``round((x - min) / scale)``.  A group with a NaN or an infinity reads back as NaN.  The slots of one
     call must differ from one another."""
-    L, P, nkv, bs, D = _kv4_geometry("kv4_write", kv4, layer)
-    dev = kv4.device
-    _expect("kv4_write", dev, k=(k, torch.bfloat16, 3), v=(v, torch.bfloat16, 3), slots=(slots, torch.int64, 1))
-    want = (slots.shape[0], nkv, D)
-    if tuple(k.shape) != want or tuple(v.shape) != want:
-        raise RuntimeError(f"kv4_write: k and v must be {want}, not {tuple(k.shape)} and {tuple(v.shape)}")
-    if slots.shape[0] == 0:
+    what = "kv4_write"
+    index, L, P, nkv, bs, D = _kv4_geometry(what, kv4, layer)
+    _expect(what, "k", k, index, torch.bfloat16, 3)
+    _expect(what, "v", v, index, torch.bfloat16, 3)
+    _expect(what, "slots", slots, index, torch.int64, 1)
+    n = slots.shape[0]
+    if k.shape != (n, nkv, D) or v.shape != (n, nkv, D):
+        raise RuntimeError(f"{what}: k and v must be {(n, nkv, D)}, not {tuple(k.shape)} and {tuple(v.shape)}")
+    if n == 0:
         return
     k, v, slots = _kv4_rows(k), _kv4_rows(v), slots.contiguous()
-    with torch.cuda.device(dev):
-        N.check(N.lib().mvb_kv4_write(kv4.data_ptr(), k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(),
-                                      v.stride(0), v.stride(1), slots.data_ptr(), slots.shape[0], nkv, D, L,
-                                      int(layer), P, bs, _st(kv4)), "kv4_write")
+    k0, k1, _ = k.stride()
+    v0, v1, _ = v.stride()
+    N.on_device(index, what, N.lib().mvb_kv4_write, kv4.data_ptr(), k.data_ptr(), k0, k1, v.data_ptr(), v0, v1,
+                slots.data_ptr(), n, nkv, D, L, int(layer), P, bs)
 
 
 def kv4_read(kv4: torch.Tensor, layer: int, slots: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     """K and V ``[tokens, Hkv, D]`` (bf16) that the slots ``slots`` (int64) of ``layer`` stand for; zeros for
     a negative slot."""
-    L, P, nkv, bs, D = _kv4_geometry("kv4_read", kv4, layer)
-    dev = kv4.device
-    _expect("kv4_read", dev, slots=(slots, torch.int64, 1))
+    what = "kv4_read"
+    index, L, P, nkv, bs, D = _kv4_geometry(what, kv4, layer)
+    _expect(what, "slots", slots, index, torch.int64, 1)
+    n = slots.shape[0]
     slots = slots.contiguous()
-    k = torch.empty(slots.shape[0], nkv, D, dtype=torch.bfloat16, device=dev)
+    k = torch.empty(n, nkv, D, dtype=torch.bfloat16, device=kv4.device)
     v = torch.empty_like(k)
-    if slots.shape[0]:
-        with torch.cuda.device(dev):
-            N.check(N.lib().mvb_kv4_read(k.data_ptr(), v.data_ptr(), kv4.data_ptr(), slots.data_ptr(), slots.shape[0],
-                                         nkv, D, L, int(layer), P, bs, _st(kv4)), "kv4_read")
+    if n:
+        N.on_device(index, what, N.lib().mvb_kv4_read, k.data_ptr(), v.data_ptr(), kv4.data_ptr(), slots.data_ptr(), n,
+                    nkv, D, L, int(layer), P, bs)
     return k, v
+
+
+@functools.lru_cache(maxsize=1024)
+def _kv4_workspace_bytes(B: int, T: int, Hq: int, nkv: int, D: int, index: int) -> int:
+    return N.lib().mvb_paged_attention_decode_kv4_workspace_bytes(B, T, Hq, nkv, D, index)
 
 
 def paged_attention_decode_kv4(q: torch.Tensor, kv4: torch.Tensor, layer: int, block_tables: torch.Tensor,
@@ -535,47 +551,56 @@ def paged_attention_decode_kv4(q: torch.Tensor, kv4: torch.Tensor, layer: int, b
     ``workspace``: uint8 of ``mvb_paged_attention_decode_kv4_workspace_bytes`` (any content, not shared by
     calls that overlap); by default each call takes its own from torch's allocator."""
     what = "paged_attention_decode_kv4"
-    L, P, nkv, bs, D = _kv4_geometry(what, kv4, layer)
-    dev = kv4.device
-    if not isinstance(q, torch.Tensor) or q.dim() not in (3, 4):
-        raise RuntimeError(f"{what}: q must be [B, Hq, D] or [B, T, Hq, D]")
-    _expect(what, dev, q=(q, torch.bfloat16, q.dim()), block_tables=(block_tables, torch.int32, 2),
-            ctx_lens=(ctx_lens, torch.int32, 1))
-    B, T = q.shape[0], q.shape[1] if q.dim() == 4 else 1
-    Hq = q.shape[-2]
-    if q.shape[-1] != D or Hq % nkv or not Hq:
-        raise RuntimeError(f"{what}: q {tuple(q.shape)} over {nkv} KV heads of {D}")
-    if block_tables.shape[0] != B or ctx_lens.shape[0] != B:
-        raise RuntimeError(f"{what}: {B} sequences, {block_tables.shape[0]} block tables, {ctx_lens.shape[0]} lengths")
-    if out is None:
-        out = torch.empty(q.shape, dtype=q.dtype, device=dev)
+    index, L, P, nkv, bs, D = _kv4_geometry(what, kv4, layer)
+    dims = q.dim() if isinstance(q, torch.Tensor) else 0
+    if dims == 4:
+        B, T, Hq, qd = q.shape
+    elif dims == 3:
+        B, Hq, qd = q.shape
+        T = 1
     else:
-        _expect(what, dev, out=(out, torch.bfloat16, q.dim()))
-        if out.shape != q.shape or not out.is_contiguous():
-            raise RuntimeError(f"{what}: out must be contiguous, of the shape of q")
+        raise RuntimeError(f"{what}: q must be [B, Hq, D] or [B, T, Hq, D]")
+    _expect(what, "q", q, index, torch.bfloat16, dims)
+    _expect(what, "block_tables", block_tables, index, torch.int32, 2)
+    _expect(what, "ctx_lens", ctx_lens, index, torch.int32, 1)
+    if qd != D or Hq % nkv or not Hq:
+        raise RuntimeError(f"{what}: q {tuple(q.shape)} over {nkv} KV heads of {D}")
+    rows, width = block_tables.shape
+    if rows != B or ctx_lens.shape[0] != B:
+        raise RuntimeError(f"{what}: {B} sequences, {rows} block tables, {ctx_lens.shape[0]} lengths")
+    if out is None:
+        out = torch.empty(q.shape, dtype=torch.bfloat16, device=q.device)
+    else:
+        _expect(what, "out", out, index, torch.bfloat16, dims)
+        if out.shape != q.shape or not out.is_contiguous() or out.data_ptr() % 16:
+            raise RuntimeError(f"{what}: out must be contiguous and 16-byte aligned, of the shape of q")
     if B == 0 or T == 0:
         return out
-    if block_tables.shape[1] == 0:
+    if width == 0:
         return out.zero_()
-    q = q.reshape(B * T, Hq, D)
-    if q.stride(2) != 1 or q.stride(1) != D or q.stride(0) % 8 or q.data_ptr() % 16:
-        q = q.clone(memory_format=torch.contiguous_format)
-    if block_tables.stride(1) != 1:
-        block_tables = block_tables.contiguous()
-    tstride = block_tables.stride(0) if B > 1 else block_tables.shape[1]
-    if tstride < block_tables.shape[1]:
-        block_tables, tstride = block_tables.contiguous(), block_tables.shape[1]
+    q_stride = Hq * D
+    if not q.is_contiguous():
+        q = q.reshape(B * T, Hq, D)
+        q_stride = q.stride(0)
+        if q.stride(2) != 1 or q.stride(1) != D or q_stride % 8 or q_stride < Hq * D:
+            q, q_stride = q.clone(memory_format=torch.contiguous_format), Hq * D
+    if q.data_ptr() % 16:
+        q, q_stride = q.clone(memory_format=torch.contiguous_format), Hq * D
+    t_stride = width
+    if not block_tables.is_contiguous():
+        t_stride = block_tables.stride(0)
+        if block_tables.stride(1) != 1 or t_stride < width:
+            block_tables, t_stride = block_tables.contiguous(), width
     ctx_lens = ctx_lens.contiguous()
-    with torch.cuda.device(dev):
-        if workspace is None:
-            need = N.lib().mvb_paged_attention_decode_kv4_workspace_bytes(B, T, Hq, nkv, D, kv4.get_device())
-            workspace = torch.empty(need, dtype=torch.uint8, device=dev)
-        else:
-            _expect(what, dev, workspace=(workspace, torch.uint8, 1))
-        N.check(N.lib().mvb_paged_attention_decode_kv4(
-            out.data_ptr(), Hq * D, q.data_ptr(), q.stride(0), kv4.data_ptr(), block_tables.data_ptr(), tstride,
-            block_tables.shape[1], ctx_lens.data_ptr(), B, T, Hq, nkv, D, L, int(layer), P, bs, float(scale),
-            float(softcap), int(window), workspace.data_ptr(), workspace.numel(), _st(kv4)), what)
+    if workspace is None:
+        workspace = torch.empty(_kv4_workspace_bytes(B, T, Hq, nkv, D, index), dtype=torch.uint8, device=q.device)
+    else:
+        _expect(what, "workspace", workspace, index, torch.uint8, 1)
+        if not workspace.is_contiguous():
+            raise RuntimeError(f"{what}: workspace must be contiguous")
+    N.on_device(index, what, N.lib().mvb_paged_attention_decode_kv4, out.data_ptr(), Hq * D, q.data_ptr(), q_stride,
+                kv4.data_ptr(), block_tables.data_ptr(), t_stride, width, ctx_lens.data_ptr(), B, T, Hq, nkv, D, L,
+                int(layer), P, bs, float(scale), float(softcap), int(window), workspace.data_ptr(), workspace.numel())
     return out
 
 
@@ -600,47 +625,49 @@ def assign_slots(block_tables: torch.Tensor, ctx_lens: torch.Tensor, new_lens: t
     ``new_lens`` for every sequence to be granted; the entries behind the last token are -1.  A sequence that does not
     fit (its table row, the free list, ``num_tokens``) takes nothing: ``granted`` 0 and slots -1."""
     what = "assign_slots"
-    if not isinstance(block_tables, torch.Tensor):
-        raise RuntimeError(f"{what}: block_tables must be a tensor")
-    dev = block_tables.device
-    _expect(what, dev, block_tables=(block_tables, torch.int32, 2), ctx_lens=(ctx_lens, torch.int32, 1),
-            new_lens=(new_lens, torch.int32, 1), free_blocks=(free_blocks, torch.int32, 1))
+    index = block_tables.get_device() if isinstance(block_tables, torch.Tensor) else -1
+    _expect(what, "block_tables", block_tables, index, torch.int32, 2)
+    _expect(what, "ctx_lens", ctx_lens, index, torch.int32, 1)
+    _expect(what, "new_lens", new_lens, index, torch.int32, 1)
+    _expect(what, "free_blocks", free_blocks, index, torch.int32, 1)
     B, width = block_tables.shape
     if ctx_lens.shape[0] != B or new_lens.shape[0] != B:
         raise RuntimeError(f"{what}: {B} block tables, {ctx_lens.shape[0]} and {new_lens.shape[0]} lengths")
-    if width > 1 and block_tables.stride(1) != 1 or B > 1 and block_tables.stride(0) < width:
-        raise RuntimeError(f"{what}: the rows of block_tables must be contiguous and apart")
+    t_stride = width
+    if not block_tables.is_contiguous():
+        t_stride = block_tables.stride(0) if B > 1 else width
+        if width > 1 and block_tables.stride(1) != 1 or t_stride < width:
+            raise RuntimeError(f"{what}: the rows of block_tables must be contiguous and apart")
     if free_head is not None:
-        _expect(what, dev, free_head=(free_head, torch.int32, 1))
+        _expect(what, "free_head", free_head, index, torch.int32, 1)
         if free_head.numel() != 1:
             raise RuntimeError(f"{what}: free_head must hold one number")
     if num_tokens < 0:
         raise RuntimeError(f"{what}: num_tokens {num_tokens}")
     ctx_lens, new_lens, free_blocks = ctx_lens.contiguous(), new_lens.contiguous(), free_blocks.contiguous()
+    dev = block_tables.device
     slots = torch.empty(num_tokens, dtype=torch.int64, device=dev)
     positions = torch.empty(num_tokens, dtype=torch.int32, device=dev)
-    small = torch.empty(2 * B + 2, dtype=torch.int32, device=dev)
-    seq_start, granted, head = small[:B + 1], small[B + 1:2 * B + 1], small[2 * B + 1:]
-    with torch.cuda.device(dev):
-        N.check(N.lib().mvb_assign_slots(
-            slots.data_ptr(), positions.data_ptr(), seq_start.data_ptr(), granted.data_ptr(), head.data_ptr(),
-            block_tables.data_ptr(), block_tables.stride(0) if B > 1 else width, width, ctx_lens.data_ptr(),
-            new_lens.data_ptr(), free_blocks.data_ptr(), free_blocks.shape[0], N.ptr(free_head), B, int(block_size),
-            int(num_tokens), _st(block_tables)), what)
+    seq_start, granted, head = torch.empty(2 * B + 2, dtype=torch.int32, device=dev).split((B + 1, B, 1))
+    start_at = seq_start.data_ptr()
+    N.on_device(index, what, N.lib().mvb_assign_slots, slots.data_ptr(), positions.data_ptr(), start_at,
+                start_at + 4 * (B + 1), start_at + 4 * (2 * B + 1), block_tables.data_ptr(), t_stride, width,
+                ctx_lens.data_ptr(), new_lens.data_ptr(), free_blocks.data_ptr(), free_blocks.shape[0],
+                N.ptr(free_head), B, int(block_size), int(num_tokens))
     return SlotPlan(slots, positions, seq_start, granted, head)
 
 
 # ------------------------------------------------------------------ drafted tokens
-def _prob_rows(t: torch.Tensor) -> torch.Tensor:
-    """``t`` [B, n, V] with rows of stride-1 entries a fixed distance apart, else a copy."""
+def _prob_rows(t: torch.Tensor) -> tuple[torch.Tensor, int]:
+    """``t`` [B, n, V] with rows of stride-1 entries a fixed distance apart, else a copy; and that distance."""
     B, n, V = t.shape
-    ok = t.stride(2) == 1 and (n == 1 or t.stride(1) >= V) and (B == 1 or n == 1 or t.stride(0) == n * t.stride(1))
-    return t if ok and (B == 1 or t.stride(0) >= V) else t.contiguous()
-
-
-def _row_stride(t: torch.Tensor) -> int:
-    B, n, V = t.shape
-    return t.stride(1) if n > 1 else t.stride(0) if B > 1 else V
+    if t.is_contiguous():
+        return t, V
+    s0, s1, s2 = t.stride()
+    row = s1 if n > 1 else s0 if B > 1 else V
+    if (s2 == 1 or V == 1) and row >= V and (B == 1 or n == 1 or s0 == n * s1):
+        return t, row
+    return t.contiguous(), V
 
 
 def verify_drafts(target_probs: torch.Tensor, draft_tokens: torch.Tensor, uniforms: torch.Tensor,
@@ -657,41 +684,37 @@ def verify_drafts(target_probs: torch.Tensor, draft_tokens: torch.Tensor, unifor
     (inverse CDF in vocabulary order with the last uniform, sums in 64 bits).  Returns ``(tokens
     int64 [B, K + 1], accepted int32 [B])``: accepted drafts, the drawn token, then -1."""
     what = "verify_drafts"
-    if not isinstance(target_probs, torch.Tensor):
-        raise RuntimeError(f"{what}: target_probs must be a tensor")
-    dev = target_probs.device
-    _expect(what, dev, target_probs=(target_probs, torch.float32, 3), draft_tokens=(draft_tokens, torch.int64, 2),
-            uniforms=(uniforms, torch.float32, 2))
+    index = target_probs.get_device() if isinstance(target_probs, torch.Tensor) else -1
+    _expect(what, "target_probs", target_probs, index, torch.float32, 3)
+    _expect(what, "draft_tokens", draft_tokens, index, torch.int64, 2)
+    _expect(what, "uniforms", uniforms, index, torch.float32, 2)
     B, rows, V = target_probs.shape
     K = rows - 1
-    if K < 0 or V == 0 or tuple(draft_tokens.shape) != (B, K) or tuple(uniforms.shape) != (B, rows):
+    if K < 0 or V == 0 or draft_tokens.shape != (B, K) or uniforms.shape != (B, rows):
         raise RuntimeError(f"{what}: target_probs {tuple(target_probs.shape)}, draft_tokens "
                            f"{tuple(draft_tokens.shape)}, uniforms {tuple(uniforms.shape)}")
     if draft_probs is not None:
-        _expect(what, dev, draft_probs=(draft_probs, torch.float32, 3))
-        if tuple(draft_probs.shape) != (B, K, V):
+        _expect(what, "draft_probs", draft_probs, index, torch.float32, 3)
+        if draft_probs.shape != (B, K, V):
             raise RuntimeError(f"{what}: draft_probs must be {(B, K, V)}, not {tuple(draft_probs.shape)}")
     if draft_lens is not None:
-        _expect(what, dev, draft_lens=(draft_lens, torch.int32, 1))
+        _expect(what, "draft_lens", draft_lens, index, torch.int32, 1)
         if draft_lens.shape[0] != B:
             raise RuntimeError(f"{what}: {B} sequences, {draft_lens.shape[0]} draft_lens")
         draft_lens = draft_lens.contiguous()
-    out = torch.empty(B, rows, dtype=torch.int64, device=dev)
-    accepted = torch.empty(B, dtype=torch.int32, device=dev)
+    out = torch.empty(B, rows, dtype=torch.int64, device=target_probs.device)
+    accepted = torch.empty(B, dtype=torch.int32, device=target_probs.device)
     if B == 0:
         return out, accepted
-    target_probs = _prob_rows(target_probs)
+    target_probs, p_stride = _prob_rows(target_probs)
     q_stride = V
     if draft_probs is not None:
         if K == 0:
             draft_probs = None
         else:
-            draft_probs = _prob_rows(draft_probs)
-            q_stride = _row_stride(draft_probs)
+            draft_probs, q_stride = _prob_rows(draft_probs)
     draft_tokens, uniforms = draft_tokens.contiguous(), uniforms.contiguous()
-    with torch.cuda.device(dev):
-        N.check(N.lib().mvb_verify_drafts(out.data_ptr(), accepted.data_ptr(), target_probs.data_ptr(),
-                                          _row_stride(target_probs), N.ptr(draft_probs), q_stride,
-                                          draft_tokens.data_ptr(), uniforms.data_ptr(), N.ptr(draft_lens), B, K, V,
-                                          _st(target_probs)), what)
+    N.on_device(index, what, N.lib().mvb_verify_drafts, out.data_ptr(), accepted.data_ptr(), target_probs.data_ptr(),
+                p_stride, N.ptr(draft_probs), q_stride, draft_tokens.data_ptr(), uniforms.data_ptr(),
+                N.ptr(draft_lens), B, K, V)
     return out, accepted
