@@ -7,9 +7,13 @@
 // A group that holds a NaN or an infinity (or spans more than fp32 holds) gets a NaN pair and reads
 // back as NaN.
 //
-// Both are bound by memory: 2 bytes a value on the bf16 side, 9/16 on the other.  A lane owns
-// 8 channels: a 16-byte load (or store) of bf16 and one 32-bit word of codes; eight lanes share a
-// group and find its minimum and maximum with three exchanges.
+// Both should be bound by memory: 2 bytes a value on the bf16 side, 9/16 on the other.  A lane owns 8 channels of
+// K and of V of a token, for one head or two (HEADS): a 16-byte load (or store) of bf16 and one 32-bit word of
+// codes each, all under way together and with one look at the token's slot.  Eight lanes share a group and
+// find its minimum and maximum, on packed bf16, with three exchanges.  That leaves writing some 6 instructions a
+// value before arithmetic costs more than memory, so a code is not a division: fma(x - m, 1 / s, 1.5 * 2^23)
+// rounds and leaves the code in the low bits.  Where 1 / s moved up and down by 2^-20 disagree (ties mostly, one
+// value in 500), the exact remainder x - m - u s of the lower code decides.
 #include "common.cuh"
 #include "host.h"
 #include "kv4.cuh"
@@ -30,8 +34,8 @@ struct Kv4Args {
   unsigned* err;
 };
 
-// Record and row of a slot; false for a slot outside the pool (negative slots are padding).
-__device__ __forceinline__ bool slot_record(const Kv4Args& a, int64_t slot, int head, int64_t& rec, int& row) {
+// Record (of head 0) and row of a slot; false for a slot outside the pool (negative slots are padding).
+__device__ __forceinline__ bool slot_record(const Kv4Args& a, int64_t slot, int64_t& rec, int& row) {
   if (slot < 0) return false;
   const int64_t t16 = slot >> 4;
   if (t16 >= a.slot_limit16) {
@@ -39,117 +43,174 @@ __device__ __forceinline__ bool slot_record(const Kv4Args& a, int64_t slot, int 
     return false;
   }
   const uint32_t t = static_cast<uint32_t>(t16);
-  const uint32_t block = t / a.recs;
-  rec = (static_cast<int64_t>(block) * a.heads + head) * a.recs + (t - block * a.recs);
+  const uint32_t block = a.recs == 1 ? t : t / a.recs;
+  rec = static_cast<int64_t>(block) * a.heads * a.recs + (t - block * a.recs);
   row = static_cast<int>(slot & 15);
   return true;
 }
 
-__device__ __forceinline__ __nv_bfloat162 as_bf162(uint32_t v) {
-  return *reinterpret_cast<__nv_bfloat162*>(&v);
-}
+__device__ __forceinline__ __nv_bfloat162 as_bf162(uint32_t v) { return *reinterpret_cast<__nv_bfloat162*>(&v); }
 __device__ __forceinline__ uint32_t as_u32(__nv_bfloat162 v) { return *reinterpret_cast<uint32_t*>(&v); }
 
-// One lane per (token, K|V, head, 8 channels).
-template <int D>
-__global__ void __launch_bounds__(kThreads) kv4_write_kernel(Kv4Args a, const __nv_bfloat16* __restrict__ k,
-                                                             const __nv_bfloat16* __restrict__ v) {
-  using P = Kv4<D>;
-  constexpr int LANES = D / 8;
-  pdl_launch_dependents();
-  pdl_wait();
-  const int64_t gt = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x;
-  const int64_t unit = gt / LANES;
-  const int cb = static_cast<int>(gt % LANES);
-  const int64_t token = unit / (2 * a.heads);
-  const int rest = static_cast<int>(unit - token * 2 * a.heads);
-  const bool is_v = rest >= a.heads;
-  const int head = is_v ? rest - a.heads : rest;
-  // all lanes of an 8-lane group share the unit, so they stay or leave together; the exchanges below
-  // name the whole warp, so no lane returns before them
-  bool live = token < a.tokens;
-  int64_t rec = 0;
-  int row = 0;
-  live = live && slot_record(a, live ? a.slots[token] : -1, head, rec, row);
-  uint4 raw = make_uint4(0u, 0u, 0u, 0u);
-  if (live) {
-    const __nv_bfloat16* src = is_v ? v + token * a.v_stride + head * a.v_head_stride
-                                    : k + token * a.k_stride + head * a.k_head_stride;
-    raw = *reinterpret_cast<const uint4*>(src + 8 * cb);
-  }
-  const uint32_t x[4] = {raw.x, raw.y, raw.z, raw.w};
-  __nv_bfloat162 lo2 = as_bf162(x[0]), hi2 = lo2;
-#pragma unroll
-  for (int i = 1; i < 4; ++i) {
-    lo2 = __hmin2_nan(lo2, as_bf162(x[i]));
-    hi2 = __hmax2_nan(hi2, as_bf162(x[i]));
-  }
-#pragma unroll
-  for (int o = 1; o < 8; o <<= 1) {
-    lo2 = __hmin2_nan(lo2, as_bf162(__shfl_xor_sync(0xffffffffu, as_u32(lo2), o)));
-    hi2 = __hmax2_nan(hi2, as_bf162(__shfl_xor_sync(0xffffffffu, as_u32(hi2), o)));
-  }
-  if (!live) return;
-  const float low = __bfloat162float(__hmin_nan(lo2.x, lo2.y));
-  const float high = __bfloat162float(__hmax_nan(hi2.x, hi2.y));
-  float scale = bf16_round(__fdiv_rn(high - low, 15.0f));
-  float base = low;
-  if (!(fabsf(scale) <= 3.3895314e38f) || !(fabsf(low) <= 3.3895314e38f))
-    scale = base = __int_as_float(0x7fc00000);
-  uint32_t word = 0;
-  if (scale > 0.0f) {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const float xv = __uint_as_float((i & 1) ? (x[i >> 1] & 0xffff0000u) : (x[i >> 1] << 16));
-      const int u = __float2int_rn(__fdiv_rn(xv - base, scale));
-      word |= static_cast<uint32_t>(min(max(u, 0), 15)) << (4 * i);
-    }
-  }
-  const int g = cb >> 3, w = cb & 7;
-  uint8_t* r = a.pool + rec * P::RECORD;
-  *reinterpret_cast<uint32_t*>(r + (is_v ? P::V_CODES : 0) + row * P::ROW + 4 * (P::NG * w + g)) = word;
-  if (w == 0)
-    *reinterpret_cast<__nv_bfloat162*>(r + (is_v ? P::V_PAIRS : P::K_PAIRS) + row * P::PAIRS + 4 * g) =
-        __floats2bfloat162_rn(scale, base);
+constexpr float kMagic = 12582912.0f;   // 1.5 * 2^23: a sum's low bits are the rounded addend
+constexpr float kFltMax = 3.40282347e38f;
+constexpr uint32_t kPackBias = 0x4B400000u * 0x11111111u;  // the magic numbers' bits in the packed word, mod 2^32
+
+// x / 15 correctly rounded: with y = RN(1 / 15) and q near the quotient, q + (x - 15 q) y rounds to it (Markstein,
+// "Computation of elementary functions on the IBM RISC System/6000 processor", 1990); the remainder is exact away
+// from underflow, where the division itself is used.
+__device__ __forceinline__ float fifteenth(float x) {
+  if (fabsf(x) < 0x1p-90f) return __fdiv_rn(x, 15.0f);
+  const float y = 1.0f / 15.0f, q = x * y;
+  return fmaf(fmaf(-15.0f, q, x), y, q);
 }
 
-// One lane per (token, K|V, head, 8 channels).  A token without a slot in the pool reads as zeros.
-template <int D>
-__global__ void __launch_bounds__(kThreads) kv4_read_kernel(Kv4Args a, __nv_bfloat16* __restrict__ k,
-                                                            __nv_bfloat16* __restrict__ v) {
+// Codes of 8 values of a group with minimum `low` and scale `scale` > 0, lowest nibble first.
+__device__ __forceinline__ uint32_t quantise8(const uint32_t (&x)[4], float low, float scale) {
+  float v[8];
+#pragma unroll
+  for (int j = 0; j < 8; ++j)
+    v[j] = __uint_as_float((j & 1) ? (x[j >> 1] & 0xffff0000u) : (x[j >> 1] << 16)) - low;
+  uint32_t word = 0;
+  if (scale < 0x1p-100f) {  // 1 / s may not be finite, and a subnormal s may leave the largest code above 15
+#pragma unroll 1
+    for (int j = 7; j >= 0; --j) {
+      const uint32_t h = j >= 6 ? x[3] : j >= 4 ? x[2] : j >= 2 ? x[1] : x[0];
+      const float y = __uint_as_float((j & 1) ? (h & 0xffff0000u) : (h << 16)) - low;
+      word = word * 16u + static_cast<uint32_t>(fminf(rintf(__fdiv_rn(y, scale)), 15.0f));
+    }
+    return word;
+  }
+  float inv;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inv) : "f"(scale));  // within 2^-22
+  const float up = inv * (1.0f + 0x1p-20f), down = inv * (1.0f - 0x1p-20f);
+  uint32_t differ = 0, below[8];
+#pragma unroll
+  for (int j = 7; j >= 0; --j) {
+    const uint32_t above = __float_as_uint(fmaf(v[j], up, kMagic));
+    below[j] = __float_as_uint(fmaf(v[j], down, kMagic));
+    differ |= above ^ below[j];
+    word = word * 16u + below[j];
+  }
+  word -= kPackBias;
+  if (differ != 0) {
+    const float half = 0.5f * scale;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const float r = fmaf(kMagic - __uint_as_float(below[j]), scale, v[j]);  // exact: a short multiple of v's last place
+      word += (r > half || (r == half && (below[j] & 1u))) ? 1u << (4 * j) : 0u;
+    }
+  }
+  return word;
+}
+
+// A lane per (token, HEADS heads, 8 channels).
+template <int D, int HEADS>
+__global__ void __launch_bounds__(kThreads) kv4_write_kernel(const Kv4Args a, const __nv_bfloat16* __restrict__ k,
+                                                             const __nv_bfloat16* __restrict__ v) {
   using P = Kv4<D>;
-  constexpr int LANES = D / 8;
+  constexpr int LANES = D / 8, N = 2 * HEADS;
   pdl_launch_dependents();
   pdl_wait();
-  const int64_t gt = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x;
-  const int64_t unit = gt / LANES;
-  const int cb = static_cast<int>(gt % LANES);
-  const int64_t token = unit / (2 * a.heads);
-  if (token >= a.tokens) return;
-  const int rest = static_cast<int>(unit - token * 2 * a.heads);
-  const bool is_v = rest >= a.heads;
-  const int head = is_v ? rest - a.heads : rest;
-  int64_t rec;
-  int row;
-  uint4 o = make_uint4(0u, 0u, 0u, 0u);
-  if (slot_record(a, a.slots[token], head, rec, row)) {
-    const uint8_t* r = a.pool + rec * P::RECORD;
-    const int g = cb >> 3, w = cb & 7;
-    const uint32_t word = *reinterpret_cast<const uint32_t*>(r + (is_v ? P::V_CODES : 0) + row * P::ROW +
-                                                             4 * (P::NG * w + g));
-    const __nv_bfloat162 pair = *reinterpret_cast<const __nv_bfloat162*>(r + (is_v ? P::V_PAIRS : P::K_PAIRS) +
-                                                                         row * P::PAIRS + 4 * g);
-    const float scale = __bfloat162float(pair.x), base = __bfloat162float(pair.y);
-    uint32_t q[4];
+  const uint32_t x0 = blockIdx.x * kThreads + threadIdx.x;
+  const uint32_t per = static_cast<uint32_t>(a.heads / HEADS) * LANES;  // lanes of a token
+  const uint32_t token = x0 / per, rest = x0 - token * per;
+  const int head = static_cast<int>(rest / LANES) * HEADS, cb = static_cast<int>(rest % LANES);
+  const int g = cb >> 3, w = cb & 7;
+  // the eight lanes of a group stay or leave together, but the exchanges below name the whole warp: no lane
+  // returns before them
+  int64_t rec = 0;
+  int row = 0;
+  const bool live = token < a.tokens && slot_record(a, a.slots[token], rec, row);
+  uint4 raw[N];
 #pragma unroll
-    for (int i = 0; i < 4; ++i)  // scale * u is exact in fp32 (8 + 4 bits): one rounding in the fma, one to bf16
-      q[i] = as_u32(__floats2bfloat162_rn(fmaf(scale, static_cast<float>((word >> (8 * i)) & 15u), base),
-                                          fmaf(scale, static_cast<float>((word >> (8 * i + 4)) & 15u), base)));
-    o = make_uint4(q[0], q[1], q[2], q[3]);
+  for (int i = 0; i < N; ++i) raw[i] = make_uint4(0u, 0u, 0u, 0u);
+  if (live) {
+    const __nv_bfloat16* ks = k + token * a.k_stride + head * a.k_head_stride + 8 * cb;
+    const __nv_bfloat16* vs = v + token * a.v_stride + head * a.v_head_stride + 8 * cb;
+#pragma unroll
+    for (int i = 0; i < N; i += 2) {
+      raw[i] = *reinterpret_cast<const uint4*>(ks);
+      raw[i + 1] = *reinterpret_cast<const uint4*>(vs);
+      ks += a.k_head_stride;
+      vs += a.v_head_stride;
+    }
   }
-  __nv_bfloat16* dst = is_v ? v + token * a.v_stride + head * a.v_head_stride
-                            : k + token * a.k_stride + head * a.k_head_stride;
-  *reinterpret_cast<uint4*>(dst + 8 * cb) = o;
+  uint8_t* at = a.pool + (rec + static_cast<int64_t>(head) * a.recs) * P::RECORD + row * P::ROW + 4 * (P::NG * w + g);
+  const int pair_at = P::K_PAIRS + row * P::PAIRS + 4 * g - (row * P::ROW + 4 * (P::NG * w + g));
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const uint32_t x[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
+    __nv_bfloat162 lo2 = as_bf162(x[0]), hi2 = lo2;
+#pragma unroll
+    for (int j = 1; j < 4; ++j) {
+      lo2 = __hmin2_nan(lo2, as_bf162(x[j]));
+      hi2 = __hmax2_nan(hi2, as_bf162(x[j]));
+    }
+    // both halves' results in one word for the exchanges: (minimum, -maximum)
+    __nv_bfloat162 m2 = __halves2bfloat162(__hmin_nan(lo2.x, lo2.y), __hneg(__hmax_nan(hi2.x, hi2.y)));
+#pragma unroll
+    for (int o = 1; o < 8; o <<= 1) m2 = __hmin2_nan(m2, as_bf162(__shfl_xor_sync(0xffffffffu, as_u32(m2), o)));
+    if (!live) continue;
+    float low = __bfloat162float(m2.x);
+    float scale = bf16_round(fifteenth(-__bfloat162float(m2.y) - low));
+    uint32_t word = 0;
+    if (!(scale <= kFltMax) || !(fabsf(low) <= kFltMax)) scale = low = __int_as_float(0x7fc00000);
+    else if (scale > 0.0f) word = quantise8(x, low, scale);
+    *reinterpret_cast<uint32_t*>(at + ((i & 1) ? P::V_CODES : 0)) = word;
+    if (w == 0)
+      *reinterpret_cast<__nv_bfloat162*>(at + pair_at + ((i & 1) ? P::V_PAIRS - P::K_PAIRS : 0)) =
+          __floats2bfloat162_rn(scale, low);
+    if (i & 1) at += a.recs * P::RECORD;
+  }
+}
+
+// A lane per (token, HEADS heads, 8 channels).  A token without a slot in the pool reads as zeros.  A code is
+// the bf16 number 128 + u by its bits; scale * u + min is one bf16 fma, rounded once.
+template <int D, int HEADS>
+__global__ void __launch_bounds__(kThreads) kv4_read_kernel(const Kv4Args a, __nv_bfloat16* __restrict__ k,
+                                                            __nv_bfloat16* __restrict__ v) {
+  using P = Kv4<D>;
+  constexpr int LANES = D / 8, N = 2 * HEADS;
+  pdl_launch_dependents();
+  pdl_wait();
+  const uint32_t x0 = blockIdx.x * kThreads + threadIdx.x;
+  const uint32_t per = static_cast<uint32_t>(a.heads / HEADS) * LANES;
+  const uint32_t token = x0 / per, rest = x0 - token * per;
+  if (token >= a.tokens) return;
+  const int head = static_cast<int>(rest / LANES) * HEADS, cb = static_cast<int>(rest % LANES);
+  const int g = cb >> 3, w = cb & 7;
+  int64_t rec = 0;
+  int row = 0;
+  const bool live = slot_record(a, a.slots[token], rec, row);
+  const uint8_t* r = a.pool + (rec + static_cast<int64_t>(head) * a.recs) * P::RECORD;
+  uint32_t word[N], pair[N];
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    word[i] = pair[i] = 0;
+    if (live) {
+      const uint8_t* at = r + (i >> 1) * a.recs * P::RECORD;
+      word[i] = *reinterpret_cast<const uint32_t*>(at + ((i & 1) ? P::V_CODES : 0) + row * P::ROW + 4 * (P::NG * w + g));
+      pair[i] = *reinterpret_cast<const uint32_t*>(at + ((i & 1) ? P::V_PAIRS : P::K_PAIRS) + row * P::PAIRS + 4 * g);
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const __nv_bfloat162 scale = as_bf162(__byte_perm(pair[i], 0, 0x1010)), low = as_bf162(__byte_perm(pair[i], 0, 0x3232));
+    const __nv_bfloat162 bias = as_bf162(0x43004300u);  // 128, 128
+    uint32_t y[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {  // codes j and j + 4
+      const uint32_t u = ((word[i] >> (4 * j)) & 0x000F000Fu) | 0x43004300u;
+      y[j] = as_u32(__hfma2(scale, __hsub2(as_bf162(u), bias), low));
+    }
+    const uint4 o = make_uint4(__byte_perm(y[0], y[1], 0x5410), __byte_perm(y[2], y[3], 0x5410),
+                               __byte_perm(y[0], y[1], 0x7632), __byte_perm(y[2], y[3], 0x7632));
+    const int h = head + (i >> 1);
+    __nv_bfloat16* dst = (i & 1) ? v + token * a.v_stride + h * a.v_head_stride
+                                 : k + token * a.k_stride + h * a.k_head_stride;
+    *reinterpret_cast<uint4*>(dst + 8 * cb) = o;
+  }
 }
 
 int kv4_args(Kv4Args& a, const char* what, const void* pool, const int64_t* slots, int64_t tokens, int64_t heads,
@@ -190,15 +251,20 @@ int stride_ok(const char* what, const void* p, int64_t stride, int64_t head_stri
 
 using namespace mvb;
 
-#define MVB_KV4_LAUNCH(NAME, KERNEL, ...)                                                                \
-  do {                                                                                                   \
-    const int64_t lanes = tokens * 2 * num_kv_heads * (head_dim / 8);                                    \
-    dim3 grid(static_cast<unsigned>((lanes + kThreads - 1) / kThreads)), block(kThreads);                \
-    switch (head_dim) {                                                                                  \
-      case 64: return launch(NAME, KERNEL<64>, grid, block, 0, st, a, __VA_ARGS__);                      \
-      case 128: return launch(NAME, KERNEL<128>, grid, block, 0, st, a, __VA_ARGS__);                    \
-      default: return launch(NAME, KERNEL<256>, grid, block, 0, st, a, __VA_ARGS__);                     \
-    }                                                                                                    \
+// Two heads a lane where they come in pairs and there are lanes enough to fill the GPU all the same.
+#define MVB_KV4_LAUNCH(NAME, KERNEL, ...)                                                                 \
+  do {                                                                                                    \
+    const int64_t lanes = tokens * num_kv_heads * (head_dim / 8);                                         \
+    const bool two = num_kv_heads % 2 == 0 && lanes >= (1 << 18);                                         \
+    dim3 grid(static_cast<unsigned>(((two ? lanes / 2 : lanes) + kThreads - 1) / kThreads)), block(kThreads); \
+    switch (head_dim + two) {                                                                             \
+      case 64: return launch(NAME, KERNEL<64, 1>, grid, block, 0, st, a, __VA_ARGS__);                    \
+      case 65: return launch(NAME, KERNEL<64, 2>, grid, block, 0, st, a, __VA_ARGS__);                    \
+      case 128: return launch(NAME, KERNEL<128, 1>, grid, block, 0, st, a, __VA_ARGS__);                  \
+      case 129: return launch(NAME, KERNEL<128, 2>, grid, block, 0, st, a, __VA_ARGS__);                  \
+      case 256: return launch(NAME, KERNEL<256, 1>, grid, block, 0, st, a, __VA_ARGS__);                  \
+      default: return launch(NAME, KERNEL<256, 2>, grid, block, 0, st, a, __VA_ARGS__);                   \
+    }                                                                                                     \
   } while (0)
 
 extern "C" int mvb_kv4_write(void* kv4, const void* k, int64_t k_stride, int64_t k_head_stride, const void* v,
