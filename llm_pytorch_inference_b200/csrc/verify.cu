@@ -10,8 +10,11 @@
 // of a vocabulary of fp32 probabilities is off by 1e-16 of the total, so the answer does not
 // depend on how the sum is split unless u lies that close to a border.
 //
-// Only one row of p (and of q) is read per sequence: bound by those 4 (8) bytes an entry, and by
-// latency for few sequences.
+// Only one row of p (and of q) is read per sequence: bound by those 4 (8) bytes an entry, and by latency for few
+// sequences.  A sequence is a cluster of up to 8 blocks: every lane looks at one draft, so that all of
+// them cost one dependent load each; every warp sums a run of the vocabulary; the blocks exchange their sums
+// through distributed shared memory; and the block in whose part the threshold falls reads one warp's run of it
+// again (out of L2), all its warps together, to find the entry.  The order of all sums is fixed.
 #include <climits>
 
 #include "common.cuh"
@@ -22,7 +25,7 @@ namespace {
 
 constexpr int kThreads = 512;
 constexpr int kWarps = kThreads / 32;
-constexpr int kMaxTiles = 2048;
+constexpr int kMaxCluster = 8;
 
 struct VerifyArgs {
   int64_t* out;
@@ -45,105 +48,197 @@ __device__ __forceinline__ double warp_sum_f64(double v) {
   return v;
 }
 
-// What entry j of the row weighs in the draw.
+// What the entries of the row weigh in the draw.
 struct Weights {
   const float* p;
   const float* q;   // the drafting row, or nullptr
   int token;        // the rejected one-hot draft, or -1
-  __device__ __forceinline__ double operator()(int j) const {
-    const double a = p[j];
-    if (q != nullptr) return fmax(a - static_cast<double>(q[j]), 0.0);
-    return j == token ? 0.0 : fmax(a, 0.0);
+  __device__ __forceinline__ double of(int j, float pj, float qj) const {
+    if (q != nullptr) return fmax(static_cast<double>(pj) - static_cast<double>(qj), 0.0);
+    return j == token ? 0.0 : fmax(static_cast<double>(pj), 0.0);
   }
 };
 
-// One CTA per sequence.
-__global__ void __launch_bounds__(kThreads) verify_kernel(VerifyArgs a) {
-  __shared__ double tile_sum[kMaxTiles];
-  __shared__ double total_s;
-  __shared__ int found;
+// Entries j .. j + 3 of a row, zeros from `end` on; VEC: j and the row are 16-byte aligned.
+template <bool VEC>
+__device__ __forceinline__ float4 load4(const float* row, int j, int end) {
+  if (VEC && j + 4 <= end) return *reinterpret_cast<const float4*>(row + j);
+  float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  if (j < end) v.x = row[j];
+  if (j + 1 < end) v.y = row[j + 1];
+  if (j + 2 < end) v.z = row[j + 2];
+  if (j + 3 < end) v.w = row[j + 3];
+  return v;
+}
+
+// The lane's share of the sum over [begin, end), begin a multiple of 4.
+template <bool VEC>
+__device__ __forceinline__ double run_sum(const Weights& w, int begin, int end, int lane) {
+  double s = 0.0;
+#pragma unroll 1
+  for (int j = begin + 4 * lane; j < end; j += 128) {
+    const float4 p = load4<VEC>(w.p, j, end);
+    const float4 q = w.q != nullptr ? load4<VEC>(w.q, j, end) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    s += (w.of(j, p.x, q.x) + w.of(j + 1, p.y, q.y)) + (w.of(j + 2, p.z, q.z) + w.of(j + 3, p.w, q.w));
+  }
+  return s;
+}
+
+// The first entry of [begin, end) at which `before` plus the weights so far exceed thr; the last one with any
+// weight if rounding leaves none; -1 if nothing weighs.
+template <bool VEC>
+__device__ __forceinline__ int run_find(const Weights& w, int begin, int end, double before, double thr, int lane) {
+  int last = -1;
+  const float4 zero = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  float4 p = load4<VEC>(w.p, begin + 4 * lane, end);
+  float4 q = w.q != nullptr ? load4<VEC>(w.q, begin + 4 * lane, end) : zero;
+  for (int j0 = begin; j0 < end; j0 += 128) {
+    const int j = j0 + 4 * lane;
+    const float4 pc = p, qc = q;
+    p = load4<VEC>(w.p, j + 128, end);  // the next ones are under way meanwhile
+    q = w.q != nullptr ? load4<VEC>(w.q, j + 128, end) : zero;
+    const double x[4] = {w.of(j, pc.x, qc.x), w.of(j + 1, pc.y, qc.y), w.of(j + 2, pc.z, qc.z), w.of(j + 3, pc.w, qc.w)};
+    const double own = (x[0] + x[1]) + (x[2] + x[3]);
+    double c = own;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const double y = __shfl_up_sync(0xffffffffu, c, o);
+      if (lane >= o) c += y;
+    }
+    double at = before + (c - own);
+    int hit = -1, some = -1;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      at += x[i];
+      if (x[i] > 0.0) {
+        some = j + i;
+        if (hit < 0 && at > thr) hit = j + i;
+      }
+    }
+    const unsigned hits = __ballot_sync(0xffffffffu, hit >= 0), any = __ballot_sync(0xffffffffu, some >= 0);
+    if (hits) return __shfl_sync(0xffffffffu, hit, __ffs(hits) - 1);
+    if (any) last = __shfl_sync(0xffffffffu, some, 31 - __clz(any));
+    before += __shfl_sync(0xffffffffu, c, 31);
+  }
+  return last;
+}
+
+// Of the n <= 32 sums of consecutive parts: the first one at which `before` plus the sums so far exceed thr (the
+// last with any weight if rounding leaves none, -1 if nothing weighs), and what lies before it.  A whole warp's.
+__device__ __forceinline__ int pick_part(const double* sums, int n, double before, double thr, int lane, double& start) {
+  const double x = lane < n ? sums[lane] : 0.0;
+  double c = x;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const double y = __shfl_up_sync(0xffffffffu, c, o);
+    if (lane >= o) c += y;
+  }
+  const unsigned hits = __ballot_sync(0xffffffffu, x > 0.0 && before + c > thr), any = __ballot_sync(0xffffffffu, x > 0.0);
+  const int at = hits ? __ffs(hits) - 1 : any ? 31 - __clz(any) : -1;
+  start = before + __shfl_sync(0xffffffffu, c - x, at < 0 ? 0 : at);
+  return at;
+}
+
+__device__ __forceinline__ double dsmem_ld_f64(const double* p, uint32_t rank) {
+  uint32_t remote;
+  double v;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(smem_u32(p)), "r"(rank));
+  asm volatile("ld.shared::cluster.f64 %0, [%1];" : "=d"(v) : "r"(remote) : "memory");
+  return v;
+}
+
+// A cluster of `blocks` blocks per sequence, warp x of it summing entries [x run, (x + 1) run).
+__global__ void __launch_bounds__(kThreads, 2) verify_kernel(const VerifyArgs a, const int blocks, const int run) {
+  __shared__ double warp_total[kWarps], part_total[kWarps];
+  __shared__ double block_total, sums[kMaxCluster];
   // dependents start at this kernel's end only: they read its outputs as step metadata before they wait
   pdl_wait();
-  const int b = blockIdx.x, tid = threadIdx.x, lane = tid & 31, wid = tid >> 5;
+  const int tid = threadIdx.x, lane = tid & 31, wid = tid >> 5;
+  const int b = blockIdx.x / blocks, rank = blockIdx.x - b * blocks;
   const int64_t* tok = a.tokens + static_cast<int64_t>(b) * a.drafts;
   const float* u = a.u + static_cast<int64_t>(b) * (a.drafts + 1);
   const int n_drafts = a.lens != nullptr ? min(max(a.lens[b], 0), a.drafts) : a.drafts;
-  int n = 0;
-  for (; n < n_drafts; ++n) {
-    const int64_t d = tok[n];
-    if (d < 0 || d >= a.vocab) {
-      if (tid == 0) report(a.err, kDevBadToken);
+  const float* p_rows = a.p + static_cast<int64_t>(b) * (a.drafts + 1) * a.p_stride;
+  const float* q_rows = a.q + static_cast<int64_t>(b) * a.drafts * a.q_stride;  // used where a.q is given
+  int n = n_drafts;  // the first draft that is not accepted
+  for (int i0 = 0; i0 < a.drafts; i0 += 32) {
+    // all given or not are looked at, so that no load waits for the number of drafts
+    const int i = i0 + lane;
+    bool ok = true, known = true;
+    if (i < a.drafts) {
+      const int64_t d = tok[i];
+      const float ui = u[i];
+      known = d >= 0 && d < a.vocab;
+      if (known) {
+        const double q = a.q != nullptr ? static_cast<double>(q_rows[i * a.q_stride + d]) : 1.0;
+        ok = static_cast<double>(ui) * q < static_cast<double>(p_rows[i * a.p_stride + d]);
+      }
+    }
+    if (i < n_drafts && !known && rank == 0 && wid == 0) report(a.err, kDevBadToken);
+    const unsigned no = __ballot_sync(0xffffffffu, i < n_drafts && !(ok && known));
+    if (no) {
+      n = i0 + __ffs(no) - 1;
       break;
     }
-    const double pd = a.p[(static_cast<int64_t>(b) * (a.drafts + 1) + n) * a.p_stride + d];
-    const double qd = a.q != nullptr ? a.q[(static_cast<int64_t>(b) * a.drafts + n) * a.q_stride + d] : 1.0;
-    if (!(static_cast<double>(u[n]) * qd < pd)) break;
   }
   const bool rejected = n < n_drafts;
   Weights w;
-  w.p = a.p + (static_cast<int64_t>(b) * (a.drafts + 1) + n) * a.p_stride;
-  w.q = rejected && a.q != nullptr ? a.q + (static_cast<int64_t>(b) * a.drafts + n) * a.q_stride : nullptr;
+  w.p = p_rows + n * a.p_stride;
+  w.q = rejected && a.q != nullptr ? q_rows + n * a.q_stride : nullptr;
   w.token = -1;
   if (rejected && a.q == nullptr && tok[n] >= 0 && tok[n] < a.vocab) w.token = static_cast<int>(tok[n]);
+  const float draw = u[a.drafts];
 
-  const int tile = (((a.vocab + kMaxTiles - 1) / kMaxTiles + 127) / 128) * 128;
-  const int tiles = (a.vocab + tile - 1) / tile;
+  const int begin = (rank * kWarps + wid) * run, end = min(begin + run, a.vocab);
+  double total = 0.0, before = 0.0;  // of the row, of the blocks before the owner
+  int owner = -1;                    // the block that the threshold falls into
+  bool vec = false;
   for (int pass = 0; pass < 2; ++pass) {
-    for (int t = wid; t < tiles; t += kWarps) {
-      double s = 0.0;
-      const int end = min((t + 1) * tile, a.vocab);
-      for (int j = t * tile + lane; j < end; j += 32) s += w(j);
-      s = warp_sum_f64(s);
-      if (lane == 0) tile_sum[t] = s;
-    }
+    vec = (reinterpret_cast<uintptr_t>(w.p) & 15) == 0 && (w.q == nullptr || (reinterpret_cast<uintptr_t>(w.q) & 15) == 0);
+    const double s = warp_sum_f64(vec ? run_sum<true>(w, begin, end, lane) : run_sum<false>(w, begin, end, lane));
+    if (lane == 0) warp_total[wid] = s;
     __syncthreads();
     if (wid == 0) {
-      double s = 0.0;
-      for (int t = lane; t < tiles; t += 32) s += tile_sum[t];
-      s = warp_sum_f64(s);
-      if (lane == 0) total_s = s;
+      const double t = warp_sum_f64(lane < kWarps ? warp_total[lane] : 0.0);
+      if (lane == 0) block_total = t;
     }
-    __syncthreads();
-    if (total_s > 0.0 || !rejected) break;
+    cluster_sync();
+    if (tid < blocks) sums[tid] = dsmem_ld_f64(&block_total, tid);
+    cluster_sync();  // everybody has read: block_total may change, or its block end
+    total = warp_sum_f64(lane < blocks ? sums[lane] : 0.0);
+    owner = pick_part(sums, blocks, 0.0, static_cast<double>(draw) * total, lane, before);
+    if (total > 0.0 || !rejected) break;
+    __syncthreads();  // sums has been read
     // nothing is left of p - q (equal rows, or rounding): draw from p itself
-    __syncthreads();
     w.q = nullptr;
     w.token = -1;
   }
-  if (wid == 0) {
-    // `total_s > 0` false: no entry weighs anything (or a NaN): no token
-    int pick = -1;
-    const double total = total_s;
-    if (total > 0.0) {
-      const double thr = static_cast<double>(u[a.drafts]) * total;
-      double before = 0.0;
-      int t = 0;
-      for (; t < tiles - 1 && !(before + tile_sum[t] > thr); ++t) before += tile_sum[t];
-      const int end = min((t + 1) * tile, a.vocab);
-      int last = -1;
-      for (int j0 = t * tile; j0 < end && pick < 0; j0 += 32) {
-        const int j = j0 + lane;
-        const double x = j < end ? w(j) : 0.0;
-        double c = x;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-          const double y = __shfl_up_sync(0xffffffffu, c, o);
-          if (lane >= o) c += y;
-        }
-        const unsigned hit = __ballot_sync(0xffffffffu, before + c > thr && x > 0.0);
-        const unsigned any = __ballot_sync(0xffffffffu, x > 0.0);
-        if (hit) pick = j0 + __ffs(hit) - 1;
-        if (any) last = j0 + 31 - __clz(any);
-        before += __shfl_sync(0xffffffffu, c, 31);
-      }
-      if (pick < 0) pick = last;
-    }
-    if (lane == 0) found = pick;
-  }
-  __syncthreads();
+
   int64_t* out = a.out + static_cast<int64_t>(b) * (a.drafts + 1);
-  for (int i = tid; i <= a.drafts; i += kThreads) out[i] = i < n ? tok[i] : i == n ? found : -1;
-  if (tid == 0) a.accepted[b] = n;
+  if (rank == 0) {
+    for (int i = tid; i <= a.drafts; i += kThreads)
+      if (i != n || owner < 0) out[i] = i < n ? tok[i] : -1;
+    if (tid == 0) a.accepted[b] = n;
+  }
+  if (rank != owner) return;
+  // Down to the entry: the warp's run that holds the threshold, summed again in kWarps parts where it is long,
+  // and scanned.
+  const double thr = static_cast<double>(draw) * total;
+  double start;
+  int first = (rank * kWarps + max(pick_part(warp_total, kWarps, before, thr, lane, start), 0)) * run;
+  int last = min(first + run, a.vocab), by = 0;
+  if (run > 512) {
+    const int part = (run / kWarps + 3) / 4 * 4, at = first + wid * part, to = min(at + part, last);
+    const double s = warp_sum_f64(vec ? run_sum<true>(w, at, to, lane) : run_sum<false>(w, at, to, lane));
+    if (lane == 0) part_total[wid] = s;
+    __syncthreads();
+    by = max(pick_part(part_total, kWarps, start, thr, lane, start), 0);
+    first += by * part;
+    last = min(first + part, last);
+  }
+  if (wid != by) return;
+  const int j = vec ? run_find<true>(w, first, last, start, thr, lane) : run_find<false>(w, first, last, start, thr, lane);
+  if (lane == 0) out[n] = j;
 }
 
 }  // namespace
@@ -167,6 +262,16 @@ extern "C" int mvb_verify_drafts(int64_t* out_tokens, int32_t* accepted, const f
               (long long)draft_stride, (long long)vocab);
   VerifyArgs a = {out_tokens, accepted, target_probs, target_stride, draft_probs, draft_stride, draft_tokens, uniforms,
                   draft_lens, static_cast<int>(max_drafts), static_cast<int>(vocab), device_status_ptr()};
-  return launch("verify_drafts", verify_kernel, dim3(static_cast<unsigned>(batch)), dim3(kThreads), 0,
-                reinterpret_cast<cudaStream_t>(stream), a);
+  // Blocks per sequence: as many as fill the GPU once (two blocks an SM), with some 2,048 entries each.  Rows of
+  // 151,936 entries: at batch 1 one block took 33.3 us, 4 took 12.6 and 8 take 8.9; at batch 64, 4 take 23.4 us
+  // (3.3 TB/s) and 8, in two waves, took 28.7.
+  const int64_t sms = current_sm_count();
+  MVB_REQUIRE(sms > 0, "mvb_verify_drafts: no device");
+  int blocks = kMaxCluster;
+  while (blocks > 1 && (vocab < 2048LL * blocks || batch * blocks > 2 * sms)) blocks /= 2;
+  const int64_t warps = static_cast<int64_t>(blocks) * kWarps;
+  const int run = static_cast<int>(((vocab + warps - 1) / warps + 127) / 128 * 128);
+  MVB_REQUIRE(batch * blocks <= INT_MAX, "mvb_verify_drafts: batch %lld", (long long)batch);
+  return launch_cluster("verify_drafts", verify_kernel, dim3(static_cast<unsigned>(batch * blocks)), dim3(kThreads),
+                        static_cast<unsigned>(blocks), 0, reinterpret_cast<cudaStream_t>(stream), a, blocks, run);
 }
