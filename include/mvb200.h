@@ -274,7 +274,8 @@ int mvb_kv4_read(void* k, void* v, const void* kv4, const int64_t* slots, int64_
  * b * table_stride, max_blocks entries of it are used.  A context past its table is cut
  * (MVB_DEV_BAD_POSITION); a block outside the pool counts as masked (MVB_DEV_BAD_BLOCK).
  * Scores and softmax statistics in fp32, deterministic.  workspace: at least ..._workspace_bytes()
- * bytes, 256-byte aligned, of any content; calls that overlap on the GPU need one each. */
+ * bytes, 256-byte aligned, of any content; calls that overlap on the GPU need one each.  Tables of at most
+ * 128 tokens (max_blocks * block_size) need none (NULL). */
 int64_t mvb_paged_attention_decode_kv4_workspace_bytes(int64_t batch, int64_t query_len, int64_t num_q_heads,
                                                        int64_t num_kv_heads, int64_t head_dim, int device);
 int mvb_paged_attention_decode_kv4(void* out, int64_t out_stride, const void* q, int64_t q_stride, const void* kv4,

@@ -41,8 +41,8 @@ namespace mvb {
 namespace {
 
 constexpr float kLog2e = 1.4426950408889634f;
-constexpr int kJoinThreads = 256;
 constexpr int kShortRecords = 8;  // items of at most this many records are never split
+constexpr int kItemCost = 2;      // what beginning an item costs a warp, in bursts, for the division of the work
 
 // A weight is 2^(score - reference): the reference is a row's maximum when last raised, and is raised
 // once a score passes it by more than kSlack (in powers of two), so that most records cost one vote instead
@@ -91,7 +91,7 @@ struct Kv4AttnArgs {
   float cap_log2;     // softcap * log2(e); 0 = no cap
   int window;
   int slab_rows;  // rows of the largest chunk
-  int per;        // records of a round, the unit of the division
+  bool split;     // items may be split: their rounds are bursts and kItemCost; else an item is one round
   // workspace
   struct Kv4Item* items;  // [batch * hkv * chunks]
   float2* part_ml;        // [2 workers][ROWS]
@@ -107,7 +107,7 @@ struct Kv4Item {
 // The rounds of the batch among the workers: each `size`, the first `more` one more.
 struct Kv4Split {
   int64_t size, more;
-  __device__ __forceinline__ Kv4Split(int64_t total, int workers) {
+  __device__ __forceinline__ void set(int64_t total, int workers) {
     if (total >> 32) {
       size = total / workers;
     } else {
@@ -206,11 +206,12 @@ __device__ __forceinline__ int tile_token(int r) {
   return 4 * c + ((i + c) & 3);
 }
 
-// What a sequence's cache has to offer: tiles [first, last) of 16 tokens, cut into rounds.
+// What a sequence's cache has to offer: records [first, last), divided in rounds.
 struct Kv4Seq {
   int ctx, first, last, rounds;
 };
-__device__ __forceinline__ Kv4Seq kv4_seq(const Kv4AttnArgs& a, int b, bool tell) {
+template <int BURST>
+__device__ __forceinline__ Kv4Seq kv4_seq(const Kv4AttnArgs& a, int b, bool tell = false) {
   Kv4Seq s;
   const int most = a.max_blocks * a.recs * kKv4Tokens;
   const int raw = a.ctx[b];
@@ -219,8 +220,14 @@ __device__ __forceinline__ Kv4Seq kv4_seq(const Kv4AttnArgs& a, int b, bool tell
   s.first = 0;
   if (a.window > 0) s.first = max(s.ctx - a.T + 1 - a.window, 0) / kKv4Tokens;
   s.last = (s.ctx + kKv4Tokens - 1) / kKv4Tokens;
-  s.rounds = max((s.last - s.first + a.per - 1) / a.per, 1);  // one for no keys too: it writes the zeros
+  s.rounds = a.split ? kItemCost + max(s.last - s.first + BURST - 1, 0) / BURST : 1;
   return s;
+}
+// Records [x, y) of rounds [r, r + n) of an item.
+template <int BURST>
+__device__ __forceinline__ int2 kv4_records(const Kv4AttnArgs& a, const Kv4Seq& s, int r, int n) {
+  if (!a.split) return make_int2(s.first, s.last);
+  return make_int2(s.first + max(r - kItemCost, 0) * BURST, min(s.first + max(r + n - kItemCost, 0) * BURST, s.last));
 }
 
 template <int D, int RT>
@@ -242,12 +249,11 @@ __global__ void __launch_bounds__(Kv4Cfg<D, RT>::WARPS * 32, 1) kv4_attn_kernel(
   using S = Kv4Smem<D, RT>;
   using R = Kv4Rows<RT>;
   constexpr int NG = P::NG, STAGES = S::STAGES, ROWS = R::ROWS, NT = R::NT, KT = R::KT, NC = R::NC;
-  constexpr int BURST = Kv4Cfg<D, RT>::BURST, WARPS = Kv4Cfg<D, RT>::WARPS, THREADS = WARPS * 32;
+  constexpr int BURST = Kv4Cfg<D, RT>::BURST, WARPS = Kv4Cfg<D, RT>::WARPS;
   constexpr unsigned ALL = (1u << BURST) - 1;
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ volatile int abort_flag;
-  __shared__ int64_t scan_warp[WARPS];
-  __shared__ int64_t scan_end[THREADS];  // rounds up to and with a sequence
+  __shared__ Kv4Split split;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int g = lane >> 2, c = lane & 3;
   uint8_t* ring = smem + warp * S::WARP;
@@ -260,71 +266,63 @@ __global__ void __launch_bounds__(Kv4Cfg<D, RT>::WARPS * 32, 1) kv4_attn_kernel(
   if (lane < STAGES) mbar_init(bars + lane, 1);
   fence_barrier_init();
   if (tid == 0) abort_flag = 0;
+  __syncthreads();
   pdl_wait();
 
-  // ---- this worker's rounds, [r0, r1) of the batch's total, and the sequence that r0 lies in
+  // ---- this worker's rounds, [r0, r1) of the batch's total, and the sequence that r0 lies in: every warp scans the
+  // lengths by itself, lane j a run of them
   const int subs = a.hkv * a.chunks;
-  int64_t carry = 0;
-  auto scan = [&](int base, bool tell) {  // rounds of THREADS sequences: their running sum into scan_end
-    const int b = base + tid;
-    int64_t incl = b < a.batch ? static_cast<int64_t>(kv4_seq(a, b, tell).rounds) * subs : 0;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int64_t y = __shfl_up_sync(0xffffffffu, incl, o);
-      if (lane >= o) incl += y;
-    }
-    __syncthreads();
-    if (lane == 31) scan_warp[warp] = incl;
-    __syncthreads();
-    int64_t all = 0;
-#pragma unroll
-    for (int w = 0; w < WARPS; ++w) {
-      if (w < warp) incl += scan_warp[w];
-      all += scan_warp[w];
-    }
-    scan_end[tid] = incl + carry;
-    carry += all;
-    __syncthreads();
-  };
-  for (int base = 0; base < a.batch; base += THREADS) scan(base, blockIdx.x == 0);
-  const int64_t total = carry;
-  const int workers = static_cast<int>(min(static_cast<int64_t>(gridDim.x) * WARPS, total));
   const int worker = warp * gridDim.x + blockIdx.x;  // few rounds: spread over the SMs
-  const bool busy = worker < workers;
-  const Kv4Split split(total, workers);
-  const int64_t r0 = busy ? split.start(worker) : 0, r1 = busy ? split.start(worker + 1) : 0;
+  const int run = (a.batch + 31) / 32, from = min(lane * run, a.batch), to = min(from + run, a.batch);
+  int64_t end = 0;  // rounds up to and with the lane's sequences
+  for (int b = from; b < to; ++b) end += static_cast<int64_t>(kv4_seq<BURST>(a, b, worker == 0).rounds) * subs;
+  int64_t begin = end;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int64_t y = __shfl_up_sync(0xffffffffu, end, o);
+    if (lane >= o) end += y;
+  }
+  begin = end - begin;
+  const int64_t total = __shfl_sync(0xffffffffu, end, 31);
+  const int workers = static_cast<int>(min(static_cast<int64_t>(gridDim.x) * WARPS, total));
+  if (worker >= workers) return;
+  int64_t r0;
+  int left;
+  {
+    Kv4Split mine;
+    mine.set(total, workers);
+    if (lane == 0) split = mine;  // the same from every warp
+    r0 = mine.start(worker);
+    left = static_cast<int>(mine.start(worker + 1) - r0);
+  }
   int seq = 0;
-  int64_t seq_first = 0;
-  if (a.batch > THREADS) carry = 0;
-  for (int base = 0; base < a.batch; base += THREADS) {
-    const int64_t before = a.batch > THREADS ? carry : 0;
-    if (a.batch > THREADS) scan(base, false);
-    for (int x = lane; x < THREADS && base + (x & ~31) < a.batch; x += 32) {
-      const int64_t end = scan_end[x], begin = x == 0 ? before : scan_end[x - 1];
-      const unsigned hit = __ballot_sync(0xffffffffu, begin <= r0 && r0 < end);
-      if (hit) {
-        const int at = __ffs(hit) - 1;
-        seq = base + (x & ~31) + at;
-        seq_first = __shfl_sync(0xffffffffu, begin, at);
-      }
+  Kv4Seq sq = {};
+  const bool mine = begin <= r0 && r0 < end;
+  if (mine) {
+    for (seq = from; seq < to; ++seq) {
+      sq = kv4_seq<BURST>(a, seq);
+      const int64_t n = static_cast<int64_t>(sq.rounds) * subs;
+      if (r0 < begin + n) break;
+      begin += n;
     }
   }
-  if (!busy) return;
-
-  Kv4Seq sq = kv4_seq(a, seq, false);
-  int sub = (r0 - seq_first) >> 31 ? static_cast<int>((r0 - seq_first) / sq.rounds)
-                                   : static_cast<int>(r0 - seq_first) / sq.rounds;
-  int ra = static_cast<int>(r0 - seq_first - static_cast<int64_t>(sub) * sq.rounds);
-  int left = static_cast<int>(r1 - r0);
-  int64_t item_first = r0 - ra;
-
+  const int owner = __ffs(__ballot_sync(0xffffffffu, mine)) - 1;
+  seq = __shfl_sync(0xffffffffu, seq, owner);
+  sq.ctx = __shfl_sync(0xffffffffu, sq.ctx, owner);
+  sq.first = __shfl_sync(0xffffffffu, sq.first, owner);
+  sq.last = __shfl_sync(0xffffffffu, sq.last, owner);
+  sq.rounds = __shfl_sync(0xffffffffu, sq.rounds, owner);
+  const int64_t in_seq = r0 - __shfl_sync(0xffffffffu, begin, owner);
+  int sub = in_seq >> 31 ? static_cast<int>(in_seq / sq.rounds) : static_cast<int>(in_seq) / sq.rounds;
+  int ra = static_cast<int>(in_seq - static_cast<int64_t>(sub) * sq.rounds);
   // ---- the worker's stream of records, STAGES bursts ahead of the arithmetic.  Up to 32 records of an item are
   // prepared at once, lane j seeing to record j: its block id is asked for a batch ahead, its copy is issued
   // by that lane when its turn comes.
   const int64_t block_bytes = static_cast<int64_t>(a.hkv) * a.recs * P::RECORD;
   int p_seq = seq, p_sub = sub, p_left = left - min(sq.rounds - ra, left);
   Kv4Seq p_sq = sq;
-  int p_t = sq.first + ra * a.per, p_end = min(sq.first + (ra + left - p_left) * a.per, sq.last);
+  const int2 p_first = kv4_records<BURST>(a, sq, ra, left - p_left);
+  int p_t = p_first.x, p_end = p_first.y;
   int ask_n = 0, ask_id = 0, ask_rec = 0, ask_sub = 0;  // the next batch: records, the lane's block and record in it
   auto ask = [&]() {
     ask_n = 0;
@@ -332,12 +330,13 @@ __global__ void __launch_bounds__(Kv4Cfg<D, RT>::WARPS * 32, 1) kv4_attn_kernel(
       if (p_left <= 0) return;
       if (++p_sub == subs) {
         p_sub = 0;
-        p_sq = kv4_seq(a, ++p_seq, false);
+        p_sq = kv4_seq<BURST>(a, ++p_seq);
       }
       const int n = min(p_sq.rounds, p_left);
       p_left -= n;
-      p_t = p_sq.first;
-      p_end = min(p_sq.first + n * a.per, p_sq.last);
+      const int2 recs = kv4_records<BURST>(a, p_sq, 0, n);
+      p_t = recs.x;
+      p_end = recs.y;
     }
     ask_n = min(p_end - p_t, 32);
     ask_sub = p_sub;
@@ -393,19 +392,28 @@ __global__ void __launch_bounds__(Kv4Cfg<D, RT>::WARPS * 32, 1) kv4_attn_kernel(
     const int h = a.chunks == 1 ? sub : sub / a.chunks;
     const int row0 = (sub - h * a.chunks) * ROWS;
     const int rows = min(a.group * a.T - row0, ROWS);
+    const int2 span = kv4_records<BURST>(a, sq, ra, n_rounds);
 
     // Q of the item, four rows at a time, eight lanes each: round(32512 q / max |q|) = 256 hi + lo, signed bytes
     __syncwarp();
-#pragma unroll 1
-    for (int pass = 0; pass < ROWS / 4; ++pass) {
-      const int r = pass * 4 + (lane >> 3), w = lane & 7;
+    auto load_rows = [&](int pass, uint4 (&raw)[NG]) {
+      const int r = pass * 4 + (lane >> 3);
       const int i = (row0 + r) / a.group, hq = h * a.group + (row0 + r) - i * a.group;
-      const __nv_bfloat16* src =
-          a.q + (static_cast<int64_t>(seq) * a.T + i) * a.q_stride + static_cast<int64_t>(hq) * D + 8 * w;
-      uint4 raw[NG];
+      const __nv_bfloat16* src = a.q + (static_cast<int64_t>(seq) * a.T + i) * a.q_stride +
+                                 static_cast<int64_t>(hq) * D + 8 * (lane & 7);
 #pragma unroll
       for (int k = 0; k < NG; ++k)
         raw[k] = r < rows ? *reinterpret_cast<const uint4*>(src + 64 * k) : make_uint4(0u, 0u, 0u, 0u);
+    };
+    uint4 next[NG];
+    load_rows(0, next);
+#pragma unroll 1
+    for (int pass = 0; pass < ROWS / 4 && span.x < span.y; ++pass) {
+      const int r = pass * 4 + (lane >> 3), w = lane & 7;
+      uint4 raw[NG];
+#pragma unroll
+      for (int k = 0; k < NG; ++k) raw[k] = next[k];
+      if (pass + 1 < ROWS / 4) load_rows(pass + 1, next);
       uint32_t big = 0;  // bits of the largest magnitude: ordered as integers, NaN and infinity on top
 #pragma unroll
       for (int k = 0; k < NG; ++k) {
@@ -679,11 +687,10 @@ __global__ void __launch_bounds__(Kv4Cfg<D, RT>::WARPS * 32, 1) kv4_attn_kernel(
       }
     };
 
-    const int t_end = min(sq.first + (ra + n_rounds) * a.per, sq.last);
     // bursts that start in [t_low, t_high] hold no token that some row does not see
     const int t_low = a.window > 0 ? max(see_most - a.window + kKv4Tokens - 1, 0) / kKv4Tokens : 0;
     const int t_high = max(see_least, 0) / kKv4Tokens - BURST;
-    for (int t = sq.first + ra * a.per; t < t_end && !dead; t += BURST) {
+    for (int t = span.x; t < span.y && !dead; t += BURST) {
       const unsigned have = came >> (cur * BURST) & ALL;
       if (have) {  // else no such blocks: their tokens count as masked
         const uint32_t parity = phase >> cur & 1u;
@@ -716,10 +723,10 @@ __global__ void __launch_bounds__(Kv4Cfg<D, RT>::WARPS * 32, 1) kv4_attn_kernel(
       }
     }
     const bool whole = ra == 0 && n_rounds == sq.rounds;
-    if (ra == 0 && lane == 0) {
+    if (ra == 0 && lane == 0 && a.items != nullptr) {  // nullptr: items are not split
       Kv4Item it;
       it.first = worker;
-      it.last = whole ? worker : split.worker(item_first + sq.rounds - 1);
+      it.last = whole ? worker : split.worker(split.start(worker + 1) - left + sq.rounds - 1);
       a.items[static_cast<int64_t>(seq) * subs + sub] = it;
     }
     const int64_t slot = 2 * static_cast<int64_t>(worker) + (ra == 0 ? 1 : 0);
@@ -753,11 +760,10 @@ __global__ void __launch_bounds__(Kv4Cfg<D, RT>::WARPS * 32, 1) kv4_attn_kernel(
       }
     }
     left -= n_rounds;
-    item_first += sq.rounds;
     ra = 0;
     if (++sub == subs && left > 0) {
       sub = 0;
-      sq = kv4_seq(a, ++seq, false);
+      sq = kv4_seq<BURST>(a, ++seq);
     }
   }
   // a stream that was given up: its copies land before the block's shared memory goes
@@ -766,11 +772,11 @@ __global__ void __launch_bounds__(Kv4Cfg<D, RT>::WARPS * 32, 1) kv4_attn_kernel(
       if (came >> (st * BURST) & ALL) mbar_wait(bars + st, phase >> st & 1u, nullptr, a.err);
 }
 
-// Adds parts p0, p0 + STEP, .. up to `last` of row r of an item to (m, l, o); eight of them under way at once.
-template <int D, int RT, int STEP>
+// Adds parts p0, p0 + STEP, .. up to the last of row r of an item to (m, l, o), AHEAD of them under way at once.
+template <int D, int RT, int STEP, int AHEAD>
 __device__ __forceinline__ void kv4_join_parts(const Kv4AttnArgs& a, const Kv4Item& it, int p0, int r, int lane, float& m,
                                                float& l, float (&o)[D / 32]) {
-  constexpr int ROWS = Kv4Rows<RT>::ROWS, N = D / 32, AHEAD = 8;
+  constexpr int ROWS = Kv4Rows<RT>::ROWS, N = D / 32;
   for (; p0 <= it.last; p0 += STEP * AHEAD) {
     float2 e[AHEAD];
     float y[AHEAD][N];
@@ -801,22 +807,24 @@ __device__ __forceinline__ void kv4_join_parts(const Kv4AttnArgs& a, const Kv4It
   }
 }
 
-// Joins the parts of the items that span workers.  A block takes `pairs` (item, row) pairs at a time, eight of them
-// or, where there are few, one: a pair of few parts is one warp's, in worker order; a pair of many is the whole
-// block's, every eighth part a warp.
-template <int D, int RT>
-__global__ void __launch_bounds__(kJoinThreads) kv4_join_kernel(const Kv4AttnArgs a, const int pairs) {
-  constexpr int ROWS = Kv4Rows<RT>::ROWS, N = D / 32, WARPS = kJoinThreads / 32, FEW = 16;
+// Joins the parts of the items that span workers.  A block of WARPS warps takes PAIRS (item, row) pairs, one per
+// warp: a pair of few parts is that warp's, in worker order; a pair of many is the whole block's, the warps
+// taking turns.
+constexpr int kFewParts = 16;
+template <int D, int RT, int PAIRS, int WARPS>
+__global__ void __launch_bounds__(32 * WARPS) kv4_join_kernel(const Kv4AttnArgs a) {
+  constexpr int ROWS = Kv4Rows<RT>::ROWS, N = D / 32;
+  constexpr int FEW = kFewParts, AHEAD = WARPS == 32 ? 512 / D : D == 256 ? 4 : 8;
   __shared__ float acc[WARPS][D];
   __shared__ float2 ml[WARPS];
   pdl_wait();
   pdl_launch_dependents();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, subs = a.hkv * a.chunks;
   const int64_t work = static_cast<int64_t>(a.batch) * subs * a.slab_rows;
-  for (int64_t x0 = static_cast<int64_t>(blockIdx.x) * pairs; x0 < work; x0 += static_cast<int64_t>(gridDim.x) * pairs) {
+  for (int64_t x0 = static_cast<int64_t>(blockIdx.x) * PAIRS; x0 < work; x0 += static_cast<int64_t>(gridDim.x) * PAIRS) {
     // lane j of every warp looks at pair x0 + j
     const int64_t x = x0 + lane;
-    const bool mine = lane < pairs && x < work;
+    const bool mine = lane < PAIRS && x < work;
     const int64_t item = x >> 31 ? x / a.slab_rows : static_cast<uint32_t>(x) / static_cast<uint32_t>(a.slab_rows);
     const int row = static_cast<int>(x - item * a.slab_rows);
     Kv4Item it = {0, 0};
@@ -826,18 +834,18 @@ __global__ void __launch_bounds__(kJoinThreads) kv4_join_kernel(const Kv4AttnArg
     const bool split = mine && it.first < it.last && at < a.group * a.T;
     const int64_t dst_at = (static_cast<int64_t>(seq) * a.T + at / a.group) * a.out_stride +
                            static_cast<int64_t>(h * a.group + at % a.group) * D;
-    const unsigned many = __ballot_sync(0xffffffffu, split && it.last - it.first >= FEW);
-    const unsigned few = __ballot_sync(0xffffffffu, split && it.last - it.first < FEW);
+    const bool shared = PAIRS == 1 || it.last - it.first >= FEW;
+    const unsigned many = __ballot_sync(0xffffffffu, split && shared), few = __ballot_sync(0xffffffffu, split && !shared);
     float m = kNone, l = 0.0f, o[N];
 #pragma unroll
     for (int j = 0; j < N; ++j) o[j] = 0.0f;
-    if (few >> warp & 1u) {
+    if (PAIRS > 1 && (few >> warp & 1u)) {
       Kv4Item one;
       one.first = __shfl_sync(0xffffffffu, it.first, warp);
       one.last = __shfl_sync(0xffffffffu, it.last, warp);
       const int r = __shfl_sync(0xffffffffu, row, warp);
       __nv_bfloat16* dst = a.out + __shfl_sync(0xffffffffu, dst_at, warp);
-      kv4_join_parts<D, RT, 1>(a, one, one.first, r, lane, m, l, o);
+      kv4_join_parts<D, RT, 1, AHEAD>(a, one, one.first, r, lane, m, l, o);
       const float inv = l == 0.0f ? 0.0f : 1.0f / l;
 #pragma unroll
       for (int j = 0; j < N; ++j) dst[32 * j + lane] = __float2bfloat16_rn(o[j] * inv);
@@ -852,7 +860,7 @@ __global__ void __launch_bounds__(kJoinThreads) kv4_join_kernel(const Kv4AttnArg
       m = kNone, l = 0.0f;
 #pragma unroll
       for (int j = 0; j < N; ++j) o[j] = 0.0f;
-      kv4_join_parts<D, RT, WARPS>(a, one, one.first + warp, r, lane, m, l, o);
+      kv4_join_parts<D, RT, WARPS, AHEAD>(a, one, one.first + warp, r, lane, m, l, o);
       __syncthreads();  // the pair before has been read
       if (lane == 0) ml[warp] = make_float2(m, l);
 #pragma unroll
@@ -861,7 +869,7 @@ __global__ void __launch_bounds__(kJoinThreads) kv4_join_kernel(const Kv4AttnArg
       float top = kNone;
 #pragma unroll
       for (int w = 0; w < WARPS; ++w) top = fmaxf(top, ml[w].x);
-      for (int ch = threadIdx.x; ch < D; ch += kJoinThreads) {
+      for (int ch = threadIdx.x; ch < D; ch += 32 * WARPS) {
         float sum = 0.0f, v = 0.0f;
 #pragma unroll
         for (int w = 0; w < WARPS; ++w) {
@@ -919,8 +927,11 @@ int kv4_launch_cap(const Kv4AttnArgs& a, int64_t grid, int64_t join_grid, int pa
                  dim3(Kv4Cfg<D, RT>::WARPS * 32), smem,
                  st, a));
   if (join_grid == 0) return MVB_OK;
-  return launch_dependent("kv4_attention_join", kv4_join_kernel<D, RT>, dim3(static_cast<unsigned>(join_grid)),
-                          dim3(kJoinThreads), 0, st, a, pairs);
+  const dim3 blocks(static_cast<unsigned>(join_grid));
+  const char* what = "kv4_attention_join";  // pairs: 8; 1; 0 = 1 and a block of 32 warps
+  if (pairs > 1) return launch_dependent(what, kv4_join_kernel<D, RT, 8, 8>, blocks, dim3(256), 0, st, a);
+  if (pairs == 0) return launch_dependent(what, kv4_join_kernel<D, RT, 1, 32>, blocks, dim3(1024), 0, st, a);
+  return launch_dependent(what, kv4_join_kernel<D, RT, 1, 8>, blocks, dim3(256), 0, st, a);
 }
 
 template <int D, int RT>
@@ -1013,28 +1024,32 @@ extern "C" int mvb_paged_attention_decode_kv4(void* out, int64_t out_stride, con
   const int64_t rows = num_q_heads / num_kv_heads * query_len;
   const Kv4Plan p = kv4_plan(sms, head_dim, rows, batch, num_kv_heads);
   MVB_REQUIRE(num_kv_heads * p.chunks <= INT_MAX, "%s: heads", what);
-  MVB_REQUIRE(workspace && aligned(workspace, 256) && workspace_bytes >= p.bytes,
-              "%s: a workspace of %lld bytes, 256-byte aligned (got %lld)", what, (long long)p.bytes,
-              (long long)workspace_bytes);
   const int64_t items = batch * num_kv_heads * p.chunks, most = max_blocks * recs;  // records of an item
   // Short tables: an item goes to one worker and nothing is left to join.
   const bool split = most > kShortRecords;
-  a.per = split ? p.burst : static_cast<int>(most);
+  MVB_REQUIRE(!split || (workspace && aligned(workspace, 256) && workspace_bytes >= p.bytes),
+              "%s: a workspace of %lld bytes, 256-byte aligned (got %lld)", what, (long long)p.bytes,
+              (long long)workspace_bytes);
+  a.split = split;
   int64_t grid = p.grid;
-  const int64_t most_rounds = split ? (most + p.burst - 1) / p.burst : 1;
+  const int64_t most_rounds = split ? kItemCost + (most + p.burst - 1) / p.burst : 1;
   if (items < grid && items * most_rounds < grid) grid = items * most_rounds;
   a.chunks = static_cast<int>(p.chunks);
   a.slab_rows = static_cast<int>(rows < p.rows ? rows : p.rows);
-  char* ws = static_cast<char*>(workspace);
-  a.items = reinterpret_cast<Kv4Item*>(ws + p.items_at);
-  a.part_ml = reinterpret_cast<float2*>(ws + p.ml_at);
-  a.part_o = reinterpret_cast<float*>(ws + p.o_at);
+  if (split) {
+    char* ws = static_cast<char*>(workspace);
+    a.items = reinterpret_cast<Kv4Item*>(ws + p.items_at);
+    a.part_ml = reinterpret_cast<float2*>(ws + p.ml_at);
+    a.part_o = reinterpret_cast<float*>(ws + p.o_at);
+  }
   int64_t join_grid = 0;
   const int64_t all_pairs = items * a.slab_rows;
-  const int pairs = all_pairs > 4LL * sms ? kJoinThreads / 32 : 1;
+  // a block per pair where there are few pairs, or where an item has many parts
+  int pairs = all_pairs <= 2LL * sms || items * kFewParts < p.grid * p.warps ? 1 : 8;
   if (split) {
     join_grid = (all_pairs + pairs - 1) / pairs;
-    if (join_grid > 8LL * sms) join_grid = 8LL * sms;
+    if (pairs == 1 && all_pairs <= 2LL * sms && items * 32 < p.grid * p.warps) pairs = 0;  // and 32 warps for very many
+    if (join_grid > 16LL * sms) join_grid = 16LL * sms;
   }
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   switch (head_dim) {

@@ -473,10 +473,20 @@ def _expect(what: str, name: str, t, index: int, dtype: torch.dtype, dims: int) 
         _refuse(what, name, t, index, dtype, dims)
 
 
+def _joint(what: str, index: int, *wanted) -> None:
+    """The detailed checks of ``(name, tensor, dtype, dims)`` one by one, for the caller whose joint test failed."""
+    for name, t, dtype, dims in wanted:
+        _expect(what, name, t, index, dtype, dims)
+
+
+_I32, _I64, _F32, _BF16, _U8 = torch.int32, torch.int64, torch.float32, torch.bfloat16, torch.uint8
+
+
 def _kv4_geometry(what: str, kv4: torch.Tensor, layer: int) -> tuple[int, int, int, int, int, int]:
     """(device, layers, blocks, KV heads, block size, head size) of a pool of ``kv_cache.kv4_pool``."""
     index = kv4.get_device() if isinstance(kv4, torch.Tensor) else -1
-    _expect(what, "kv4", kv4, index, torch.uint8, 5)
+    if index < 0 or kv4.dtype is not _U8 or kv4.dim() != 5:
+        _expect(what, "kv4", kv4, index, _U8, 5)
     L, P, nkv, recs, rec = kv4.shape
     if rec % 18 or not kv4.is_contiguous():
         raise RuntimeError(f"{what}: kv4 must be a contiguous pool of kv_cache.kv4_pool, not {tuple(kv4.shape)}")
@@ -504,12 +514,17 @@ def kv4_write(k: torch.Tensor, v: torch.Tensor, kv4: torch.Tensor, layer: int, s
     call must differ from one another."""
     what = "kv4_write"
     index, L, P, nkv, bs, D = _kv4_geometry(what, kv4, layer)
-    _expect(what, "k", k, index, torch.bfloat16, 3)
-    _expect(what, "v", v, index, torch.bfloat16, 3)
-    _expect(what, "slots", slots, index, torch.int64, 1)
+    try:
+        ok = (k.dtype is _BF16 and v.dtype is _BF16 and slots.dtype is _I64 and slots.dim() == 1
+              and k.get_device() == index and v.get_device() == index and slots.get_device() == index)
+    except AttributeError:
+        ok = False
+    if not ok:
+        _joint(what, index, ("k", k, _BF16, 3), ("v", v, _BF16, 3), ("slots", slots, _I64, 1))
     n = slots.shape[0]
-    if k.shape != (n, nkv, D) or v.shape != (n, nkv, D):
-        raise RuntimeError(f"{what}: k and v must be {(n, nkv, D)}, not {tuple(k.shape)} and {tuple(v.shape)}")
+    want = (n, nkv, D)
+    if k.shape != want or v.shape != want:
+        raise RuntimeError(f"{what}: k and v must be {want}, not {tuple(k.shape)} and {tuple(v.shape)}")
     if n == 0:
         return
     k, v, slots = _kv4_rows(k), _kv4_rows(v), slots.contiguous()
@@ -535,6 +550,9 @@ def kv4_read(kv4: torch.Tensor, layer: int, slots: torch.Tensor) -> tuple[torch.
     return k, v
 
 
+_KV4_UNSPLIT_TOKENS = 128  # tables of at most this many tokens need no workspace: their cache is never split
+
+
 @functools.lru_cache(maxsize=1024)
 def _kv4_workspace_bytes(B: int, T: int, Hq: int, nkv: int, D: int, index: int) -> int:
     return N.lib().mvb_paged_attention_decode_kv4_workspace_bytes(B, T, Hq, nkv, D, index)
@@ -549,7 +567,7 @@ def paged_attention_decode_kv4(q: torch.Tensor, kv4: torch.Tensor, layer: int, b
     query tokens among them: query i sees the first ``ctx_lens[b] - T + 1 + i`` keys, with ``window`` > 0
     the newest ``window`` of those.  A query without a key gives zeros.  Returns the shape of q.
     ``workspace``: uint8 of ``mvb_paged_attention_decode_kv4_workspace_bytes`` (any content, not shared by
-    calls that overlap); by default each call takes its own from torch's allocator."""
+    calls that overlap); by default each call takes its own from torch's allocator, where it needs one."""
     what = "paged_attention_decode_kv4"
     index, L, P, nkv, bs, D = _kv4_geometry(what, kv4, layer)
     dims = q.dim() if isinstance(q, torch.Tensor) else 0
@@ -560,16 +578,22 @@ def paged_attention_decode_kv4(q: torch.Tensor, kv4: torch.Tensor, layer: int, b
         T = 1
     else:
         raise RuntimeError(f"{what}: q must be [B, Hq, D] or [B, T, Hq, D]")
-    _expect(what, "q", q, index, torch.bfloat16, dims)
-    _expect(what, "block_tables", block_tables, index, torch.int32, 2)
-    _expect(what, "ctx_lens", ctx_lens, index, torch.int32, 1)
+    try:
+        ok = (q.dtype is _BF16 and block_tables.dtype is _I32 and ctx_lens.dtype is _I32 and q.get_device() == index
+              and block_tables.get_device() == index and ctx_lens.get_device() == index and block_tables.dim() == 2
+              and ctx_lens.dim() == 1)
+    except AttributeError:
+        ok = False
+    if not ok:
+        _joint(what, index, ("q", q, _BF16, dims), ("block_tables", block_tables, _I32, 2),
+               ("ctx_lens", ctx_lens, _I32, 1))
     if qd != D or Hq % nkv or not Hq:
         raise RuntimeError(f"{what}: q {tuple(q.shape)} over {nkv} KV heads of {D}")
     rows, width = block_tables.shape
     if rows != B or ctx_lens.shape[0] != B:
         raise RuntimeError(f"{what}: {B} sequences, {rows} block tables, {ctx_lens.shape[0]} lengths")
     if out is None:
-        out = torch.empty(q.shape, dtype=torch.bfloat16, device=q.device)
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
     else:
         _expect(what, "out", out, index, torch.bfloat16, dims)
         if out.shape != q.shape or not out.is_contiguous() or out.data_ptr() % 16:
@@ -592,15 +616,20 @@ def paged_attention_decode_kv4(q: torch.Tensor, kv4: torch.Tensor, layer: int, b
         if block_tables.stride(1) != 1 or t_stride < width:
             block_tables, t_stride = block_tables.contiguous(), width
     ctx_lens = ctx_lens.contiguous()
+    ws_at, ws_bytes = None, 0
     if workspace is None:
-        workspace = torch.empty(_kv4_workspace_bytes(B, T, Hq, nkv, D, index), dtype=torch.uint8, device=q.device)
+        if width * bs > _KV4_UNSPLIT_TOKENS:
+            ws_bytes = _kv4_workspace_bytes(B, T, Hq, nkv, D, index)
+            workspace = torch.empty(ws_bytes, dtype=_U8, device=q.device)
+            ws_at = workspace.data_ptr()
     else:
         _expect(what, "workspace", workspace, index, torch.uint8, 1)
         if not workspace.is_contiguous():
             raise RuntimeError(f"{what}: workspace must be contiguous")
+        ws_at, ws_bytes = workspace.data_ptr(), workspace.numel()
     N.on_device(index, what, N.lib().mvb_paged_attention_decode_kv4, out.data_ptr(), Hq * D, q.data_ptr(), q_stride,
                 kv4.data_ptr(), block_tables.data_ptr(), t_stride, width, ctx_lens.data_ptr(), B, T, Hq, nkv, D, L,
-                int(layer), P, bs, float(scale), float(softcap), int(window), workspace.data_ptr(), workspace.numel())
+                int(layer), P, bs, float(scale), float(softcap), int(window), ws_at, ws_bytes)
     return out
 
 
@@ -626,10 +655,16 @@ def assign_slots(block_tables: torch.Tensor, ctx_lens: torch.Tensor, new_lens: t
     fit (its table row, the free list, ``num_tokens``) takes nothing: ``granted`` 0 and slots -1."""
     what = "assign_slots"
     index = block_tables.get_device() if isinstance(block_tables, torch.Tensor) else -1
-    _expect(what, "block_tables", block_tables, index, torch.int32, 2)
-    _expect(what, "ctx_lens", ctx_lens, index, torch.int32, 1)
-    _expect(what, "new_lens", new_lens, index, torch.int32, 1)
-    _expect(what, "free_blocks", free_blocks, index, torch.int32, 1)
+    try:
+        ok = (index >= 0 and block_tables.dtype is _I32 and ctx_lens.dtype is _I32 and new_lens.dtype is _I32
+              and free_blocks.dtype is _I32 and ctx_lens.get_device() == index and new_lens.get_device() == index
+              and free_blocks.get_device() == index and block_tables.dim() == 2 and ctx_lens.dim() == 1
+              and new_lens.dim() == 1 and free_blocks.dim() == 1)
+    except AttributeError:
+        ok = False
+    if not ok:
+        _joint(what, index, ("block_tables", block_tables, _I32, 2), ("ctx_lens", ctx_lens, _I32, 1),
+               ("new_lens", new_lens, _I32, 1), ("free_blocks", free_blocks, _I32, 1))
     B, width = block_tables.shape
     if ctx_lens.shape[0] != B or new_lens.shape[0] != B:
         raise RuntimeError(f"{what}: {B} block tables, {ctx_lens.shape[0]} and {new_lens.shape[0]} lengths")
@@ -645,15 +680,16 @@ def assign_slots(block_tables: torch.Tensor, ctx_lens: torch.Tensor, new_lens: t
     if num_tokens < 0:
         raise RuntimeError(f"{what}: num_tokens {num_tokens}")
     ctx_lens, new_lens, free_blocks = ctx_lens.contiguous(), new_lens.contiguous(), free_blocks.contiguous()
-    dev = block_tables.device
-    slots = torch.empty(num_tokens, dtype=torch.int64, device=dev)
-    positions = torch.empty(num_tokens, dtype=torch.int32, device=dev)
-    seq_start, granted, head = torch.empty(2 * B + 2, dtype=torch.int32, device=dev).split((B + 1, B, 1))
-    start_at = seq_start.data_ptr()
-    N.on_device(index, what, N.lib().mvb_assign_slots, slots.data_ptr(), positions.data_ptr(), start_at,
-                start_at + 4 * (B + 1), start_at + 4 * (2 * B + 1), block_tables.data_ptr(), t_stride, width,
-                ctx_lens.data_ptr(), new_lens.data_ptr(), free_blocks.data_ptr(), free_blocks.shape[0],
-                N.ptr(free_head), B, int(block_size), int(num_tokens))
+    # one allocation: slots (two words each), positions, starts, granted, the head
+    words = torch.empty(3 * num_tokens + 2 * B + 2, dtype=_I32, device=block_tables.device)
+    at = words.data_ptr()
+    slots, positions, seq_start, granted, head = words.split_with_sizes((2 * num_tokens, num_tokens, B + 1, B, 1))
+    start = at + 12 * num_tokens
+    N.on_device(index, what, N.lib().mvb_assign_slots, at, at + 8 * num_tokens, start, start + 4 * (B + 1),
+                start + 4 * (2 * B + 1), block_tables.data_ptr(), t_stride, width, ctx_lens.data_ptr(),
+                new_lens.data_ptr(), free_blocks.data_ptr(), free_blocks.shape[0], N.ptr(free_head), B,
+                int(block_size), int(num_tokens))
+    slots = slots.view(_I64)
     return SlotPlan(slots, positions, seq_start, granted, head)
 
 
@@ -685,9 +721,14 @@ def verify_drafts(target_probs: torch.Tensor, draft_tokens: torch.Tensor, unifor
     int64 [B, K + 1], accepted int32 [B])``: accepted drafts, the drawn token, then -1."""
     what = "verify_drafts"
     index = target_probs.get_device() if isinstance(target_probs, torch.Tensor) else -1
-    _expect(what, "target_probs", target_probs, index, torch.float32, 3)
-    _expect(what, "draft_tokens", draft_tokens, index, torch.int64, 2)
-    _expect(what, "uniforms", uniforms, index, torch.float32, 2)
+    try:
+        ok = (index >= 0 and target_probs.dtype is _F32 and draft_tokens.dtype is _I64 and uniforms.dtype is _F32
+              and target_probs.dim() == 3 and draft_tokens.get_device() == index and uniforms.get_device() == index)
+    except AttributeError:
+        ok = False
+    if not ok:
+        _joint(what, index, ("target_probs", target_probs, _F32, 3), ("draft_tokens", draft_tokens, _I64, 2),
+               ("uniforms", uniforms, _F32, 2))
     B, rows, V = target_probs.shape
     K = rows - 1
     if K < 0 or V == 0 or draft_tokens.shape != (B, K) or uniforms.shape != (B, rows):
