@@ -42,7 +42,7 @@ namespace {
 
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr int kShortRecords = 8;  // items of at most this many records are never split
-constexpr int kItemCost = 2;      // what beginning an item costs a warp, in bursts, for the division of the work
+constexpr int kItemCost = 3;      // what beginning an item costs a warp, in bursts, for the division of the work
 
 // A weight is 2^(score - reference): the reference is a row's maximum when last raised, and is raised
 // once a score passes it by more than kSlack (in powers of two), so that most records cost one vote instead
@@ -72,7 +72,7 @@ template <int D, int RT>
 struct Kv4Cfg {
   static constexpr int BURST = D == 256 || RT > 1 ? 1 : D == 128 ? 2 : RT == 0 ? 4 : 2;
   static constexpr int STAGES = D == 256 ? (RT > 1 ? 2 : 3) : D == 128 ? (RT > 1 ? 4 : 2) : RT == 0 ? 2 : 4;
-  static constexpr int WARPS = D == 256 ? (RT == 0 ? 12 : 8) : RT > 1 ? 8 : 16;
+  static constexpr int WARPS = (D == 256 && RT > 0) || (D == 128 && RT > 1) || RT > 2 ? 8 : 12;
 };
 
 struct Kv4AttnArgs {

@@ -521,7 +521,7 @@ def kv4_write(k: torch.Tensor, v: torch.Tensor, kv4: torch.Tensor, layer: int, s
         ok = False
     if not ok:
         _joint(what, index, ("k", k, _BF16, 3), ("v", v, _BF16, 3), ("slots", slots, _I64, 1))
-    n = slots.shape[0]
+    n = slots.numel()
     want = (n, nkv, D)
     if k.shape != want or v.shape != want:
         raise RuntimeError(f"{what}: k and v must be {want}, not {tuple(k.shape)} and {tuple(v.shape)}")
@@ -540,7 +540,7 @@ def kv4_read(kv4: torch.Tensor, layer: int, slots: torch.Tensor) -> tuple[torch.
     what = "kv4_read"
     index, L, P, nkv, bs, D = _kv4_geometry(what, kv4, layer)
     _expect(what, "slots", slots, index, torch.int64, 1)
-    n = slots.shape[0]
+    n = slots.numel()
     slots = slots.contiguous()
     k = torch.empty(n, nkv, D, dtype=torch.bfloat16, device=kv4.device)
     v = torch.empty_like(k)
@@ -590,8 +590,8 @@ def paged_attention_decode_kv4(q: torch.Tensor, kv4: torch.Tensor, layer: int, b
     if qd != D or Hq % nkv or not Hq:
         raise RuntimeError(f"{what}: q {tuple(q.shape)} over {nkv} KV heads of {D}")
     rows, width = block_tables.shape
-    if rows != B or ctx_lens.shape[0] != B:
-        raise RuntimeError(f"{what}: {B} sequences, {rows} block tables, {ctx_lens.shape[0]} lengths")
+    if rows != B or ctx_lens.numel() != B:
+        raise RuntimeError(f"{what}: {B} sequences, {rows} block tables, {ctx_lens.numel()} lengths")
     if out is None:
         out = torch.empty_like(q, memory_format=torch.contiguous_format)
     else:
@@ -666,8 +666,8 @@ def assign_slots(block_tables: torch.Tensor, ctx_lens: torch.Tensor, new_lens: t
         _joint(what, index, ("block_tables", block_tables, _I32, 2), ("ctx_lens", ctx_lens, _I32, 1),
                ("new_lens", new_lens, _I32, 1), ("free_blocks", free_blocks, _I32, 1))
     B, width = block_tables.shape
-    if ctx_lens.shape[0] != B or new_lens.shape[0] != B:
-        raise RuntimeError(f"{what}: {B} block tables, {ctx_lens.shape[0]} and {new_lens.shape[0]} lengths")
+    if ctx_lens.numel() != B or new_lens.numel() != B:
+        raise RuntimeError(f"{what}: {B} block tables, {ctx_lens.numel()} and {new_lens.numel()} lengths")
     t_stride = width
     if not block_tables.is_contiguous():
         t_stride = block_tables.stride(0) if B > 1 else width
@@ -687,7 +687,7 @@ def assign_slots(block_tables: torch.Tensor, ctx_lens: torch.Tensor, new_lens: t
     start = at + 12 * num_tokens
     N.on_device(index, what, N.lib().mvb_assign_slots, at, at + 8 * num_tokens, start, start + 4 * (B + 1),
                 start + 4 * (2 * B + 1), block_tables.data_ptr(), t_stride, width, ctx_lens.data_ptr(),
-                new_lens.data_ptr(), free_blocks.data_ptr(), free_blocks.shape[0], N.ptr(free_head), B,
+                new_lens.data_ptr(), free_blocks.data_ptr(), free_blocks.numel(), N.ptr(free_head), B,
                 int(block_size), int(num_tokens))
     slots = slots.view(_I64)
     return SlotPlan(slots, positions, seq_start, granted, head)
