@@ -62,6 +62,9 @@ struct Kv4Rows {
   static constexpr int KT = RT == 0 ? 1 : 2 * RT;   // of the first
   static constexpr int NC = RT == 0 ? 1 : 2 * RT;   // rows per lane
   static constexpr int ROWS = RT == 0 ? 4 : 8 * RT;
+  // With two or three row tiles a second integer plane costs more (its sums put together per score) than the
+  // two operations a word that fp16 operands cost: see above.
+  static constexpr bool HALF_K = RT > 1;
 };
 
 // BURST: records that a warp takes at once (one wait, one vote, one refill); STAGES of them are held, so that
@@ -156,6 +159,13 @@ __device__ __forceinline__ void mma_u8s8_16832_from(int (&d)[4], uint32_t a0, ui
       "{%10, %10, %10, %10};"
       : "=r"(d[0]), "=r"(d[1]), "=r"(d[2]), "=r"(d[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "r"(init));
+}
+__device__ __forceinline__ void mma_f16_16816_zero(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                                                   uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+      "{%10, %10, %10, %10};"
+      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.0f));
 }
 __device__ __forceinline__ uint32_t transposed(uint32_t x) {  // movmatrix_trans, free to be scheduled
   uint32_t d;
@@ -424,31 +434,58 @@ __global__ void __launch_bounds__(Kv4Cfg<D, RT>::WARPS * 32, 1) kv4_attn_kernel(
 #pragma unroll
       for (int o = 1; o < 8; o <<= 1) big = max(big, __shfl_xor_sync(0xffffffffu, big, o));
       const bool fine = big < 0x7f800000u;
-      const float up = big > 0 && fine ? fminf(32512.0f / __uint_as_float(big), 1e38f) : 0.0f;
-      const int n0 = RT == 0 ? 2 * r : r % 8, t0 = RT == 0 ? 0 : 2 * (r / 8);
-      const int n1 = RT == 0 ? 2 * r + 1 : r % 8, t1 = RT == 0 ? 0 : t0 + 1;
+      if constexpr (R::HALF_K) {
+        // times a power of two that puts the largest magnitude into [2^10, 2^11): exact in fp16 but for what lies
+        // 2^-25 below that
+        const int e = big > 0 && fine ? min(max(137 - static_cast<int>(big >> 23), -126), 126) : 0;
+        const float up = __uint_as_float(static_cast<uint32_t>(e + 127) << 23);
 #pragma unroll
-      for (int k = 0; k < NG; ++k) {
-        const uint32_t x[4] = {raw[k].x, raw[k].y, raw[k].z, raw[k].w};
-        // word w of the group is word w % 2 of lane w / 2; its even codes are the first operand, the odd ones the second
-        uint32_t hi[2] = {0, 0}, lo[2] = {0, 0};
-        int sum = 0;
+        for (int k = 0; k < NG; ++k) {
+          const uint32_t x[4] = {raw[k].x, raw[k].y, raw[k].z, raw[k].w};
+          float v[8], sum = 0.0f;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          const float xv = __uint_as_float((j & 1) ? x[j >> 1] & 0xffff0000u : x[j >> 1] << 16);
-          const int v = fine ? __float2int_rn(xv * up) : 0, vh = (v + 128) >> 8;
-          sum += v;
-          hi[j & 1] |= (static_cast<uint32_t>(vh) & 255u) << (8 * (j >> 1));
-          lo[j & 1] |= (static_cast<uint32_t>(v) & 255u) << (8 * (j >> 1));  // v - 256 vh in its low byte
+          for (int j = 0; j < 8; ++j) {
+            v[j] = fine ? __uint_as_float((j & 1) ? x[j >> 1] & 0xffff0000u : x[j >> 1] << 16) * up : 0.0f;
+            sum += v[j];
+          }
+          // word w of the group is word w % 2 of lane w / 2; codes 2 h and 2 h + 4 are the first operand of half h,
+          // 2 h + 1 and 2 h + 5 the second, which stands 4 bits higher
+#pragma unroll
+          for (int hh = 0; hh < 2; ++hh)
+            qf[(((k * 2 + (w & 1)) * 2 + hh) * NT + r / 8) * 32 + (r % 8) * 4 + (w >> 1)] =
+                make_uint2(pack_f16(v[2 * hh] * 16.0f, v[2 * hh + 4] * 16.0f), pack_f16(v[2 * hh + 1], v[2 * hh + 5]));
+#pragma unroll
+          for (int o = 1; o < 8; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+          if (w == 0) col_q[r * NG + k] = sum * 0x1p-20f;
         }
-        const int ks = k * 2 + (w & 1);
-        qf[(ks * KT + t0) * 32 + n0 * 4 + (w >> 1)] = make_uint2(hi[0], hi[1]);
-        qf[(ks * KT + t1) * 32 + n1 * 4 + (w >> 1)] = make_uint2(lo[0], lo[1]);
+        if (w == 0) col_f[r] = !fine ? __int_as_float(0x7fc00000) : ldexpf(a.score_scale, 20 - e);
+      } else {
+        const float up = big > 0 && fine ? fminf(32512.0f / __uint_as_float(big), 1e38f) : 0.0f;
+        const int n0 = RT == 0 ? 2 * r : r % 8, t0 = RT == 0 ? 0 : 2 * (r / 8);
+        const int n1 = RT == 0 ? 2 * r + 1 : r % 8, t1 = RT == 0 ? 0 : t0 + 1;
 #pragma unroll
-        for (int o = 1; o < 8; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-        if (w == 0) col_q[r * NG + k] = static_cast<float>(sum);
+        for (int k = 0; k < NG; ++k) {
+          const uint32_t x[4] = {raw[k].x, raw[k].y, raw[k].z, raw[k].w};
+          // word w of the group is word w % 2 of lane w / 2; its even codes are the first operand, the odd ones the second
+          uint32_t hi[2] = {0, 0}, lo[2] = {0, 0};
+          int sum = 0;
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            const float xv = __uint_as_float((j & 1) ? x[j >> 1] & 0xffff0000u : x[j >> 1] << 16);
+            const int v = fine ? __float2int_rn(xv * up) : 0, vh = (v + 128) >> 8;
+            sum += v;
+            hi[j & 1] |= (static_cast<uint32_t>(vh) & 255u) << (8 * (j >> 1));
+            lo[j & 1] |= (static_cast<uint32_t>(v) & 255u) << (8 * (j >> 1));  // v - 256 vh in its low byte
+          }
+          const int ks = k * 2 + (w & 1);
+          qf[(ks * KT + t0) * 32 + n0 * 4 + (w >> 1)] = make_uint2(hi[0], hi[1]);
+          qf[(ks * KT + t1) * 32 + n1 * 4 + (w >> 1)] = make_uint2(lo[0], lo[1]);
+#pragma unroll
+          for (int o = 1; o < 8; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+          if (w == 0) col_q[r * NG + k] = static_cast<float>(sum);
+        }
+        if (w == 0) col_f[r] = !fine ? __int_as_float(0x7fc00000) : up > 0.0f ? a.score_scale / up : 0.0f;
       }
-      if (w == 0) col_f[r] = !fine ? __int_as_float(0x7fc00000) : up > 0.0f ? a.score_scale / up : 0.0f;
     }
     __syncwarp();
 
@@ -500,31 +537,59 @@ __global__ void __launch_bounds__(Kv4Cfg<D, RT>::WARPS * 32, 1) kv4_attn_kernel(
         }
 #pragma unroll
         for (int k = 0; k < NG; ++k) {
-          int acc[KT][4];
+          if constexpr (R::HALF_K) {
+            float acc[NT][4];
 #pragma unroll
-          for (int wi = 0; wi < 2; ++wi) {
-            const uint32_t w0 = kw[0][NG * wi + k], w1 = kw[1][NG * wi + k];
-            const uint32_t a0 = w0 & 0x0F0F0F0Fu, a1 = w1 & 0x0F0F0F0Fu, a2 = (w0 >> 4) & 0x0F0F0F0Fu,
-                           a3 = (w1 >> 4) & 0x0F0F0F0Fu;
+            for (int wi = 0; wi < 2; ++wi)
 #pragma unroll
-            for (int nt = 0; nt < KT; ++nt) {
-              const uint2 b = qf[((k * 2 + wi) * KT + nt) * 32 + lane];
-              if (wi == 0)
-                mma_u8s8_16832_from(acc[nt], a0, a1, a2, a3, b.x, b.y, kMagicBits);
-              else
-                mma_u8s8_16832(acc[nt], a0, a1, a2, a3, b.x, b.y);
+              for (int hh = 0; hh < 2; ++hh) {
+                const uint32_t x0 = kw[0][NG * wi + k] >> (8 * hh), x1 = kw[1][NG * wi + k] >> (8 * hh);
+                const uint32_t a0 = x0 & 0x000F000Fu, a1 = x1 & 0x000F000Fu, a2 = x0 & 0x00F000F0u,
+                               a3 = x1 & 0x00F000F0u;
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) {
+                  const uint2 b = qf[(((k * 2 + wi) * 2 + hh) * NT + nt) * 32 + lane];
+                  if (wi + hh == 0)
+                    mma_f16_16816_zero(acc[nt], a0, a1, a2, a3, b.x, b.y);
+                  else
+                    mma_f16_16816(acc[nt], a0, a1, a2, a3, b.x, b.y);
+                }
+              }
+#pragma unroll
+            for (int e = 0; e < 2; ++e)
+#pragma unroll
+              for (int q = 0; q < NC; ++q) {
+                const float part = fmaf(pair_scale(kp[e][k]), acc[(q >> 1) % NT][2 * e + (q & 1)], k == 0 ? 0.0f : s[u][e][q]);
+                s[u][e][q] = fmaf(pair_min(kp[e][k]), qs[q][k], part);
+              }
+          } else {
+            int acc[KT][4];
+#pragma unroll
+            for (int wi = 0; wi < 2; ++wi) {
+              const uint32_t w0 = kw[0][NG * wi + k], w1 = kw[1][NG * wi + k];
+              const uint32_t a0 = w0 & 0x0F0F0F0Fu, a1 = w1 & 0x0F0F0F0Fu, a2 = (w0 >> 4) & 0x0F0F0F0Fu,
+                             a3 = (w1 >> 4) & 0x0F0F0F0Fu;
+#pragma unroll
+              for (int nt = 0; nt < KT; ++nt) {
+                const uint2 b = qf[((k * 2 + wi) * KT + nt) * 32 + lane];
+                if (wi == 0)
+                  mma_u8s8_16832_from(acc[nt], a0, a1, a2, a3, b.x, b.y, kMagicBits);
+                else
+                  mma_u8s8_16832(acc[nt], a0, a1, a2, a3, b.x, b.y);
+              }
             }
+#pragma unroll
+            for (int e = 0; e < 2; ++e)
+#pragma unroll
+              for (int q = 0; q < NC; ++q) {
+                const int hi = RT == 0 ? acc[0][2 * e] : acc[(q >> 1) * 2 % KT][2 * e + (q & 1)];
+                const int lo = RT == 0 ? acc[0][2 * e + 1] : acc[((q >> 1) * 2 + 1) % KT][2 * e + (q & 1)];
+                const float dot = fmaf(__int_as_float(hi) - kMagic, 256.0f, __int_as_float(lo) - kMagic);
+                const float part = fmaf(pair_scale(kp[e][k]), dot, k == 0 ? 0.0f : s[u][e][q]);
+                s[u][e][q] = fmaf(pair_min(kp[e][k]), qs[q][k], part);
+              }
+        
           }
-#pragma unroll
-          for (int e = 0; e < 2; ++e)
-#pragma unroll
-            for (int q = 0; q < NC; ++q) {
-              const int hi = RT == 0 ? acc[0][2 * e] : acc[(q >> 1) * 2 % KT][2 * e + (q & 1)];
-              const int lo = RT == 0 ? acc[0][2 * e + 1] : acc[((q >> 1) * 2 + 1) % KT][2 * e + (q & 1)];
-              const float dot = fmaf(__int_as_float(hi) - kMagic, 256.0f, __int_as_float(lo) - kMagic);
-              const float part = fmaf(pair_scale(kp[e][k]), dot, k == 0 ? 0.0f : s[u][e][q]);
-              s[u][e][q] = fmaf(pair_min(kp[e][k]), qs[q][k], part);
-            }
         }
         if constexpr (CAP)
 #pragma unroll
