@@ -502,12 +502,15 @@ __global__ void __launch_bounds__(Kv4Cfg<D, RT>::WARPS * 32, 1) kv4_attn_kernel(
     const int see_least = sq.ctx - a.T + 1 + row0 / a.group;
     const int see_most = sq.ctx - a.T + 1 + (row0 + rows - 1) / a.group;
 
-    float o[4 * NG][NT][4];  // m tiles: (group, high half of the word, half of that), 16 channels each
+    // m tiles of 16 x 8 outputs.  RT > 0: (group, high half of the word, half of that), 16 channels x 8 rows each;
+    // RT = 0: (group, half of a half word), 32 channels x 4 rows
+    constexpr int OT = (RT == 0 ? 2 : 4) * NG;
+    float o[OT][NT][4];
     float l[NC], mref[NC], mo[NC][NG];
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-      for (int k = 0; k < 4 * NG; ++k)
+      for (int k = 0; k < OT; ++k)
 #pragma unroll
         for (int e = 0; e < 4; ++e) o[k][nt][e] = 0.0f;
 #pragma unroll
@@ -684,7 +687,7 @@ __global__ void __launch_bounds__(Kv4Cfg<D, RT>::WARPS * 32, 1) kv4_attn_kernel(
         }
         if (!empty)
 #pragma unroll
-          for (int k = 0; k < 4 * NG; ++k)
+          for (int k = 0; k < OT; ++k)
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -732,7 +735,23 @@ __global__ void __launch_bounds__(Kv4Cfg<D, RT>::WARPS * 32, 1) kv4_attn_kernel(
             }
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt)
-              b[nt][e] = transposed(RT == 0 ? pack_f16(w[0], 0.0f) : pack_f16(w[2 * nt % NC], w[(2 * nt + 1) % NC]));
+              b[nt][e] = transposed(RT == 0 ? pack_f16(w[0], w[0]) : pack_f16(w[2 * nt % NC], w[(2 * nt + 1) % NC]));
+          }
+          if constexpr (RT == 0) {
+            // Both halves of a masked word are operands of one token: channel j in its low half, j + 4 in its high one.
+            // Column 2 r takes the weight of row r against the low halves, column 2 r + 1 against the high ones.
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {  // tokens vtok[2 e], vtok[2 e + 1]
+              const uint32_t b0 = __byte_perm(b[0][e], 0, g & 1 ? 0x1044 : 0x4410);
+              const uint32_t b1 = __byte_perm(b[0][e], 0, g & 1 ? 0x3244 : 0x4432);
+#pragma unroll
+              for (int hh = 0; hh < 2; ++hh) {
+                const uint32_t x0 = vw[2 * e][k] >> (8 * hh), x1 = vw[2 * e + 1][k] >> (8 * hh);
+                mma_f16_16816(o[(k * 2 + hh) % OT][0], x0 & 0x000F000Fu, x0 & 0x00F000F0u, x1 & 0x000F000Fu,
+                              x1 & 0x00F000F0u, b0, b1);
+              }
+            }
+            continue;
           }
 #pragma unroll
           for (int hv = 0; hv < 2; ++hv) {
@@ -745,7 +764,7 @@ __global__ void __launch_bounds__(Kv4Cfg<D, RT>::WARPS * 32, 1) kv4_attn_kernel(
                              a3 = x1 & 0x00F000F0u;
 #pragma unroll
               for (int nt = 0; nt < NT; ++nt)
-                mma_f16_16816(o[(k * 2 + hv) * 2 + hh][nt], a0, a1, a2, a3, b[nt][0], b[nt][1]);
+                mma_f16_16816(o[((k * 2 + hv) * 2 + hh) % OT][nt], a0, a1, a2, a3, b[nt][0], b[nt][1]);
             }
           }
         }
@@ -811,8 +830,10 @@ __global__ void __launch_bounds__(Kv4Cfg<D, RT>::WARPS * 32, 1) kv4_attn_kernel(
         float v[8];  // channels 8 g + 4 hv + 2 hh (codes as u 2^-24) and the next one (u 2^-20)
 #pragma unroll
         for (int x = 0; x < 4; ++x) {
-          v[2 * x] = fmaf(o[k * 4 + x][nt][j] * 0x1p24f, inv, mo[q][k]);
-          v[2 * x + 1] = fmaf(o[k * 4 + x][nt][j + 2] * 0x1p20f, inv, mo[q][k]);
+          const float(&y)[4] = RT == 0 ? o[(k * 2 + x % 2) % OT][0] : o[(k * 4 + x) % OT][nt];
+          const int at = RT == 0 ? x / 2 : j;
+          v[2 * x] = fmaf(y[at] * 0x1p24f, inv, mo[q][k]);
+          v[2 * x + 1] = fmaf(y[at + 2] * 0x1p20f, inv, mo[q][k]);
         }
         if (whole) {
           *reinterpret_cast<uint4*>(dst + 64 * k) =
