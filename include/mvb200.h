@@ -253,8 +253,8 @@ int mvb_paged_attention_decode_noalloc(void* out, int64_t out_stride, const void
  * quantised into slot slots[i] = block * block_size + offset: min = bf16(min x),
  * scale = bf16((max x - min) / 15), u = round-to-even((x - min) / scale).  A group with a NaN or an
  * infinity reads back as NaN.  A negative slot is skipped; one past the pool too, with
- * MVB_DEV_BAD_BLOCK.  Slots of one call are distinct (of a slot given twice, either token's
- * values may be kept, per group).
+ * MVB_DEV_BAD_BLOCK.  The slots of one call must differ: what a
+ * slot given twice holds afterwards is undefined (the others are not affected).
  * mvb_kv4_read: k, v [tokens, Hkv, D] bf16 (contiguous) of the slots; zeros where a slot is
  * negative or past the pool (MVB_DEV_BAD_BLOCK). */
 int mvb_kv4_write(void* kv4, const void* k, int64_t k_stride, int64_t k_head_stride, const void* v, int64_t v_stride,
@@ -273,7 +273,7 @@ int mvb_kv4_read(void* k, void* v, const void* kv4, const int64_t* slots, int64_
  * q_stride / out_stride elements (multiples of 8, 16-byte aligned).  block_tables: row b at
  * b * table_stride, max_blocks entries of it are used.  A context past its table is cut
  * (MVB_DEV_BAD_POSITION); a block outside the pool counts as masked (MVB_DEV_BAD_BLOCK).
- * Scores and softmax statistics in fp32, deterministic.  workspace: at least ..._workspace_bytes()
+ * batch <= 65536, query_len <= 1024, Hq <= 4096.  Scores and softmax statistics in fp32, deterministic.  workspace: at least ..._workspace_bytes()
  * bytes, 256-byte aligned, of any content; calls that overlap on the GPU need one each.  Tables of at most
  * 128 tokens (max_blocks * block_size) need none (NULL). */
 int64_t mvb_paged_attention_decode_kv4_workspace_bytes(int64_t batch, int64_t query_len, int64_t num_q_heads,

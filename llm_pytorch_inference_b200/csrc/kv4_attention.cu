@@ -371,7 +371,7 @@ __global__ void __launch_bounds__(Kv4Cfg<D, RT>::WARPS * 32, 1) kv4_attn_kernel(
       batch_ok = __ballot_sync(0xffffffffu, good);
       if (mine && !good) report(a.err, kDevBadBlock);
       const int h = a.chunks == 1 ? ask_sub : ask_sub / a.chunks;
-      if (good) batch_src = a.pool + ask_id * block_bytes + (h * a.recs + ask_rec) * P::RECORD;
+      if (good) batch_src = a.pool + ask_id * block_bytes + (static_cast<int64_t>(h) * a.recs + ask_rec) * P::RECORD;
       ask();
     }
     const unsigned ok = batch_ok >> batch_at & ALL;
@@ -1061,9 +1061,9 @@ extern "C" int mvb_paged_attention_decode_kv4(void* out, int64_t out_stride, con
                                               int64_t window, void* workspace, int64_t workspace_bytes,
                                               mvb_stream_t stream) {
   const char* what = "mvb_paged_attention_decode_kv4";
-  MVB_REQUIRE(batch >= 0 && batch <= (1 << 20), "%s: batch %lld", what, (long long)batch);
+  MVB_REQUIRE(batch >= 0 && batch <= 65536, "%s: batch %lld (at most 65536)", what, (long long)batch);
   MVB_REQUIRE(query_len >= 1 && query_len <= 1024, "%s: %lld query tokens (1 to 1024)", what, (long long)query_len);
-  MVB_REQUIRE(num_q_heads > 0 && num_kv_heads > 0 && num_q_heads % num_kv_heads == 0 && num_q_heads <= 65536,
+  MVB_REQUIRE(num_q_heads > 0 && num_kv_heads > 0 && num_q_heads % num_kv_heads == 0 && num_q_heads <= 4096,
               "%s: %lld query heads over %lld KV heads", what, (long long)num_q_heads, (long long)num_kv_heads);
   MVB_REQUIRE(head_dim == 64 || head_dim == 128 || head_dim == 256, "%s: head_dim %lld (64, 128 or 256)", what,
               (long long)head_dim);
@@ -1075,7 +1075,9 @@ extern "C" int mvb_paged_attention_decode_kv4(void* out, int64_t out_stride, con
               "%s: %lld blocks", what, (long long)num_blocks);
   MVB_REQUIRE(max_blocks > 0 && max_blocks <= (int64_t(1) << 30) / block_size, "%s: %lld blocks a sequence", what,
               (long long)max_blocks);
-  MVB_REQUIRE(window >= 0 && softcap >= 0.0f && scale == scale, "%s: window, softcap or scale", what);
+  MVB_REQUIRE(window >= 0 && softcap >= 0.0f && softcap <= kFltMax && fabsf(scale) <= kFltMax &&
+                  (softcap == 0.0f || fabsf(scale / softcap) <= kFltMax),
+              "%s: window, softcap or scale", what);
   if (batch == 0) return MVB_OK;
   MVB_REQUIRE(out && q && kv4 && block_tables && ctx_lens, "%s: null pointer", what);
   MVB_REQUIRE(table_stride >= max_blocks, "%s: table_stride %lld < max_blocks %lld", what, (long long)table_stride,

@@ -74,12 +74,22 @@ __device__ __forceinline__ float4 load4(const float* row, int j, int end) {
 // The lane's share of the sum over [begin, end), begin a multiple of 4.
 template <bool VEC>
 __device__ __forceinline__ double run_sum(const Weights& w, int begin, int end, int lane) {
+  const float4 zero = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
   double s = 0.0;
+  float4 p[2], q[2];  // two steps under way while one is summed
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    p[i] = load4<VEC>(w.p, begin + 128 * i + 4 * lane, end);
+    q[i] = w.q != nullptr ? load4<VEC>(w.q, begin + 128 * i + 4 * lane, end) : zero;
+  }
 #pragma unroll 1
   for (int j = begin + 4 * lane; j < end; j += 128) {
-    const float4 p = load4<VEC>(w.p, j, end);
-    const float4 q = w.q != nullptr ? load4<VEC>(w.q, j, end) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    s += (w.of(j, p.x, q.x) + w.of(j + 1, p.y, q.y)) + (w.of(j + 2, p.z, q.z) + w.of(j + 3, p.w, q.w));
+    const float4 pc = p[0], qc = q[0];
+    p[0] = p[1];
+    q[0] = q[1];
+    p[1] = load4<VEC>(w.p, j + 256, end);
+    q[1] = w.q != nullptr ? load4<VEC>(w.q, j + 256, end) : zero;
+    s += (w.of(j, pc.x, qc.x) + w.of(j + 1, pc.y, qc.y)) + (w.of(j + 2, pc.z, qc.z) + w.of(j + 3, pc.w, qc.w));
   }
   return s;
 }
@@ -263,8 +273,8 @@ extern "C" int mvb_verify_drafts(int64_t* out_tokens, int32_t* accepted, const f
   VerifyArgs a = {out_tokens, accepted, target_probs, target_stride, draft_probs, draft_stride, draft_tokens, uniforms,
                   draft_lens, static_cast<int>(max_drafts), static_cast<int>(vocab), device_status_ptr()};
   // Blocks per sequence: as many as fill the GPU once (two blocks an SM), with some 2,048 entries each.  Rows of
-  // 151,936 entries: at batch 1 one block took 33.3 us, 4 took 12.6 and 8 take 8.9; at batch 64, 4 take 23.4 us
-  // (3.3 TB/s) and 8, in two waves, took 28.7.
+  // 151,936 entries: at batch 1 one block took 33 us, 4 took 12.6 and 8 take 8.5; at batch 64, 4 take 23.1 us
+  // (3.4 TB/s) and 8, in two waves, took 28.7.
   const int64_t sms = current_sm_count();
   MVB_REQUIRE(sms > 0, "mvb_verify_drafts: no device");
   int blocks = kMaxCluster;

@@ -511,7 +511,7 @@ def kv4_write(k: torch.Tensor, v: torch.Tensor, kv4: torch.Tensor, layer: int, s
     ``slots`` (int64 ``[tokens]``, ``block * block_size + offset``; negative: not written) of a pool of
     ``kv_cache.kv4_pool``.  Per group of 64 channels: ``min``, ``scale = (max - min) / 15`` (both bf16) and
     ``round((x - min) / scale)``.  A group with a NaN or an infinity reads back as NaN.  The slots of one
-    call must differ from one another."""
+    call must differ: what a slot given twice holds afterwards is undefined."""
     what = "kv4_write"
     index, L, P, nkv, bs, D = _kv4_geometry(what, kv4, layer)
     try:

@@ -316,9 +316,34 @@ def test_attention_strides_and_table_views():
     check(dict(c, q=c["q"][:1], table=c["table"][:1], ctx=c["ctx"][:1]), one)
 
 
-def test_attention_many_sequences():
-    lens = [(37 * i) % 190 for i in range(700)]
-    c = attend_case(14, lens, 1, 4, 2, 64)
+@pytest.mark.parametrize("batch,D,T", [(700, 64, 1), (1500, 128, 1), (33, 128, 1), (32, 128, 5), (257, 256, 2)])
+def test_attention_many_sequences(batch, D, T):
+    """More sequences than lanes, than warps; all short, and with a few long ones among them."""
+    lens = [(37 * i) % 190 for i in range(batch)]
+    c = attend_case(batch, lens, T, 4, 2, D)
+    check(c, attend(c))
+    for i in (0, batch // 2, batch - 1):
+        lens[i] = 3000 + i
+    c = attend_case(batch + 1, lens, T, 4, 2, D)
+    check(c, attend(c))
+
+
+@pytest.mark.parametrize("lens", [[128] * 40, [100, 7, 128, 1, 0]])
+def test_attention_short_tables(lens):
+    """Tables of at most 128 tokens, whose items are not split; the same sequences under a wider table."""
+    for T, Hq, Hkv, D in ((1, 32, 8, 128), (3, 8, 4, 256), (2, 6, 6, 64), (9, 8, 2, 128)):
+        c = attend_case(len(lens) + T, lens, T, Hq, Hkv, D, bs=32)
+        out = attend(c)
+        check(c, out)
+        wide = torch.cat([c["table"], torch.full_like(c["table"], -1)], 1)
+        check(c, attend(dict(c, table=wide)))
+
+
+def test_attention_sequences_that_share_blocks():
+    """A common prefix held once: the same blocks in several tables, and twice in one."""
+    c = attend_case(23, [700, 700, 700], 1, 8, 2, 128)
+    c["table"][1, :20] = c["table"][0, :20]
+    c["table"][2, 30:40] = c["table"][2, :10]
     check(c, attend(c))
 
 
@@ -360,6 +385,11 @@ def test_attention_workspace_argument():
     need = N.lib().mvb_paged_attention_decode_kv4_workspace_bytes(1, 1, 32, 8, 128, 0)
     ws = torch.randint(0, 256, (max(need, 1),), dtype=torch.uint8, device=DEV)
     assert torch.equal(attend(c, workspace=ws), attend(c))
+    for bad in (ws[:-1], ws[1:], ws[:0], ws[::2], ws.int()):
+        with pytest.raises(RuntimeError):
+            attend(c, workspace=bad)
+    short = attend_case(18, [3, 128], 1, 32, 8, 128)            # at most 128 tokens: none is needed
+    assert torch.equal(attend(short, workspace=ws[:0]), attend(short))
 
 
 def test_attention_under_programmatic_launch():

@@ -51,7 +51,8 @@ def test_kv4_write_and_read_refuse(change, text):
     (dict(qs=4095), "16-byte aligned"), (dict(qs=4088), "rows at least a token apart"),
     (dict(os=2048), "rows at least a token apart"), (dict(q=A + 4), "16-byte aligned"),
     (dict(window=-1), "window"), (dict(cap=-1.0), "softcap"), (dict(scale=float("nan")), "scale"),
-    (dict(cap=float("nan")), "softcap"),
+    (dict(cap=float("nan")), "softcap"), (dict(cap=float("inf")), "softcap"), (dict(scale=float("inf")), "scale"),
+    (dict(cap=1e-40), "softcap"), (dict(B=65537), "batch 65537"), (dict(hq=8192, qs=1 << 20, os=1 << 20), "8192 query heads"),
 ])
 def test_kv4_attention_refuses(change, text):
     a = dict(out=A, os=4096, q=A, qs=4096, kv4=A, bt=A, ts=9, mb=9, ctx=A, B=2, T=1, hq=32, hkv=8, D=128, L=2, layer=0,
