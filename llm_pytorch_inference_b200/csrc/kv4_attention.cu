@@ -7,11 +7,13 @@
 // values a clock, and its integer pipe takes 64 lane-operations a clock, so codes never become floating-point
 // numbers one by one:
 //   * Scores: q . k = sum_g s_g (q_g . u_g) + m_g sum(q_g) over the groups of 64 channels, the pairs outside
-//     the products.  Codes are bytes for the integer tensor cores (u8 x s8, exact): three operations turn a word
-//     of 8 codes into two operands.  q of a row is held in 16 bits of its largest magnitude, as two signed bytes
-//     (planes) that are columns of their own; the rounding is 2^-16 of that magnitude, below what fp32 sums of
-//     the products would lose at long rows.  The sums stay below 2^22 and start at 1.5 * 2^23, so that their bits
-//     are the fp32 number itself and need no conversion.
+//     the products.  Up to 8 query rows, codes are bytes for the integer tensor cores (u8 x s8, exact): three
+//     operations turn a word of 8 codes into two operands.  q of a row is held in 16 bits of its largest magnitude, as
+//     two signed bytes (planes) that are columns of their own; the rounding is 2^-16 of that magnitude, below
+//     what fp32 sums of the products would lose at long rows.  The sums stay below 2^22 and start at
+//     1.5 * 2^23, so that their bits are the fp32 number itself and need no conversion.  With more rows the
+//     planes cost more than they save: codes are then fp16 operands, as below, and q is exact in fp16, times a
+//     power of two (24 rows: 77.0 -> 69.6 us at 4 sequences of 16K-32K).
 //   * Outputs: fp16 holds u * 2^-24 and u * 2^-20 as bit patterns with the code in bits 0-3 or 4-7 (subnormal
 //     numbers, exact), so one AND of a word yields two matrix operands.  The weight of a token times s' is
 //     the other operand, and p m' is summed per group and query, on the side.  That weight is the one
@@ -21,7 +23,8 @@
 // side: S^T = K Q^T (16 tokens x rows), O^T = V^T P^T.  The k index of the first product runs over the channels
 // in the order in which a lane's words hold them (Q is stored in that order); the tokens of the second are
 // permuted (tile_token) so that lanes reading the same word of different tokens fall into different banks.
-// Up to 4 rows (RT = 0) their two planes fill one n = 8 tile; above that a plane takes a tile of its own.
+// Up to 4 rows (RT = 0) fill the 8 columns as well: two planes each in the first product, the two halves of a masked
+// word (two channels of one token) in the second, which halves its accumulators.
 //
 // Work split: the cache of an item (sequence, KV head, chunk of query rows) is a run of records of 16 tokens.
 // The records of the whole batch are laid end to end and divided evenly over the resident warps, whatever the
@@ -29,6 +32,12 @@
 // through a ring in shared memory (one bulk copy a record, several in flight) and keeps the running
 // maximum, sum and output of an item in registers.  An item that spans workers leaves partial results, joined in
 // worker order by a second small kernel: no atomics, nothing to clear, the same bits every time.
+//
+// Measured on a B200 (6.55 TB/s copy), device time with inputs turned over: 64 sequences of 1024-2048 tokens, 32 query
+// and 8 KV heads of 128: 30.1 us for 115 MB, of which 3 us pass before the first copy, 17 at the rate of
+// memory and 7 in the last workers and the join.  One sequence of 131072: 36.6 us (151 MB).  16 sequences of
+// 4096-8192, 16 query and 8 KV heads of 256, capped: 47.1 us (226 MB, 4.8 TB/s).  5 query tokens of 4 sequences of
+// 16K-32K: 69.6 us (115 MB), bound by issued instructions.  One short sequence: 6.8 us, latency.
 #include <climits>
 #include <type_traits>
 
@@ -42,7 +51,9 @@ namespace {
 
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr int kShortRecords = 8;  // items of at most this many records are never split
-constexpr int kItemCost = 3;      // what beginning an item costs a warp, in bursts, for the division of the work
+// What beginning an item costs a warp (its Q, its result), in bursts, for the division of the work: 64 sequences of
+// 1024-2048 tokens and 8 query rows took 39.2 us at 1 and take 37.6 at 3.
+constexpr int kItemCost = 3;
 
 // A weight is 2^(score - reference): the reference is a row's maximum when last raised, and is raised
 // once a score passes it by more than kSlack (in powers of two), so that most records cost one vote instead
@@ -62,15 +73,17 @@ struct Kv4Rows {
   static constexpr int KT = RT == 0 ? 1 : 2 * RT;   // of the first
   static constexpr int NC = RT == 0 ? 1 : 2 * RT;   // rows per lane
   static constexpr int ROWS = RT == 0 ? 4 : 8 * RT;
-  // With two or three row tiles a second integer plane costs more (its sums put together per score) than the
-  // two operations a word that fp16 operands cost: see above.
+  // fp16 operands for the scores: with two or three row tiles the second integer plane costs more (its sums are put
+  // together score by score) than the two more operations a word.
   static constexpr bool HALF_K = RT > 1;
 };
 
 // BURST: records that a warp takes at once (one wait, one vote, one refill); STAGES of them are held, so that
-// an SM has some 45 KB or more under way while it computes; WARPS of the one block per SM by the registers.
-// One block of 16 warps, not two of 8: the scheduler prefers the older block, whose warps then ended
-// after 21 us of a call where the other's took 27 (batch 64, context 1024-2048).
+// an SM has some 45 KB or more under way while it computes.  WARPS of the one block per SM: 64 sequences of
+// 1024-2048 tokens, 4 rows of 128: 33.3 us with 8, 30.1 with 12, 31.0 with 16 (128 registers); 8 rows: 40.9, 37.6,
+// 44.1 (spills); 4 rows of 256, 16 x 4096-8192: 57, 47.1, 49.1.  16 rows and more of 128 or 256 need over 168
+// registers.  One block, not two: the scheduler prefers the older one, whose warps then ended after 21 us of a
+// call where the other's took 27.
 template <int D, int RT>
 struct Kv4Cfg {
   static constexpr int BURST = D == 256 || RT > 1 ? 1 : D == 128 ? 2 : RT == 0 ? 4 : 2;
@@ -93,7 +106,7 @@ struct Kv4AttnArgs {
   float score_scale;  // scale * log2(e), or scale / softcap under a cap
   float cap_log2;     // softcap * log2(e); 0 = no cap
   int window;
-  int slab_rows;  // rows of the largest chunk
+  int chunk_rows;  // rows of the largest chunk
   bool split;     // items may be split: their rounds are bursts and kItemCost; else an item is one round
   // workspace
   struct Kv4Item* items;  // [batch * hkv * chunks]
@@ -906,13 +919,13 @@ __global__ void __launch_bounds__(32 * WARPS) kv4_join_kernel(const Kv4AttnArgs 
   pdl_wait();
   pdl_launch_dependents();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, subs = a.hkv * a.chunks;
-  const int64_t work = static_cast<int64_t>(a.batch) * subs * a.slab_rows;
+  const int64_t work = static_cast<int64_t>(a.batch) * subs * a.chunk_rows;
   for (int64_t x0 = static_cast<int64_t>(blockIdx.x) * PAIRS; x0 < work; x0 += static_cast<int64_t>(gridDim.x) * PAIRS) {
     // lane j of every warp looks at pair x0 + j
     const int64_t x = x0 + lane;
     const bool mine = lane < PAIRS && x < work;
-    const int64_t item = x >> 31 ? x / a.slab_rows : static_cast<uint32_t>(x) / static_cast<uint32_t>(a.slab_rows);
-    const int row = static_cast<int>(x - item * a.slab_rows);
+    const int64_t item = x >> 31 ? x / a.chunk_rows : static_cast<uint32_t>(x) / static_cast<uint32_t>(a.chunk_rows);
+    const int row = static_cast<int>(x - item * a.chunk_rows);
     Kv4Item it = {0, 0};
     if (mine) it = a.items[item];
     const int seq = static_cast<int>(item / subs), sub = static_cast<int>(item - static_cast<int64_t>(seq) * subs);
@@ -1123,7 +1136,7 @@ extern "C" int mvb_paged_attention_decode_kv4(void* out, int64_t out_stride, con
   const int64_t most_rounds = split ? kItemCost + (most + p.burst - 1) / p.burst : 1;
   if (items < grid && items * most_rounds < grid) grid = items * most_rounds;
   a.chunks = static_cast<int>(p.chunks);
-  a.slab_rows = static_cast<int>(rows < p.rows ? rows : p.rows);
+  a.chunk_rows = static_cast<int>(rows < p.rows ? rows : p.rows);
   if (split) {
     char* ws = static_cast<char*>(workspace);
     a.items = reinterpret_cast<Kv4Item*>(ws + p.items_at);
@@ -1131,7 +1144,7 @@ extern "C" int mvb_paged_attention_decode_kv4(void* out, int64_t out_stride, con
     a.part_o = reinterpret_cast<float*>(ws + p.o_at);
   }
   int64_t join_grid = 0;
-  const int64_t all_pairs = items * a.slab_rows;
+  const int64_t all_pairs = items * a.chunk_rows;
   // a block per pair where there are few pairs, or where an item has many parts
   int pairs = all_pairs <= 2LL * sms || items * kFewParts < p.grid * p.warps ? 1 : 8;
   if (split) {
