@@ -11,9 +11,11 @@
 // K and of V of a token, for one head or two (HEADS): a 16-byte load (or store) of bf16 and one 32-bit word of
 // codes each, all under way together and with one look at the token's slot.  Eight lanes share a group and
 // find its minimum and maximum, on packed bf16, with three exchanges.  That leaves writing some 6 instructions a
-// value before arithmetic costs more than memory, so a code is not a division: fma(x - m, 1 / s, 1.5 * 2^23)
-// rounds and leaves the code in the low bits.  Where 1 / s moved up and down by 2^-20 disagree (ties mostly, one
-// value in 500), the exact remainder x - m - u s of the lower code decides.
+// value before arithmetic costs more than memory, so a quotient is a product and its correction, added to
+// 1.5 * 2^23, which rounds it to even and leaves the code in the low bits, and a multiply-add puts it into the word.
+// Measured on a B200, K and V of 8 heads of 128: writing 16,384 tokens takes 25 us for 86 MB (3.4 TB/s, bound by
+// issued instructions: 5 a value); with IEEE divisions it took 57.  64 tokens: 2.2 us.
+// Reading 32,768 tokens: 30.0 us for 172 MB (5.7 TB/s, copying reaches 6.55).
 #include "common.cuh"
 #include "host.h"
 #include "kv4.cuh"
@@ -56,52 +58,35 @@ constexpr float kMagic = 12582912.0f;   // 1.5 * 2^23: a sum's low bits are the 
 constexpr float kFltMax = 3.40282347e38f;
 constexpr uint32_t kPackBias = 0x4B400000u * 0x11111111u;  // the magic numbers' bits in the packed word, mod 2^32
 
-// x / 15 correctly rounded: with y = RN(1 / 15) and q near the quotient, q + (x - 15 q) y rounds to it (Markstein,
-// "Computation of elementary functions on the IBM RISC System/6000 processor", 1990); the remainder is exact away
-// from underflow, where the division itself is used.
-__device__ __forceinline__ float fifteenth(float x) {
-  if (fabsf(x) < 0x1p-90f) return __fdiv_rn(x, 15.0f);
-  const float y = 1.0f / 15.0f, q = x * y;
-  return fmaf(fmaf(-15.0f, q, x), y, q);
+// x / d correctly rounded, with y = RN(1 / d): q = RN(x y) is near the quotient, and q + (x - d q) y rounds to it
+// (Markstein, "Computation of elementary functions on the IBM RISC System/6000 processor", 1990).  The remainder is
+// exact away from underflow.
+__device__ __forceinline__ float divided(float x, float d, float y) {
+  const float q = x * y;
+  return fmaf(fmaf(-d, q, x), y, q);
 }
+
+constexpr float kTiny = 0x1p-90f;  // magnitudes from here on are away from underflow
 
 // Codes of 8 values of a group with minimum `low` and scale `scale` > 0, lowest nibble first.
 __device__ __forceinline__ uint32_t quantise8(const uint32_t (&x)[4], float low, float scale) {
-  float v[8];
-#pragma unroll
-  for (int j = 0; j < 8; ++j)
-    v[j] = __uint_as_float((j & 1) ? (x[j >> 1] & 0xffff0000u) : (x[j >> 1] << 16)) - low;
   uint32_t word = 0;
-  if (scale < 0x1p-100f) {  // 1 / s may not be finite, and a subnormal s may leave the largest code above 15
+  if (scale < kTiny) {  // a subnormal scale may leave the largest code above 15
 #pragma unroll 1
     for (int j = 7; j >= 0; --j) {
       const uint32_t h = j >= 6 ? x[3] : j >= 4 ? x[2] : j >= 2 ? x[1] : x[0];
-      const float y = __uint_as_float((j & 1) ? (h & 0xffff0000u) : (h << 16)) - low;
-      word = word * 16u + static_cast<uint32_t>(fminf(rintf(__fdiv_rn(y, scale)), 15.0f));
+      const float v = __uint_as_float((j & 1) ? (h & 0xffff0000u) : (h << 16)) - low;
+      word = word * 16u + static_cast<uint32_t>(fminf(rintf(__fdiv_rn(v, scale)), 15.0f));
     }
     return word;
   }
-  float inv;
-  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inv) : "f"(scale));  // within 2^-22
-  const float up = inv * (1.0f + 0x1p-20f), down = inv * (1.0f - 0x1p-20f);
-  uint32_t differ = 0, below[8];
+  const float inv = __frcp_rn(scale);
 #pragma unroll
   for (int j = 7; j >= 0; --j) {
-    const uint32_t above = __float_as_uint(fmaf(v[j], up, kMagic));
-    below[j] = __float_as_uint(fmaf(v[j], down, kMagic));
-    differ |= above ^ below[j];
-    word = word * 16u + below[j];
+    const float v = __uint_as_float((j & 1) ? (x[j >> 1] & 0xffff0000u) : (x[j >> 1] << 16)) - low;
+    word = word * 16u + __float_as_uint(divided(v, scale, inv) + kMagic);  // at most 15: scale is within 2^-9
   }
-  word -= kPackBias;
-  if (differ != 0) {
-    const float half = 0.5f * scale;
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const float r = fmaf(kMagic - __uint_as_float(below[j]), scale, v[j]);  // exact: a short multiple of v's last place
-      word += (r > half || (r == half && (below[j] & 1u))) ? 1u << (4 * j) : 0u;
-    }
-  }
-  return word;
+  return word - kPackBias;
 }
 
 // A lane per (token, HEADS heads, 8 channels).
@@ -153,7 +138,8 @@ __global__ void __launch_bounds__(kThreads) kv4_write_kernel(const Kv4Args a, co
     for (int o = 1; o < 8; o <<= 1) m2 = __hmin2_nan(m2, as_bf162(__shfl_xor_sync(0xffffffffu, as_u32(m2), o)));
     if (!live) continue;
     float low = __bfloat162float(m2.x);
-    float scale = bf16_round(fifteenth(-__bfloat162float(m2.y) - low));
+    const float span = -__bfloat162float(m2.y) - low;
+    float scale = bf16_round(span < kTiny ? __fdiv_rn(span, 15.0f) : divided(span, 15.0f, 1.0f / 15.0f));
     uint32_t word = 0;
     if (!(scale <= kFltMax) || !(fabsf(low) <= kFltMax)) scale = low = __int_as_float(0x7fc00000);
     else if (scale > 0.0f) word = quantise8(x, low, scale);
