@@ -376,7 +376,8 @@ __global__ void __launch_bounds__(Kv4Cfg<D, RT>::WARPS * 32, 1) kv4_attn_kernel(
   unsigned came = 0, phase = 0;   // per stage: the records that came; parity of its barrier
   int pending = 0;                // stages whose records are still to be waited for
   auto issue = [&](int st) {
-    if (batch_at >= batch_n) {
+    const bool turned = batch_at >= batch_n;
+    if (turned) {
       if (ask_n == 0) return;
       batch_n = ask_n;
       batch_at = 0;
@@ -385,7 +386,6 @@ __global__ void __launch_bounds__(Kv4Cfg<D, RT>::WARPS * 32, 1) kv4_attn_kernel(
       if (mine && !good) report(a.err, kDevBadBlock);
       const int h = a.chunks == 1 ? ask_sub : ask_sub / a.chunks;
       if (good) batch_src = a.pool + ask_id * block_bytes + (static_cast<int64_t>(h) * a.recs + ask_rec) * P::RECORD;
-      ask();
     }
     const unsigned ok = batch_ok >> batch_at & ALL;
     came = (came & ~(ALL << (st * BURST))) | ok << (st * BURST);
@@ -396,6 +396,7 @@ __global__ void __launch_bounds__(Kv4Cfg<D, RT>::WARPS * 32, 1) kv4_attn_kernel(
       bulk_load(ring + (st * BURST + turn) * P::RECORD, batch_src, P::RECORD, bars + st);
     batch_at += BURST;
     ++pending;
+    if (turned) ask();
   };
   ask();
 #pragma unroll 1
@@ -998,9 +999,11 @@ void kv4_plan_rows(Kv4Plan& p, int64_t sms) {
 }
 template <int D>
 void kv4_plan_dim(Kv4Plan& p, int64_t rows, int64_t sms) {
-  if (rows <= 4) kv4_plan_rows<D, 0>(p, sms);
-  else if (rows <= 8) kv4_plan_rows<D, 1>(p, sms);
-  else if (rows <= 16 || D == 256) kv4_plan_rows<D, 2>(p, sms);
+  // rows beyond the largest chunk go into equal chunks, not a full one and a rest
+  const int64_t most = D == 256 ? 16 : 24, chunks = (rows + most - 1) / most, per = (rows + chunks - 1) / chunks;
+  if (per <= 4) kv4_plan_rows<D, 0>(p, sms);
+  else if (per <= 8) kv4_plan_rows<D, 1>(p, sms);
+  else if (per <= 16 || D == 256) kv4_plan_rows<D, 2>(p, sms);
   else kv4_plan_rows<D, 3>(p, sms);
 }
 Kv4Plan kv4_plan(int64_t sms, int64_t head_dim, int64_t rows, int64_t batch, int64_t hkv) {
