@@ -534,8 +534,10 @@ __global__ void __launch_bounds__(Kv4Cfg<D, RT>::WARPS * 32, 1) kv4_attn_kernel(
 #pragma unroll
       for (int k = 0; k < NG; ++k) mo[q][k] = 0.0f;
     }
-    float vscale = 1.0f;  // power of two that the value scales are multiplied by
-    bool fresh = true, none = true;  // no scaling chosen, no reference chosen
+    // power of two that the value scales are multiplied by, and what the products may reach: chosen at the first scale
+    // above zero (until then the outputs hold nothing but zeros), and only ever lowered after that
+    float vscale = 1.0f, limit = 0.0f;
+    bool none = true;  // no reference chosen: nothing summed yet
 
     // One burst from record t on, `have`: which of its records came.  MASKED: some row does not see some token.
     auto burst = [&](auto masked_tag, int t, unsigned have) {
@@ -664,7 +666,7 @@ __global__ void __launch_bounds__(Kv4Cfg<D, RT>::WARPS * 32, 1) kv4_attn_kernel(
           }
         }
       // ---- new references and scaling, where a score or a scale outgrew them
-      if (__any_sync(0xffffffffu, far > kSlack || top > kScaleMax)) {
+      if (__any_sync(0xffffffffu, far > kSlack || top > limit)) {
         float smax = 0.0f;
 #pragma unroll
         for (int u = 0; u < BURST; ++u)
@@ -676,14 +678,14 @@ __global__ void __launch_bounds__(Kv4Cfg<D, RT>::WARPS * 32, 1) kv4_attn_kernel(
 #pragma unroll
         for (int off = 4; off < 32; off <<= 1) smax = fmaxf(smax, __shfl_xor_sync(0xffffffffu, smax, off));
         float fo = 1.0f;
-        if (smax > 0.0f && (fresh || smax * vscale > kScaleMax)) {
+        if (smax * vscale > limit) {
           const float ns = ldexpf(1.0f, min(kScaleTarget - ilogbf(smax), 126));
-          fo = fresh ? 1.0f : ns / vscale;
+          fo = limit == 0.0f ? 1.0f : ns / vscale;
           vscale = ns;
-          fresh = false;
+          limit = kScaleMax;
         }
         float fac[NC];
-        const bool empty = none;  // nothing summed yet
+        const bool empty = none;
         none = false;
 #pragma unroll
         for (int q = 0; q < NC; ++q) {

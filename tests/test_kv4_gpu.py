@@ -266,6 +266,34 @@ def test_attention_values_of_mixed_magnitude():
             check(c, attend(c, window=200), window=200)
 
 
+@pytest.mark.parametrize("later", [1.0, 1e-6, 1e6])
+@pytest.mark.parametrize("T,Hq,Hkv,D", [(1, 8, 2, 128), (1, 16, 2, 256), (5, 8, 2, 128)])
+def test_attention_constant_values_first(later, T, Hq, Hkv, D):
+    """Values without a spread (scale 0) for a while, then ordinary, tiny or large ones, and scores that rise late, so
+    that the references and the scaling of the weights change after sums have begun."""
+    g = gen(int(math.log10(later)) + 50 + D)
+    n = 640
+    pool = kv4_pool(40, 16, 2, Hkv, D)
+    slots = torch.arange(n, device=DEV)
+    k, v = normal(g, n, Hkv, D), normal(g, n, Hkv, D).float() * later
+    v[:100] = 0.25
+    v[300:310] *= 1e-3
+    q = normal(g, 1, T, Hq, D)
+    # keys along the first query head's direction, ever longer
+    d = q[0, 0].view(Hkv, Hq // Hkv, D)[:, 0].float()
+    k = (k.float() * 0.3 + torch.arange(n, device=DEV)[:, None, None] / n * 3 * d / d.norm(dim=-1, keepdim=True)).to(BF)
+    ops.kv4_write(k, v.to(BF), pool, 1, slots)
+    c = dict(q=q, pool=pool, table=torch.arange(40, dtype=torch.int32, device=DEV)[None],
+             ctx=torch.tensor([n], dtype=torch.int32, device=DEV), scale=2 / math.sqrt(D))
+    check(c, attend(c))
+    # one worker's 128 tokens: constant values up to 32, scores some 20 powers of two higher from 112 on
+    v[:32], v[32:128] = 0.25, normal(g, 96, Hkv, D).float() * later
+    k[:112], k[112:128] = k[:112] * 0.1, (4 * d / d.norm(dim=-1, keepdim=True) + 0.1 * k[112:128].float()).to(BF)
+    ops.kv4_write(k, v.to(BF), pool, 1, slots)
+    c = dict(c, ctx=torch.tensor([128], dtype=torch.int32, device=DEV), table=c["table"][:, :8])
+    check(c, attend(c))
+
+
 def test_attention_nan_value_stays_with_those_that_see_it():
     """A drafted token whose V is NaN reaches the queries that see it and no other."""
     c = attend_case(9, [200, 200], 3, 8, 2, 128)
