@@ -295,12 +295,15 @@ int mvb_paged_attention_decode_kv4(void* out, int64_t out_stride, const void* q,
  * means 0, and the two may not be the same word).  A sequence that does not fit -- in its table row, in
  * what is left of the free list, or in the num_tokens of the outputs -- takes no block:
  * granted 0, its tokens' slots -1; those behind it may still fit.  Negative lengths are refused the
- * same way, with MVB_DEV_BAD_POSITION.  Entries of slots past the last token are -1.  batch <= 8192. */
+ * same way, with MVB_DEV_BAD_POSITION.  Entries of slots past the last token are -1.  batch <= 1048576;
+ * more than 8192 sequences need a workspace of mvb_assign_slots_workspace_bytes(batch) bytes (0 for fewer: NULL),
+ * 8-byte aligned, of any content. */
+int64_t mvb_assign_slots_workspace_bytes(int64_t batch);
 int mvb_assign_slots(int64_t* slots, int32_t* positions, int32_t* seq_start, int32_t* granted,
                      int32_t* free_head_out, int32_t* block_tables, int64_t table_stride, int64_t max_blocks,
                      const int32_t* ctx_lens, const int32_t* new_lens, const int32_t* free_blocks, int64_t num_free,
                      const int32_t* free_head, int64_t batch, int64_t block_size, int64_t num_tokens,
-                     mvb_stream_t stream);
+                     void* workspace, int64_t workspace_bytes, mvb_stream_t stream);
 
 /* Verification of drafted tokens (speculative decoding; no counterpart in the reference).
  * target_probs: fp32 rows, row b * (max_drafts + 1) + i (target_stride elements apart) the target's

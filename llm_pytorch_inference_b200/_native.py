@@ -63,8 +63,9 @@ SIGNATURES: dict[str, tuple] = {
     "mvb_paged_attention_decode_kv4_workspace_bytes": (_i64, [_i64, _i64, _i64, _i64, _i64, _i32]),
     "mvb_paged_attention_decode_kv4": (_i32, [_vp, _i64, _vp, _i64, _vp, _vp, _i64, _i64, _vp] + [_i64] * 9 +
                                        [_f32, _f32, _i64, _vp, _i64, _vp]),
+    "mvb_assign_slots_workspace_bytes": (_i64, [_i64]),
     "mvb_assign_slots": (_i32, [_vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _vp, _vp, _vp, _i64, _vp, _i64, _i64, _i64,
-                                _vp]),
+                                _vp, _i64, _vp]),
     "mvb_verify_drafts": (_i32, [_vp, _vp, _vp, _i64, _vp, _i64, _vp, _vp, _vp, _i64, _i64, _i64, _vp]),
     "mvb_gemm_workspace_bytes": (_i64, [_i64, _i64, _i64, _i32]),
     "mvb_gemm_bf16": (_i32, [_vp, _i64, _vp, _i64, _vp, _i64, _i64, _i64, _i64, _i32, _vp, _i64, _vp, _i64, _vp]),

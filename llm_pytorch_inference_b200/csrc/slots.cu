@@ -9,7 +9,12 @@
 // CTA), then maps its share of the tokens; a token finds its sequence by bisecting the scanned
 // starts in shared memory.  A token at the first position of a new block writes that block into
 // the table.  No CTA reads what another writes: entries below ceil(ctx_b / bs) are only read, the
-// ones above only written.  Bound by latency: a scan, a bisection and two dependent loads.
+// ones above only written.  Bound by latency: a scan, a bisection and two dependent loads (4.3 us for 64 sequences of
+// one token, 5.5 for 200 of 500 to 1000).
+//
+// A batch whose starts do not fit into shared memory is cut into pieces of 4,096 sequences, a block each: sums of
+// the pieces, then starts and sums of the blocks needed, then offsets into the free list, then the tokens, a
+// launch each.
 #include <climits>
 
 #include "common.cuh"
@@ -19,7 +24,10 @@ namespace mvb {
 namespace {
 
 constexpr int kThreads = 512;
-constexpr int kMaxBatch = 8192;  // starts and block offsets of the whole batch in shared memory
+constexpr int kMaxShared = 8192;          // sequences whose starts and offsets one block holds in shared memory
+constexpr int kMaxBatch = 1 << 20;
+constexpr int kPer = 8;                   // sequences of a thread in the launches over pieces
+constexpr int kPiece = kPer * kThreads;
 
 struct SlotArgs {
   int64_t* slots;
@@ -66,7 +74,40 @@ __device__ __forceinline__ void block_scan2(int64_t& x, int64_t& y, int64_t (*wa
   }
 }
 
-__global__ void __launch_bounds__(kThreads) assign_slots_kernel(SlotArgs a) {
+// Slots and positions of this block's tokens.
+__device__ __forceinline__ void map_tokens(const SlotArgs& a, int64_t head, const int32_t* start, const int32_t* first) {
+  const int64_t step = static_cast<int64_t>(gridDim.x) * kThreads;
+  const int32_t last = start[a.batch];
+  for (int64_t t = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x; t < a.tokens; t += step) {
+    int64_t slot = -1;
+    int64_t pos = 0;
+    if (t < last) {
+      int lo = 0, hi = a.batch;  // start[lo] <= t < start[hi]
+      while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (start[mid] <= t) lo = mid; else hi = mid;
+      }
+      const int64_t ctx = max(a.ctx[lo], 0);
+      pos = ctx + (t - start[lo]);
+      if (first[lo] >= 0) {
+        const int64_t bi = pos / a.bs, held = ceil_div(ctx, a.bs);
+        int32_t* row = a.tables + lo * a.table_stride;
+        int32_t id;
+        if (bi < held) {
+          id = row[bi];
+        } else {
+          id = a.free_blocks[head + first[lo] + (bi - held)];
+          if (pos == bi * a.bs) row[bi] = id;
+        }
+        slot = id < 0 ? -1 : static_cast<int64_t>(id) * a.bs + (pos - bi * a.bs);
+      }
+    }
+    a.slots[t] = slot;
+    a.positions[t] = static_cast<int32_t>(min(pos, int64_t(INT_MAX)));
+  }
+}
+
+__global__ void __launch_bounds__(kThreads) assign_slots_kernel(const SlotArgs a) {
   extern __shared__ int32_t sm[];
   __shared__ int64_t warps[kThreads / 32][2];
   __shared__ int64_t carry[2];
@@ -158,48 +199,155 @@ __global__ void __launch_bounds__(kThreads) assign_slots_kernel(SlotArgs a) {
     for (int b = tid; b < a.batch; b += kThreads) a.granted[b] = first[b] >= 0 ? 1 : 0;
     if (tid == 0) *a.head_out = static_cast<int32_t>(head + carry[1]);
   }
+  map_tokens(a, head, start, first);
+}
 
-  const int64_t step = static_cast<int64_t>(gridDim.x) * kThreads;
-  const int32_t last = start[a.batch];
-  for (int64_t t = static_cast<int64_t>(blockIdx.x) * kThreads + tid; t < a.tokens; t += step) {
-    int64_t slot = -1;
-    int64_t pos = 0;
-    if (t < last) {
-      int lo = 0, hi = a.batch;  // start[lo] <= t < start[hi]
-      while (hi - lo > 1) {
-        const int mid = (lo + hi) >> 1;
-        if (start[mid] <= t) lo = mid; else hi = mid;
+// ---- batches of more than kMaxShared sequences
+struct BigArgs {
+  int64_t* piece_add;   // [pieces] tokens of a piece
+  int64_t* piece_need;  // [pieces] blocks it needs
+  int32_t* first;       // [batch] blocks needed (-1: refused), then the offset of the first one
+};
+
+// Sum over the block, in every thread.
+__device__ __forceinline__ int64_t block_sum(int64_t x, int64_t (*warps)[2]) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
+  __syncthreads();
+  if ((threadIdx.x & 31) == 0) warps[threadIdx.x >> 5][0] = x;
+  __syncthreads();
+  int64_t all = 0;
+  for (int w = 0; w < kThreads / 32; ++w) all += warps[w][0];
+  return all;
+}
+// Sum of v[0 .. n), in every thread.
+__device__ __forceinline__ int64_t sum_before(const int64_t* v, int n, int64_t (*warps)[2]) {
+  int64_t x = 0;
+  for (int i = threadIdx.x; i < n; i += kThreads) x += v[i];
+  return block_sum(x, warps);
+}
+
+__global__ void __launch_bounds__(kThreads) slot_sums_kernel(const SlotArgs a, const BigArgs g) {
+  __shared__ int64_t warps[kThreads / 32][2];
+  pdl_wait();
+  const int64_t b0 = static_cast<int64_t>(blockIdx.x) * kPiece + threadIdx.x * kPer;
+  int64_t add = 0;
+  for (int i = 0; i < kPer; ++i)
+    if (b0 + i < a.batch) add += max(a.add[b0 + i], 0);
+  add = block_sum(add, warps);
+  if (threadIdx.x == 0) g.piece_add[blockIdx.x] = add;
+}
+
+__global__ void __launch_bounds__(kThreads) slot_starts_kernel(const SlotArgs a, const BigArgs g) {
+  __shared__ int64_t warps[kThreads / 32][2];
+  const int64_t b0 = static_cast<int64_t>(blockIdx.x) * kPiece + threadIdx.x * kPer;
+  int64_t own = 0, zero = 0;
+  for (int i = 0; i < kPer; ++i)
+    if (b0 + i < a.batch) own += max(a.add[b0 + i], 0);
+  int64_t at = own;
+  const int64_t before = sum_before(g.piece_add, blockIdx.x, warps);
+  block_scan2(at, zero, warps);
+  at += before - own;
+  if (blockIdx.x == 0 && threadIdx.x == 0) a.seq_start[0] = 0;
+  int64_t needs = 0;
+  for (int i = 0; i < kPer; ++i) {
+    const int64_t b = b0 + i;
+    if (b >= a.batch) break;
+    const int64_t ctx = a.ctx[b], add = a.add[b];
+    bool ok = ctx >= 0 && add >= 0;
+    if (!ok) report(a.err, kDevBadPosition);
+    at += max(add, int64_t(0));
+    a.seq_start[b + 1] = static_cast<int32_t>(min(at, int64_t(INT_MAX)));
+    ok = ok && ctx + add <= a.max_blocks * a.bs && at <= a.tokens;
+    const int64_t need = ok ? ceil_div(ctx + add, a.bs) - ceil_div(ctx, a.bs) : 0;
+    needs += need;
+    g.first[b] = ok ? static_cast<int32_t>(need) : -1;
+  }
+  needs = block_sum(needs, warps);
+  if (threadIdx.x == 0) g.piece_need[blockIdx.x] = needs;
+}
+
+__global__ void __launch_bounds__(kThreads) slot_offsets_kernel(const SlotArgs a, const BigArgs g) {
+  __shared__ int64_t warps[kThreads / 32][2];
+  const int64_t head = a.head_in != nullptr ? max(static_cast<int64_t>(*a.head_in), int64_t(0)) : 0;
+  const int64_t avail = max(a.num_free - head, int64_t(0));
+  const int64_t all = sum_before(g.piece_need, gridDim.x, warps);
+  if (all > avail) {  // short: in row order, 32 sequences at a time, one by one where they do not all fit
+    if (blockIdx.x != 0 || threadIdx.x >= 32) return;
+    const int lane = threadIdx.x;
+    int64_t taken = 0;
+    for (int64_t b = lane; b - lane < a.batch; b += 32) {
+      const int need = b < a.batch ? g.first[b] : -1;
+      int64_t sum = max(need, 0);
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int64_t y = __shfl_up_sync(0xffffffffu, sum, o);
+        if (lane >= o) sum += y;
       }
-      const int64_t ctx = max(a.ctx[lo], 0);
-      pos = ctx + (t - start[lo]);
-      if (first[lo] >= 0) {
-        const int64_t bi = pos / a.bs, held = ceil_div(ctx, a.bs);
-        int32_t* row = a.tables + lo * a.table_stride;
-        int32_t id;
-        if (bi < held) {
-          id = row[bi];
-        } else {
-          id = a.free_blocks[head + first[lo] + (bi - held)];
-          if (pos == bi * a.bs) row[bi] = id;
+      const int64_t last = __shfl_sync(0xffffffffu, sum, 31);
+      int64_t at = need < 0 ? -1 : taken + sum - need;
+      if (taken + last <= avail) {
+        taken += last;
+      } else {
+        for (int j = 0; j < 32; ++j) {
+          const int want = __shfl_sync(0xffffffffu, need, j);
+          const bool fits = want >= 0 && taken + want <= avail;
+          if (j == lane) at = fits ? taken : -1;
+          if (fits) taken += want;
         }
-        slot = id < 0 ? -1 : static_cast<int64_t>(id) * a.bs + (pos - bi * a.bs);
+      }
+      if (b < a.batch) {
+        g.first[b] = static_cast<int32_t>(at);
+        a.granted[b] = at >= 0 ? 1 : 0;
       }
     }
-    a.slots[t] = slot;
-    a.positions[t] = static_cast<int32_t>(min(pos, int64_t(INT_MAX)));
+    if (lane == 0) *a.head_out = static_cast<int32_t>(head + taken);
+    return;
   }
+  const int64_t b0 = static_cast<int64_t>(blockIdx.x) * kPiece + threadIdx.x * kPer;
+  int32_t need[kPer];
+  int64_t own = 0, zero = 0;
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) {
+    need[i] = b0 + i < a.batch ? g.first[b0 + i] : -1;
+    own += max(need[i], 0);
+  }
+  int64_t at = own;
+  const int64_t before = sum_before(g.piece_need, blockIdx.x, warps);
+  block_scan2(at, zero, warps);
+  at += before - own;
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) {
+    if (b0 + i >= a.batch) break;
+    g.first[b0 + i] = need[i] < 0 ? -1 : static_cast<int32_t>(at);
+    a.granted[b0 + i] = need[i] < 0 ? 0 : 1;
+    at += max(need[i], 0);
+  }
+  if (blockIdx.x == 0 && threadIdx.x == 0) *a.head_out = static_cast<int32_t>(head + all);
 }
+
+__global__ void __launch_bounds__(kThreads) slot_tokens_kernel(const SlotArgs a, const BigArgs g) {
+  const int64_t head = a.head_in != nullptr ? max(static_cast<int64_t>(*a.head_in), int64_t(0)) : 0;
+  map_tokens(a, head, a.seq_start, g.first);
+}
+
+int64_t slot_pieces(int64_t batch) { return (batch + kPiece - 1) / kPiece; }
 
 }  // namespace
 }  // namespace mvb
 
 using namespace mvb;
 
+extern "C" int64_t mvb_assign_slots_workspace_bytes(int64_t batch) {
+  return batch <= kMaxShared ? 0 : slot_pieces(batch) * 16 + batch * 4;
+}
+
 extern "C" int mvb_assign_slots(int64_t* slots, int32_t* positions, int32_t* seq_start, int32_t* granted,
                                 int32_t* free_head_out, int32_t* block_tables, int64_t table_stride,
                                 int64_t max_blocks, const int32_t* ctx_lens, const int32_t* new_lens,
                                 const int32_t* free_blocks, int64_t num_free, const int32_t* free_head,
-                                int64_t batch, int64_t block_size, int64_t num_tokens, mvb_stream_t stream) {
+                                int64_t batch, int64_t block_size, int64_t num_tokens, void* workspace,
+                                int64_t workspace_bytes, mvb_stream_t stream) {
   MVB_REQUIRE(seq_start && free_head_out, "mvb_assign_slots: null pointer");
   MVB_REQUIRE(batch >= 0 && batch <= kMaxBatch, "mvb_assign_slots: batch %lld (at most %d)", (long long)batch,
               kMaxBatch);
@@ -218,10 +366,28 @@ extern "C" int mvb_assign_slots(int64_t* slots, int32_t* positions, int32_t* seq
   SlotArgs a = {slots,    positions, seq_start,   granted,   free_head_out, block_tables, table_stride,
                 max_blocks, ctx_lens,  new_lens,    free_blocks, free_head,  num_free,     num_tokens,
                 static_cast<int>(batch), static_cast<int>(block_size), device_status_ptr()};
-  const size_t smem = (2 * batch + 1) * sizeof(int32_t);
-  if (smem > 48 * 1024) MVB_TRY(set_smem(assign_slots_kernel, smem, "assign_slots"));
+  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   int64_t grid = (num_tokens + 2 * kThreads - 1) / (2 * kThreads);
   grid = grid < 1 ? 1 : grid > sms ? sms : grid;
-  return launch("assign_slots", assign_slots_kernel, dim3(static_cast<unsigned>(grid)), dim3(kThreads), smem,
-                reinterpret_cast<cudaStream_t>(stream), a);
+  const dim3 blocks(static_cast<unsigned>(grid)), threads(kThreads);
+  if (batch <= kMaxShared) {
+    const size_t smem = (2 * batch + 1) * sizeof(int32_t);
+    if (smem > 48 * 1024) MVB_TRY(set_smem(assign_slots_kernel, smem, "assign_slots"));
+    return launch("assign_slots", assign_slots_kernel, blocks, threads, smem, st, a);
+  }
+  MVB_REQUIRE(workspace && aligned(workspace, 8) && workspace_bytes >= mvb_assign_slots_workspace_bytes(batch),
+              "mvb_assign_slots: a workspace of %lld bytes, 8-byte aligned (got %lld)",
+              (long long)mvb_assign_slots_workspace_bytes(batch), (long long)workspace_bytes);
+  const int64_t n = slot_pieces(batch);
+  BigArgs g;
+  g.piece_add = static_cast<int64_t*>(workspace);
+  g.piece_need = g.piece_add + n;
+  g.first = reinterpret_cast<int32_t*>(g.piece_need + n);
+  const dim3 pieces(static_cast<unsigned>(n));
+  // the launches after the first one are plain: each reads what the one before it wrote
+  MVB_TRY(launch("assign_slots", slot_sums_kernel, pieces, threads, 0, st, a, g));
+  slot_starts_kernel<<<pieces, threads, 0, st>>>(a, g);
+  slot_offsets_kernel<<<pieces, threads, 0, st>>>(a, g);
+  slot_tokens_kernel<<<blocks, threads, 0, st>>>(a, g);
+  return cuda_status(cudaGetLastError(), "assign_slots");
 }

@@ -685,10 +685,14 @@ def assign_slots(block_tables: torch.Tensor, ctx_lens: torch.Tensor, new_lens: t
     at = words.data_ptr()
     slots, positions, seq_start, granted, head = words.split_with_sizes((2 * num_tokens, num_tokens, B + 1, B, 1))
     start = at + 12 * num_tokens
+    ws, ws_bytes = None, 0
+    if B > 8192:
+        ws_bytes = N.lib().mvb_assign_slots_workspace_bytes(B)
+        ws = torch.empty(ws_bytes, dtype=_U8, device=block_tables.device)
     N.on_device(index, what, N.lib().mvb_assign_slots, at, at + 8 * num_tokens, start, start + 4 * (B + 1),
                 start + 4 * (2 * B + 1), block_tables.data_ptr(), t_stride, width, ctx_lens.data_ptr(),
                 new_lens.data_ptr(), free_blocks.data_ptr(), free_blocks.numel(), N.ptr(free_head), B,
-                int(block_size), int(num_tokens))
+                int(block_size), int(num_tokens), N.ptr(ws), ws_bytes)
     slots = slots.view(_I64)
     return SlotPlan(slots, positions, seq_start, granted, head)
 

@@ -65,14 +65,14 @@ def test_kv4_attention_refuses(change, text):
 
 @pytest.mark.parametrize("change, text", [
     (dict(start=None), "null pointer"), (dict(granted=None), "null pointer"), (dict(ctx=None), "null pointer"),
-    (dict(bt=None), "block_tables"), (dict(batch=8193), "batch 8193"), (dict(batch=-1), "batch -1"),
+    (dict(bt=None), "block_tables"), (dict(batch=1 << 21), "batch 2097152"), (dict(batch=-1), "batch -1"),
     (dict(ts=3), "table_stride 3"), (dict(free=None), "free list"), (dict(nf=-1), "free list"),
     (dict(bs=0), "block_size 0"), (dict(mb=1 << 30, ts=1 << 30), "blocks a sequence"), (dict(n=-1), "num_tokens"),
     (dict(slots=None), "num_tokens"), (dict(head=A + 4), "free_head_out may not be free_head"),
 ])
 def test_assign_slots_refuses(change, text):
     a = dict(slots=A, pos=A, start=A, granted=A, head_out=A + 4, bt=A, ts=8, mb=8, ctx=A, new=A, free=A, nf=10,
-             head=None, batch=3, bs=16, n=12)
+             head=None, batch=3, bs=16, n=12, ws=None, ws_bytes=0)
     a.update(change)
     refused(N.lib().mvb_assign_slots(*a.values(), None), text)
 

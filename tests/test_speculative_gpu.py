@@ -42,7 +42,8 @@ def run_slots(tables, ctx, new, free, bs, n, head=None):
 
 
 @pytest.mark.parametrize("batch,most,bs", [(1, 1, 16), (1, 5000, 16), (3, 1, 16), (64, 1, 16), (65, 9, 4), (511, 3, 16),
-                                           (512, 40, 32), (513, 40, 7), (1500, 100, 16), (8192, 2, 16), (2, 0, 16)])
+                                           (512, 40, 32), (513, 40, 7), (1500, 100, 16), (8192, 2, 16), (2, 0, 16),
+                                           (8193, 3, 16), (12288, 1, 4), (50001, 2, 16)])
 def test_slots(batch, most, bs):
     """Ragged lengths, zero-token sequences, tables with room to spare, against the sequences one by one."""
     r = random.Random(batch * 1000 + most)
@@ -69,8 +70,27 @@ def test_slots_that_do_not_fit(seed):
         run_slots(tables, ctx, new, list(range(1000, 1000 + free)), bs, sum(new))
         run_slots(tables, ctx, new, list(range(1000, 1000 + free)), bs, sum(new) // 2)
         run_slots(tables, ctx, new, list(range(1000, 1000 + free)), bs, sum(new), head=free // 2)
+    if seed < 2:                                                      # a batch cut into pieces
+        batch = 9000 + 4000 * seed
+        ctx, new = [r.randint(-1, 24) for _ in range(batch)], [r.randint(0, 12) for _ in range(batch)]
+        tables = [[r.randint(0, 999) for _ in range(4)] for _ in range(batch)]
+        for free in (0, 1, 700, 3000, 20000):
+            run_slots(tables, ctx, new, list(range(1000, 1000 + free)), bs, sum(new), head=1)
+            run_slots(tables, ctx, new, list(range(1000, 1000 + free)), bs, sum(new) // 2)
+        assert N.device_status(clear=True) == N.DEV_BAD_POSITION
+        return
     run_slots(tables, ctx, new, [1, 2, 3], bs, sum(new), head=9)      # a head past the list: nothing left
     run_slots([[] for _ in ctx], ctx, new, [1, 2, 3], bs, sum(new))   # no table entries at all
+
+
+def test_slots_of_a_large_batch_need_a_workspace():
+    x = torch.zeros(9001, dtype=torch.int32, device=DEV)
+    p = x.data_ptr()
+    need = N.lib().mvb_assign_slots_workspace_bytes(9000)
+    assert need > 0 and N.lib().mvb_assign_slots_workspace_bytes(8192) == 0
+    for ws, size in ((None, need), (p, need - 1), (p + 4, need)):
+        rc = N.lib().mvb_assign_slots(p, p, p, p, p + 8, p, 1, 1, p, p, p, 5, None, 9000, 16, 0, ws, size, N.stream_handle())
+        assert rc == 1 and b"workspace" in N.lib().mvb_last_error()
 
 
 def test_slots_negative_lengths_are_refused():
