@@ -146,7 +146,7 @@ __device__ __forceinline__ float ex2(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
-// tanh x = 1 - 2 / (e^2x + 1): absolute error of a few 2^-24, where a score capped at c keeps c times that.
+// tanh x = 1 - 2 / (e^2x + 1), with an absolute error of a few 2^-24: c times that in a score capped at c.
 __device__ __forceinline__ float tanh_exp(float x) {
   return 1.0f - __fdividef(2.0f, ex2(x * (2.0f * kLog2e)) + 1.0f);
 }
@@ -338,6 +338,7 @@ __global__ void __launch_bounds__(Kv4Cfg<D, RT>::WARPS * 32, 1) kv4_attn_kernel(
   const int64_t in_seq = r0 - __shfl_sync(0xffffffffu, begin, owner);
   int sub = in_seq >> 31 ? static_cast<int>(in_seq / sq.rounds) : static_cast<int>(in_seq) / sq.rounds;
   int ra = static_cast<int>(in_seq - static_cast<int64_t>(sub) * sq.rounds);
+
   // ---- the worker's stream of records, STAGES bursts ahead of the arithmetic.  Up to 32 records of an item are
   // prepared at once, lane j seeing to record j: its block id is asked for a batch ahead, its copy is issued
   // by that lane when its turn comes.
@@ -418,7 +419,8 @@ __global__ void __launch_bounds__(Kv4Cfg<D, RT>::WARPS * 32, 1) kv4_attn_kernel(
     const int rows = min(a.group * a.T - row0, ROWS);
     const int2 span = kv4_records<BURST>(a, sq, ra, n_rounds);
 
-    // Q of the item, four rows at a time, eight lanes each: round(32512 q / max |q|) = 256 hi + lo, signed bytes
+    // Q of the item, four rows at a time, eight lanes each, in the order of the first product's operands:
+    // round(32512 q / max |q|) = 256 hi + lo as signed bytes, or fp16
     __syncwarp();
     auto load_rows = [&](int pass, uint4 (&raw)[NG]) {
       const int r = pass * 4 + (lane >> 3);
@@ -607,7 +609,6 @@ __global__ void __launch_bounds__(Kv4Cfg<D, RT>::WARPS * 32, 1) kv4_attn_kernel(
                 const float part = fmaf(pair_scale(kp[e][k]), dot, k == 0 ? 0.0f : s[u][e][q]);
                 s[u][e][q] = fmaf(pair_min(kp[e][k]), qs[q][k], part);
               }
-        
           }
         }
         if constexpr (CAP)
