@@ -495,15 +495,16 @@ def _kv4_geometry(what: str, kv4: torch.Tensor, layer: int) -> tuple[int, int, i
     return index, L, P, nkv, 16 * recs, rec // 18
 
 
-def _kv4_rows(t: torch.Tensor) -> torch.Tensor:
-    """``t`` [tokens, heads, D] if its rows can be read with 16-byte loads, else a copy."""
-    if t.data_ptr() % 16 == 0:
-        if t.is_contiguous():
-            return t
+def _kv4_rows(t: torch.Tensor, heads: int, head_dim: int) -> tuple[torch.Tensor, int, int]:
+    """``t`` [tokens, heads, D] if its rows can be read with 16-byte loads, else a copy; and the elements
+    between tokens and between heads (a dimension of one has any stride, so a dense tensor's are not asked)."""
+    if t.data_ptr() % 16 == 0 and not t.is_contiguous():
         s0, s1, s2 = t.stride()
         if s2 == 1 and s0 % 8 == 0 and s1 % 8 == 0:
-            return t
-    return t.clone(memory_format=torch.contiguous_format)
+            return t, s0, s1
+    if t.data_ptr() % 16 or not t.is_contiguous():
+        t = t.clone(memory_format=torch.contiguous_format)
+    return t, heads * head_dim, head_dim
 
 
 def kv4_write(k: torch.Tensor, v: torch.Tensor, kv4: torch.Tensor, layer: int, slots: torch.Tensor) -> None:
@@ -527,9 +528,7 @@ def kv4_write(k: torch.Tensor, v: torch.Tensor, kv4: torch.Tensor, layer: int, s
         raise RuntimeError(f"{what}: k and v must be {want}, not {tuple(k.shape)} and {tuple(v.shape)}")
     if n == 0:
         return
-    k, v, slots = _kv4_rows(k), _kv4_rows(v), slots.contiguous()
-    k0, k1, _ = k.stride()
-    v0, v1, _ = v.stride()
+    (k, k0, k1), (v, v0, v1), slots = _kv4_rows(k, nkv, D), _kv4_rows(v, nkv, D), slots.contiguous()
     N.on_device(index, what, N.lib().mvb_kv4_write, kv4.data_ptr(), k.data_ptr(), k0, k1, v.data_ptr(), v0, v1,
                 slots.data_ptr(), n, nkv, D, L, int(layer), P, bs)
 

@@ -74,6 +74,23 @@ def test_write_odd_strides_and_views():
     assert torch.equal(gv.cpu(), ref.stored(e.cpu()).float().to(BF))
 
 
+def test_write_dense_rows_under_any_stride():
+    """A dimension of one may have any stride: one token out of a wide row, one head of an odd pitch."""
+    g = gen(6)
+    slots = torch.tensor([17, 5], device=DEV)
+    for tokens, heads in ((1, 2), (1, 1), (2, 1)):
+        base = normal(g, 4 * 128)
+        sizes, dense = (tokens, heads, 128), (heads * 128, 128)
+        strides = [s if n > 1 else 257 for n, s in zip(sizes, dense)] + [1]
+        k, v = base.as_strided(sizes, strides), base.as_strided(sizes, strides, 256)
+        assert k.is_contiguous() and 257 in k.stride()
+        pool = kv4_pool(2, 16, 1, heads, 128)
+        ops.kv4_write(k, v, pool, 0, slots[:tokens])
+        gk, gv = ops.kv4_read(pool, 0, slots[:tokens])
+        assert torch.equal(gk.cpu(), ref.stored(k.cpu()).float().to(BF))
+        assert torch.equal(gv.cpu(), ref.stored(v.cpu()).float().to(BF))
+
+
 def test_write_extreme_values():
     """Constant groups, ties between two codes, tiny and huge values, and NaN and infinity in one group only."""
     pool = kv4_pool(2, 16, 1, 1, 128)
