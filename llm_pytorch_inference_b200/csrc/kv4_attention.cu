@@ -78,16 +78,19 @@ struct Kv4Rows {
   static constexpr bool HALF_K = RT > 1;
 };
 
-// BURST: records that a warp takes at once (one wait, one vote, one refill); STAGES of them are held, so that
-// an SM has some 45 KB or more under way while it computes.  WARPS of the one block per SM: 64 sequences of
+// BURST: records that a warp takes at once (one wait, one refill); STAGES of them are held, so that
+// an SM has some 45 KB or more under way while it computes.  A wait and refill cost some 90 instructions, a record of
+// 24 rows 510: 5 query tokens of 4 sequences of 16K-32K took 70.2 us with bursts of 1, 64.5 with 2, 61.9 with 4; one
+// sequence of 500, which 4 spread over fewer workers, 17.3, 17.6 and 19.0.  WARPS of the one block per SM: 64 sequences of
 // 1024-2048 tokens, 4 rows of 128: 33.3 us with 8, 30.1 with 12, 31.0 with 16 (128 registers); 8 rows: 40.9, 37.6,
 // 44.1 (spills); 4 rows of 256, 16 x 4096-8192: 57, 47.1, 49.1.  16 rows and more of 128 or 256 need over 168
 // registers.  One block, not two: the scheduler prefers the older one, whose warps then ended after 21 us of a
 // call where the other's took 27.
 template <int D, int RT>
 struct Kv4Cfg {
-  static constexpr int BURST = D == 256 || RT > 1 ? 1 : D == 128 ? 2 : RT == 0 ? 4 : 2;
-  static constexpr int STAGES = D == 256 ? (RT > 1 ? 2 : 3) : D == 128 ? (RT > 1 ? 4 : 2) : RT == 0 ? 2 : 4;
+  static constexpr int BURST = D == 256 ? 1 : D == 128 ? (RT > 1 ? 4 : 2) : RT == 0 ? 4 : 2;
+  static constexpr int STAGES = D == 256 ? (RT > 1 ? 2 : 3) : D == 128 ? 2 : RT == 0 ? 2 : RT > 1 ? 3 : 4;
+  static constexpr int MATH = RT > 1 ? 1 : BURST;  // records whose scores are in registers at once
   static constexpr int WARPS = (D == 256 && RT > 0) || (D == 128 && RT > 1) || RT > 2 ? 8 : 12;
 };
 
@@ -272,7 +275,7 @@ __global__ void __launch_bounds__(Kv4Cfg<D, RT>::WARPS * 32, 1) kv4_attn_kernel(
   using S = Kv4Smem<D, RT>;
   using R = Kv4Rows<RT>;
   constexpr int NG = P::NG, STAGES = S::STAGES, ROWS = R::ROWS, NT = R::NT, KT = R::KT, NC = R::NC;
-  constexpr int BURST = Kv4Cfg<D, RT>::BURST, WARPS = Kv4Cfg<D, RT>::WARPS;
+  constexpr int BURST = Kv4Cfg<D, RT>::BURST, MATH = Kv4Cfg<D, RT>::MATH, WARPS = Kv4Cfg<D, RT>::WARPS;
   constexpr unsigned ALL = (1u << BURST) - 1;
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ volatile int abort_flag;
@@ -371,38 +374,47 @@ __global__ void __launch_bounds__(Kv4Cfg<D, RT>::WARPS * 32, 1) kv4_attn_kernel(
     }
     p_t += ask_n;
   };
-  int batch_n = 0, batch_at = 0;  // records of the current batch, the next one to copy
-  unsigned batch_ok = 0;          // those whose block is inside the pool
+  int batch_left = 0, turn = 0;   // records of the current batch still to copy; the lane's own among them
+  unsigned batch_ok = 0;          // those of them whose block is inside the pool
   const uint8_t* batch_src = a.pool;
-  unsigned came = 0, phase = 0;   // per stage: the records that came; parity of its barrier
-  int pending = 0;                // stages whose records are still to be waited for
-  auto issue = [&](int st) {
-    const bool turned = batch_at >= batch_n;
+  unsigned came = 0;              // the records in the ring whose block is, the current stage's lowest
+  int pending = 0;                // stages still to be waited for
+  auto issue = [&](int st, int place) {  // into stage st, `place` stages behind the current one
+    const bool turned = batch_left <= 0;
     if (turned) {
       if (ask_n == 0) return;
-      batch_n = ask_n;
-      batch_at = 0;
+      batch_left = ask_n;
+      turn = lane;
       const bool mine = lane < ask_n, good = mine && static_cast<unsigned>(ask_id) < static_cast<unsigned>(a.num_blocks);
       batch_ok = __ballot_sync(0xffffffffu, good);
       if (mine && !good) report(a.err, kDevBadBlock);
       const int h = a.chunks == 1 ? ask_sub : ask_sub / a.chunks;
       if (good) batch_src = a.pool + ask_id * block_bytes + (static_cast<int64_t>(h) * a.recs + ask_rec) * P::RECORD;
     }
-    const unsigned ok = batch_ok >> batch_at & ALL;
-    came = (came & ~(ALL << (st * BURST))) | ok << (st * BURST);
-    const unsigned turn = static_cast<unsigned>(lane - batch_at);
-    if (ok && turn == 0) mbar_arrive_expect_tx(bars + st, BURST == 1 ? P::RECORD : __popc(ok) * P::RECORD);
-    if constexpr (BURST > 1) __syncwarp();
-    if (turn < BURST && (ok >> turn & 1u))
-      bulk_load(ring + (st * BURST + turn) * P::RECORD, batch_src, P::RECORD, bars + st);
-    batch_at += BURST;
+    const unsigned ok = batch_ok & ALL;
+    batch_ok >>= BURST;
+    came |= ok << (place * BURST);
+    if constexpr (BURST == 1) {
+      if (turn == 0) {
+        mbar_arrive_expect_tx(bars + st, ok * P::RECORD);
+        if (ok) bulk_load(ring + st * P::RECORD, batch_src, P::RECORD, bars + st);
+      }
+    } else {
+      if (turn == 0) mbar_arrive_expect_tx(bars + st, __popc(ok) * P::RECORD);
+      __syncwarp();
+      if (static_cast<unsigned>(turn) < BURST && (ok >> turn & 1u))
+        bulk_load(ring + (st * BURST + turn) * P::RECORD, batch_src, P::RECORD, bars + st);
+    }
+    turn -= BURST;
+    batch_left -= BURST;
     ++pending;
     if (turned) ask();
   };
   ask();
 #pragma unroll 1
-  for (int st = 0; st < STAGES; ++st) issue(st);
+  for (int st = 0; st < STAGES; ++st) issue(st, st);
   int cur = 0;
+  uint32_t parity = 0;  // of the ring's current turn
   bool dead = false;
 
   const int tok0 = tile_token(g), tok1 = tile_token(g + 8);
@@ -505,14 +517,22 @@ __global__ void __launch_bounds__(Kv4Cfg<D, RT>::WARPS * 32, 1) kv4_attn_kernel(
     }
     __syncwarp();
 
-    float f[NC], qs[NC][NG];
+    auto load_f = [&](float (&f)[NC]) {
+#pragma unroll
+      for (int q = 0; q < NC; ++q) f[q] = col_f[row_of(q)];
+    };
+    auto load_qs = [&](float (&qs)[NC][NG]) {
+#pragma unroll
+      for (int q = 0; q < NC; ++q)
+#pragma unroll
+        for (int k = 0; k < NG; ++k) qs[q][k] = col_q[row_of(q) * NG + k];
+    };
+    float f_item[NC], qs_item[NC][NG];
+    if constexpr (!R::HALF_K) load_f(f_item), load_qs(qs_item);
     int see[NC];  // keys that the row sees
 #pragma unroll
     for (int q = 0; q < NC; ++q) {
       const int r = row_of(q);
-      f[q] = col_f[r];
-#pragma unroll
-      for (int k = 0; k < NG; ++k) qs[q][k] = col_q[r * NG + k];
       see[q] = r < rows ? sq.ctx - a.T + 1 + (row0 + r) / a.group : -(1 << 30);
     }
     const int see_least = sq.ctx - a.T + 1 + row0 / a.group;
@@ -542,13 +562,17 @@ __global__ void __launch_bounds__(Kv4Cfg<D, RT>::WARPS * 32, 1) kv4_attn_kernel(
     bool none = true;  // no reference chosen: nothing summed yet
 
     // One burst from record t on, `have`: which of its records came.  MASKED: some row does not see some token.
-    auto burst = [&](auto masked_tag, int t, unsigned have) {
+    auto burst = [&](auto masked_tag, int t, unsigned have, const uint8_t* recs) {
       constexpr bool MASKED = decltype(masked_tag)::value;
-      const uint8_t* recs = ring + cur * (BURST * P::RECORD);
+      asm volatile("" ::: "memory");  // Q is read from shared memory each time: held in registers it would spill
+      float f_own[NC], qs_own[NC][NG];
+      if constexpr (R::HALF_K) load_f(f_own), load_qs(qs_own);
+      const float(&f)[NC] = R::HALF_K ? f_own : f_item;
+      const float(&qs)[NC][NG] = R::HALF_K ? qs_own : qs_item;
       // ---- scores
-      float s[BURST][2][NC];
+      float s[MATH][2][NC];
 #pragma unroll
-      for (int u = 0; u < BURST; ++u) {
+      for (int u = 0; u < MATH; ++u) {
         const uint8_t* rec = recs + u * P::RECORD;
         uint32_t kw[2][2 * NG], kp[2][NG];
 #pragma unroll
@@ -618,10 +642,10 @@ __global__ void __launch_bounds__(Kv4Cfg<D, RT>::WARPS * 32, 1) kv4_attn_kernel(
             for (int q = 0; q < NC; ++q) s[u][e][q] = a.cap_log2 * tanh_exp(s[u][e][q] * f[q]);
       }
       // ---- distance of the scores to their references; the value scales as operands
-      uint32_t vp[BURST][2][NG];
-      unsigned in[BURST] = {};  // bit e * NC + q
+      uint32_t vp[MATH][2][NG];
+      unsigned in[MATH] = {};  // bit e * NC + q
 #pragma unroll
-      for (int u = 0; u < BURST; ++u) {
+      for (int u = 0; u < MATH; ++u) {
         const uint8_t* rec = recs + u * P::RECORD;
 #pragma unroll
         for (int e = 0; e < 2; ++e) load_words(rec + P::V_PAIRS + (e ? tok1 : tok0) * P::PAIRS, vp[u][e]);
@@ -649,10 +673,10 @@ __global__ void __launch_bounds__(Kv4Cfg<D, RT>::WARPS * 32, 1) kv4_attn_kernel(
         const float x = CAP ? s[u][e][q] : s[u][e][q] * f[q];
         return !MASKED || (in[u] >> (e * NC + q) & 1u) ? x : -INFINITY;
       };
-      float d[BURST][2][NC], vs[BURST][2][NG];
+      float d[MATH][2][NC], vs[MATH][2][NG];
       float far = -INFINITY, top = 0.0f;
 #pragma unroll
-      for (int u = 0; u < BURST; ++u)
+      for (int u = 0; u < MATH; ++u)
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
 #pragma unroll
@@ -670,7 +694,7 @@ __global__ void __launch_bounds__(Kv4Cfg<D, RT>::WARPS * 32, 1) kv4_attn_kernel(
       if (__any_sync(0xffffffffu, far > kSlack || top > limit)) {
         float smax = 0.0f;
 #pragma unroll
-        for (int u = 0; u < BURST; ++u)
+        for (int u = 0; u < MATH; ++u)
 #pragma unroll
           for (int k = 0; k < NG; ++k)
 #pragma unroll
@@ -692,7 +716,7 @@ __global__ void __launch_bounds__(Kv4Cfg<D, RT>::WARPS * 32, 1) kv4_attn_kernel(
         for (int q = 0; q < NC; ++q) {
           float m = -INFINITY;
 #pragma unroll
-          for (int u = 0; u < BURST; ++u) m = fmaxf(m, fmaxf(score(u, 0, q), score(u, 1, q)));
+          for (int u = 0; u < MATH; ++u) m = fmaxf(m, fmaxf(score(u, 0, q), score(u, 1, q)));
 #pragma unroll
           for (int off = 4; off < 32; off <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, off));
           m = fmaxf(m, mref[q]);
@@ -710,7 +734,7 @@ __global__ void __launch_bounds__(Kv4Cfg<D, RT>::WARPS * 32, 1) kv4_attn_kernel(
 #pragma unroll
               for (int e = 0; e < 4; ++e) o[k][nt][e] *= fac[RT == 0 ? 0 : (nt * 2 + (e & 1)) % NC] * fo;
 #pragma unroll
-        for (int u = 0; u < BURST; ++u)
+        for (int u = 0; u < MATH; ++u)
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
 #pragma unroll
@@ -721,7 +745,7 @@ __global__ void __launch_bounds__(Kv4Cfg<D, RT>::WARPS * 32, 1) kv4_attn_kernel(
       }
       // ---- weights, and outputs
 #pragma unroll
-      for (int u = 0; u < BURST; ++u) {
+      for (int u = 0; u < MATH; ++u) {
         const uint8_t* rec = recs + u * P::RECORD;
         uint32_t vw[4][NG];
 #pragma unroll
@@ -791,28 +815,27 @@ __global__ void __launch_bounds__(Kv4Cfg<D, RT>::WARPS * 32, 1) kv4_attn_kernel(
     // bursts that start in [t_low, t_high] hold no token that some row does not see
     const int t_low = a.window > 0 ? max(see_most - a.window + kKv4Tokens - 1, 0) / kKv4Tokens : 0;
     const int t_high = max(see_least, 0) / kKv4Tokens - BURST;
-    for (int t = span.x; t < span.y && !dead; t += BURST) {
-      const unsigned have = came >> (cur * BURST) & ALL;
-      if (have) {  // else no such blocks: their tokens count as masked
-        const uint32_t parity = phase >> cur & 1u;
-        bool ok = mbar_try_wait(smem_u32(bars + cur), parity);
-        if (!ok) ok = wait_slow(bars + cur, parity, &abort_flag, a.err);
-        if (!__all_sync(0xffffffffu, ok)) {
-          dead = true;
-          break;
-        }
-        phase ^= 1u << cur;
-        if (have != ALL || t > t_high || t < t_low)
-          burst(std::true_type{}, t, have);
-        else
-          burst(std::false_type{}, t, have);
+    for (int t = dead ? span.y : span.x; t < span.y; t += BURST) {  // given up: the items still get an entry
+      if (!__all_sync(0xffffffffu, mbar_try_wait(smem_u32(bars + cur), parity)) &&
+          !__all_sync(0xffffffffu, wait_slow(bars + cur, parity, &abort_flag, a.err))) {
+        dead = true;
+        break;
+      }
+      const unsigned have = came & ALL;
+      const uint8_t* recs = ring + cur * (BURST * P::RECORD);
+      if (have == ALL && t >= t_low && t <= t_high) {
+#pragma unroll 1
+        for (int x = 0; x < BURST; x += MATH) burst(std::false_type{}, t + x, ALL, recs + x * P::RECORD);
+      } else if (have) {  // else no such blocks: their tokens count as masked
+#pragma unroll 1
+        for (int x = 0; x < BURST; x += MATH) burst(std::true_type{}, t + x, have >> x, recs + x * P::RECORD);
       }
       __syncwarp();
+      came >>= BURST;
       --pending;
-      issue(cur);
-      cur = cur + 1 == STAGES ? 0 : cur + 1;
+      issue(cur, STAGES - 1);
+      if (++cur == STAGES) cur = 0, parity ^= 1u;
     }
-
     // ---- the item's result, or this worker's part of it
 #pragma unroll
     for (int q = 0; q < NC; ++q) {
@@ -871,8 +894,10 @@ __global__ void __launch_bounds__(Kv4Cfg<D, RT>::WARPS * 32, 1) kv4_attn_kernel(
   }
   // a stream that was given up: its copies land before the block's shared memory goes
   if (dead)
-    for (int st = cur; pending > 0; --pending, st = st + 1 == STAGES ? 0 : st + 1)
-      if (came >> (st * BURST) & ALL) mbar_wait(bars + st, phase >> st & 1u, nullptr, a.err);
+    for (; pending > 0; --pending) {
+      mbar_wait(bars + cur, parity, nullptr, a.err);
+      if (++cur == STAGES) cur = 0, parity ^= 1u;
+    }
 }
 
 // Adds parts p0, p0 + STEP, .. up to the last of row r of an item to (m, l, o), AHEAD of them under way at once.
