@@ -259,12 +259,12 @@ __device__ __forceinline__ int2 kv4_records(const Kv4AttnArgs& a, const Kv4Seq& 
 template <int D, int RT>
 struct Kv4Smem {
   static constexpr int STAGES = Kv4Cfg<D, RT>::STAGES, ROWS = Kv4Rows<RT>::ROWS;
-  // per warp: the ring, Q operands [D / 32][KT][32 lanes] x 8 bytes, per row the score factor and the
-  // sums of q per group, the ring's barriers
+  // per warp: the ring, Q operands [D / 32][KT][32 lanes] x 8 bytes, per row the score factor, the
+  // sums of q per group and the number of keys it sees, the ring's barriers
   static constexpr int RING = STAGES * Kv4Cfg<D, RT>::BURST * Kv4<D>::RECORD;
   static constexpr int QF = RING;
   static constexpr int COL = QF + D / 32 * Kv4Rows<RT>::KT * 256;
-  static constexpr int BAR = (COL + ROWS * (1 + Kv4<D>::NG) * 4 + 7) / 8 * 8;
+  static constexpr int BAR = (COL + ROWS * (2 + Kv4<D>::NG) * 4 + 7) / 8 * 8;
   static constexpr int WARP = (BAR + STAGES * 8 + 127) / 128 * 128;
   static constexpr int BYTES = Kv4Cfg<D, RT>::WARPS * WARP;
 };
@@ -286,6 +286,7 @@ __global__ void __launch_bounds__(Kv4Cfg<D, RT>::WARPS * 32, 1) kv4_attn_kernel(
   uint2* qf = reinterpret_cast<uint2*>(ring + S::QF);
   float* col_f = reinterpret_cast<float*>(ring + S::COL);
   float* col_q = col_f + ROWS;  // [ROWS][NG]
+  int* col_see = reinterpret_cast<int*>(col_q + ROWS * NG);
   uint64_t* bars = reinterpret_cast<uint64_t*>(ring + S::BAR);
 
   pdl_launch_dependents();
@@ -410,7 +411,26 @@ __global__ void __launch_bounds__(Kv4Cfg<D, RT>::WARPS * 32, 1) kv4_attn_kernel(
     ++pending;
     if (turned) ask();
   };
+  // ---- Q, four rows at a time, eight lanes each; TAKE such passes under way at once, the first ones before any
+  // copy, behind which they would wait
+  constexpr int PASSES = ROWS / 4, TAKE = RT == 3 ? 3 : RT == 0 ? 1 : 2;
+  uint4 raw_q[TAKE][NG];
+  auto load_rows = [&](int pass) {
+    const int h = a.chunks == 1 ? sub : sub / a.chunks, row0 = (sub - h * a.chunks) * ROWS;
+#pragma unroll
+    for (int x = 0; x < TAKE; ++x) {
+      const int r = row0 + (pass + x) * 4 + (lane >> 3);
+      const int i = r / a.group, hq = h * a.group + r - i * a.group;
+      const __nv_bfloat16* src = a.q + (static_cast<int64_t>(seq) * a.T + i) * a.q_stride +
+                                 static_cast<int64_t>(hq) * D + 8 * (lane & 7);
+      const bool there = r < min(row0 + ROWS, a.group * a.T);
+#pragma unroll
+      for (int k = 0; k < NG; ++k)
+        raw_q[x][k] = there ? *reinterpret_cast<const uint4*>(src + 64 * k) : make_uint4(0u, 0u, 0u, 0u);
+    }
+  };
   ask();
+  load_rows(0);
 #pragma unroll 1
   for (int st = 0; st < STAGES; ++st) issue(st, st);
   int cur = 0;
@@ -431,88 +451,79 @@ __global__ void __launch_bounds__(Kv4Cfg<D, RT>::WARPS * 32, 1) kv4_attn_kernel(
     const int rows = min(a.group * a.T - row0, ROWS);
     const int2 span = kv4_records<BURST>(a, sq, ra, n_rounds);
 
-    // Q of the item, four rows at a time, eight lanes each, in the order of the first product's operands:
-    // round(32512 q / max |q|) = 256 hi + lo as signed bytes, or fp16
+    // Q of the item in the order of the first product's operands: round(32512 q / max |q|) = 256 hi + lo as signed
+    // bytes, or fp16
     __syncwarp();
-    auto load_rows = [&](int pass, uint4 (&raw)[NG]) {
-      const int r = pass * 4 + (lane >> 3);
-      const int i = (row0 + r) / a.group, hq = h * a.group + (row0 + r) - i * a.group;
-      const __nv_bfloat16* src = a.q + (static_cast<int64_t>(seq) * a.T + i) * a.q_stride +
-                                 static_cast<int64_t>(hq) * D + 8 * (lane & 7);
-#pragma unroll
-      for (int k = 0; k < NG; ++k)
-        raw[k] = r < rows ? *reinterpret_cast<const uint4*>(src + 64 * k) : make_uint4(0u, 0u, 0u, 0u);
-    };
-    uint4 next[NG];
-    load_rows(0, next);
 #pragma unroll 1
-    for (int pass = 0; pass < ROWS / 4 && span.x < span.y; ++pass) {
-      const int r = pass * 4 + (lane >> 3), w = lane & 7;
-      uint4 raw[NG];
+    for (int pass0 = 0; pass0 < PASSES && span.x < span.y; pass0 += TAKE) {
+      if (pass0 > 0) load_rows(pass0);
 #pragma unroll
-      for (int k = 0; k < NG; ++k) raw[k] = next[k];
-      if (pass + 1 < ROWS / 4) load_rows(pass + 1, next);
-      uint32_t big = 0;  // bits of the largest magnitude: ordered as integers, NaN and infinity on top
-#pragma unroll
-      for (int k = 0; k < NG; ++k) {
-        const uint32_t x[4] = {raw[k].x, raw[k].y, raw[k].z, raw[k].w};
-#pragma unroll
-        for (int j = 0; j < 4; ++j) big = max(big, max((x[j] << 16) & 0x7fffffffu, x[j] & 0x7fff0000u));
-      }
-#pragma unroll
-      for (int o = 1; o < 8; o <<= 1) big = max(big, __shfl_xor_sync(0xffffffffu, big, o));
-      const bool fine = big < 0x7f800000u;
-      if constexpr (R::HALF_K) {
-        // times a power of two that puts the largest magnitude into [2^10, 2^11): exact in fp16 but for what lies
-        // 2^-25 below that
-        const int e = big > 0 && fine ? min(max(137 - static_cast<int>(big >> 23), -126), 126) : 0;
-        const float up = __uint_as_float(static_cast<uint32_t>(e + 127) << 23);
+      for (int x = 0; x < TAKE; ++x) {
+        const int r = (pass0 + x) * 4 + (lane >> 3), w = lane & 7;
+        const uint4(&raw)[NG] = raw_q[x];
+        if (w == 0) col_see[r] = r < rows ? sq.ctx - a.T + 1 + (row0 + r) / a.group : -(1 << 30);
+        uint32_t big = 0;  // bits of the largest magnitude: ordered as integers, NaN and infinity on top
 #pragma unroll
         for (int k = 0; k < NG; ++k) {
           const uint32_t x[4] = {raw[k].x, raw[k].y, raw[k].z, raw[k].w};
-          float v[8], sum = 0.0f;
 #pragma unroll
-          for (int j = 0; j < 8; ++j) {
-            v[j] = fine ? __uint_as_float((j & 1) ? x[j >> 1] & 0xffff0000u : x[j >> 1] << 16) * up : 0.0f;
-            sum += v[j];
-          }
-          // word w of the group is word w % 2 of lane w / 2; codes 2 h and 2 h + 4 are the first operand of half h,
-          // 2 h + 1 and 2 h + 5 the second, which stands 4 bits higher
-#pragma unroll
-          for (int hh = 0; hh < 2; ++hh)
-            qf[(((k * 2 + (w & 1)) * 2 + hh) * NT + r / 8) * 32 + (r % 8) * 4 + (w >> 1)] =
-                make_uint2(pack_f16(v[2 * hh] * 16.0f, v[2 * hh + 4] * 16.0f), pack_f16(v[2 * hh + 1], v[2 * hh + 5]));
-#pragma unroll
-          for (int o = 1; o < 8; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-          if (w == 0) col_q[r * NG + k] = sum * 0x1p-20f;
+          for (int j = 0; j < 4; ++j) big = max(big, max((x[j] << 16) & 0x7fffffffu, x[j] & 0x7fff0000u));
         }
-        if (w == 0) col_f[r] = !fine ? __int_as_float(0x7fc00000) : ldexpf(a.score_scale, 20 - e);
-      } else {
-        const float up = big > 0 && fine ? fminf(32512.0f / __uint_as_float(big), 1e38f) : 0.0f;
-        const int n0 = RT == 0 ? 2 * r : r % 8, t0 = RT == 0 ? 0 : 2 * (r / 8);
-        const int n1 = RT == 0 ? 2 * r + 1 : r % 8, t1 = RT == 0 ? 0 : t0 + 1;
 #pragma unroll
-        for (int k = 0; k < NG; ++k) {
-          const uint32_t x[4] = {raw[k].x, raw[k].y, raw[k].z, raw[k].w};
-          // word w of the group is word w % 2 of lane w / 2; its even codes are the first operand, the odd ones the second
-          uint32_t hi[2] = {0, 0}, lo[2] = {0, 0};
-          int sum = 0;
+        for (int o = 1; o < 8; o <<= 1) big = max(big, __shfl_xor_sync(0xffffffffu, big, o));
+        const bool fine = big < 0x7f800000u;
+        if constexpr (R::HALF_K) {
+          // times a power of two that puts the largest magnitude into [2^10, 2^11): exact in fp16 but for what lies
+          // 2^-25 below that
+          const int e = big > 0 && fine ? min(max(137 - static_cast<int>(big >> 23), -126), 126) : 0;
+          const float up = __uint_as_float(static_cast<uint32_t>(e + 127) << 23);
 #pragma unroll
-          for (int j = 0; j < 8; ++j) {
-            const float xv = __uint_as_float((j & 1) ? x[j >> 1] & 0xffff0000u : x[j >> 1] << 16);
-            const int v = fine ? __float2int_rn(xv * up) : 0, vh = (v + 128) >> 8;
-            sum += v;
-            hi[j & 1] |= (static_cast<uint32_t>(vh) & 255u) << (8 * (j >> 1));
-            lo[j & 1] |= (static_cast<uint32_t>(v) & 255u) << (8 * (j >> 1));  // v - 256 vh in its low byte
+          for (int k = 0; k < NG; ++k) {
+            const uint32_t x[4] = {raw[k].x, raw[k].y, raw[k].z, raw[k].w};
+            float v[8], sum = 0.0f;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+              v[j] = fine ? __uint_as_float((j & 1) ? x[j >> 1] & 0xffff0000u : x[j >> 1] << 16) * up : 0.0f;
+              sum += v[j];
+            }
+            // word w of the group is word w % 2 of lane w / 2; codes 2 h and 2 h + 4 are the first operand of half h,
+            // 2 h + 1 and 2 h + 5 the second, which stands 4 bits higher
+#pragma unroll
+            for (int hh = 0; hh < 2; ++hh)
+              qf[(((k * 2 + (w & 1)) * 2 + hh) * NT + r / 8) * 32 + (r % 8) * 4 + (w >> 1)] =
+                  make_uint2(pack_f16(v[2 * hh] * 16.0f, v[2 * hh + 4] * 16.0f), pack_f16(v[2 * hh + 1], v[2 * hh + 5]));
+#pragma unroll
+            for (int o = 1; o < 8; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+            if (w == 0) col_q[r * NG + k] = sum * 0x1p-20f;
           }
-          const int ks = k * 2 + (w & 1);
-          qf[(ks * KT + t0) * 32 + n0 * 4 + (w >> 1)] = make_uint2(hi[0], hi[1]);
-          qf[(ks * KT + t1) * 32 + n1 * 4 + (w >> 1)] = make_uint2(lo[0], lo[1]);
+          if (w == 0) col_f[r] = !fine ? __int_as_float(0x7fc00000) : ldexpf(a.score_scale, 20 - e);
+        } else {
+          const float up = big > 0 && fine ? fminf(32512.0f / __uint_as_float(big), 1e38f) : 0.0f;
+          const int n0 = RT == 0 ? 2 * r : r % 8, t0 = RT == 0 ? 0 : 2 * (r / 8);
+          const int n1 = RT == 0 ? 2 * r + 1 : r % 8, t1 = RT == 0 ? 0 : t0 + 1;
 #pragma unroll
-          for (int o = 1; o < 8; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-          if (w == 0) col_q[r * NG + k] = static_cast<float>(sum);
+          for (int k = 0; k < NG; ++k) {
+            const uint32_t x[4] = {raw[k].x, raw[k].y, raw[k].z, raw[k].w};
+            // word w of the group is word w % 2 of lane w / 2; its even codes are the first operand, the odd ones the second
+            uint32_t hi[2] = {0, 0}, lo[2] = {0, 0};
+            int sum = 0;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+              const float xv = __uint_as_float((j & 1) ? x[j >> 1] & 0xffff0000u : x[j >> 1] << 16);
+              const int v = fine ? __float2int_rn(xv * up) : 0, vh = (v + 128) >> 8;
+              sum += v;
+              hi[j & 1] |= (static_cast<uint32_t>(vh) & 255u) << (8 * (j >> 1));
+              lo[j & 1] |= (static_cast<uint32_t>(v) & 255u) << (8 * (j >> 1));  // v - 256 vh in its low byte
+            }
+            const int ks = k * 2 + (w & 1);
+            qf[(ks * KT + t0) * 32 + n0 * 4 + (w >> 1)] = make_uint2(hi[0], hi[1]);
+            qf[(ks * KT + t1) * 32 + n1 * 4 + (w >> 1)] = make_uint2(lo[0], lo[1]);
+#pragma unroll
+            for (int o = 1; o < 8; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+            if (w == 0) col_q[r * NG + k] = static_cast<float>(sum);
+          }
+          if (w == 0) col_f[r] = !fine ? __int_as_float(0x7fc00000) : up > 0.0f ? a.score_scale / up : 0.0f;
         }
-        if (w == 0) col_f[r] = !fine ? __int_as_float(0x7fc00000) : up > 0.0f ? a.score_scale / up : 0.0f;
       }
     }
     __syncwarp();
@@ -529,14 +540,7 @@ __global__ void __launch_bounds__(Kv4Cfg<D, RT>::WARPS * 32, 1) kv4_attn_kernel(
     };
     float f_item[NC], qs_item[NC][NG];
     if constexpr (!R::HALF_K) load_f(f_item), load_qs(qs_item);
-    int see[NC];  // keys that the row sees
-#pragma unroll
-    for (int q = 0; q < NC; ++q) {
-      const int r = row_of(q);
-      see[q] = r < rows ? sq.ctx - a.T + 1 + (row0 + r) / a.group : -(1 << 30);
-    }
-    const int see_least = sq.ctx - a.T + 1 + row0 / a.group;
-    const int see_most = sq.ctx - a.T + 1 + (row0 + rows - 1) / a.group;
+    const int see_least = col_see[0], see_most = col_see[rows - 1];  // keys that the first and the last row see
 
     // m tiles of 16 x 8 outputs.  RT > 0: (group, high half of the word, half of that), 16 channels x 8 rows each;
     // RT = 0: (group, half of a half word), 32 channels x 4 rows
@@ -650,6 +654,9 @@ __global__ void __launch_bounds__(Kv4Cfg<D, RT>::WARPS * 32, 1) kv4_attn_kernel(
 #pragma unroll
         for (int e = 0; e < 2; ++e) load_words(rec + P::V_PAIRS + (e ? tok1 : tok0) * P::PAIRS, vp[u][e]);
         if constexpr (MASKED) {
+          int see[NC];
+#pragma unroll
+          for (int q = 0; q < NC; ++q) see[q] = col_see[row_of(q)];
           const int low = a.window > 0 ? see_least - a.window : 0;
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
@@ -886,11 +893,13 @@ __global__ void __launch_bounds__(Kv4Cfg<D, RT>::WARPS * 32, 1) kv4_attn_kernel(
       }
     }
     left -= n_rounds;
+    if (left <= 0) break;
     ra = 0;
-    if (++sub == subs && left > 0) {
+    if (++sub == subs) {
       sub = 0;
       sq = kv4_seq<BURST>(a, ++seq);
     }
+    load_rows(0);
   }
   // a stream that was given up: its copies land before the block's shared memory goes
   if (dead)
