@@ -372,7 +372,10 @@ extern "C" int mvb_assign_slots(int64_t* slots, int32_t* positions, int32_t* seq
   const dim3 blocks(static_cast<unsigned>(grid)), threads(kThreads);
   if (batch <= kMaxShared) {
     const size_t smem = (2 * batch + 1) * sizeof(int32_t);
-    if (smem > 48 * 1024) MVB_TRY(set_smem(assign_slots_kernel, smem, "assign_slots"));
+    // past 48 KB together with the kernel's static arrays a launch has to be allowed for: once, for the largest batch
+    static std::atomic<uint64_t> done{0};
+    if (smem > 40 * 1024)
+      MVB_TRY(set_smem_once(done, assign_slots_kernel, (2 * kMaxShared + 1) * sizeof(int32_t), "assign_slots"));
     return launch("assign_slots", assign_slots_kernel, blocks, threads, smem, st, a);
   }
   MVB_REQUIRE(workspace && aligned(workspace, 8) && workspace_bytes >= mvb_assign_slots_workspace_bytes(batch),

@@ -58,6 +58,13 @@ def test_slots(batch, most, bs):
     run_slots(tables, ctx, new, ids, bs, sum(new), head=5)
 
 
+@pytest.mark.parametrize("batch", [5119, 5120, 6100, 6111, 6120, 6143, 6144, 8191])
+def test_slots_around_the_default_shared_memory(batch):
+    """Lengths held in shared memory up to and past 48 KB, the kernel's own arrays beside them."""
+    run_slots([[b, -1] for b in range(batch)], [b % 17 for b in range(batch)], [b % 3 for b in range(batch)],
+              list(range(batch, 3 * batch)), 16, 3 * batch)
+
+
 @pytest.mark.parametrize("seed", range(6))
 def test_slots_that_do_not_fit(seed):
     """Short of blocks, of table entries, or of room in the outputs: refused one by one, later ones served."""
