@@ -9,13 +9,16 @@
 //
 // Both should be bound by memory: 2 bytes a value on the bf16 side, 9/16 on the other.  A lane owns 8 channels of
 // K and of V of a token, for one head or two (HEADS): a 16-byte load (or store) of bf16 and one 32-bit word of
-// codes each, all under way together and with one look at the token's slot.  Eight lanes share a group and
-// find its minimum and maximum, on packed bf16, with three exchanges.  That leaves writing some 6 instructions a
-// value before arithmetic costs more than memory, so a quotient is a product and its correction, added to
-// 1.5 * 2^23, which rounds it to even and leaves the code in the low bits, and a multiply-add puts it into the word.
-// Measured on a B200, K and V of 8 heads of 128: writing 16,384 tokens takes 25 us for 86 MB (3.4 TB/s, bound by
-// issued instructions: 5 a value); with IEEE divisions it took 57.  64 tokens: 2.2 us.
-// Reading 32,768 tokens: 30.0 us for 172 MB (5.7 TB/s, copying reaches 6.55).
+// codes each, all under way together and with one look at the token's slot.  Eight lanes share a group.  Its minimum
+// and maximum, on packed bf16, are exchanged so that each lane ends up with one of the 2 to 8 groups, works out that
+// group's pair alone and hands it round.  Writing is bound by issued instructions all the same, so a quotient is a
+// product and its correction, two values to an instruction, added to 1.5 * 2^23, which rounds it to even and leaves the
+// code in the low bits, and a multiply-add puts it into the word.
+// Measured on a B200, K and V of 8 heads of 128: writing 16,384 tokens takes 18.0 us for 86 MB (4.8 TB/s); with every
+// lane working out all pairs, values one by one, it took 25, with IEEE divisions 57.  64 tokens: 1.9 us.
+// Reading 16,384 tokens: 13.7 us (6.3 TB/s, copying reaches 6.55); 32,768: 29.7 us.
+#include <type_traits>
+
 #include "common.cuh"
 #include "host.h"
 #include "kv4.cuh"
@@ -23,7 +26,7 @@
 namespace mvb {
 namespace {
 
-constexpr int kThreads = 256;
+constexpr int kThreads = 128;  // 64 and 256 took 37.4 and 34.2 us where 128 took 31.6 (the calls at MVB_KV4_LAUNCH)
 
 struct Kv4Args {
   uint8_t* pool;          // the layer's first record
@@ -68,25 +71,55 @@ __device__ __forceinline__ float divided(float x, float d, float y) {
 
 constexpr float kTiny = 0x1p-90f;  // magnitudes from here on are away from underflow
 
-// Codes of 8 values of a group with minimum `low` and scale `scale` > 0, lowest nibble first.
-__device__ __forceinline__ uint32_t quantise8(const uint32_t (&x)[4], float low, float scale) {
+// Two fp32 numbers to an instruction (the lower one first), each rounded as by its own.
+__device__ __forceinline__ uint64_t two(float a, float b) {
+  uint64_t d;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "f"(a), "f"(b));
+  return d;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+  return d;
+}
+
+__device__ __forceinline__ float bf16_low(uint32_t x) { return __uint_as_float(x << 16); }
+__device__ __forceinline__ float bf16_high(uint32_t x) { return __uint_as_float(x & 0xffff0000u); }
+
+// Codes of 8 values of a group with minimum `low` and scale `scale`, lowest nibble first; inv = RN(1 / scale) where
+// scale >= kTiny, which PLAIN says of every group of the warp.
+template <bool PLAIN>
+__device__ __forceinline__ uint32_t quantise8(const uint32_t (&x)[4], float low, float scale, float inv) {
   uint32_t word = 0;
-  if (scale < kTiny) {  // a subnormal scale may leave the largest code above 15
-#pragma unroll 1
-    for (int j = 7; j >= 0; --j) {
-      const uint32_t h = j >= 6 ? x[3] : j >= 4 ? x[2] : j >= 2 ? x[1] : x[0];
-      const float v = __uint_as_float((j & 1) ? (h & 0xffff0000u) : (h << 16)) - low;
-      word = word * 16u + static_cast<uint32_t>(fminf(rintf(__fdiv_rn(v, scale)), 15.0f));
-    }
-    return word;
-  }
-  const float inv = __frcp_rn(scale);
+  if (PLAIN || scale >= kTiny) {
+    const uint64_t low2 = two(-low, -low), scale2 = two(-scale, -scale), inv2 = two(inv, inv);
+    const uint64_t magic2 = two(kMagic, kMagic);
 #pragma unroll
-  for (int j = 7; j >= 0; --j) {
-    const float v = __uint_as_float((j & 1) ? (x[j >> 1] & 0xffff0000u) : (x[j >> 1] << 16)) - low;
-    word = word * 16u + __float_as_uint(divided(v, scale, inv) + kMagic);  // at most 15: scale is within 2^-9
+    for (int j = 3; j >= 0; --j) {  // `divided`, two at a time
+      const uint64_t v = add2(two(bf16_low(x[j]), bf16_high(x[j])), low2), q = mul2(v, inv2);
+      const uint64_t u = add2(fma2(fma2(scale2, q, v), inv2, q), magic2);  // at most 15: scale is within 2^-9
+      word = (word * 16u + static_cast<uint32_t>(u >> 32)) * 16u + static_cast<uint32_t>(u);
+    }
+    return word - kPackBias;
   }
-  return word - kPackBias;
+  if (!(scale > 0.0f)) return 0u;  // one value throughout, or none that is a number
+#pragma unroll 1
+  for (int j = 7; j >= 0; --j) {  // a subnormal scale may leave the largest code above 15
+    const uint32_t h = j >= 6 ? x[3] : j >= 4 ? x[2] : j >= 2 ? x[1] : x[0];
+    const float v = ((j & 1) ? bf16_high(h) : bf16_low(h)) - low;
+    word = word * 16u + static_cast<uint32_t>(fminf(rintf(__fdiv_rn(v, scale)), 15.0f));
+  }
+  return word;
 }
 
 // A lane per (token, HEADS heads, 8 channels).
@@ -94,7 +127,7 @@ template <int D, int HEADS>
 __global__ void __launch_bounds__(kThreads) kv4_write_kernel(const Kv4Args a, const __nv_bfloat16* __restrict__ k,
                                                              const __nv_bfloat16* __restrict__ v) {
   using P = Kv4<D>;
-  constexpr int LANES = D / 8, N = 2 * HEADS;
+  constexpr int LANES = D / 8, N = 2 * HEADS;  // N groups: K and V of each head
   pdl_launch_dependents();
   pdl_wait();
   const uint32_t x0 = blockIdx.x * kThreads + threadIdx.x;
@@ -121,8 +154,8 @@ __global__ void __launch_bounds__(kThreads) kv4_write_kernel(const Kv4Args a, co
       vs += a.v_head_stride;
     }
   }
-  uint8_t* at = a.pool + (rec + static_cast<int64_t>(head) * a.recs) * P::RECORD + row * P::ROW + 4 * (P::NG * w + g);
-  const int pair_at = P::K_PAIRS + row * P::PAIRS + 4 * g - (row * P::ROW + 4 * (P::NG * w + g));
+  // (minimum, -maximum) of the lane's values of each group, in one word
+  uint32_t ext[N];
 #pragma unroll
   for (int i = 0; i < N; ++i) {
     const uint32_t x[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
@@ -132,23 +165,49 @@ __global__ void __launch_bounds__(kThreads) kv4_write_kernel(const Kv4Args a, co
       lo2 = __hmin2_nan(lo2, as_bf162(x[j]));
       hi2 = __hmax2_nan(hi2, as_bf162(x[j]));
     }
-    // both halves' results in one word for the exchanges: (minimum, -maximum)
-    __nv_bfloat162 m2 = __halves2bfloat162(__hmin_nan(lo2.x, lo2.y), __hneg(__hmax_nan(hi2.x, hi2.y)));
-#pragma unroll
-    for (int o = 1; o < 8; o <<= 1) m2 = __hmin2_nan(m2, as_bf162(__shfl_xor_sync(0xffffffffu, as_u32(m2), o)));
-    if (!live) continue;
-    float low = __bfloat162float(m2.x);
-    const float span = -__bfloat162float(m2.y) - low;
-    float scale = bf16_round(span < kTiny ? __fdiv_rn(span, 15.0f) : divided(span, 15.0f, 1.0f / 15.0f));
-    uint32_t word = 0;
-    if (!(scale <= kFltMax) || !(fabsf(low) <= kFltMax)) scale = low = __int_as_float(0x7fc00000);
-    else if (scale > 0.0f) word = quantise8(x, low, scale);
-    *reinterpret_cast<uint32_t*>(at + ((i & 1) ? P::V_CODES : 0)) = word;
-    if (w == 0)
-      *reinterpret_cast<__nv_bfloat162*>(at + pair_at + ((i & 1) ? P::V_PAIRS - P::K_PAIRS : 0)) =
-          __floats2bfloat162_rn(scale, low);
-    if (i & 1) at += a.recs * P::RECORD;
+    ext[i] = as_u32(__halves2bfloat162(__hmin_nan(lo2.x, lo2.y), __hneg(__hmax_nan(hi2.x, hi2.y))));
   }
+  // Exchanged among the eight lanes so that lane w ends up with group w % N: half of the groups are handed over at a
+  // time.  That group's pair is this lane's work; all read it afterwards.
+  auto least = [](uint32_t x, uint32_t y) { return as_u32(__hmin2_nan(as_bf162(x), as_bf162(y))); };
+#pragma unroll
+  for (int o = 1; o < N; o <<= 1) {
+    const bool odd = w & o;
+#pragma unroll
+    for (int i = 0; i < N / 2 / o; ++i) {  // those left: numbers i and i + 1 differ in bit o of the group
+      const uint32_t keep = odd ? ext[2 * i + 1] : ext[2 * i], give = odd ? ext[2 * i] : ext[2 * i + 1];
+      ext[i] = least(keep, __shfl_xor_sync(0xffffffffu, give, o));
+    }
+  }
+#pragma unroll
+  for (int o = N; o < 8; o <<= 1) ext[0] = least(ext[0], __shfl_xor_sync(0xffffffffu, ext[0], o));
+  float low = bf16_low(ext[0]);
+  const float span = -bf16_high(ext[0]) - low;
+  float scale = bf16_round(span < kTiny ? __fdiv_rn(span, 15.0f) : divided(span, 15.0f, 1.0f / 15.0f));
+  if (!(scale <= kFltMax) || !(fabsf(low) <= kFltMax)) scale = low = __int_as_float(0x7fc00000);
+  const float inv = __frcp_rn(scale);
+  const uint32_t pair = as_u32(__floats2bfloat162_rn(scale, low));
+
+  uint8_t* at = a.pool + (rec + static_cast<int64_t>(head) * a.recs) * P::RECORD;
+  if (live && w < N)
+    *reinterpret_cast<uint32_t*>(at + (w >> 1) * a.recs * P::RECORD + ((w & 1) ? P::V_PAIRS : P::K_PAIRS) +
+                                 row * P::PAIRS + 4 * g) = pair;
+  at += row * P::ROW + 4 * (P::NG * w + g);
+  auto store = [&](auto plain_tag) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int from = (threadIdx.x & 24) | i;
+      const uint32_t pi = __shfl_sync(0xffffffffu, pair, from);
+      const float inv_i = __shfl_sync(0xffffffffu, inv, from);
+      const uint32_t x[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
+      const uint32_t word = quantise8<decltype(plain_tag)::value>(x, bf16_high(pi), bf16_low(pi), inv_i);
+      if (live) *reinterpret_cast<uint32_t*>(at + (i >> 1) * a.recs * P::RECORD + ((i & 1) ? P::V_CODES : 0)) = word;
+    }
+  };
+  if (__all_sync(0xffffffffu, scale >= kTiny))  // no branch a group: 33.4 -> 32.5 us at head size 256
+    store(std::true_type{});
+  else
+    store(std::false_type{});
 }
 
 // A lane per (token, HEADS heads, 8 channels).  A token without a slot in the pool reads as zeros.  A code is
@@ -237,19 +296,23 @@ int stride_ok(const char* what, const void* p, int64_t stride, int64_t head_stri
 
 using namespace mvb;
 
-// Two heads a lane where they come in pairs and there are lanes enough to fill the GPU all the same.
+// Two or four heads a lane where they come in such numbers and there are lanes enough to fill the GPU all the same.
+// Writing and reading 16,384 tokens, K and V of 8 heads of 128: 34.0 us with two, 31.6 with four.
 #define MVB_KV4_LAUNCH(NAME, KERNEL, ...)                                                                 \
   do {                                                                                                    \
     const int64_t lanes = tokens * num_kv_heads * (head_dim / 8);                                         \
-    const bool two = num_kv_heads % 2 == 0 && lanes >= (1 << 18);                                         \
-    dim3 grid(static_cast<unsigned>(((two ? lanes / 2 : lanes) + kThreads - 1) / kThreads)), block(kThreads); \
-    switch (head_dim + two) {                                                                             \
-      case 64: return launch(NAME, KERNEL<64, 1>, grid, block, 0, st, a, __VA_ARGS__);                    \
-      case 65: return launch(NAME, KERNEL<64, 2>, grid, block, 0, st, a, __VA_ARGS__);                    \
-      case 128: return launch(NAME, KERNEL<128, 1>, grid, block, 0, st, a, __VA_ARGS__);                  \
-      case 129: return launch(NAME, KERNEL<128, 2>, grid, block, 0, st, a, __VA_ARGS__);                  \
-      case 256: return launch(NAME, KERNEL<256, 1>, grid, block, 0, st, a, __VA_ARGS__);                  \
-      default: return launch(NAME, KERNEL<256, 2>, grid, block, 0, st, a, __VA_ARGS__);                   \
+    const int each = lanes < (1 << 18) || num_kv_heads % 2 ? 1 : lanes < (1 << 19) || num_kv_heads % 4 ? 2 : 4; \
+    const dim3 grid(static_cast<unsigned>((lanes / each + kThreads - 1) / kThreads)), block(kThreads);    \
+    switch (head_dim + each) {                                                                            \
+      case 65: return launch(NAME, KERNEL<64, 1>, grid, block, 0, st, a, __VA_ARGS__);                    \
+      case 66: return launch(NAME, KERNEL<64, 2>, grid, block, 0, st, a, __VA_ARGS__);                    \
+      case 68: return launch(NAME, KERNEL<64, 4>, grid, block, 0, st, a, __VA_ARGS__);                    \
+      case 129: return launch(NAME, KERNEL<128, 1>, grid, block, 0, st, a, __VA_ARGS__);                  \
+      case 130: return launch(NAME, KERNEL<128, 2>, grid, block, 0, st, a, __VA_ARGS__);                  \
+      case 132: return launch(NAME, KERNEL<128, 4>, grid, block, 0, st, a, __VA_ARGS__);                  \
+      case 257: return launch(NAME, KERNEL<256, 1>, grid, block, 0, st, a, __VA_ARGS__);                  \
+      case 258: return launch(NAME, KERNEL<256, 2>, grid, block, 0, st, a, __VA_ARGS__);                  \
+      default: return launch(NAME, KERNEL<256, 4>, grid, block, 0, st, a, __VA_ARGS__);                   \
     }                                                                                                     \
   } while (0)
 

@@ -91,6 +91,36 @@ def test_write_dense_rows_under_any_stride():
         assert torch.equal(gv.cpu(), ref.stored(v.cpu()).float().to(BF))
 
 
+@pytest.mark.parametrize("tokens,heads,D", [(8300, 8, 64), (4100, 8, 128), (2049, 12, 256), (8200, 6, 64), (4100, 5, 128),
+                                            (2500, 12, 128)])
+def test_long_writes_and_reads_are_those_of_short_ones(tokens, heads, D):
+    """A lane takes up to four heads of a long call: the same bytes and values as token by token runs of a few."""
+    g = gen(tokens + heads)
+    k, v = normal(g, tokens, heads, D), normal(g, tokens, heads, D) * 5 - 2
+    k[5:40:7] = 3.0                                   # groups of one value
+    v[6:60:9, 1] *= 1e-38                             # subnormal scales
+    k[100, 2, 7], v[101, 3, 60], k[102, 0, 0] = float("nan"), float("inf"), float("-inf")
+    k[103, 1, :2] = torch.tensor([3e38, -3e38], device=DEV).to(BF)
+    bs = 32
+    pools = [kv4_pool(tokens // bs + 2, bs, 2, heads, D) for _ in range(2)]
+    slots = torch.randperm(pools[0].shape[1] * bs, generator=g, device=DEV)[:tokens]
+    slots[50:60] = -1
+    ops.kv4_write(k, v, pools[0], 1, slots)
+    for i in range(0, tokens, 200):
+        ops.kv4_write(k[i:i + 200], v[i:i + 200], pools[1], 1, slots[i:i + 200])
+    assert torch.equal(pools[0], pools[1])
+    gk, gv = ops.kv4_read(pools[0], 1, slots)
+    for i in range(0, tokens, 200):
+        pk, pv = ops.kv4_read(pools[0], 1, slots[i:i + 200])
+        assert torch.equal(gk[i:i + 200].view(torch.int16), pk.view(torch.int16))
+        assert torch.equal(gv[i:i + 200].view(torch.int16), pv.view(torch.int16))
+    live = slots >= 0
+    for x, got in ((k, gk), (v, gv)):
+        assert torch.equal(got[:200][live[:200]].cpu().isnan(), ref.stored(x[:200][live[:200]].cpu()).isnan())
+        some = torch.arange(104, 200, device=DEV)
+        assert torch.equal(got[some].cpu(), ref.stored(x[some].cpu()).float().to(BF))
+
+
 def test_write_extreme_values():
     """Constant groups, ties between two codes, tiny and huge values, and NaN and infinity in one group only."""
     pool = kv4_pool(2, 16, 1, 1, 128)
