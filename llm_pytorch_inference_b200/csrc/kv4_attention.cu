@@ -607,9 +607,12 @@ __global__ void __launch_bounds__(Kv4Cfg<D, RT>::WARPS * 32, 1) kv4_attn_kernel(
 #pragma unroll
             for (int e = 0; e < 2; ++e)
 #pragma unroll
-              for (int q = 0; q < NC; ++q) {
-                const float part = fmaf(pair_scale(kp[e][k]), acc[(q >> 1) % NT][2 * e + (q & 1)], k == 0 ? 0.0f : s[u][e][q]);
-                s[u][e][q] = fmaf(pair_min(kp[e][k]), qs[q][k], part);
+              for (int q = 0; q < NC; q += 2) {
+                const float ps = pair_scale(kp[e][k]), pm = pair_min(kp[e][k]);
+                const F2 dot = {acc[(q >> 1) % NT][2 * e], acc[(q >> 1) % NT][2 * e + 1]};
+                const F2 part = k == 0 ? mul2({ps, ps}, dot) : fma2({ps, ps}, dot, {s[u][e][q], s[u][e][q + 1]});
+                const F2 sum = fma2({pm, pm}, {qs[q][k], qs[q + 1][k]}, part);
+                s[u][e][q] = sum.x, s[u][e][q + 1] = sum.y;
               }
           } else {
             int acc[KT][4];
@@ -627,16 +630,23 @@ __global__ void __launch_bounds__(Kv4Cfg<D, RT>::WARPS * 32, 1) kv4_attn_kernel(
                   mma_u8s8_16832(acc[nt], a0, a1, a2, a3, b.x, b.y);
               }
             }
+            // two scores at a time: of both tokens of the row (RT = 0), or of two rows
 #pragma unroll
-            for (int e = 0; e < 2; ++e)
-#pragma unroll
-              for (int q = 0; q < NC; ++q) {
-                const int hi = RT == 0 ? acc[0][2 * e] : acc[(q >> 1) * 2 % KT][2 * e + (q & 1)];
-                const int lo = RT == 0 ? acc[0][2 * e + 1] : acc[((q >> 1) * 2 + 1) % KT][2 * e + (q & 1)];
-                const float dot = fmaf(__int_as_float(hi) - kMagic, 256.0f, __int_as_float(lo) - kMagic);
-                const float part = fmaf(pair_scale(kp[e][k]), dot, k == 0 ? 0.0f : s[u][e][q]);
-                s[u][e][q] = fmaf(pair_min(kp[e][k]), qs[q][k], part);
-              }
+            for (int i = 0; i < NC; ++i) {
+              const int e = RT == 0 ? 0 : i & 1, q = RT == 0 ? 0 : i & ~1;
+              const int e1 = RT == 0 ? 1 : e, q1 = RT == 0 ? 0 : q + 1;
+              const int th = RT == 0 ? 0 : q % KT, tl = RT == 0 ? 0 : (q + 1) % KT;  // tiles of the planes
+              const F2 hi = {__int_as_float(acc[th][2 * e]), __int_as_float(acc[th][RT == 0 ? 2 : 2 * e + 1])};
+              const F2 lo = {__int_as_float(acc[tl][RT == 0 ? 1 : 2 * e]),
+                             __int_as_float(acc[tl][RT == 0 ? 3 : 2 * e + 1])};
+              const F2 off = {-kMagic, -kMagic}, up = {256.0f, 256.0f};
+              const F2 dot = fma2(add2(hi, off), up, add2(lo, off));
+              const F2 ps = {pair_scale(kp[e][k]), pair_scale(kp[e1][k])};
+              const F2 pm = {pair_min(kp[e][k]), pair_min(kp[e1][k])};
+              const F2 part = k == 0 ? mul2(ps, dot) : fma2(ps, dot, {s[u][e][q], s[u][e1][q1]});
+              const F2 sum = fma2(pm, {qs[q][k], qs[q1][k]}, part);
+              s[u][e][q] = sum.x, s[u][e1][q1] = sum.y;
+            }
           }
         }
         if constexpr (CAP)
@@ -686,16 +696,26 @@ __global__ void __launch_bounds__(Kv4Cfg<D, RT>::WARPS * 32, 1) kv4_attn_kernel(
       for (int u = 0; u < MATH; ++u)
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
+          if constexpr (!MASKED && RT > 0 && !CAP) {
 #pragma unroll
-          for (int q = 0; q < NC; ++q) {
-            d[u][e][q] = distance(u, e, q);
-            far = fmaxf(far, d[u][e][q]);
+            for (int q = 0; q < NC; q += 2) {
+              const F2 x = fma2({s[u][e][q], s[u][e][q + 1]}, {f[q], f[q + 1]}, {-mref[q], -mref[q + 1]});
+              d[u][e][q] = x.x, d[u][e][q + 1] = x.y;
+            }
+          } else {
+#pragma unroll
+            for (int q = 0; q < NC; ++q) d[u][e][q] = distance(u, e, q);
           }
 #pragma unroll
-          for (int k = 0; k < NG; ++k) {
-            vs[u][e][k] = pair_scale(vp[u][e][k]) * vscale;
-            top = fmaxf(top, vs[u][e][k]);
+          for (int q = 0; q < NC; ++q) far = fmaxf(far, d[u][e][q]);
+#pragma unroll
+          for (int k = 0; k < NG; k += 2) {
+            const F2 x = mul2({pair_scale(vp[u][e][k]), pair_scale(vp[u][e][(k + 1) % NG])}, {vscale, vscale});
+            vs[u][e][k] = x.x;
+            if (k + 1 < NG) vs[u][e][(k + 1) % NG] = x.y;
           }
+#pragma unroll
+          for (int k = 0; k < NG; ++k) top = fmaxf(top, vs[u][e][k]);
         }
       // ---- new references and scaling, where a score or a scale outgrew them
       if (__any_sync(0xffffffffu, far > kSlack || top > limit)) {
@@ -770,16 +790,34 @@ __global__ void __launch_bounds__(Kv4Cfg<D, RT>::WARPS * 32, 1) kv4_attn_kernel(
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
             float w[NC];
-#pragma unroll
-            for (int q = 0; q < NC; ++q) {
-              w[q] = d[u][e][q] * vs[u][e][k];
-              if constexpr (MASKED) {  // a NaN pair that only later rows see
-                const bool x = in[u] >> (e * NC + q) & 1u;
-                w[q] = x ? w[q] : 0.0f;
-                mo[q][k] += x ? d[u][e][q] * pair_min(vp[u][e][k]) : 0.0f;
-              } else {
-                mo[q][k] = fmaf(d[u][e][q], pair_min(vp[u][e][k]), mo[q][k]);
+            if constexpr (!MASKED && RT == 0 && NG > 1) {
+              if (k % 2 == 0) {  // two groups at a time, the second one's weight kept for its turn
+                const F2 p = {d[u][e][0], d[u][e][0]}, x = mul2(p, {vs[u][e][k], vs[u][e][(k + 1) % NG]});
+                const F2 m = {pair_min(vp[u][e][k]), pair_min(vp[u][e][(k + 1) % NG])};
+                const F2 y = fma2(p, m, {mo[0][k], mo[0][(k + 1) % NG]});
+                vs[u][e][k] = x.x, vs[u][e][(k + 1) % NG] = x.y;
+                mo[0][k] = y.x, mo[0][(k + 1) % NG] = y.y;
               }
+              w[0] = vs[u][e][k];
+            } else if constexpr (!MASKED && RT > 0) {
+              const float pm = pair_min(vp[u][e][k]), ps = vs[u][e][k];
+#pragma unroll
+              for (int q = 0; q < NC; q += 2) {
+                const F2 p = {d[u][e][q], d[u][e][q + 1]}, x = mul2(p, {ps, ps});
+                const F2 y = fma2(p, {pm, pm}, {mo[q][k], mo[q + 1][k]});
+                w[q] = x.x, w[q + 1] = x.y;
+                mo[q][k] = y.x, mo[q + 1][k] = y.y;
+              }
+            } else if constexpr (MASKED) {
+#pragma unroll
+              for (int q = 0; q < NC; ++q) {
+                const bool x = in[u] >> (e * NC + q) & 1u;  // a NaN pair that only later rows see
+                w[q] = x ? d[u][e][q] * vs[u][e][k] : 0.0f;
+                mo[q][k] += x ? d[u][e][q] * pair_min(vp[u][e][k]) : 0.0f;
+              }
+            } else {
+              w[0] = d[u][e][0] * vs[u][e][k];
+              mo[0][k] = fmaf(d[u][e][0], pair_min(vp[u][e][k]), mo[0][k]);
             }
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt)

@@ -71,28 +71,6 @@ __device__ __forceinline__ float divided(float x, float d, float y) {
 
 constexpr float kTiny = 0x1p-90f;  // magnitudes from here on are away from underflow
 
-// Two fp32 numbers to an instruction (the lower one first), each rounded as by its own.
-__device__ __forceinline__ uint64_t two(float a, float b) {
-  uint64_t d;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "f"(a), "f"(b));
-  return d;
-}
-__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
-  uint64_t d;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
-  return d;
-}
-__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
-  uint64_t d;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
-  return d;
-}
-__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
-  uint64_t d;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
-  return d;
-}
-
 __device__ __forceinline__ float bf16_low(uint32_t x) { return __uint_as_float(x << 16); }
 __device__ __forceinline__ float bf16_high(uint32_t x) { return __uint_as_float(x & 0xffff0000u); }
 
@@ -102,13 +80,12 @@ template <bool PLAIN>
 __device__ __forceinline__ uint32_t quantise8(const uint32_t (&x)[4], float low, float scale, float inv) {
   uint32_t word = 0;
   if (PLAIN || scale >= kTiny) {
-    const uint64_t low2 = two(-low, -low), scale2 = two(-scale, -scale), inv2 = two(inv, inv);
-    const uint64_t magic2 = two(kMagic, kMagic);
+    const F2 low2 = {-low, -low}, scale2 = {-scale, -scale}, inv2 = {inv, inv}, magic2 = {kMagic, kMagic};
 #pragma unroll
     for (int j = 3; j >= 0; --j) {  // `divided`, two at a time
-      const uint64_t v = add2(two(bf16_low(x[j]), bf16_high(x[j])), low2), q = mul2(v, inv2);
-      const uint64_t u = add2(fma2(fma2(scale2, q, v), inv2, q), magic2);  // at most 15: scale is within 2^-9
-      word = (word * 16u + static_cast<uint32_t>(u >> 32)) * 16u + static_cast<uint32_t>(u);
+      const F2 v = add2({bf16_low(x[j]), bf16_high(x[j])}, low2), q = mul2(v, inv2);
+      const F2 u = add2(fma2(fma2(scale2, q, v), inv2, q), magic2);  // at most 15: scale is within 2^-9
+      word = (word * 16u + __float_as_uint(u.y)) * 16u + __float_as_uint(u.x);
     }
     return word - kPackBias;
   }
