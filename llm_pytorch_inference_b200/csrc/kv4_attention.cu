@@ -34,10 +34,11 @@
 // worker order by a second small kernel: no atomics, nothing to clear, the same bits every time.
 //
 // Measured on a B200 (6.55 TB/s copy), device time with inputs turned over: 64 sequences of 1024-2048 tokens, 32 query
-// and 8 KV heads of 128: 30.1 us for 115 MB, of which 3 us pass before the first copy, 17 at the rate of
-// memory and 7 in the last workers and the join.  One sequence of 131072: 36.6 us (151 MB).  16 sequences of
-// 4096-8192, 16 query and 8 KV heads of 256, capped: 47.1 us (226 MB, 4.8 TB/s).  5 query tokens of 4 sequences of
-// 16K-32K: 69.6 us (115 MB), bound by issued instructions.  One short sequence: 6.8 us, latency.
+// and 8 KV heads of 128: 28.0 us for 115 MB, of which 3.5 us pass before the first copy, 18 until the median worker has
+// seen its records, at the rate of memory, and 6 in the last workers and the join.  One sequence of 131072: 34.6 us
+// (151 MB).  16 sequences of 4096-8192, 16 query and 8 KV heads of 256, capped: 45.0 us (226 MB, 5.0 TB/s).  5 query
+// tokens of 4 sequences of 16K-32K: 58.2 us (115 MB), bound by what 8 warps of an SM can issue.  One short sequence:
+// 6.4 us, latency.
 #include <climits>
 #include <type_traits>
 
@@ -52,7 +53,7 @@ namespace {
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr int kShortRecords = 8;  // items of at most this many records are never split
 // What beginning an item costs a warp (its Q, its result), in bursts, for the division of the work: 64 sequences of
-// 1024-2048 tokens and 8 query rows took 39.2 us at 1 and take 37.6 at 3.
+// 1024-2048 tokens and 8 query rows took 39.2 us at 1 and 37.6 at 3.
 constexpr int kItemCost = 3;
 
 // A weight is 2^(score - reference): the reference is a row's maximum when last raised, and is raised
@@ -81,9 +82,9 @@ struct Kv4Rows {
 // BURST: records that a warp takes at once (one wait, one refill); STAGES of them are held, so that
 // an SM has some 45 KB or more under way while it computes.  A wait and refill cost some 90 instructions, a record of
 // 24 rows 510: 5 query tokens of 4 sequences of 16K-32K took 70.2 us with bursts of 1, 64.5 with 2, 61.9 with 4; one
-// sequence of 500, which 4 spread over fewer workers, 17.3, 17.6 and 19.0.  WARPS of the one block per SM: 64 sequences of
-// 1024-2048 tokens, 4 rows of 128: 33.3 us with 8, 30.1 with 12, 31.0 with 16 (128 registers); 8 rows: 40.9, 37.6,
-// 44.1 (spills); 4 rows of 256, 16 x 4096-8192: 57, 47.1, 49.1.  16 rows and more of 128 or 256 need over 168
+// sequence of 500, which 4 spread over fewer workers, 17.3, 17.6 and 19.0.  WARPS of the one block per SM: 64 sequences
+// of 1024-2048 tokens, 4 rows of 128, took 33.3 us with 8, 30.1 with 12, 31.0 with 16 (128 registers); 8 rows 40.9,
+// 37.6, 44.1 (spills); 4 rows of 256, 16 x 4096-8192, 57, 47.1, 49.1.  16 rows and more of 128 or 256 need over 168
 // registers.  One block, not two: the scheduler prefers the older one, whose warps then ended after 21 us of a
 // call where the other's took 27.
 template <int D, int RT>
