@@ -295,15 +295,28 @@ int mvb_paged_attention_decode_kv4(void* out, int64_t out_stride, const void* q,
  * means 0, and the two may not be the same word).  A sequence that does not fit -- in its table row, in
  * what is left of the free list, or in the num_tokens of the outputs -- takes no block:
  * granted 0, its tokens' slots -1; those behind it may still fit.  Negative lengths are refused the
- * same way, with MVB_DEV_BAD_POSITION.  Entries of slots past the last token are -1.  batch <= 1048576;
+ * same way, with MVB_DEV_BAD_POSITION.  Entries of slots past the last token are -1, and those under a negative table
+ * entry.  batch <= 1048576;
  * more than 8192 sequences need a workspace of mvb_assign_slots_workspace_bytes(batch) bytes (0 for fewer: NULL),
- * 8-byte aligned, of any content. */
+ * 8-byte aligned, of any content.
+ * A sequence whose length goes back (rejected drafts) keeps the blocks that it was given, which ceil(ctx / block_size)
+ * no longer counts: mvb_assign_slots would take new ones over them.  mvb_assign_slots_ex has held_blocks int32 [batch]
+ * for it, the entries of its row that a sequence holds (0 for a new one): those below are used again, what
+ * ceil((ctx + new) / block_size) exceeds them by comes off the free list, and a granted sequence's count is updated.
+ * A count below ceil(ctx / block_size) or past the row is refused, with MVB_DEV_BAD_POSITION.  NULL: mvb_assign_slots.
+ * The length of a sequence that was not granted must stay as it was: its row has no entries for the new tokens. */
 int64_t mvb_assign_slots_workspace_bytes(int64_t batch);
 int mvb_assign_slots(int64_t* slots, int32_t* positions, int32_t* seq_start, int32_t* granted,
                      int32_t* free_head_out, int32_t* block_tables, int64_t table_stride, int64_t max_blocks,
                      const int32_t* ctx_lens, const int32_t* new_lens, const int32_t* free_blocks, int64_t num_free,
                      const int32_t* free_head, int64_t batch, int64_t block_size, int64_t num_tokens,
                      void* workspace, int64_t workspace_bytes, mvb_stream_t stream);
+int mvb_assign_slots_ex(int64_t* slots, int32_t* positions, int32_t* seq_start, int32_t* granted,
+                        int32_t* free_head_out, int32_t* block_tables, int64_t table_stride, int64_t max_blocks,
+                        const int32_t* ctx_lens, const int32_t* new_lens, int32_t* held_blocks,
+                        const int32_t* free_blocks, int64_t num_free, const int32_t* free_head, int64_t batch,
+                        int64_t block_size, int64_t num_tokens, void* workspace, int64_t workspace_bytes,
+                        mvb_stream_t stream);
 
 /* Verification of drafted tokens (speculative decoding; no counterpart in the reference).
  * target_probs: fp32 rows, row b * (max_drafts + 1) + i (target_stride elements apart) the target's

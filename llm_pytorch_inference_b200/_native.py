@@ -66,6 +66,8 @@ SIGNATURES: dict[str, tuple] = {
     "mvb_assign_slots_workspace_bytes": (_i64, [_i64]),
     "mvb_assign_slots": (_i32, [_vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _vp, _vp, _vp, _i64, _vp, _i64, _i64, _i64,
                                 _vp, _i64, _vp]),
+    "mvb_assign_slots_ex": (_i32, [_vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _vp, _vp, _vp, _vp, _i64, _vp, _i64, _i64,
+                                   _i64, _vp, _i64, _vp]),
     "mvb_verify_drafts": (_i32, [_vp, _vp, _vp, _i64, _vp, _i64, _vp, _vp, _vp, _i64, _i64, _i64, _vp]),
     "mvb_gemm_workspace_bytes": (_i64, [_i64, _i64, _i64, _i32]),
     "mvb_gemm_bf16": (_i32, [_vp, _i64, _vp, _i64, _vp, _i64, _i64, _i64, _i64, _i32, _vp, _i64, _vp, _i64, _vp]),

@@ -5,11 +5,15 @@
 // block manager on the host pops them (engine/kv_cache.py:40-74).  Token i of it lies at position
 // ctx_b + i, slot table[b][position / bs] * bs + position % bs.
 //
+// Where lengths go back (rejected drafts) ceil(ctx_b / bs) is less than what the sequence was given, so the caller
+// keeps the count of blocks, held_b: the sequence grows by what ceil((ctx_b + new_b) / bs) exceeds it, entries below
+// held_b are used again, and held_b becomes the larger of the two.
+//
 // One launch: every CTA scans the batch's lengths by itself (a few KB, out of L2 after the first
 // CTA), then maps its share of the tokens; a token finds its sequence by bisecting the scanned
 // starts in shared memory.  A token at the first position of a new block writes that block into
-// the table.  No CTA reads what another writes: entries below ceil(ctx_b / bs) are only read, the
-// ones above only written.  Bound by latency: a scan, a bisection and two dependent loads (4.3 us for 64 sequences of
+// the table.  No CTA reads what another writes: entries below held_b are only read, the ones above only written,
+// and held_b is updated when all have read it, by the one CTA or by a launch of its own.  Bound by latency: a scan, a bisection and two dependent loads (4.3 us for 64 sequences of
 // one token, 5.5 for 200 of 500 to 1000).
 //
 // A batch whose starts do not fit into shared memory is cut into pieces of 4,096 sequences, a block each: sums of
@@ -40,6 +44,7 @@ struct SlotArgs {
   int64_t max_blocks;
   const int32_t* ctx;
   const int32_t* add;
+  int32_t* held;  // blocks that a sequence holds, updated; nullptr: ceil(ctx / bs)
   const int32_t* free_blocks;
   const int32_t* head_in;
   int64_t num_free;
@@ -50,6 +55,24 @@ struct SlotArgs {
 };
 
 __device__ __forceinline__ int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
+
+__device__ __forceinline__ int64_t held_blocks(const SlotArgs& a, int64_t b, int64_t ctx) {
+  return a.held != nullptr ? a.held[b] : ceil_div(ctx, a.bs);
+}
+// Blocks that sequence b lacks for its new tokens, its lengths being good.
+__device__ __forceinline__ int64_t blocks_lacking(const SlotArgs& a, int64_t b, int64_t ctx, int64_t add) {
+  return max(ceil_div(ctx + add, a.bs) - held_blocks(a, b, ctx), int64_t(0));
+}
+// Lengths of a sequence that can be: none negative, and the blocks it holds enough for what it has, and in its row.
+__device__ __forceinline__ bool lengths_good(const SlotArgs& a, int64_t b, int64_t ctx, int64_t add) {
+  if (ctx < 0 || add < 0) return false;
+  if (a.held == nullptr) return true;
+  const int64_t held = a.held[b];
+  return held >= ceil_div(ctx, a.bs) && held <= a.max_blocks;
+}
+__device__ __forceinline__ void update_held(const SlotArgs& a, int64_t b, bool granted) {
+  if (granted) a.held[b] = static_cast<int32_t>(max(int64_t(a.held[b]), ceil_div(int64_t(a.ctx[b]) + a.add[b], a.bs)));
+}
 
 // Inclusive scan over the block of two 64-bit values per thread.
 __device__ __forceinline__ void block_scan2(int64_t& x, int64_t& y, int64_t (*warps)[2]) {
@@ -90,7 +113,7 @@ __device__ __forceinline__ void map_tokens(const SlotArgs& a, int64_t head, cons
       const int64_t ctx = max(a.ctx[lo], 0);
       pos = ctx + (t - start[lo]);
       if (first[lo] >= 0) {
-        const int64_t bi = pos / a.bs, held = ceil_div(ctx, a.bs);
+        const int64_t bi = pos / a.bs, held = held_blocks(a, lo, ctx);
         int32_t* row = a.tables + lo * a.table_stride;
         int32_t id;
         if (bi < held) {
@@ -129,11 +152,11 @@ __global__ void __launch_bounds__(kThreads) assign_slots_kernel(const SlotArgs a
     if (b < a.batch) {
       const int64_t ctx = a.ctx[b];
       add = a.add[b];
-      ok = ctx >= 0 && add >= 0;
+      ok = lengths_good(a, b, ctx, add);
       if (!ok && blockIdx.x == 0) report(a.err, kDevBadPosition);
       add = max(add, int64_t(0));
       ok = ok && ctx + add <= a.max_blocks * a.bs;
-      need = ok ? ceil_div(ctx + add, a.bs) - ceil_div(ctx, a.bs) : 0;
+      need = ok ? blocks_lacking(a, b, ctx, add) : 0;
     }
     total = add;
     block_scan2(total, need, warps);  // need becomes inclusive; what the sequence asks for is in `blocks`
@@ -164,8 +187,7 @@ __global__ void __launch_bounds__(kThreads) assign_slots_kernel(const SlotArgs a
       const int b = base + tid;
       int64_t need = 0, zero = 0;
       if (b < a.batch && first[b] >= 0) {
-        const int64_t ctx = a.ctx[b];
-        need = ceil_div(ctx + a.add[b], a.bs) - ceil_div(ctx, a.bs);
+        need = blocks_lacking(a, b, a.ctx[b], a.add[b]);
       }
       const int64_t own = need;
       block_scan2(zero, need, warps);
@@ -180,8 +202,7 @@ __global__ void __launch_bounds__(kThreads) assign_slots_kernel(const SlotArgs a
       int64_t taken = 0;
       for (int b = 0; b < a.batch; ++b) {
         if (first[b] < 0) continue;
-        const int64_t ctx = a.ctx[b];
-        const int64_t need = ceil_div(ctx + a.add[b], a.bs) - ceil_div(ctx, a.bs);
+        const int64_t need = blocks_lacking(a, b, a.ctx[b], a.add[b]);
         if (taken + need <= avail) {
           first[b] = static_cast<int32_t>(taken);
           taken += need;
@@ -200,6 +221,16 @@ __global__ void __launch_bounds__(kThreads) assign_slots_kernel(const SlotArgs a
     if (tid == 0) *a.head_out = static_cast<int32_t>(head + carry[1]);
   }
   map_tokens(a, head, start, first);
+  if (a.held != nullptr && gridDim.x == 1) {
+    __syncthreads();  // all have read
+    for (int b = tid; b < a.batch; b += kThreads) update_held(a, b, first[b] >= 0);
+  }
+}
+
+// The held blocks of a call of several CTAs.
+__global__ void __launch_bounds__(kThreads) slot_held_kernel(const SlotArgs a) {
+  const int64_t b = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x;
+  if (b < a.batch) update_held(a, b, a.granted[b] != 0);
 }
 
 // ---- batches of more than kMaxShared sequences
@@ -254,12 +285,12 @@ __global__ void __launch_bounds__(kThreads) slot_starts_kernel(const SlotArgs a,
     const int64_t b = b0 + i;
     if (b >= a.batch) break;
     const int64_t ctx = a.ctx[b], add = a.add[b];
-    bool ok = ctx >= 0 && add >= 0;
+    bool ok = lengths_good(a, b, ctx, add);
     if (!ok) report(a.err, kDevBadPosition);
     at += max(add, int64_t(0));
     a.seq_start[b + 1] = static_cast<int32_t>(min(at, int64_t(INT_MAX)));
     ok = ok && ctx + add <= a.max_blocks * a.bs && at <= a.tokens;
-    const int64_t need = ok ? ceil_div(ctx + add, a.bs) - ceil_div(ctx, a.bs) : 0;
+    const int64_t need = ok ? blocks_lacking(a, b, ctx, add) : 0;
     needs += need;
     g.first[b] = ok ? static_cast<int32_t>(need) : -1;
   }
@@ -348,6 +379,17 @@ extern "C" int mvb_assign_slots(int64_t* slots, int32_t* positions, int32_t* seq
                                 const int32_t* free_blocks, int64_t num_free, const int32_t* free_head,
                                 int64_t batch, int64_t block_size, int64_t num_tokens, void* workspace,
                                 int64_t workspace_bytes, mvb_stream_t stream) {
+  return mvb_assign_slots_ex(slots, positions, seq_start, granted, free_head_out, block_tables, table_stride, max_blocks,
+                             ctx_lens, new_lens, nullptr, free_blocks, num_free, free_head, batch, block_size, num_tokens,
+                             workspace, workspace_bytes, stream);
+}
+
+extern "C" int mvb_assign_slots_ex(int64_t* slots, int32_t* positions, int32_t* seq_start, int32_t* granted,
+                                   int32_t* free_head_out, int32_t* block_tables, int64_t table_stride,
+                                   int64_t max_blocks, const int32_t* ctx_lens, const int32_t* new_lens,
+                                   int32_t* held_blocks, const int32_t* free_blocks, int64_t num_free,
+                                   const int32_t* free_head, int64_t batch, int64_t block_size, int64_t num_tokens,
+                                   void* workspace, int64_t workspace_bytes, mvb_stream_t stream) {
   MVB_REQUIRE(seq_start && free_head_out, "mvb_assign_slots: null pointer");
   MVB_REQUIRE(batch >= 0 && batch <= kMaxBatch, "mvb_assign_slots: batch %lld (at most %d)", (long long)batch,
               kMaxBatch);
@@ -361,22 +403,28 @@ extern "C" int mvb_assign_slots(int64_t* slots, int32_t* positions, int32_t* seq
   MVB_REQUIRE(num_tokens >= 0 && num_tokens <= INT_MAX && (num_tokens == 0 || (slots && positions)),
               "mvb_assign_slots: num_tokens %lld", (long long)num_tokens);
   MVB_REQUIRE(free_head_out != free_head, "mvb_assign_slots: free_head_out may not be free_head");
+  MVB_REQUIRE(held_blocks == nullptr || batch == 0 || (held_blocks != ctx_lens && held_blocks != new_lens),
+              "mvb_assign_slots: held_blocks may not be a length");
   const int sms = current_sm_count();
   MVB_REQUIRE(sms > 0, "mvb_assign_slots: no device");
   SlotArgs a = {slots,    positions, seq_start,   granted,   free_head_out, block_tables, table_stride,
-                max_blocks, ctx_lens,  new_lens,    free_blocks, free_head,  num_free,     num_tokens,
-                static_cast<int>(batch), static_cast<int>(block_size), device_status_ptr()};
+                max_blocks, ctx_lens,  new_lens,    held_blocks, free_blocks,   free_head,    num_free,
+                num_tokens, static_cast<int>(batch), static_cast<int>(block_size), device_status_ptr()};
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   int64_t grid = (num_tokens + 2 * kThreads - 1) / (2 * kThreads);
   grid = grid < 1 ? 1 : grid > sms ? sms : grid;
   const dim3 blocks(static_cast<unsigned>(grid)), threads(kThreads);
+  const dim3 per_sequence(static_cast<unsigned>((batch + kThreads - 1) / kThreads));
   if (batch <= kMaxShared) {
     const size_t smem = (2 * batch + 1) * sizeof(int32_t);
     // past 48 KB together with the kernel's static arrays a launch has to be allowed for: once, for the largest batch
     static std::atomic<uint64_t> done{0};
     if (smem > 40 * 1024)
       MVB_TRY(set_smem_once(done, assign_slots_kernel, (2 * kMaxShared + 1) * sizeof(int32_t), "assign_slots"));
-    return launch("assign_slots", assign_slots_kernel, blocks, threads, smem, st, a);
+    MVB_TRY(launch("assign_slots", assign_slots_kernel, blocks, threads, smem, st, a));
+    if (held_blocks == nullptr || grid == 1) return MVB_OK;
+    slot_held_kernel<<<per_sequence, threads, 0, st>>>(a);  // a plain launch: the one before has ended
+    return cuda_status(cudaGetLastError(), "assign_slots");
   }
   MVB_REQUIRE(workspace && aligned(workspace, 8) && workspace_bytes >= mvb_assign_slots_workspace_bytes(batch),
               "mvb_assign_slots: a workspace of %lld bytes, 8-byte aligned (got %lld)",
@@ -392,5 +440,6 @@ extern "C" int mvb_assign_slots(int64_t* slots, int32_t* positions, int32_t* seq
   slot_starts_kernel<<<pieces, threads, 0, st>>>(a, g);
   slot_offsets_kernel<<<pieces, threads, 0, st>>>(a, g);
   slot_tokens_kernel<<<blocks, threads, 0, st>>>(a, g);
+  if (held_blocks != nullptr) slot_held_kernel<<<per_sequence, threads, 0, st>>>(a);
   return cuda_status(cudaGetLastError(), "assign_slots");
 }

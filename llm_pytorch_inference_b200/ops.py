@@ -644,14 +644,20 @@ class SlotPlan(NamedTuple):
 
 def assign_slots(block_tables: torch.Tensor, ctx_lens: torch.Tensor, new_lens: torch.Tensor,
                  free_blocks: torch.Tensor, block_size: int, num_tokens: int,
-                 free_head: torch.Tensor | None = None) -> SlotPlan:
+                 free_head: torch.Tensor | None = None, held_blocks: torch.Tensor | None = None) -> SlotPlan:
     """Grows the block tables of a step on the GPU and maps its tokens to slots, in the order in which
     ``KVCacheManager`` pops its free list.  Sequence b holds ``ctx_lens[b]`` tokens (int32) in the first
     blocks of its row of ``block_tables`` (int32 ``[B, max_blocks]``, updated in place) and takes
     ``new_lens[b]`` more; the blocks it lacks come off ``free_blocks`` (int32), from ``free_head``
     (int32 ``[1]``, default 0) on.  ``num_tokens``: length of the per-token outputs, at least the sum of
     ``new_lens`` for every sequence to be granted; the entries behind the last token are -1.  A sequence that does not
-    fit (its table row, the free list, ``num_tokens``) takes nothing: ``granted`` 0 and slots -1."""
+    fit (its table row, the free list, ``num_tokens``) takes nothing: ``granted`` 0 and slots -1, and its length must
+    stay as it was.
+
+    ``held_blocks`` (int32 ``[B]``, updated in place): how many entries of its row each sequence holds, 0 for a new
+    one.  Needed where lengths go back, as rejected drafts make them: the blocks behind a shorter length are then used
+    again, where without a count new ones would be taken over them.  A count below what ``ctx_lens`` needs, or past the
+    row, is refused like a negative length."""
     what = "assign_slots"
     index = block_tables.get_device() if isinstance(block_tables, torch.Tensor) else -1
     try:
@@ -676,6 +682,10 @@ def assign_slots(block_tables: torch.Tensor, ctx_lens: torch.Tensor, new_lens: t
         _expect(what, "free_head", free_head, index, torch.int32, 1)
         if free_head.numel() != 1:
             raise RuntimeError(f"{what}: free_head must hold one number")
+    if held_blocks is not None:
+        _expect(what, "held_blocks", held_blocks, index, torch.int32, 1)
+        if held_blocks.numel() != B or not held_blocks.is_contiguous():
+            raise RuntimeError(f"{what}: held_blocks must be contiguous, one number for each of {B} sequences")
     if num_tokens < 0:
         raise RuntimeError(f"{what}: num_tokens {num_tokens}")
     ctx_lens, new_lens, free_blocks = ctx_lens.contiguous(), new_lens.contiguous(), free_blocks.contiguous()
@@ -688,10 +698,10 @@ def assign_slots(block_tables: torch.Tensor, ctx_lens: torch.Tensor, new_lens: t
     if B > 8192:
         ws_bytes = N.lib().mvb_assign_slots_workspace_bytes(B)
         ws = torch.empty(ws_bytes, dtype=_U8, device=block_tables.device)
-    N.on_device(index, what, N.lib().mvb_assign_slots, at, at + 8 * num_tokens, start, start + 4 * (B + 1),
+    N.on_device(index, what, N.lib().mvb_assign_slots_ex, at, at + 8 * num_tokens, start, start + 4 * (B + 1),
                 start + 4 * (2 * B + 1), block_tables.data_ptr(), t_stride, width, ctx_lens.data_ptr(),
-                new_lens.data_ptr(), free_blocks.data_ptr(), free_blocks.numel(), N.ptr(free_head), B,
-                int(block_size), int(num_tokens), N.ptr(ws), ws_bytes)
+                new_lens.data_ptr(), N.ptr(held_blocks), free_blocks.data_ptr(), free_blocks.numel(), N.ptr(free_head),
+                B, int(block_size), int(num_tokens), N.ptr(ws), ws_bytes)
     slots = slots.view(_I64)
     return SlotPlan(slots, positions, seq_start, granted, head)
 

@@ -51,7 +51,7 @@ DECODE_SCHEMAS = [
     "paged_attention_decode_kv4(Tensor q, Tensor kv4, int layer, Tensor block_tables, Tensor ctx_lens, "
     "float scale, float softcap, int window) -> Tensor",
     "assign_slots(Tensor(a!) block_tables, Tensor ctx_lens, Tensor new_lens, Tensor free_blocks, int block_size, "
-    "int num_tokens, Tensor? free_head) -> (Tensor, Tensor, Tensor, Tensor, Tensor)",
+    "int num_tokens, Tensor? free_head, Tensor(b!)? held_blocks=None) -> (Tensor, Tensor, Tensor, Tensor, Tensor)",
     "verify_drafts(Tensor target_probs, Tensor draft_tokens, Tensor uniforms, Tensor? draft_probs, "
     "Tensor? draft_lens) -> (Tensor, Tensor)",
 ]

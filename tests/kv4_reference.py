@@ -130,6 +130,33 @@ def assign(tables, ctx, new, free, block_size, num_tokens, head=0):
     return slots, positions, start, granted, taken
 
 
+def assign_held(tables, ctx, new, held, free, block_size, num_tokens, head=0):
+    """The same with the count of blocks that each sequence holds (a list, changed)."""
+    slots, positions, start, granted = [-1] * num_tokens, [0] * num_tokens, [0], []
+    taken = max(head, 0)
+    for b, (row, n, add) in enumerate(zip(tables, ctx, new)):
+        ok = n >= 0 and add >= 0 and -(-n // block_size) <= held[b] <= len(row)
+        add = max(add, 0)
+        end = start[-1] + add
+        need = -(-(max(n, 0) + add) // block_size)
+        ok = ok and need <= len(row) and end <= num_tokens
+        ok = ok and taken + max(need - held[b], 0) <= max(len(free), taken)
+        if ok:
+            for i in range(held[b], need):
+                row[i] = free[taken]
+                taken += 1
+            held[b] = max(held[b], need)
+        for i in range(add):
+            t, pos = start[-1] + i, max(n, 0) + i
+            if t < num_tokens:
+                positions[t] = pos
+                block = row[pos // block_size] if ok else -1          # an entry that names no block gives no slot
+                slots[t] = block * block_size + pos % block_size if block >= 0 else -1
+        start.append(end)
+        granted.append(int(ok))
+    return slots, positions, start, granted, taken
+
+
 # ------------------------------------------------------------------ drafts
 def verify(target, tokens, uniforms, draft=None, lens=None):
     """(tokens [B, K + 1], accepted [B]) on the CPU; probabilities in, sums in 64 bits."""

@@ -78,6 +78,27 @@ def test_assign_slots_refuses(change, text):
 
 
 @pytest.mark.parametrize("change, text", [
+    (dict(granted=None), "null pointer"), (dict(bs=0), "block_size 0"), (dict(held=A + 64), "held_blocks"),
+    (dict(held=A + 96), "held_blocks"),
+])
+def test_assign_slots_ex_refuses(change, text):
+    a = dict(slots=A, pos=A, start=A, granted=A, head_out=A + 4, bt=A, ts=8, mb=8, ctx=A + 64, new=A + 96, held=A + 128,
+             free=A, nf=10, head=None, batch=3, bs=16, n=12, ws=None, ws_bytes=0)
+    a.update(change)
+    refused(N.lib().mvb_assign_slots_ex(*a.values(), None), text)
+
+
+def test_reference_slots_with_counts():
+    """Where lengths only grow, counting the blocks changes nothing; after a step back they are used again."""
+    a, b, held = [[-1] * 4], [[-1] * 4], [0]
+    for n, add, head in ((0, 5, 0), (5, 4, 2), (9, 1, 3)):
+        assert ref.assign(a, [n], [add], [7, 8, 9], 4, add, head) == ref.assign_held(b, [n], [add], held, [7, 8, 9], 4, add,
+                                                                                     head)
+    assert a == b == [[7, 8, 9, -1]] and held == [3]
+    assert ref.assign_held(b, [3], [6], held, [7, 8, 9], 4, 6, 3)[::4] == ([31, 32, 33, 34, 35, 36], 3)
+
+
+@pytest.mark.parametrize("change, text", [
     (dict(out=None), "null pointer"), (dict(p=None), "null pointer"), (dict(u=None), "null pointer"),
     (dict(tok=None), "null pointer"), (dict(ps=99), "rows of 99"), (dict(qs=99), "rows of 100 and 99"),
     (dict(batch=-1), "batch -1"), (dict(K=-1), "-1 drafts"), (dict(K=5000), "5000 drafts"), (dict(V=0), "vocab 0"),
