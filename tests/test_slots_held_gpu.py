@@ -1,5 +1,6 @@
 """Slot assignment on the GPU where lengths go back, as rejected drafts make them: the caller keeps the count of blocks
 that each sequence holds."""
+import math
 import random
 
 import pytest
@@ -8,6 +9,7 @@ import torch
 import kv4_reference as ref
 from llm_pytorch_inference_b200 import _native as N
 from llm_pytorch_inference_b200 import ops
+from llm_pytorch_inference_b200.kv_cache import kv4_pool
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda"
@@ -135,3 +137,73 @@ def test_counts_of_the_wrong_kind_are_refused():
                  i32([[1, 1]])):
         with pytest.raises(RuntimeError):
             ops.assign_slots(table, x, i32([1, 1]), i32([5]), 16, 2, held_blocks=held)
+
+
+@pytest.mark.parametrize("captured", [False, True])
+def test_refused_sequences_touch_nothing(captured):
+    """Speculative steps with too few blocks: a refused sequence keeps its length, gets zeros and changes no record, the
+    granted one goes on, and once blocks come back the refused one resumes where it was."""
+    B, T, Hq, Hkv, D, bs, V = 3, 2, 4, 2, 64, 16, 11
+    g = torch.Generator(device=DEV).manual_seed(5)
+    pool = kv4_pool(6, bs, 1, Hkv, D)
+    table = torch.zeros(B, 4, dtype=torch.int32, device=DEV)               # entries never given name block 0
+    ctx, new, held, head = i32([31, 15, 3]), i32([T] * B), i32([0] * B), i32([0])
+    free = i32([0, 1, 2, 3, 5, 4])
+    first = ops.assign_slots(table, i32([0] * B), ctx, free[:4], bs, 49, free_head=head, held_blocks=held)
+    head.copy_(first.free_head)
+    assert table[0, :2].tolist() == [0, 1] and int(table[1, 0]) == 2 and int(table[2, 0]) == 3 and int(head) == 4
+    fill = torch.randn(2, 49, Hkv, D, generator=g, device=DEV).bfloat16()
+    ops.kv4_write(fill[0], fill[1], pool, 0, first.slots)
+    x = torch.randn(B * T, Hq + 2 * Hkv, D, generator=g, device=DEV).bfloat16()
+    probs = torch.rand(B, T, V, generator=g, device=DEV)
+    drafts = torch.randint(0, V, (B, T - 1), generator=g, device=DEV)
+    u = torch.rand(B, T, generator=g, device=DEV)
+
+    def step(n):
+        plan = ops.assign_slots(table, ctx, new, free[:n], bs, B * T, free_head=head, held_blocks=held)
+        seen = (ctx + new) * plan.granted
+        ops.kv4_write(x[:, Hq:Hq + Hkv], x[:, Hq + Hkv:], pool, 0, plan.slots)
+        out = ops.paged_attention_decode_kv4(x[:, :Hq].unflatten(0, (B, T)), pool, 0, table, seen, 1 / math.sqrt(D))
+        tokens, accepted = ops.verify_drafts(probs, drafts, u)
+        ctx.add_((accepted + 1) * plan.granted)
+        head.copy_(plan.free_head)
+        return plan, out
+
+    graph = None
+    if captured:
+        keep = [t.clone() for t in (table, ctx, held, head, pool)]
+        step(4)
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            plan, out = step(4)
+        for t, old in zip((table, ctx, held, head, pool), keep):
+            t.copy_(old)
+    before, length = pool.clone(), 3
+    for _ in range(4):
+        if captured:
+            graph.replay()
+        else:
+            plan, out = step(4)
+        assert plan.granted.tolist() == [0, 0, 1] and plan.slots[:4].tolist() == [-1] * 4
+        assert ctx.tolist()[:2] == [31, 15] and length < int(ctx[2]) <= length + T
+        assert held.tolist() == [2, 1, 1] and int(head) == 4
+        assert not bool(out[:2].any()) and bool(out[2].any())
+        assert torch.equal(pool[:, :3], before[:, :3]) and torch.equal(pool[:, 4:], before[:, 4:])
+        length = int(ctx[2])
+    plan, out = step(6)                                                    # two blocks more
+    assert plan.granted.tolist() == [1, 1, 1] and held.tolist() == [3, 2, 1] and int(head) == 6
+    assert table.tolist() == [[0, 1, 5, 0], [2, 4, 0, 0], [3, 0, 0, 0]]
+    assert plan.slots[:4].tolist() == [31, 5 * 16, 2 * 16 + 15, 4 * 16]
+    gk, gv = ops.kv4_read(pool, 0, first.slots)                            # the prompts are as they were written
+    assert torch.equal(gk.cpu(), ref.stored(fill[0].cpu()).float().bfloat16())
+    assert torch.equal(gv.cpu(), ref.stored(fill[1].cpu()).float().bfloat16())
+
+
+def test_a_refused_length_that_moved_on_is_refused():
+    """The step without the mask: the length counts entries that were never given (zeros: block 0, another sequence's)."""
+    table, held, head = i32([[0, 1, 0], [2, 0, 0]]), i32([2, 1]), i32([0])
+    for ctx in ([31, 17], [31, 19]):
+        plan = ops.assign_slots(table, i32(ctx), i32([2, 2]), i32([9])[:0], 16, 4, free_head=head, held_blocks=held)
+        assert plan.granted.tolist() == [0, 0] and plan.slots.tolist() == [-1] * 4 and held.tolist() == [2, 1]
+        assert N.device_status(clear=True) == N.DEV_BAD_POSITION
