@@ -145,6 +145,7 @@ __global__ void __launch_bounds__(kThreads) assign_slots_kernel(const SlotArgs a
     carry[0] = carry[1] = 0;
     start[0] = 0;
   }
+  __syncthreads();  // the scans hold others, but there are none for an empty batch
   for (int base = 0; base < a.batch; base += kThreads) {
     const int b = base + tid;
     int64_t add = 0, need = 0, total, blocks;

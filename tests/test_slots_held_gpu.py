@@ -207,3 +207,15 @@ def test_a_refused_length_that_moved_on_is_refused():
         plan = ops.assign_slots(table, i32(ctx), i32([2, 2]), i32([9])[:0], 16, 4, free_head=head, held_blocks=held)
         assert plan.granted.tolist() == [0, 0] and plan.slots.tolist() == [-1] * 4 and held.tolist() == [2, 1]
         assert N.device_status(clear=True) == N.DEV_BAD_POSITION
+
+
+@pytest.mark.parametrize("tokens", [0, 1, 700, 5000])
+def test_slots_of_an_empty_batch(tokens):
+    """No sequence, any padding, with and without a head: the head stays and every slot is -1."""
+    none = i32([])
+    for head, n in ((0, 0), (3, 9), (9, 9), (12, 9)):
+        for held in (None, none.clone()):
+            plan = ops.assign_slots(none.view(0, 4), none, none, i32(list(range(n))), 16, tokens, free_head=i32([head]),
+                                    held_blocks=held)
+            assert plan.slots.tolist() == [-1] * tokens and plan.seq_start.tolist() == [0]
+            assert plan.free_head.tolist() == [head] and plan.granted.numel() == 0
