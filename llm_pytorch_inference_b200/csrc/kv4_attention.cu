@@ -6,25 +6,23 @@
 // What it must read is 9/16 of a byte per cached value, once: the bound is memory.  That leaves an SM some 44
 // values a clock, and its integer pipe takes 64 lane-operations a clock, so codes never become floating-point
 // numbers one by one:
+//   * fp16 holds u * 2^-24 and u * 2^-20 as bit patterns with the code in bits 0-3 or 4-7 (subnormal numbers, exact), so
+//     one AND of a word yields two matrix operands.
 //   * Scores: q . k = sum_g s_g (q_g . u_g) + m_g sum(q_g) over the groups of 64 channels, the pairs outside
-//     the products.  Up to 8 query rows, codes are bytes for the integer tensor cores (u8 x s8, exact): three
-//     operations turn a word of 8 codes into two operands.  q of a row is held in 16 bits of its largest magnitude, as
-//     two signed bytes (planes) that are columns of their own; the rounding is 2^-16 of that magnitude, below
-//     what fp32 sums of the products would lose at long rows.  The sums stay below 2^22 and start at
-//     1.5 * 2^23, so that their bits are the fp32 number itself and need no conversion.  With more rows the
-//     planes cost more than they save: codes are then fp16 operands, as below, and q is exact in fp16, times a
-//     power of two (24 rows: 77.0 -> 69.6 us at 4 sequences of 16K-32K).
-//   * Outputs: fp16 holds u * 2^-24 and u * 2^-20 as bit patterns with the code in bits 0-3 or 4-7 (subnormal
-//     numbers, exact), so one AND of a word yields two matrix operands.  The weight of a token times s' is
-//     the other operand, and p m' is summed per group and query, on the side.  That weight is the one
-//     rounding (11 bits, 8 times finer than the result's bf16); it is scaled by a power of two that
-//     follows the largest s' seen.  Scores, statistics and sums are fp32.
+//     the products.  The other operand is q times a power of two that puts its row's largest magnitude below 2^11:
+//     exact in fp16 for what is above 2^-27 of that magnitude, and off by 2^-35 of it below.  So the scores are off by
+//     what fp32 sums lose, whatever the number of rows.  (q as two signed bytes for the integer tensor cores, one
+//     operation a word less, took 28.0 us where this takes 28.8 and 45.0 where this takes 47.1, but left q 16 bits of
+//     its row's largest magnitude, which loses the small channels beside a large one.)
+//   * Outputs: the weight of a token times s' is the other operand, and p m' is summed per group and query, on the
+//     side.  That weight is rounded to 11 bits (8 times finer than the result's bf16); it is scaled by a power of two
+//     that follows the largest s' seen.  Scores, statistics and sums are fp32.
 // Both products run transposed on mma.sync, the query rows (query heads of the KV head times T) being the n = 8
 // side: S^T = K Q^T (16 tokens x rows), O^T = V^T P^T.  The k index of the first product runs over the channels
 // in the order in which a lane's words hold them (Q is stored in that order); the tokens of the second are
 // permuted (tile_token) so that lanes reading the same word of different tokens fall into different banks.
-// Up to 4 rows (RT = 0) fill the 8 columns as well: two planes each in the first product, the two halves of a masked
-// word (two channels of one token) in the second, which halves its accumulators.
+// Up to 4 rows (RT = 0) take every other column of the first product, and all 8 of the second: the two halves of a
+// masked word (two channels of one token) have one each, which halves its accumulators.
 //
 // Work split: the cache of an item (sequence, KV head, chunk of query rows) is a run of records of 16 tokens.
 // The records of the whole batch are laid end to end and divided evenly over the resident warps, whatever the
@@ -34,10 +32,10 @@
 // worker order by a second small kernel: no atomics, nothing to clear, the same bits every time.
 //
 // Measured on a B200 (6.55 TB/s copy), device time with inputs turned over: 64 sequences of 1024-2048 tokens, 32 query
-// and 8 KV heads of 128: 28.0 us for 115 MB, of which 3.5 us pass before the first copy, 18 until the median worker has
-// seen its records, at the rate of memory, and 6 in the last workers and the join.  One sequence of 131072: 34.6 us
-// (151 MB).  16 sequences of 4096-8192, 16 query and 8 KV heads of 256, capped: 45.0 us (226 MB, 5.0 TB/s).  5 query
-// tokens of 4 sequences of 16K-32K: 58.2 us (115 MB), bound by what 8 warps of an SM can issue.  One short sequence:
+// and 8 KV heads of 128: 28.8 us for 115 MB, of which 3.5 us pass before the first copy, 18 until the median worker has
+// seen its records, at the rate of memory, and 6 in the last workers and the join.  One sequence of 131072: 35.4 us
+// (151 MB).  16 sequences of 4096-8192, 16 query and 8 KV heads of 256, capped: 47.1 us (226 MB, 4.8 TB/s).  5 query
+// tokens of 4 sequences of 16K-32K: 59.2 us (115 MB), bound by what 8 warps of an SM can issue.  One short sequence:
 // 6.4 us, latency.
 #include <climits>
 #include <type_traits>
@@ -64,19 +62,14 @@ constexpr float kScaleMax = 512.0f;  // of s' times its scaling; a new scaling p
 constexpr int kScaleTarget = 7;
 constexpr float kFltMax = 3.40282347e38f;
 constexpr float kNone = -kFltMax;     // reference of a row without a key: no special cases, any score passes it
-constexpr float kMagic = 12582912.0f; // 1.5 * 2^23: its bits plus a small integer are the bits of the sum
-constexpr int kMagicBits = 0x4B400000;
 
 // RT: 0 = up to 4 query rows per chunk, else up to 8 RT.
 template <int RT>
 struct Kv4Rows {
-  static constexpr int NT = RT == 0 ? 1 : RT;       // n = 8 tiles of the second product
-  static constexpr int KT = RT == 0 ? 1 : 2 * RT;   // of the first
+  static constexpr int NT = RT == 0 ? 1 : RT;       // n = 8 tiles
   static constexpr int NC = RT == 0 ? 1 : 2 * RT;   // rows per lane
   static constexpr int ROWS = RT == 0 ? 4 : 8 * RT;
-  // fp16 operands for the scores: with two or three row tiles the second integer plane costs more (its sums are put
-  // together score by score) than the two more operations a word.
-  static constexpr bool HALF_K = RT > 1;
+  static constexpr bool HOLD_Q = RT < 2;            // the rows' factors and sums of q stay in registers
 };
 
 // BURST: records that a warp takes at once (one wait, one refill); STAGES of them are held, so that
@@ -162,21 +155,6 @@ __device__ __forceinline__ void mma_f16_16816(float (&d)[4], uint32_t a0, uint32
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
-__device__ __forceinline__ void mma_u8s8_16832(int (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
-                                               uint32_t b0, uint32_t b1) {
-  asm("mma.sync.aligned.m16n8k32.row.col.s32.u8.s8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
-      "{%0, %1, %2, %3};"
-      : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3])
-      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-}
-// The first step of a sum: every element starts at `init`.
-__device__ __forceinline__ void mma_u8s8_16832_from(int (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
-                                                    uint32_t b0, uint32_t b1, int init) {
-  asm("mma.sync.aligned.m16n8k32.row.col.s32.u8.s8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
-      "{%10, %10, %10, %10};"
-      : "=r"(d[0]), "=r"(d[1]), "=r"(d[2]), "=r"(d[3])
-      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "r"(init));
-}
 __device__ __forceinline__ void mma_f16_16816_zero(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
                                                    uint32_t b0, uint32_t b1) {
   asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
@@ -260,11 +238,11 @@ __device__ __forceinline__ int2 kv4_records(const Kv4AttnArgs& a, const Kv4Seq& 
 template <int D, int RT>
 struct Kv4Smem {
   static constexpr int STAGES = Kv4Cfg<D, RT>::STAGES, ROWS = Kv4Rows<RT>::ROWS;
-  // per warp: the ring, Q operands [D / 32][KT][32 lanes] x 8 bytes, per row the score factor, the
+  // per warp: the ring, Q operands [D / 32][NT][32 lanes] x 16 bytes, per row the score factor, the
   // sums of q per group and the number of keys it sees, the ring's barriers
   static constexpr int RING = STAGES * Kv4Cfg<D, RT>::BURST * Kv4<D>::RECORD;
   static constexpr int QF = RING;
-  static constexpr int COL = QF + D / 32 * Kv4Rows<RT>::KT * 256;
+  static constexpr int COL = QF + D / 32 * Kv4Rows<RT>::NT * 512;
   static constexpr int BAR = (COL + ROWS * (2 + Kv4<D>::NG) * 4 + 7) / 8 * 8;
   static constexpr int WARP = (BAR + STAGES * 8 + 127) / 128 * 128;
   static constexpr int BYTES = Kv4Cfg<D, RT>::WARPS * WARP;
@@ -275,7 +253,7 @@ __global__ void __launch_bounds__(Kv4Cfg<D, RT>::WARPS * 32, 1) kv4_attn_kernel(
   using P = Kv4<D>;
   using S = Kv4Smem<D, RT>;
   using R = Kv4Rows<RT>;
-  constexpr int NG = P::NG, STAGES = S::STAGES, ROWS = R::ROWS, NT = R::NT, KT = R::KT, NC = R::NC;
+  constexpr int NG = P::NG, STAGES = S::STAGES, ROWS = R::ROWS, NT = R::NT, NC = R::NC;
   constexpr int BURST = Kv4Cfg<D, RT>::BURST, MATH = Kv4Cfg<D, RT>::MATH, WARPS = Kv4Cfg<D, RT>::WARPS;
   constexpr unsigned ALL = (1u << BURST) - 1;
   extern __shared__ __align__(128) uint8_t smem[];
@@ -284,7 +262,7 @@ __global__ void __launch_bounds__(Kv4Cfg<D, RT>::WARPS * 32, 1) kv4_attn_kernel(
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int g = lane >> 2, c = lane & 3;
   uint8_t* ring = smem + warp * S::WARP;
-  uint2* qf = reinterpret_cast<uint2*>(ring + S::QF);
+  uint4* qf = reinterpret_cast<uint4*>(ring + S::QF);
   float* col_f = reinterpret_cast<float*>(ring + S::COL);
   float* col_q = col_f + ROWS;  // [ROWS][NG]
   int* col_see = reinterpret_cast<int*>(col_q + ROWS * NG);
@@ -292,6 +270,9 @@ __global__ void __launch_bounds__(Kv4Cfg<D, RT>::WARPS * 32, 1) kv4_attn_kernel(
 
   pdl_launch_dependents();
   if (lane < STAGES) mbar_init(bars + lane, 1);
+  if constexpr (RT == 0)
+#pragma unroll
+    for (int i = 0; i < 2 * NG; ++i) qf[i * 32 + lane] = make_uint4(0u, 0u, 0u, 0u);  // the columns without a row
   fence_barrier_init();
   if (tid == 0) abort_flag = 0;
   __syncthreads();
@@ -452,8 +433,7 @@ __global__ void __launch_bounds__(Kv4Cfg<D, RT>::WARPS * 32, 1) kv4_attn_kernel(
     const int rows = min(a.group * a.T - row0, ROWS);
     const int2 span = kv4_records<BURST>(a, sq, ra, n_rounds);
 
-    // Q of the item in the order of the first product's operands: round(32512 q / max |q|) = 256 hi + lo as signed
-    // bytes, or fp16
+    // Q of the item in the order of the first product's operands
     __syncwarp();
 #pragma unroll 1
     for (int pass0 = 0; pass0 < PASSES && span.x < span.y; pass0 += TAKE) {
@@ -473,58 +453,29 @@ __global__ void __launch_bounds__(Kv4Cfg<D, RT>::WARPS * 32, 1) kv4_attn_kernel(
 #pragma unroll
         for (int o = 1; o < 8; o <<= 1) big = max(big, __shfl_xor_sync(0xffffffffu, big, o));
         const bool fine = big < 0x7f800000u;
-        if constexpr (R::HALF_K) {
-          // times a power of two that puts the largest magnitude into [2^10, 2^11): exact in fp16 but for what lies
-          // 2^-25 below that
-          const int e = big > 0 && fine ? min(max(137 - static_cast<int>(big >> 23), -126), 126) : 0;
-          const float up = __uint_as_float(static_cast<uint32_t>(e + 127) << 23);
+        // times a power of two that puts the largest magnitude into [2^10, 2^11)
+        const int e = big > 0 && fine ? min(max(137 - static_cast<int>(big >> 23), -126), 126) : 0;
+        const float up = __uint_as_float(static_cast<uint32_t>(e + 127) << 23);
 #pragma unroll
-          for (int k = 0; k < NG; ++k) {
-            const uint32_t x[4] = {raw[k].x, raw[k].y, raw[k].z, raw[k].w};
-            float v[8], sum = 0.0f;
+        for (int k = 0; k < NG; ++k) {
+          const uint32_t x[4] = {raw[k].x, raw[k].y, raw[k].z, raw[k].w};
+          float v[8], sum = 0.0f;
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-              v[j] = fine ? __uint_as_float((j & 1) ? x[j >> 1] & 0xffff0000u : x[j >> 1] << 16) * up : 0.0f;
-              sum += v[j];
-            }
-            // word w of the group is word w % 2 of lane w / 2; codes 2 h and 2 h + 4 are the first operand of half h,
-            // 2 h + 1 and 2 h + 5 the second, which stands 4 bits higher
-#pragma unroll
-            for (int hh = 0; hh < 2; ++hh)
-              qf[(((k * 2 + (w & 1)) * 2 + hh) * NT + r / 8) * 32 + (r % 8) * 4 + (w >> 1)] =
-                  make_uint2(pack_f16(v[2 * hh] * 16.0f, v[2 * hh + 4] * 16.0f), pack_f16(v[2 * hh + 1], v[2 * hh + 5]));
-#pragma unroll
-            for (int o = 1; o < 8; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-            if (w == 0) col_q[r * NG + k] = sum * 0x1p-20f;
+          for (int j = 0; j < 8; ++j) {
+            v[j] = fine ? __uint_as_float((j & 1) ? x[j >> 1] & 0xffff0000u : x[j >> 1] << 16) * up : 0.0f;
+            sum += v[j];
           }
-          if (w == 0) col_f[r] = !fine ? __int_as_float(0x7fc00000) : ldexpf(a.score_scale, 20 - e);
-        } else {
-          const float up = big > 0 && fine ? fminf(32512.0f / __uint_as_float(big), 1e38f) : 0.0f;
-          const int n0 = RT == 0 ? 2 * r : r % 8, t0 = RT == 0 ? 0 : 2 * (r / 8);
-          const int n1 = RT == 0 ? 2 * r + 1 : r % 8, t1 = RT == 0 ? 0 : t0 + 1;
+          // word w of the group is word w % 2 of lane w / 2; codes 2 h and 2 h + 4 are the first operand of half h,
+          // 2 h + 1 and 2 h + 5 the second, which stands 4 bits higher
+          const int col = RT == 0 ? 2 * r : r % 8;
+          qf[((k * 2 + (w & 1)) * NT + (RT == 0 ? 0 : r / 8)) * 32 + col * 4 + (w >> 1)] =
+              make_uint4(pack_f16(v[0] * 16.0f, v[4] * 16.0f), pack_f16(v[1], v[5]),
+                         pack_f16(v[2] * 16.0f, v[6] * 16.0f), pack_f16(v[3], v[7]));
 #pragma unroll
-          for (int k = 0; k < NG; ++k) {
-            const uint32_t x[4] = {raw[k].x, raw[k].y, raw[k].z, raw[k].w};
-            // word w of the group is word w % 2 of lane w / 2; its even codes are the first operand, the odd ones the second
-            uint32_t hi[2] = {0, 0}, lo[2] = {0, 0};
-            int sum = 0;
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-              const float xv = __uint_as_float((j & 1) ? x[j >> 1] & 0xffff0000u : x[j >> 1] << 16);
-              const int v = fine ? __float2int_rn(xv * up) : 0, vh = (v + 128) >> 8;
-              sum += v;
-              hi[j & 1] |= (static_cast<uint32_t>(vh) & 255u) << (8 * (j >> 1));
-              lo[j & 1] |= (static_cast<uint32_t>(v) & 255u) << (8 * (j >> 1));  // v - 256 vh in its low byte
-            }
-            const int ks = k * 2 + (w & 1);
-            qf[(ks * KT + t0) * 32 + n0 * 4 + (w >> 1)] = make_uint2(hi[0], hi[1]);
-            qf[(ks * KT + t1) * 32 + n1 * 4 + (w >> 1)] = make_uint2(lo[0], lo[1]);
-#pragma unroll
-            for (int o = 1; o < 8; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-            if (w == 0) col_q[r * NG + k] = static_cast<float>(sum);
-          }
-          if (w == 0) col_f[r] = !fine ? __int_as_float(0x7fc00000) : up > 0.0f ? a.score_scale / up : 0.0f;
+          for (int o = 1; o < 8; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+          if (w == 0) col_q[r * NG + k] = sum;
         }
+        if (w == 0) col_f[r] = !fine ? __int_as_float(0x7fc00000) : ldexpf(a.score_scale, -e);
       }
     }
     __syncwarp();
@@ -540,7 +491,7 @@ __global__ void __launch_bounds__(Kv4Cfg<D, RT>::WARPS * 32, 1) kv4_attn_kernel(
         for (int k = 0; k < NG; ++k) qs[q][k] = col_q[row_of(q) * NG + k];
     };
     float f_item[NC], qs_item[NC][NG];
-    if constexpr (!R::HALF_K) load_f(f_item), load_qs(qs_item);
+    if constexpr (R::HOLD_Q) load_f(f_item), load_qs(qs_item);
     const int see_least = col_see[0], see_most = col_see[rows - 1];  // keys that the first and the last row see
 
     // m tiles of 16 x 8 outputs.  RT > 0: (group, high half of the word, half of that), 16 channels x 8 rows each;
@@ -571,9 +522,9 @@ __global__ void __launch_bounds__(Kv4Cfg<D, RT>::WARPS * 32, 1) kv4_attn_kernel(
       constexpr bool MASKED = decltype(masked_tag)::value;
       asm volatile("" ::: "memory");  // Q is read from shared memory each time: held in registers it would spill
       float f_own[NC], qs_own[NC][NG];
-      if constexpr (R::HALF_K) load_f(f_own), load_qs(qs_own);
-      const float(&f)[NC] = R::HALF_K ? f_own : f_item;
-      const float(&qs)[NC][NG] = R::HALF_K ? qs_own : qs_item;
+      if constexpr (!R::HOLD_Q) load_f(f_own), load_qs(qs_own);
+      const float(&f)[NC] = R::HOLD_Q ? f_item : f_own;
+      const float(&qs)[NC][NG] = R::HOLD_Q ? qs_item : qs_own;
       // ---- scores
       float s[MATH][2][NC];
 #pragma unroll
@@ -587,67 +538,42 @@ __global__ void __launch_bounds__(Kv4Cfg<D, RT>::WARPS * 32, 1) kv4_attn_kernel(
         }
 #pragma unroll
         for (int k = 0; k < NG; ++k) {
-          if constexpr (R::HALF_K) {
-            float acc[NT][4];
+          float acc[NT][4];
 #pragma unroll
-            for (int wi = 0; wi < 2; ++wi)
+          for (int wi = 0; wi < 2; ++wi) {
+            uint4 b[NT];
 #pragma unroll
-              for (int hh = 0; hh < 2; ++hh) {
-                const uint32_t x0 = kw[0][NG * wi + k] >> (8 * hh), x1 = kw[1][NG * wi + k] >> (8 * hh);
-                const uint32_t a0 = x0 & 0x000F000Fu, a1 = x1 & 0x000F000Fu, a2 = x0 & 0x00F000F0u,
-                               a3 = x1 & 0x00F000F0u;
+            for (int nt = 0; nt < NT; ++nt) b[nt] = qf[((k * 2 + wi) * NT + nt) * 32 + lane];
 #pragma unroll
-                for (int nt = 0; nt < NT; ++nt) {
-                  const uint2 b = qf[(((k * 2 + wi) * 2 + hh) * NT + nt) * 32 + lane];
-                  if (wi + hh == 0)
-                    mma_f16_16816_zero(acc[nt], a0, a1, a2, a3, b.x, b.y);
-                  else
-                    mma_f16_16816(acc[nt], a0, a1, a2, a3, b.x, b.y);
-                }
-              }
+            for (int hh = 0; hh < 2; ++hh) {
+              const uint32_t x0 = kw[0][NG * wi + k] >> (8 * hh), x1 = kw[1][NG * wi + k] >> (8 * hh);
+              const uint32_t a0 = x0 & 0x000F000Fu, a1 = x1 & 0x000F000Fu, a2 = x0 & 0x00F000F0u,
+                             a3 = x1 & 0x00F000F0u;
 #pragma unroll
-            for (int e = 0; e < 2; ++e)
-#pragma unroll
-              for (int q = 0; q < NC; q += 2) {
-                const float ps = pair_scale(kp[e][k]), pm = pair_min(kp[e][k]);
-                const F2 dot = {acc[(q >> 1) % NT][2 * e], acc[(q >> 1) % NT][2 * e + 1]};
-                const F2 part = k == 0 ? mul2({ps, ps}, dot) : fma2({ps, ps}, dot, {s[u][e][q], s[u][e][q + 1]});
-                const F2 sum = fma2({pm, pm}, {qs[q][k], qs[q + 1][k]}, part);
-                s[u][e][q] = sum.x, s[u][e][q + 1] = sum.y;
-              }
-          } else {
-            int acc[KT][4];
-#pragma unroll
-            for (int wi = 0; wi < 2; ++wi) {
-              const uint32_t w0 = kw[0][NG * wi + k], w1 = kw[1][NG * wi + k];
-              const uint32_t a0 = w0 & 0x0F0F0F0Fu, a1 = w1 & 0x0F0F0F0Fu, a2 = (w0 >> 4) & 0x0F0F0F0Fu,
-                             a3 = (w1 >> 4) & 0x0F0F0F0Fu;
-#pragma unroll
-              for (int nt = 0; nt < KT; ++nt) {
-                const uint2 b = qf[((k * 2 + wi) * KT + nt) * 32 + lane];
-                if (wi == 0)
-                  mma_u8s8_16832_from(acc[nt], a0, a1, a2, a3, b.x, b.y, kMagicBits);
+              for (int nt = 0; nt < NT; ++nt) {
+                const uint32_t b0 = hh ? b[nt].z : b[nt].x, b1 = hh ? b[nt].w : b[nt].y;
+                if (wi + hh == 0)
+                  mma_f16_16816_zero(acc[nt], a0, a1, a2, a3, b0, b1);
                 else
-                  mma_u8s8_16832(acc[nt], a0, a1, a2, a3, b.x, b.y);
+                  mma_f16_16816(acc[nt], a0, a1, a2, a3, b0, b1);
               }
             }
-            // two scores at a time: of both tokens of the row (RT = 0), or of two rows
+          }
+          // The products are 2^-20 of what they stand for: made good on the scales, so that neither a row's factor nor
+          // a small key's score leaves fp32's range.  Two scores at a time: of both tokens of the row (RT = 0), or of
+          // two rows.
+          const F2 scales = mul2({pair_scale(kp[0][k]), pair_scale(kp[1][k])}, {0x1p20f, 0x1p20f});
 #pragma unroll
-            for (int i = 0; i < NC; ++i) {
-              const int e = RT == 0 ? 0 : i & 1, q = RT == 0 ? 0 : i & ~1;
-              const int e1 = RT == 0 ? 1 : e, q1 = RT == 0 ? 0 : q + 1;
-              const int th = RT == 0 ? 0 : q % KT, tl = RT == 0 ? 0 : (q + 1) % KT;  // tiles of the planes
-              const F2 hi = {__int_as_float(acc[th][2 * e]), __int_as_float(acc[th][RT == 0 ? 2 : 2 * e + 1])};
-              const F2 lo = {__int_as_float(acc[tl][RT == 0 ? 1 : 2 * e]),
-                             __int_as_float(acc[tl][RT == 0 ? 3 : 2 * e + 1])};
-              const F2 off = {-kMagic, -kMagic}, up = {256.0f, 256.0f};
-              const F2 dot = fma2(add2(hi, off), up, add2(lo, off));
-              const F2 ps = {pair_scale(kp[e][k]), pair_scale(kp[e1][k])};
-              const F2 pm = {pair_min(kp[e][k]), pair_min(kp[e1][k])};
-              const F2 part = k == 0 ? mul2(ps, dot) : fma2(ps, dot, {s[u][e][q], s[u][e1][q1]});
-              const F2 sum = fma2(pm, {qs[q][k], qs[q1][k]}, part);
-              s[u][e][q] = sum.x, s[u][e1][q1] = sum.y;
-            }
+          for (int i = 0; i < NC; ++i) {
+            const int e = RT == 0 ? 0 : i & 1, q = RT == 0 ? 0 : i & ~1;
+            const int e1 = RT == 0 ? 1 : e, q1 = RT == 0 ? 0 : q + 1;
+            const int nt = (q >> 1) % NT;
+            const F2 dot = {acc[nt][2 * e], RT == 0 ? acc[nt][2] : acc[nt][2 * e + 1]};
+            const F2 ps = {e ? scales.y : scales.x, e1 ? scales.y : scales.x};
+            const F2 pm = {pair_min(kp[e][k]), pair_min(kp[e1][k])};
+            const F2 part = k == 0 ? mul2(ps, dot) : fma2(ps, dot, {s[u][e][q], s[u][e1][q1]});
+            const F2 sum = fma2(pm, {qs[q][k], qs[q1][k]}, part);
+            s[u][e][q] = sum.x, s[u][e1][q1] = sum.y;
           }
         }
         if constexpr (CAP)

@@ -89,8 +89,8 @@ def attention(q, pool, layer, tables, ctx, scale, softcap=0.0, window=0):
             if softcap:
                 z = softcap * torch.tanh(z / softcap)
             out[b, t] = torch.einsum("hrn,nhd->hrd", z.softmax(-1), vv).flatten(0, 1)
-            # Score: q is held in 16 bits of its row's largest magnitude (half a step of |q|max / 32512 a channel, against
-            # k), and at most D + 64 fp32 roundings of terms whose magnitudes sum to m (the products, or scale * code
+            # Score: room for a q in 16 bits of its row's largest magnitude (half a step of |q|max / 32512 a channel, against
+            # k; attention_each has none), and at most D + 64 fp32 roundings of terms whose magnitudes sum to m (the products, or scale * code
             # products and the min's part, each within 4 times |q| |k|max).  The softmax turns an error d of the scores
             # into 2 d of a weight.  Weights: rounded to 11 bits before the product with the codes (2^-11 of the
             # span of a group), plus 2^-21 for exp2 and sums.
@@ -102,6 +102,70 @@ def attention(q, pool, layer, tables, ctx, scale, softcap=0.0, window=0):
             tol[b, t] = (weight[..., None] * vmax + 2.0 ** -11 * 1.1 * (span + 2.0 ** -10 * vmax)).expand(
                 -1, -1, D).flatten(0, 1)
     return out, tol + out.abs() * 2.0 ** -8                            # and the rounding of the result to bf16
+
+
+def attention_each(q, pool, layer, tables, ctx, scale, softcap=0.0, window=0):
+    """The same, with a bound for each output by itself: from what its row's scores and the values of its group of
+    channels, weighted as they are, can lose.
+
+    A score is sum_g s_g (q_g . u_g) + m_g sum(q_g), with q exact.  With M = sum |q| (|k - m| + |m|) of the key, its terms
+    magnitude by magnitude, fp32 sums of 64 terms, truncated by the matrix instruction (2^-23 each, a running sum and a
+    term), and some 2 a group and 8 more roundings put it off by (4 * 64 + 2 groups + 8) 2^-24 M; a capped score by 2^-21
+    of the cap more; its factor, its distance to the reference and exp2 by 2^-22 of its magnitude and 2^-21 of the weight.
+    An error e_n of weight n moves the output by p_n e_n (v_n - out).  The weight in the product with the codes is rounded
+    to 11 bits: 2^-11 p_n |v_n - m_n|.  Below 2^-14 of 2^7 times the largest weight in the output's own row and group (that
+    is where it is scaled to, at least) it is off by 2^-32 of that one, times 15.  fp32 sums of the outputs, over 16 keys at
+    a time, lose 2^-23 of the magnitudes each, twice where a part is scaled again and joined."""
+    B, T, Hq, D = q.shape
+    heads, bs, ng = pool.shape[2], 16 * pool.shape[3], q.shape[-1] // 64
+    out = torch.zeros(B, T, Hq, D, dtype=torch.float64, device=q.device)
+    tol = torch.zeros_like(out)
+    for b in range(B):
+        n = int(ctx[b])
+        if n <= 0:
+            continue
+        blocks = tables[b, :(n + bs - 1) // bs].tolist()
+        assert len(blocks) * bs >= n and all(0 <= i < pool.shape[1] for i in blocks)   # before the GPU indexes with them
+        at = torch.tensor(blocks, device=pool.device)
+        k, v = unpack(pool, layer, at)
+        km, vm = mins(pool, layer, at)                                  # [tokens, heads, D]: the group's min
+        for t in range(T):
+            end = n - T + 1 + t
+            lo = max(0, end - window) if window else 0
+            if end <= lo:
+                continue
+            qt = q[b, t].double().unflatten(0, (heads, Hq // heads))
+            z = torch.einsum("hrd,nhd->hrn", qt, k[lo:end]) * scale
+            M = torch.einsum("hrd,nhd->hrn", qt.abs(), (k - km)[lo:end].abs() + km[lo:end].abs()) * abs(scale)
+            off = (4 * 64 + 2 * ng + 8) * 2.0 ** -24 * M
+            if softcap:
+                z = softcap * torch.tanh(z / softcap)
+                off = off + 2.0 ** -21 * softcap
+            p = z.softmax(-1)
+            off = off + 2.0 ** -22 * (z.abs() + z.amax(-1, keepdim=True).abs()) + 2.0 ** -21
+            vv, part = v[lo:end], (v - vm)[lo:end].abs()
+            o = torch.einsum("hrn,nhd->hrd", p, vv)
+            away = (vv.permute(1, 0, 2)[:, None] - o[:, :, None]).abs()  # [heads, rows, n, D]
+            err = torch.einsum("hrn,hrnd->hrd", p * off, away) * 1.05
+            err = err + 2.0 ** -11 * torch.einsum("hrn,nhd->hrd", p, part)
+            top = (p[..., None] * part.permute(1, 0, 2)[:, None]).unflatten(-1, (ng, 64)).amax((2, 4))   # of the group
+            err = err + 2.0 ** -32 * 15 * (end - lo) * top.repeat_interleave(64, -1)
+            steps = (end - lo) // 16 + 4
+            err = err + 2.0 ** -22 * steps * torch.einsum("hrn,nhd->hrd", p, part + vm[lo:end].abs())
+            out[b, t], tol[b, t] = o.flatten(0, 1), err.flatten(0, 1)
+    return out, tol + out.abs() * 2.0 ** -8                            # and the rounding of the result to bf16
+
+
+def mins(pool, layer, blocks):
+    """The group minima of K and V of all tokens of `blocks`, [tokens, heads, D] in 64 bits."""
+    r = pool[layer, blocks].permute(0, 2, 1, 3).flatten(0, 1)
+    D = pool.shape[-1] // 18
+
+    def of(at):
+        p = r[..., at:at + D].contiguous().view(torch.bfloat16).double().reshape(*r.shape[:2], 16, D // 64, 2)[..., 1]
+        return p.permute(0, 2, 1, 3).flatten(0, 1).repeat_interleave(64, -1)
+
+    return of(16 * D), of(17 * D)
 
 
 # ------------------------------------------------------------------ slots
