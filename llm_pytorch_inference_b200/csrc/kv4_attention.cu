@@ -15,8 +15,12 @@
 //     operation a word less, took 28.0 us where this takes 28.8 and 45.0 where this takes 47.1, but left q 16 bits of
 //     its row's largest magnitude, which loses the small channels beside a large one.)
 //   * Outputs: the weight of a token times s' is the other operand, and p m' is summed per group and query, on the
-//     side.  That weight is rounded to 11 bits (8 times finer than the result's bf16); it is scaled by a power of two
-//     that follows the largest s' seen.  Scores, statistics and sums are fp32.
+//     side.  That product p s' is rounded to 11 bits (8 times finer than the result's bf16).  It is scaled by a power of
+//     two of its row and group, which follows the products themselves (choose_scale): a value scale however large does
+//     not cost the others their bits unless its token has the weight to matter.  (One scaling for all groups and rows,
+//     following the largest s', took 28.8 us where this takes 29.3 and 58.7 where this takes 63.5; it lost a group of
+//     2^-14 of its neighbour's values 0.5 %, and all that came after a value of 2^20 30 %.  Value scales that vary by
+//     2^4 either way cost another 8 to 17 %.)  Scores, statistics and sums are fp32.
 // Both products run transposed on mma.sync, the query rows (query heads of the KV head times T) being the n = 8
 // side: S^T = K Q^T (16 tokens x rows), O^T = V^T P^T.  The k index of the first product runs over the channels
 // in the order in which a lane's words hold them (Q is stored in that order); the tokens of the second are
@@ -32,10 +36,10 @@
 // worker order by a second small kernel: no atomics, nothing to clear, the same bits every time.
 //
 // Measured on a B200 (6.55 TB/s copy), device time with inputs turned over: 64 sequences of 1024-2048 tokens, 32 query
-// and 8 KV heads of 128: 28.8 us for 115 MB, of which 3.5 us pass before the first copy, 18 until the median worker has
-// seen its records, at the rate of memory, and 6 in the last workers and the join.  One sequence of 131072: 35.4 us
-// (151 MB).  16 sequences of 4096-8192, 16 query and 8 KV heads of 256, capped: 47.1 us (226 MB, 4.8 TB/s).  5 query
-// tokens of 4 sequences of 16K-32K: 59.2 us (115 MB), bound by what 8 warps of an SM can issue.  One short sequence:
+// and 8 KV heads of 128: 29.3 us for 115 MB, of which 3.5 us pass before the first copy, 18 until the median worker has
+// seen its records, at the rate of memory, and 6 in the last workers and the join.  One sequence of 131072: 35.8 us
+// (151 MB).  16 sequences of 4096-8192, 16 query and 8 KV heads of 256, capped: 48.0 us (226 MB, 4.7 TB/s).  5 query
+// tokens of 4 sequences of 16K-32K: 63.5 us (115 MB), bound by what 8 warps of an SM can issue.  One short sequence:
 // 6.4 us, latency.
 #include <climits>
 #include <type_traits>
@@ -58,8 +62,9 @@ constexpr int kItemCost = 3;
 // once a score passes it by more than kSlack (in powers of two), so that most records cost one vote instead
 // of a reduction.  The weight times the scaled s' stays below 2^(kSlack + 9) = 2^15 in fp16.
 constexpr float kSlack = 6.0f;
-constexpr float kScaleMax = 512.0f;  // of s' times its scaling; a new scaling puts the largest s' into [2^7, 2^8)
-constexpr int kScaleTarget = 7;
+constexpr float kScaleMax = 512.0f;  // of s' times its scaling, where nothing else was chosen
+constexpr int kFirstScale = 120;     // log2 of the scaling before any s', and its largest: times 2^kSlack in fp32's range
+constexpr int kNothing = -10000;     // log2 of zero
 constexpr float kFltMax = 3.40282347e38f;
 constexpr float kNone = -kFltMax;     // reference of a row without a key: no special cases, any score passes it
 
@@ -136,6 +141,24 @@ struct Kv4Split {
                  : static_cast<int>(more) + static_cast<uint32_t>(y) / static_cast<uint32_t>(size);
   }
 };
+
+// floor(log2 x) of x >= 0, at least -127 for numbers above zero.
+__device__ __forceinline__ int log2_of(float x) {
+  return x > 0.0f ? static_cast<int>(__float_as_uint(x) >> 23) - 127 : kNothing;
+}
+__device__ __forceinline__ float power_of_2(int e) { return __uint_as_float(static_cast<uint32_t>(e + 127) << 23); }
+// log2 of the scaling of a row's products p s' in a group of channels, from logarithms: `old`, the present one;
+// s, the largest s' of the records at hand; w, their largest product; o, what has been summed, as the sum of products
+// that it stands for.  In fp16 a product below 2^-14 loses bits and is off by 2^-25 at most: the n products of a worker
+// keep all but n 2^-25 of the largest one, or of their sum, where that is scaled to 2^0 or above.  The scaling stays while
+// s' is within kScaleMax, and falls to where s' is within it, both while the products keep their bits; else it stays as
+// long as the products themselves fit, and else follows them.
+__device__ __forceinline__ int choose_scale(int old, int s, int w, int o) {
+  const int most = max(w, o);
+  int e = s + old <= 8 ? old : 7 - s;
+  if (most > kNothing && e + most < 0) e = old + most >= 0 && old + w <= 8 ? old : 7 - most;
+  return min(max(e, -kFirstScale), kFirstScale);
+}
 
 // exp2 with results below 2^-126 flushed to zero.
 __device__ __forceinline__ float ex2(float x) {
@@ -239,13 +262,14 @@ template <int D, int RT>
 struct Kv4Smem {
   static constexpr int STAGES = Kv4Cfg<D, RT>::STAGES, ROWS = Kv4Rows<RT>::ROWS;
   // per warp: the ring, Q operands [D / 32][NT][32 lanes] x 16 bytes, per row the score factor, the
-  // sums of q per group and the number of keys it sees, the ring's barriers
+  // sums of q and the scalings per group and the number of keys it sees, room to choose scalings, the ring's barriers
   static constexpr int RING = STAGES * Kv4Cfg<D, RT>::BURST * Kv4<D>::RECORD;
   static constexpr int QF = RING;
   static constexpr int COL = QF + D / 32 * Kv4Rows<RT>::NT * 512;
-  static constexpr int BAR = (COL + ROWS * (2 + Kv4<D>::NG) * 4 + 7) / 8 * 8;
+  static constexpr int BAR = (COL + ROWS * (3 + 4 * Kv4<D>::NG) * 4 + 7) / 8 * 8;
   static constexpr int WARP = (BAR + STAGES * 8 + 127) / 128 * 128;
   static constexpr int BYTES = Kv4Cfg<D, RT>::WARPS * WARP;
+  static_assert(BYTES + 1024 <= 227 * 1024, "shared memory of an SM");
 };
 
 template <int D, int RT, bool CAP>
@@ -255,7 +279,7 @@ __global__ void __launch_bounds__(Kv4Cfg<D, RT>::WARPS * 32, 1) kv4_attn_kernel(
   using R = Kv4Rows<RT>;
   constexpr int NG = P::NG, STAGES = S::STAGES, ROWS = R::ROWS, NT = R::NT, NC = R::NC;
   constexpr int BURST = Kv4Cfg<D, RT>::BURST, MATH = Kv4Cfg<D, RT>::MATH, WARPS = Kv4Cfg<D, RT>::WARPS;
-  constexpr unsigned ALL = (1u << BURST) - 1;
+  constexpr unsigned ALL = (1u << BURST) - 1, MATH_ALL = (1u << MATH) - 1;
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ volatile int abort_flag;
   __shared__ Kv4Split split;
@@ -265,7 +289,11 @@ __global__ void __launch_bounds__(Kv4Cfg<D, RT>::WARPS * 32, 1) kv4_attn_kernel(
   uint4* qf = reinterpret_cast<uint4*>(ring + S::QF);
   float* col_f = reinterpret_cast<float*>(ring + S::COL);
   float* col_q = col_f + ROWS;  // [ROWS][NG]
-  int* col_see = reinterpret_cast<int*>(col_q + ROWS * NG);
+  float* col_v = col_q + ROWS * NG;  // [ROWS][NG], where the rows' scalings differ
+  int* col_see = reinterpret_cast<int*>(col_v + ROWS * NG);
+  int* row_w = col_see + ROWS;    // [ROWS][NG]
+  int* row_o = row_w + ROWS * NG;
+  float* row_drop = reinterpret_cast<float*>(row_o + ROWS * NG);
   uint64_t* bars = reinterpret_cast<uint64_t*>(ring + S::BAR);
 
   pdl_launch_dependents();
@@ -508,27 +536,43 @@ __global__ void __launch_bounds__(Kv4Cfg<D, RT>::WARPS * 32, 1) kv4_attn_kernel(
 #pragma unroll
     for (int q = 0; q < NC; ++q) {
       l[q] = 0.0f;
-      mref[q] = kNone;
+      mref[q] = row_of(q) < rows ? kNone : kFltMax;  // a column without a row: no score passes it
 #pragma unroll
       for (int k = 0; k < NG; ++k) mo[q][k] = 0.0f;
     }
-    // power of two that the value scales are multiplied by, and what the products may reach: chosen at the first scale
-    // above zero (until then the outputs hold nothing but zeros), and only ever lowered after that
-    float vscale = 1.0f, limit = 0.0f;
+    // Scaling of the products p s' per group: the lane's row's (RT = 0), or the largest of the rows', which is that of
+    // all of them while `same`
+    float vscale[NG];
+#pragma unroll
+    for (int k = 0; k < NG; ++k) vscale[k] = power_of_2(kFirstScale);
+    bool same = true;
     bool none = true;  // no reference chosen: nothing summed yet
 
-    // One burst from record t on, `have`: which of its records came.  MASKED: some row does not see some token.
-    auto burst = [&](auto masked_tag, int t, unsigned have, const uint8_t* recs) {
+    auto load_v = [&](float (&v)[NC][NG]) {
+#pragma unroll
+      for (int q = 0; q < NC; ++q)
+#pragma unroll
+        for (int k = 0; k < NG; ++k) v[q][k] = vscale[k];
+      if (RT > 0 && !same)
+#pragma unroll
+        for (int q = 0; q < NC; ++q)
+#pragma unroll
+          for (int k = 0; k < NG; ++k) v[q][k] = col_v[row_of(q) * NG + k];
+    };
+    // MATH records from record t on, or with MASKED one: some row does not see some token, or the rows' scalings differ
+    // or have to be chosen one by one; without it the records are left undone, false, where they have.
+    auto burst = [&](auto masked_tag, int t, const uint8_t* recs) -> bool {
       constexpr bool MASKED = decltype(masked_tag)::value;
+      constexpr int N = MASKED ? 1 : MATH;  // records
       asm volatile("" ::: "memory");  // Q is read from shared memory each time: held in registers it would spill
       float f_own[NC], qs_own[NC][NG];
       if constexpr (!R::HOLD_Q) load_f(f_own), load_qs(qs_own);
       const float(&f)[NC] = R::HOLD_Q ? f_item : f_own;
       const float(&qs)[NC][NG] = R::HOLD_Q ? qs_item : qs_own;
       // ---- scores
-      float s[MATH][2][NC];
+      float s[N][2][NC];
 #pragma unroll
-      for (int u = 0; u < MATH; ++u) {
+      for (int u = 0; u < N; ++u) {
         const uint8_t* rec = recs + u * P::RECORD;
         uint32_t kw[2][2 * NG], kp[2][NG];
 #pragma unroll
@@ -583,10 +627,10 @@ __global__ void __launch_bounds__(Kv4Cfg<D, RT>::WARPS * 32, 1) kv4_attn_kernel(
             for (int q = 0; q < NC; ++q) s[u][e][q] = a.cap_log2 * tanh_exp(s[u][e][q] * f[q]);
       }
       // ---- distance of the scores to their references; the value scales as operands
-      uint32_t vp[MATH][2][NG];
-      unsigned in[MATH] = {};  // bit e * NC + q
+      uint32_t vp[N][2][NG];
+      unsigned in[N] = {};  // bit e * NC + q
 #pragma unroll
-      for (int u = 0; u < MATH; ++u) {
+      for (int u = 0; u < N; ++u) {
         const uint8_t* rec = recs + u * P::RECORD;
 #pragma unroll
         for (int e = 0; e < 2; ++e) load_words(rec + P::V_PAIRS + (e ? tok1 : tok0) * P::PAIRS, vp[u][e]);
@@ -598,13 +642,12 @@ __global__ void __launch_bounds__(Kv4Cfg<D, RT>::WARPS * 32, 1) kv4_attn_kernel(
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
             const int at = (t + u) * kKv4Tokens + (e ? tok1 : tok0);
-            const bool here = have >> u & 1u;
-            if (!(here && at < see_most && at >= low))  // no row sees the token: its pairs hold anything
+                        if (!(at < see_most && at >= low))  // no row sees the token: its pairs hold anything
 #pragma unroll
               for (int k = 0; k < NG; ++k) vp[u][e][k] = 0;
 #pragma unroll
             for (int q = 0; q < NC; ++q)
-              in[u] |= static_cast<unsigned>(here && at < see[q] && (a.window <= 0 || at >= see[q] - a.window))
+              in[u] |= static_cast<unsigned>(at < see[q] && (a.window <= 0 || at >= see[q] - a.window))
                        << (e * NC + q);
           }
         }
@@ -617,10 +660,10 @@ __global__ void __launch_bounds__(Kv4Cfg<D, RT>::WARPS * 32, 1) kv4_attn_kernel(
         const float x = CAP ? s[u][e][q] : s[u][e][q] * f[q];
         return !MASKED || (in[u] >> (e * NC + q) & 1u) ? x : -INFINITY;
       };
-      float d[MATH][2][NC], vs[MATH][2][NG];
+      float d[N][2][NC], vs[N][2][NG];
       float far = -INFINITY, top = 0.0f;
 #pragma unroll
-      for (int u = 0; u < MATH; ++u)
+      for (int u = 0; u < N; ++u)
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
           if constexpr (!MASKED && RT > 0 && !CAP) {
@@ -637,69 +680,188 @@ __global__ void __launch_bounds__(Kv4Cfg<D, RT>::WARPS * 32, 1) kv4_attn_kernel(
           for (int q = 0; q < NC; ++q) far = fmaxf(far, d[u][e][q]);
 #pragma unroll
           for (int k = 0; k < NG; k += 2) {
-            const F2 x = mul2({pair_scale(vp[u][e][k]), pair_scale(vp[u][e][(k + 1) % NG])}, {vscale, vscale});
+            const F2 x = mul2({pair_scale(vp[u][e][k]), pair_scale(vp[u][e][(k + 1) % NG])},
+                              {vscale[k], vscale[(k + 1) % NG]});
             vs[u][e][k] = x.x;
             if (k + 1 < NG) vs[u][e][(k + 1) % NG] = x.y;
           }
 #pragma unroll
           for (int k = 0; k < NG; ++k) top = fmaxf(top, vs[u][e][k]);
         }
-      // ---- new references and scaling, where a score or a scale outgrew them
-      if (__any_sync(0xffffffffu, far > kSlack || top > limit)) {
-        float smax = 0.0f;
-#pragma unroll
-        for (int u = 0; u < MATH; ++u)
-#pragma unroll
-          for (int k = 0; k < NG; ++k)
-#pragma unroll
-            for (int e = 0; e < 2; ++e)
-              if (pair_scale(vp[u][e][k]) <= kFltMax) smax = fmaxf(smax, pair_scale(vp[u][e][k]));
-#pragma unroll
-        for (int off = 4; off < 32; off <<= 1) smax = fmaxf(smax, __shfl_xor_sync(0xffffffffu, smax, off));
-        float fo = 1.0f;
-        if (smax * vscale > limit) {
-          const float ns = ldexpf(1.0f, min(kScaleTarget - ilogbf(smax), 126));
-          fo = limit == 0.0f ? 1.0f : ns / vscale;
-          vscale = ns;
-          limit = kScaleMax;
-        }
-        float fac[NC];
+      // ---- new references and scalings, where a score or a value scale outgrew them
+      if (__any_sync(0xffffffffu, far > kSlack || top > kScaleMax)) {
         const bool empty = none;
-        none = false;
+        float m[NC];  // the references to be
 #pragma unroll
         for (int q = 0; q < NC; ++q) {
-          float m = -INFINITY;
+          m[q] = -INFINITY;
 #pragma unroll
-          for (int u = 0; u < MATH; ++u) m = fmaxf(m, fmaxf(score(u, 0, q), score(u, 1, q)));
+          for (int u = 0; u < N; ++u) m[q] = fmaxf(m[q], fmaxf(score(u, 0, q), score(u, 1, q)));
 #pragma unroll
-          for (int off = 4; off < 32; off <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, off));
-          m = fmaxf(m, mref[q]);
-          fac[q] = ex2(mref[q] - m);
-          mref[q] = m;
+          for (int off = 4; off < 32; off <<= 1) m[q] = fmaxf(m[q], __shfl_xor_sync(0xffffffffu, m[q], off));
+          m[q] = fmaxf(m[q], mref[q]);
+        }
+        // Where s' is within kScaleMax and above 2^0 for the tokens that set new references, both as scaled now, nothing
+        // but references changes.  The first scaling puts the largest s' into [2^7, 2^8).
+        bool plain = RT == 0 || same;
+        bool light[N][2] = {};  // tokens of a smaller s'
+#pragma unroll
+        for (int k = 0; k < NG; ++k) {
+          float hi = 0.0f;
+#pragma unroll
+          for (int u = 0; u < N; ++u) hi = fmaxf(hi, fmaxf(pair_scale(vp[u][0][k]), pair_scale(vp[u][1][k])));
+          if (empty) {
+#pragma unroll
+            for (int off = 4; off < 32; off <<= 1) hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, off));
+            vscale[k] = power_of_2(choose_scale(kFirstScale, log2_of(hi), kNothing, kNothing));
+          }
+          plain = plain && hi * vscale[k] <= kScaleMax;
+#pragma unroll
+          for (int u = 0; u < N; ++u)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) light[u][e] = light[u][e] || !(pair_scale(vp[u][e][k]) * vscale[k] >= 1.0f);
+        }
+#pragma unroll
+        for (int q = 0; q < NC; ++q)
+#pragma unroll
+          for (int u = 0; u < N; ++u)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) plain = plain && !(light[u][e] && m[q] > mref[q] && score(u, e, q) == m[q]);
+        plain = __all_sync(0xffffffffu, plain);
+        if constexpr (!MASKED)
+          if (__builtin_expect(!plain, 0)) return false;
+        none = false;
+        float fac[NC];
+#pragma unroll
+        for (int q = 0; q < NC; ++q) {
+          fac[q] = ex2(mref[q] - m[q]);
+          if (MASKED && !plain && g == 0) row_drop[row_of(q)] = fmaxf(mref[q] - m[q], -1000.0f);
+          mref[q] = m[q];
           l[q] *= fac[q];
 #pragma unroll
           for (int k = 0; k < NG; ++k) mo[q][k] *= fac[q];
+#pragma unroll
+          for (int u = 0; u < N; ++u)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) d[u][e][q] = distance(u, e, q);
         }
-        if (!empty)
+        if (__builtin_expect(plain, 1)) {
+          if (!empty) {
 #pragma unroll
-          for (int k = 0; k < OT; ++k)
+            for (int k = 0; k < OT; ++k)
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt)
+              for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-              for (int e = 0; e < 4; ++e) o[k][nt][e] *= fac[RT == 0 ? 0 : (nt * 2 + (e & 1)) % NC] * fo;
+                for (int e = 0; e < 4; ++e) o[k][nt][e] *= fac[RT == 0 ? 0 : (nt * 2 + (e & 1)) % NC];
+          } else if constexpr (!MASKED) {
 #pragma unroll
-        for (int u = 0; u < MATH; ++u)
+            for (int u = 0; u < N; ++u)
 #pragma unroll
-          for (int e = 0; e < 2; ++e) {
+              for (int e = 0; e < 2; ++e)
 #pragma unroll
-            for (int q = 0; q < NC; ++q) d[u][e][q] = distance(u, e, q);
-#pragma unroll
-            for (int k = 0; k < NG; ++k) vs[u][e][k] = pair_scale(vp[u][e][k]) * vscale;
+                for (int k = 0; k < NG; ++k) vs[u][e][k] = pair_scale(vp[u][e][k]) * vscale[k];
           }
+        } else if constexpr (MASKED) {
+          // Row by row and group by group, from the largest product and the largest sum of each, which a lane looks at:
+          // code that hardly ever runs is to be small, as every kernel of 16 rows and more outgrows the instruction
+          // cache (5 query tokens of 64 sequences of 2048: 94 us with all of it unrolled, 81 like this, 77 since records
+          // that all rows see whole are not masked).
+          for (int i = lane; i < ROWS * NG; i += 32) row_w[i] = row_o[i] = 0;
+          if (RT == 0 || same)
+#pragma unroll
+            for (int q = 0; q < NC; ++q)
+#pragma unroll
+              for (int k = 0; k < NG; ++k)
+                if (g == 0) col_v[row_of(q) * NG + k] = vscale[k];
+          __syncwarp();
+          float smax[NG];
+#pragma unroll
+          for (int k = 0; k < NG; ++k) {
+            const float p0 = pair_scale(vp[0][0][k]), p1 = pair_scale(vp[0][1][k]);
+            const float s0 = p0 <= kFltMax ? p0 : 0.0f, s1 = p1 <= kFltMax ? p1 : 0.0f;
+            smax[k] = fmaxf(s0, s1);
+#pragma unroll
+            for (int q = 0; q < NC; ++q) {
+              float sum = 0.0f;
+#pragma unroll
+              for (int x = 0; x < 4; ++x) {
+                const float(&y)[4] = RT == 0 ? o[(k * 2 + x % 2) % OT][0] : o[(k * 4 + x) % OT][q >> 1];
+                const int at = RT == 0 ? x / 2 : q & 1;
+                sum = fmaxf(sum, fmaxf(y[at], y[at + 2] * 0x1p-4f));
+              }
+              const float w = fmaxf(fmaxf(ex2(d[0][0][q]) * s0, ex2(d[0][1][q]) * s1), 0.0f);
+              atomicMax(row_w + row_of(q) * NG + k, __float_as_int(w));  // above zero bits are ordered as the numbers
+              atomicMax(row_o + row_of(q) * NG + k, __float_as_int(sum));
+            }
+          }
+#pragma unroll
+          for (int k = 0; k < NG; ++k)
+#pragma unroll
+            for (int off = 4; off < 32; off <<= 1) smax[k] = fmaxf(smax[k], __shfl_xor_sync(0xffffffffu, smax[k], off));
+          __syncwarp();
+          int most = kNothing, least = -kNothing;  // of the lane's group, over the rows that anything weighs in
+          float mine = smax[0];
+#pragma unroll
+          for (int k = 1; k < NG; ++k) mine = lane % NG == k ? smax[k] : mine;
+          const int s_log = log2_of(mine);
+#pragma unroll 1
+          for (int i = lane; i < ROWS * NG; i += 32) {
+            const float w = __int_as_float(row_w[i]), sum = __int_as_float(row_o[i]), drop = row_drop[i / NG];
+            const int old = log2_of(col_v[i]);
+            int chosen = kNothing;
+            if (RT == 0 || w > 0.0f || sum > 0.0f) {
+              // o holds code times product times 2^-24, at most 15 of the first
+              chosen = choose_scale(old, s_log, log2_of(w),
+                                    sum > 0.0f ? log2_of(sum) + 20 + __float2int_rd(drop) - old : kNothing);
+              most = max(most, chosen);
+              least = min(least, chosen);
+              col_v[i] = power_of_2(chosen);
+            }
+            row_w[i] = chosen;
+            row_o[i] = __float_as_int(sum > 0.0f ? ldexpf(ex2(drop), chosen - old) : 1.0f);  // what o is multiplied by
+          }
+          if constexpr (RT > 0) {
+#pragma unroll
+            for (int off = NG; off < 32; off <<= 1) {
+              most = max(most, __shfl_xor_sync(0xffffffffu, most, off));
+              least = min(least, __shfl_xor_sync(0xffffffffu, least, off));
+            }
+            if (most == kNothing) {
+              float v = vscale[0];
+#pragma unroll
+              for (int k = 1; k < NG; ++k) v = lane % NG == k ? vscale[k] : v;
+              most = least = choose_scale(log2_of(v), s_log, kNothing, kNothing);
+            }
+#pragma unroll 1
+            for (int i = lane; i < ROWS * NG; i += 32)
+              if (row_w[i] == kNothing) col_v[i] = power_of_2(most);
+            same = __all_sync(0xffffffffu, most == least);
+#pragma unroll
+            for (int k = 0; k < NG; ++k) vscale[k] = __shfl_sync(0xffffffffu, power_of_2(most), k);
+          }
+          __syncwarp();
+#pragma unroll
+          for (int k = 0; k < NG; ++k) {
+            if constexpr (RT == 0) vscale[k] = col_v[row_of(0) * NG + k];
+#pragma unroll
+            for (int q = 0; q < NC; ++q) {
+              const float f = __int_as_float(row_o[row_of(q) * NG + k]);
+#pragma unroll
+              for (int x = 0; x < (RT == 0 ? 2 : 4); ++x) {
+                float(&y)[4] = RT == 0 ? o[(k * 2 + x) % OT][0] : o[(k * 4 + x) % OT][q >> 1];
+#pragma unroll
+                for (int j = 0; j < (RT == 0 ? 4 : 2); ++j) y[RT == 0 ? j : 2 * j + (q & 1)] *= f;
+              }
+            }
+          }
+          __syncwarp();
+        }
       }
       // ---- weights, and outputs
+      float v[NC][NG];
+      if constexpr (MASKED) load_v(v);
 #pragma unroll
-      for (int u = 0; u < MATH; ++u) {
+      for (int u = 0; u < N; ++u) {
         const uint8_t* rec = recs + u * P::RECORD;
         uint32_t vw[4][NG];
 #pragma unroll
@@ -739,7 +901,7 @@ __global__ void __launch_bounds__(Kv4Cfg<D, RT>::WARPS * 32, 1) kv4_attn_kernel(
 #pragma unroll
               for (int q = 0; q < NC; ++q) {
                 const bool x = in[u] >> (e * NC + q) & 1u;  // a NaN pair that only later rows see
-                w[q] = x ? d[u][e][q] * vs[u][e][k] : 0.0f;
+                w[q] = x ? d[u][e][q] * v[q][k] * pair_scale(vp[u][e][k]) : 0.0f;
                 mo[q][k] += x ? d[u][e][q] * pair_min(vp[u][e][k]) : 0.0f;
               }
             } else {
@@ -782,11 +944,12 @@ __global__ void __launch_bounds__(Kv4Cfg<D, RT>::WARPS * 32, 1) kv4_attn_kernel(
           }
         }
       }
+      return true;
     };
 
-    // bursts that start in [t_low, t_high] hold no token that some row does not see
+    // MATH records from one in [t_low, t_high] on hold no token that some row does not see
     const int t_low = a.window > 0 ? max(see_most - a.window + kKv4Tokens - 1, 0) / kKv4Tokens : 0;
-    const int t_high = max(see_least, 0) / kKv4Tokens - BURST;
+    const int t_high = max(see_least, 0) / kKv4Tokens - MATH;
     for (int t = dead ? span.y : span.x; t < span.y; t += BURST) {  // given up: the items still get an entry
       if (!__all_sync(0xffffffffu, mbar_try_wait(smem_u32(bars + cur), parity)) &&
           !__all_sync(0xffffffffu, wait_slow(bars + cur, parity, &abort_flag, a.err))) {
@@ -795,12 +958,13 @@ __global__ void __launch_bounds__(Kv4Cfg<D, RT>::WARPS * 32, 1) kv4_attn_kernel(
       }
       const unsigned have = came & ALL;
       const uint8_t* recs = ring + cur * (BURST * P::RECORD);
-      if (have == ALL && t >= t_low && t <= t_high) {
 #pragma unroll 1
-        for (int x = 0; x < BURST; x += MATH) burst(std::false_type{}, t + x, ALL, recs + x * P::RECORD);
-      } else if (have) {  // else no such blocks: their tokens count as masked
+      for (int x = 0; x < BURST; x += MATH) {
+        const bool all_seen = (have >> x & MATH_ALL) == MATH_ALL && t + x >= t_low && t + x <= t_high;
+        if (all_seen && same && burst(std::false_type{}, t + x, recs + x * P::RECORD)) continue;
 #pragma unroll 1
-        for (int x = 0; x < BURST; x += MATH) burst(std::true_type{}, t + x, have >> x, recs + x * P::RECORD);
+        for (int y = x; y < x + MATH; ++y)  // a record without a block inside the pool: its tokens count as masked
+          if (have >> y & 1u) burst(std::true_type{}, t + y, recs + y * P::RECORD);
       }
       __syncwarp();
       came >>= BURST;
@@ -825,8 +989,9 @@ __global__ void __launch_bounds__(Kv4Cfg<D, RT>::WARPS * 32, 1) kv4_attn_kernel(
       it.last = whole ? worker : split.worker(split.start(worker + 1) - left + sq.rounds - 1);
       a.items[static_cast<int64_t>(seq) * subs + sub] = it;
     }
+    float v_item[NC][NG];
+    load_v(v_item);
     const int64_t slot = 2 * static_cast<int64_t>(worker) + (ra == 0 ? 1 : 0);
-    const float inv = 1.0f / vscale;
 #pragma unroll
     for (int q = 0; q < NC; ++q) {
       const int r = row_of(q), nt = q >> 1, j = q & 1;
@@ -839,6 +1004,7 @@ __global__ void __launch_bounds__(Kv4Cfg<D, RT>::WARPS * 32, 1) kv4_attn_kernel(
       if (!whole && g == 0) a.part_ml[slot * ROWS + r] = make_float2(mref[q], l[q]);
 #pragma unroll
       for (int k = 0; k < NG; ++k) {
+        const float inv = 1.0f / v_item[q][k];
         float v[8];  // channels 8 g + 4 hv + 2 hh (codes as u 2^-24) and the next one (u 2^-20)
 #pragma unroll
         for (int x = 0; x < 4; ++x) {

@@ -113,8 +113,9 @@ def attention_each(q, pool, layer, tables, ctx, scale, softcap=0.0, window=0):
     term), and some 2 a group and 8 more roundings put it off by (4 * 64 + 2 groups + 8) 2^-24 M; a capped score by 2^-21
     of the cap more; its factor, its distance to the reference and exp2 by 2^-22 of its magnitude and 2^-21 of the weight.
     An error e_n of weight n moves the output by p_n e_n (v_n - out).  The weight in the product with the codes is rounded
-    to 11 bits: 2^-11 p_n |v_n - m_n|.  Below 2^-14 of 2^7 times the largest weight in the output's own row and group (that
-    is where it is scaled to, at least) it is off by 2^-32 of that one, times 15.  fp32 sums of the outputs, over 16 keys at
+    to 11 bits: 2^-11 p_n |v_n - m_n|.  A p s below 2^-14 as scaled is off by 2^-25 there, times a code of 15.  The largest
+    p s of the output's row and group, or their sum, is scaled to 2^0 at least, so in the channel of its largest code, 14 at
+    least, the sum of p |v - m| stands at 14 or above: n errors are 15 / 14 n 2^-25 of that channel's sum.  fp32 sums of the outputs, over 16 keys at
     a time, lose 2^-23 of the magnitudes each, twice where a part is scaled again and joined."""
     B, T, Hq, D = q.shape
     heads, bs, ng = pool.shape[2], 16 * pool.shape[3], q.shape[-1] // 64
@@ -148,8 +149,8 @@ def attention_each(q, pool, layer, tables, ctx, scale, softcap=0.0, window=0):
             away = (vv.permute(1, 0, 2)[:, None] - o[:, :, None]).abs()  # [heads, rows, n, D]
             err = torch.einsum("hrn,hrnd->hrd", p * off, away) * 1.05
             err = err + 2.0 ** -11 * torch.einsum("hrn,nhd->hrd", p, part)
-            top = (p[..., None] * part.permute(1, 0, 2)[:, None]).unflatten(-1, (ng, 64)).amax((2, 4))   # of the group
-            err = err + 2.0 ** -32 * 15 * (end - lo) * top.repeat_interleave(64, -1)
+            top = torch.einsum("hrn,nhd->hrd", p, part).unflatten(-1, (ng, 64)).amax(-1)   # of the group
+            err = err + 2.0 ** -25 * 15 / 14 * (end - lo) * top.repeat_interleave(64, -1)
             steps = (end - lo) // 16 + 4
             err = err + 2.0 ** -22 * steps * torch.einsum("hrn,nhd->hrd", p, part + vm[lo:end].abs())
             out[b, t], tol[b, t] = o.flatten(0, 1), err.flatten(0, 1)
