@@ -657,7 +657,15 @@ def assign_slots(block_tables: torch.Tensor, ctx_lens: torch.Tensor, new_lens: t
     ``held_blocks`` (int32 ``[B]``, updated in place): how many entries of its row each sequence holds, 0 for a new
     one.  Needed where lengths go back, as rejected drafts make them: the blocks behind a shorter length are then used
     again, where without a count new ones would be taken over them.  A count below what ``ctx_lens`` needs, or past the
-    row, is refused like a negative length."""
+    row, is refused like a negative length.
+
+    The outputs are cut from one allocation: one that is kept keeps all of it."""
+    return _assign_slots(block_tables, ctx_lens, new_lens, free_blocks, block_size, num_tokens, free_head, held_blocks)
+
+
+def _assign_slots(block_tables, ctx_lens, new_lens, free_blocks, block_size, num_tokens, free_head=None,
+                  held_blocks=None, apart: bool = False) -> SlotPlan:
+    """``assign_slots``; with ``apart`` each output is a tensor of its own."""
     what = "assign_slots"
     index = block_tables.get_device() if isinstance(block_tables, torch.Tensor) else -1
     try:
@@ -689,20 +697,25 @@ def assign_slots(block_tables: torch.Tensor, ctx_lens: torch.Tensor, new_lens: t
     if num_tokens < 0:
         raise RuntimeError(f"{what}: num_tokens {num_tokens}")
     ctx_lens, new_lens, free_blocks = ctx_lens.contiguous(), new_lens.contiguous(), free_blocks.contiguous()
-    # one allocation: slots (two words each), positions, starts, granted, the head
-    words = torch.empty(3 * num_tokens + 2 * B + 2, dtype=_I32, device=block_tables.device)
-    at = words.data_ptr()
-    slots, positions, seq_start, granted, head = words.split_with_sizes((2 * num_tokens, num_tokens, B + 1, B, 1))
-    start = at + 12 * num_tokens
+    device = block_tables.device
+    if apart:
+        slots = torch.empty(num_tokens, dtype=_I64, device=device)
+        positions, seq_start, granted, head = (torch.empty(n, dtype=_I32, device=device) for n in (num_tokens, B + 1, B, 1))
+        at = [t.data_ptr() for t in (slots, positions, seq_start, granted, head)]
+    else:  # one allocation: slots (two words each), positions, starts, granted, the head
+        words = torch.empty(3 * num_tokens + 2 * B + 2, dtype=_I32, device=device)
+        base = words.data_ptr()
+        slots, positions, seq_start, granted, head = words.split_with_sizes((2 * num_tokens, num_tokens, B + 1, B, 1))
+        slots = slots.view(_I64)
+        start = base + 12 * num_tokens
+        at = (base, base + 8 * num_tokens, start, start + 4 * (B + 1), start + 4 * (2 * B + 1))
     ws, ws_bytes = None, 0
     if B > 8192:
         ws_bytes = N.lib().mvb_assign_slots_workspace_bytes(B)
-        ws = torch.empty(ws_bytes, dtype=_U8, device=block_tables.device)
-    N.on_device(index, what, N.lib().mvb_assign_slots_ex, at, at + 8 * num_tokens, start, start + 4 * (B + 1),
-                start + 4 * (2 * B + 1), block_tables.data_ptr(), t_stride, width, ctx_lens.data_ptr(),
-                new_lens.data_ptr(), N.ptr(held_blocks), free_blocks.data_ptr(), free_blocks.numel(), N.ptr(free_head),
-                B, int(block_size), int(num_tokens), N.ptr(ws), ws_bytes)
-    slots = slots.view(_I64)
+        ws = torch.empty(ws_bytes, dtype=_U8, device=device)
+    N.on_device(index, what, N.lib().mvb_assign_slots_ex, *at, block_tables.data_ptr(), t_stride, width,
+                ctx_lens.data_ptr(), new_lens.data_ptr(), N.ptr(held_blocks), free_blocks.data_ptr(), free_blocks.numel(),
+                N.ptr(free_head), B, int(block_size), int(num_tokens), N.ptr(ws), ws_bytes)
     return SlotPlan(slots, positions, seq_start, granted, head)
 
 

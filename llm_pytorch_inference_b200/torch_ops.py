@@ -108,7 +108,7 @@ IMPLS = {
     "kv4_read": ops.kv4_read,
     "paged_attention_decode_kv4": lambda q, kv4, layer, block_tables, ctx_lens, scale, softcap, window:
         ops.paged_attention_decode_kv4(q, kv4, layer, block_tables, ctx_lens, scale, softcap=softcap, window=window),
-    "assign_slots": lambda *args: tuple(ops.assign_slots(*args)),
+    "assign_slots": lambda *args: tuple(ops._assign_slots(*args, apart=True)),  # outputs may not alias
     "verify_drafts": ops.verify_drafts,
 }
 
