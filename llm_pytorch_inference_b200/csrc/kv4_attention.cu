@@ -153,6 +153,8 @@ __device__ __forceinline__ float power_of_2(int e) { return __uint_as_float(stat
 // keep all but n 2^-25 of the largest one, or of their sum, where that is scaled to 2^0 or above.  The scaling stays while
 // s' is within kScaleMax, and falls to where s' is within it, both while the products keep their bits; else it stays as
 // long as the products themselves fit, and else follows them.
+// What is not looked at again: where a row's heaviest tokens have no spread in a group (s' = 0), what weighs less than
+// 2^-31 of them may count with its minimum alone, p m'.
 __device__ __forceinline__ int choose_scale(int old, int s, int w, int o) {
   const int most = max(w, o);
   int e = s + old <= 8 ? old : 7 - s;

@@ -203,3 +203,23 @@ def test_groups_without_a_spread(T, Hq, Hkv):
     v[:300, :, :64] = -0.25
     v[400:, :, :64] *= 2.0 ** -20
     check(case(normal(g, T, Hq, D), normal(g, n, Hkv, D), v, 1 / math.sqrt(D)))
+
+
+# ------------------------------------------------------------------ the largest counts that are accepted
+@pytest.mark.parametrize("T,Hq,Hkv,n", [(1024, 4, 2, 1024), (1024, 2, 1, 40), (1024, 3, 1, 1300), (1, 4096, 8, 100),
+                                        (1, 4096, 4096, 50), (2, 4096, 1, 200), (49, 4, 4, 300), (50, 10, 2, 77)])
+def test_many_query_rows(T, Hq, Hkv, n):
+    """1,024 query tokens, 4,096 query heads, chunks of rows that do not divide evenly."""
+    g = gen(T + Hq + n)
+    D = 64
+    check(case(normal(g, T, Hq, D), normal(g, n, Hkv, D), normal(g, n, Hkv, D), 1 / math.sqrt(D)))
+    check(case(normal(g, T, Hq, D), normal(g, n, Hkv, D), normal(g, n, Hkv, D), 1 / math.sqrt(D)), window=30)
+
+
+def test_more_query_rows_are_refused():
+    z = torch.zeros(1, 1025, 1, 64, dtype=BF, device=DEV)
+    pool, table, n = kv4_pool(1, 16, 1, 1, 64), torch.zeros(1, 1, dtype=torch.int32, device=DEV), torch.ones(
+        1, dtype=torch.int32, device=DEV)
+    for q in (z, z[:, :1].expand(1, 1, 4097, 64)):
+        with pytest.raises(RuntimeError):
+            ops.paged_attention_decode_kv4(q, pool, 0, table, n, 1.0)
