@@ -273,7 +273,9 @@ int mvb_kv4_read(void* k, void* v, const void* kv4, const int64_t* slots, int64_
  * q_stride / out_stride elements (multiples of 8, 16-byte aligned).  block_tables: row b at
  * b * table_stride, max_blocks entries of it are used.  A context past its table is cut
  * (MVB_DEV_BAD_POSITION); a block outside the pool counts as masked (MVB_DEV_BAD_BLOCK).
- * batch <= 65536, query_len <= 1024, Hq <= 4096.  Scores and softmax statistics in fp32, deterministic.  workspace: at least ..._workspace_bytes()
+ * batch <= 65536, query_len <= 1024, Hq <= 4096.  Scores (q exact), softmax statistics and sums in fp32, deterministic;
+ * the weights, times the value scales, are rounded to 11 bits.  Keys are to stay below 2^104 in magnitude, and values so
+ * that 2^6 |v| times the keys of a sequence stays in fp32's range.  workspace: at least ..._workspace_bytes()
  * bytes, 256-byte aligned, of any content; calls that overlap on the GPU need one each.  Tables of at most
  * 128 tokens (max_blocks * block_size) need none (NULL). */
 int64_t mvb_paged_attention_decode_kv4_workspace_bytes(int64_t batch, int64_t query_len, int64_t num_q_heads,

@@ -11,7 +11,8 @@
 // K and of V of a token, for one head or two (HEADS): a 16-byte load (or store) of bf16 and one 32-bit word of
 // codes each, all under way together and with one look at the token's slot.  Eight lanes share a group.  Its minimum
 // and maximum, on packed bf16, are exchanged so that each lane ends up with one of the 2 to 8 groups, works out that
-// group's pair alone and hands it round.  Writing is bound by issued instructions all the same, so a quotient is a
+// group's pair alone and hands it round.  Writing still takes 63 % of the issue slots, beside two loads in a row that it
+// waits for (the slot, then the rows of K and V; 57 registers leave half of the warps to cover them), so a quotient is a
 // product and its correction, two values to an instruction, added to 1.5 * 2^23, which rounds it to even and leaves the
 // code in the low bits, and a multiply-add puts it into the word.
 // Measured on a B200, K and V of 8 heads of 128: writing 16,384 tokens takes 18.0 us for 86 MB (4.8 TB/s); with every

@@ -13,8 +13,8 @@
 // CTA), then maps its share of the tokens; a token finds its sequence by bisecting the scanned
 // starts in shared memory.  A token at the first position of a new block writes that block into
 // the table.  No CTA reads what another writes: entries below held_b are only read, the ones above only written,
-// and held_b is updated when all have read it, by the one CTA or by a launch of its own.  Bound by latency: a scan, a bisection and two dependent loads (4.3 us for 64 sequences of
-// one token, 5.5 for 200 of 500 to 1000).
+// and held_b is updated when all have read it, by the one CTA or by a launch of its own.  Bound by latency: a scan, a
+// bisection and two dependent loads (4.4 us for 64 sequences of one token, 5.7 for 200 of 500 to 1000).
 //
 // A batch whose starts do not fit into shared memory is cut into pieces of 4,096 sequences, a block each: sums of
 // the pieces, then starts and sums of the blocks needed, then offsets into the free list, then the tokens, a

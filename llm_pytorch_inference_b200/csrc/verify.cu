@@ -11,10 +11,11 @@
 // depend on how the sum is split unless u lies that close to a border.
 //
 // Only one row of p (and of q) is read per sequence: bound by those 4 (8) bytes an entry, and by latency for few
-// sequences.  A sequence is a cluster of up to 8 blocks: every lane looks at one draft, so that all of
-// them cost one dependent load each; every warp sums a run of the vocabulary; the blocks exchange their sums
-// through distributed shared memory; and the block in whose part the threshold falls reads one warp's run of it
-// again (out of L2), all its warps together, to find the entry.  The order of all sums is fixed.
+// sequences.  (64 sequences of 151,936 entries are 256 blocks on 296 places: an SM is busy for 72 % of the call.)
+// A sequence is a cluster of up to 8 blocks: every lane looks at one draft, so that all of them cost one dependent load
+// each; every warp sums a run of the vocabulary; the blocks exchange their sums through distributed shared memory; and
+// the block in whose part the threshold falls reads one warp's run of it again (out of L2), all its warps together, to
+// find the entry.  The order of all sums is fixed.
 #include <climits>
 
 #include "common.cuh"
