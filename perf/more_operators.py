@@ -10,7 +10,7 @@ A weight is ``scale * (code - zero)``: codes and zeros of 0 to 15, bf16 scales, 
 group of 32, 64 or 128 columns.  They are held in records of 16 rows by 128 columns, uint8 ``[records, 1024 + 64 *
 (128 / group)]``.  First the codes, 64 bytes a row: 16 bytes at place ``p`` of row ``r`` hold the columns
 ``32 i + 8 t .. + 7`` of word ``i = 0 .. 3``, with ``t = p ^ (r / 2 % 4)``, and a word's nibbles, lowest first, are its
-columns 0, 2, 4, 6, 1, 3, 5, 7.  Then one 32-bit word per group and row: the scale's bits, and the bf16 number
+columns 0, 2, 4, 6, 1, 3, 5, 7.  Then for each row one 32-bit word per group: the scale's bits, and the bf16 number
 ``128 + zero`` above them.  What lies behind the last row or column is zero.  The records of 128 rows stand
 together: for each 128 columns the 8 (behind the last whole 128 rows: the remaining) records of those rows.
 """
@@ -106,7 +106,7 @@ def _records(codes, scales, zeros, group):
     pairs = torch.zeros(tiles * 16, blocks * per, 2, dtype=torch.int16, device=DEV)
     pairs[:n, :scales.shape[1], 0] = scales.view(torch.int16)
     pairs[:n, :scales.shape[1], 1] = zeros.to(torch.int16) + 0x4300  # the bits of 128 + zero
-    pairs = pairs.view(tiles, 16, blocks, per, 2).permute(0, 2, 3, 1, 4).contiguous()
+    pairs = pairs.view(tiles, 16, blocks, per, 2).transpose(1, 2).contiguous()
     out[..., 1024:] = pairs.view(torch.uint8).flatten(2)
     head = tiles // 8 * 8
     return torch.cat([out[:head].unflatten(0, (-1, 8)).transpose(1, 2).flatten(0, 2), out[head:].transpose(0, 1).flatten(0, 1)])
@@ -152,7 +152,7 @@ def _weights(records, n, k, group):
     word = r[..., :1024].view(tiles, blocks, 16, 4, 4, 4)[:, :, row, place].permute(0, 2, 1, 4, 3, 5)
     u = torch.stack([word & 15, word >> 4], -1).flatten(-2)[..., [0, 4, 1, 5, 2, 6, 3, 7]]
     u = u.reshape(tiles * 16, blocks * per, group)
-    p = r[..., 1024:].reshape(tiles, blocks, per, 16, 4).permute(0, 3, 1, 2, 4).contiguous()
+    p = r[..., 1024:].reshape(tiles, blocks, 16, per, 4).transpose(1, 2).contiguous()
     p = p.view(torch.bfloat16).float().reshape(tiles * 16, blocks * per, 2)
     return (p[..., :1] * (u.float() - (p[..., 1:] - 128).clamp_min(0))).flatten(1)[:n, :k]
 
@@ -248,7 +248,7 @@ def _exact_part(records, rows, n, k, group):
     nibble = torch.tensor([0, 4, 1, 5, 2, 6, 3, 7], device=DEV)[col % 8]
     u = flat[at + 64 * r + 16 * place + 4 * (col % 128 // 32) + nibble // 2].int()
     u = torch.where(nibble % 2 == 1, u // 16, u % 16)
-    pair = at + 1024 + 64 * (col % 128 // group) + 4 * r
+    pair = at + 1024 + 512 // group * r + 4 * (col % 128 // group)
     scale = ((flat[pair].int() << 16) + (flat[pair + 1].int() << 24)).view(torch.float32).double()
     return scale * (u - flat[pair + 2].int() % 128).double()
 
