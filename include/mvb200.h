@@ -585,6 +585,57 @@ int mvb_tp_wait(mvb_tp_comm* comm, int point, mvb_stream_t stream);
  * dependents start only at their end, are fine.  Returns the previous setting. */
 int mvb_set_pdl(int enable);
 
+/* ---- rows in 8 bits, weights in 4 bits ---------------------------------------
+ * No counterpart in the reference: the linear layers of models/model.py:69-117, :154-243 and ops/mlp.py:46-84 with
+ * weights in 4 bits, next to mvb_gemm_bf16, mvb_fused_add_rmsnorm and mvb_fused_mlp.
+ *
+ * A row in 8 bits: codes q (int8, -127 .. 127) and an fp32 scale; element i stands for q[i] * scale.
+ * With amax = max |y|: q = rint(127 y / amax), scale = amax / 127.  A row with an infinity or a NaN gets the scale NaN,
+ * a row of zeros the scale 0.  values: [rows, width] (contiguous), scales: [rows].  y, in 32 bits throughout:
+ *   mvb_quantise_q8           in
+ *   mvb_rmsnorm_q8            in * w / sqrt(mean(in^2) + eps), w = weight or 1 + weight (plus_one)
+ *   mvb_fused_add_rmsnorm_q8  the same of residual + in (rounded to the dtype), which goes to residual_out
+ *                             (may be residual or in)
+ *   mvb_gated_q8              act(gate) * up
+ * Strides: elements between rows.  dtype: MVB_F32, MVB_F16 or MVB_BF16, of every operand.
+ * mvb_dequantise_q8: out[rows, width] = values * scales, rounded to the dtype. */
+int mvb_quantise_q8(int8_t* values, float* scales, const void* in, int64_t in_stride, int64_t rows, int64_t width,
+                    int dtype, mvb_stream_t stream);
+int mvb_rmsnorm_q8(int8_t* values, float* scales, const void* in, int64_t in_stride, const void* weight, int64_t rows,
+                   int64_t hidden, float eps, int plus_one, int dtype, mvb_stream_t stream);
+int mvb_fused_add_rmsnorm_q8(int8_t* values, float* scales, void* residual_out, int64_t out_stride,
+                             const void* residual, int64_t residual_stride, const void* in, int64_t in_stride,
+                             const void* weight, int64_t rows, int64_t hidden, float eps, int plus_one, int dtype,
+                             mvb_stream_t stream);
+int mvb_gated_q8(int8_t* values, float* scales, const void* gate, int64_t gate_stride, const void* up,
+                 int64_t up_stride, int64_t rows, int64_t width, int act, int dtype, mvb_stream_t stream);
+int mvb_dequantise_q8(void* out, const int8_t* values, int64_t values_stride, const float* scales, int64_t rows,
+                      int64_t width, int dtype, mvb_stream_t stream);
+
+/* A weight matrix [n, k] in 4 bits: element (i, j) stands for scale * (code - zero), code and zero in 0 .. 15, one
+ * bf16 scale and one zero per row and group of 32, 64 or 128 columns (the last group may be shorter).  k: a
+ * multiple of 32.  records: mvb_w4_bytes(n, k, group) bytes (-1: sizes that are not taken), 16-byte aligned, in the
+ * layout of csrc/w4.cuh.
+ *   mvb_quantise_w4    from bf16 (rows weight_stride elements apart, 16-byte aligned): per group lo = min(0, min w),
+ *                      hi = max(0, max w), scale = bf16((hi - lo) / 15), zero = rint(-lo / scale),
+ *                      code = rint(w / scale) + zero, cut to 0 .. 15.  A group with an infinity or a NaN reads back as NaN.
+ *   mvb_pack_w4        from codes [n, k] and zeros [n, ceil(k / group)] (a byte each, the low 4 bits; zeros NULL: 8) and
+ *                      scales [n, ceil(k / group)] (bf16)
+ *   mvb_dequantise_w4  out[n, k], MVB_BF16 (rounded) or MVB_F32 (exact but for subnormal results)
+ *   mvb_linear_w4      y[rows, n] (bf16, rows ldy elements apart) = x times the matrix transposed.  x: rows of k bf16, or
+ *                      with row_scales (fp32 [rows]) rows of k codes of 8 bits; ldx elements between rows, 16-byte aligned.
+ *                      Sums in 32 bits; no product is rounded before it.  rows <= 262144, k <= 32768.
+ * With mvb_set_pdl(1) mvb_linear_w4 reads records before it waits for the kernel launched before it. */
+int64_t mvb_w4_bytes(int64_t n, int64_t k, int64_t group);
+int mvb_quantise_w4(void* records, const void* weight, int64_t weight_stride, int64_t n, int64_t k, int64_t group,
+                    mvb_stream_t stream);
+int mvb_pack_w4(void* records, const uint8_t* codes, const void* scales, const uint8_t* zeros, int64_t n, int64_t k,
+                int64_t group, mvb_stream_t stream);
+int mvb_dequantise_w4(void* out, const void* records, int64_t n, int64_t k, int64_t group, int dtype,
+                      mvb_stream_t stream);
+int mvb_linear_w4(void* y, int64_t ldy, const void* x, int64_t ldx, const float* row_scales, const void* records,
+                  int64_t rows, int64_t n, int64_t k, int64_t group, mvb_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -69,6 +69,17 @@ SIGNATURES: dict[str, tuple] = {
     "mvb_assign_slots_ex": (_i32, [_vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _vp, _vp, _vp, _vp, _i64, _vp, _i64, _i64,
                                    _i64, _vp, _i64, _vp]),
     "mvb_verify_drafts": (_i32, [_vp, _vp, _vp, _i64, _vp, _i64, _vp, _vp, _vp, _i64, _i64, _i64, _vp]),
+    "mvb_quantise_q8": (_i32, [_vp, _vp, _vp, _i64, _i64, _i64, _i32, _vp]),
+    "mvb_rmsnorm_q8": (_i32, [_vp, _vp, _vp, _i64, _vp, _i64, _i64, _f32, _i32, _i32, _vp]),
+    "mvb_fused_add_rmsnorm_q8": (_i32, [_vp, _vp, _vp, _i64, _vp, _i64, _vp, _i64, _vp, _i64, _i64, _f32, _i32, _i32,
+                                        _vp]),
+    "mvb_gated_q8": (_i32, [_vp, _vp, _vp, _i64, _vp, _i64, _i64, _i64, _i32, _i32, _vp]),
+    "mvb_dequantise_q8": (_i32, [_vp, _vp, _i64, _vp, _i64, _i64, _i32, _vp]),
+    "mvb_w4_bytes": (_i64, [_i64, _i64, _i64]),
+    "mvb_quantise_w4": (_i32, [_vp, _vp, _i64, _i64, _i64, _i64, _vp]),
+    "mvb_pack_w4": (_i32, [_vp, _vp, _vp, _vp, _i64, _i64, _i64, _vp]),
+    "mvb_dequantise_w4": (_i32, [_vp, _vp, _i64, _i64, _i64, _i32, _vp]),
+    "mvb_linear_w4": (_i32, [_vp, _i64, _vp, _i64, _vp, _vp, _i64, _i64, _i64, _i64, _vp]),
     "mvb_gemm_workspace_bytes": (_i64, [_i64, _i64, _i64, _i32]),
     "mvb_gemm_bf16": (_i32, [_vp, _i64, _vp, _i64, _vp, _i64, _i64, _i64, _i64, _i32, _vp, _i64, _vp, _i64, _vp]),
     "mvb_swiglu_gemm": (_i32, [_vp, _i64, _vp, _i64, _i64, _i64, _vp]),

@@ -1,0 +1,370 @@
+// Rows in 8 bits with one scale each, made where the values are made: RMSNorm (with the residual's addition), the
+// gated activations, plain rows; and read back.
+//
+// A row y stands as codes q = rint(127 y / amax) in -127 .. 127 and the scale amax / 127, amax = max |y|.
+//   plain     y = x
+//   norm      y = h w r, r = 1 / sqrt(mean(h^2) + eps); h = x, or T(residual + x), which is written too
+//   gated     y = act(gate) up
+// all in 32 bits, without the roundings to T that the unquantised forms have in between.  In the norm r cancels out of
+// 127 y / amax, so the codes are those of p = h w, and the mean goes into the scale alone: one pass, in which the sum
+// of squares and the maximum are reduced together.  For bf16 p is exact in 32 bits, and so is 127 p: the codes
+// are then the correctly rounded ones.
+//
+// A row with an infinity or a NaN (in y, before r) gets the scale NaN: it reads back as NaN, and so does a product with it.
+// A row of zeros gets the scale 0.
+#include <climits>
+
+#include "common.cuh"
+#include "host.h"
+
+namespace mvb {
+namespace {
+
+enum Kind { kPlain, kNorm, kAddNorm, kSilu, kGelu };
+
+struct RowArgs {
+  int8_t* q;        // [rows, width]
+  float* scale;     // [rows]
+  const void* a;    // x; the residual; gate
+  int64_t a_stride;
+  const void* b;    // x of the addition; up
+  int64_t b_stride;
+  void* sum;        // residual + x
+  int64_t sum_stride;
+  const void* w;
+  int width;
+  float eps;
+  float one;        // 1 for the (1 + w) norm, else 0
+};
+
+// g act'(g), by the logistic function: silu(g) = g / (1 + e^-g), and gelu's 0.5 g (1 + tanh z) = g / (1 + e^-2z).
+// The quotient and the exponential are the hardware's (some 1e-6 relative, against half a code's 4e-3).
+template <int KIND>
+__device__ __forceinline__ float act_of(float g) {
+  const float z = KIND == kSilu ? g : 1.5957691216057308f * g * fmaf(0.044715f * g, g, 1.0f);  // 2 sqrt(2 / pi)
+  return __fdividef(g, 1.0f + __expf(-z));
+}
+
+template <int KIND, typename T>
+__device__ __forceinline__ float value_of(float a, float b, float w, float one, float& h, float& ss) {
+  if (KIND == kNorm || KIND == kAddNorm) {
+    h = KIND == kAddNorm ? rnd<T>(a + b) : a;
+    ss = fmaf(h, h, ss);
+    return h * (w + one);
+  }
+  if (KIND == kSilu || KIND == kGelu) return act_of<KIND>(a) * b;
+  return a;
+}
+
+// The codes of one row.  127 y and amax are taken times a power of two where the quotient would leave fp32's range.
+struct Coder {
+  float f, amax, inv;
+  __device__ __forceinline__ explicit Coder(float top) {
+    f = top > 1.2676506e30f ? 5.4210109e-20f : top < 8.2718061e-25f ? 1.8446744e19f : 1.0f;  // 2^100, 2^-64, 2^-80, 2^64
+    amax = top * f;
+    inv = amax > 0.0f ? 127.0f / amax : 0.0f;
+  }
+  // The low byte of the result.  The product with the reciprocal is off by less than 2e-5; only where it comes so near
+  // a border between two codes is the quotient worked out.
+  __device__ __forceinline__ uint32_t of(float y) const {
+    constexpr float kMagic = 12582912.0f;  // 1.5 * 2^23: the sum's low bits are the nearest whole number
+    const float p = y * f, t = p * inv;
+    float m = t + kMagic;
+    if (fabsf(t - (m - kMagic)) > 0.49998f) m = __fdiv_rn(127.0f * p, amax) + kMagic;
+    return __float_as_uint(m);
+  }
+};
+__device__ __forceinline__ uint32_t pack4(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+  return __byte_perm(__byte_perm(a, b, 0x0040), __byte_perm(c, d, 0x0040), 0x5410);
+}
+
+__device__ __forceinline__ float abs_max(float m, float y) {  // the larger size by its bits: a NaN is above all
+  return __uint_as_float(max(__float_as_uint(m), __float_as_uint(y) & 0x7fffffffu));
+}
+
+// The block's sum and its largest size, in every thread.
+__device__ __forceinline__ void block_both(float& ss, float& top, float2* red) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    ss += __shfl_xor_sync(0xffffffffu, ss, o);
+    top = abs_max(top, __shfl_xor_sync(0xffffffffu, top, o));
+  }
+  const int warps = blockDim.x >> 5, lane = threadIdx.x & 31;
+  if (warps == 1) return;
+  if (lane == 0) red[threadIdx.x >> 5] = make_float2(ss, top);
+  __syncthreads();
+  const float2 v = lane < warps ? red[lane] : make_float2(0.0f, 0.0f);
+  ss = v.x;
+  top = v.y;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    ss += __shfl_xor_sync(0xffffffffu, ss, o);
+    top = abs_max(top, __shfl_xor_sync(0xffffffffu, top, o));
+  }
+}
+
+template <int KIND>
+__device__ __forceinline__ float row_scale(const RowArgs& a, float ss, float top) {
+  if (__float_as_uint(top) >= 0x7f800000u) return __uint_as_float(0x7fc00000u);
+  if (KIND == kNorm || KIND == kAddNorm) return top * (1.0f / sqrtf(ss / static_cast<float>(a.width) + a.eps)) / 127.0f;
+  return top / 127.0f;
+}
+
+template <typename T>
+__device__ __forceinline__ void load8(const T* p, float (&v)[8]) {
+  if (sizeof(T) == 4) {
+    const float4 x = reinterpret_cast<const float4*>(p)[0], y = reinterpret_cast<const float4*>(p)[1];
+    v[0] = x.x, v[1] = x.y, v[2] = x.z, v[3] = x.w, v[4] = y.x, v[5] = y.y, v[6] = y.z, v[7] = y.w;
+  } else {
+    const uint4 x = *reinterpret_cast<const uint4*>(p);
+    const T* e = reinterpret_cast<const T*>(&x);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = to_f<T>(e[i]);
+  }
+}
+template <typename T>
+__device__ __forceinline__ void store8(T* p, const float (&v)[8]) {
+  if (sizeof(T) == 4) {
+    reinterpret_cast<float4*>(p)[0] = make_float4(v[0], v[1], v[2], v[3]);
+    reinterpret_cast<float4*>(p)[1] = make_float4(v[4], v[5], v[6], v[7]);
+  } else {
+    uint4 x;
+    T* e = reinterpret_cast<T*>(&x);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) e[i] = from_f<T>(v[i]);
+    *reinterpret_cast<uint4*>(p) = x;
+  }
+}
+
+// A block per row, which stays in registers: vector j of a thread holds elements 8 (j blockDim + thread) .. + 7.
+template <int KIND, typename T, int VPT>
+__global__ void __launch_bounds__(1024) q8_rows_kernel(const RowArgs a) {
+  __shared__ float2 red[32];
+  pdl_launch_dependents();
+  pdl_wait();
+  const int64_t row = blockIdx.x;
+  const T* pa = static_cast<const T*>(a.a) + row * a.a_stride;
+  const T* pb = static_cast<const T*>(a.b) + row * a.b_stride;
+  const int vectors = a.width >> 3;
+  float y[VPT][8];
+  float ss = 0.0f, top = 0.0f;
+#pragma unroll
+  for (int j = 0; j < VPT; ++j) {
+    const int v = j * blockDim.x + threadIdx.x;
+    if (v < vectors) {
+      float x[8], z[8], w[8], h[8];
+      load8<T>(pa + 8 * v, x);
+      if (KIND >= kAddNorm) load8<T>(pb + 8 * v, z);
+      if (KIND == kNorm || KIND == kAddNorm) load8<T>(static_cast<const T*>(a.w) + 8 * v, w);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        y[j][i] = value_of<KIND, T>(x[i], z[i], w[i], a.one, h[i], ss);
+        top = abs_max(top, y[j][i]);
+      }
+      if (KIND == kAddNorm) store8<T>(static_cast<T*>(a.sum) + row * a.sum_stride + 8 * v, h);
+    }
+  }
+  block_both(ss, top, red);
+  const float scale = row_scale<KIND>(a, ss, top);
+  if (threadIdx.x == 0) a.scale[row] = scale;
+  const bool fine = __float_as_uint(top) < 0x7f800000u;
+  const Coder code(fine ? top : 0.0f);
+  uint2* q = reinterpret_cast<uint2*>(a.q + row * a.width);
+#pragma unroll
+  for (int j = 0; j < VPT; ++j) {
+    const int v = j * blockDim.x + threadIdx.x;
+    if (v < vectors) {
+      uint32_t c[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) c[i] = fine ? code.of(y[j][i]) : 0u;
+      q[v] = make_uint2(pack4(c[0], c[1], c[2], c[3]), pack4(c[4], c[5], c[6], c[7]));
+    }
+  }
+}
+
+// Any width and alignment: element by element, worked out again for the codes.
+template <int KIND, typename T>
+__global__ void __launch_bounds__(256) q8_any_kernel(const RowArgs a) {
+  __shared__ float2 red[32];
+  pdl_launch_dependents();
+  pdl_wait();
+  const int64_t row = blockIdx.x;
+  const T* pa = static_cast<const T*>(a.a) + row * a.a_stride;
+  const T* pb = static_cast<const T*>(a.b) + row * a.b_stride;
+  const T* pw = static_cast<const T*>(a.w);
+  T* sum = static_cast<T*>(a.sum) + row * a.sum_stride;
+  float ss = 0.0f, top = 0.0f, h = 0.0f;
+  for (int i = threadIdx.x; i < a.width; i += blockDim.x) {
+    const float w = KIND == kNorm || KIND == kAddNorm ? to_f<T>(pw[i]) : 0.0f;
+    const float y = value_of<KIND, T>(to_f<T>(pa[i]), KIND >= kAddNorm ? to_f<T>(pb[i]) : 0.0f, w, a.one, h, ss);
+    if (KIND == kAddNorm) sum[i] = from_f<T>(h);
+    top = abs_max(top, y);
+  }
+  block_both(ss, top, red);
+  if (threadIdx.x == 0) a.scale[row] = row_scale<KIND>(a, ss, top);
+  const bool fine = __float_as_uint(top) < 0x7f800000u;
+  const Coder code(fine ? top : 0.0f);
+  for (int i = threadIdx.x; i < a.width; i += blockDim.x) {
+    float y;
+    if (KIND == kAddNorm)
+      y = to_f<T>(sum[i]) * (to_f<T>(pw[i]) + a.one);  // what this thread has written: the residual may be gone
+    else
+      y = value_of<KIND, T>(to_f<T>(pa[i]), KIND >= kAddNorm ? to_f<T>(pb[i]) : 0.0f,
+                            KIND == kNorm ? to_f<T>(pw[i]) : 0.0f, a.one, h, ss);
+    a.q[row * a.width + i] = fine ? static_cast<int8_t>(code.of(y) & 0xffu) : int8_t(0);
+  }
+}
+
+template <typename T, bool VEC>
+__global__ void __launch_bounds__(256) dequantise_q8_kernel(T* __restrict__ out, const int8_t* __restrict__ q,
+                                                            int64_t q_stride, const float* __restrict__ scale,
+                                                            int64_t rows, int width) {
+  pdl_launch_dependents();
+  pdl_wait();
+  constexpr int N = VEC ? 8 : 1;
+  const int per = width / N;
+  const int64_t n = rows * per, step = static_cast<int64_t>(gridDim.x) * blockDim.x;
+  for (int64_t i = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x; i < n; i += step) {
+    const int64_t row = i / per;
+    const int col = static_cast<int>(i - row * per) * N;
+    const float s = scale[row];
+    if (VEC) {
+      const uint2 c = *reinterpret_cast<const uint2*>(q + row * q_stride + col);
+      const int8_t* e = reinterpret_cast<const int8_t*>(&c);
+      float v[8];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) v[k] = static_cast<float>(e[k]) * s;
+      store8<T>(out + row * width + col, v);
+    } else {
+      out[row * width + col] = from_f<T>(static_cast<float>(q[row * q_stride + col]) * s);
+    }
+  }
+}
+
+template <int KIND, typename T>
+int run_rows(const char* name, const RowArgs& a, int64_t rows, cudaStream_t stream) {
+  const size_t e = sizeof(T);
+  auto whole = [&](const void* p, int64_t stride) { return aligned(p, 16) && stride * e % 16 == 0; };
+  const bool vec = a.width % 8 == 0 && aligned(a.q, 8) && whole(a.a, a.a_stride) && whole(a.w, 0) &&
+                   (KIND < kAddNorm || whole(a.b, a.b_stride)) && (KIND != kAddNorm || whole(a.sum, a.sum_stride));
+  const int vectors = a.width / 8;
+  const dim3 grid(static_cast<unsigned>(rows));
+  if (!vec || vectors > 4 * 1024)
+    return launch(name, q8_any_kernel<KIND, T>, grid, dim3(256), 0, stream, a);
+  const int most = rows <= 2 * current_sm_count() ? 1 : 4;  // vectors of a thread
+  int threads = (vectors + most - 1) / most;
+  threads = threads > 1024 ? 1024 : (threads + 31) / 32 * 32;
+  const int per = (vectors + threads - 1) / threads;
+  const dim3 block(static_cast<unsigned>(threads));
+  if (per <= 1) return launch(name, q8_rows_kernel<KIND, T, 1>, grid, block, 0, stream, a);
+  if (per <= 2) return launch(name, q8_rows_kernel<KIND, T, 2>, grid, block, 0, stream, a);
+  return launch(name, q8_rows_kernel<KIND, T, 4>, grid, block, 0, stream, a);
+}
+
+template <int KIND>
+int run_kind(const char* name, const RowArgs& a, int64_t rows, int dtype, cudaStream_t stream) {
+  switch (dtype) {
+    case MVB_F32: return run_rows<KIND, float>(name, a, rows, stream);
+    case MVB_F16: return run_rows<KIND, __half>(name, a, rows, stream);
+    case MVB_BF16: return run_rows<KIND, __nv_bfloat16>(name, a, rows, stream);
+  }
+  return fail(MVB_ERR_INVALID_ARG, "%s: dtype code %d", name, dtype);
+}
+
+int check_rows(const char* name, int64_t rows, int64_t width, int dtype) {
+  MVB_REQUIRE(rows >= 0 && rows <= INT_MAX, "%s: %lld rows", name, (long long)rows);
+  MVB_REQUIRE(width > 0 && width <= (1 << 24), "%s: rows of %lld elements", name, (long long)width);
+  MVB_REQUIRE(dtype == MVB_F32 || dtype == MVB_F16 || dtype == MVB_BF16, "%s: dtype code %d", name, dtype);
+  return MVB_OK;
+}
+
+}  // namespace
+}  // namespace mvb
+
+using namespace mvb;
+
+extern "C" int mvb_quantise_q8(int8_t* values, float* scales, const void* in, int64_t in_stride, int64_t rows,
+                               int64_t width, int dtype, mvb_stream_t stream) {
+  const char* name = "mvb_quantise_q8";
+  MVB_TRY(check_rows(name, rows, width, dtype));
+  if (rows == 0) return MVB_OK;
+  MVB_REQUIRE(values && scales && in, "%s: null pointer", name);
+  MVB_REQUIRE(rows == 1 || in_stride >= width, "%s: rows %lld apart", name, (long long)in_stride);
+  RowArgs a = {};
+  a.q = values, a.scale = scales, a.a = in, a.a_stride = in_stride, a.width = static_cast<int>(width);
+  return run_kind<kPlain>(name, a, rows, dtype, reinterpret_cast<cudaStream_t>(stream));
+}
+
+extern "C" int mvb_rmsnorm_q8(int8_t* values, float* scales, const void* in, int64_t in_stride, const void* weight,
+                              int64_t rows, int64_t hidden, float eps, int plus_one, int dtype, mvb_stream_t stream) {
+  const char* name = "mvb_rmsnorm_q8";
+  MVB_TRY(check_rows(name, rows, hidden, dtype));
+  if (rows == 0) return MVB_OK;
+  MVB_REQUIRE(values && scales && in && weight, "%s: null pointer", name);
+  MVB_REQUIRE(rows == 1 || in_stride >= hidden, "%s: rows %lld apart", name, (long long)in_stride);
+  RowArgs a = {};
+  a.q = values, a.scale = scales, a.a = in, a.a_stride = in_stride, a.w = weight;
+  a.width = static_cast<int>(hidden), a.eps = eps, a.one = plus_one ? 1.0f : 0.0f;
+  return run_kind<kNorm>(name, a, rows, dtype, reinterpret_cast<cudaStream_t>(stream));
+}
+
+extern "C" int mvb_fused_add_rmsnorm_q8(int8_t* values, float* scales, void* residual_out, int64_t out_stride,
+                                        const void* residual, int64_t residual_stride, const void* in,
+                                        int64_t in_stride, const void* weight, int64_t rows, int64_t hidden, float eps,
+                                        int plus_one, int dtype, mvb_stream_t stream) {
+  const char* name = "mvb_fused_add_rmsnorm_q8";
+  MVB_TRY(check_rows(name, rows, hidden, dtype));
+  if (rows == 0) return MVB_OK;
+  MVB_REQUIRE(values && scales && residual_out && residual && in && weight, "%s: null pointer", name);
+  MVB_REQUIRE(rows == 1 || (in_stride >= hidden && residual_stride >= hidden && out_stride >= hidden),
+              "%s: rows %lld, %lld and %lld apart", name, (long long)in_stride, (long long)residual_stride,
+              (long long)out_stride);
+  RowArgs a = {};
+  a.q = values, a.scale = scales, a.a = residual, a.a_stride = residual_stride, a.b = in, a.b_stride = in_stride;
+  a.sum = residual_out, a.sum_stride = out_stride, a.w = weight;
+  a.width = static_cast<int>(hidden), a.eps = eps, a.one = plus_one ? 1.0f : 0.0f;
+  return run_kind<kAddNorm>(name, a, rows, dtype, reinterpret_cast<cudaStream_t>(stream));
+}
+
+extern "C" int mvb_gated_q8(int8_t* values, float* scales, const void* gate, int64_t gate_stride, const void* up,
+                            int64_t up_stride, int64_t rows, int64_t width, int act, int dtype, mvb_stream_t stream) {
+  const char* name = "mvb_gated_q8";
+  MVB_TRY(check_rows(name, rows, width, dtype));
+  MVB_REQUIRE(act == MVB_ACT_SILU || act == MVB_ACT_GELU_TANH, "%s: activation %d", name, act);
+  if (rows == 0) return MVB_OK;
+  MVB_REQUIRE(values && scales && gate && up, "%s: null pointer", name);
+  MVB_REQUIRE(rows == 1 || (gate_stride >= width && up_stride >= width), "%s: rows %lld and %lld apart", name,
+              (long long)gate_stride, (long long)up_stride);
+  RowArgs a = {};
+  a.q = values, a.scale = scales, a.a = gate, a.a_stride = gate_stride, a.b = up, a.b_stride = up_stride;
+  a.width = static_cast<int>(width);
+  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  return act == MVB_ACT_SILU ? run_kind<kSilu>(name, a, rows, dtype, st) : run_kind<kGelu>(name, a, rows, dtype, st);
+}
+
+extern "C" int mvb_dequantise_q8(void* out, const int8_t* values, int64_t values_stride, const float* scales,
+                                 int64_t rows, int64_t width, int dtype, mvb_stream_t stream) {
+  const char* name = "mvb_dequantise_q8";
+  MVB_TRY(check_rows(name, rows, width, dtype));
+  if (rows == 0) return MVB_OK;
+  MVB_REQUIRE(out && values && scales, "%s: null pointer", name);
+  MVB_REQUIRE(rows == 1 || values_stride >= width, "%s: rows %lld apart", name, (long long)values_stride);
+  const bool vec = width % 8 == 0 && aligned(values, 8) && values_stride % 8 == 0 && aligned(out, 16);
+  const int64_t n = rows * (vec ? width / 8 : width);
+  const int64_t sms = current_sm_count();
+  MVB_REQUIRE(sms > 0, "%s: no device", name);
+  const int64_t blocks = (n + 255) / 256;
+  const dim3 grid(static_cast<unsigned>(blocks < 8 * sms ? blocks : 8 * sms));
+  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  const int w = static_cast<int>(width);
+  auto run = [&](auto* o) {
+    using T = std::remove_pointer_t<decltype(o)>;
+    return vec ? launch(name, dequantise_q8_kernel<T, true>, grid, dim3(256), 0, st, o, values, values_stride, scales,
+                        rows, w)
+               : launch(name, dequantise_q8_kernel<T, false>, grid, dim3(256), 0, st, o, values, values_stride, scales,
+                        rows, w);
+  };
+  if (dtype == MVB_F32) return run(static_cast<float*>(out));
+  if (dtype == MVB_F16) return run(static_cast<__half*>(out));
+  return run(static_cast<__nv_bfloat16*>(out));
+}

@@ -27,7 +27,9 @@ __all__ = [
     "precompute_freqs_cis", "rotate_half", "apply_rotary_pos_emb", "silu", "gelu", "swiglu", "geglu",
     "greedy_sample", "top_k_top_p_filter", "softmax_multinomial_sample", "embedding", "Embedding", "softmax",
     "FusedMLP", "linear", "paged_attention_decode", "qk_norm_rope_kv_write", "sample", "kv4_write", "kv4_read",
-    "paged_attention_decode_kv4", "assign_slots", "SlotPlan", "verify_drafts",
+    "paged_attention_decode_kv4", "assign_slots", "SlotPlan", "verify_drafts", "Q8Rows", "quantise_q8",
+    "dequantise_q8", "rmsnorm_q8", "fused_add_rmsnorm_q8", "swiglu_q8", "geglu_q8", "W4Weight", "quantise_w4",
+    "pack_w4", "dequantise_w4", "linear_w4",
 ]
 
 
@@ -785,3 +787,310 @@ def verify_drafts(target_probs: torch.Tensor, draft_tokens: torch.Tensor, unifor
                 p_stride, N.ptr(draft_probs), q_stride, draft_tokens.data_ptr(), uniforms.data_ptr(),
                 N.ptr(draft_lens), B, K, V)
     return out, accepted
+
+
+# --------------------------------------------------------------------- rows in 8 bits
+class Q8Rows(NamedTuple):
+    """Rows in 8 bits with one scale each: element i of a row stands for ``values[..., i] * scales[...]``."""
+    values: torch.Tensor  # int8 [..., width], codes of -127 to 127
+    scales: torch.Tensor  # fp32 [...]
+
+
+_I8, _F16 = torch.int8, torch.float16
+_DTYPE_CODE = {_F32: N.F32, _F16: N.F16, _BF16: N.BF16}
+
+
+def _float_rows(what: str, name: str, t, index: int | None = None, dtype=None, shape=None) -> tuple[int, int]:
+    """Checks rows of a float type on a GPU; (device, dtype code)."""
+    if not isinstance(t, torch.Tensor):
+        raise RuntimeError(f"{what}: {name} must be a tensor")
+    at = t.get_device()
+    code = _DTYPE_CODE.get(t.dtype)
+    if at < 0:
+        N.require_cuda(t)
+    if code is None or t.dim() == 0 or t.shape[-1] == 0:
+        raise RuntimeError(f"{what}: {name} must be rows of float32, float16 or bfloat16, not {tuple(t.shape)} {t.dtype}")
+    if index is not None and (at != index or t.dtype is not dtype or t.shape != shape):
+        raise RuntimeError(f"{what}: {name} is {tuple(t.shape)} {t.dtype} on {t.device}, not {tuple(shape)} {dtype} on "
+                           f"cuda:{index}")
+    return at, code
+
+
+def _row_view(t: torch.Tensor) -> tuple[torch.Tensor, int] | None:
+    """``t`` as rows of stride-1 elements a fixed distance apart, and that distance; None if it is not."""
+    width = t.shape[-1]
+    if t.is_contiguous():
+        return t, width
+    if width > 1 and t.stride(-1) != 1:
+        return None
+    if t.dim() == 1:
+        return t, width
+    row, size = 0, 1  # rows of the dimensions so far are `row` apart
+    for n, stride in zip(reversed(t.shape[:-1]), reversed(t.stride()[:-1])):
+        if n == 1:
+            continue
+        if row and stride != row * size:
+            return None
+        row = row or stride
+        size *= n
+    row = row or width
+    return (t, row) if row >= width else None
+
+
+def _rows_of(t: torch.Tensor) -> tuple[torch.Tensor, int]:
+    """``_row_view``, of a copy where ``t`` is laid out otherwise."""
+    view = _row_view(t)
+    return view if view is not None else (t.contiguous(), t.shape[-1])
+
+
+def _q8_out(like: torch.Tensor) -> tuple[Q8Rows, int]:
+    shape = like.shape
+    values = torch.empty(shape, dtype=_I8, device=like.device)
+    scales = torch.empty(shape[:-1], dtype=_F32, device=like.device)
+    return Q8Rows(values, scales), scales.numel()
+
+
+def quantise_q8(input: torch.Tensor) -> Q8Rows:
+    """Rows ``[..., width]`` in 8 bits: per row ``amax = max |x|``, codes ``rint(127 x / amax)``, scale
+    ``amax / 127``.  A row with an infinity or a NaN reads back as NaN."""
+    what = "quantise_q8"
+    index, code = _float_rows(what, "input", input)
+    x, stride = _rows_of(input)
+    out, rows = _q8_out(x)
+    if rows:
+        N.on_device(index, what, N.lib().mvb_quantise_q8, out.values.data_ptr(), out.scales.data_ptr(), x.data_ptr(),
+                    stride, rows, x.shape[-1], code)
+    return out
+
+
+def _norm_weight(what: str, weight, index: int, width: int, dtype: torch.dtype) -> torch.Tensor:
+    if not isinstance(weight, torch.Tensor) or weight.get_device() != index or weight.shape != (width,):
+        if isinstance(weight, torch.Tensor):
+            N.require_cuda(weight)
+        raise RuntimeError(f"{what}: weight must be [{width}] on cuda:{index}")
+    if weight.dtype is not dtype:
+        weight = weight.to(dtype)
+    return weight.contiguous()
+
+
+def rmsnorm_q8(input: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6, plus_one: bool = False) -> Q8Rows:
+    """``rmsnorm`` (``plus_one``: with ``1 + weight``) whose result goes to 8 bits from its 32, without a
+    rounding to the dtype in between.  Rows, non-finite ones too, as in ``quantise_q8``."""
+    what = "rmsnorm_q8"
+    index, code = _float_rows(what, "input", input)
+    width = input.shape[-1]
+    w = _norm_weight(what, weight, index, width, input.dtype)
+    x, stride = _rows_of(input)
+    out, rows = _q8_out(x)
+    if rows:
+        N.on_device(index, what, N.lib().mvb_rmsnorm_q8, out.values.data_ptr(), out.scales.data_ptr(), x.data_ptr(),
+                    stride, w.data_ptr(), rows, width, float(eps), int(plus_one), code)
+    return out
+
+
+def fused_add_rmsnorm_q8(residual: torch.Tensor, input: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6,
+                         plus_one: bool = False,
+                         residual_out: torch.Tensor | None = None) -> tuple[Q8Rows, torch.Tensor]:
+    """``fused_add_rmsnorm`` with its result in 8 bits: ``residual + input``, rounded to the dtype, goes to
+    ``residual_out`` (default: into ``residual``, in place), its norm to 8 bits as in ``rmsnorm_q8``.
+    Returns ``(rows, residual_out)``."""
+    what = "fused_add_rmsnorm_q8"
+    index, code = _float_rows(what, "input", input)
+    _float_rows(what, "residual", residual, index, input.dtype, input.shape)
+    width = input.shape[-1]
+    w = _norm_weight(what, weight, index, width, input.dtype)
+    if residual_out is None:
+        residual_out = residual
+    else:
+        _float_rows(what, "residual_out", residual_out, index, input.dtype, input.shape)
+    view = _row_view(residual_out)
+    if view is None:
+        raise RuntimeError(f"{what}: the rows of {'residual' if residual_out is residual else 'residual_out'} must be "
+                           "contiguous and evenly apart: they are written")
+    out_stride = view[1]
+    x, stride = _rows_of(input)
+    res, res_stride = _rows_of(residual)
+    out, rows = _q8_out(x)
+    if rows:
+        N.on_device(index, what, N.lib().mvb_fused_add_rmsnorm_q8, out.values.data_ptr(), out.scales.data_ptr(),
+                    residual_out.data_ptr(), out_stride, res.data_ptr(), res_stride, x.data_ptr(), stride, w.data_ptr(),
+                    rows, width, float(eps), int(plus_one), code)
+    return out, residual_out
+
+
+def _gated_q8(what: str, gate, up, act: int) -> Q8Rows:
+    index, code = _float_rows(what, "gate", gate)
+    _float_rows(what, "up", up, index, gate.dtype, gate.shape)
+    (g, g_stride), (u, u_stride) = _rows_of(gate), _rows_of(up)
+    out, rows = _q8_out(g)
+    if rows:
+        N.on_device(index, what, N.lib().mvb_gated_q8, out.values.data_ptr(), out.scales.data_ptr(), g.data_ptr(), g_stride,
+                    u.data_ptr(), u_stride, rows, g.shape[-1], act, code)
+    return out
+
+
+def swiglu_q8(gate: torch.Tensor, up: torch.Tensor) -> Q8Rows:
+    """``swiglu`` with its result in 8 bits: ``silu(gate) * up`` in 32 bits, then as in ``quantise_q8``.  The halves
+    of a projection's ``[..., 2 I]`` output (``.chunk(2, -1)``) are read where they are."""
+    return _gated_q8("swiglu_q8", gate, up, N.ACT_SILU)
+
+
+def geglu_q8(gate: torch.Tensor, up: torch.Tensor) -> Q8Rows:
+    """``geglu`` (tanh approximation) with its result in 8 bits, as ``swiglu_q8``."""
+    return _gated_q8("geglu_q8", gate, up, N.ACT_GELU_TANH)
+
+
+def _check_q8(what: str, rows) -> int:
+    """Device of rows in 8 bits, checked."""
+    v, s = rows
+    if not (isinstance(v, torch.Tensor) and isinstance(s, torch.Tensor)):
+        raise RuntimeError(f"{what}: values and scales must be tensors")
+    index = v.get_device()
+    if index < 0 or s.get_device() < 0:
+        N.require_cuda(v, s)
+    if (v.dtype is not _I8 or s.dtype is not _F32 or v.dim() == 0 or v.shape[-1] == 0 or s.shape != v.shape[:-1]
+            or s.get_device() != index):
+        raise RuntimeError(f"{what}: values {tuple(v.shape)} {v.dtype} and scales {tuple(s.shape)} {s.dtype} are not int8 "
+                           "rows with an fp32 scale each, on one GPU")
+    return index
+
+
+def dequantise_q8(rows: Q8Rows, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
+    """What rows in 8 bits stand for, rounded to ``dtype`` (float32, float16 or bfloat16)."""
+    what = "dequantise_q8"
+    index = _check_q8(what, rows)
+    code = _DTYPE_CODE.get(dtype)
+    if code is None:
+        raise RuntimeError(f"{what}: float32, float16 or bfloat16, not {dtype}")
+    v, stride = _rows_of(rows.values)
+    scales = rows.scales.contiguous()
+    out = torch.empty(v.shape, dtype=dtype, device=v.device)
+    if scales.numel():
+        N.on_device(index, what, N.lib().mvb_dequantise_q8, out.data_ptr(), v.data_ptr(), stride, scales.data_ptr(),
+                    scales.numel(), v.shape[-1], code)
+    return out
+
+
+# --------------------------------------------------------------------- weights in 4 bits
+class W4Weight(NamedTuple):
+    """A weight matrix ``[n, k]`` in 4 bits with group scales, as ``quantise_w4`` and ``pack_w4`` lay it out."""
+    records: torch.Tensor  # uint8 [ceil(n / 16) * ceil(k / 128), 1024 + 64 * (128 / group)]
+    n: int
+    k: int
+    group: int
+
+
+def _w4_records(what: str, n: int, k: int, group: int, device: torch.device) -> torch.Tensor:
+    if group not in (32, 64, 128):
+        raise RuntimeError(f"{what}: groups of 32, 64 or 128 columns, not {group}")
+    if k <= 0 or k % 32:
+        raise RuntimeError(f"{what}: a multiple of 32 columns, not {k}")
+    return torch.empty((n + 15) // 16 * ((k + 127) // 128), 1024 + 8192 // group, dtype=_U8, device=device)
+
+
+def quantise_w4(weight: torch.Tensor, group: int = 128) -> W4Weight:
+    """A bf16 weight matrix ``[n, k]`` (k a multiple of 32) in 4 bits, once, for ``linear_w4``.  Per row and group
+    of 32, 64 or 128 columns: ``lo = min(0, min w)``, ``hi = max(0, max w)``, ``scale = bf16((hi - lo) / 15)``,
+    ``zero = rint(-lo / scale)``, ``code = rint(w / scale) + zero``; a weight stands for
+    ``scale * (code - zero)``.  A group with a NaN or an infinity reads back as NaN."""
+    what = "quantise_w4"
+    index = weight.get_device() if isinstance(weight, torch.Tensor) else -1
+    _expect(what, "weight", weight, index, _BF16, 2)
+    n, k = weight.shape
+    records = _w4_records(what, n, k, group, weight.device)
+    w, stride = _rows_of(weight)
+    if w.data_ptr() % 16 or stride % 8:
+        w, stride = w.clone(memory_format=torch.contiguous_format), k
+    if n:
+        N.on_device(index, what, N.lib().mvb_quantise_w4, records.data_ptr(), w.data_ptr(), stride, n, k, group)
+    return W4Weight(records, n, k, group)
+
+
+def pack_w4(codes: torch.Tensor, scales: torch.Tensor, zeros: torch.Tensor | None = None, group: int = 128) -> W4Weight:
+    """The same from a checkpoint's numbers: ``codes`` uint8 ``[n, k]``, ``scales`` bf16 and ``zeros`` uint8
+    ``[n, ceil(k / group)]`` (None: 8 everywhere, a symmetric checkpoint).  Of codes and zeros the low 4 bits count."""
+    what = "pack_w4"
+    index = codes.get_device() if isinstance(codes, torch.Tensor) else -1
+    _expect(what, "codes", codes, index, _U8, 2)
+    _expect(what, "scales", scales, index, _BF16, 2)
+    n, k = codes.shape
+    records = _w4_records(what, n, k, group, codes.device)
+    want = (n, (k + group - 1) // group)
+    if zeros is not None:
+        _expect(what, "zeros", zeros, index, _U8, 2)
+    if scales.shape != want or zeros is not None and zeros.shape != want:
+        raise RuntimeError(f"{what}: scales and zeros of {tuple(codes.shape)} codes in groups of {group} must be {want}")
+    codes, scales = codes.contiguous(), scales.contiguous()
+    if codes.data_ptr() % 8:
+        codes = codes.clone()
+    if zeros is not None:
+        zeros = zeros.contiguous()
+    if n:
+        N.on_device(index, what, N.lib().mvb_pack_w4, records.data_ptr(), codes.data_ptr(), scales.data_ptr(),
+                    N.ptr(zeros), n, k, group)
+    return W4Weight(records, n, k, group)
+
+
+def _check_w4(what: str, weight: W4Weight) -> int:
+    """Device of a 4-bit weight, checked."""
+    r, n, k, group = weight
+    if (not isinstance(r, torch.Tensor) or r.dtype is not _U8 or group not in (32, 64, 128) or k <= 0 or k % 32 or n < 0
+            or r.shape != ((n + 15) // 16 * ((k + 127) // 128), 1024 + 8192 // group) or not r.is_contiguous()
+            or r.data_ptr() % 16):
+        raise RuntimeError(f"{what}: weight must be what quantise_w4 or pack_w4 gave")
+    index = r.get_device()
+    if index < 0:
+        N.require_cuda(r)
+    return index
+
+
+def dequantise_w4(weight: W4Weight, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
+    """The matrix ``[n, k]`` that a 4-bit weight stands for, rounded to bfloat16, or in float32."""
+    what = "dequantise_w4"
+    index = _check_w4(what, weight)
+    if dtype not in (_BF16, _F32):
+        raise RuntimeError(f"{what}: float32 or bfloat16, not {dtype}")
+    records, n, k, group = weight
+    out = torch.empty(n, k, dtype=dtype, device=records.device)
+    if n:
+        N.on_device(index, what, N.lib().mvb_dequantise_w4, out.data_ptr(), records.data_ptr(), n, k, group,
+                    _DTYPE_CODE[dtype])
+    return out
+
+
+def linear_w4(x: torch.Tensor | Q8Rows, weight: W4Weight, out: torch.Tensor | None = None) -> torch.Tensor:
+    """``linear`` with a 4-bit weight: ``x @ w.T`` (bf16) for bf16 rows ``[..., k]`` or rows in 8 bits (``Q8Rows``), one
+    row to many.  Sums run in 32 bits and are rounded once; no weight or product is rounded before.
+    ``out``: bf16 ``[rows, n]`` with contiguous rows."""
+    what = "linear_w4"
+    index = _check_w4(what, weight)
+    records, n, k, group = weight
+    scales = None
+    if type(x) is Q8Rows:
+        if _check_q8(what, x) != index:
+            raise RuntimeError(f"{what}: x is on {x.values.device}, the weight on {records.device}")
+        scales = x.scales.contiguous()
+        x = x.values
+    elif not isinstance(x, torch.Tensor) or x.dtype is not _BF16 or x.get_device() != index or x.dim() == 0:
+        if isinstance(x, torch.Tensor):
+            N.require_cuda(x)
+        raise RuntimeError(f"{what}: x must be bfloat16 rows or Q8Rows on {records.device}")
+    shape = x.shape
+    if shape[-1] != k:
+        raise RuntimeError(f"{what}: rows of {shape[-1]} elements for {k} columns")
+    x, ldx = _rows_of(x)
+    if x.data_ptr() % 16 or ldx * x.element_size() % 16:
+        x, ldx = x.clone(memory_format=torch.contiguous_format), k
+    rows = x.numel() // k
+    if out is None:
+        out = torch.empty(*shape[:-1], n, dtype=_BF16, device=x.device)
+        ldy = n
+    else:
+        _expect(what, "out", out, index, _BF16, 2)
+        ldy = out.stride(0) if rows > 1 else n
+        if out.shape != (rows, n) or n > 1 and out.stride(1) != 1 or ldy < n:
+            raise RuntimeError(f"{what}: out must be {(rows, n)} with contiguous rows, apart")
+    if rows and n:
+        N.on_device(index, what, N.lib().mvb_linear_w4, out.data_ptr(), ldy, x.data_ptr(), ldx, N.ptr(scales),
+                    records.data_ptr(), rows, n, k, group)
+    return out.reshape(*shape[:-1], n) if out.dim() != len(shape) else out
