@@ -1,0 +1,508 @@
+// Products of many rows with 4-bit weights, on tcgen05 (few rows: w4_linear.cu, with the formula).
+//
+// Codes less zeros are whole numbers of -15 .. 15, exact in bf16 and in 8 bits.  They are unpacked from shared memory into
+// TMEM, where they are the 128-row operand of tcgen05.mma; rows of x are its columns, from shared memory as TMA brings
+// them: bf16 products with fp32 sums, or 8-bit ones with whole sums.  A group's sum is scaled as it leaves TMEM and added
+// up in registers, in 32 bits: no weight and no product is rounded.
+//
+// A block takes up to 256 weight rows, as two halves of 128 lanes, by BN rows of x.  Roles:
+//   warp 0        one bulk copy per run of records and a TMA box of x for 128 columns, into a ring
+//   warp 1        the products of a half's group, into one of four accumulators
+//   warps 4 - 11  two teams that unpack halves in turn, a weight row a thread, into one of four operands in TMEM
+//   warps 12 - 19 a team per half: accumulator out of TMEM, times the row's scale, onto the sums; the results' rows
+// Weight rows are given out in tiles of 16, so that few of them leave no SM idle; a cluster of up to 8 blocks splits the
+// columns where there are fewer, and its sums meet in distributed shared memory in the order of the blocks.
+#include <climits>
+
+#include "common.cuh"
+#include "host.h"
+#include "w4.cuh"
+#include "w4_linear.h"
+
+namespace mvb {
+namespace {
+
+constexpr int kThreads = 640;
+constexpr int kMaxTiles = 16;  // 16-row tiles of a block
+constexpr int kMaxStages = 8;
+constexpr int kMaxCluster = 8;
+constexpr size_t kMostSmem = 227 * 1024;
+
+struct GemmW4Args {
+  __nv_bfloat16* y;
+  int64_t ldy;
+  const float* a;  // scales of the rows of x
+  const uint8_t* records;
+  int rows, n;
+  int tiles, blocks;  // 16-row tiles, 128-column blocks
+  int chunk, chunks;  // tiles of an item; items down the weight rows
+  int columns;        // items across the rows of x
+  int cluster, stages;
+  unsigned* err;
+};
+
+// D[tmem] (+)= A[tmem] * B[smem]^T: bf16 with fp32 sums, or 8 bits with whole ones.
+template <bool Q8>
+__device__ __forceinline__ void umma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+  if (Q8)
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::i8 [%0], [%1], %2, %3, p;\n\t}\n" ::"r"(d),
+        "r"(a), "l"(b), "r"(idesc), "r"(accumulate)
+        : "memory");
+  else
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}\n" ::"r"(d),
+        "r"(a), "l"(b), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+
+// Instruction descriptor of kind::i8: D = s32, A = B = s8, both K-major.
+__host__ __device__ constexpr uint32_t umma_idesc_s8(int M, int N) {
+  return (2u << 4) | (1u << 7) | (1u << 10) | (static_cast<uint32_t>(N >> 3) << 17) | (static_cast<uint32_t>(M >> 4) << 24);
+}
+
+__device__ __forceinline__ void tmem_st_x16(uint32_t taddr, const uint32_t* r) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+      "%16};" ::"r"(taddr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+      : "memory");
+}
+__device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+// (w >> 4 j) of a word, less the zero: two bf16 numbers code - zero (z2: 128 + zero twice)
+__device__ __forceinline__ uint32_t codes_bf16(uint32_t w, uint32_t z2) {
+  uint32_t v = (w & 0x000f000fu) | 0x43004300u, d;
+  asm("sub.rn.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(v), "r"(z2));
+  return d;
+}
+// The low nibbles of four bytes, less the zero (z4: four times): with the top bit set no byte borrows from the next.
+__device__ __forceinline__ uint32_t codes_s8(uint32_t w, uint32_t z4) {
+  return (((w & 0x0f0f0f0fu) | 0x80808080u) - z4) ^ 0x80808080u;
+}
+
+__device__ __forceinline__ void copy_bulk(void* dst, const void* src, uint32_t bytes, uint64_t* bar, uint64_t policy) {
+  asm volatile(
+      "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes.L2::cache_hint [%0], [%1], %2, [%3], %4;" ::"r"(
+          smem_u32(dst)),
+      "l"(src), "r"(bytes), "r"(smem_u32(bar)), "l"(policy)
+      : "memory");
+}
+
+// Shared memory: barriers; the ring of x boxes; the ring of records; the cluster's sums.
+template <bool Q8, int GROUP, int BN>
+struct Layout {
+  static constexpr int PER = kW4Cols / GROUP;
+  static constexpr int REC = w4_record_bytes(GROUP);
+  static constexpr int BOX = BN * 128;              // bytes of a box of x: 128 of each row
+  static constexpr int X_STAGE = BOX * (Q8 ? 1 : 2);
+  static constexpr int FIXED = 1024;
+  int chunk, stages;
+  bool cluster;
+  __host__ __device__ int w_stage() const { return chunk * REC; }
+  __host__ __device__ int x() const { return FIXED; }
+  __host__ __device__ int w() const { return x() + stages * X_STAGE; }
+  __host__ __device__ int part() const { return w() + stages * w_stage(); }
+  // 1023 more: the boxes begin on 1024 bytes
+  __host__ __device__ size_t bytes() const { return 1023 + part() + (cluster ? BN * chunk * kW4Rows * 4 : 0); }
+};
+
+struct Item {
+  int tile, count, column;  // first tile and number of tiles; first row of x / BN
+  __device__ __forceinline__ Item(const GemmW4Args& a, int i) {
+    const int r = i / a.columns;
+    column = i - r * a.columns;
+    tile = r * a.chunk;
+    count = min(a.chunk, a.tiles - tile);
+  }
+};
+
+template <bool Q8, int GROUP, int BN>
+__global__ void __launch_bounds__(kThreads, 1)
+    w4_gemm_kernel(const __grid_constant__ CUtensorMap tmX, const GemmW4Args a) {
+  using L = Layout<Q8, GROUP, BN>;
+  constexpr int PER = L::PER;
+  constexpr int KSTEPS = Q8 ? 4 : 8;           // steps of 32 bytes of x in 128 columns
+  constexpr int A_COLS = Q8 ? 32 : 64;         // TMEM columns of an operand
+  constexpr uint32_t IDESC = Q8 ? umma_idesc_s8(128, BN) : umma_idesc_bf16(128, BN);
+  constexpr uint32_t TMEM_COLS = 512;          // a power of two above 4 operands and 4 accumulators
+  static_assert(4 * A_COLS + 4 * BN <= 512, "TMEM");
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem);
+  uint64_t* empty = full + kMaxStages;
+  uint64_t* a_full = empty + kMaxStages;  // [4]
+  uint64_t* a_empty = a_full + 4;
+  uint64_t* d_full = a_empty + 4;
+  uint64_t* d_empty = d_full + 4;
+  uint64_t* drain = d_empty + 4;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int c = a.cluster, rank = static_cast<int>(blockIdx.x) % c, unit = static_cast<int>(blockIdx.x) / c;
+  const int units = static_cast<int>(gridDim.x) / c;
+  const L at = {a.chunk, a.stages, c > 1};
+  uint8_t* sx = smem + at.x();
+  uint8_t* sw = smem + at.w();
+  float* part = reinterpret_cast<float*>(smem + at.part());  // [BN][16 chunk]
+  const int S = a.stages;
+  const int halves = a.chunk > 8 ? 2 : 1;
+  const int items = a.chunks * a.columns;
+  const int mine = unit < items ? (items - unit + units - 1) / units : 0;
+  const int block0 = static_cast<int>(static_cast<int64_t>(rank) * a.blocks / c);
+  const int nk = static_cast<int>(static_cast<int64_t>(rank + 1) * a.blocks / c) - block0;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < S; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], halves * 8 + 1);
+    }
+    for (int i = 0; i < 4; ++i) {
+      mbar_init(&a_full[i], 4);
+      mbar_init(&a_empty[i], 1);
+      mbar_init(&d_full[i], 1);
+      mbar_init(&d_empty[i], 4);
+    }
+    mbar_init(drain, 1);
+    *abort_flag = 0;
+    fence_barrier_init();
+  }
+  if (warp == 1) {
+    tmem_alloc(tmem_slot, TMEM_COLS);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  if (threadIdx.x == 0) pdl_launch_dependents();
+  if (warp != 0) pdl_wait();
+
+  // Which accumulator a half's e-th group goes to, and its parity.
+  auto d_at = [&](int h, int e) { return h + halves * (halves == 2 ? e & 1 : e & 3); };
+  auto d_par = [&](int e) { return static_cast<uint32_t>(halves == 2 ? e >> 1 : e >> 2) & 1u; };
+
+  int issued = 0;  // producer: stages asked for
+  bool ok = true;
+  int it = 0;      // 128-column steps so far, over all items
+  // A cluster's blocks add their sums of an item up.  They have the same items, so they meet as often, in every role.
+  auto meet = [&](const Item& item) {
+    if (c == 1) return;
+    __syncwarp();
+    cluster_sync();
+    const int row0 = item.column * BN, rows = min(BN, a.rows - row0), width = item.count * kW4Rows;
+    for (int i = rank * kThreads + static_cast<int>(threadIdx.x); i < rows * width; i += c * kThreads) {
+      const int m = i / width, r = i - m * width, col = item.tile * kW4Rows + r;
+      if (col >= a.n) continue;
+      float v = 0.0f;
+      for (int p = 0; p < c; ++p) v += dsmem_ld_f32(part + m * (a.chunk * kW4Rows) + r, p);
+      if (Q8) v *= __ldg(a.a + row0 + m);
+      a.y[(row0 + m) * a.ldy + col] = __float2bfloat16_rn(v);
+    }
+    cluster_sync();  // everybody has read: the sums may change, or their block end
+  };
+  if (warp == 0) {
+    const uint64_t pol_w = l2_policy_evict_first(), pol_x = l2_policy_evict_last();
+    for (int n = 0; n < mine; ++n) {
+      const Item item(a, unit + n * units);
+      if (lane == 0 && ok) {
+        const uint32_t bytes = item.count * L::REC + L::X_STAGE;
+        auto load_w = [&](int s, int kb) {
+          for (int t = 0; t < item.count;) {  // runs of records that lie together: up to three
+            const int tile = item.tile + t, run = min(item.count - t, 8 - (tile & 7));
+            copy_bulk(sw + s * at.w_stage() + t * L::REC,
+                      a.records + w4_record(tile, block0 + kb, a.tiles, a.blocks) * L::REC, run * L::REC, &full[s], pol_w);
+            t += run;
+          }
+        };
+        auto load_x = [&](int s, int kb) {
+          const int col = (block0 + kb) * kW4Cols;
+          tma_load_2d(sx + s * L::X_STAGE, &tmX, &full[s], col, item.column * BN, pol_x);
+          if (!Q8) tma_load_2d(sx + s * L::X_STAGE + L::BOX, &tmX, &full[s], col + 64, item.column * BN, pol_x);
+        };
+        int kb = 0;
+        if (n == 0) {
+          // weights are constant: their copies need not wait for the kernel before
+          const int pro = min(S, nk);
+          for (; kb < pro; ++kb) {
+            mbar_arrive_expect_tx(&full[kb], bytes);
+            load_w(kb, kb);
+          }
+          pdl_wait();
+          for (int i = 0; i < pro; ++i) load_x(i, i);
+          issued = pro;
+        }
+        for (; kb < nk; ++kb) {
+          const int s = issued % S;
+          if (!mbar_wait(&empty[s], (issued / S & 1) ^ 1, abort_flag, a.err)) {
+            ok = false;
+            break;
+          }
+          mbar_arrive_expect_tx(&full[s], bytes);
+          load_w(s, kb);
+          load_x(s, kb);
+          ++issued;
+        }
+      }
+      meet(item);
+    }
+  } else if (warp == 1) {
+    for (int n = 0; n < mine; ++n) {
+      if (lane == 0) {
+        for (int kb = 0; kb < nk && ok; ++kb, ++it) {
+          const int s = it % S;
+          ok = mbar_wait(&full[s], it / S & 1, abort_flag, a.err);
+          const uint64_t bd = umma_desc_sw128(smem_u32(sx + s * L::X_STAGE));
+          for (int h = 0; h < halves && ok; ++h) {
+            const int j = it * halves + h;
+            ok = mbar_wait(&a_full[j & 3], j >> 2 & 1, abort_flag, a.err);
+            const uint32_t ta = tmem + (j & 3) * A_COLS;
+#pragma unroll
+            for (int g = 0; g < PER; ++g) {
+              const int e = it * PER + g, buf = d_at(h, e);
+              ok = ok && mbar_wait(&d_empty[buf], d_par(e) ^ 1, abort_flag, a.err);
+              if (!ok) break;
+              tc_fence_after();
+#pragma unroll
+              for (int k = g * KSTEPS / PER; k < (g + 1) * KSTEPS / PER; ++k)
+                umma_ts<Q8>(tmem + 4 * A_COLS + buf * BN, ta + 8 * k, bd + (k & 3) * 2 + (k >> 2) * (L::BOX >> 4), IDESC,
+                            k > g * KSTEPS / PER ? 1u : 0u);
+              umma_commit(&d_full[buf]);
+            }
+            if (ok) umma_commit(&a_empty[j & 3]);
+          }
+          if (ok) umma_commit(&empty[s]);
+        }
+      }
+      meet(Item(a, unit + n * units));
+    }
+  } else if (warp >= 4 && warp < 12) {
+    const int team = (warp - 4) >> 2, q = warp & 3;
+    const uint32_t lanes = static_cast<uint32_t>(q * 32) << 16;
+    for (int n = 0; n < mine; ++n) {
+      const Item item(a, unit + n * units);
+      for (int kb = 0; kb < nk && ok; ++kb, ++it) {
+        const int s = it % S;
+        for (int h = 0; h < halves; ++h) {
+          const int j = it * halves + h;
+          if ((j & 1) != team) continue;
+          ok = mbar_wait(&full[s], it / S & 1, abort_flag, a.err) &&
+               mbar_wait(&a_empty[j & 3], (j >> 2 & 1) ^ 1, abort_flag, a.err);
+          ok = __all_sync(0xffffffffu, ok);
+          if (!ok) break;
+          const int tile = h * 8 + q * 2;
+          if (tile < item.count) {  // of a warp's two tiles the first at least
+            const uint8_t* rec = sw + s * at.w_stage() + min(tile + (lane >> 4), item.count - 1) * L::REC;
+            uint32_t w[4][4], pair[PER];
+#pragma unroll
+            for (int t = 0; t < 4; ++t) {
+              const uint4 v = *reinterpret_cast<const uint4*>(rec + (lane & 15) * 64 + w4_place(t, lane) * 16);
+              w[0][t] = v.x, w[1][t] = v.y, w[2][t] = v.z, w[3][t] = v.w;
+            }
+#pragma unroll
+            for (int g = 0; g < PER; ++g)
+              pair[g] = reinterpret_cast<const uint32_t*>(rec + kW4CodeBytes)[(lane & 15) * PER + g];
+            tc_fence_after();
+            const uint32_t ta = tmem + lanes + (j & 3) * A_COLS;
+            if (Q8) {
+#pragma unroll
+              for (int i = 0; i < 4; i += 2) {
+                uint32_t o[16];
+#pragma unroll
+                for (int z = 0; z < 2; ++z) {
+                  const uint32_t z4 = __byte_perm(pair[(i + z) * PER / 4], 0, 0x2222) & 0x0f0f0f0fu;
+#pragma unroll
+                  for (int t = 0; t < 4; ++t) {
+                    const uint32_t lo = codes_s8(w[i + z][t], z4), hi = codes_s8(w[i + z][t] >> 4, z4);
+                    o[z * 8 + t * 2] = __byte_perm(lo, hi, 0x6420);
+                    o[z * 8 + t * 2 + 1] = __byte_perm(lo, hi, 0x7531);
+                  }
+                }
+                tmem_st_x16(ta + i * 8, o);
+              }
+            } else {
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                const uint32_t z2 = __byte_perm(pair[i * PER / 4], 0, 0x3232);
+                uint32_t o[16];
+#pragma unroll
+                for (int t = 0; t < 4; ++t)
+#pragma unroll
+                  for (int e = 0; e < 4; ++e) o[t * 4 + e] = codes_bf16(w[i][t] >> (4 * e), z2);
+                tmem_st_x16(ta + i * 16, o);
+              }
+            }
+            tmem_st_wait();
+            tc_fence_before();
+          }
+          __syncwarp();
+          if (lane == 0) {
+            mbar_arrive(&a_full[j & 3]);
+            mbar_arrive(&empty[s]);
+          }
+        }
+      }
+      meet(item);
+    }
+  } else if (warp >= 12 && (warp - 12) >> 2 < halves) {
+    const int h = (warp - 12) >> 2, q = warp & 3;
+    const int tile = h * 8 + q * 2 + (lane >> 4);  // of the item
+    const uint32_t td = tmem + (static_cast<uint32_t>(q * 32) << 16) + 4 * A_COLS;
+    for (int n = 0; n < mine; ++n) {
+      const Item item(a, unit + n * units);
+      const bool some = h * 8 + q * 2 < item.count;
+      float acc[BN];
+#pragma unroll
+      for (int i = 0; i < BN; ++i) acc[i] = 0.0f;
+      for (int kb = 0; kb < nk && ok; ++kb, ++it) {
+        const int s = it % S;
+        ok = __all_sync(0xffffffffu, mbar_wait(&full[s], it / S & 1, abort_flag, a.err));
+        if (!ok) break;
+        float scale[PER];
+        const uint8_t* rec = sw + s * at.w_stage() + min(tile, item.count - 1) * L::REC;
+#pragma unroll
+        for (int g = 0; g < PER; ++g)
+          scale[g] = __uint_as_float(reinterpret_cast<const uint32_t*>(rec + kW4CodeBytes)[(lane & 15) * PER + g] << 16);
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&empty[s]);
+#pragma unroll
+        for (int g = 0; g < PER; ++g) {
+          const int e = it * PER + g, buf = d_at(h, e);
+          ok = __all_sync(0xffffffffu, ok && mbar_wait(&d_full[buf], d_par(e), abort_flag, a.err));
+          if (ok) {
+            tc_fence_after();
+            if (some) {
+#pragma unroll
+              for (int c0 = 0; c0 < BN; c0 += 16) {
+                uint32_t d[16];
+                tmem_ld_x16(td + buf * BN + c0, d);
+                tmem_ld_wait();
+#pragma unroll
+                for (int i = 0; i < 16; ++i)
+                  acc[c0 + i] = fmaf(scale[g], Q8 ? static_cast<float>(static_cast<int>(d[i])) : __uint_as_float(d[i]), acc[c0 + i]);
+              }
+            }
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&d_empty[buf]);
+          }
+        }
+      }
+      const int row0 = item.column * BN, rows = min(BN, a.rows - row0);
+      const int col = (item.tile + tile) * kW4Rows + (lane & 15);
+      int width = a.chunk * kW4Rows;
+      int64_t ldy = a.ldy;
+      asm volatile("" : "+r"(width), "+l"(ldy));  // not known outside: or all their multiples are kept, in local memory
+      if (c > 1) {
+        if (tile < item.count) {
+          float* to = part + tile * kW4Rows + (lane & 15);
+#pragma unroll
+          for (int i = 0; i < BN; ++i) {
+            if (i < rows) *to = acc[i];
+            to += width;
+          }
+        }
+      } else if (tile < item.count && col < a.n) {
+        __nv_bfloat16* y = a.y + row0 * a.ldy + col;
+        const float* scales = a.a + row0;
+#pragma unroll
+        for (int i = 0; i < BN; ++i) {
+          if (i < rows) *y = __float2bfloat16_rn(Q8 ? acc[i] * __ldg(scales + i) : acc[i]);
+          y += ldy;
+        }
+      }
+      meet(item);
+    }
+  } else {
+    for (int n = 0; n < mine; ++n) meet(Item(a, unit + n * units));
+  }
+
+  // Every product has ended before TMEM is given back, and every copy before the block ends.
+  if (warp == 1 && lane == 0) {
+    umma_commit(drain);
+    mbar_wait(drain, 0, nullptr, a.err);
+  }
+  if (warp == 0 && lane == 0) {
+    const int first = issued > S ? issued - S : 0;
+    for (int i = first; i < issued; ++i) mbar_wait(&full[i % S], i / S & 1, nullptr, a.err);
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem, TMEM_COLS);
+  }
+}
+
+template <bool Q8, int GROUP, int BN>
+int run(const char* name, const W4LinearCall& call, cudaStream_t stream) {
+  using L = Layout<Q8, GROUP, BN>;
+  const int sms = current_sm_count();
+  MVB_REQUIRE(sms > 0, "%s: no device", name);
+  auto kernel = w4_gemm_kernel<Q8, GROUP, BN>;
+  static std::atomic<uint64_t> done{0};
+  MVB_TRY(set_smem_once(done, kernel, kMostSmem, name));
+  GemmW4Args a = {};
+  a.y = call.y, a.ldy = call.ldy, a.a = call.row_scales, a.records = call.records, a.rows = call.rows, a.n = call.n;
+  a.tiles = (call.n + kW4Rows - 1) / kW4Rows;
+  a.blocks = (call.k + kW4Cols - 1) / kW4Cols;
+  a.columns = (call.rows + BN - 1) / BN;
+  a.err = device_status_ptr();
+  // Tiles of an item and blocks of a cluster: the fewest bytes through an SM's port (records and x, as often as they
+  // are read), with what a cluster's meeting costs.
+  double least = 0;
+  for (int c = 1; c <= kMaxCluster && c <= a.blocks; ++c) {
+    const int units = sms / c;
+    for (int chunk = 1; chunk <= kMaxTiles && chunk <= a.tiles; ++chunk) {
+      const int64_t items = static_cast<int64_t>((a.tiles + chunk - 1) / chunk) * a.columns;
+      const double waves = static_cast<double>((items + units - 1) / units);
+      const double cost = waves * ((a.blocks + c - 1) / c * static_cast<double>(chunk * L::REC + L::X_STAGE) +
+                                   (c > 1 ? 60000.0 : 20000.0));
+      if (a.chunk == 0 || cost < least) least = cost, a.cluster = c, a.chunk = chunk;
+    }
+  }
+  a.chunks = (a.tiles + a.chunk - 1) / a.chunk;
+  L at = {a.chunk, kMaxStages, a.cluster > 1};
+  while (at.bytes() > kMostSmem) --at.stages;
+  a.stages = at.stages;
+  // One block an SM, whatever it needs: a second would wait for the first one's TMEM, and where both are of one cluster the
+  // first for the second.
+  const size_t smem = at.bytes() > 120 * 1024 ? at.bytes() : 120 * 1024;
+  const int64_t items = static_cast<int64_t>(a.chunks) * a.columns;
+  const int units = items < sms / a.cluster ? static_cast<int>(items) : sms / a.cluster;
+
+  CUtensorMap tm;
+  const uint64_t dims[2] = {static_cast<uint64_t>(call.k), static_cast<uint64_t>(call.rows)};
+  const uint64_t strides[1] = {static_cast<uint64_t>(call.ldx) * (Q8 ? 1 : 2)};
+  const uint32_t box[2] = {Q8 ? 128u : 64u, BN};
+  MVB_TRY(encode_tiled(&tm, Q8 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, call.x, dims, strides,
+                       box, CU_TENSOR_MAP_SWIZZLE_128B));
+  const dim3 grid(static_cast<unsigned>(units * a.cluster));
+  if (a.cluster == 1) return launch(name, kernel, grid, dim3(kThreads), smem, stream, tm, a);
+  return launch_cluster(name, kernel, grid, dim3(kThreads), static_cast<unsigned>(a.cluster), smem,
+                        stream, tm, a);
+}
+
+template <bool Q8, int GROUP>
+int run_rows(const char* name, const W4LinearCall& call, cudaStream_t stream) {
+  return call.rows <= 32 ? run<Q8, GROUP, 32>(name, call, stream) : run<Q8, GROUP, 64>(name, call, stream);
+}
+
+template <bool Q8>
+int run_group(const char* name, const W4LinearCall& call, cudaStream_t stream) {
+  if (call.group == 32) return run_rows<Q8, 32>(name, call, stream);
+  if (call.group == 64) return run_rows<Q8, 64>(name, call, stream);
+  return run_rows<Q8, 128>(name, call, stream);
+}
+
+}  // namespace
+
+int w4_gemm(const char* name, const W4LinearCall& call, cudaStream_t stream) {
+  return call.row_scales != nullptr ? run_group<true>(name, call, stream) : run_group<false>(name, call, stream);
+}
+
+}  // namespace mvb
