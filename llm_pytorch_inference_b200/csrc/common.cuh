@@ -97,6 +97,26 @@ __device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, volati
   return false;
 }
 
+// The same for waits that end soon and follow one another, where the clock's first reading (some hundreds of cycles)
+// would be most of the wait: it is read from the 64th poll on.
+__device__ __forceinline__ bool mbar_wait_soon(uint64_t* bar, uint32_t parity, volatile int* abort_flag,
+                                               unsigned* err) {
+  const uint32_t addr = smem_u32(bar);
+  unsigned long long t0 = 0;
+  for (unsigned polls = 1; polls < kWaitMaxPolls; ++polls) {
+    if (mbar_try_wait(addr, parity)) return true;
+    if ((polls & 63u) == 0) {
+      if (abort_flag != nullptr && *abort_flag) return false;
+      const unsigned long long now = globaltimer_ns();
+      if (t0 == 0) t0 = now;
+      if (now - t0 > kWaitLimitNs) break;
+    }
+  }
+  report(err, kDevWaitTimeout);
+  if (abort_flag != nullptr) *abort_flag = 1;
+  return false;
+}
+
 // ------------------------------------------------------------------ TMA
 __device__ __forceinline__ uint64_t l2_policy_evict_first() {
   uint64_t p;

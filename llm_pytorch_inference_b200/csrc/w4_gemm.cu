@@ -6,15 +6,16 @@
 // up in registers, in 32 bits: no weight and no product is rounded.
 //
 // A block takes up to 256 weight rows, as two halves of 128 lanes, by BN rows of x.  Roles:
-//   warp 0        one bulk copy per run of records and a TMA box of x for 128 columns, into a ring
-//   warp 1        the products of a half's group, into one of four accumulators
-//   warps 4 - 11  two teams that unpack halves in turn, a weight row a thread, into one of four operands in TMEM
-//   warps 12 - 19 a team per half: accumulator out of TMEM, times the row's scale, onto the sums; the results' rows
+//   warps 0, 2    for 128 columns the records, a bulk copy per run that lies together, and a TMA box of x, into a ring
+//   warp 1        the products of a group, into one of two accumulators a half
+//   warps 4 - 11  unpack, a weight row a thread, into one of two operands a half in TMEM
+//   warps 12 - 19 accumulator out of TMEM, times the row's scale, onto the sums; the results' rows
 // Weight rows are given out in tiles of 16, so that few of them leave no SM idle; a cluster of up to 8 blocks splits the
 // columns where there are fewer, and its sums meet in distributed shared memory in the order of the blocks.
 #include <climits>
 
 #include "common.cuh"
+#include "f32x2.cuh"
 #include "host.h"
 #include "w4.cuh"
 #include "w4_linear.h"
@@ -63,6 +64,12 @@ __host__ __device__ constexpr uint32_t umma_idesc_s8(int M, int N) {
   return (2u << 4) | (1u << 7) | (1u << 10) | (static_cast<uint32_t>(N >> 3) << 17) | (static_cast<uint32_t>(M >> 4) << 24);
 }
 
+__device__ __forceinline__ bool elect_one() {
+  uint32_t p;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}\n" : "=r"(p));
+  return p != 0;
+}
+
 __device__ __forceinline__ void tmem_st_x16(uint32_t taddr, const uint32_t* r) {
   asm volatile(
       "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
@@ -82,6 +89,65 @@ __device__ __forceinline__ uint32_t codes_bf16(uint32_t w, uint32_t z2) {
 // The low nibbles of four bytes, less the zero (z4: four times): with the top bit set no byte borrows from the next.
 __device__ __forceinline__ uint32_t codes_s8(uint32_t w, uint32_t z4) {
   return (((w & 0x0f0f0f0fu) | 0x80808080u) - z4) ^ 0x80808080u;
+}
+
+// Sums out of TMEM, two at a time.  Whole sums are below 2^18 in size: added to the bits of 1.5 * 2^23 they are its low
+// bits, where the conversion instruction would take a quarter of the rate.
+template <bool Q8>
+__device__ __forceinline__ F2 sums_of(uint32_t a, uint32_t b) {
+  if (!Q8) return F2{__uint_as_float(a), __uint_as_float(b)};
+  return add2(F2{__uint_as_float(a + 0x4b400000u), __uint_as_float(b + 0x4b400000u)}, F2{-12582912.0f, -12582912.0f});
+}
+
+// Waits for all of up to three barriers.  A poll of a barrier takes some 120 cycles even where its phase is over, so
+// they are polled together.
+struct Wait {
+  uint32_t bar, parity;
+  __device__ __forceinline__ Wait(uint64_t* b, uint32_t p) : bar(smem_u32(b)), parity(p & 1u) {}
+};
+__device__ __forceinline__ bool polls(Wait a, Wait b, Wait c) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p, q, r;\n\t"
+      "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      "mbarrier.try_wait.parity.shared::cta.b64 q, [%3], %4;\n\t"
+      "mbarrier.try_wait.parity.shared::cta.b64 r, [%5], %6;\n\t"
+      "and.pred p, p, q;\n\tand.pred p, p, r;\n\tselp.u32 %0, 1, 0, p;\n\t}\n"
+      : "=r"(ok)
+      : "r"(a.bar), "r"(a.parity), "r"(b.bar), "r"(b.parity), "r"(c.bar), "r"(c.parity)
+      : "memory");
+  return ok != 0;
+}
+__device__ __forceinline__ bool polls(Wait a, Wait b) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t"
+      "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      "mbarrier.try_wait.parity.shared::cta.b64 q, [%3], %4;\n\t"
+      "and.pred p, p, q;\n\tselp.u32 %0, 1, 0, p;\n\t}\n"
+      : "=r"(ok)
+      : "r"(a.bar), "r"(a.parity), "r"(b.bar), "r"(b.parity)
+      : "memory");
+  return ok != 0;
+}
+__device__ __forceinline__ bool polls(Wait a) { return mbar_try_wait(a.bar, a.parity); }
+
+// Bounded like mbar_wait; the clock is first read at the 64th poll.
+template <typename... W>
+__device__ __forceinline__ bool wait_all(volatile int* abort_flag, unsigned* err, W... w) {
+  unsigned long long t0 = 0;
+  for (unsigned n = 1; n < kWaitMaxPolls; ++n) {
+    if (polls(w...)) return true;
+    if ((n & 63u) == 0) {
+      if (*abort_flag) return false;
+      const unsigned long long now = globaltimer_ns();
+      if (t0 == 0) t0 = now;
+      if (now - t0 > kWaitLimitNs) break;
+    }
+  }
+  report(err, kDevWaitTimeout);
+  *abort_flag = 1;
+  return false;
 }
 
 __device__ __forceinline__ void copy_bulk(void* dst, const void* src, uint32_t bytes, uint64_t* bar, uint64_t policy) {
@@ -134,11 +200,11 @@ __global__ void __launch_bounds__(kThreads, 1)
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint64_t* full = reinterpret_cast<uint64_t*>(smem);
   uint64_t* empty = full + kMaxStages;
-  uint64_t* a_full = empty + kMaxStages;  // [4]
-  uint64_t* a_empty = a_full + 4;
-  uint64_t* d_full = a_empty + 4;
-  uint64_t* d_empty = d_full + 4;
-  uint64_t* drain = d_empty + 4;
+  uint64_t* a_full = empty + kMaxStages;  // [2] operands unpacked
+  uint64_t* a_empty = a_full + 2;         // [2] and used
+  uint64_t* d_full = a_empty + 2;         // [2] a group's sums made
+  uint64_t* d_empty = d_full + 2;         // [2] and read
+  uint64_t* drain = d_empty + 2;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
@@ -157,15 +223,15 @@ __global__ void __launch_bounds__(kThreads, 1)
   const int nk = static_cast<int>(static_cast<int64_t>(rank + 1) * a.blocks / c) - block0;
 
   if (threadIdx.x == 0) {
-    for (int s = 0; s < S; ++s) {
-      mbar_init(&full[s], 1);
-      mbar_init(&empty[s], halves * 8 + 1);
+    for (int i = 0; i < S; ++i) {
+      mbar_init(&full[i], 2);
+      mbar_init(&empty[i], halves * 8);
     }
-    for (int i = 0; i < 4; ++i) {
-      mbar_init(&a_full[i], 4);
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&a_full[i], halves * 4);
       mbar_init(&a_empty[i], 1);
       mbar_init(&d_full[i], 1);
-      mbar_init(&d_empty[i], 4);
+      mbar_init(&d_empty[i], halves * 4);
     }
     mbar_init(drain, 1);
     *abort_flag = 0;
@@ -180,18 +246,20 @@ __global__ void __launch_bounds__(kThreads, 1)
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
   if (threadIdx.x == 0) pdl_launch_dependents();
-  if (warp != 0) pdl_wait();
+  if (warp != 0) pdl_wait();  // warp 0 reads weights alone, which are constant
 
-  // Which accumulator a half's e-th group goes to, and its parity.
-  auto d_at = [&](int h, int e) { return h + halves * (halves == 2 ? e & 1 : e & 3); };
-  auto d_par = [&](int e) { return static_cast<uint32_t>(halves == 2 ? e >> 1 : e >> 2) & 1u; };
-
-  int issued = 0;  // producer: stages asked for
   bool ok = true;
-  int it = 0;      // 128-column steps so far, over all items
+  int it = 0;      // 128-column steps so far, over all items; their place in the ring and its parity
+  int s = 0;
+  uint32_t ph = 0;
+  auto step = [&]() {
+    ++it;
+    if (++s == S) s = 0, ph ^= 1;
+  };
   // A cluster's blocks add their sums of an item up.  They have the same items, so they meet as often, in every role.
   auto meet = [&](const Item& item) {
     if (c == 1) return;
+    if (warp == 0) pdl_wait();
     __syncwarp();
     cluster_sync();
     const int row0 = item.column * BN, rows = min(BN, a.rows - row0), width = item.count * kW4Rows;
@@ -205,145 +273,125 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     cluster_sync();  // everybody has read: the sums may change, or their block end
   };
-  if (warp == 0) {
-    const uint64_t pol_w = l2_policy_evict_first(), pol_x = l2_policy_evict_last();
+  auto all = [](bool x) { return __all_sync(0xffffffffu, x) != 0; };
+  if (warp == 0 || warp == 2) {
+    // Weights, and x.
+    const uint64_t policy = warp == 0 ? l2_policy_evict_first() : l2_policy_evict_last();
     for (int n = 0; n < mine; ++n) {
       const Item item(a, unit + n * units);
-      if (lane == 0 && ok) {
-        const uint32_t bytes = item.count * L::REC + L::X_STAGE;
-        auto load_w = [&](int s, int kb) {
-          for (int t = 0; t < item.count;) {  // runs of records that lie together: up to three
-            const int tile = item.tile + t, run = min(item.count - t, 8 - (tile & 7));
-            copy_bulk(sw + s * at.w_stage() + t * L::REC,
-                      a.records + w4_record(tile, block0 + kb, a.tiles, a.blocks) * L::REC, run * L::REC, &full[s], pol_w);
-            t += run;
+      for (int kb = 0; kb < nk && ok; ++kb, step()) {
+        ok = all(wait_all(abort_flag, a.err, Wait(&empty[s], ph ^ 1)));
+        if (!ok) break;
+        if (lane == 0) {
+          if (warp == 0) {
+            mbar_arrive_expect_tx(&full[s], item.count * L::REC);
+            for (int t = 0; t < item.count;) {  // runs of records that lie together: up to three
+              const int tile = item.tile + t, run = min(item.count - t, 8 - (tile & 7));
+              copy_bulk(sw + s * at.w_stage() + t * L::REC,
+                        a.records + w4_record(tile, block0 + kb, a.tiles, a.blocks) * L::REC, run * L::REC, &full[s], policy);
+              t += run;
+            }
+          } else {
+            mbar_arrive_expect_tx(&full[s], L::X_STAGE);
+            const int col = (block0 + kb) * kW4Cols;
+            tma_load_2d(sx + s * L::X_STAGE, &tmX, &full[s], col, item.column * BN, policy);
+            if (!Q8) tma_load_2d(sx + s * L::X_STAGE + L::BOX, &tmX, &full[s], col + 64, item.column * BN, policy);
           }
-        };
-        auto load_x = [&](int s, int kb) {
-          const int col = (block0 + kb) * kW4Cols;
-          tma_load_2d(sx + s * L::X_STAGE, &tmX, &full[s], col, item.column * BN, pol_x);
-          if (!Q8) tma_load_2d(sx + s * L::X_STAGE + L::BOX, &tmX, &full[s], col + 64, item.column * BN, pol_x);
-        };
-        int kb = 0;
-        if (n == 0) {
-          // weights are constant: their copies need not wait for the kernel before
-          const int pro = min(S, nk);
-          for (; kb < pro; ++kb) {
-            mbar_arrive_expect_tx(&full[kb], bytes);
-            load_w(kb, kb);
-          }
-          pdl_wait();
-          for (int i = 0; i < pro; ++i) load_x(i, i);
-          issued = pro;
         }
-        for (; kb < nk; ++kb) {
-          const int s = issued % S;
-          if (!mbar_wait(&empty[s], (issued / S & 1) ^ 1, abort_flag, a.err)) {
-            ok = false;
-            break;
-          }
-          mbar_arrive_expect_tx(&full[s], bytes);
-          load_w(s, kb);
-          load_x(s, kb);
-          ++issued;
-        }
+        __syncwarp();
       }
       meet(item);
     }
   } else if (warp == 1) {
+    // The whole warp runs the loops, so that addresses and descriptors stay in uniform registers; one thread issues.
+    const bool leader = elect_one();
     for (int n = 0; n < mine; ++n) {
-      if (lane == 0) {
-        for (int kb = 0; kb < nk && ok; ++kb, ++it) {
-          const int s = it % S;
-          ok = mbar_wait(&full[s], it / S & 1, abort_flag, a.err);
-          const uint64_t bd = umma_desc_sw128(smem_u32(sx + s * L::X_STAGE));
-          for (int h = 0; h < halves && ok; ++h) {
-            const int j = it * halves + h;
-            ok = mbar_wait(&a_full[j & 3], j >> 2 & 1, abort_flag, a.err);
-            const uint32_t ta = tmem + (j & 3) * A_COLS;
+      for (int kb = 0; kb < nk && ok; ++kb, step()) {
+        const uint64_t bd = umma_desc_sw128(smem_u32(sx + s * L::X_STAGE));
+        const uint32_t ta = tmem + (it & 1) * 2 * A_COLS;
 #pragma unroll
-            for (int g = 0; g < PER; ++g) {
-              const int e = it * PER + g, buf = d_at(h, e);
-              ok = ok && mbar_wait(&d_empty[buf], d_par(e) ^ 1, abort_flag, a.err);
-              if (!ok) break;
-              tc_fence_after();
+        for (int g = 0; g < PER; ++g) {
+          const int e = it * PER + g;
+          const Wait room(&d_empty[e & 1], (e >> 1) ^ 1);
+          if (g == 0)
+            ok = all(wait_all(abort_flag, a.err, Wait(&full[s], ph), Wait(&a_full[it & 1], it >> 1), room));
+          else
+            ok = ok && all(wait_all(abort_flag, a.err, room));
+          if (!ok) break;
+          tc_fence_after();
+          if (leader) {
+            const uint32_t td = tmem + 4 * A_COLS + (e & 1) * 2 * BN;
+            for (int h = 0; h < halves; ++h)
 #pragma unroll
               for (int k = g * KSTEPS / PER; k < (g + 1) * KSTEPS / PER; ++k)
-                umma_ts<Q8>(tmem + 4 * A_COLS + buf * BN, ta + 8 * k, bd + (k & 3) * 2 + (k >> 2) * (L::BOX >> 4), IDESC,
+                umma_ts<Q8>(td + h * BN, ta + h * A_COLS + 8 * k, bd + (k & 3) * 2 + (k >> 2) * (L::BOX >> 4), IDESC,
                             k > g * KSTEPS / PER ? 1u : 0u);
-              umma_commit(&d_full[buf]);
-            }
-            if (ok) umma_commit(&a_empty[j & 3]);
+            umma_commit(&d_full[e & 1]);
+            if (PER > 1 && g == PER - 1) umma_commit(&a_empty[it & 1]);
           }
-          if (ok) umma_commit(&empty[s]);
+          __syncwarp();
         }
       }
       meet(Item(a, unit + n * units));
     }
-  } else if (warp >= 4 && warp < 12) {
-    const int team = (warp - 4) >> 2, q = warp & 3;
+  } else if (warp >= 4 && warp < 12 && (warp - 4) >> 2 < halves) {
+    const int h = (warp - 4) >> 2, q = warp & 3, tile = h * 8 + q * 2;  // a warp's two tiles
     const uint32_t lanes = static_cast<uint32_t>(q * 32) << 16;
     for (int n = 0; n < mine; ++n) {
       const Item item(a, unit + n * units);
-      for (int kb = 0; kb < nk && ok; ++kb, ++it) {
-        const int s = it % S;
-        for (int h = 0; h < halves; ++h) {
-          const int j = it * halves + h;
-          if ((j & 1) != team) continue;
-          ok = mbar_wait(&full[s], it / S & 1, abort_flag, a.err) &&
-               mbar_wait(&a_empty[j & 3], (j >> 2 & 1) ^ 1, abort_flag, a.err);
-          ok = __all_sync(0xffffffffu, ok);
-          if (!ok) break;
-          const int tile = h * 8 + q * 2;
-          if (tile < item.count) {  // of a warp's two tiles the first at least
-            const uint8_t* rec = sw + s * at.w_stage() + min(tile + (lane >> 4), item.count - 1) * L::REC;
-            uint32_t w[4][4], pair[PER];
+      const int offset = min(tile + (lane >> 4), item.count - 1) * L::REC + (lane & 15) * 64;
+      for (int kb = 0; kb < nk && ok; ++kb, step()) {
+        // The operand's last use: the products of two steps ago.  Groups of 128 columns show it by their sums.
+        ok = all(wait_all(abort_flag, a.err, Wait(&full[s], ph), Wait(PER > 1 ? &a_empty[it & 1] : &d_full[it & 1], (it >> 1) ^ 1)));
+        if (!ok) break;
+        if (tile < item.count) {
+          const uint8_t* row = sw + s * at.w_stage() + offset;
+          uint32_t w[4][4], pair[PER];
 #pragma unroll
-            for (int t = 0; t < 4; ++t) {
-              const uint4 v = *reinterpret_cast<const uint4*>(rec + (lane & 15) * 64 + w4_place(t, lane) * 16);
-              w[0][t] = v.x, w[1][t] = v.y, w[2][t] = v.z, w[3][t] = v.w;
-            }
+          for (int t = 0; t < 4; ++t) {
+            const uint4 v = *reinterpret_cast<const uint4*>(row + w4_place(t, lane) * 16);
+            w[0][t] = v.x, w[1][t] = v.y, w[2][t] = v.z, w[3][t] = v.w;
+          }
+          const uint32_t* pairs = reinterpret_cast<const uint32_t*>(row - (lane & 15) * (64 - PER * 4) + kW4CodeBytes);
 #pragma unroll
-            for (int g = 0; g < PER; ++g)
-              pair[g] = reinterpret_cast<const uint32_t*>(rec + kW4CodeBytes)[(lane & 15) * PER + g];
-            tc_fence_after();
-            const uint32_t ta = tmem + lanes + (j & 3) * A_COLS;
-            if (Q8) {
+          for (int g = 0; g < PER; ++g) pair[g] = pairs[g];
+          tc_fence_after();
+          const uint32_t ta = tmem + lanes + ((it & 1) * 2 + h) * A_COLS;
+          if (Q8) {
 #pragma unroll
-              for (int i = 0; i < 4; i += 2) {
-                uint32_t o[16];
+            for (int i = 0; i < 4; i += 2) {
+              uint32_t o[16];
 #pragma unroll
-                for (int z = 0; z < 2; ++z) {
-                  const uint32_t z4 = __byte_perm(pair[(i + z) * PER / 4], 0, 0x2222) & 0x0f0f0f0fu;
+              for (int z = 0; z < 2; ++z) {
+                const uint32_t z4 = __byte_perm(pair[(i + z) * PER / 4], 0, 0x2222) & 0x0f0f0f0fu;
 #pragma unroll
-                  for (int t = 0; t < 4; ++t) {
-                    const uint32_t lo = codes_s8(w[i + z][t], z4), hi = codes_s8(w[i + z][t] >> 4, z4);
-                    o[z * 8 + t * 2] = __byte_perm(lo, hi, 0x6420);
-                    o[z * 8 + t * 2 + 1] = __byte_perm(lo, hi, 0x7531);
-                  }
+                for (int t = 0; t < 4; ++t) {
+                  const uint32_t lo = codes_s8(w[i + z][t], z4), hi = codes_s8(w[i + z][t] >> 4, z4);
+                  o[z * 8 + t * 2] = __byte_perm(lo, hi, 0x6420);
+                  o[z * 8 + t * 2 + 1] = __byte_perm(lo, hi, 0x7531);
                 }
-                tmem_st_x16(ta + i * 8, o);
               }
-            } else {
-#pragma unroll
-              for (int i = 0; i < 4; ++i) {
-                const uint32_t z2 = __byte_perm(pair[i * PER / 4], 0, 0x3232);
-                uint32_t o[16];
-#pragma unroll
-                for (int t = 0; t < 4; ++t)
-#pragma unroll
-                  for (int e = 0; e < 4; ++e) o[t * 4 + e] = codes_bf16(w[i][t] >> (4 * e), z2);
-                tmem_st_x16(ta + i * 16, o);
-              }
+              tmem_st_x16(ta + i * 8, o);
             }
-            tmem_st_wait();
-            tc_fence_before();
+          } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const uint32_t z2 = __byte_perm(pair[i * PER / 4], 0, 0x3232);
+              uint32_t o[16];
+#pragma unroll
+              for (int t = 0; t < 4; ++t)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) o[t * 4 + e] = codes_bf16(w[i][t] >> (4 * e), z2);
+              tmem_st_x16(ta + i * 16, o);
+            }
           }
-          __syncwarp();
-          if (lane == 0) {
-            mbar_arrive(&a_full[j & 3]);
-            mbar_arrive(&empty[s]);
-          }
+          tmem_st_wait();
+          tc_fence_before();
+        }
+        __syncwarp();
+        if (lane == 0) {
+          mbar_arrive(&a_full[it & 1]);
+          mbar_arrive(&empty[s]);
         }
       }
       meet(item);
@@ -351,44 +399,47 @@ __global__ void __launch_bounds__(kThreads, 1)
   } else if (warp >= 12 && (warp - 12) >> 2 < halves) {
     const int h = (warp - 12) >> 2, q = warp & 3;
     const int tile = h * 8 + q * 2 + (lane >> 4);  // of the item
-    const uint32_t td = tmem + (static_cast<uint32_t>(q * 32) << 16) + 4 * A_COLS;
+    const uint32_t td = tmem + (static_cast<uint32_t>(q * 32) << 16) + 4 * A_COLS + h * BN;
     for (int n = 0; n < mine; ++n) {
       const Item item(a, unit + n * units);
       const bool some = h * 8 + q * 2 < item.count;
-      float acc[BN];
+      const int offset = min(tile, item.count - 1) * L::REC + kW4CodeBytes + (lane & 15) * PER * 4;
+      F2 acc[BN / 2];
 #pragma unroll
-      for (int i = 0; i < BN; ++i) acc[i] = 0.0f;
-      for (int kb = 0; kb < nk && ok; ++kb, ++it) {
-        const int s = it % S;
-        ok = __all_sync(0xffffffffu, mbar_wait(&full[s], it / S & 1, abort_flag, a.err));
-        if (!ok) break;
+      for (int i = 0; i < BN / 2; ++i) acc[i] = F2{0.0f, 0.0f};
+      for (int kb = 0; kb < nk && ok; ++kb, step()) {
         float scale[PER];
-        const uint8_t* rec = sw + s * at.w_stage() + min(tile, item.count - 1) * L::REC;
-#pragma unroll
-        for (int g = 0; g < PER; ++g)
-          scale[g] = __uint_as_float(reinterpret_cast<const uint32_t*>(rec + kW4CodeBytes)[(lane & 15) * PER + g] << 16);
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&empty[s]);
 #pragma unroll
         for (int g = 0; g < PER; ++g) {
-          const int e = it * PER + g, buf = d_at(h, e);
-          ok = __all_sync(0xffffffffu, ok && mbar_wait(&d_full[buf], d_par(e), abort_flag, a.err));
-          if (ok) {
-            tc_fence_after();
-            if (some) {
+          const int e = it * PER + g;
+          const Wait made(&d_full[e & 1], e >> 1);
+          if (g == 0) {
+            ok = all(wait_all(abort_flag, a.err, Wait(&full[s], ph), made));
+            const uint32_t* pairs = reinterpret_cast<const uint32_t*>(sw + s * at.w_stage() + offset);
 #pragma unroll
-              for (int c0 = 0; c0 < BN; c0 += 16) {
-                uint32_t d[16];
-                tmem_ld_x16(td + buf * BN + c0, d);
-                tmem_ld_wait();
+            for (int i = 0; i < PER; ++i) scale[i] = __uint_as_float(pairs[i] << 16);
+          } else {
+            ok = ok && all(wait_all(abort_flag, a.err, made));
+          }
+          if (!ok) break;
+          tc_fence_after();
+          if (some) {
+            const F2 s2 = {scale[g], scale[g]};
 #pragma unroll
-                for (int i = 0; i < 16; ++i)
-                  acc[c0 + i] = fmaf(scale[g], Q8 ? static_cast<float>(static_cast<int>(d[i])) : __uint_as_float(d[i]), acc[c0 + i]);
-              }
+            for (int c0 = 0; c0 < BN; c0 += 16) {
+              uint32_t d[16];
+              tmem_ld_x16(td + (e & 1) * 2 * BN + c0, d);
+              tmem_ld_wait();
+#pragma unroll
+              for (int i = 0; i < 16; i += 2)
+                acc[(c0 + i) / 2] = fma2(s2, sums_of<Q8>(d[i], d[i + 1]), acc[(c0 + i) / 2]);
             }
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&d_empty[buf]);
+          }
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) {
+            mbar_arrive(&d_empty[e & 1]);
+            if (g == PER - 1) mbar_arrive(&empty[s]);  // the products have ended too: x is free
           }
         }
       }
@@ -402,7 +453,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           float* to = part + tile * kW4Rows + (lane & 15);
 #pragma unroll
           for (int i = 0; i < BN; ++i) {
-            if (i < rows) *to = acc[i];
+            if (i < rows) *to = i & 1 ? acc[i / 2].y : acc[i / 2].x;
             to += width;
           }
         }
@@ -411,7 +462,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         const float* scales = a.a + row0;
 #pragma unroll
         for (int i = 0; i < BN; ++i) {
-          if (i < rows) *y = __float2bfloat16_rn(Q8 ? acc[i] * __ldg(scales + i) : acc[i]);
+          const float v = i & 1 ? acc[i / 2].y : acc[i / 2].x;
+          if (i < rows) *y = __float2bfloat16_rn(Q8 ? v * __ldg(scales + i) : v);
           y += ldy;
         }
       }
@@ -422,13 +474,12 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
 
   // Every product has ended before TMEM is given back, and every copy before the block ends.
-  if (warp == 1 && lane == 0) {
+  if (warp == 1 && elect_one()) {
     umma_commit(drain);
     mbar_wait(drain, 0, nullptr, a.err);
   }
-  if (warp == 0 && lane == 0) {
-    const int first = issued > S ? issued - S : 0;
-    for (int i = first; i < issued; ++i) mbar_wait(&full[i % S], i / S & 1, nullptr, a.err);
+  if ((warp == 0 || warp == 2) && lane == 0) {
+    for (int i = it > S ? it - S : 0; i < it; ++i) mbar_wait(&full[i % S], i / S & 1, nullptr, a.err);
   }
   tc_fence_before();
   __syncthreads();

@@ -308,7 +308,7 @@ __global__ void __launch_bounds__(kThreads, 1) w4_linear_kernel(const LinearArgs
 #pragma unroll
           for (int q = 0; q < 4; ++q) acc[s][nt][q] = 0.0f;
       for (int b = kw; b < blocks; b += split) {
-        mbar_wait(&bars[stage], phase, abort_flag, a.err);
+        mbar_wait_soon(&bars[stage], phase, abort_flag, a.err);
         compute<GROUP, P, NT>(ring + stage * 2 * L::REC, sx, info, b, lane, acc);
         __syncwarp();  // every lane has read: the next copy may come
         if (lane == 0) ask();
@@ -362,7 +362,7 @@ __global__ void __launch_bounds__(kThreads, 1) w4_linear_kernel(const LinearArgs
   }
   // Every copy has been waited for, unless a wait gave up: then those under way are, before the block ends.
   if (*abort_flag && lane == 0)
-    for (int s = 0; s < a.stages; ++s) mbar_wait(&bars[s], phase ^ (s < stage ? 0 : 1), nullptr, a.err);
+    for (int s = 0; s < a.stages; ++s) mbar_wait_soon(&bars[s], phase ^ (s < stage ? 0 : 1), nullptr, a.err);
 }
 
 template <int GROUP, int P, int NT>
