@@ -6,7 +6,7 @@
 // up in registers, in 32 bits: no weight and no product is rounded.
 //
 // A block takes up to 256 weight rows, as two halves of 128 lanes, by BN rows of x.  Roles:
-//   warps 0, 2    for 128 columns the records, a bulk copy per run that lies together, and a TMA box of x, into a ring
+//   warp 0        for 128 columns the records, a bulk copy per run that lies together, and TMA boxes of x, into a ring
 //   warp 1        the products of a group, into one of two accumulators a half
 //   warps 4 - 11  unpack, a weight row a thread, into one of two operands a half in TMEM
 //   warps 12 - 19 accumulator out of TMEM, times the row's scale, onto the sums; the results' rows
@@ -15,7 +15,6 @@
 #include <climits>
 
 #include "common.cuh"
-#include "f32x2.cuh"
 #include "host.h"
 #include "w4.cuh"
 #include "w4_linear.h"
@@ -94,60 +93,52 @@ __device__ __forceinline__ uint32_t codes_s8(uint32_t w, uint32_t z4) {
 // Sums out of TMEM, two at a time.  Whole sums are below 2^18 in size: added to the bits of 1.5 * 2^23 they are its low
 // bits, where the conversion instruction would take a quarter of the rate.
 template <bool Q8>
-__device__ __forceinline__ F2 sums_of(uint32_t a, uint32_t b) {
-  if (!Q8) return F2{__uint_as_float(a), __uint_as_float(b)};
-  return add2(F2{__uint_as_float(a + 0x4b400000u), __uint_as_float(b + 0x4b400000u)}, F2{-12582912.0f, -12582912.0f});
+__device__ __forceinline__ float2 sums_of(uint32_t a, uint32_t b) {
+  if (!Q8) return make_float2(__uint_as_float(a), __uint_as_float(b));
+  return __fadd2_rn(make_float2(__uint_as_float(a + 0x4b400000u), __uint_as_float(b + 0x4b400000u)),
+                    make_float2(-12582912.0f, -12582912.0f));
 }
 
-// Waits for all of up to three barriers.  A poll of a barrier takes some 120 cycles even where its phase is over, so
-// they are polled together.
-struct Wait {
-  uint32_t bar, parity;
-  __device__ __forceinline__ Wait(uint64_t* b, uint32_t p) : bar(smem_u32(b)), parity(p & 1u) {}
-};
-__device__ __forceinline__ bool polls(Wait a, Wait b, Wait c) {
-  uint32_t ok;
-  asm volatile(
-      "{\n\t.reg .pred p, q, r;\n\t"
-      "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
-      "mbarrier.try_wait.parity.shared::cta.b64 q, [%3], %4;\n\t"
-      "mbarrier.try_wait.parity.shared::cta.b64 r, [%5], %6;\n\t"
-      "and.pred p, p, q;\n\tand.pred p, p, r;\n\tselp.u32 %0, 1, 0, p;\n\t}\n"
-      : "=r"(ok)
-      : "r"(a.bar), "r"(a.parity), "r"(b.bar), "r"(b.parity), "r"(c.bar), "r"(c.parity)
-      : "memory");
-  return ok != 0;
+__device__ __forceinline__ void commit(uint32_t bar) {
+  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
 }
-__device__ __forceinline__ bool polls(Wait a, Wait b) {
-  uint32_t ok;
-  asm volatile(
-      "{\n\t.reg .pred p, q;\n\t"
-      "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
-      "mbarrier.try_wait.parity.shared::cta.b64 q, [%3], %4;\n\t"
-      "and.pred p, p, q;\n\tselp.u32 %0, 1, 0, p;\n\t}\n"
-      : "=r"(ok)
-      : "r"(a.bar), "r"(a.parity), "r"(b.bar), "r"(b.parity)
-      : "memory");
-  return ok != 0;
+__device__ __forceinline__ void arrive(uint32_t bar) {
+  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
 }
-__device__ __forceinline__ bool polls(Wait a) { return mbar_try_wait(a.bar, a.parity); }
-
-// Bounded like mbar_wait; the clock is first read at the 64th poll.
-template <typename... W>
-__device__ __forceinline__ bool wait_all(volatile int* abort_flag, unsigned* err, W... w) {
+// A whole warp's wait for the phase of parity `parity` (its low bit), bounded like mbar_wait; the clock is first read at
+// the 64th poll.  Even where the phase is over a poll takes some 120 cycles, and polls do not overlap: the loops below
+// are laid out for as few as they can.
+__device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag, unsigned* err) {
   unsigned long long t0 = 0;
+  bool ok = false;
   for (unsigned n = 1; n < kWaitMaxPolls; ++n) {
-    if (polls(w...)) return true;
+    ok = mbar_try_wait(bar, parity & 1u);
+    if (ok) break;
     if ((n & 63u) == 0) {
-      if (*abort_flag) return false;
+      if (*abort_flag) break;
       const unsigned long long now = globaltimer_ns();
       if (t0 == 0) t0 = now;
-      if (now - t0 > kWaitLimitNs) break;
+      if (now - t0 > kWaitLimitNs) {
+        report(err, kDevWaitTimeout);
+        *abort_flag = 1;
+        break;
+      }
     }
   }
-  report(err, kDevWaitTimeout);
-  *abort_flag = 1;
-  return false;
+  return __all_sync(0xffffffffu, ok) != 0;
+}
+
+template <int N>
+__device__ __forceinline__ void load_words(uint32_t (&v)[N], const uint8_t* p) {
+  if (N == 1) {
+    v[0] = __ldg(reinterpret_cast<const uint32_t*>(p));
+  } else if (N == 2) {
+    const uint2 x = __ldg(reinterpret_cast<const uint2*>(p));
+    v[0] = x.x, v[1 % N] = x.y;
+  } else {
+    const uint4 x = __ldg(reinterpret_cast<const uint4*>(p));
+    v[0] = x.x, v[1 % N] = x.y, v[2 % N] = x.z, v[3 % N] = x.w;
+  }
 }
 
 __device__ __forceinline__ void copy_bulk(void* dst, const void* src, uint32_t bytes, uint64_t* bar, uint64_t policy) {
@@ -198,13 +189,13 @@ __global__ void __launch_bounds__(kThreads, 1)
   static_assert(4 * A_COLS + 4 * BN <= 512, "TMEM");
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  uint64_t* full = reinterpret_cast<uint64_t*>(smem);
-  uint64_t* empty = full + kMaxStages;
-  uint64_t* a_full = empty + kMaxStages;  // [2] operands unpacked
-  uint64_t* a_empty = a_full + 2;         // [2] and used
-  uint64_t* d_full = a_empty + 2;         // [2] a group's sums made
-  uint64_t* d_empty = d_full + 2;         // [2] and read
-  uint64_t* drain = d_empty + 2;
+  uint64_t* full_at = reinterpret_cast<uint64_t*>(smem);  // [stages] a ring's place filled
+  uint64_t* drain = full_at + 2 * kMaxStages + 8;
+  const uint32_t full = smem_u32(smem), empty = full + 8 * kMaxStages;  // [stages] and read
+  const uint32_t a_full = empty + 8 * kMaxStages;  // [2] operands unpacked (groups of 128: and the accumulators read)
+  const uint32_t a_empty = a_full + 16;            // [2] and used (groups of 128: d_full says so)
+  const uint32_t d_full = a_empty + 16;            // [2] a group's sums made
+  const uint32_t d_empty = d_full + 16;            // [2] and read
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
@@ -224,14 +215,14 @@ __global__ void __launch_bounds__(kThreads, 1)
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < S; ++i) {
-      mbar_init(&full[i], 2);
-      mbar_init(&empty[i], halves * 8);
+      mbar_init(full_at + i, 1);
+      mbar_init(full_at + kMaxStages + i, halves * 4 + 1);
     }
     for (int i = 0; i < 2; ++i) {
-      mbar_init(&a_full[i], halves * 4);
-      mbar_init(&a_empty[i], 1);
-      mbar_init(&d_full[i], 1);
-      mbar_init(&d_empty[i], halves * 4);
+      mbar_init(full_at + 2 * kMaxStages + i, halves * (PER > 1 ? 4 : 8));
+      mbar_init(full_at + 2 * kMaxStages + 2 + i, 1);
+      mbar_init(full_at + 2 * kMaxStages + 4 + i, 1);
+      mbar_init(full_at + 2 * kMaxStages + 6 + i, halves * 4);
     }
     mbar_init(drain, 1);
     *abort_flag = 0;
@@ -246,7 +237,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
   if (threadIdx.x == 0) pdl_launch_dependents();
-  if (warp != 0) pdl_wait();  // warp 0 reads weights alone, which are constant
+  if (warp != 0) pdl_wait();  // warp 0 asks for weights first, which are constant
 
   bool ok = true;
   int it = 0;      // 128-column steps so far, over all items; their place in the ring and its parity
@@ -259,7 +250,6 @@ __global__ void __launch_bounds__(kThreads, 1)
   // A cluster's blocks add their sums of an item up.  They have the same items, so they meet as often, in every role.
   auto meet = [&](const Item& item) {
     if (c == 1) return;
-    if (warp == 0) pdl_wait();
     __syncwarp();
     cluster_sync();
     const int row0 = item.column * BN, rows = min(BN, a.rows - row0), width = item.count * kW4Rows;
@@ -273,31 +263,48 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     cluster_sync();  // everybody has read: the sums may change, or their block end
   };
-  auto all = [](bool x) { return __all_sync(0xffffffffu, x) != 0; };
-  if (warp == 0 || warp == 2) {
-    // Weights, and x.
-    const uint64_t policy = warp == 0 ? l2_policy_evict_first() : l2_policy_evict_last();
+  auto wait = [&](uint32_t bar, uint32_t parity) { return warp_wait(bar, parity, abort_flag, a.err); };
+  if (warp == 0) {
+    // Lanes 0 - 2 each ask for a run of records that lie together (up to three), lanes 3 and 4 for a box of x.
+    const uint64_t policy = lane < 3 ? l2_policy_evict_first() : l2_policy_evict_last();
     for (int n = 0; n < mine; ++n) {
       const Item item(a, unit + n * units);
-      for (int kb = 0; kb < nk && ok; ++kb, step()) {
-        ok = all(wait_all(abort_flag, a.err, Wait(&empty[s], ph ^ 1)));
+      const int first = 8 - (item.tile & 7);  // tiles of the first run
+      const int from = lane == 0 ? 0 : first + 8 * (lane - 1), to = min(item.count, first + 8 * lane);
+      const int run = (lane < 3 ? max(to - from, 0) : 0) * L::REC;
+      const int tile = item.tile + from;
+      const uint8_t* src = a.records;
+      int64_t apart = 0;  // bytes between the run's records of consecutive 128 columns
+      if (run > 0) {
+        src += w4_record(tile, block0, a.tiles, a.blocks) * L::REC;
+        apart = static_cast<int64_t>(min(8, a.tiles - (tile & ~7))) * L::REC;
+      }
+      const bool box = lane == 3 || (!Q8 && lane == 4);
+      const int row = item.column * BN;
+      int col = block0 * kW4Cols + (lane == 4 ? 64 : 0);
+      auto ask_w = [&](int at_stage) {
+        if (lane == 0) mbar_arrive_expect_tx(&full_at[at_stage], item.count * L::REC + L::X_STAGE);
+        if (run > 0) copy_bulk(sw + at_stage * at.w_stage() + from * L::REC, src, run, &full_at[at_stage], policy);
+        src += apart;
+      };
+      auto ask_x = [&](int at_stage) {
+        if (box)
+          tma_load_2d(sx + at_stage * L::X_STAGE + (lane == 4 ? L::BOX : 0), &tmX, &full_at[at_stage], col, row, policy);
+        col += kW4Cols;
+      };
+      int kb = 0;
+      if (n == 0) {
+        // weights are constant: their copies need not wait for the kernel before
+        const int pro = min(S, nk);
+        for (int i = 0; i < pro; ++i) ask_w(i);
+        pdl_wait();
+        for (; kb < pro; ++kb, step()) ask_x(kb);
+      }
+      for (; kb < nk && ok; ++kb, step()) {
+        ok = wait(empty + 8 * s, ph ^ 1);
         if (!ok) break;
-        if (lane == 0) {
-          if (warp == 0) {
-            mbar_arrive_expect_tx(&full[s], item.count * L::REC);
-            for (int t = 0; t < item.count;) {  // runs of records that lie together: up to three
-              const int tile = item.tile + t, run = min(item.count - t, 8 - (tile & 7));
-              copy_bulk(sw + s * at.w_stage() + t * L::REC,
-                        a.records + w4_record(tile, block0 + kb, a.tiles, a.blocks) * L::REC, run * L::REC, &full[s], policy);
-              t += run;
-            }
-          } else {
-            mbar_arrive_expect_tx(&full[s], L::X_STAGE);
-            const int col = (block0 + kb) * kW4Cols;
-            tma_load_2d(sx + s * L::X_STAGE, &tmX, &full[s], col, item.column * BN, policy);
-            if (!Q8) tma_load_2d(sx + s * L::X_STAGE + L::BOX, &tmX, &full[s], col + 64, item.column * BN, policy);
-          }
-        }
+        ask_w(s);
+        ask_x(s);
         __syncwarp();
       }
       meet(item);
@@ -312,11 +319,8 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
         for (int g = 0; g < PER; ++g) {
           const int e = it * PER + g;
-          const Wait room(&d_empty[e & 1], (e >> 1) ^ 1);
-          if (g == 0)
-            ok = all(wait_all(abort_flag, a.err, Wait(&full[s], ph), Wait(&a_full[it & 1], it >> 1), room));
-          else
-            ok = ok && all(wait_all(abort_flag, a.err, room));
+          if (g == 0) ok = wait(a_full + 8 * (it & 1), it >> 1);  // x has come too: who unpacked has seen it
+          if (PER > 1) ok = ok && wait(d_empty + 8 * (e & 1), (e >> 1) ^ 1);
           if (!ok) break;
           tc_fence_after();
           if (leader) {
@@ -326,8 +330,9 @@ __global__ void __launch_bounds__(kThreads, 1)
               for (int k = g * KSTEPS / PER; k < (g + 1) * KSTEPS / PER; ++k)
                 umma_ts<Q8>(td + h * BN, ta + h * A_COLS + 8 * k, bd + (k & 3) * 2 + (k >> 2) * (L::BOX >> 4), IDESC,
                             k > g * KSTEPS / PER ? 1u : 0u);
-            umma_commit(&d_full[e & 1]);
-            if (PER > 1 && g == PER - 1) umma_commit(&a_empty[it & 1]);
+            commit(d_full + 8 * (e & 1));
+            if (PER > 1 && g == PER - 1) commit(a_empty + 8 * (it & 1));
+            if (g == PER - 1) commit(empty + 8 * s);
           }
           __syncwarp();
         }
@@ -342,7 +347,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int offset = min(tile + (lane >> 4), item.count - 1) * L::REC + (lane & 15) * 64;
       for (int kb = 0; kb < nk && ok; ++kb, step()) {
         // The operand's last use: the products of two steps ago.  Groups of 128 columns show it by their sums.
-        ok = all(wait_all(abort_flag, a.err, Wait(&full[s], ph), Wait(PER > 1 ? &a_empty[it & 1] : &d_full[it & 1], (it >> 1) ^ 1)));
+        ok = wait(full + 8 * s, ph) && wait((PER > 1 ? a_empty : d_full) + 8 * (it & 1), (it >> 1) ^ 1);
         if (!ok) break;
         if (tile < item.count) {
           const uint8_t* row = sw + s * at.w_stage() + offset;
@@ -390,8 +395,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         __syncwarp();
         if (lane == 0) {
-          mbar_arrive(&a_full[it & 1]);
-          mbar_arrive(&empty[s]);
+          arrive(a_full + 8 * (it & 1));
+          arrive(empty + 8 * s);
         }
       }
       meet(item);
@@ -400,31 +405,33 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int h = (warp - 12) >> 2, q = warp & 3;
     const int tile = h * 8 + q * 2 + (lane >> 4);  // of the item
     const uint32_t td = tmem + (static_cast<uint32_t>(q * 32) << 16) + 4 * A_COLS + h * BN;
+    if (PER == 1 && lane == 0) arrive(a_full), arrive(a_full + 8);  // nothing to read yet
     for (int n = 0; n < mine; ++n) {
       const Item item(a, unit + n * units);
       const bool some = h * 8 + q * 2 < item.count;
-      const int offset = min(tile, item.count - 1) * L::REC + kW4CodeBytes + (lane & 15) * PER * 4;
-      F2 acc[BN / 2];
+      // The rows' scales come straight from memory, a step ahead: no wait for the ring.
+      const int at_tile = item.tile + min(tile, item.count - 1);
+      const uint8_t* src = a.records + w4_record(at_tile, block0, a.tiles, a.blocks) * L::REC + kW4CodeBytes + (lane & 15) * PER * 4;
+      const int64_t apart = static_cast<int64_t>(min(8, a.tiles - (at_tile & ~7))) * L::REC;
+      float2 acc[BN / 2];
 #pragma unroll
-      for (int i = 0; i < BN / 2; ++i) acc[i] = F2{0.0f, 0.0f};
+      for (int i = 0; i < BN / 2; ++i) acc[i] = make_float2(0.0f, 0.0f);
+      uint32_t pair[PER], next[PER];
+      load_words<PER>(next, src);
       for (int kb = 0; kb < nk && ok; ++kb, step()) {
-        float scale[PER];
+#pragma unroll
+        for (int g = 0; g < PER; ++g) pair[g] = next[g];
+        src += apart;
+        if (kb + 1 < nk) load_words<PER>(next, src);
 #pragma unroll
         for (int g = 0; g < PER; ++g) {
           const int e = it * PER + g;
-          const Wait made(&d_full[e & 1], e >> 1);
-          if (g == 0) {
-            ok = all(wait_all(abort_flag, a.err, Wait(&full[s], ph), made));
-            const uint32_t* pairs = reinterpret_cast<const uint32_t*>(sw + s * at.w_stage() + offset);
-#pragma unroll
-            for (int i = 0; i < PER; ++i) scale[i] = __uint_as_float(pairs[i] << 16);
-          } else {
-            ok = ok && all(wait_all(abort_flag, a.err, made));
-          }
+          ok = ok && wait(d_full + 8 * (e & 1), e >> 1);
           if (!ok) break;
           tc_fence_after();
           if (some) {
-            const F2 s2 = {scale[g], scale[g]};
+            const float scale = __uint_as_float(pair[g] << 16);
+            const float2 s2 = make_float2(scale, scale);
 #pragma unroll
             for (int c0 = 0; c0 < BN; c0 += 16) {
               uint32_t d[16];
@@ -432,15 +439,12 @@ __global__ void __launch_bounds__(kThreads, 1)
               tmem_ld_wait();
 #pragma unroll
               for (int i = 0; i < 16; i += 2)
-                acc[(c0 + i) / 2] = fma2(s2, sums_of<Q8>(d[i], d[i + 1]), acc[(c0 + i) / 2]);
+                acc[(c0 + i) / 2] = __ffma2_rn(s2, sums_of<Q8>(d[i], d[i + 1]), acc[(c0 + i) / 2]);
             }
           }
           tc_fence_before();
           __syncwarp();
-          if (lane == 0) {
-            mbar_arrive(&d_empty[e & 1]);
-            if (g == PER - 1) mbar_arrive(&empty[s]);  // the products have ended too: x is free
-          }
+          if (lane == 0) arrive((PER > 1 ? d_empty : a_full) + 8 * (e & 1));
         }
       }
       const int row0 = item.column * BN, rows = min(BN, a.rows - row0);
@@ -478,8 +482,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     umma_commit(drain);
     mbar_wait(drain, 0, nullptr, a.err);
   }
-  if ((warp == 0 || warp == 2) && lane == 0) {
-    for (int i = it > S ? it - S : 0; i < it; ++i) mbar_wait(&full[i % S], i / S & 1, nullptr, a.err);
+  if (warp == 0 && lane == 0) {
+    for (int i = it > S ? it - S : 0; i < it; ++i) mbar_wait(&full_at[i % S], i / S & 1, nullptr, a.err);
   }
   tc_fence_before();
   __syncthreads();
