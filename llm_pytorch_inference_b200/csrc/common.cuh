@@ -97,26 +97,6 @@ __device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, volati
   return false;
 }
 
-// The same for waits that end soon and follow one another, where the clock's first reading (some hundreds of cycles)
-// would be most of the wait: it is read from the 64th poll on.
-__device__ __forceinline__ bool mbar_wait_soon(uint64_t* bar, uint32_t parity, volatile int* abort_flag,
-                                               unsigned* err) {
-  const uint32_t addr = smem_u32(bar);
-  unsigned long long t0 = 0;
-  for (unsigned polls = 1; polls < kWaitMaxPolls; ++polls) {
-    if (mbar_try_wait(addr, parity)) return true;
-    if ((polls & 63u) == 0) {
-      if (abort_flag != nullptr && *abort_flag) return false;
-      const unsigned long long now = globaltimer_ns();
-      if (t0 == 0) t0 = now;
-      if (now - t0 > kWaitLimitNs) break;
-    }
-  }
-  report(err, kDevWaitTimeout);
-  if (abort_flag != nullptr) *abort_flag = 1;
-  return false;
-}
-
 // ------------------------------------------------------------------ TMA
 __device__ __forceinline__ uint64_t l2_policy_evict_first() {
   uint64_t p;
@@ -334,6 +314,29 @@ __device__ __forceinline__ float dsmem_ld_f32(const float* p, uint32_t rank) {
   float v;
   asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(remote) : "memory");
   return v;
+}
+
+// The sum over the first `blocks` CTAs of this cluster, in their order, of four floats at the offset of `p` (16-byte
+// aligned).  All loads are under way before the first is added.
+__device__ __forceinline__ float4 dsmem_sum4(const float* p, int blocks) {
+  const uint32_t here = smem_u32(p);
+  float4 v[8];
+#pragma unroll
+  for (int b = 0; b < 8; ++b) {
+    if (b < blocks) {
+      uint32_t there;
+      asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(there) : "r"(here), "r"(b));
+      asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+                   : "=f"(v[b].x), "=f"(v[b].y), "=f"(v[b].z), "=f"(v[b].w)
+                   : "r"(there)
+                   : "memory");
+    }
+  }
+  float4 sum = v[0];
+#pragma unroll
+  for (int b = 1; b < 8; ++b)
+    if (b < blocks) sum.x += v[b].x, sum.y += v[b].y, sum.z += v[b].z, sum.w += v[b].w;
+  return sum;
 }
 
 // ------------------------------------------------------------------ numerics

@@ -179,7 +179,7 @@ struct Item {
 
 template <bool Q8, int GROUP, int BN>
 __global__ void __launch_bounds__(kThreads, 1)
-    w4_gemm_kernel(const __grid_constant__ CUtensorMap tmX, const GemmW4Args a) {
+    w4_gemm_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ GemmW4Args a) {
   using L = Layout<Q8, GROUP, BN>;
   constexpr int PER = L::PER;
   constexpr int KSTEPS = Q8 ? 4 : 8;           // steps of 32 bytes of x in 128 columns
@@ -188,7 +188,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   constexpr uint32_t TMEM_COLS = 512;          // a power of two above 4 operands and 4 accumulators
   static_assert(4 * A_COLS + 4 * BN <= 512, "TMEM");
   extern __shared__ uint8_t smem_raw[];
-  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* smem = smem_raw + (-smem_u32(smem_raw) & 1023u);  // an offset: a cast address would be read as a generic one
   uint64_t* full_at = reinterpret_cast<uint64_t*>(smem);  // [stages] a ring's place filled
   uint64_t* drain = full_at + 2 * kMaxStages + 8;
   const uint32_t full = smem_u32(smem), empty = full + 8 * kMaxStages;  // [stages] and read
@@ -247,22 +247,6 @@ __global__ void __launch_bounds__(kThreads, 1)
     ++it;
     if (++s == S) s = 0, ph ^= 1;
   };
-  // A cluster's blocks add their sums of an item up.  They have the same items, so they meet as often, in every role.
-  auto meet = [&](const Item& item) {
-    if (c == 1) return;
-    __syncwarp();
-    cluster_sync();
-    const int row0 = item.column * BN, rows = min(BN, a.rows - row0), width = item.count * kW4Rows;
-    for (int i = rank * kThreads + static_cast<int>(threadIdx.x); i < rows * width; i += c * kThreads) {
-      const int m = i / width, r = i - m * width, col = item.tile * kW4Rows + r;
-      if (col >= a.n) continue;
-      float v = 0.0f;
-      for (int p = 0; p < c; ++p) v += dsmem_ld_f32(part + m * (a.chunk * kW4Rows) + r, p);
-      if (Q8) v *= __ldg(a.a + row0 + m);
-      a.y[(row0 + m) * a.ldy + col] = __float2bfloat16_rn(v);
-    }
-    cluster_sync();  // everybody has read: the sums may change, or their block end
-  };
   auto wait = [&](uint32_t bar, uint32_t parity) { return warp_wait(bar, parity, abort_flag, a.err); };
   if (warp == 0) {
     // Lanes 0 - 2 each ask for a run of records that lie together (up to three), lanes 3 and 4 for a box of x.
@@ -307,7 +291,6 @@ __global__ void __launch_bounds__(kThreads, 1)
         ask_x(s);
         __syncwarp();
       }
-      meet(item);
     }
   } else if (warp == 1) {
     // The whole warp runs the loops, so that addresses and descriptors stay in uniform registers; one thread issues.
@@ -337,7 +320,6 @@ __global__ void __launch_bounds__(kThreads, 1)
           __syncwarp();
         }
       }
-      meet(Item(a, unit + n * units));
     }
   } else if (warp >= 4 && warp < 12 && (warp - 4) >> 2 < halves) {
     const int h = (warp - 4) >> 2, q = warp & 3, tile = h * 8 + q * 2;  // a warp's two tiles
@@ -399,7 +381,6 @@ __global__ void __launch_bounds__(kThreads, 1)
           arrive(empty + 8 * s);
         }
       }
-      meet(item);
     }
   } else if (warp >= 12 && (warp - 12) >> 2 < halves) {
     const int h = (warp - 12) >> 2, q = warp & 3;
@@ -471,12 +452,29 @@ __global__ void __launch_bounds__(kThreads, 1)
           y += ldy;
         }
       }
-      meet(item);
     }
-  } else {
-    for (int n = 0; n < mine; ++n) meet(Item(a, unit + n * units));
   }
 
+  if (c > 1) {
+    // A cluster has one item at most, so its blocks meet once: each adds up a share of the sums.
+    __syncwarp();
+    cluster_sync();
+    if (mine > 0) {
+      const Item item(a, unit);
+      const int row0 = item.column * BN, rows = min(BN, a.rows - row0), fours = item.count * kW4Rows / 4;
+      for (int i = rank * kThreads + static_cast<int>(threadIdx.x); i < rows * fours; i += c * kThreads) {
+        const int m = i / fours, r = 4 * (i - m * fours), col = item.tile * kW4Rows + r;
+        const float4 v = dsmem_sum4(part + m * (a.chunk * kW4Rows) + r, c);
+        const float scale = Q8 ? __ldg(a.a + row0 + m) : 1.0f;
+        const float y4[4] = {v.x * scale, v.y * scale, v.z * scale, v.w * scale};
+        __nv_bfloat16* y = a.y + (row0 + m) * a.ldy + col;
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          if (col + k < a.n) y[k] = __float2bfloat16_rn(y4[k]);
+      }
+    }
+    cluster_sync();  // everybody has read: a block may end
+  }
   // Every product has ended before TMEM is given back, and every copy before the block ends.
   if (warp == 1 && elect_one()) {
     umma_commit(drain);
@@ -507,16 +505,22 @@ int run(const char* name, const W4LinearCall& call, cudaStream_t stream) {
   a.blocks = (call.k + kW4Cols - 1) / kW4Cols;
   a.columns = (call.rows + BN - 1) / BN;
   a.err = device_status_ptr();
-  // Tiles of an item and blocks of a cluster: the fewest bytes through an SM's port (records and x, as often as they
-  // are read), with what a cluster's meeting costs.
+  // Tiles of an item and blocks of a cluster, by what a step of 128 columns takes (in us: 0.65 with one half, 1.0 with
+  // two, whatever their tiles; a group more 0.22 or 0.25) and what an item does besides (0.5; in a cluster 6).
+  // Of what comes out alike the smallest items.
+  static std::atomic<int> clusters[kMaxCluster + 1] = {};
+  auto units_of = [&](int c) {
+    return c == 1 ? sms : clusters_at_once(clusters[c], kernel, c, kThreads, kMostSmem);
+  };
   double least = 0;
   for (int c = 1; c <= kMaxCluster && c <= a.blocks; ++c) {
-    const int units = sms / c;
+    const int units = units_of(c);
     for (int chunk = 1; chunk <= kMaxTiles && chunk <= a.tiles; ++chunk) {
       const int64_t items = static_cast<int64_t>((a.tiles + chunk - 1) / chunk) * a.columns;
+      if (c > 1 && items > units) continue;  // a cluster meets once
       const double waves = static_cast<double>((items + units - 1) / units);
-      const double cost = waves * ((a.blocks + c - 1) / c * static_cast<double>(chunk * L::REC + L::X_STAGE) +
-                                   (c > 1 ? 60000.0 : 20000.0));
+      const double step = chunk > 8 ? 0.75 + 0.25 * L::PER : 0.43 + 0.22 * L::PER;
+      const double cost = waves * ((a.blocks + c - 1) / c * step + (c > 1 ? 6.0 : 0.5));
       if (a.chunk == 0 || cost < least) least = cost, a.cluster = c, a.chunk = chunk;
     }
   }
@@ -528,7 +532,7 @@ int run(const char* name, const W4LinearCall& call, cudaStream_t stream) {
   // first for the second.
   const size_t smem = at.bytes() > 120 * 1024 ? at.bytes() : 120 * 1024;
   const int64_t items = static_cast<int64_t>(a.chunks) * a.columns;
-  const int units = items < sms / a.cluster ? static_cast<int>(items) : sms / a.cluster;
+  const int units = items < units_of(a.cluster) ? static_cast<int>(items) : units_of(a.cluster);
 
   CUtensorMap tm;
   const uint64_t dims[2] = {static_cast<uint64_t>(call.k), static_cast<uint64_t>(call.rows)};

@@ -308,7 +308,7 @@ __global__ void __launch_bounds__(kThreads, 1) w4_linear_kernel(const LinearArgs
 #pragma unroll
           for (int q = 0; q < 4; ++q) acc[s][nt][q] = 0.0f;
       for (int b = kw; b < blocks; b += split) {
-        mbar_wait_soon(&bars[stage], phase, abort_flag, a.err);
+        mbar_wait(&bars[stage], phase, abort_flag, a.err);
         compute<GROUP, P, NT>(ring + stage * 2 * L::REC, sx, info, b, lane, acc);
         __syncwarp();  // every lane has read: the next copy may come
         if (lane == 0) ask();
@@ -347,22 +347,22 @@ __global__ void __launch_bounds__(kThreads, 1) w4_linear_kernel(const LinearArgs
     }
     if (c > 1) {
       cluster_sync();
-      const int rows = min(L::ROWS, a.rows - row0), n = (j1 - j0) * rows * 32;
+      const int rows = min(L::ROWS, a.rows - row0), n = (j1 - j0) * rows * 8;
       for (int i = rank * kThreads + tid; i < n; i += c * kThreads) {
-        const int r = i & 31, m = (i >> 5) % rows, j = (i >> 5) / rows;
+        const int r = 4 * (i & 7), m = (i >> 3) % rows, j = (i >> 3) / rows;
         const int row = row0 + m, col = (unit + (j0 + j) * units) * 32 + r;
-        if (col >= a.n) continue;
-        float v = 0.0f;
-        for (int q = 0; q < c; ++q) v += dsmem_ld_f32(part + (j * L::ROWS + m) * kPitch + r, q);
-        if (P == 1) v *= a.a[row];
-        a.y[row * a.ldy + col] = __float2bfloat16_rn(v);
+        const float4 v = dsmem_sum4(part + (j * L::ROWS + m) * kPitch + r, c);
+        const float scale = P == 1 ? a.a[row] : 1.0f, y4[4] = {v.x * scale, v.y * scale, v.z * scale, v.w * scale};
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          if (col + k < a.n) a.y[row * a.ldy + col + k] = __float2bfloat16_rn(y4[k]);
       }
       cluster_sync();  // everybody has read: the sums may change, or their block end
     }
   }
   // Every copy has been waited for, unless a wait gave up: then those under way are, before the block ends.
   if (*abort_flag && lane == 0)
-    for (int s = 0; s < a.stages; ++s) mbar_wait_soon(&bars[s], phase ^ (s < stage ? 0 : 1), nullptr, a.err);
+    for (int s = 0; s < a.stages; ++s) mbar_wait(&bars[s], phase ^ (s < stage ? 0 : 1), nullptr, a.err);
 }
 
 template <int GROUP, int P, int NT>
@@ -374,17 +374,21 @@ int run(const char* name, LinearArgs a, cudaStream_t stream) {
   static std::atomic<uint64_t> done{0};
   MVB_TRY(set_smem_once(done, kernel, kMostSmem, name));
   // The cluster: what its blocks' work takes, in records of a pair of tiles, and what a cluster's meeting costs.
+  static std::atomic<int> clusters[kMaxCluster + 1] = {};
+  auto units_of = [&](int c) {
+    return c == 1 ? sms : clusters_at_once(clusters[c], kernel, c, kThreads, kMostSmem);
+  };
   int best = 0;
   double least = 0;
   for (int c = 1; c <= kMaxCluster; c *= 2) {
     if (L{(a.blocks + c - 1) / c, 2, c > 1}.bytes() > kMostSmem || c > a.blocks) continue;
-    const int units = sms / c;
+    const int units = units_of(c);
     const double cost = double((a.pairs + units - 1) / units) * ((a.blocks + c - 1) / c) + (c > 1 ? 24 : 0);
     if (best == 0 || cost < least) best = c, least = cost;
   }
   MVB_REQUIRE(best > 0, "%s: %d columns", name, a.k);
   a.cluster = best;
-  const int units = a.pairs < sms / best ? a.pairs : sms / best;
+  const int units = a.pairs < units_of(best) ? a.pairs : units_of(best);
   const int blocks = a.blocks / best;
   a.split = 1;
   while (a.split < kWarps && a.split < blocks) a.split *= 2;
