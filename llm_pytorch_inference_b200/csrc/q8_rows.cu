@@ -56,31 +56,50 @@ __device__ __forceinline__ float value_of(float a, float b, float w, float one, 
   return a;
 }
 
-// The codes of one row.  127 y and amax are taken times a power of two where the quotient would leave fp32's range.
+// The codes of one row, eight at a time, each in the low byte of its result.  The product with 127 / amax is off by less
+// than 2e-5; only where one of the eight comes so near a border between two codes are the quotients worked out.  So
+// they are where 127 / amax or 127 y would leave fp32's range, from numbers taken times a power of two.
 struct Coder {
-  float f, amax, inv;
+  float amax, inv;
+  bool edge;
   __device__ __forceinline__ explicit Coder(float top) {
-    f = top > 1.2676506e30f ? 5.4210109e-20f : top < 8.2718061e-25f ? 1.8446744e19f : 1.0f;  // 2^100, 2^-64, 2^-80, 2^64
-    amax = top * f;
-    inv = amax > 0.0f ? 127.0f / amax : 0.0f;
+    edge = top > 1.2676506e30f || top < 8.2718061e-25f;  // 2^100, 2^-80
+    amax = top;
+    inv = edge ? 0.0f : 127.0f / top;
   }
-  // The low byte of the result.  The product with the reciprocal is off by less than 2e-5; only where it comes so near
-  // a border between two codes is the quotient worked out.
-  __device__ __forceinline__ uint32_t of(float y) const {
+  __device__ __forceinline__ void of(const float (&y)[8], uint32_t (&c)[8]) const {
     constexpr float kMagic = 12582912.0f;  // 1.5 * 2^23: the sum's low bits are the nearest whole number
-    const float p = y * f, t = p * inv;
-    float m = t + kMagic;
-    if (fabsf(t - (m - kMagic)) > 0.49998f) m = __fdiv_rn(127.0f * p, amax) + kMagic;
-    return __float_as_uint(m);
+    float far = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 8; i += 2) {
+      const float2 t = __fmul2_rn(make_float2(y[i], y[i + 1]), make_float2(inv, inv));
+      const float2 m = __fadd2_rn(t, make_float2(kMagic, kMagic));
+      const float2 n = __fadd2_rn(m, make_float2(-kMagic, -kMagic));
+      const float2 d = __fadd2_rn(t, make_float2(-n.x, -n.y));
+      far = fmaxf(far, fmaxf(fabsf(d.x), fabsf(d.y)));
+      c[i] = __float_as_uint(m.x);
+      c[i + 1] = __float_as_uint(m.y);
+    }
+    if (far > 0.49998f || edge) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) c[i] = quotient(y[i], amax, edge);
+    }
+  }
+  static __device__ __noinline__ uint32_t quotient(float y, float amax, bool edge) {
+    const float f = !edge ? 1.0f : amax > 1.0f ? 5.4210109e-20f : 1.8446744e19f;  // 2^-64, 2^64
+    return __float_as_uint(amax > 0.0f ? __fdiv_rn(127.0f * (y * f), amax * f) + 12582912.0f : 0.0f);
   }
 };
 __device__ __forceinline__ uint32_t pack4(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
   return __byte_perm(__byte_perm(a, b, 0x0040), __byte_perm(c, d, 0x0040), 0x5410);
 }
 
-__device__ __forceinline__ float abs_max(float m, float y) {  // the larger size by its bits: a NaN is above all
-  return __uint_as_float(max(__float_as_uint(m), __float_as_uint(y) & 0x7fffffffu));
+__device__ __forceinline__ float abs_max(float m, float y) {  // the larger size; NaN where either is
+  float d;
+  asm("{\n\t.reg .f32 a;\n\tabs.f32 a, %2;\n\tmax.NaN.f32 %0, %1, a;\n\t}" : "=f"(d) : "f"(m), "f"(y));
+  return d;
 }
+__device__ __forceinline__ bool is_fine(float top) { return top <= 3.4028235e38f; }  // neither infinite nor NaN
 
 // The block's sum and its largest size, in every thread.
 __device__ __forceinline__ void block_both(float& ss, float& top, float2* red) {
@@ -105,7 +124,7 @@ __device__ __forceinline__ void block_both(float& ss, float& top, float2* red) {
 
 template <int KIND>
 __device__ __forceinline__ float row_scale(const RowArgs& a, float ss, float top) {
-  if (__float_as_uint(top) >= 0x7f800000u) return __uint_as_float(0x7fc00000u);
+  if (!is_fine(top)) return __uint_as_float(0x7fc00000u);
   if (KIND == kNorm || KIND == kAddNorm) return top * (1.0f / sqrtf(ss / static_cast<float>(a.width) + a.eps)) / 127.0f;
   return top / 127.0f;
 }
@@ -167,17 +186,18 @@ __global__ void __launch_bounds__(1024) q8_rows_kernel(const RowArgs a) {
   block_both(ss, top, red);
   const float scale = row_scale<KIND>(a, ss, top);
   if (threadIdx.x == 0) a.scale[row] = scale;
-  const bool fine = __float_as_uint(top) < 0x7f800000u;
-  const Coder code(fine ? top : 0.0f);
+  const bool fine = is_fine(top);
+  const Coder code(top);
   uint2* q = reinterpret_cast<uint2*>(a.q + row * a.width);
 #pragma unroll
   for (int j = 0; j < VPT; ++j) {
     const int v = j * blockDim.x + threadIdx.x;
     if (v < vectors) {
       uint32_t c[8];
-#pragma unroll
-      for (int i = 0; i < 8; ++i) c[i] = fine ? code.of(y[j][i]) : 0u;
-      q[v] = make_uint2(pack4(c[0], c[1], c[2], c[3]), pack4(c[4], c[5], c[6], c[7]));
+      code.of(y[j], c);
+      uint2 bytes = make_uint2(pack4(c[0], c[1], c[2], c[3]), pack4(c[4], c[5], c[6], c[7]));
+      if (!fine) bytes = make_uint2(0, 0);
+      q[v] = bytes;
     }
   }
 }
@@ -202,8 +222,8 @@ __global__ void __launch_bounds__(256) q8_any_kernel(const RowArgs a) {
   }
   block_both(ss, top, red);
   if (threadIdx.x == 0) a.scale[row] = row_scale<KIND>(a, ss, top);
-  const bool fine = __float_as_uint(top) < 0x7f800000u;
-  const Coder code(fine ? top : 0.0f);
+  const bool fine = is_fine(top);
+  const Coder code(top);
   for (int i = threadIdx.x; i < a.width; i += blockDim.x) {
     float y;
     if (KIND == kAddNorm)
@@ -211,32 +231,51 @@ __global__ void __launch_bounds__(256) q8_any_kernel(const RowArgs a) {
     else
       y = value_of<KIND, T>(to_f<T>(pa[i]), KIND >= kAddNorm ? to_f<T>(pb[i]) : 0.0f,
                             KIND == kNorm ? to_f<T>(pw[i]) : 0.0f, a.one, h, ss);
-    a.q[row * a.width + i] = fine ? static_cast<int8_t>(code.of(y) & 0xffu) : int8_t(0);
+    const float one[8] = {y};
+    uint32_t c[8];
+    code.of(one, c);
+    a.q[row * a.width + i] = fine ? static_cast<int8_t>(c[0] & 0xffu) : int8_t(0);
   }
 }
 
+// Codes times scales.  VEC: 8 codes a thread and step, four steps under way; `per` of them make a row.
 template <typename T, bool VEC>
 __global__ void __launch_bounds__(256) dequantise_q8_kernel(T* __restrict__ out, const int8_t* __restrict__ q,
                                                             int64_t q_stride, const float* __restrict__ scale,
                                                             int64_t rows, int width) {
   pdl_launch_dependents();
   pdl_wait();
-  constexpr int N = VEC ? 8 : 1;
-  const int per = width / N;
-  const int64_t n = rows * per, step = static_cast<int64_t>(gridDim.x) * blockDim.x;
-  for (int64_t i = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x; i < n; i += step) {
-    const int64_t row = i / per;
-    const int col = static_cast<int>(i - row * per) * N;
-    const float s = scale[row];
-    if (VEC) {
-      const uint2 c = *reinterpret_cast<const uint2*>(q + row * q_stride + col);
-      const int8_t* e = reinterpret_cast<const int8_t*>(&c);
-      float v[8];
+  constexpr int N = VEC ? 8 : 1, STEPS = VEC ? 4 : 1;
+  const uint32_t per = width / N;
+  const int64_t n = rows * per, all = static_cast<int64_t>(gridDim.x) * blockDim.x;
+  for (int64_t i0 = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x; i0 < n; i0 += STEPS * all) {
+    int64_t row[STEPS];
+    int col[STEPS];
+    float s[STEPS];
+    uint2 c[STEPS];
 #pragma unroll
-      for (int k = 0; k < 8; ++k) v[k] = static_cast<float>(e[k]) * s;
-      store8<T>(out + row * width + col, v);
-    } else {
-      out[row * width + col] = from_f<T>(static_cast<float>(q[row * q_stride + col]) * s);
+    for (int j = 0; j < STEPS; ++j) {
+      const int64_t i = i0 + j * all;
+      if (i >= n) continue;
+      // whole numbers of 32 bits divide at a third of the cost of 64
+      row[j] = i < (int64_t{1} << 32) ? static_cast<uint32_t>(i) / per : i / per;
+      col[j] = static_cast<int>(i - row[j] * per) * N;
+      s[j] = scale[row[j]];
+      if (VEC) c[j] = *reinterpret_cast<const uint2*>(q + row[j] * q_stride + col[j]);
+    }
+#pragma unroll
+    for (int j = 0; j < STEPS; ++j) {
+      if (i0 + j * all >= n) continue;
+      T* o = out + row[j] * width + col[j];
+      if (VEC) {
+        const int8_t* e = reinterpret_cast<const int8_t*>(&c[j]);
+        float v[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) v[k] = static_cast<float>(e[k]) * s[j];
+        store8<T>(o, v);
+      } else {
+        *o = from_f<T>(static_cast<float>(q[row[j] * q_stride + col[j]]) * s[j]);
+      }
     }
   }
 }

@@ -35,6 +35,7 @@ constexpr int kPitch = 36;  // floats between columns of a pair's 32 sums: 4 col
 constexpr int kRound = 16;  // pairs after which the blocks of a cluster add up
 constexpr int kMaxCluster = 8;
 constexpr int kMaxStages = 8;
+constexpr double kPairEnd = 3.0;
 constexpr size_t kMostSmem = 227 * 1024;
 
 struct LinearArgs {
@@ -389,9 +390,15 @@ int run(const char* name, LinearArgs a, cudaStream_t stream) {
   MVB_REQUIRE(best > 0, "%s: %d columns", name, a.k);
   a.cluster = best;
   const int units = a.pairs < units_of(best) ? a.pairs : units_of(best);
-  const int blocks = a.blocks / best;
-  a.split = 1;
-  while (a.split < kWarps && a.split < blocks) a.split *= 2;
+  // The warps that share a pair's columns: in items, what they compute and what a pair's end takes (some 3).
+  const int blocks = (a.blocks + best - 1) / best, mine = (a.pairs + units - 1) / units;
+  double fewest = 0;
+  a.split = 0;
+  for (int split = kWarps; split >= 1; split /= 2) {
+    const int teams = kWarps / split;
+    const double items = ((mine + teams - 1) / teams) * ((blocks + split - 1) / split + kPairEnd);
+    if (a.split == 0 || items < fewest) fewest = items, a.split = split;
+  }
   L at = {(a.blocks + best - 1) / best, kMaxStages, best > 1};
   while (at.bytes() > kMostSmem) --at.stages;
   a.stages = at.stages;

@@ -49,7 +49,12 @@ __device__ __forceinline__ uint32_t word_of(const uint32_t (&u)[8]) {
   return w;
 }
 
-// max of two pairs of bf16, NaN where either is
+// Larger and smaller numbers of two pairs of bf16, NaN where either is.
+__device__ __forceinline__ uint32_t min2(uint32_t a, uint32_t b) {
+  uint32_t d;
+  asm("min.NaN.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+  return d;
+}
 __device__ __forceinline__ uint32_t max2(uint32_t a, uint32_t b) {
   uint32_t d;
   asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
@@ -57,6 +62,13 @@ __device__ __forceinline__ uint32_t max2(uint32_t a, uint32_t b) {
 }
 __device__ __forceinline__ float low_bf16(uint32_t v) { return __uint_as_float(v << 16); }
 __device__ __forceinline__ float high_bf16(uint32_t v) { return __uint_as_float(v & 0xffff0000u); }
+
+// x / 15, rounded once: the product with 1/15 and what it leaves over.
+__device__ __forceinline__ float fifteenth(float x) {
+  const float q = x * (1.0f / 15.0f);
+  const float left = fmaf(-15.0f, q, x);
+  return fabsf(x) > 1.0e-30f && fabsf(x) < 1.0e38f ? fmaf(left, 1.0f / 15.0f, q) : __fdiv_rn(x, 15.0f);
+}
 
 template <int GROUP>
 __global__ void __launch_bounds__(kThreads) quantise_w4_kernel(uint8_t* __restrict__ records,
@@ -82,43 +94,48 @@ __global__ void __launch_bounds__(kThreads) quantise_w4_kernel(uint8_t* __restri
     const int row = 2 * i + half;
     const uint32_t v[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
     // high: the largest, low: the largest of the negated
-    uint32_t up = max2(max2(v[0], v[1]), max2(v[2], v[3]));
-    uint32_t down = max2(max2(v[0] ^ 0x80008000u, v[1] ^ 0x80008000u), max2(v[2] ^ 0x80008000u, v[3] ^ 0x80008000u));
+    const uint32_t up = max2(max2(v[0], v[1]), max2(v[2], v[3]));
+    const uint32_t down = min2(min2(v[0], v[1]), min2(v[2], v[3])) ^ 0x80008000u;
     uint32_t both = max2(__byte_perm(down, up, 0x5410), __byte_perm(down, up, 0x7632));
     both = max2(both, 0u);
 #pragma unroll
     for (int o = LANES / 2; o > 0; o >>= 1) both = max2(both, __shfl_xor_sync(0xffffffffu, both, o));
     const float low = low_bf16(both), high = high_bf16(both);  // -lo and hi
-    const __nv_bfloat16 sb = __float2bfloat16_rn(__fdiv_rn(high + low, 15.0f));
+    const __nv_bfloat16 sb = __float2bfloat16_rn(fifteenth(high + low));
     const float scale = __bfloat162float(sb);
-    uint32_t u[8], zero = 0;
+    uint32_t word = 0, zero = 0;
     if (scale > 0.0f && scale < __uint_as_float(0x7f800000u)) {
-      const float z = fminf(rintf(__fdiv_rn(low, scale)), 15.0f);
-      zero = static_cast<uint32_t>(z);
-      const float inv = 1.0f / scale;
       // Quotients of two bf16 numbers below 16 either fall on a border between codes or are 1e-3 away from it, and
-      // the product with the reciprocal is off by 2e-6: rounded to a multiple of 2^-13, it falls on the right
-      // side, or on the border.  (A reciprocal of a scale below 2^-126 would overflow: the quotient itself.)
+      // the product with the reciprocal is off by 4e-6: rounded to a multiple of 2^-13 (the sum with 1536), it falls on the
+      // right side, or on the border.  The whole number then is the low bits of the sum with 1.5 * 2^23.  None is below
+      // -zero, since rounding is monotonic and odd; the most is cut.  (A reciprocal of a scale below 2^-126 would
+      // overflow: the quotient itself.)
+      constexpr float kMagic = 12582912.0f;
       const bool tiny = scale < 1.1754944e-38f;
+      float inv;
+      asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inv) : "f"(scale));
+      const float z = rintf((tiny ? __fdiv_rn(low, scale) : low * inv) + 1536.0f - 1536.0f);
+      zero = static_cast<uint32_t>(z);
+      const float most = kMagic + 15.0f - z;
+      uint32_t u[8];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const float y = e & 1 ? high_bf16(v[e >> 1]) : low_bf16(v[e >> 1]);
-        float t = tiny ? __fdiv_rn(y, scale) : y * inv;
-        t = (t + 1536.0f) - 1536.0f;
-        u[e] = static_cast<uint32_t>(fminf(fmaxf(rintf(t) + z, 0.0f), 15.0f));
+      for (int e = 0; e < 8; e += 2) {
+        float2 t = make_float2(low_bf16(v[e >> 1]), high_bf16(v[e >> 1]));
+        t = tiny ? make_float2(__fdiv_rn(t.x, scale), __fdiv_rn(t.y, scale)) : __fmul2_rn(t, make_float2(inv, inv));
+        t = __fadd2_rn(__fadd2_rn(t, make_float2(1536.0f, 1536.0f)), make_float2(-1536.0f, -1536.0f));
+        t = __fadd2_rn(t, make_float2(kMagic, kMagic));
+        t = __fadd2_rn(make_float2(fminf(t.x, most), fminf(t.y, most)), make_float2(z, z));
+        u[e] = __float_as_uint(t.x);
+        u[e + 1] = __float_as_uint(t.y);
       }
-    } else {
-#pragma unroll
-      for (int e = 0; e < 8; ++e) u[e] = 0;
+      // a code is its number's low byte: those of columns 0 4 1 5 below, 2 6 3 7 above
+      const uint32_t below = __byte_perm(__byte_perm(u[0], u[4], 0x0040), __byte_perm(u[1], u[5], 0x0040), 0x5410);
+      const uint32_t above = __byte_perm(__byte_perm(u[2], u[6], 0x0040), __byte_perm(u[3], u[7], 0x0040), 0x5410);
+      word = below | above << 4;
     }
-    if (at.tile * kW4Rows + row >= s.n || col >= s.k) {
-#pragma unroll
-      for (int e = 0; e < 8; ++e) u[e] = 0;
-    }
-    *reinterpret_cast<uint32_t*>(rec + row * 64 + w4_place(part & 3, row) * 16 + (part >> 2) * 4) = word_of(u);
+    const bool some = at.tile * kW4Rows + row < s.n && col < s.k;  // else it stays zero
+    *reinterpret_cast<uint32_t*>(rec + row * 64 + w4_place(part & 3, row) * 16 + (part >> 2) * 4) = some ? word : 0u;
     if (part % LANES == 0) {
-      // a group without a column stays zero
-      const bool some = at.tile * kW4Rows + row < s.n && col < s.k;
       const uint32_t pair = __bfloat16_as_ushort(sb) | (0x4300u | zero) << 16;
       *reinterpret_cast<uint32_t*>(rec + kW4CodeBytes + (row * PER + part / LANES) * 4) = some ? pair : 0u;
     }
