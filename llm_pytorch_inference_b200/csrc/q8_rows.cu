@@ -10,6 +10,10 @@
 // of squares and the maximum are reduced together.  For bf16 p is exact in 32 bits, and so is 127 p: the codes
 // are then the correctly rounded ones.
 //
+// Bound by memory for many rows (2 bytes in and 1 out an element, 4 and 3 with the addition, 4 and 1 gated), by the way
+// through a row for few.  What an SM can do in that time is some 20 instructions an element, so pairs of 16-bit
+// numbers are taken apart and made two at a time, and so are products and sums.
+//
 // A row with an infinity or a NaN (in y, before r) gets the scale NaN: it reads back as NaN, and so does a product with it.
 // A row of zeros gets the scale 0.
 #include <climits>
@@ -32,6 +36,7 @@ struct RowArgs {
   void* sum;        // residual + x
   int64_t sum_stride;
   const void* w;
+  int64_t rows;
   int width;
   float eps;
   float one;        // 1 for the (1 + w) norm, else 0
@@ -57,15 +62,20 @@ __device__ __forceinline__ float value_of(float a, float b, float w, float one, 
 }
 
 // The codes of one row, eight at a time, each in the low byte of its result.  The product with 127 / amax is off by less
-// than 2e-5; only where one of the eight comes so near a border between two codes are the quotients worked out.  So
-// they are where 127 / amax or 127 y would leave fp32's range, from numbers taken times a power of two.
+// than 2e-5 of a code.  Where one of the eight comes so near a border between two (or lies on it, which 8-bit numbers
+// often do), 127 y - code amax, exact in one multiply-add for bf16, tells on which side each is.  In rows below 2^-80 or
+// above 2^100, where 127 / amax or 127 y would leave fp32's range, the quotients are worked out, from numbers taken
+// times a power of two.
 struct Coder {
   float amax, inv;
   bool edge;
-  __device__ __forceinline__ explicit Coder(float top) {
-    edge = top > 1.2676506e30f || top < 8.2718061e-25f;  // 2^100, 2^-80
-    amax = top;
+  __device__ __forceinline__ explicit Coder(float top) : amax(top), edge(top > 1.2676506e30f || top < 8.2718061e-25f) {
     inv = edge ? 0.0f : 127.0f / top;
+  }
+  // not inlined: it is hardly ever called
+  static __device__ __noinline__ uint32_t quotient(float y, float amax, bool edge) {
+    const float f = !edge ? 1.0f : amax > 1.0f ? 5.4210109e-20f : 1.8446744e19f;  // 2^-64, 2^64
+    return __float_as_uint(amax > 0.0f ? __fdiv_rn(127.0f * (y * f), amax * f) + 12582912.0f : 0.0f);
   }
   __device__ __forceinline__ void of(const float (&y)[8], uint32_t (&c)[8]) const {
     constexpr float kMagic = 12582912.0f;  // 1.5 * 2^23: the sum's low bits are the nearest whole number
@@ -75,19 +85,22 @@ struct Coder {
       const float2 t = __fmul2_rn(make_float2(y[i], y[i + 1]), make_float2(inv, inv));
       const float2 m = __fadd2_rn(t, make_float2(kMagic, kMagic));
       const float2 n = __fadd2_rn(m, make_float2(-kMagic, -kMagic));
-      const float2 d = __fadd2_rn(t, make_float2(-n.x, -n.y));
-      far = fmaxf(far, fmaxf(fabsf(d.x), fabsf(d.y)));
+      const float2 d = __ffma2_rn(n, make_float2(-1.0f, -1.0f), t);
+      far = fmaxf(fmaxf(far, fabsf(d.x)), fabsf(d.y));
       c[i] = __float_as_uint(m.x);
       c[i + 1] = __float_as_uint(m.y);
     }
-    if (far > 0.49998f || edge) {
+    if (far > 0.49998f) {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) c[i] = quotient(y[i], amax, edge);
+      for (int i = 0; i < 8; ++i) {
+        const float left = fmaf(kMagic - __uint_as_float(c[i]), amax, 127.0f * y[i]), twice = 2.0f * fabsf(left);
+        if (twice > amax || (twice == amax && (c[i] & 1u))) c[i] += left > 0.0f ? 1u : ~0u;
+      }
     }
-  }
-  static __device__ __noinline__ uint32_t quotient(float y, float amax, bool edge) {
-    const float f = !edge ? 1.0f : amax > 1.0f ? 5.4210109e-20f : 1.8446744e19f;  // 2^-64, 2^64
-    return __float_as_uint(amax > 0.0f ? __fdiv_rn(127.0f * (y * f), amax * f) + 12582912.0f : 0.0f);
+    if (edge) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) c[i] = quotient(y[i], amax, true);
+    }
   }
 };
 __device__ __forceinline__ uint32_t pack4(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
@@ -101,8 +114,8 @@ __device__ __forceinline__ float abs_max(float m, float y) {  // the larger size
 }
 __device__ __forceinline__ bool is_fine(float top) { return top <= 3.4028235e38f; }  // neither infinite nor NaN
 
-// The block's sum and its largest size, in every thread.
-__device__ __forceinline__ void block_both(float& ss, float& top, float2* red) {
+// The row's sum and its largest size, in every thread of its blockDim.x.
+__device__ __forceinline__ void row_both(float& ss, float& top, float2* red) {
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) {
     ss += __shfl_xor_sync(0xffffffffu, ss, o);
@@ -129,61 +142,96 @@ __device__ __forceinline__ float row_scale(const RowArgs& a, float ss, float top
   return top / 127.0f;
 }
 
+// Eight elements, taken apart and rounded in pairs.
+__device__ __forceinline__ void load8(const float* p, float (&v)[8]) {
+  const float4 x = reinterpret_cast<const float4*>(p)[0], y = reinterpret_cast<const float4*>(p)[1];
+  v[0] = x.x, v[1] = x.y, v[2] = x.z, v[3] = x.w, v[4] = y.x, v[5] = y.y, v[6] = y.z, v[7] = y.w;
+}
+__device__ __forceinline__ void apart(const uint4& x, float (&v)[8], __nv_bfloat16) {
+  const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) v[2 * i] = __uint_as_float(w[i] << 16), v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+}
+__device__ __forceinline__ void apart(const uint4& x, float (&v)[8], __half) {
+  const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+    v[2 * i] = f.x, v[2 * i + 1] = f.y;
+  }
+}
 template <typename T>
 __device__ __forceinline__ void load8(const T* p, float (&v)[8]) {
-  if (sizeof(T) == 4) {
-    const float4 x = reinterpret_cast<const float4*>(p)[0], y = reinterpret_cast<const float4*>(p)[1];
-    v[0] = x.x, v[1] = x.y, v[2] = x.z, v[3] = x.w, v[4] = y.x, v[5] = y.y, v[6] = y.z, v[7] = y.w;
-  } else {
-    const uint4 x = *reinterpret_cast<const uint4*>(p);
-    const T* e = reinterpret_cast<const T*>(&x);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = to_f<T>(e[i]);
-  }
+  apart(*reinterpret_cast<const uint4*>(p), v, T());
+}
+__device__ __forceinline__ uint32_t round2(float a, float b, __nv_bfloat16) {
+  const __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
+__device__ __forceinline__ uint32_t round2(float a, float b, __half) {
+  const __half2 v = __floats2half2_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
+// Stores v rounded to T, and leaves in v what was stored.
+__device__ __forceinline__ void store8(float* p, float (&v)[8]) {
+  reinterpret_cast<float4*>(p)[0] = make_float4(v[0], v[1], v[2], v[3]);
+  reinterpret_cast<float4*>(p)[1] = make_float4(v[4], v[5], v[6], v[7]);
 }
 template <typename T>
-__device__ __forceinline__ void store8(T* p, const float (&v)[8]) {
-  if (sizeof(T) == 4) {
-    reinterpret_cast<float4*>(p)[0] = make_float4(v[0], v[1], v[2], v[3]);
-    reinterpret_cast<float4*>(p)[1] = make_float4(v[4], v[5], v[6], v[7]);
-  } else {
-    uint4 x;
-    T* e = reinterpret_cast<T*>(&x);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) e[i] = from_f<T>(v[i]);
-    *reinterpret_cast<uint4*>(p) = x;
-  }
+__device__ __forceinline__ void store8(T* p, float (&v)[8]) {
+  const uint4 x = make_uint4(round2(v[0], v[1], T()), round2(v[2], v[3], T()), round2(v[4], v[5], T()), round2(v[6], v[7], T()));
+  *reinterpret_cast<uint4*>(p) = x;
+  apart(x, v, T());
 }
 
-// A block per row, which stays in registers: vector j of a thread holds elements 8 (j blockDim + thread) .. + 7.
+// A row stays in registers: vector j of a thread holds elements 8 (j blockDim.x + thread) .. + 7.  A block has one row,
+// or (32 threads a row) several.
 template <int KIND, typename T, int VPT>
 __global__ void __launch_bounds__(1024) q8_rows_kernel(const RowArgs a) {
+  constexpr bool NORM = KIND == kNorm || KIND == kAddNorm;
   __shared__ float2 red[32];
   pdl_launch_dependents();
   pdl_wait();
-  const int64_t row = blockIdx.x;
+  const int64_t row = static_cast<int64_t>(blockIdx.x) * blockDim.y + threadIdx.y;
+  if (row >= a.rows) return;  // a warp has a row, or the block one
   const T* pa = static_cast<const T*>(a.a) + row * a.a_stride;
   const T* pb = static_cast<const T*>(a.b) + row * a.b_stride;
   const int vectors = a.width >> 3;
   float y[VPT][8];
-  float ss = 0.0f, top = 0.0f;
+  float2 squares = make_float2(0.0f, 0.0f);
+  float top = 0.0f;
 #pragma unroll
   for (int j = 0; j < VPT; ++j) {
     const int v = j * blockDim.x + threadIdx.x;
     if (v < vectors) {
-      float x[8], z[8], w[8], h[8];
-      load8<T>(pa + 8 * v, x);
-      if (KIND >= kAddNorm) load8<T>(pb + 8 * v, z);
-      if (KIND == kNorm || KIND == kAddNorm) load8<T>(static_cast<const T*>(a.w) + 8 * v, w);
+      float x[8], z[8], w[8];
+      load8(pa + 8 * v, x);
+      if (KIND >= kAddNorm) load8(pb + 8 * v, z);
+      if (NORM) load8(static_cast<const T*>(a.w) + 8 * v, w);
+      if (KIND == kAddNorm) {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        y[j][i] = value_of<KIND, T>(x[i], z[i], w[i], a.one, h[i], ss);
-        top = abs_max(top, y[j][i]);
+        for (int i = 0; i < 8; i += 2) {
+          const float2 h = __fadd2_rn(make_float2(x[i], x[i + 1]), make_float2(z[i], z[i + 1]));
+          x[i] = h.x, x[i + 1] = h.y;
+        }
+        store8(static_cast<T*>(a.sum) + row * a.sum_stride + 8 * v, x);
       }
-      if (KIND == kAddNorm) store8<T>(static_cast<T*>(a.sum) + row * a.sum_stride + 8 * v, h);
+#pragma unroll
+      for (int i = 0; i < 8; i += 2) {
+        float2 u = make_float2(x[i], x[i + 1]);
+        if (NORM) {
+          squares = __ffma2_rn(u, u, squares);
+          u = __fmul2_rn(u, __fadd2_rn(make_float2(w[i], w[i + 1]), make_float2(a.one, a.one)));
+        }
+        if (KIND == kSilu || KIND == kGelu)
+          u = __fmul2_rn(make_float2(act_of<KIND>(u.x), act_of<KIND>(u.y)), make_float2(z[i], z[i + 1]));
+        top = abs_max(abs_max(top, u.x), u.y);
+        y[j][i] = u.x, y[j][i + 1] = u.y;
+      }
     }
   }
-  block_both(ss, top, red);
+  float ss = squares.x + squares.y;
+  row_both(ss, top, red);
   const float scale = row_scale<KIND>(a, ss, top);
   if (threadIdx.x == 0) a.scale[row] = scale;
   const bool fine = is_fine(top);
@@ -220,7 +268,7 @@ __global__ void __launch_bounds__(256) q8_any_kernel(const RowArgs a) {
     if (KIND == kAddNorm) sum[i] = from_f<T>(h);
     top = abs_max(top, y);
   }
-  block_both(ss, top, red);
+  row_both(ss, top, red);
   if (threadIdx.x == 0) a.scale[row] = row_scale<KIND>(a, ss, top);
   const bool fine = is_fine(top);
   const Coder code(top);
@@ -231,10 +279,7 @@ __global__ void __launch_bounds__(256) q8_any_kernel(const RowArgs a) {
     else
       y = value_of<KIND, T>(to_f<T>(pa[i]), KIND >= kAddNorm ? to_f<T>(pb[i]) : 0.0f,
                             KIND == kNorm ? to_f<T>(pw[i]) : 0.0f, a.one, h, ss);
-    const float one[8] = {y};
-    uint32_t c[8];
-    code.of(one, c);
-    a.q[row * a.width + i] = fine ? static_cast<int8_t>(c[0] & 0xffu) : int8_t(0);
+    a.q[row * a.width + i] = fine ? static_cast<int8_t>(Coder::quotient(y, code.amax, code.edge) & 0xffu) : int8_t(0);
   }
 }
 
@@ -272,7 +317,7 @@ __global__ void __launch_bounds__(256) dequantise_q8_kernel(T* __restrict__ out,
         float v[8];
 #pragma unroll
         for (int k = 0; k < 8; ++k) v[k] = static_cast<float>(e[k]) * s[j];
-        store8<T>(o, v);
+        store8(o, v);
       } else {
         *o = from_f<T>(static_cast<float>(q[row[j] * q_stride + col[j]]) * s[j]);
       }
@@ -287,14 +332,15 @@ int run_rows(const char* name, const RowArgs& a, int64_t rows, cudaStream_t stre
   const bool vec = a.width % 8 == 0 && aligned(a.q, 8) && whole(a.a, a.a_stride) && whole(a.w, 0) &&
                    (KIND < kAddNorm || whole(a.b, a.b_stride)) && (KIND != kAddNorm || whole(a.sum, a.sum_stride));
   const int vectors = a.width / 8;
-  const dim3 grid(static_cast<unsigned>(rows));
   if (!vec || vectors > 4 * 1024)
-    return launch(name, q8_any_kernel<KIND, T>, grid, dim3(256), 0, stream, a);
-  const int most = rows <= 2 * current_sm_count() ? 1 : 4;  // vectors of a thread
+    return launch(name, q8_any_kernel<KIND, T>, dim3(static_cast<unsigned>(rows)), dim3(256), 0, stream, a);
+  // Few rows: a vector a thread, the shortest way through a row.  Many: four, and rows of up to 1024 elements a warp each.
+  const int most = rows <= 2 * current_sm_count() ? 1 : 4;
   int threads = (vectors + most - 1) / most;
   threads = threads > 1024 ? 1024 : (threads + 31) / 32 * 32;
-  const int per = (vectors + threads - 1) / threads;
-  const dim3 block(static_cast<unsigned>(threads));
+  const int per = (vectors + threads - 1) / threads, together = threads == 32 ? 8 : 1;
+  const dim3 block(static_cast<unsigned>(threads), static_cast<unsigned>(together));
+  const dim3 grid(static_cast<unsigned>((rows + together - 1) / together));
   if (per <= 1) return launch(name, q8_rows_kernel<KIND, T, 1>, grid, block, 0, stream, a);
   if (per <= 2) return launch(name, q8_rows_kernel<KIND, T, 2>, grid, block, 0, stream, a);
   return launch(name, q8_rows_kernel<KIND, T, 4>, grid, block, 0, stream, a);
@@ -330,6 +376,7 @@ extern "C" int mvb_quantise_q8(int8_t* values, float* scales, const void* in, in
   MVB_REQUIRE(values && scales && in, "%s: null pointer", name);
   MVB_REQUIRE(rows == 1 || in_stride >= width, "%s: rows %lld apart", name, (long long)in_stride);
   RowArgs a = {};
+  a.rows = rows;
   a.q = values, a.scale = scales, a.a = in, a.a_stride = in_stride, a.width = static_cast<int>(width);
   return run_kind<kPlain>(name, a, rows, dtype, reinterpret_cast<cudaStream_t>(stream));
 }
@@ -342,6 +389,7 @@ extern "C" int mvb_rmsnorm_q8(int8_t* values, float* scales, const void* in, int
   MVB_REQUIRE(values && scales && in && weight, "%s: null pointer", name);
   MVB_REQUIRE(rows == 1 || in_stride >= hidden, "%s: rows %lld apart", name, (long long)in_stride);
   RowArgs a = {};
+  a.rows = rows;
   a.q = values, a.scale = scales, a.a = in, a.a_stride = in_stride, a.w = weight;
   a.width = static_cast<int>(hidden), a.eps = eps, a.one = plus_one ? 1.0f : 0.0f;
   return run_kind<kNorm>(name, a, rows, dtype, reinterpret_cast<cudaStream_t>(stream));
@@ -359,6 +407,7 @@ extern "C" int mvb_fused_add_rmsnorm_q8(int8_t* values, float* scales, void* res
               "%s: rows %lld, %lld and %lld apart", name, (long long)in_stride, (long long)residual_stride,
               (long long)out_stride);
   RowArgs a = {};
+  a.rows = rows;
   a.q = values, a.scale = scales, a.a = residual, a.a_stride = residual_stride, a.b = in, a.b_stride = in_stride;
   a.sum = residual_out, a.sum_stride = out_stride, a.w = weight;
   a.width = static_cast<int>(hidden), a.eps = eps, a.one = plus_one ? 1.0f : 0.0f;
@@ -375,6 +424,7 @@ extern "C" int mvb_gated_q8(int8_t* values, float* scales, const void* gate, int
   MVB_REQUIRE(rows == 1 || (gate_stride >= width && up_stride >= width), "%s: rows %lld and %lld apart", name,
               (long long)gate_stride, (long long)up_stride);
   RowArgs a = {};
+  a.rows = rows;
   a.q = values, a.scale = scales, a.a = gate, a.a_stride = gate_stride, a.b = up, a.b_stride = up_stride;
   a.width = static_cast<int>(width);
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);

@@ -63,12 +63,14 @@ __device__ __forceinline__ uint32_t max2(uint32_t a, uint32_t b) {
 __device__ __forceinline__ float low_bf16(uint32_t v) { return __uint_as_float(v << 16); }
 __device__ __forceinline__ float high_bf16(uint32_t v) { return __uint_as_float(v & 0xffff0000u); }
 
-// x / 15, rounded once: the product with 1/15 and what it leaves over.
+// x / 15, rounded once: the product with 1/15 and what it leaves over.  NaN for an infinity.
 __device__ __forceinline__ float fifteenth(float x) {
   const float q = x * (1.0f / 15.0f);
-  const float left = fmaf(-15.0f, q, x);
-  return fabsf(x) > 1.0e-30f && fabsf(x) < 1.0e38f ? fmaf(left, 1.0f / 15.0f, q) : __fdiv_rn(x, 15.0f);
+  return fmaf(fmaf(-15.0f, q, x), 1.0f / 15.0f, q);
 }
+
+// Where a scale's reciprocal would leave fp32's range (not inlined: it is hardly ever called).
+__device__ __noinline__ float quotient(float x, float scale) { return __fdiv_rn(x, scale); }
 
 template <int GROUP>
 __global__ void __launch_bounds__(kThreads) quantise_w4_kernel(uint8_t* __restrict__ records,
@@ -114,14 +116,19 @@ __global__ void __launch_bounds__(kThreads) quantise_w4_kernel(uint8_t* __restri
       const bool tiny = scale < 1.1754944e-38f;
       float inv;
       asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inv) : "f"(scale));
-      const float z = rintf((tiny ? __fdiv_rn(low, scale) : low * inv) + 1536.0f - 1536.0f);
+      float z = low * inv;
+      if (tiny) z = quotient(low, scale);
+      z = rintf((z + 1536.0f) - 1536.0f);
       zero = static_cast<uint32_t>(z);
       const float most = kMagic + 15.0f - z;
       uint32_t u[8];
 #pragma unroll
       for (int e = 0; e < 8; e += 2) {
         float2 t = make_float2(low_bf16(v[e >> 1]), high_bf16(v[e >> 1]));
-        t = tiny ? make_float2(__fdiv_rn(t.x, scale), __fdiv_rn(t.y, scale)) : __fmul2_rn(t, make_float2(inv, inv));
+        if (tiny)
+          t = make_float2(quotient(t.x, scale), quotient(t.y, scale));
+        else
+          t = __fmul2_rn(t, make_float2(inv, inv));
         t = __fadd2_rn(__fadd2_rn(t, make_float2(1536.0f, 1536.0f)), make_float2(-1536.0f, -1536.0f));
         t = __fadd2_rn(t, make_float2(kMagic, kMagic));
         t = __fadd2_rn(make_float2(fminf(t.x, most), fminf(t.y, most)), make_float2(z, z));
