@@ -800,33 +800,52 @@ _I8, _F16 = torch.int8, torch.float16
 _DTYPE_CODE = {_F32: N.F32, _F16: N.F16, _BF16: N.BF16}
 
 
-def _float_rows(what: str, name: str, t, index: int | None = None, dtype=None, shape=None) -> tuple[int, int]:
-    """Checks rows of a float type on a GPU; (device, dtype code)."""
+def _refuse_rows(what: str, name: str, t, index: int | None = None, dtype=None, shape=None) -> None:
+    """Why ``t`` is not rows of a float type on a GPU, or not those of the other operand."""
     if not isinstance(t, torch.Tensor):
         raise RuntimeError(f"{what}: {name} must be a tensor")
-    at = t.get_device()
-    code = _DTYPE_CODE.get(t.dtype)
-    if at < 0:
-        N.require_cuda(t)
-    if code is None or t.dim() == 0 or t.shape[-1] == 0:
+    N.require_cuda(t)
+    if t.dtype not in _DTYPE_CODE or t.dim() == 0 or t.shape[-1] == 0:
         raise RuntimeError(f"{what}: {name} must be rows of float32, float16 or bfloat16, not {tuple(t.shape)} {t.dtype}")
-    if index is not None and (at != index or t.dtype is not dtype or t.shape != shape):
-        raise RuntimeError(f"{what}: {name} is {tuple(t.shape)} {t.dtype} on {t.device}, not {tuple(shape)} {dtype} on "
-                           f"cuda:{index}")
-    return at, code
+    raise RuntimeError(f"{what}: {name} is {tuple(t.shape)} {t.dtype} on {t.device}, not {tuple(shape)} {dtype} on "
+                       f"cuda:{index}")
+
+
+def _float_rows(what: str, name: str, t) -> tuple[int, int, torch.Size]:
+    """Rows of a float type on a GPU: device, dtype code, shape."""
+    try:
+        index, code, shape = t.get_device(), _DTYPE_CODE[t.dtype], t.shape
+        if index >= 0 and shape[-1]:
+            return index, code, shape
+    except (AttributeError, KeyError, IndexError, TypeError):
+        pass
+    return _refuse_rows(what, name, t)
+
+
+def _same_rows(what: str, name: str, t, index: int, dtype: torch.dtype, shape: torch.Size) -> None:
+    """The other operand's rows: its device, type and shape."""
+    try:
+        if t.dtype is dtype and t.shape == shape and t.get_device() == index:
+            return
+    except AttributeError:
+        pass
+    _refuse_rows(what, name, t, index, dtype, shape)
 
 
 def _row_view(t: torch.Tensor) -> tuple[torch.Tensor, int] | None:
     """``t`` as rows of stride-1 elements a fixed distance apart, and that distance; None if it is not."""
-    width = t.shape[-1]
+    shape = t.shape
+    width = shape[-1]
     if t.is_contiguous():
         return t, width
-    if width > 1 and t.stride(-1) != 1:
+    strides = t.stride()
+    if width > 1 and strides[-1] != 1:
         return None
-    if t.dim() == 1:
-        return t, width
+    if len(shape) == 2:
+        row = strides[0] if shape[0] > 1 else width
+        return (t, row) if row >= width else None
     row, size = 0, 1  # rows of the dimensions so far are `row` apart
-    for n, stride in zip(reversed(t.shape[:-1]), reversed(t.stride()[:-1])):
+    for n, stride in zip(reversed(shape[:-1]), reversed(strides[:-1])):
         if n == 1:
             continue
         if row and stride != row * size:
@@ -839,52 +858,59 @@ def _row_view(t: torch.Tensor) -> tuple[torch.Tensor, int] | None:
 
 def _rows_of(t: torch.Tensor) -> tuple[torch.Tensor, int]:
     """``_row_view``, of a copy where ``t`` is laid out otherwise."""
+    if t.is_contiguous():
+        return t, t.shape[-1]
     view = _row_view(t)
     return view if view is not None else (t.contiguous(), t.shape[-1])
 
 
-def _q8_out(like: torch.Tensor) -> tuple[Q8Rows, int]:
-    shape = like.shape
-    values = torch.empty(shape, dtype=_I8, device=like.device)
-    scales = torch.empty(shape[:-1], dtype=_F32, device=like.device)
-    return Q8Rows(values, scales), scales.numel()
+def _q8_out(like: torch.Tensor, shape: torch.Size) -> Q8Rows:
+    return Q8Rows(like.new_empty(shape, dtype=_I8), like.new_empty(shape[:-1], dtype=_F32))
 
 
 def quantise_q8(input: torch.Tensor) -> Q8Rows:
     """Rows ``[..., width]`` in 8 bits: per row ``amax = max |x|``, codes ``rint(127 x / amax)``, scale
     ``amax / 127``.  A row with an infinity or a NaN reads back as NaN."""
     what = "quantise_q8"
-    index, code = _float_rows(what, "input", input)
+    index, code, shape = _float_rows(what, "input", input)
     x, stride = _rows_of(input)
-    out, rows = _q8_out(x)
+    out = _q8_out(x, shape)
+    values, scales = out
+    rows = scales.numel()
     if rows:
-        N.on_device(index, what, N.lib().mvb_quantise_q8, out.values.data_ptr(), out.scales.data_ptr(), x.data_ptr(),
-                    stride, rows, x.shape[-1], code)
+        N.on_device(index, what, N.lib().mvb_quantise_q8, values.data_ptr(), scales.data_ptr(), x.data_ptr(), stride, rows,
+                    shape[-1], code)
     return out
 
 
 def _norm_weight(what: str, weight, index: int, width: int, dtype: torch.dtype) -> torch.Tensor:
-    if not isinstance(weight, torch.Tensor) or weight.get_device() != index or weight.shape != (width,):
+    try:
+        ok = weight.shape == (width,) and weight.get_device() == index
+    except AttributeError:
+        ok = False
+    if not ok:
         if isinstance(weight, torch.Tensor):
             N.require_cuda(weight)
         raise RuntimeError(f"{what}: weight must be [{width}] on cuda:{index}")
     if weight.dtype is not dtype:
         weight = weight.to(dtype)
-    return weight.contiguous()
+    return weight if weight.is_contiguous() else weight.contiguous()
 
 
 def rmsnorm_q8(input: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6, plus_one: bool = False) -> Q8Rows:
     """``rmsnorm`` (``plus_one``: with ``1 + weight``) whose result goes to 8 bits from its 32, without a
     rounding to the dtype in between.  Rows, non-finite ones too, as in ``quantise_q8``."""
     what = "rmsnorm_q8"
-    index, code = _float_rows(what, "input", input)
-    width = input.shape[-1]
+    index, code, shape = _float_rows(what, "input", input)
+    width = shape[-1]
     w = _norm_weight(what, weight, index, width, input.dtype)
     x, stride = _rows_of(input)
-    out, rows = _q8_out(x)
+    out = _q8_out(x, shape)
+    values, scales = out
+    rows = scales.numel()
     if rows:
-        N.on_device(index, what, N.lib().mvb_rmsnorm_q8, out.values.data_ptr(), out.scales.data_ptr(), x.data_ptr(),
-                    stride, w.data_ptr(), rows, width, float(eps), int(plus_one), code)
+        N.on_device(index, what, N.lib().mvb_rmsnorm_q8, values.data_ptr(), scales.data_ptr(), x.data_ptr(), stride,
+                    w.data_ptr(), rows, width, float(eps), int(plus_one), code)
     return out
 
 
@@ -895,37 +921,40 @@ def fused_add_rmsnorm_q8(residual: torch.Tensor, input: torch.Tensor, weight: to
     ``residual_out`` (default: into ``residual``, in place), its norm to 8 bits as in ``rmsnorm_q8``.
     Returns ``(rows, residual_out)``."""
     what = "fused_add_rmsnorm_q8"
-    index, code = _float_rows(what, "input", input)
-    _float_rows(what, "residual", residual, index, input.dtype, input.shape)
-    width = input.shape[-1]
-    w = _norm_weight(what, weight, index, width, input.dtype)
+    index, code, shape = _float_rows(what, "input", input)
+    dtype, width = input.dtype, shape[-1]
+    _same_rows(what, "residual", residual, index, dtype, shape)
+    w = _norm_weight(what, weight, index, width, dtype)
     if residual_out is None:
         residual_out = residual
     else:
-        _float_rows(what, "residual_out", residual_out, index, input.dtype, input.shape)
+        _same_rows(what, "residual_out", residual_out, index, dtype, shape)
     view = _row_view(residual_out)
     if view is None:
         raise RuntimeError(f"{what}: the rows of {'residual' if residual_out is residual else 'residual_out'} must be "
                            "contiguous and evenly apart: they are written")
-    out_stride = view[1]
     x, stride = _rows_of(input)
     res, res_stride = _rows_of(residual)
-    out, rows = _q8_out(x)
+    out = _q8_out(x, shape)
+    values, scales = out
+    rows = scales.numel()
     if rows:
-        N.on_device(index, what, N.lib().mvb_fused_add_rmsnorm_q8, out.values.data_ptr(), out.scales.data_ptr(),
-                    residual_out.data_ptr(), out_stride, res.data_ptr(), res_stride, x.data_ptr(), stride, w.data_ptr(),
-                    rows, width, float(eps), int(plus_one), code)
+        N.on_device(index, what, N.lib().mvb_fused_add_rmsnorm_q8, values.data_ptr(), scales.data_ptr(),
+                    residual_out.data_ptr(), view[1], res.data_ptr(), res_stride, x.data_ptr(), stride, w.data_ptr(), rows,
+                    width, float(eps), int(plus_one), code)
     return out, residual_out
 
 
 def _gated_q8(what: str, gate, up, act: int) -> Q8Rows:
-    index, code = _float_rows(what, "gate", gate)
-    _float_rows(what, "up", up, index, gate.dtype, gate.shape)
+    index, code, shape = _float_rows(what, "gate", gate)
+    _same_rows(what, "up", up, index, gate.dtype, shape)
     (g, g_stride), (u, u_stride) = _rows_of(gate), _rows_of(up)
-    out, rows = _q8_out(g)
+    out = _q8_out(g, shape)
+    values, scales = out
+    rows = scales.numel()
     if rows:
-        N.on_device(index, what, N.lib().mvb_gated_q8, out.values.data_ptr(), out.scales.data_ptr(), g.data_ptr(), g_stride,
-                    u.data_ptr(), u_stride, rows, g.shape[-1], act, code)
+        N.on_device(index, what, N.lib().mvb_gated_q8, values.data_ptr(), scales.data_ptr(), g.data_ptr(), g_stride,
+                    u.data_ptr(), u_stride, rows, shape[-1], act, code)
     return out
 
 
@@ -943,16 +972,16 @@ def geglu_q8(gate: torch.Tensor, up: torch.Tensor) -> Q8Rows:
 def _check_q8(what: str, rows) -> int:
     """Device of rows in 8 bits, checked."""
     v, s = rows
-    if not (isinstance(v, torch.Tensor) and isinstance(s, torch.Tensor)):
-        raise RuntimeError(f"{what}: values and scales must be tensors")
-    index = v.get_device()
-    if index < 0 or s.get_device() < 0:
-        N.require_cuda(v, s)
-    if (v.dtype is not _I8 or s.dtype is not _F32 or v.dim() == 0 or v.shape[-1] == 0 or s.shape != v.shape[:-1]
-            or s.get_device() != index):
-        raise RuntimeError(f"{what}: values {tuple(v.shape)} {v.dtype} and scales {tuple(s.shape)} {s.dtype} are not int8 "
-                           "rows with an fp32 scale each, on one GPU")
-    return index
+    try:
+        index, shape = v.get_device(), v.shape
+        if (v.dtype is _I8 and s.dtype is _F32 and index >= 0 and s.get_device() == index and len(shape)
+                and s.shape == shape[:-1] and shape[-1]):
+            return index
+    except AttributeError:
+        raise RuntimeError(f"{what}: values and scales must be tensors") from None
+    N.require_cuda(v, s)
+    raise RuntimeError(f"{what}: values {tuple(v.shape)} {v.dtype} and scales {tuple(s.shape)} {s.dtype} are not int8 "
+                       "rows with an fp32 scale each, on one GPU")
 
 
 def dequantise_q8(rows: Q8Rows, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
@@ -962,12 +991,14 @@ def dequantise_q8(rows: Q8Rows, dtype: torch.dtype = torch.bfloat16) -> torch.Te
     code = _DTYPE_CODE.get(dtype)
     if code is None:
         raise RuntimeError(f"{what}: float32, float16 or bfloat16, not {dtype}")
-    v, stride = _rows_of(rows.values)
-    scales = rows.scales.contiguous()
-    out = torch.empty(v.shape, dtype=dtype, device=v.device)
-    if scales.numel():
-        N.on_device(index, what, N.lib().mvb_dequantise_q8, out.data_ptr(), v.data_ptr(), stride, scales.data_ptr(),
-                    scales.numel(), v.shape[-1], code)
+    values, scales = rows
+    v, stride = _rows_of(values)
+    scales = scales.contiguous()
+    out = v.new_empty(v.shape, dtype=dtype)
+    n = scales.numel()
+    if n:
+        N.on_device(index, what, N.lib().mvb_dequantise_q8, out.data_ptr(), v.data_ptr(), stride, scales.data_ptr(), n,
+                    v.shape[-1], code)
     return out
 
 
@@ -981,11 +1012,11 @@ class W4Weight(NamedTuple):
 
 
 def _w4_records(what: str, n: int, k: int, group: int, device: torch.device) -> torch.Tensor:
-    if group not in (32, 64, 128):
+    if group not in _W4_BYTES:
         raise RuntimeError(f"{what}: groups of 32, 64 or 128 columns, not {group}")
     if k <= 0 or k % 32:
         raise RuntimeError(f"{what}: a multiple of 32 columns, not {k}")
-    return torch.empty((n + 15) // 16 * ((k + 127) // 128), 1024 + 8192 // group, dtype=_U8, device=device)
+    return torch.empty((n + 15) // 16 * ((k + 127) // 128), _W4_BYTES[group], dtype=_U8, device=device)
 
 
 def quantise_w4(weight: torch.Tensor, group: int = 128) -> W4Weight:
@@ -1031,17 +1062,21 @@ def pack_w4(codes: torch.Tensor, scales: torch.Tensor, zeros: torch.Tensor | Non
     return W4Weight(records, n, k, group)
 
 
+_W4_BYTES = {32: 1280, 64: 1152, 128: 1088}  # of a record, by the group
+
+
 def _check_w4(what: str, weight: W4Weight) -> int:
     """Device of a 4-bit weight, checked."""
-    r, n, k, group = weight
-    if (not isinstance(r, torch.Tensor) or r.dtype is not _U8 or group not in (32, 64, 128) or k <= 0 or k % 32 or n < 0
-            or r.shape != ((n + 15) // 16 * ((k + 127) // 128), 1024 + 8192 // group) or not r.is_contiguous()
-            or r.data_ptr() % 16):
-        raise RuntimeError(f"{what}: weight must be what quantise_w4 or pack_w4 gave")
-    index = r.get_device()
-    if index < 0:
-        N.require_cuda(r)
-    return index
+    try:
+        r, n, k, group = weight
+        index = r.get_device()
+        if (r.dtype is _U8 and r.shape == ((n + 15) // 16 * ((k + 127) // 128), _W4_BYTES[group]) and r.is_contiguous()
+                and index >= 0 and k > 0 and k % 32 == 0 and r.data_ptr() % 16 == 0):
+            return index
+    except (AttributeError, KeyError, TypeError, ValueError):
+        raise RuntimeError(f"{what}: weight must be what quantise_w4 or pack_w4 gave") from None
+    N.require_cuda(r)
+    raise RuntimeError(f"{what}: weight must be what quantise_w4 or pack_w4 gave")
 
 
 def dequantise_w4(weight: W4Weight, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
@@ -1061,7 +1096,7 @@ def dequantise_w4(weight: W4Weight, dtype: torch.dtype = torch.bfloat16) -> torc
 def linear_w4(x: torch.Tensor | Q8Rows, weight: W4Weight, out: torch.Tensor | None = None) -> torch.Tensor:
     """``linear`` with a 4-bit weight: ``x @ w.T`` (bf16) for bf16 rows ``[..., k]`` or rows in 8 bits (``Q8Rows``), one
     row to many.  Sums run in 32 bits and are rounded once; no weight or product is rounded before.
-    ``out``: bf16 ``[rows, n]`` with contiguous rows."""
+    ``out``: bf16 ``[rows, n]`` with contiguous rows, and then what is returned."""
     what = "linear_w4"
     index = _check_w4(what, weight)
     records, n, k, group = weight
@@ -1069,8 +1104,8 @@ def linear_w4(x: torch.Tensor | Q8Rows, weight: W4Weight, out: torch.Tensor | No
     if type(x) is Q8Rows:
         if _check_q8(what, x) != index:
             raise RuntimeError(f"{what}: x is on {x.values.device}, the weight on {records.device}")
-        scales = x.scales.contiguous()
-        x = x.values
+        x, scales = x
+        scales = scales.contiguous()
     elif not isinstance(x, torch.Tensor) or x.dtype is not _BF16 or x.get_device() != index or x.dim() == 0:
         if isinstance(x, torch.Tensor):
             N.require_cuda(x)
@@ -1083,14 +1118,15 @@ def linear_w4(x: torch.Tensor | Q8Rows, weight: W4Weight, out: torch.Tensor | No
         x, ldx = x.clone(memory_format=torch.contiguous_format), k
     rows = x.numel() // k
     if out is None:
-        out = torch.empty(*shape[:-1], n, dtype=_BF16, device=x.device)
+        y = x.new_empty(shape[:-1] + (n,), dtype=_BF16)
         ldy = n
     else:
         _expect(what, "out", out, index, _BF16, 2)
         ldy = out.stride(0) if rows > 1 else n
         if out.shape != (rows, n) or n > 1 and out.stride(1) != 1 or ldy < n:
             raise RuntimeError(f"{what}: out must be {(rows, n)} with contiguous rows, apart")
+        y = out
     if rows and n:
-        N.on_device(index, what, N.lib().mvb_linear_w4, out.data_ptr(), ldy, x.data_ptr(), ldx, N.ptr(scales),
+        N.on_device(index, what, N.lib().mvb_linear_w4, y.data_ptr(), ldy, x.data_ptr(), ldx, N.ptr(scales),
                     records.data_ptr(), rows, n, k, group)
-    return out.reshape(*shape[:-1], n) if out.dim() != len(shape) else out
+    return y
