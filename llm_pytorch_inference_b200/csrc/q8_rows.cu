@@ -42,12 +42,15 @@ struct RowArgs {
   float one;        // 1 for the (1 + w) norm, else 0
 };
 
-// g act'(g), by the logistic function: silu(g) = g / (1 + e^-g), and gelu's 0.5 g (1 + tanh z) = g / (1 + e^-2z).
-// The quotient and the exponential are the hardware's (some 1e-6 relative, against half a code's 4e-3).
+// The activations by the logistic function: silu(g) = g / (1 + e^-z) with z = g, and gelu's 0.5 g (1 + tanh(z / 2)) the same
+// with its z.  With e = e^-|z| it is g / (1 + e) or g e / (1 + e), so that nothing leaves fp32's range before the result
+// does.  The quotient and the exponential are the hardware's: (6 + 1.2 |z|) 2^-24 relative, for gelu 3 |z| 2^-24 more by
+// the rounding of z; half a code is 4e-3 of the row's largest.
 template <int KIND>
 __device__ __forceinline__ float act_of(float g) {
   const float z = KIND == kSilu ? g : 1.5957691216057308f * g * fmaf(0.044715f * g, g, 1.0f);  // 2 sqrt(2 / pi)
-  return __fdividef(g, 1.0f + __expf(-z));
+  const float e = __expf(-fabsf(z));
+  return __fdividef(z < 0.0f ? g * e : g, 1.0f + e);
 }
 
 template <int KIND, typename T>

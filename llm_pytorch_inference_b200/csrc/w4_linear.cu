@@ -10,9 +10,9 @@
 //
 // A bf16 row is taken apart into three rows of 8 bits, by group: with 2^E the size of the group's largest element,
 // x = 2^(E - 5) (q0 + 2^-7 q1 + 2^-14 q2), each the nearest whole number to what is left.  That is exact but for elements
-// below 2^-13 of the group's largest, which are off by at most 2^-22 of it: less than rounding to 32 bits
-// in a sum of the group's products is.  A group's three sums are scaled and added in 32 bits; a group with an infinity or a
-// NaN gives NaN.
+// below 2^(E - 12), which are off by at most 2^(E - 20): as much as rounding a sum of the size of the group's largest
+// product to 32 bits a few times.  A group's three sums are scaled and added in 32 bits; a group with an infinity or a NaN
+// gives NaN.
 //
 // A block works on pairs of 16 weight rows.  Its warps split the columns; each is a worker with a ring of its own,
 // into which one bulk copy brings the records of both tiles for 128 columns.  x lies in shared memory in the order of

@@ -29,7 +29,7 @@ __all__ = [
     "FusedMLP", "linear", "paged_attention_decode", "qk_norm_rope_kv_write", "sample", "kv4_write", "kv4_read",
     "paged_attention_decode_kv4", "assign_slots", "SlotPlan", "verify_drafts", "Q8Rows", "quantise_q8",
     "dequantise_q8", "rmsnorm_q8", "fused_add_rmsnorm_q8", "swiglu_q8", "geglu_q8", "W4Weight", "quantise_w4",
-    "pack_w4", "dequantise_w4", "linear_w4",
+    "pack_w4", "dequantise_w4", "linear_w4", "FusedMLPW4",
 ]
 
 
@@ -1130,3 +1130,32 @@ def linear_w4(x: torch.Tensor | Q8Rows, weight: W4Weight, out: torch.Tensor | No
         N.on_device(index, what, N.lib().mvb_linear_w4, y.data_ptr(), ldy, x.data_ptr(), ldx, N.ptr(scales),
                     records.data_ptr(), rows, n, k, group)
     return y
+
+
+class FusedMLPW4(nn.Module):
+    """A ``FusedMLP`` with weights in 4 bits, made from one: gate_up product, act(gate) * up, down product.
+
+    ``rows``: what the products read.  8: rows in 8 bits (bf16 rows that come in are quantised, ``Q8Rows``
+    from ``fused_add_rmsnorm_q8`` taken as they are; the activation's result goes to 8 bits where it is made).
+    16: bf16 rows."""
+
+    def __init__(self, mlp: FusedMLP, group: int = 128, rows: int = 8):
+        super().__init__()
+        if rows not in (8, 16):
+            raise ValueError(f"rows of 8 or 16 bits, not {rows}")
+        self.rows, self.group, self._act_code = rows, group, mlp._act_code
+        self.intermediate_size, self.hidden_size = mlp.intermediate_size, mlp.down_proj.weight.shape[0]
+        for name in ("gate_up", "down"):
+            weight = getattr(mlp, name + "_proj").weight.detach()
+            self.register_buffer(name, quantise_w4(weight.to(torch.bfloat16), group).records)
+
+    def forward(self, x: torch.Tensor | Q8Rows) -> torch.Tensor:
+        inter, hidden = self.intermediate_size, self.hidden_size
+        gate_up, down = W4Weight(self.gate_up, 2 * inter, hidden, self.group), W4Weight(self.down, hidden, inter, self.group)
+        if self.rows == 8 and type(x) is not Q8Rows:
+            x = quantise_q8(x)
+        gu = linear_w4(x, gate_up)
+        if self.rows == 16:
+            return linear_w4(fused_mlp_forward(gu, inter, self._act_code), down)
+        gate, up = gu.chunk(2, -1)
+        return linear_w4((swiglu_q8 if self._act_code == 0 else geglu_q8)(gate, up), down)

@@ -54,6 +54,16 @@ DECODE_SCHEMAS = [
     "int num_tokens, Tensor? free_head, Tensor(b!)? held_blocks=None) -> (Tensor, Tensor, Tensor, Tensor, Tensor)",
     "verify_drafts(Tensor target_probs, Tensor draft_tokens, Tensor uniforms, Tensor? draft_probs, "
     "Tensor? draft_lens) -> (Tensor, Tensor)",
+    "quantise_q8(Tensor input) -> (Tensor, Tensor)",
+    "dequantise_q8(Tensor values, Tensor scales) -> Tensor",
+    "rmsnorm_q8(Tensor input, Tensor weight, float eps, bool plus_one) -> (Tensor, Tensor)",
+    "fused_add_rmsnorm_q8(Tensor(a!) residual, Tensor input, Tensor weight, float eps, bool plus_one) "
+    "-> (Tensor, Tensor)",
+    "gated_q8(Tensor gate, Tensor up, int activation) -> (Tensor, Tensor)",
+    "quantise_w4(Tensor weight, int group) -> Tensor",
+    "pack_w4(Tensor codes, Tensor scales, Tensor? zeros, int group) -> Tensor",
+    "dequantise_w4(Tensor records, int n, int k, int group) -> Tensor",
+    "linear_w4(Tensor x, Tensor? row_scales, Tensor records, int n, int k, int group) -> Tensor",
 ]
 
 
@@ -78,6 +88,12 @@ def _filter_inplace(logits: torch.Tensor, top_k: int, top_p: float) -> None:
         N.check(N.lib().mvb_top_k_top_p_filter(logits.data_ptr(), logits.numel() // V, V, int(top_k), float(top_p),
                                                N.dtype_code(logits), N.stream_handle(logits.device)),
                 "top_k_top_p_filter")
+
+
+def _gated_q8(gate: torch.Tensor, up: torch.Tensor, activation: int) -> tuple[torch.Tensor, torch.Tensor]:
+    if activation not in (N.ACT_SILU, N.ACT_GELU_TANH):
+        raise RuntimeError(f"gated_q8: activation {activation}")
+    return tuple((ops.swiglu_q8 if activation == N.ACT_SILU else ops.geglu_q8)(gate, up))
 
 
 IMPLS = {
@@ -110,6 +126,16 @@ IMPLS = {
         ops.paged_attention_decode_kv4(q, kv4, layer, block_tables, ctx_lens, scale, softcap=softcap, window=window),
     "assign_slots": lambda *args: tuple(ops._assign_slots(*args, apart=True)),  # outputs may not alias
     "verify_drafts": ops.verify_drafts,
+    "quantise_q8": lambda input: tuple(ops.quantise_q8(input)),
+    "dequantise_q8": lambda values, scales: ops.dequantise_q8(ops.Q8Rows(values, scales)),
+    "rmsnorm_q8": lambda *args: tuple(ops.rmsnorm_q8(*args)),
+    "fused_add_rmsnorm_q8": lambda *args: tuple(ops.fused_add_rmsnorm_q8(*args)[0]),
+    "gated_q8": _gated_q8,
+    "quantise_w4": lambda weight, group: ops.quantise_w4(weight, group).records,
+    "pack_w4": lambda codes, scales, zeros, group: ops.pack_w4(codes, scales, zeros, group).records,
+    "dequantise_w4": lambda records, n, k, group: ops.dequantise_w4(ops.W4Weight(records, n, k, group)),
+    "linear_w4": lambda x, row_scales, records, n, k, group: ops.linear_w4(
+        x if row_scales is None else ops.Q8Rows(x, row_scales), ops.W4Weight(records, n, k, group)),
 }
 
 _LIB: torch.library.Library | None = None
