@@ -79,15 +79,21 @@ __device__ __forceinline__ void tmem_st_x16(uint32_t taddr, const uint32_t* r) {
 }
 __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
+// (a & b) | c as one instruction: of two constants the compiler makes two.
+__device__ __forceinline__ uint32_t and_or(uint32_t a, uint32_t b, uint32_t c) {
+  uint32_t d;
+  asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(d) : "r"(a), "r"(b), "r"(c));
+  return d;
+}
 // (w >> 4 j) of a word, less the zero: two bf16 numbers code - zero (z2: 128 + zero twice)
 __device__ __forceinline__ uint32_t codes_bf16(uint32_t w, uint32_t z2) {
-  uint32_t v = (w & 0x000f000fu) | 0x43004300u, d;
+  uint32_t v = and_or(w, 0x000f000fu, 0x43004300u), d;
   asm("sub.rn.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(v), "r"(z2));
   return d;
 }
 // The low nibbles of four bytes, less the zero (z4: four times): with the top bit set no byte borrows from the next.
 __device__ __forceinline__ uint32_t codes_s8(uint32_t w, uint32_t z4) {
-  return (((w & 0x0f0f0f0fu) | 0x80808080u) - z4) ^ 0x80808080u;
+  return (and_or(w, 0x0f0f0f0fu, 0x80808080u) - z4) ^ 0x80808080u;
 }
 
 // Sums out of TMEM, two at a time.  Whole sums are below 2^18 in size: added to the bits of 1.5 * 2^23 they are its low

@@ -463,7 +463,7 @@ extern "C" int mvb_linear_w4(void* y, int64_t ldy, const void* x, int64_t ldx, c
   a.blocks = (a.k + kW4Cols - 1) / kW4Cols;
   a.pairs = (a.tiles + 1) / 2;
   a.err = device_status_ptr();
-  if (rows > (row_scales != nullptr ? 16 : 5)) {
+  if (rows > (row_scales != nullptr ? 16 : 8)) {
     const int64_t apart = rows > 1 ? ldx : k;
     const W4LinearCall call = {a.y, ldy, x, apart, row_scales, a.records, a.rows, a.n, a.k, static_cast<int>(group)};
     return w4_gemm(name, call, reinterpret_cast<cudaStream_t>(stream));
