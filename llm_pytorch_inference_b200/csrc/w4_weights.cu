@@ -69,9 +69,6 @@ __device__ __forceinline__ float fifteenth(float x) {
   return fmaf(fmaf(-15.0f, q, x), 1.0f / 15.0f, q);
 }
 
-// Where a scale's reciprocal would leave fp32's range (not inlined: it is hardly ever called).
-__device__ __noinline__ float quotient(float x, float scale) { return __fdiv_rn(x, scale); }
-
 template <int GROUP>
 __global__ void __launch_bounds__(kThreads) quantise_w4_kernel(uint8_t* __restrict__ records,
                                                                const __nv_bfloat16* __restrict__ w, int64_t w_stride,
@@ -109,35 +106,35 @@ __global__ void __launch_bounds__(kThreads) quantise_w4_kernel(uint8_t* __restri
     if (scale > 0.0f && scale < __uint_as_float(0x7f800000u)) {
       // Quotients of two bf16 numbers below 16 either fall on a border between codes or are 1e-3 away from it, and
       // the product with the reciprocal is off by 4e-6: rounded to a multiple of 2^-13 (the sum with 1536), it falls on the
-      // right side, or on the border.  The whole number then is the low bits of the sum with 1.5 * 2^23.  None is below
-      // -zero, since rounding is monotonic and odd; the most is cut.  (A reciprocal of a scale below 2^-126 would
-      // overflow: the quotient itself.)
-      constexpr float kMagic = 12582912.0f;
-      const bool tiny = scale < 1.1754944e-38f;
+      // right side, or on the border.  The next sum, 1.5 * 2^23 and 16 above the quotient, has the whole number and
+      // 16 for its low bits.  It is never below -zero, since rounding is monotonic and odd; the most is cut.
+      constexpr float kMagic = 12582928.0f;
+      float y[8], least = low, by = scale;
+#pragma unroll
+      for (int e = 0; e < 8; e += 2) y[e] = low_bf16(v[e >> 1]), y[e + 1] = high_bf16(v[e >> 1]);
+      if (scale < 1.1754944e-38f) {  // whose reciprocal would overflow: all times 2^64
+        constexpr float kUp = 1.8446744e19f;
+        least *= kUp, by *= kUp;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) y[e] *= kUp;
+      }
       float inv;
-      asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inv) : "f"(scale));
-      float z = low * inv;
-      if (tiny) z = quotient(low, scale);
-      z = rintf((z + 1536.0f) - 1536.0f);
-      zero = static_cast<uint32_t>(z);
-      const float most = kMagic + 15.0f - z;
+      asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inv) : "f"(by));
+      const float z = (least * inv + 1536.0f) + (kMagic - 1536.0f);
+      zero = __float_as_uint(z) - __float_as_uint(kMagic);
+      const float most = (kMagic + 15.0f) - (z - kMagic);
       uint32_t u[8];
 #pragma unroll
       for (int e = 0; e < 8; e += 2) {
-        float2 t = make_float2(low_bf16(v[e >> 1]), high_bf16(v[e >> 1]));
-        if (tiny)
-          t = make_float2(quotient(t.x, scale), quotient(t.y, scale));
-        else
-          t = __fmul2_rn(t, make_float2(inv, inv));
-        t = __fadd2_rn(__fadd2_rn(t, make_float2(1536.0f, 1536.0f)), make_float2(-1536.0f, -1536.0f));
-        t = __fadd2_rn(t, make_float2(kMagic, kMagic));
-        t = __fadd2_rn(make_float2(fminf(t.x, most), fminf(t.y, most)), make_float2(z, z));
-        u[e] = __float_as_uint(t.x);
-        u[e + 1] = __float_as_uint(t.y);
+        float2 t = __fmul2_rn(make_float2(y[e], y[e + 1]), make_float2(inv, inv));
+        t = __fadd2_rn(__fadd2_rn(t, make_float2(1536.0f, 1536.0f)), make_float2(kMagic - 1536.0f, kMagic - 1536.0f));
+        u[e] = __float_as_uint(fminf(t.x, most));
+        u[e + 1] = __float_as_uint(fminf(t.y, most));
       }
-      // a code is its number's low byte: those of columns 0 4 1 5 below, 2 6 3 7 above
-      const uint32_t below = __byte_perm(__byte_perm(u[0], u[4], 0x0040), __byte_perm(u[1], u[5], 0x0040), 0x5410);
-      const uint32_t above = __byte_perm(__byte_perm(u[2], u[6], 0x0040), __byte_perm(u[3], u[7], 0x0040), 0x5410);
+      // The low bytes of columns 0 4 1 5 make the low nibbles, those of 2 6 3 7 the high ones; all less 16 plus zero.
+      const uint32_t more = zero * 0x01010101u - 0x10101010u;
+      const uint32_t below = __byte_perm(__byte_perm(u[0], u[4], 0x0040), __byte_perm(u[1], u[5], 0x0040), 0x5410) + more;
+      const uint32_t above = __byte_perm(__byte_perm(u[2], u[6], 0x0040), __byte_perm(u[3], u[7], 0x0040), 0x5410) + more;
       word = below | above << 4;
     }
     const bool some = at.tile * kW4Rows + row < s.n && col < s.k;  // else it stays zero
