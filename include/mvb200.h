@@ -618,7 +618,8 @@ int mvb_dequantise_q8(void* out, const int8_t* values, int64_t values_stride, co
  * layout of csrc/w4.cuh.
  *   mvb_quantise_w4    from bf16 (rows weight_stride elements apart, 16-byte aligned): per group lo = min(0, min w),
  *                      hi = max(0, max w), scale = bf16((hi - lo) / 15), zero = rint(-lo / scale),
- *                      code = rint(w / scale) + zero, cut to 0 .. 15.  A group with an infinity or a NaN reads back as NaN.
+ *                      code = rint(w / scale) + zero, cut to 0 .. 15.  A group with an infinity or a NaN, or whose hi - lo leaves fp32's
+ *                      range, reads back as NaN.
  *   mvb_pack_w4        from codes [n, k] and zeros [n, ceil(k / group)] (a byte each, the low 4 bits; zeros NULL: 8) and
  *                      scales [n, ceil(k / group)] (bf16)
  *   mvb_dequantise_w4  out[n, k], MVB_BF16 (rounded) or MVB_F32 (exact but for subnormal results)

@@ -14,6 +14,9 @@
 // through a row for few.  What an SM can do in that time is some 20 instructions an element, so pairs of 16-bit
 // numbers are taken apart and made two at a time, and so are products and sums.
 //
+// Measured: addition and norm of 16384 x 4096 82 us (87 % of the rate of a copy), SwiGLU of 8192 x 14336 138
+// (65 %); both issue in two thirds of the slots.  64 x 4096, norm and reading back, 3.8: two launches.
+//
 // A row with an infinity or a NaN (in y, before r) gets the scale NaN: it reads back as NaN, and so does a product with it.
 // A row of zeros gets the scale 0.
 #include <climits>

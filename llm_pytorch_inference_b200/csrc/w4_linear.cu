@@ -19,6 +19,10 @@
 // the lanes.  The warps' sums of a pair meet in shared memory and are added in the order of the warps.  A cluster of
 // up to 8 blocks splits the columns further, where few weight rows would leave SMs idle or x would not fit; its sums
 // meet in distributed shared memory, in the order of the blocks.  So every result is the same on every call.
+//
+// Measured, one row, groups of 128: 151936 x 4096 bf16 55.8 us (49.4 at the rate of a copy), 24576 x 4096 14.4 (8.0),
+// 4096 x 4096 6.35, 2048 x 1024 4.6.  The long ones stream; 24576 x 4096 gives an SM 5 or 6 pairs and issues in 48 % of
+// the slots on average, start and end included; the short ones are their launch, x and a chain of latencies.
 #include <climits>
 
 #include "common.cuh"
@@ -35,6 +39,8 @@ constexpr int kPitch = 36;  // floats between columns of a pair's 32 sums: 4 col
 constexpr int kRound = 16;  // pairs after which the blocks of a cluster add up
 constexpr int kMaxCluster = 8;
 constexpr int kMaxStages = 8;
+// What a pair's end (sums through shared memory, one barrier, the results) takes, in items of 128 columns.  Against 1.5:
+// 24576 x 4096 14.3 us and 15.1, 151936 x 4096 55.9 and 54.6, one row.
 constexpr double kPairEnd = 3.0;
 constexpr size_t kMostSmem = 227 * 1024;
 
@@ -374,7 +380,8 @@ int run(const char* name, LinearArgs a, cudaStream_t stream) {
   auto kernel = w4_linear_kernel<GROUP, P, NT>;
   static std::atomic<uint64_t> done{0};
   MVB_TRY(set_smem_once(done, kernel, kMostSmem, name));
-  // The cluster: what its blocks' work takes, in records of a pair of tiles, and what a cluster's meeting costs.
+  // The cluster: what its blocks' work takes, in records of a pair of tiles, and what a cluster's meeting costs (two cluster
+  // barriers and remote reads, some 1.2 us, take as long as 24 records).
   static std::atomic<int> clusters[kMaxCluster + 1] = {};
   auto units_of = [&](int c) {
     return c == 1 ? sms : clusters_at_once(clusters[c], kernel, c, kThreads, kMostSmem);
@@ -390,7 +397,7 @@ int run(const char* name, LinearArgs a, cudaStream_t stream) {
   MVB_REQUIRE(best > 0, "%s: %d columns", name, a.k);
   a.cluster = best;
   const int units = a.pairs < units_of(best) ? a.pairs : units_of(best);
-  // The warps that share a pair's columns: in items, what they compute and what a pair's end takes (some 3).
+  // The warps that share a pair's columns: in items, what they compute and what a pair's end takes.
   const int blocks = (a.blocks + best - 1) / best, mine = (a.pairs + units - 1) / units;
   double fewest = 0;
   a.split = 0;
@@ -463,9 +470,11 @@ extern "C" int mvb_linear_w4(void* y, int64_t ldy, const void* x, int64_t ldx, c
   a.blocks = (a.k + kW4Cols - 1) / kW4Cols;
   a.pairs = (a.tiles + 1) / 2;
   a.err = device_status_ptr();
+  // Few rows here, more on tcgen05.  A bf16 row is three columns of the product here.  8 bf16 rows, here and on tcgen05:
+  // 24576 x 4096 25.8 us and 32.7, 4096 x 4096 10.1 and 15.0, 4096 x 12288 24.6 and 23.0.  20 to 24 rows of 8 bits, here and
+  // there: 24576 x 4096 36.2 and 29.5, 4096 x 4096 18.8 and 14.2, 4096 x 12288 31.2 and 21.2, 2048 x 1024 5.8 and 9.3.
   if (rows > (row_scales != nullptr ? 16 : 8)) {
-    const int64_t apart = rows > 1 ? ldx : k;
-    const W4LinearCall call = {a.y, ldy, x, apart, row_scales, a.records, a.rows, a.n, a.k, static_cast<int>(group)};
+    const W4LinearCall call = {a.y, ldy, x, ldx, row_scales, a.records, a.rows, a.n, a.k, static_cast<int>(group)};
     return w4_gemm(name, call, reinterpret_cast<cudaStream_t>(stream));
   }
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);

@@ -2,12 +2,18 @@
 //
 // Quantised, per row and group: lo = min(0, min w), hi = max(0, max w), scale = bf16((hi - lo) / 15),
 // zero = rint(-lo / scale), code = rint(w / scale) + zero, both cut to 0 .. 15.  The codes are chosen against the rounded
-// scale, so that its rounding adds nothing to their half step.  A group with a NaN or an infinity gets a NaN or
-// infinite scale and reads back as such.
+// scale, so that its rounding adds nothing to their half step.  A group with a NaN or an infinity, or whose hi - lo leaves
+// fp32's range, gets the scale NaN and reads back as NaN.
 //
 // Bound by memory: 2 bytes in and 0.53 out per weight (and back).  Half a warp takes 128 columns of a row, 8 a lane:
 // one 16-byte load, and one word of codes; a warp takes a record, 8 pairs of rows, whose loads are all under way first.
 // A group's extremes cross 16, 8 or 4 lanes as one packed pair (max of -w and of w), 4, 3 or 2 exchanges.
+// Measured, 24576 x 4096 in groups of 64 (255 MB either way, 39 us at the rate of a copy): quantising 57 us, bound by
+// what it computes (81 % of the issue slots before its last step, which took two sums a code out); reading back 42.6 us,
+// bound by memory.
+//
+// The makers let no kernel start before they end, and what they wrote is at the GPU's scope before they do: products read
+// records before they wait for the kernel before them.
 #include <climits>
 
 #include "common.cuh"
@@ -144,6 +150,7 @@ __global__ void __launch_bounds__(kThreads) quantise_w4_kernel(uint8_t* __restri
       *reinterpret_cast<uint32_t*>(rec + kW4CodeBytes + (row * PER + part / LANES) * 4) = some ? pair : 0u;
     }
   }
+  __threadfence();
 }
 
 template <int GROUP>
@@ -181,6 +188,7 @@ __global__ void __launch_bounds__(kThreads) pack_w4_kernel(uint8_t* __restrict__
       *reinterpret_cast<uint32_t*>(rec + kW4CodeBytes + (row * PER + part / LANES) * 4) = pair;
     }
   }
+  __threadfence();
 }
 
 template <int GROUP, typename T>

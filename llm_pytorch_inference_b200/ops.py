@@ -1023,7 +1023,8 @@ def quantise_w4(weight: torch.Tensor, group: int = 128) -> W4Weight:
     """A bf16 weight matrix ``[n, k]`` (k a multiple of 32) in 4 bits, once, for ``linear_w4``.  Per row and group
     of 32, 64 or 128 columns: ``lo = min(0, min w)``, ``hi = max(0, max w)``, ``scale = bf16((hi - lo) / 15)``,
     ``zero = rint(-lo / scale)``, ``code = rint(w / scale) + zero``; a weight stands for
-    ``scale * (code - zero)``.  A group with a NaN or an infinity reads back as NaN."""
+    ``scale * (code - zero)``.  A group with a NaN or an infinity, or whose ``hi - lo`` leaves fp32's range, reads back
+    as NaN."""
     what = "quantise_w4"
     index = weight.get_device() if isinstance(weight, torch.Tensor) else -1
     _expect(what, "weight", weight, index, _BF16, 2)
@@ -1095,8 +1096,10 @@ def dequantise_w4(weight: W4Weight, dtype: torch.dtype = torch.bfloat16) -> torc
 
 def linear_w4(x: torch.Tensor | Q8Rows, weight: W4Weight, out: torch.Tensor | None = None) -> torch.Tensor:
     """``linear`` with a 4-bit weight: ``x @ w.T`` (bf16) for bf16 rows ``[..., k]`` or rows in 8 bits (``Q8Rows``), one
-    row to many.  Sums run in 32 bits and are rounded once; no weight or product is rounded before.
-    ``out``: bf16 ``[rows, n]`` with contiguous rows, and then what is returned."""
+    row (of at most 262144) to many.  Sums run in 32 bits and are rounded once; no weight or product is rounded before.
+    k is at most 32768.  A bf16 row with an infinity or a NaN has results that are not finite (NaN where there are 8
+    rows or fewer), and leaves the other rows alone.  ``out``: bf16 ``[rows, n]`` with contiguous rows, and then what is
+    returned; it must not overlap ``x``."""
     what = "linear_w4"
     index = _check_w4(what, weight)
     records, n, k, group = weight

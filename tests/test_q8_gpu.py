@@ -234,3 +234,20 @@ def test_graph_stream_and_namespace():
     assert torch.equal(space.quantise_q8(x)[0], ops.quantise_q8(x).values)
     assert torch.equal(space.rmsnorm_q8(x, w, 1e-6, True)[1], ops.rmsnorm_q8(x, w, 1e-6, True).scales)
     assert N.device_status() == 0
+
+
+def test_offsets_beyond_32_bits():
+    """2.3e9 elements: the last rows are what they are by themselves."""
+    x = torch.zeros(140000, 16384, dtype=torch.bfloat16, device=DEV)
+    x[-5:] = rows_of(90, 5, 16384)
+    last = x[-5:].clone()
+    weight = rows_of(91, 16384, wide=False)
+    for call in (ops.quantise_q8, lambda t: ops.rmsnorm_q8(t, weight), lambda t: ops.swiglu_q8(t, t),
+                 lambda t: ops.fused_add_rmsnorm_q8(t, t, weight, residual_out=torch.empty_like(t))[0]):
+        got, want = call(x), call(last)
+        assert torch.equal(got.values[-5:], want.values)
+        torch.testing.assert_close(got.scales[-5:], want.scales, rtol=2 ** -20, atol=0)  # squares are shared out otherwise
+        assert not got.scales[:-5].any() and not got.values[:-5].any()
+        back = ops.dequantise_q8(got)
+        assert torch.equal(back[-5:], ops.dequantise_q8(ops.Q8Rows(got.values[-5:], got.scales[-5:])))
+        assert not back[:-5].any()

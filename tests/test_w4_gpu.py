@@ -429,3 +429,60 @@ def test_launches_that_follow_one_another_early():
     finally:
         N.set_pdl(before)
     assert N.device_status() == 0
+
+
+def test_products_right_after_their_weight_is_made():
+    """A product asks for records before it waits for the kernel before it, which here makes them."""
+    before = N.set_pdl(True)
+    try:
+        for seed in range(6):
+            weight, (x, _) = weight_of(50 + seed, 2048, 1024), rows_of(60 + seed, 3, 1024, False)
+            many = x.repeat(30, 1)
+            torch.cuda.synchronize()
+            got = ops.linear_w4(x, ops.quantise_w4(weight))
+            got_many = ops.linear_w4(many, ops.quantise_w4(weight, 32))
+            codes = torch.randint(0, 16, (2048, 1024), generator=gen(70 + seed), device=DEV, dtype=torch.uint8)
+            scales = torch.rand(2048, 8, generator=gen(80 + seed), device=DEV).bfloat16()
+            got_packed = ops.linear_w4(x, ops.pack_w4(codes, scales))
+            torch.cuda.synchronize()
+            for weight_of_it, rows, y in ((ops.quantise_w4(weight), x, got), (ops.quantise_w4(weight, 32), many, got_many),
+                                          (ops.pack_w4(codes, scales), x, got_packed)):
+                torch.cuda.synchronize()
+                assert torch.equal(y, ops.linear_w4(rows, weight_of_it))
+    finally:
+        N.set_pdl(before)
+
+
+def test_an_extent_beyond_fp32():
+    """hi - lo infinite in fp32: the group reads back as NaN, its neighbours as what they are."""
+    weight = weight_of(52, 32, 128)
+    weight[3, 5], weight[3, 9] = 3e38, -3e38
+    back = ops.dequantise_w4(ops.quantise_w4(weight, 32))
+    assert back[3, :32].isnan().all()
+    back[3, :32] = 0
+    rest = weight.clone()
+    rest[3, :32] = 0
+    assert torch.equal(back, ops.dequantise_w4(ops.quantise_w4(rest, 32)))
+
+
+@pytest.mark.parametrize("q8", [False, True])
+def test_offsets_beyond_32_bits(q8):
+    """Records of 2.6 GB, results of 3.0e9 elements: the last rows are those of a weight of their own."""
+    n, k = 300000, 16384
+    weight = torch.zeros(n, k, dtype=torch.bfloat16, device=DEV)
+    weight[-48:] = weight_of(53, 48, k)
+    own = ops.quantise_w4(weight[-48:])
+    w = ops.quantise_w4(weight)
+    assert torch.equal(ops.dequantise_w4(w)[-48:], ops.dequantise_w4(own))
+    del weight
+    for rows in (2, 40):
+        x, x64 = rows_of(54, rows, k, q8)
+        y = ops.linear_w4(x, w)
+        assert (y[:, :-48] == 0).all()
+        check(y[:, -48:], x64, ops.dequantise_w4(own, torch.float32).double(), 128)
+    del w
+    small, exact = packed(55, 150000, 64, 64)
+    x, x64 = rows_of(56, 20000, 64, q8)
+    y = ops.linear_w4(x, small)
+    check(y[-3:], x64[-3:], exact, 64)
+    check(y[:, -3:], x64, exact[-3:], 64)
