@@ -8,6 +8,7 @@
 // A block takes up to 256 weight rows, as two halves of 128 lanes, by BN rows of x.  Roles:
 //   warp 0        for 128 columns the records, a bulk copy per run that lies together, and TMA boxes of x, into a ring
 //   warp 1        the products of a group, into one of two accumulators a half
+//   warps 2 and 3 wait for what has no thread behind it (copies, products) and tell those who unpack, and take sums out
 //   warps 4 - 11  unpack, a weight row a thread, into one of two operands a half in TMEM
 //   warps 12 - 19 accumulator out of TMEM, times the row's scale, onto the sums; the results' rows
 // Weight rows are given out in tiles of 16, so that few of them leave no SM idle; a cluster of up to 8 blocks splits the
@@ -15,9 +16,10 @@
 //
 // Bound by the chain of a step of 128 columns (records there, unpacked, products, sums read), whose parts meet at barriers:
 // some 1 us with two halves and 0.65 with one, whatever their tiles, at 40 to 60 % of the issue slots (unpacking and
-// scaling on 16 warps), 15 to 30 % of the tensor pipe, 20 % of the memory's rate.  Measured, 24576 x 4096 in groups of 64: 64
-// rows 34.9 us bf16, 30.7 8-bit; 2048 rows 490 and 513 (0.84 and 0.80 PFLOP/s).  More warps with fewer registers each,
-// warps that both unpack and sum, zeros taken out of the sums instead of the codes: all slower (38, 36 and 40 us for 33).
+// scaling on 16 warps), 15 to 30 % of the tensor pipe, 20 % of the memory's rate.  Measured, 24576 x 4096 in groups of 128: 64
+// rows 30.4 us bf16, 30.3 8-bit (groups of 64: 32.8, 41.2); 2048 rows 490 and 510 (0.84 and 0.81 PFLOP/s).  More warps with
+// fewer registers each, warps that both unpack and sum, words read a step ahead, two blocks an SM with a half each, zeros
+// taken out of the sums instead of the codes: all the same or slower (38, 36, 33, 32 and 40 us for some 31).
 #include <climits>
 
 #include "common.cuh"
@@ -114,12 +116,27 @@ __device__ __forceinline__ float2 sums_of(uint32_t a, uint32_t b) {
 __device__ __forceinline__ void commit(uint32_t bar) {
   asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
 }
-__device__ __forceinline__ void arrive(uint32_t bar) {
-  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
+// The block's barriers of the instruction `bar`, by whole warps: `threads` take part, those who sync also wait.  Sixteen warps
+// that poll an mbarrier each keep the unit that shared memory is read through busy (4 cycles a poll); where one warp polls
+// and tells the others so, 64 rows by 24576 x 4096 in groups of 64 take 32.8 us for 34.7, 200 by 4096 x 4096 21.8 for 23.3.
+// No wait here has a limit, and none needs one: the order below makes every arrival that a wait is for follow from arrivals
+// before it, whether the polls of warps 2 and 3 end well or give up, and no barrier gets arrivals of its next use before
+// this one is over:
+//   kUnpack    warp 2 -> who unpacks: records and x of a step there, its operand free
+//   kProducts  who unpacks (groups of 128: and takes sums out, two steps later) -> warp 1: operand written (sums read)
+//   kToUnpack  warp 1 -> warp 2: products of a step begun; waited for before kUnpack two steps later
+//   kToSums    warp 1 -> warp 3: products of a group issued
+//   kSums      warp 3 -> who takes sums out: a group's sums there
+//   kRead      who takes sums out -> warp 1 (groups of 32 and 64): sums read, two groups later
+__device__ __forceinline__ void bar_sync(int id, int threads) {
+  asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory");
 }
+__device__ __forceinline__ void bar_arrive(int id, int threads) {
+  asm volatile("bar.arrive %0, %1;" ::"r"(id), "r"(threads) : "memory");
+}
+enum Bar { kUnpack = 1, kProducts = 3, kSums = 5, kRead = 7, kToUnpack = 9, kToSums = 11 };  // two of each
 // A whole warp's wait for the phase of parity `parity` (its low bit), bounded like mbar_wait; the clock is first read at
-// the 64th poll.  Even where the phase is over a poll takes some 120 cycles, and polls do not overlap: the loops below
-// are laid out for as few as they can.
+// the 64th poll.
 __device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag, unsigned* err) {
   unsigned long long t0 = 0;
   bool ok = false;
@@ -202,12 +219,10 @@ __global__ void __launch_bounds__(kThreads, 1)
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = smem_raw + (-smem_u32(smem_raw) & 1023u);  // an offset: a cast address would be read as a generic one
   uint64_t* full_at = reinterpret_cast<uint64_t*>(smem);  // [stages] a ring's place filled
-  uint64_t* drain = full_at + 2 * kMaxStages + 8;
+  uint64_t* drain = full_at + 2 * kMaxStages + 4;
   const uint32_t full = smem_u32(smem), empty = full + 8 * kMaxStages;  // [stages] and read
-  const uint32_t a_full = empty + 8 * kMaxStages;  // [2] operands unpacked (groups of 128: and the accumulators read)
-  const uint32_t a_empty = a_full + 16;            // [2] and used (groups of 128: d_full says so)
-  const uint32_t d_full = a_empty + 16;            // [2] a group's sums made
-  const uint32_t d_empty = d_full + 16;            // [2] and read
+  const uint32_t a_empty = empty + 8 * kMaxStages;  // [2] operands used (groups of 128: d_full says so)
+  const uint32_t d_full = a_empty + 16;             // [2] a group's sums made
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
@@ -228,13 +243,11 @@ __global__ void __launch_bounds__(kThreads, 1)
   if (threadIdx.x == 0) {
     for (int i = 0; i < S; ++i) {
       mbar_init(full_at + i, 1);
-      mbar_init(full_at + kMaxStages + i, halves * 4 + 1);
+      mbar_init(full_at + kMaxStages + i, 1);
     }
     for (int i = 0; i < 2; ++i) {
-      mbar_init(full_at + 2 * kMaxStages + i, halves * (PER > 1 ? 4 : 8));
+      mbar_init(full_at + 2 * kMaxStages + i, 1);
       mbar_init(full_at + 2 * kMaxStages + 2 + i, 1);
-      mbar_init(full_at + 2 * kMaxStages + 4 + i, 1);
-      mbar_init(full_at + 2 * kMaxStages + 6 + i, halves * 4);
     }
     mbar_init(drain, 1);
     *abort_flag = 0;
@@ -259,6 +272,9 @@ __global__ void __launch_bounds__(kThreads, 1)
     ++it;
     if (++s == S) s = 0, ph ^= 1;
   };
+  const int steps = mine * nk;
+  const int team = halves * 128;  // threads that unpack, and that take sums out
+  const int products = 32 + team + (PER > 1 ? 0 : team);
   auto wait = [&](uint32_t bar, uint32_t parity) { return warp_wait(bar, parity, abort_flag, a.err); };
   if (warp == 0) {
     // Lanes 0 - 2 each ask for a run of records that lie together (up to three), lanes 3 and 4 for a box of x.
@@ -308,15 +324,17 @@ __global__ void __launch_bounds__(kThreads, 1)
     // The whole warp runs the loops, so that addresses and descriptors stay in uniform registers; one thread issues.
     const bool leader = elect_one();
     for (int n = 0; n < mine; ++n) {
-      for (int kb = 0; kb < nk && ok; ++kb, step()) {
+      for (int kb = 0; kb < nk; ++kb, step()) {
         const uint64_t bd = umma_desc_sw128(smem_u32(sx + s * L::X_STAGE));
         const uint32_t ta = tmem + (it & 1) * 2 * A_COLS;
 #pragma unroll
         for (int g = 0; g < PER; ++g) {
           const int e = it * PER + g;
-          if (g == 0) ok = wait(a_full + 8 * (it & 1), it >> 1);  // x has come too: who unpacked has seen it
-          if (PER > 1) ok = ok && wait(d_empty + 8 * (e & 1), (e >> 1) ^ 1);
-          if (!ok) break;
+          if (g == 0) {
+            bar_sync(kProducts + (it & 1), products);  // x has come too: who unpacked has been told
+            bar_arrive(kToUnpack + (it & 1), 64);
+          }
+          if (PER > 1 && e > 1) bar_sync(kRead + (e & 1), 32 + team);
           tc_fence_after();
           if (leader) {
             const uint32_t td = tmem + 4 * A_COLS + (e & 1) * 2 * BN;
@@ -330,8 +348,28 @@ __global__ void __launch_bounds__(kThreads, 1)
             if (g == PER - 1) commit(empty + 8 * s);
           }
           __syncwarp();
+          bar_arrive(kToSums + (e & 1), 64);
         }
       }
+    }
+  } else if (warp == 2) {
+    for (; it < steps; step()) {
+      if (it > 1) bar_sync(kToUnpack + (it & 1), 64);
+      // The operand's last use: the products of two steps ago.  Groups of 128 columns show it by their sums.
+      ok = ok && wait(full + 8 * s, ph) && wait((PER > 1 ? a_empty : d_full) + 8 * (it & 1), (it >> 1) ^ 1);
+      tc_fence_after();
+      tc_fence_before();
+      bar_sync(kUnpack + (it & 1), 32 + team);
+    }
+    for (int i = steps; i < steps + 2; ++i)
+      if (i > 1) bar_sync(kToUnpack + (i & 1), 64);
+  } else if (warp == 3) {
+    for (int e = 0; e < steps * PER; ++e) {
+      bar_sync(kToSums + (e & 1), 64);
+      ok = ok && wait(d_full + 8 * (e & 1), e >> 1);
+      tc_fence_after();
+      tc_fence_before();
+      bar_sync(kSums + (e & 1), 32 + team);
     }
   } else if (warp >= 4 && warp < 12 && (warp - 4) >> 2 < halves) {
     const int h = (warp - 4) >> 2, q = warp & 3, tile = h * 8 + q * 2;  // a warp's two tiles
@@ -339,10 +377,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     for (int n = 0; n < mine; ++n) {
       const Item item(a, unit + n * units);
       const int offset = min(tile + (lane >> 4), item.count - 1) * L::REC + (lane & 15) * 64;
-      for (int kb = 0; kb < nk && ok; ++kb, step()) {
-        // The operand's last use: the products of two steps ago.  Groups of 128 columns show it by their sums.
-        ok = wait(full + 8 * s, ph) && wait((PER > 1 ? a_empty : d_full) + 8 * (it & 1), (it >> 1) ^ 1);
-        if (!ok) break;
+      for (int kb = 0; kb < nk; ++kb, step()) {
+        bar_sync(kUnpack + (it & 1), 32 + team);
         if (tile < item.count) {
           const uint8_t* row = sw + s * at.w_stage() + offset;
           uint32_t w[4][4], pair[PER];
@@ -388,17 +424,17 @@ __global__ void __launch_bounds__(kThreads, 1)
           tc_fence_before();
         }
         __syncwarp();
-        if (lane == 0) {
-          arrive(a_full + 8 * (it & 1));
-          arrive(empty + 8 * s);
-        }
+        bar_arrive(kProducts + (it & 1), products);
       }
     }
   } else if (warp >= 12 && (warp - 12) >> 2 < halves) {
     const int h = (warp - 12) >> 2, q = warp & 3;
     const int tile = h * 8 + q * 2 + (lane >> 4);  // of the item
     const uint32_t td = tmem + (static_cast<uint32_t>(q * 32) << 16) + 4 * A_COLS + h * BN;
-    if (PER == 1 && lane == 0) arrive(a_full), arrive(a_full + 8);  // nothing to read yet
+    if (PER == 1) {  // nothing to read yet
+      if (steps > 0) bar_arrive(kProducts, products);
+      if (steps > 1) bar_arrive(kProducts + 1, products);
+    }
     for (int n = 0; n < mine; ++n) {
       const Item item(a, unit + n * units);
       const bool some = h * 8 + q * 2 < item.count;
@@ -411,7 +447,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       for (int i = 0; i < BN / 2; ++i) acc[i] = make_float2(0.0f, 0.0f);
       uint32_t pair[PER], next[PER];
       load_words<PER>(next, src);
-      for (int kb = 0; kb < nk && ok; ++kb, step()) {
+      for (int kb = 0; kb < nk; ++kb, step()) {
 #pragma unroll
         for (int g = 0; g < PER; ++g) pair[g] = next[g];
         src += apart;
@@ -419,8 +455,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
         for (int g = 0; g < PER; ++g) {
           const int e = it * PER + g;
-          ok = ok && wait(d_full + 8 * (e & 1), e >> 1);
-          if (!ok) break;
+          bar_sync(kSums + (e & 1), 32 + team);
           tc_fence_after();
           if (some) {
             const float scale = __uint_as_float(pair[g] << 16);
@@ -437,7 +472,10 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
           tc_fence_before();
           __syncwarp();
-          if (lane == 0) arrive((PER > 1 ? d_empty : a_full) + 8 * (e & 1));
+          if (e + 2 < steps * PER) {
+            if (PER > 1) bar_arrive(kRead + (e & 1), 32 + team);
+            else bar_arrive(kProducts + (e & 1), products);
+          }
         }
       }
       const int row0 = item.column * BN, rows = min(BN, a.rows - row0);
