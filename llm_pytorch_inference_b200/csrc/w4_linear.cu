@@ -471,8 +471,8 @@ extern "C" int mvb_linear_w4(void* y, int64_t ldy, const void* x, int64_t ldx, c
   a.pairs = (a.tiles + 1) / 2;
   a.err = device_status_ptr();
   // Few rows here, more on tcgen05.  A bf16 row is three columns of the product here.  8 bf16 rows, here and on tcgen05:
-  // 24576 x 4096 25.8 us and 32.7, 4096 x 4096 10.1 and 15.0, 4096 x 12288 24.6 and 23.0.  20 to 24 rows of 8 bits, here and
-  // there: 24576 x 4096 36.2 and 29.5, 4096 x 4096 18.8 and 14.2, 4096 x 12288 31.2 and 21.2, 2048 x 1024 5.8 and 9.3.
+  // 24576 x 4096 25.8 us and 26.3, 4096 x 4096 10.0 and 13.6, 4096 x 12288 24.4 and 18.8.  16 rows of 8 bits: 21.5 and 24.8,
+  // 11.9 and 13.2, 17.2 and 18.3, 2048 x 1024 5.8 and 9.1; 20 by 24576 x 4096 36.0 and 24.8, 24 by 4096 x 4096 18.6 and 13.4.
   if (rows > (row_scales != nullptr ? 16 : 8)) {
     const W4LinearCall call = {a.y, ldy, x, ldx, row_scales, a.records, a.rows, a.n, a.k, static_cast<int>(group)};
     return w4_gemm(name, call, reinterpret_cast<cudaStream_t>(stream));
