@@ -5,21 +5,23 @@
 // them: bf16 products with fp32 sums, or 8-bit ones with whole sums.  A group's sum is scaled as it leaves TMEM and added
 // up in registers, in 32 bits: no weight and no product is rounded.
 //
-// A block takes up to 256 weight rows, as two halves of 128 lanes, by BN rows of x.  Roles:
+// A block takes up to 256 weight rows, as two halves of 128 lanes, by BN rows of x (32 or 64); or (SPLIT) up to 128 weight
+// rows by 32, 64 or 128, the columns of a step shared by the two sets of warps that unpack, and the rows of x by the two
+// that take sums out.  Roles:
 //   warp 0        for 128 columns the records, a bulk copy per run that lies together, and TMA boxes of x, into a ring
 //   warp 1        the products of a group, into one of two accumulators a half
 //   warps 2 and 3 wait for what has no thread behind it (copies, products) and tell those who unpack, and take sums out
-//   warps 4 - 11  unpack, a weight row a thread, into one of two operands a half in TMEM
+//   warps 4 - 11  unpack, a weight row (or half of its columns) a thread, into one of two operands a half in TMEM
 //   warps 12 - 19 accumulator out of TMEM, times the row's scale, onto the sums; the results' rows
 // Weight rows are given out in tiles of 16, so that few of them leave no SM idle; a cluster of up to 8 blocks splits the
 // columns where there are fewer, and its sums meet in distributed shared memory in the order of the blocks.
 //
-// Bound by the chain of a step of 128 columns (records there, unpacked, products, sums read), whose parts meet at barriers:
-// some 1 us with two halves and 0.65 with one, whatever their tiles, at 40 to 60 % of the issue slots (unpacking and
-// scaling on 16 warps), 15 to 30 % of the tensor pipe, 20 % of the memory's rate.  Measured, 24576 x 4096 in groups of 128: 64
-// rows 30.4 us bf16, 30.3 8-bit (groups of 64: 32.8, 41.2); 2048 rows 490 and 510 (0.84 and 0.81 PFLOP/s).  More warps with
-// fewer registers each, warps that both unpack and sum, words read a step ahead, two blocks an SM with a half each, zeros
-// taken out of the sums instead of the codes: all the same or slower (38, 36, 33, 32 and 40 us for some 31).
+// Bound by the chain of a step of 128 columns (words read, unpacked and stored to TMEM, products, sums read and scaled),
+// whose parts meet at barriers: 0.4 to 0.7 us in groups of 128 whatever the tiles, at 40 to 60 % of the issue slots, 15 to 30 % of
+// the tensor pipe and 20 % of the memory's rate for 64 rows.  Measured, 24576 x 4096 in groups of 128: 64 rows 30.4 us bf16, 30.3
+// 8-bit (groups of 64: 32.8, 41.2); 2048 rows 361 and 426 (1.14 and 0.97 PFLOP/s).  More warps with fewer registers each, warps
+// that both unpack and sum, words read a step ahead, two blocks an SM with a half each, zeros taken out of the sums instead of
+// the codes: all the same or slower (38, 36, 33, 32 and 40 us for some 31).
 #include <climits>
 
 #include "common.cuh"
@@ -31,7 +33,6 @@ namespace mvb {
 namespace {
 
 constexpr int kThreads = 640;
-constexpr int kMaxTiles = 16;  // 16-row tiles of a block
 constexpr int kMaxStages = 8;
 constexpr int kMaxCluster = 8;
 constexpr size_t kMostSmem = 227 * 1024;
@@ -179,10 +180,18 @@ __device__ __forceinline__ void copy_bulk(void* dst, const void* src, uint32_t b
 }
 
 // Shared memory: barriers; the ring of x boxes; the ring of records; the cluster's sums.
-template <bool Q8, int GROUP, int BN>
+template <bool Q8, int GROUP, int BN, bool SPLIT>
 struct Layout {
   static constexpr int PER = kW4Cols / GROUP;
   static constexpr int REC = w4_record_bytes(GROUP);
+  // 16-row tiles of a block: up to 8, or above that
+  static constexpr int LEAST = SPLIT ? 1 : 9, MOST = SPLIT ? 8 : 16;
+  // What a step of 128 columns takes, in us, measured with a wave of blocks and 16 and 48 steps.
+  static constexpr double step_us() {
+    constexpr double bf16[3][5] = {{0.58, 0.69, 0.41, 0.39, 0.45}, {0.60, 0.77, 0.40, 0.41, 0.55}, {0.87, 1.26, 0.60, 0.64, 0.96}};
+    constexpr double q8[3][5] = {{0.54, 0.66, 0.37, 0.40, 0.53}, {0.62, 1.07, 0.42, 0.54, 0.89}, {1.05, 2.01, 0.67, 0.96, 1.69}};
+    return (Q8 ? q8 : bf16)[PER >> 1][(SPLIT ? 2 : 0) + (BN >> 6)];
+  }
   static constexpr int BOX = BN * 128;              // bytes of a box of x: 128 of each row
   static constexpr int X_STAGE = BOX * (Q8 ? 1 : 2);
   static constexpr int FIXED = 1024;
@@ -206,16 +215,19 @@ struct Item {
   }
 };
 
-template <bool Q8, int GROUP, int BN>
+template <bool Q8, int GROUP, int BN, bool SPLIT>
 __global__ void __launch_bounds__(kThreads, 1)
     w4_gemm_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ GemmW4Args a) {
-  using L = Layout<Q8, GROUP, BN>;
+  using L = Layout<Q8, GROUP, BN, SPLIT>;
   constexpr int PER = L::PER;
   constexpr int KSTEPS = Q8 ? 4 : 8;           // steps of 32 bytes of x in 128 columns
   constexpr int A_COLS = Q8 ? 32 : 64;         // TMEM columns of an operand
   constexpr uint32_t IDESC = Q8 ? umma_idesc_s8(128, BN) : umma_idesc_bf16(128, BN);
-  constexpr uint32_t TMEM_COLS = 512;          // a power of two above 4 operands and 4 accumulators
-  static_assert(4 * A_COLS + 4 * BN <= 512, "TMEM");
+  constexpr int HALVES = SPLIT ? 1 : 2;         // of 128 weight rows
+  constexpr int WORDS = SPLIT ? 2 : 4;          // words of each 16 bytes of a row that a thread unpacks
+  constexpr int CN = SPLIT ? BN / 2 : BN;       // rows of x whose sums a thread takes
+  constexpr uint32_t TMEM_COLS = 512;          // a power of two above two operands and two accumulators a half
+  static_assert(2 * HALVES * (A_COLS + BN) <= 512, "TMEM");
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = smem_raw + (-smem_u32(smem_raw) & 1023u);  // an offset: a cast address would be read as a generic one
   uint64_t* full_at = reinterpret_cast<uint64_t*>(smem);  // [stages] a ring's place filled
@@ -234,7 +246,6 @@ __global__ void __launch_bounds__(kThreads, 1)
   uint8_t* sw = smem + at.w();
   float* part = reinterpret_cast<float*>(smem + at.part());  // [BN][16 chunk]
   const int S = a.stages;
-  const int halves = a.chunk > 8 ? 2 : 1;
   const int items = a.chunks * a.columns;
   const int mine = unit < items ? (items - unit + units - 1) / units : 0;
   const int block0 = static_cast<int>(static_cast<int64_t>(rank) * a.blocks / c);
@@ -273,8 +284,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (++s == S) s = 0, ph ^= 1;
   };
   const int steps = mine * nk;
-  const int team = halves * 128;  // threads that unpack, and that take sums out
-  const int products = 32 + team + (PER > 1 ? 0 : team);
+  constexpr int team = 256;  // threads that unpack, and that take sums out
+  constexpr int products = 32 + team + (PER > 1 ? 0 : team);
   auto wait = [&](uint32_t bar, uint32_t parity) { return warp_wait(bar, parity, abort_flag, a.err); };
   if (warp == 0) {
     // Lanes 0 - 2 each ask for a run of records that lie together (up to three), lanes 3 and 4 for a box of x.
@@ -326,7 +337,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     for (int n = 0; n < mine; ++n) {
       for (int kb = 0; kb < nk; ++kb, step()) {
         const uint64_t bd = umma_desc_sw128(smem_u32(sx + s * L::X_STAGE));
-        const uint32_t ta = tmem + (it & 1) * 2 * A_COLS;
+        const uint32_t ta = tmem + (it & 1) * HALVES * A_COLS;
 #pragma unroll
         for (int g = 0; g < PER; ++g) {
           const int e = it * PER + g;
@@ -337,8 +348,8 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (PER > 1 && e > 1) bar_sync(kRead + (e & 1), 32 + team);
           tc_fence_after();
           if (leader) {
-            const uint32_t td = tmem + 4 * A_COLS + (e & 1) * 2 * BN;
-            for (int h = 0; h < halves; ++h)
+            const uint32_t td = tmem + HALVES * (2 * A_COLS + (e & 1) * BN);
+            for (int h = 0; h < HALVES; ++h)
 #pragma unroll
               for (int k = g * KSTEPS / PER; k < (g + 1) * KSTEPS / PER; ++k)
                 umma_ts<Q8>(td + h * BN, ta + h * A_COLS + 8 * k, bd + (k & 3) * 2 + (k >> 2) * (L::BOX >> 4), IDESC,
@@ -371,8 +382,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       tc_fence_before();
       bar_sync(kSums + (e & 1), 32 + team);
     }
-  } else if (warp >= 4 && warp < 12 && (warp - 4) >> 2 < halves) {
-    const int h = (warp - 4) >> 2, q = warp & 3, tile = h * 8 + q * 2;  // a warp's two tiles
+  } else if (warp >= 4 && warp < 12) {
+    const int h = (warp - 4) >> 2, q = warp & 3, tile = (SPLIT ? 0 : h * 8) + q * 2;  // a warp's two tiles
     const uint32_t lanes = static_cast<uint32_t>(q * 32) << 16;
     for (int n = 0; n < mine; ++n) {
       const Item item(a, unit + n * units);
@@ -381,20 +392,26 @@ __global__ void __launch_bounds__(kThreads, 1)
         bar_sync(kUnpack + (it & 1), 32 + team);
         if (tile < item.count) {
           const uint8_t* row = sw + s * at.w_stage() + offset;
-          uint32_t w[4][4], pair[PER];
+          constexpr int PAIRS = PER * WORDS > 4 ? PER * WORDS / 4 : 1;
+          uint32_t w[WORDS][4], pair[PAIRS];
 #pragma unroll
           for (int t = 0; t < 4; ++t) {
-            const uint4 v = *reinterpret_cast<const uint4*>(row + w4_place(t, lane) * 16);
-            w[0][t] = v.x, w[1][t] = v.y, w[2][t] = v.z, w[3][t] = v.w;
+            if (SPLIT) {
+              const uint2 v = *reinterpret_cast<const uint2*>(row + w4_place(t, lane) * 16 + h * 8);
+              w[0][t] = v.x, w[1][t] = v.y;
+            } else {
+              const uint4 v = *reinterpret_cast<const uint4*>(row + w4_place(t, lane) * 16);
+              w[0][t] = v.x, w[1][t] = v.y, w[2 % WORDS][t] = v.z, w[3 % WORDS][t] = v.w;
+            }
           }
           const uint32_t* pairs = reinterpret_cast<const uint32_t*>(row - (lane & 15) * (64 - PER * 4) + kW4CodeBytes);
 #pragma unroll
-          for (int g = 0; g < PER; ++g) pair[g] = pairs[g];
+          for (int g = 0; g < PAIRS; ++g) pair[g] = pairs[g + (SPLIT ? h * PER / 2 : 0)];
           tc_fence_after();
-          const uint32_t ta = tmem + lanes + ((it & 1) * 2 + h) * A_COLS;
+          const uint32_t ta = tmem + lanes + (SPLIT ? (it & 1) * A_COLS + h * (A_COLS / 2) : ((it & 1) * 2 + h) * A_COLS);
           if (Q8) {
 #pragma unroll
-            for (int i = 0; i < 4; i += 2) {
+            for (int i = 0; i < WORDS; i += 2) {
               uint32_t o[16];
 #pragma unroll
               for (int z = 0; z < 2; ++z) {
@@ -410,7 +427,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
           } else {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
+            for (int i = 0; i < WORDS; ++i) {
               const uint32_t z2 = __byte_perm(pair[i * PER / 4], 0, 0x3232);
               uint32_t o[16];
 #pragma unroll
@@ -427,24 +444,25 @@ __global__ void __launch_bounds__(kThreads, 1)
         bar_arrive(kProducts + (it & 1), products);
       }
     }
-  } else if (warp >= 12 && (warp - 12) >> 2 < halves) {
+  } else {
     const int h = (warp - 12) >> 2, q = warp & 3;
-    const int tile = h * 8 + q * 2 + (lane >> 4);  // of the item
-    const uint32_t td = tmem + (static_cast<uint32_t>(q * 32) << 16) + 4 * A_COLS + h * BN;
+    const int tile = (SPLIT ? 0 : h * 8) + q * 2 + (lane >> 4);  // of the item
+    const int first = SPLIT ? h * CN : 0;                        // row of x of the item
+    const uint32_t td = tmem + (static_cast<uint32_t>(q * 32) << 16) + HALVES * 2 * A_COLS + (SPLIT ? first : h * BN);
     if (PER == 1) {  // nothing to read yet
       if (steps > 0) bar_arrive(kProducts, products);
       if (steps > 1) bar_arrive(kProducts + 1, products);
     }
     for (int n = 0; n < mine; ++n) {
       const Item item(a, unit + n * units);
-      const bool some = h * 8 + q * 2 < item.count;
+      const bool some = (SPLIT ? 0 : h * 8) + q * 2 < item.count;
       // The rows' scales come straight from memory, a step ahead: no wait for the ring.
       const int at_tile = item.tile + min(tile, item.count - 1);
       const uint8_t* src = a.records + w4_record(at_tile, block0, a.tiles, a.blocks) * L::REC + kW4CodeBytes + (lane & 15) * PER * 4;
       const int64_t apart = static_cast<int64_t>(min(8, a.tiles - (at_tile & ~7))) * L::REC;
-      float2 acc[BN / 2];
+      float2 acc[CN / 2];
 #pragma unroll
-      for (int i = 0; i < BN / 2; ++i) acc[i] = make_float2(0.0f, 0.0f);
+      for (int i = 0; i < CN / 2; ++i) acc[i] = make_float2(0.0f, 0.0f);
       uint32_t pair[PER], next[PER];
       load_words<PER>(next, src);
       for (int kb = 0; kb < nk; ++kb, step()) {
@@ -461,9 +479,9 @@ __global__ void __launch_bounds__(kThreads, 1)
             const float scale = __uint_as_float(pair[g] << 16);
             const float2 s2 = make_float2(scale, scale);
 #pragma unroll
-            for (int c0 = 0; c0 < BN; c0 += 16) {
+            for (int c0 = 0; c0 < CN; c0 += 16) {
               uint32_t d[16];
-              tmem_ld_x16(td + (e & 1) * 2 * BN + c0, d);
+              tmem_ld_x16(td + (e & 1) * HALVES * BN + c0, d);
               tmem_ld_wait();
 #pragma unroll
               for (int i = 0; i < 16; i += 2)
@@ -478,16 +496,16 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
         }
       }
-      const int row0 = item.column * BN, rows = min(BN, a.rows - row0);
+      const int row0 = item.column * BN + first, rows = min(CN, a.rows - row0);
       const int col = (item.tile + tile) * kW4Rows + (lane & 15);
       int width = a.chunk * kW4Rows;
       int64_t ldy = a.ldy;
       asm volatile("" : "+r"(width), "+l"(ldy));  // not known outside: or all their multiples are kept, in local memory
       if (c > 1) {
         if (tile < item.count) {
-          float* to = part + tile * kW4Rows + (lane & 15);
+          float* to = part + first * width + tile * kW4Rows + (lane & 15);
 #pragma unroll
-          for (int i = 0; i < BN; ++i) {
+          for (int i = 0; i < CN; ++i) {
             if (i < rows) *to = i & 1 ? acc[i / 2].y : acc[i / 2].x;
             to += width;
           }
@@ -496,7 +514,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         __nv_bfloat16* y = a.y + row0 * a.ldy + col;
         const float* scales = a.a + row0;
 #pragma unroll
-        for (int i = 0; i < BN; ++i) {
+        for (int i = 0; i < CN; ++i) {
           const float v = i & 1 ? acc[i / 2].y : acc[i / 2].x;
           if (i < rows) *y = __float2bfloat16_rn(Q8 ? v * __ldg(scales + i) : v);
           y += ldy;
@@ -541,39 +559,56 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
 }
 
-template <bool Q8, int GROUP, int BN>
-int run(const char* name, const W4LinearCall& call, cudaStream_t stream) {
-  using L = Layout<Q8, GROUP, BN>;
-  const int sms = current_sm_count();
-  MVB_REQUIRE(sms > 0, "%s: no device", name);
-  auto kernel = w4_gemm_kernel<Q8, GROUP, BN>;
+// What a call is made of: tiles of an item and blocks of a cluster, and what that is taken to cost, in us: a step takes the same
+// whatever its tiles, an item 0.5 besides, a cluster's meeting 3.3.  Of what comes out alike the smallest items.
+struct Plan {
+  double cost;
+  int cluster, chunk;
+};
+
+template <bool Q8, int GROUP, int BN, bool SPLIT>
+int units_of(int c, int sms) {
+  static std::atomic<int> clusters[kMaxCluster + 1] = {};
+  return c == 1 ? sms : clusters_at_once(clusters[c], w4_gemm_kernel<Q8, GROUP, BN, SPLIT>, c, kThreads, kMostSmem);
+}
+
+template <bool Q8, int GROUP, int BN, bool SPLIT>
+int prepare(const char* name) {
   static std::atomic<uint64_t> done{0};
-  MVB_TRY(set_smem_once(done, kernel, kMostSmem, name));
+  return set_smem_once(done, w4_gemm_kernel<Q8, GROUP, BN, SPLIT>, kMostSmem, name);
+}
+
+template <bool Q8, int GROUP, int BN, bool SPLIT>
+Plan plan_of(const W4LinearCall& call, int sms) {
+  using L = Layout<Q8, GROUP, BN, SPLIT>;
+  const int tiles = (call.n + kW4Rows - 1) / kW4Rows, blocks = (call.k + kW4Cols - 1) / kW4Cols;
+  const int columns = (call.rows + BN - 1) / BN;
+  Plan best = {0, 0, 0};
+  for (int c = 1; c <= kMaxCluster && c <= blocks; ++c) {
+    const int units = units_of<Q8, GROUP, BN, SPLIT>(c, sms);
+    for (int chunk = L::LEAST; chunk <= L::MOST && chunk <= tiles; ++chunk) {
+      const int64_t items = static_cast<int64_t>((tiles + chunk - 1) / chunk) * columns;
+      if (c > 1 && items > units) continue;  // a cluster meets once
+      const double waves = static_cast<double>((items + units - 1) / units);
+      const double cost = waves * ((blocks + c - 1) / c * L::step_us() + 0.5) + (c > 1 ? 3.3 : 0.0);
+      if (best.chunk == 0 || cost < best.cost) best = {cost, c, chunk};
+    }
+  }
+  return best;
+}
+
+template <bool Q8, int GROUP, int BN, bool SPLIT>
+int run(const char* name, const W4LinearCall& call, const Plan& plan, int sms, cudaStream_t stream) {
+  using L = Layout<Q8, GROUP, BN, SPLIT>;
+  auto kernel = w4_gemm_kernel<Q8, GROUP, BN, SPLIT>;
   GemmW4Args a = {};
   a.y = call.y, a.ldy = call.ldy, a.a = call.row_scales, a.records = call.records, a.rows = call.rows, a.n = call.n;
   a.tiles = (call.n + kW4Rows - 1) / kW4Rows;
   a.blocks = (call.k + kW4Cols - 1) / kW4Cols;
   a.columns = (call.rows + BN - 1) / BN;
   a.err = device_status_ptr();
-  // Tiles of an item and blocks of a cluster, by what a step of 128 columns takes (in us: 0.65 with one half, 1.0 with
-  // two, whatever their tiles; a group more 0.22 or 0.25) and what an item does besides (0.5; in a cluster 6).
-  // Of what comes out alike the smallest items.
-  static std::atomic<int> clusters[kMaxCluster + 1] = {};
-  auto units_of = [&](int c) {
-    return c == 1 ? sms : clusters_at_once(clusters[c], kernel, c, kThreads, kMostSmem);
-  };
-  double least = 0;
-  for (int c = 1; c <= kMaxCluster && c <= a.blocks; ++c) {
-    const int units = units_of(c);
-    for (int chunk = 1; chunk <= kMaxTiles && chunk <= a.tiles; ++chunk) {
-      const int64_t items = static_cast<int64_t>((a.tiles + chunk - 1) / chunk) * a.columns;
-      if (c > 1 && items > units) continue;  // a cluster meets once
-      const double waves = static_cast<double>((items + units - 1) / units);
-      const double step = chunk > 8 ? 0.75 + 0.25 * L::PER : 0.43 + 0.22 * L::PER;
-      const double cost = waves * ((a.blocks + c - 1) / c * step + (c > 1 ? 6.0 : 0.5));
-      if (a.chunk == 0 || cost < least) least = cost, a.cluster = c, a.chunk = chunk;
-    }
-  }
+  a.cluster = plan.cluster;
+  a.chunk = plan.chunk;
   a.chunks = (a.tiles + a.chunk - 1) / a.chunk;
   L at = {a.chunk, kMaxStages, a.cluster > 1};
   while (at.bytes() > kMostSmem) --at.stages;
@@ -582,7 +617,7 @@ int run(const char* name, const W4LinearCall& call, cudaStream_t stream) {
   // another: a second would wait for the first one's TMEM, and where both are of one cluster the first for the second.
   const size_t smem = at.bytes() > 120 * 1024 ? at.bytes() : 120 * 1024;
   const int64_t items = static_cast<int64_t>(a.chunks) * a.columns;
-  const int units = items < units_of(a.cluster) ? static_cast<int>(items) : units_of(a.cluster);
+  const int most = units_of<Q8, GROUP, BN, SPLIT>(a.cluster, sms), units = items < most ? static_cast<int>(items) : most;
 
   CUtensorMap tm;
   const uint64_t dims[2] = {static_cast<uint64_t>(call.k), static_cast<uint64_t>(call.rows)};
@@ -596,10 +631,26 @@ int run(const char* name, const W4LinearCall& call, cudaStream_t stream) {
                         stream, tm, a);
 }
 
+template <bool Q8, int GROUP, int BN>
+int run_either(const char* name, const W4LinearCall& call, int sms, cudaStream_t stream) {
+  MVB_TRY((prepare<Q8, GROUP, BN, true>(name)));
+  MVB_TRY((prepare<Q8, GROUP, BN, false>(name)));
+  const Plan one = plan_of<Q8, GROUP, BN, true>(call, sms), two = plan_of<Q8, GROUP, BN, false>(call, sms);
+  if (two.chunk == 0 || one.cost <= two.cost) return run<Q8, GROUP, BN, true>(name, call, one, sms, stream);
+  return run<Q8, GROUP, BN, false>(name, call, two, sms, stream);
+}
+
 template <bool Q8, int GROUP>
 int run_rows(const char* name, const W4LinearCall& call, cudaStream_t stream) {
-  // Half the accumulators to read out where they hold all rows.
-  return call.rows <= 32 ? run<Q8, GROUP, 32>(name, call, stream) : run<Q8, GROUP, 64>(name, call, stream);
+  const int sms = current_sm_count();
+  MVB_REQUIRE(sms > 0, "%s: no device", name);
+  // As few columns as hold all rows, with as many weight rows as come out cheaper: 64 by 24576 x 4096 takes 33.0 us with up to 16 tiles
+  // and 36.5 with up to 8, 64 by 4096 x 4096 14.6 and 13.4.  Above 64 rows half the weight rows by twice the columns, so that
+  // half is unpacked: 2048 by 24576 x 4096 361 us for 490 (8 bits: 426 for 512), 128 rows 37.7 for 49.1.
+  if (call.rows <= 32) return run_either<Q8, GROUP, 32>(name, call, sms, stream);
+  if (call.rows <= 64) return run_either<Q8, GROUP, 64>(name, call, sms, stream);
+  MVB_TRY((prepare<Q8, GROUP, 128, true>(name)));
+  return run<Q8, GROUP, 128, true>(name, call, plan_of<Q8, GROUP, 128, true>(call, sms), sms, stream);
 }
 
 template <bool Q8>
