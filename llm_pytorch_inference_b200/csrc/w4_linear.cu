@@ -423,7 +423,8 @@ template <int GROUP, int P>
 int run_rows(const char* name, const LinearArgs& a, cudaStream_t stream) {
   // as many columns of the product as the rows need, where x then fits into a cluster's shared memory
   const int need = (a.rows * P + 7) / 8;
-  if (need > 2 && fits<GROUP, P, 3>(a)) return run<GROUP, P, 3>(name, a, stream);
+  if constexpr (P == 3)
+    if (need > 2 && fits<GROUP, P, 3>(a)) return run<GROUP, P, 3>(name, a, stream);
   if (need > 1 && fits<GROUP, P, 2>(a)) return run<GROUP, P, 2>(name, a, stream);
   return run<GROUP, P, 1>(name, a, stream);
 }
@@ -471,9 +472,11 @@ extern "C" int mvb_linear_w4(void* y, int64_t ldy, const void* x, int64_t ldx, c
   a.pairs = (a.tiles + 1) / 2;
   a.err = device_status_ptr();
   // Few rows here, more on tcgen05.  A bf16 row is three columns of the product here.  8 bf16 rows, here and on tcgen05:
-  // 24576 x 4096 25.8 us and 26.3, 4096 x 4096 10.0 and 13.6, 4096 x 12288 24.4 and 18.8.  16 rows of 8 bits: 21.5 and 24.8,
-  // 11.9 and 13.2, 17.2 and 18.3, 2048 x 1024 5.8 and 9.1; 20 by 24576 x 4096 36.0 and 24.8, 24 by 4096 x 4096 18.6 and 13.4.
-  if (rows > (row_scales != nullptr ? 16 : 8)) {
+  // 24576 x 4096 25.9 us and 26.2, 12288 x 4096 15.5 and 19.8, 4096 x 8192 15.1 and 16.8; but 4096 x 12288 24.7 and 19.6, 3584 x
+  // 14336 29.6 and 19.0, because the columns of 6 rows and more leave too little shared memory there for a block by itself (5
+  // rows: 13.8 and 19.5, 17.1 and 18.6).  16 rows of 8 bits: 24576 x 4096 21.5 and 24.8, 4096 x 12288 17.4 and 19.1, 2048 x 1024
+  // 5.8 and 9.1; 20 by 24576 x 4096 36.0 and 24.8, 24 by 4096 x 4096 18.6 and 13.4.
+  if (rows > (row_scales != nullptr ? 16 : k > 8192 ? 5 : 8)) {
     const W4LinearCall call = {a.y, ldy, x, ldx, row_scales, a.records, a.rows, a.n, a.k, static_cast<int>(group)};
     return w4_gemm(name, call, reinterpret_cast<cudaStream_t>(stream));
   }

@@ -1097,8 +1097,8 @@ def dequantise_w4(weight: W4Weight, dtype: torch.dtype = torch.bfloat16) -> torc
 def linear_w4(x: torch.Tensor | Q8Rows, weight: W4Weight, out: torch.Tensor | None = None) -> torch.Tensor:
     """``linear`` with a 4-bit weight: ``x @ w.T`` (bf16) for bf16 rows ``[..., k]`` or rows in 8 bits (``Q8Rows``), one
     row (of at most 262144) to many.  Sums run in 32 bits and are rounded once; no weight or product is rounded before.
-    k is at most 32768.  A bf16 row with an infinity or a NaN has results that are not finite (NaN where there are 8
-    rows or fewer), and leaves the other rows alone.  ``out``: bf16 ``[rows, n]`` with contiguous rows, and then what is
+    k is at most 32768.  A bf16 row with an infinity or a NaN has results that are not finite (NaN in calls
+    of few rows), and leaves the other rows alone.  ``out``: bf16 ``[rows, n]`` with contiguous rows, and then what is
     returned; it must not overlap ``x``."""
     what = "linear_w4"
     index = _check_w4(what, weight)

@@ -251,3 +251,24 @@ def test_offsets_beyond_32_bits():
         back = ops.dequantise_q8(got)
         assert torch.equal(back[-5:], ops.dequantise_q8(ops.Q8Rows(got.values[-5:], got.scales[-5:])))
         assert not back[:-5].any()
+
+
+@pytest.mark.parametrize("rows, width", [(1, 8191), (400, 8193), (2, 16385), (600, 4099), (3, 32767), (1, 32769), (310, 32773),
+                                         (5, 8192), (2, 16384), (700, 16392)])
+def test_rows_that_do_not_begin_on_16_bytes(rows, width):
+    """Single elements, 8, 16 or 32 a thread, or worked out twice: what the aligned copy gives where there is one."""
+    g = torch.Generator(device=DEV).manual_seed(width)
+    base = torch.randn(2 * rows * width + 16, generator=g, device=DEV).bfloat16()
+    x, z = base[1:1 + rows * width].view(rows, width), base[3 + rows * width:3 + 2 * rows * width].view(rows, width)
+    weight = (1 + 0.2 * torch.randn(width + 1, generator=g, device=DEV)).bfloat16()[1:]
+    h = (x.float() + z.float()).bfloat16()
+    y = h.double() * weight.double()
+    rstd = 1 / (h.double().square().mean(-1) + 1e-6).sqrt()
+    got, residual = ops.fused_add_rmsnorm_q8(x.clone(), z, weight)
+    assert torch.equal(residual, h)
+    check(got, y, R.q8(y)[1] * rstd, True, 0.0)
+    plain = ops.quantise_q8(x)
+    check(plain, x.double(), R.q8(x.double())[1], True, 0.0)
+    assert torch.equal(ops.dequantise_q8(plain), (plain.values.float() * plain.scales[:, None]).bfloat16())
+    act = x.double() * torch.sigmoid(x.double()) * z.double()
+    check(ops.swiglu_q8(x, z), act, R.q8(act)[1], False, gated_off(x, z, act, False))

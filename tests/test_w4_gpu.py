@@ -486,3 +486,17 @@ def test_offsets_beyond_32_bits(q8):
     y = ops.linear_w4(x, small)
     check(y[-3:], x64[-3:], exact, 64)
     check(y[:, -3:], x64, exact[-3:], 64)
+
+
+@pytest.mark.parametrize("rows, n, k, group, q8", [
+    (5, 40, 12288, 128, False), (6, 40, 12288, 128, False), (8, 600, 8192, 64, False), (8, 600, 8224, 32, False),
+    (16, 100, 32768, 128, True), (17, 2400, 1024, 64, True), (65, 2000, 1024, 32, False), (128, 2500, 544, 128, True),
+    (129, 130, 4096, 64, False), (300, 1000, 4096, 32, True), (64, 24576, 256, 64, False), (30, 24576, 288, 32, True),
+    (640, 4096, 512, 128, False), (1100, 136, 2048, 64, True),
+])
+def test_either_side_of_every_choice_of_kernel(rows, n, k, group, q8):
+    """Few rows and more by rows and k, one or two halves of weight rows, 32, 64 or 128 rows of x, columns split or not."""
+    w, exact = packed(rows + n, n, k, group)
+    x, x64 = rows_of(rows, rows, k, q8)
+    check(ops.linear_w4(x, w), x64, exact, group)
+    assert N.device_status() == 0
