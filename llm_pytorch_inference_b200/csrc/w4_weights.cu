@@ -150,7 +150,7 @@ __global__ void __launch_bounds__(kThreads) quantise_w4_kernel(uint8_t* __restri
       *reinterpret_cast<uint32_t*>(rec + kW4CodeBytes + (row * PER + part / LANES) * 4) = some ? pair : 0u;
     }
   }
-  __threadfence();
+  fence_acq_rel_gpu();
 }
 
 template <int GROUP>
@@ -188,7 +188,7 @@ __global__ void __launch_bounds__(kThreads) pack_w4_kernel(uint8_t* __restrict__
       *reinterpret_cast<uint32_t*>(rec + kW4CodeBytes + (row * PER + part / LANES) * 4) = pair;
     }
   }
-  __threadfence();
+  fence_acq_rel_gpu();
 }
 
 template <int GROUP, typename T>
