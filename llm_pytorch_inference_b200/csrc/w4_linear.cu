@@ -24,6 +24,7 @@
 // 4096 x 4096 6.35, 2048 x 1024 4.6.  The long ones stream; 24576 x 4096 gives an SM 5 or 6 pairs and issues in 48 % of
 // the slots on average, start and end included; the short ones are their launch, x and a chain of latencies.
 #include <climits>
+#include <type_traits>
 
 #include "common.cuh"
 #include "host.h"
@@ -120,59 +121,71 @@ __device__ __forceinline__ void stage_x(uint8_t* sx, Info* info, const LinearArg
   constexpr int LANES = GROUP / 8;
   const int chunks = blocks * 16, rows = min(L::ROWS, a.rows - row0), n = rows * chunks;
   const int lane = threadIdx.x & 31;
+  // 8-bit rows: four chunks a thread are asked for at a time (16 by 4096 x 4096 11.8 us for one, 10.5 for four).  Taking a
+  // bf16 row apart is longer than its wait, and four were the same.
+  using Raw = std::conditional_t<P == 1, uint2, uint4>;
+  constexpr int AHEAD = P == 1 ? 4 : 1;
+  Raw raw[AHEAD];
 #pragma unroll 1
-  for (int i0 = threadIdx.x & ~31; i0 < n; i0 += kThreads) {  // whole warps, for the exchanges
-    const int i = i0 + lane, m = i / chunks, c = i - m * chunks;
-    const int col = block0 * kW4Cols + 8 * c;
-    const bool some = i < n && col < a.k;
-    uint32_t q[P][2];
-    float scale = 1.0f;
-    if (P == 1) {
-      uint2 v = make_uint2(0, 0);
-      if (some) v = *reinterpret_cast<const uint2*>(static_cast<const int8_t*>(a.x) + (row0 + m) * a.ldx + col);
-      q[0][0] = v.x, q[0][1] = v.y;
-    } else {
-      uint4 v = make_uint4(0, 0, 0, 0);
-      if (some) v = *reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(a.x) + (row0 + m) * a.ldx + col);
-      const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-      uint32_t top = 0;
+  for (int first = threadIdx.x & ~31; first < n; first += AHEAD * kThreads) {  // whole warps, for the exchanges
 #pragma unroll
-      for (int e = 0; e < 4; ++e) top = max(top, max(w[e] << 16 & 0x7fff0000u, w[e] & 0x7fff0000u));
+    for (int u = 0; u < AHEAD; ++u) {
+      const int i = first + u * kThreads + lane, m = i / chunks, c = i - m * chunks;
+      const int col = block0 * kW4Cols + 8 * c;
+      raw[u] = Raw{};
+      if (i < n && col < a.k)
+        raw[u] = *reinterpret_cast<const Raw*>(static_cast<const uint8_t*>(a.x) + ((row0 + m) * a.ldx + col) * (P == 1 ? 1 : 2));
+    }
 #pragma unroll
-      for (int o = LANES / 2; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
-      // 2^(E - 5), and its reciprocal; below 2^-105 nothing is told apart
-      const uint32_t exponent = max(top >> 23, 22u);
-      scale = top == 0 ? 0.0f : __uint_as_float((exponent - 5) << 23);
-      const float inv = __uint_as_float((259 - exponent) << 23);
-      const bool fine = top < 0x7f800000u;
-      if (!fine) scale = __uint_as_float(0x7fc00000u);
-      constexpr float kMagic = 12582912.0f;
-      float p[3][8];
+    for (int u = 0; u < AHEAD; ++u) {
+      const int i0 = first + u * kThreads;
+      if (i0 >= n) break;
+      const int i = i0 + lane, m = i / chunks, c = i - m * chunks;
+      uint32_t q[P][2];
+      float scale = 1.0f;
+      if constexpr (P == 1) {
+        q[0][0] = raw[u].x, q[0][1] = raw[u].y;
+      } else {
+        const uint32_t w[4] = {raw[u].x, raw[u].y, raw[u].z, raw[u].w};
+        uint32_t top = 0;
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const float y = fine ? __uint_as_float(e & 1 ? w[e >> 1] & 0xffff0000u : w[e >> 1] << 16) * inv : 0.0f;
-        p[0][e] = y + kMagic;
-        const float r = (y - (p[0][e] - kMagic)) * 128.0f;
-        p[1][e] = r + kMagic;
-        p[2][e] = (r - (p[1][e] - kMagic)) * 128.0f + kMagic;
+        for (int e = 0; e < 4; ++e) top = max(top, max(w[e] << 16 & 0x7fff0000u, w[e] & 0x7fff0000u));
+#pragma unroll
+        for (int o = LANES / 2; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+        // 2^(E - 5), and its reciprocal; below 2^-105 nothing is told apart
+        const uint32_t exponent = max(top >> 23, 22u);
+        scale = top == 0 ? 0.0f : __uint_as_float((exponent - 5) << 23);
+        const float inv = __uint_as_float((259 - exponent) << 23);
+        const bool fine = top < 0x7f800000u;
+        if (!fine) scale = __uint_as_float(0x7fc00000u);
+        constexpr float kMagic = 12582912.0f;
+        float p[3][8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const float y = fine ? __uint_as_float(e & 1 ? w[e >> 1] & 0xffff0000u : w[e >> 1] << 16) * inv : 0.0f;
+          p[0][e] = y + kMagic;
+          const float r = (y - (p[0][e] - kMagic)) * 128.0f;
+          p[1][e] = r + kMagic;
+          p[2][e] = (r - (p[1][e] - kMagic)) * 128.0f + kMagic;
+        }
+#pragma unroll
+        for (int z = 0; z < P; ++z) {
+          q[z][0] = low_bytes(p[z % 3][0], p[z % 3][1], p[z % 3][2], p[z % 3][3]);
+          q[z][1] = low_bytes(p[z % 3][4], p[z % 3][5], p[z % 3][6], p[z % 3][7]);
+        }
       }
 #pragma unroll
       for (int z = 0; z < P; ++z) {
-        q[z][0] = low_bytes(p[z % 3][0], p[z % 3][1], p[z % 3][2], p[z % 3][3]);
-        q[z][1] = low_bytes(p[z % 3][4], p[z % 3][5], p[z % 3][6], p[z % 3][7]);
-      }
-    }
+        int sum = __dp4a(static_cast<int>(q[z][0]), 0x01010101, __dp4a(static_cast<int>(q[z][1]), 0x01010101, 0));
 #pragma unroll
-    for (int z = 0; z < P; ++z) {
-      int sum = __dp4a(static_cast<int>(q[z][0]), 0x01010101, __dp4a(static_cast<int>(q[z][1]), 0x01010101, 0));
-#pragma unroll
-      for (int o = LANES / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-      if (i < n) {
-        const int v = m * P + z, nt = v >> 3, b = c >> 4, step = c >> 2 & 3;
-        *reinterpret_cast<uint2*>(sx + (((b * NT + nt) * 2 + (step >> 1)) * 32 + (v & 7) * 4 + (c & 3)) * 16 + (step & 1) * 8) =
-            ordered(q[z][0], q[z][1]);
-        if (c % LANES == 0)
-          info[(c / LANES) * 8 * NT + v] = {sum, z == 0 ? scale : z == 1 ? scale * 0.0078125f : scale * 6.1035156e-5f};
+        for (int o = LANES / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+        if (i < n) {
+          const int v = m * P + z, nt = v >> 3, b = c >> 4, step = c >> 2 & 3;
+          *reinterpret_cast<uint2*>(sx + (((b * NT + nt) * 2 + (step >> 1)) * 32 + (v & 7) * 4 + (c & 3)) * 16 + (step & 1) * 8) =
+              ordered(q[z][0], q[z][1]);
+          if (c % LANES == 0)
+            info[(c / LANES) * 8 * NT + v] = {sum, z == 0 ? scale : z == 1 ? scale * 0.0078125f : scale * 6.1035156e-5f};
+        }
       }
     }
   }
@@ -474,8 +487,8 @@ extern "C" int mvb_linear_w4(void* y, int64_t ldy, const void* x, int64_t ldx, c
   // Few rows here, more on tcgen05.  A bf16 row is three columns of the product here.  8 bf16 rows, here and on tcgen05:
   // 24576 x 4096 25.9 us and 26.2, 12288 x 4096 15.5 and 19.8, 4096 x 8192 15.1 and 16.8; but 4096 x 12288 24.7 and 19.6, 3584 x
   // 14336 29.6 and 19.0, because the columns of 6 rows and more leave too little shared memory there for a block by itself (5
-  // rows: 13.8 and 19.5, 17.1 and 18.6).  16 rows of 8 bits: 24576 x 4096 21.5 and 24.8, 4096 x 12288 17.4 and 19.1, 2048 x 1024
-  // 5.8 and 9.1; 20 by 24576 x 4096 36.0 and 24.8, 24 by 4096 x 4096 18.6 and 13.4.
+  // rows: 13.8 and 19.5, 17.1 and 18.6).  16 rows of 8 bits: 24576 x 4096 20.4 and 24.8, 4096 x 12288 17.4 and 19.1, 2048 x 1024
+  // 5.5 and 9.1; 20 by 24576 x 4096 36.0 and 24.8, 24 by 4096 x 4096 18.6 and 13.4.
   if (rows > (row_scales != nullptr ? 16 : k > 8192 ? 5 : 8)) {
     const W4LinearCall call = {a.y, ldy, x, ldx, row_scales, a.records, a.rows, a.n, a.k, static_cast<int>(group)};
     return w4_gemm(name, call, reinterpret_cast<cudaStream_t>(stream));
