@@ -844,15 +844,17 @@ def _row_view(t: torch.Tensor) -> tuple[torch.Tensor, int] | None:
     if len(shape) == 2:
         row = strides[0] if shape[0] > 1 else width
         return (t, row) if row >= width else None
-    row, size = 0, 1  # rows of the dimensions so far are `row` apart
+    row, size = None, 1  # rows of the dimensions so far are `row` apart; 0 where one is broadcast
     for n, stride in zip(reversed(shape[:-1]), reversed(strides[:-1])):
         if n == 1:
             continue
-        if row and stride != row * size:
+        if row is None:
+            row = stride
+        elif stride != row * size:
             return None
-        row = row or stride
         size *= n
-    row = row or width
+    if row is None:
+        row = width
     return (t, row) if row >= width else None
 
 
