@@ -3,7 +3,9 @@
 // Codes less zeros are whole numbers of -15 .. 15, exact in bf16 and in 8 bits.  They are unpacked from shared memory into
 // TMEM, where they are the 128-row operand of tcgen05.mma; rows of x are its columns, from shared memory as TMA brings
 // them: bf16 products with fp32 sums, or 8-bit ones with whole sums.  A group's sum is scaled as it leaves TMEM and added
-// up in registers, in 32 bits: no weight and no product is rounded.
+// up in registers, in 32 bits: no weight and no product is rounded.  In bf16 the whole numbers are taken times 2^-11, and the
+// results times 2^11: so a group's sum, 128 times 15 times 2^-11 of its largest element at most, never leaves fp32's range
+// (and at the other end 12 bits of product times bf16's least number, 2^-144, is still a number of fp32).
 //
 // A block takes up to 256 weight rows, as two halves of 128 lanes, by BN rows of x (32 or 64); or (SPLIT) up to 128 weight
 // rows by 32, 64 or 128, the columns of a step shared by the two sets of warps that unpack, and the rows of x by the two
@@ -94,9 +96,12 @@ __device__ __forceinline__ uint32_t and_or(uint32_t a, uint32_t b, uint32_t c) {
   asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(d) : "r"(a), "r"(b), "r"(c));
   return d;
 }
-// (w >> 4 j) of a word, less the zero: two bf16 numbers code - zero (z2: 128 + zero twice)
+// The low nibbles of two halves as 2^-4 + 2^-11 code in bf16.
+__device__ __forceinline__ uint32_t nibbles_bf16(uint32_t w) { return and_or(w, 0x000f000fu, 0x3d803d80u); }
+constexpr float kUnit = 2048.0f;
+// (w >> 4 j) of a word, less the zero: two bf16 numbers 2^-11 (code - zero) (z2: the zero's twice)
 __device__ __forceinline__ uint32_t codes_bf16(uint32_t w, uint32_t z2) {
-  uint32_t v = and_or(w, 0x000f000fu, 0x43004300u), d;
+  uint32_t v = nibbles_bf16(w), d;
   asm("sub.rn.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(v), "r"(z2));
   return d;
 }
@@ -428,7 +433,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           } else {
 #pragma unroll
             for (int i = 0; i < WORDS; ++i) {
-              const uint32_t z2 = __byte_perm(pair[i * PER / 4], 0, 0x3232);
+              const uint32_t z2 = nibbles_bf16(__byte_perm(pair[i * PER / 4], 0, 0x3232));
               uint32_t o[16];
 #pragma unroll
               for (int t = 0; t < 4; ++t)
@@ -516,7 +521,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
         for (int i = 0; i < CN; ++i) {
           const float v = i & 1 ? acc[i / 2].y : acc[i / 2].x;
-          if (i < rows) *y = __float2bfloat16_rn(Q8 ? v * __ldg(scales + i) : v);
+          if (i < rows) *y = __float2bfloat16_rn(v * (Q8 ? __ldg(scales + i) : kUnit));
           y += ldy;
         }
       }
@@ -533,7 +538,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       for (int i = rank * kThreads + static_cast<int>(threadIdx.x); i < rows * fours; i += c * kThreads) {
         const int m = i / fours, r = 4 * (i - m * fours), col = item.tile * kW4Rows + r;
         const float4 v = dsmem_sum4(part + m * (a.chunk * kW4Rows) + r, c);
-        const float scale = Q8 ? __ldg(a.a + row0 + m) : 1.0f;
+        const float scale = Q8 ? __ldg(a.a + row0 + m) : kUnit;
         const float y4[4] = {v.x * scale, v.y * scale, v.z * scale, v.w * scale};
         __nv_bfloat16* y = a.y + (row0 + m) * a.ldy + col;
 #pragma unroll
