@@ -118,11 +118,14 @@ __global__ void __launch_bounds__(kThreads) quantise_w4_kernel(uint8_t* __restri
       float y[8], least = low, by = scale;
 #pragma unroll
       for (int e = 0; e < 8; e += 2) y[e] = low_bf16(v[e >> 1]), y[e + 1] = high_bf16(v[e >> 1]);
-      if (scale < 1.1754944e-38f) {  // whose reciprocal would overflow: all times 2^64
+      if (scale < 1.1754944e-38f) {
+        // Its reciprocal would overflow: all times 2^64.  And it may have been rounded down by so much that -lo is more than
+        // 15.5 of it (normal scales: 15.06 at most): cut to 15 there, and with it what is below -15.
         constexpr float kUp = 1.8446744e19f;
-        least *= kUp, by *= kUp;
+        by *= kUp;
+        least = fminf(least * kUp, 15.0f * by);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) y[e] *= kUp;
+        for (int e = 0; e < 8; ++e) y[e] = fmaxf(y[e] * kUp, -15.0f * by);
       }
       float inv;
       asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inv) : "f"(by));
