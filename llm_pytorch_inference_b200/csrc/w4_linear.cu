@@ -112,13 +112,13 @@ struct Layout {
   int most;  // 128-column blocks of a block
   int stages;
   bool cluster;
-  __host__ __device__ size_t ring() const { return FIXED; }
-  __host__ __device__ size_t x() const { return ring() + static_cast<size_t>(kWarps) * stages * 2 * REC; }
-  __host__ __device__ size_t info() const { return x() + static_cast<size_t>(most) * X_BLOCK; }
-  __host__ __device__ size_t left() const { return info() + static_cast<size_t>(most) * INFO_BLOCK; }
-  __host__ __device__ size_t red() const { return left() + static_cast<size_t>(most) * LEFT_BLOCK; }
-  __host__ __device__ size_t part() const { return red() + 2 * kWarps * SUMS * 4; }
-  __host__ __device__ size_t bytes() const { return part() + (cluster ? kRound * ROWS * PITCH * 4 : 0); }
+  __host__ __device__ constexpr size_t ring() const { return FIXED; }
+  __host__ __device__ constexpr size_t x() const { return ring() + static_cast<size_t>(kWarps) * stages * 2 * REC; }
+  __host__ __device__ constexpr size_t info() const { return x() + static_cast<size_t>(most) * X_BLOCK; }
+  __host__ __device__ constexpr size_t left() const { return info() + static_cast<size_t>(most) * INFO_BLOCK; }
+  __host__ __device__ constexpr size_t red() const { return left() + static_cast<size_t>(most) * LEFT_BLOCK; }
+  __host__ __device__ constexpr size_t part() const { return red() + 2 * kWarps * SUMS * 4; }
+  __host__ __device__ constexpr size_t bytes() const { return part() + (cluster ? kRound * ROWS * PITCH * 4 : 0); }
 };
 
 // What a group of a row of x needs beside its codes.  Rows of 8 bits: their sum, an int.  Digits:
@@ -641,30 +641,44 @@ int run(const char* name, LinearArgs a, cudaStream_t stream) {
   return launch_cluster(name, kernel, grid, dim3(kThreads), static_cast<unsigned>(best), at.bytes(), stream, a);
 }
 
+// Whether shared memory holds x of these columns, a cluster's blocks sharing them.
 template <int GROUP, int D, int NT>
-bool fits(const LinearArgs& a) {
-  return Layout<GROUP, D, NT>{(a.blocks + kMaxCluster - 1) / kMaxCluster, 1, true}.bytes() <= kMostSmem;
+constexpr bool fits(int blocks, int cluster) {
+  return Layout<GROUP, D, NT>{(blocks + cluster - 1) / cluster, 1, true}.bytes() <= kMostSmem;
 }
 
-// As many columns of the product as the rows need, where x then fits into a cluster's shared memory.
-template <int GROUP>
-int run_q8(const char* name, const LinearArgs& a, cudaStream_t stream) {
-  if (a.rows > 8 && fits<GROUP, 1, 2>(a)) return run<GROUP, 1, 2>(name, a, stream);
-  return run<GROUP, 1, 1>(name, a, stream);
-}
-template <int GROUP>
-int run_bf16(const char* name, const LinearArgs& a, cudaStream_t stream) {
-  if (a.rows > 6 && fits<GROUP, 4, 4>(a)) return run<GROUP, 4, 4>(name, a, stream);
-  if (a.rows > 4 && fits<GROUP, 4, 3>(a)) return run<GROUP, 4, 3>(name, a, stream);
-  if (a.rows > 2 && fits<GROUP, 4, 2>(a)) return run<GROUP, 4, 2>(name, a, stream);
-  return run<GROUP, 4, 1>(name, a, stream);
+// As many columns of the product as the rows need; other calls go to tcgen05, `few` false.  A kernel here reads the records
+// once.
+//   8 rows of bf16, here and on tcgen05, where a cluster of 4 holds x: 24576 x 4096 22.8 us and 26.4, 4096 x 12288 18.8 and 19.8, in
+//   groups of 32 21.4 and 23.0, 16384 x 8192 36.8 and 34.7.  A cluster of 8 leaves SMs idle, which few weight rows do not need:
+//   4096 x 20480 26.8 and 26.0, in groups of 32 39.6 and 31.3; but 1024 x 20480 13.7 and 17.1, in groups of 32 16.6 and 21.3.
+//   Up to 6 rows fit at any k: 4096 x 24576 26.8 and 28.6, in groups of 32 33.1 and 34.7, at worst (32768) 45.9 and 43.0.
+//   16 rows of 8 bits: 24576 x 4096 20.2 and 24.8, 4096 x 12288 14.8 and 18.9, in groups of 32 18.0 and 26.4, at worst (4096 x
+//   32768) 35.0 and 33.3; 20 by 24576 x 4096 36.0 and 24.8, 24 by 4096 x 4096 18.6 and 13.4.
+template <int GROUP, bool Q8>
+int run_few(const char* name, const LinearArgs& a, cudaStream_t stream, bool& few) {
+  constexpr int MOST = 32768 / kW4Cols;
+  few = true;
+  if constexpr (Q8) {
+    static_assert(fits<GROUP, 1, 2>(MOST, kMaxCluster), "16 rows");
+    if (a.rows <= 8) return run<GROUP, 1, 1>(name, a, stream);
+    if (a.rows <= 16) return run<GROUP, 1, 2>(name, a, stream);
+  } else {
+    static_assert(fits<GROUP, 4, 3>(MOST, kMaxCluster), "6 rows");
+    if (a.rows <= 2) return run<GROUP, 4, 1>(name, a, stream);
+    if (a.rows <= 4) return run<GROUP, 4, 2>(name, a, stream);
+    if (a.rows <= 6) return run<GROUP, 4, 3>(name, a, stream);
+    if (a.rows <= 8 && fits<GROUP, 4, 4>(a.blocks, a.pairs <= 64 ? kMaxCluster : 4)) return run<GROUP, 4, 4>(name, a, stream);
+  }
+  few = false;
+  return MVB_OK;
 }
 
 template <bool Q8>
-int run_group(const char* name, const LinearArgs& a, int64_t group, cudaStream_t stream) {
-  if (group == 32) return Q8 ? run_q8<32>(name, a, stream) : run_bf16<32>(name, a, stream);
-  if (group == 64) return Q8 ? run_q8<64>(name, a, stream) : run_bf16<64>(name, a, stream);
-  return Q8 ? run_q8<128>(name, a, stream) : run_bf16<128>(name, a, stream);
+int run_group(const char* name, const LinearArgs& a, int64_t group, cudaStream_t stream, bool& few) {
+  if (group == 32) return run_few<32, Q8>(name, a, stream, few);
+  if (group == 64) return run_few<64, Q8>(name, a, stream, few);
+  return run_few<128, Q8>(name, a, stream, few);
 }
 
 }  // namespace
@@ -702,15 +716,10 @@ extern "C" int mvb_linear_w4(void* y, int64_t ldy, const void* x, int64_t ldx, c
   a.blocks = (a.k + kW4Cols - 1) / kW4Cols;
   a.pairs = (a.tiles + 1) / 2;
   a.err = device_status_ptr();
-  // Few rows here, more on tcgen05.  A bf16 row is three columns of the product here.  8 bf16 rows, here and on tcgen05:
-  // 24576 x 4096 25.9 us and 26.2, 12288 x 4096 15.5 and 19.8, 4096 x 8192 15.1 and 16.8; but 4096 x 12288 24.7 and 19.6, 3584 x
-  // 14336 29.6 and 19.0, because the columns of 6 rows and more leave too little shared memory there for a block by itself (5
-  // rows: 13.8 and 19.5, 17.1 and 18.6).  16 rows of 8 bits: 24576 x 4096 20.4 and 24.8, 4096 x 12288 17.4 and 19.1, 2048 x 1024
-  // 5.5 and 9.1; 20 by 24576 x 4096 36.0 and 24.8, 24 by 4096 x 4096 18.6 and 13.4.
-  if (rows > (row_scales != nullptr ? 16 : k > 8192 ? 5 : 8)) {
-    const W4LinearCall call = {a.y, ldy, x, ldx, row_scales, a.records, a.rows, a.n, a.k, static_cast<int>(group)};
-    return w4_gemm(name, call, reinterpret_cast<cudaStream_t>(stream));
-  }
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-  return row_scales != nullptr ? run_group<true>(name, a, group, st) : run_group<false>(name, a, group, st);
+  bool few = false;
+  MVB_TRY(row_scales != nullptr ? run_group<true>(name, a, group, st, few) : run_group<false>(name, a, group, st, few));
+  if (few) return MVB_OK;
+  const W4LinearCall call = {a.y, ldy, x, ldx, row_scales, a.records, a.rows, a.n, a.k, static_cast<int>(group)};
+  return w4_gemm(name, call, st);
 }
