@@ -32,6 +32,7 @@
 #include "host.h"
 #include "w4.cuh"
 #include "w4_linear.h"
+#include "w4_ring.h"
 
 namespace mvb {
 namespace {
@@ -76,7 +77,7 @@ __device__ __forceinline__ void copy_bulk(void* dst, const void* src, uint32_t b
       : "memory");
 }
 
-// Shared memory, from its start: barriers [warp][stages]; the rings [warp][stages][2 records]; x; what the
+// Shared memory, from its start: flags; barriers [warp][stages]; the rings [warp][stages][2 records]; x; what the
 // groups of x need; what its digits leave out; the warps' sums; the cluster's sums.
 // Digits D: 1 for rows of 8 bits, 4 for bf16.
 template <int GROUP, int D, int NT>
@@ -454,8 +455,9 @@ __global__ void __launch_bounds__(kThreads, 1) w4_linear_kernel(const LinearArgs
   const int blocks = static_cast<int>(static_cast<int64_t>(rank + 1) * a.blocks / c) - block0;
   const L at = {(a.blocks + c - 1) / c, a.stages, c > 1};
   volatile int* abort_flag = reinterpret_cast<volatile int*>(smem);
+  int* lost = reinterpret_cast<int*>(smem) + 16 + wid;  // this warp's place whose wait gave up
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + 128) + wid * kMaxStages;
-  uint8_t* ring = smem + at.ring() + static_cast<size_t>(wid) * a.stages * 2 * L::REC;
+  uint8_t* places = smem + at.ring() + static_cast<size_t>(wid) * a.stages * 2 * L::REC;
   uint8_t* sx = smem + at.x();
   uint8_t* info = smem + at.info();
   uint32_t* left = reinterpret_cast<uint32_t*>(smem + at.left());  // [blocks][LEFT_ROWS]
@@ -468,19 +470,20 @@ __global__ void __launch_bounds__(kThreads, 1) w4_linear_kernel(const LinearArgs
   const int mine = unit < a.pairs ? (a.pairs - unit + units - 1) / units : 0;  // pairs of this block
 
   // The copies of this warp's items, lane 0's: the next one to ask for.
-  int load_j = team, load_b = kw, load_at = 0;
+  W4Ring ring(team);
+  int load_b = kw;
   uint64_t policy = 0;
   auto ask = [&]() {
-    if (load_b >= blocks || load_j >= mine) return;  // (a warp without columns asks for none)
-    const int tile = 2 * (unit + load_j * units);
+    if (load_b >= blocks || ring.pair >= mine) return;  // (a warp without columns asks for none)
+    const int tile = 2 * (unit + ring.pair * units);
     const int64_t r = w4_record(tile, block0 + load_b, a.tiles, a.blocks);
     // the last pair may lack its second tile: what its place holds then is computed with and not written
     const uint32_t bytes = (tile + 1 < a.tiles ? 2 : 1) * L::REC;
-    mbar_arrive_expect_tx(&bars[load_at], bytes);
-    copy_bulk(ring + load_at * 2 * L::REC, a.records + r * L::REC, bytes, &bars[load_at], policy);
-    load_at = load_at + 1 == a.stages ? 0 : load_at + 1;
+    mbar_arrive_expect_tx(&bars[ring.fill], bytes);
+    copy_bulk(places + ring.fill * 2 * L::REC, a.records + r * L::REC, bytes, &bars[ring.fill], policy);
+    ring.asked(a.stages);
     load_b += split;
-    if (load_b >= blocks) load_b = kw, load_j += teams;
+    if (load_b >= blocks) load_b = kw, ring.pair += teams;
   };
   if (tid == 0) *abort_flag = 0;
   if (lane == 0) {
@@ -498,8 +501,6 @@ __global__ void __launch_bounds__(kThreads, 1) w4_linear_kernel(const LinearArgs
   if (D > 1) some_left = __syncthreads_or(some_left) != 0;
   else __syncthreads();
 
-  int stage = 0;
-  uint32_t phase = 0;
   const int rounds = c > 1 ? (mine + kRound - 1) / kRound : 1;  // the same in every block of a cluster
   for (int round = 0; round < rounds; ++round) {
     const int j0 = c > 1 ? round * kRound : 0, j1 = c > 1 ? min(mine, j0 + kRound) : mine;
@@ -518,15 +519,17 @@ __global__ void __launch_bounds__(kThreads, 1) w4_linear_kernel(const LinearArgs
       auto items = [&](auto with_left) {
         uint32_t had = 0;
         for (int b = kw; b < blocks; b += split) {
-          mbar_wait(&bars[stage], phase, abort_flag, a.err);
-          compute<GROUP, D, NT>(ring + stage * 2 * L::REC, sx, info, b, lane, acc);
+          // where it gives up the item is computed all the same, and the rest, so that all barriers are met
+          if (!mbar_wait(&bars[ring.read], ring.phase, abort_flag, a.err) && lane == 0) ring.stop(*lost);
+          const uint8_t* rec = places + ring.read * 2 * L::REC;
+          compute<GROUP, D, NT>(rec, sx, info, b, lane, acc);
           if constexpr (decltype(with_left)::value)
-            left_out<GROUP, D, NT>(ring + stage * 2 * L::REC, left + b * L::LEFT_ROWS,
+            left_out<GROUP, D, NT>(rec, left + b * L::LEFT_ROWS,
                                    static_cast<const __nv_bfloat16*>(a.x) + row0 * a.ldx + (block0 + b) * kW4Cols, a.ldx,
                                    reinterpret_cast<const Info*>(info + b * L::INFO_BLOCK), out, lane, had);
           __syncwarp();  // every lane has read: the next copy may come
           if (lane == 0) ask();
-          if (++stage == a.stages) stage = 0, phase ^= 1;
+          ring.next(a.stages);
         }
         if constexpr (decltype(with_left)::value) {
 #pragma unroll
@@ -588,8 +591,11 @@ __global__ void __launch_bounds__(kThreads, 1) w4_linear_kernel(const LinearArgs
     }
   }
   // Every copy has been waited for, unless a wait gave up: then those under way are, before the block ends.
-  if (*abort_flag && lane == 0)
-    for (int s = 0; s < a.stages; ++s) mbar_wait(&bars[s], phase ^ (s < stage ? 0 : 1), nullptr, a.err);
+  if (lane == 0 && ring.stopped()) {
+    ring.back(*lost);
+    do mbar_wait(&bars[ring.read], ring.phase, nullptr, a.err);
+    while (ring.more(a.stages));
+  }
 }
 
 template <int GROUP, int D, int NT>
