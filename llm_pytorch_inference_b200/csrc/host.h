@@ -11,6 +11,7 @@
 #include <utility>
 
 #include "../../include/mvb200.h"
+#include "per_device.h"
 
 namespace mvb {
 
@@ -131,30 +132,33 @@ int set_smem_once(std::atomic<uint64_t>& done, void (*kernel)(KArgs...), size_t 
   return rc;
 }
 
-// Clusters of `cluster` blocks of `kernel` that the GPU holds at once.  They lie within its groups of SMs, so that larger
-// ones leave SMs over (on B200, one block an SM: 74 of 2, 45 of 3, 33 of 4, 15 of 8).  Asked of the driver once per
-// kernel and size: `known` is a static of the call site, 0 where not asked yet.
+// Clusters of `cluster` blocks of `kernel` that the current device holds at once.  They lie within its groups of SMs, so that
+// larger ones leave SMs over (on B200, one block an SM: 74 of 2, 45 of 3, 33 of 4, 15 of 8).  Asked of the driver once per
+// kernel, size and device: `known` is a static of the call site.  Where the driver does not say, 1 is taken for this call.
 template <typename... KArgs>
-int clusters_at_once(std::atomic<int>& known, void (*kernel)(KArgs...), int cluster, int threads, size_t smem) {
-  int n = known.load(std::memory_order_relaxed);
-  if (n > 0) return n;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(static_cast<unsigned>(cluster));
-  cfg.blockDim = dim3(static_cast<unsigned>(threads));
-  cfg.dynamicSmemBytes = smem;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = static_cast<unsigned>(cluster);
-  attr[0].val.clusterDim.y = 1;
-  attr[0].val.clusterDim.z = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  if (cudaOccupancyMaxActiveClusters(&n, kernel, &cfg) != cudaSuccess || n <= 0) {
-    cudaGetLastError();
-    n = 1;
-  }
-  known.store(n, std::memory_order_relaxed);
-  return n;
+int clusters_at_once(PerDevice& known, void (*kernel)(KArgs...), int cluster, int threads, size_t smem) {
+  int device = -1;
+  if (cudaGetDevice(&device) != cudaSuccess) device = -1;
+  auto ask = [&] {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(static_cast<unsigned>(cluster));
+    cfg.blockDim = dim3(static_cast<unsigned>(threads));
+    cfg.dynamicSmemBytes = smem;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = static_cast<unsigned>(cluster);
+    attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    int n = 0;
+    if (cudaOccupancyMaxActiveClusters(&n, kernel, &cfg) != cudaSuccess) {
+      cudaGetLastError();
+      n = 0;
+    }
+    return n;
+  };
+  return known.get(device, ask, 1);
 }
 
 }  // namespace mvb

@@ -573,7 +573,7 @@ struct Plan {
 
 template <bool Q8, int GROUP, int BN, bool SPLIT>
 int units_of(int c, int sms) {
-  static std::atomic<int> clusters[kMaxCluster + 1] = {};
+  static PerDevice clusters[kMaxCluster + 1];
   return c == 1 ? sms : clusters_at_once(clusters[c], w4_gemm_kernel<Q8, GROUP, BN, SPLIT>, c, kThreads, kMostSmem);
 }
 

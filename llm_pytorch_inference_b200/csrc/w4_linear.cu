@@ -620,7 +620,7 @@ int run(const char* name, LinearArgs a, cudaStream_t stream) {
   // for what its threads ask for at once, and 0.05 for 128 columns of a row) and a cluster's meeting (20).  Of 1, 2, 4 and 8 blocks
   // measured at 80 sizes that picks what is 0.4 % above the best on average, 5 % at most: 8 rows by 4096 x 4096, bf16, 12.9, 10.9,
   // 9.5 and 10.5 us, by 24576 x 4096 28.0, 22.7, 25.5 and 35.1; 1 row by 4096 x 4096 6.0, 6.6, 6.7 and 7.4.
-  static std::atomic<int> clusters[kMaxCluster + 1] = {};
+  static PerDevice clusters[kMaxCluster + 1];
   auto units_of = [&](int c) {
     return c == 1 ? sms : clusters_at_once(clusters[c], kernel, c, kThreads, kMostSmem);
   };
