@@ -176,14 +176,6 @@ __device__ __forceinline__ void load_words(uint32_t (&v)[N], const uint8_t* p) {
   }
 }
 
-__device__ __forceinline__ void copy_bulk(void* dst, const void* src, uint32_t bytes, uint64_t* bar, uint64_t policy) {
-  asm volatile(
-      "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes.L2::cache_hint [%0], [%1], %2, [%3], %4;" ::"r"(
-          smem_u32(dst)),
-      "l"(src), "r"(bytes), "r"(smem_u32(bar)), "l"(policy)
-      : "memory");
-}
-
 // Shared memory: barriers; the ring of x boxes; the ring of records; the cluster's sums.
 template <bool Q8, int GROUP, int BN, bool SPLIT>
 struct Layout {
