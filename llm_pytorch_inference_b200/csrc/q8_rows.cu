@@ -422,7 +422,7 @@ int run_rows(const char* name, const RowArgs& a, int64_t rows, cudaStream_t stre
   if (a.width > 32 * 1024)
     return launch(name, q8_any_kernel<KIND, T>, dim3(static_cast<unsigned>(rows)), dim3(1024), 0, stream, a);
   if (!vec) {
-    // Few rows: 8 elements a thread where 1024 threads hold a row so.  Many: 16, as many rows in an SM as its threads allow.
+    // The fewest elements a thread (8, 16 or 32) with which 1024 threads hold a row, whatever the number of rows.
     const int ept = a.width > 16 * 1024 ? 32 : a.width > 8 * 1024 ? 16 : 8;
     const dim3 grid(static_cast<unsigned>(rows)), block(static_cast<unsigned>(((a.width + ept - 1) / ept + 31) / 32 * 32));
     if (ept == 8) return launch(name, q8_ragged_kernel<KIND, T, 8>, grid, block, 0, stream, a);
