@@ -973,14 +973,14 @@ def geglu_q8(gate: torch.Tensor, up: torch.Tensor) -> Q8Rows:
 
 def _check_q8(what: str, rows) -> int:
     """Device of rows in 8 bits, checked."""
-    v, s = rows
     try:
+        v, s = rows
         index, shape = v.get_device(), v.shape
         if (v.dtype is _I8 and s.dtype is _F32 and index >= 0 and s.get_device() == index and len(shape)
                 and s.shape == shape[:-1] and shape[-1]):
             return index
-    except AttributeError:
-        raise RuntimeError(f"{what}: values and scales must be tensors") from None
+    except (AttributeError, TypeError, ValueError):  # no pair, or not of tensors
+        raise RuntimeError(f"{what}: rows must be Q8Rows, values and scales both tensors") from None
     N.require_cuda(v, s)
     raise RuntimeError(f"{what}: values {tuple(v.shape)} {v.dtype} and scales {tuple(s.shape)} {s.dtype} are not int8 "
                        "rows with an fp32 scale each, on one GPU")
