@@ -591,11 +591,12 @@ int mvb_set_pdl(int enable);
  *
  * A row in 8 bits: codes q (int8, -127 .. 127) and an fp32 scale; element i stands for q[i] * scale.
  * With amax = max |y|: q = rint(127 y / amax), scale = amax / 127.  A row with an infinity or a NaN gets the scale NaN,
- * a row of zeros the scale 0.  values: [rows, width] (contiguous), scales: [rows].  y, in 32 bits throughout:
+ * a row of zeros the scale 0.  values: [rows, width] (contiguous), scales: [rows].  y, in 32 bits throughout (so a norm's row
+ * gets the scale 0 where the sum of its squares passes fp32's range, and NaN where a product with the weight does):
  *   mvb_quantise_q8           in
  *   mvb_rmsnorm_q8            in * w / sqrt(mean(in^2) + eps), w = weight or 1 + weight (plus_one)
  *   mvb_fused_add_rmsnorm_q8  the same of residual + in (rounded to the dtype), which goes to residual_out
- *                             (may be residual or in)
+ *                             (may be residual or in, and overlaps neither otherwise)
  *   mvb_gated_q8              act(gate) * up
  * Strides: elements between rows.  dtype: MVB_F32, MVB_F16 or MVB_BF16, of every operand.
  * mvb_dequantise_q8: out[rows, width] = values * scales, rounded to the dtype. */
@@ -625,7 +626,8 @@ int mvb_dequantise_q8(void* out, const int8_t* values, int64_t values_stride, co
  *   mvb_dequantise_w4  out[n, k], MVB_BF16 (rounded) or MVB_F32 (exact but for subnormal results)
  *   mvb_linear_w4      y[rows, n] (bf16, rows ldy elements apart) = x times the matrix transposed.  x: rows of k bf16, or
  *                      with row_scales (fp32 [rows]) rows of k codes of 8 bits; ldx elements between rows, 16-byte aligned.
- *                      Sums in 32 bits; no product is rounded before it.  rows <= 262144, k <= 32768.
+ *                      Sums in 32 bits; no product is rounded before it, whatever the sizes of a row's elements.  y overlaps
+ *                      nothing.  rows <= 262144, k <= 32768.
  * With mvb_set_pdl(1) mvb_linear_w4 reads records before it waits for the kernel launched before it. */
 int64_t mvb_w4_bytes(int64_t n, int64_t k, int64_t group);
 int mvb_quantise_w4(void* records, const void* weight, int64_t weight_stride, int64_t n, int64_t k, int64_t group,

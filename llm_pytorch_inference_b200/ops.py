@@ -901,7 +901,9 @@ def _norm_weight(what: str, weight, index: int, width: int, dtype: torch.dtype) 
 
 def rmsnorm_q8(input: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6, plus_one: bool = False) -> Q8Rows:
     """``rmsnorm`` (``plus_one``: with ``1 + weight``) whose result goes to 8 bits from its 32, without a
-    rounding to the dtype in between.  Rows, non-finite ones too, as in ``quantise_q8``."""
+    rounding to the dtype in between.  Rows, non-finite ones too, as in ``quantise_q8``; the mean of the squares and the
+    products with the weight are held in 32 bits, so a row reads back as zeros where the sum of its squares passes fp32's
+    range (elements of some 1e19, as in ``rmsnorm``), and as NaN where a product ``x * weight`` does."""
     what = "rmsnorm_q8"
     index, code, shape = _float_rows(what, "input", input)
     width = shape[-1]
@@ -920,8 +922,8 @@ def fused_add_rmsnorm_q8(residual: torch.Tensor, input: torch.Tensor, weight: to
                          plus_one: bool = False,
                          residual_out: torch.Tensor | None = None) -> tuple[Q8Rows, torch.Tensor]:
     """``fused_add_rmsnorm`` with its result in 8 bits: ``residual + input``, rounded to the dtype, goes to
-    ``residual_out`` (default: into ``residual``, in place), its norm to 8 bits as in ``rmsnorm_q8``.
-    Returns ``(rows, residual_out)``."""
+    ``residual_out`` (default: into ``residual``, in place; it may be ``input`` too, but overlap neither of them
+    otherwise, nor ``weight``), its norm to 8 bits as in ``rmsnorm_q8``.  Returns ``(rows, residual_out)``."""
     what = "fused_add_rmsnorm_q8"
     index, code, shape = _float_rows(what, "input", input)
     dtype, width = input.dtype, shape[-1]
@@ -1042,7 +1044,8 @@ def quantise_w4(weight: torch.Tensor, group: int = 128) -> W4Weight:
 
 def pack_w4(codes: torch.Tensor, scales: torch.Tensor, zeros: torch.Tensor | None = None, group: int = 128) -> W4Weight:
     """The same from a checkpoint's numbers: ``codes`` uint8 ``[n, k]``, ``scales`` bf16 and ``zeros`` uint8
-    ``[n, ceil(k / group)]`` (None: 8 everywhere, a symmetric checkpoint).  Of codes and zeros the low 4 bits count."""
+    ``[n, ceil(k / group)]`` (None: 8 everywhere, a symmetric checkpoint).  Of codes and zeros the low 4 bits count.
+    A checkpoint's fp16 scales lose three of their 11 bits in bf16."""
     what = "pack_w4"
     index = codes.get_device() if isinstance(codes, torch.Tensor) else -1
     _expect(what, "codes", codes, index, _U8, 2)
