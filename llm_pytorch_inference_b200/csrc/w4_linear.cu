@@ -22,9 +22,11 @@
 // up to 8 blocks splits the columns further, where few weight rows would leave SMs idle or x would not fit; its sums
 // meet in distributed shared memory, in the order of the blocks.  So every result is the same on every call.
 //
-// Measured, one row, groups of 128: 151936 x 4096 bf16 55.8 us (49.4 at the rate of a copy), 24576 x 4096 14.4 (8.0),
-// 4096 x 4096 6.35, 2048 x 1024 4.6.  The long ones stream; 24576 x 4096 gives an SM 5 or 6 pairs and issues in 48 % of
-// the slots on average, start and end included; the short ones are their launch, x and a chain of latencies.
+// Measured, groups of 128: one bf16 row by 151936 x 4096 55.3 us (49.4 at the rate of a copy), 24576 x 4096 14.2 (8.0), 4096 x
+// 4096 6.4, 2048 x 1024 4.4; 8 rows by 24576 x 4096 22.7, 4096 x 4096 9.7.  The long ones stream; 24576 x 4096 gives an SM 5 or 6
+// pairs and issues in half of the slots on average, start and end included; the short ones are their launch, x and a chain of
+// latencies.  Beside a column of 1e4 times the others' size 24576 x 4096 takes 14.2 us with 1 row and 25.8 with 8, beside one of 1e6
+// 17.5 and 46.3.
 #include <climits>
 #include <type_traits>
 
