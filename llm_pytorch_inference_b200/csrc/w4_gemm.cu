@@ -21,7 +21,7 @@
 // Bound by the chain of a step of 128 columns (words read, unpacked and stored to TMEM, products, sums read and scaled),
 // whose parts meet at barriers: 0.4 to 0.7 us in groups of 128 whatever the tiles, at 40 to 60 % of the issue slots, 15 to 30 % of
 // the tensor pipe and 20 % of the memory's rate for 64 rows.  Measured, 24576 x 4096 in groups of 128: 64 rows 29.6 us bf16, 28.7
-// 8-bit (groups of 64: 32.7, 40.5); 2048 rows 359 and 430 (1.15 and 0.96 PFLOP/s).  More warps with fewer registers each, warps
+// 8-bit (groups of 64: 32.8, 40.2; of 32: 44.4, 69.6); 2048 rows 365 and 440 (1.13 and 0.94 PFLOP/s).  More warps with fewer registers each, warps
 // that both unpack and sum, words read a step ahead, two blocks an SM with a half each, zeros taken out of the sums instead of
 // the codes: all the same or slower (38, 36, 33, 32 and 40 us for some 31).
 #include <climits>

@@ -8,7 +8,7 @@
 // Bound by memory: 2 bytes in and 0.53 out per weight (and back).  Half a warp takes 128 columns of a row, 8 a lane:
 // one 16-byte load, and one word of codes; a warp takes a record, 8 pairs of rows, whose loads are all under way first.
 // A group's extremes cross 16, 8 or 4 lanes as one packed pair (max of -w and of w), 4, 3 or 2 exchanges.
-// Measured, 24576 x 4096 in groups of 64 (255 MB either way, 39 us at the rate of a copy): quantising 57 us, bound by
+// Measured, 24576 x 4096 in groups of 64 (255 MB either way, 39 us at the rate of a copy): quantising 59 us, bound by
 // what it computes (81 % of the issue slots before its last step, which took two sums a code out); reading back 42.6 us,
 // bound by memory.
 //
