@@ -121,7 +121,7 @@ def test_rows_of_subnormal_elements(rows):
 
 
 def test_many_rows_of_large_elements():
-    """Up to 1e35 a group's sum of many rows' products stays in fp32's range."""
+    """Large elements of both signs (test_w4_range_gpu goes to the ends of the range)."""
     n, k, group = 40, 256, 128
     codes, scales, zeros = packed(16, n, k, group)
     w, exact = made(codes, scales, zeros, group)
