@@ -78,7 +78,7 @@ template <int GROUP, int D, int NT>
 struct Layout {
   static constexpr int PER = kW4Cols / GROUP;
   static constexpr int REC = w4_record_bytes(GROUP);
-  static constexpr int ROWS = 8 * NT / D;                      // rows of x of a block
+  static constexpr int ROWS = 8 * NT / D;                      // the most rows of x
   static constexpr int WHOLE = D == 1 ? ROWS : NT / 2 * 4;     // of them those with one column of sums; others have two
   static constexpr int COLS = 2 * ROWS - WHOLE;                // columns of a warp's sums of a pair
   static constexpr int PER_LANE = COLS / 4;                    // of them a lane has so many, for 4 weight rows
@@ -154,16 +154,16 @@ __device__ __forceinline__ bool is_one(uint32_t left) { return left >> 16 != 0; 
 // and lane 16 bytes, 8 a step.  The lane's column of the product is lane / 4, its columns of x 8 (lane % 4) .. + 7 of
 // the step's.  Returns whether this thread has noted elements that the digits do not hold.
 template <int GROUP, int D, int NT>
-__device__ __forceinline__ bool stage_x(uint8_t* sx, uint8_t* info, uint32_t* left, const LinearArgs& a, int row0, int block0,
+__device__ __forceinline__ bool stage_x(uint8_t* sx, uint8_t* info, uint32_t* left, const LinearArgs& a, int block0,
                                         int blocks) {
   using L = Layout<GROUP, D, NT>;
   constexpr int LANES = GROUP / 8;
-  const int chunks = blocks * 16, rows = min(L::ROWS, a.rows - row0), n = rows * chunks;
+  const int chunks = blocks * 16, n = a.rows * chunks;
   const int lane = threadIdx.x & 31;
   bool noted = false;
   if (D > 1)  // rows that are not there leave nothing
     for (int i = threadIdx.x; i < blocks * L::LEFT_ROWS; i += kThreads)
-      if (i % L::LEFT_ROWS >= rows) left[i] = 0;
+      if (i % L::LEFT_ROWS >= a.rows) left[i] = 0;
   // 8-bit rows: four chunks a thread are asked for at a time (16 by 4096 x 4096 11.8 us for one, 10.5 for four).  Taking a
   // bf16 row apart is longer than its wait, and four were the same.
   using Raw = std::conditional_t<D == 1, uint2, uint4>;
@@ -177,7 +177,7 @@ __device__ __forceinline__ bool stage_x(uint8_t* sx, uint8_t* info, uint32_t* le
       const int col = block0 * kW4Cols + 8 * c;
       raw[u] = Raw{};
       if (i < n && col < a.k)
-        raw[u] = *reinterpret_cast<const Raw*>(static_cast<const uint8_t*>(a.x) + ((row0 + m) * a.ldx + col) * (D == 1 ? 1 : 2));
+        raw[u] = *reinterpret_cast<const Raw*>(static_cast<const uint8_t*>(a.x) + (m * a.ldx + col) * (D == 1 ? 1 : 2));
     }
 #pragma unroll
     for (int u = 0; u < AHEAD; ++u) {
@@ -412,7 +412,7 @@ __device__ __forceinline__ float left_sum(const uint8_t* rec, uint32_t left, con
 }
 
 // What an item's rows leave out, added up in shared memory where a warp's sums of the pair will be; `had`: the rows that have
-// left something in this pair.  x: this block's first row, at the item's columns.
+// left something in this pair.  x: the first row, at the item's columns.
 template <int GROUP, int D, int NT>
 __device__ __forceinline__ void left_out(const uint8_t* rec, const uint32_t* left, const __nv_bfloat16* x, int64_t ldx,
                                          const Info* info, float* out, int lane, uint32_t& had) {
@@ -444,7 +444,6 @@ __global__ void __launch_bounds__(kThreads, 1) w4_linear_kernel(const LinearArgs
   const int tid = threadIdx.x, lane = tid & 31, wid = tid >> 5;
   const int c = a.cluster, rank = static_cast<int>(blockIdx.x) % c, unit = static_cast<int>(blockIdx.x) / c;
   const int units = static_cast<int>(gridDim.x) / c;
-  const int row0 = blockIdx.y * L::ROWS;
   const int block0 = static_cast<int>(static_cast<int64_t>(rank) * a.blocks / c);
   const int blocks = static_cast<int>(static_cast<int64_t>(rank + 1) * a.blocks / c) - block0;
   const L at = {(a.blocks + c - 1) / c, a.stages, c > 1};
@@ -491,7 +490,7 @@ __global__ void __launch_bounds__(kThreads, 1) w4_linear_kernel(const LinearArgs
   pdl_wait();
   // Whether the digits of all this block's rows hold them, which is usual: the loop without left_out then runs (with the branch
   // in it 4 by 24576 x 4096 took 20.2 us for 18.3).
-  bool some_left = stage_x<GROUP, D, NT>(sx, info, left, a, row0, block0, blocks);
+  bool some_left = stage_x<GROUP, D, NT>(sx, info, left, a, block0, blocks);
   if (D > 1) some_left = __syncthreads_or(some_left) != 0;
   else __syncthreads();
 
@@ -509,7 +508,7 @@ __global__ void __launch_bounds__(kThreads, 1) w4_linear_kernel(const LinearArgs
 #pragma unroll
           for (int i = 0; i < L::PER_LANE; ++i) acc[s][h][i] = 0.0f;
       float* out = red + (buf * kWarps + wid) * L::SUMS;  // two pairs ago everybody had read it
-      float* own = out + lane / 4;                   // of this lane's weight rows
+      float* own = out + lane / 4;                        // of this lane's weight rows
       auto items = [&](auto with_left) {
         uint32_t had = 0;
         for (int b = kw; b < blocks; b += split) {
@@ -519,7 +518,7 @@ __global__ void __launch_bounds__(kThreads, 1) w4_linear_kernel(const LinearArgs
           compute<GROUP, D, NT>(rec, sx, info, b, lane, acc);
           if constexpr (decltype(with_left)::value)
             left_out<GROUP, D, NT>(rec, left + b * L::LEFT_ROWS,
-                                   static_cast<const __nv_bfloat16*>(a.x) + row0 * a.ldx + (block0 + b) * kW4Cols, a.ldx,
+                                   static_cast<const __nv_bfloat16*>(a.x) + (block0 + b) * kW4Cols, a.ldx,
                                    reinterpret_cast<const Info*>(info + b * L::INFO_BLOCK), out, lane, had);
           __syncwarp();  // every lane has read: the next copy may come
           if (lane == 0) ask();
@@ -547,8 +546,7 @@ __global__ void __launch_bounds__(kThreads, 1) w4_linear_kernel(const LinearArgs
       else __syncwarp();
       const float* in = red + (buf * kWarps + team * split) * L::SUMS;
       const int pair = unit + j * units;
-      const int rows = min(L::ROWS, a.rows - row0);
-      for (int i = kw * 32 + lane; i < 32 * rows; i += 32 * split) {
+      for (int i = kw * 32 + lane; i < 32 * a.rows; i += 32 * split) {
         const int m = i >> 5, r = i & 31;
         float v = 0.0f;
         const float* of_row = in + L::column_of(m) * L::PITCH + r;
@@ -560,10 +558,10 @@ __global__ void __launch_bounds__(kThreads, 1) w4_linear_kernel(const LinearArgs
         if (c > 1) {
           part[((j - j0) * L::ROWS + m) * L::PITCH + r] = v;
         } else {
-          const int row = row0 + m, col = pair * 32 + r;
+          const int col = pair * 32 + r;
           if (col < a.n) {
-            if (D == 1) v *= a.a[row];
-            a.y[row * a.ldy + col] = __float2bfloat16_rn(v);
+            if (D == 1) v *= a.a[m];
+            a.y[m * a.ldy + col] = __float2bfloat16_rn(v);
           }
         }
       }
@@ -571,15 +569,15 @@ __global__ void __launch_bounds__(kThreads, 1) w4_linear_kernel(const LinearArgs
     }
     if (c > 1) {
       cluster_sync();
-      const int rows = min(L::ROWS, a.rows - row0), n = (j1 - j0) * rows * 8;
+      const int n = (j1 - j0) * a.rows * 8;
       for (int i = rank * kThreads + tid; i < n; i += c * kThreads) {
-        const int r = 4 * (i & 7), m = (i >> 3) % rows, j = (i >> 3) / rows;
-        const int row = row0 + m, col = (unit + (j0 + j) * units) * 32 + r;
+        const int r = 4 * (i & 7), m = (i >> 3) % a.rows, j = (i >> 3) / a.rows;
+        const int col = (unit + (j0 + j) * units) * 32 + r;
         const float4 v = dsmem_sum4(part + (j * L::ROWS + m) * L::PITCH + r, c);
-        const float scale = D == 1 ? a.a[row] : 1.0f, y4[4] = {v.x * scale, v.y * scale, v.z * scale, v.w * scale};
+        const float scale = D == 1 ? a.a[m] : 1.0f, y4[4] = {v.x * scale, v.y * scale, v.z * scale, v.w * scale};
 #pragma unroll
         for (int k = 0; k < 4; ++k)
-          if (col + k < a.n) a.y[row * a.ldy + col + k] = __float2bfloat16_rn(y4[k]);
+          if (col + k < a.n) a.y[m * a.ldy + col + k] = __float2bfloat16_rn(y4[k]);
       }
       cluster_sync();  // everybody has read: the sums may change, or their block end
     }
@@ -625,7 +623,7 @@ int run(const char* name, LinearArgs a, cudaStream_t stream) {
     if (L{blocks, 1, c > 1}.bytes() > kMostSmem || c > a.blocks) continue;
     double warp = 0;
     const int split = split_of(mine, blocks, warp);
-    const int of_x = (a.rows < L::ROWS ? a.rows : L::ROWS) * blocks, at_once = kThreads * L::AHEAD / 16;
+    const int of_x = a.rows * blocks, at_once = kThreads * L::AHEAD / 16;
     const double cost = double(mine) * (blocks + 1) + 5 * warp + (c > 1 ? 20 : 0) + 8 * ((of_x + at_once - 1) / at_once) +
                         0.05 * of_x;
     if (best == 0 || cost < least) best = c, least = cost, a.split = split;
@@ -636,7 +634,7 @@ int run(const char* name, LinearArgs a, cudaStream_t stream) {
   L at = {(a.blocks + best - 1) / best, kMaxStages, best > 1};
   while (at.bytes() > kMostSmem) --at.stages;
   a.stages = at.stages;
-  const dim3 grid(static_cast<unsigned>(units * best), static_cast<unsigned>((a.rows + L::ROWS - 1) / L::ROWS));
+  const dim3 grid(static_cast<unsigned>(units * best));
   if (best == 1) return launch(name, kernel, grid, dim3(kThreads), at.bytes(), stream, a);
   return launch_cluster(name, kernel, grid, dim3(kThreads), static_cast<unsigned>(best), at.bytes(), stream, a);
 }

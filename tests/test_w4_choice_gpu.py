@@ -38,7 +38,7 @@ def check(rows, n, k, group, q8):
     *[(r, n, k, g) for r in (7, 8) for g, k in ((128, 15872), (128, 15904), (64, 15360), (64, 15392), (32, 13824), (32, 13856))
       for n in (40, 2080)],
     # and of a cluster of 8
-    *[(8, 48, k, g) for g, k in ((128, 31744), (128, 31776), (64, 30720), (64, 30752), (32, 27648), (32, 27680))],
+    *[(8, 48, k, g) for g, k in ((128, 31744), (128, 31776), (64, 30688), (64, 30752), (32, 27648), (32, 27680))],
     # whatever k, up to 6 rows
     *[(r, 70, 32768, g) for r in (1, 2, 3, 4, 5, 6) for g in (32, 64, 128)], (5, 4000, 8224, 32), (8, 600, 5152, 32), (6, 1000, 8192, 32),
 ])
